@@ -1,0 +1,326 @@
+// Attention of drafted trees over a paged cache (64-token pages): every node of a tree sees the request's committed tokens, inside a chunk
+// or a window, its ancestors and itself.
+//
+//   o[j][h] = sum_i p_i v_i / (sum_i p_i + e^(sink_h)),  p_i = e^(cap tanh(scale q.k_i / cap) + bias[h][d] - slope_h d),  d: distance of the
+//   positions; a row that sees nothing is 0.  Statistics and sums are fp32 and kept against the running maximum.
+//
+//   tree_tile    FP32 units: the 32-bit mode and head sizes the tensor-core kernel does not take
+//   tree_merge   joins the parts of items that several CTAs share, and zeroes the rows behind the last request
+#include "../common/tree_work.cuh"
+
+namespace spark {
+
+// ------------------------------------------------------------------------------------------------ FP32 units
+constexpr int TT_BM = 32, TT_THREADS = 128, TT_LDK = 68, TT_LDV = 132, TT_LDS = 68;
+
+// Scores: four rows x four keys per thread over 64-wide pieces of the head; outputs: four rows x eight columns per 128-wide piece of V.
+template <typename T, int VC>
+__global__ void __launch_bounds__(TT_THREADS)
+tree_tile_kernel(const __grid_constant__ TreeAttn a) {
+  extern __shared__ __align__(16) float smem_tt[];
+  __shared__ long long sh[TT_THREADS / 32 + 2];
+  __shared__ float s_m[TT_BM], s_l[TT_BM], s_f[TT_BM];
+  __shared__ int s_pos[TT_BM], s_first[TT_BM], s_at[TA_PAGE];
+  const int D = a.D, V = a.V, LDQ = (D + 63) / 64 * 64 + 4, rep = a.H / a.G;
+  float* Qs = smem_tt;                                       // [32][LDQ]
+  float* Ks = Qs + TT_BM * LDQ;                              // [64][68]
+  float* Vs = Ks + TA_PAGE * TT_LDK;                         // [64][132]
+  float* Ss = Vs + TA_PAGE * TT_LDV;                         // [32][68]
+  const int t = threadIdx.x, ty = t >> 4, tx = t & 15;
+  pdl_wait();
+  pdl_trigger();
+  TreeRange range = ta_range<TT_THREADS, TT_BM>(a, sh);
+  if (t == 0) a.split[blockIdx.x] = make_int4(0, 0, 0, 0);
+  TreeItem it;
+  while (ta_next<TT_BM>(a, range, it)) {
+    const TreeSeg& sg = it.seg;
+    const int slot = a.slots ? a.slots[it.s] : it.s, pairs = min(TT_BM, sg.n * rep - it.rt * TT_BM);
+    __syncthreads();
+    for (int i = t; i < TT_BM * (LDQ / 4); i += TT_THREADS) {
+      const int row = i / (LDQ / 4), c = (i - row * (LDQ / 4)) * 4, f = it.rt * TT_BM + row;
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (row < pairs && c < D) x = ldf4(static_cast<const T*>(a.q) + static_cast<size_t>(sg.r0 + f / rep) * a.ldq + static_cast<size_t>(it.g * rep + f % rep) * a.hq + c);
+      *reinterpret_cast<float4*>(Qs + row * LDQ + c) = x;
+    }
+    if (t < TT_BM) {
+      const int p = t < pairs ? a.pos[sg.r0 + (it.rt * TT_BM + t) / rep] : 0;
+      s_pos[t] = p;
+      s_first[t] = ta_first_visible(a, p);
+      s_m[t] = -INFINITY;
+      s_l[t] = 0.f;
+    }
+    float o[VC][4][8] = {};
+    for (int j = it.j; j < it.j + it.nj; ++j) {
+      const int page = ta_page(a, slot, j), tok0 = j * TA_PAGE;
+      if (page < 0 && t == 0) set_status(a.status, ST_BOUNDS, sg.r0, tok0, slot);
+      const int valid = page < 0 ? 0 : min(TA_PAGE, sg.len + sg.n - tok0);
+      const T* kp = static_cast<const T*>(a.k) + max(page, 0) * a.k_page + static_cast<size_t>(it.g) * D;
+      const T* vp = static_cast<const T*>(a.v) + max(page, 0) * a.v_page + static_cast<size_t>(it.g) * V;
+      if (t < TA_PAGE) {
+        const int node = tok0 + t - sg.len;
+        s_at[t] = node < 0 ? tok0 + t : (node < sg.n ? a.pos[sg.r0 + node] : 0);
+      }
+      float s[4][4] = {};
+      for (int d0 = 0; d0 < D; d0 += 64) {
+        __syncthreads();
+        for (int i = t; i < TA_PAGE * 16; i += TT_THREADS) {
+          const int row = i >> 4, c = (i & 15) * 4;
+          float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (row < valid && d0 + c < D) x = ldf4(kp + row * a.k_tok + d0 + c);
+          *reinterpret_cast<float4*>(Ks + row * TT_LDK + c) = x;
+        }
+        __syncthreads();
+#pragma unroll 4
+        for (int c = 0; c < 64; c += 4) {
+          float4 q[4], k[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) q[i] = *reinterpret_cast<const float4*>(Qs + (ty * 4 + i) * LDQ + d0 + c);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) k[i] = *reinterpret_cast<const float4*>(Ks + (tx + 16 * i) * TT_LDK + c);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              s[i][e] = fmaf(q[i].x, k[e].x, fmaf(q[i].y, k[e].y, fmaf(q[i].z, k[e].z, fmaf(q[i].w, k[e].w, s[i][e]))));
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = ty * 4 + i, f = it.rt * TT_BM + row, h = it.g * rep + f % rep, node = f / rep;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int key = tx + 16 * e, kn = tok0 + key - sg.len;
+          bool on = row < pairs && key < valid && s_at[key] >= s_first[row];
+          if (on && kn >= 0) on = a.anc ? (kn >> 5) < a.words && (a.anc[static_cast<size_t>(sg.r0 + node) * a.words + (kn >> 5)] >> (kn & 31)) & 1u : kn <= node;
+          float x = -INFINITY;
+          if (on) {
+            const int dist = s_pos[row] - s_at[key];
+            x = s[i][e] * a.scale;
+            if (a.cap > 0.f) x = a.cap * tanhf(x / a.cap);
+            if (a.bias) x += a.bias[static_cast<size_t>(h) * a.bias_n + min(max(dist, 0), a.bias_n - 1)];
+            if (a.slopes) x -= a.slopes[h] * static_cast<float>(dist);
+          }
+          Ss[row * TT_LDS + key] = x;
+        }
+      }
+      __syncthreads();
+      {                                                      // statistics: four threads per row
+        const int row = t >> 2, c = t & 3;
+        float* sr = Ss + row * TT_LDS + c;
+        float mx = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sr[4 * i]);
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float m0 = s_m[row], m = fmaxf(m0, mx), ref = m == -INFINITY ? 0.f : m;
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float e = expf(sr[4 * i] - ref);
+          sr[4 * i] = e;
+          sum += e;
+        }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        __syncwarp();
+        if (c == 0) {
+          const float f = expf(m0 - ref);
+          s_f[row] = f;
+          s_m[row] = m;
+          s_l[row] = s_l[row] * f + sum;
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float f = s_f[ty * 4 + i];
+#pragma unroll
+        for (int v = 0; v < VC; ++v)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) o[v][i][e] *= f;
+      }
+#pragma unroll
+      for (int v = 0; v < VC; ++v) {
+        if (v) __syncthreads();
+        for (int i = t; i < TA_PAGE * 32; i += TT_THREADS) {
+          const int row = i >> 5, c = (i & 31) * 4;
+          float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (row < valid && v * 128 + c < V) x = ldf4(vp + row * a.v_tok + v * 128 + c);
+          *reinterpret_cast<float4*>(Vs + row * TT_LDV + c) = x;
+        }
+        __syncthreads();
+        for (int k = 0; k < TA_PAGE; ++k) {
+          const float4 x = *reinterpret_cast<const float4*>(Vs + k * TT_LDV + tx * 4), y = *reinterpret_cast<const float4*>(Vs + k * TT_LDV + 64 + tx * 4);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float p = Ss[(ty * 4 + i) * TT_LDS + k];
+            if (p != 0.f) {                                  // what a row does not see stays out of it, whatever it holds
+              o[v][i][0] = fmaf(p, x.x, o[v][i][0]); o[v][i][1] = fmaf(p, x.y, o[v][i][1]);
+              o[v][i][2] = fmaf(p, x.z, o[v][i][2]); o[v][i][3] = fmaf(p, x.w, o[v][i][3]);
+              o[v][i][4] = fmaf(p, y.x, o[v][i][4]); o[v][i][5] = fmaf(p, y.y, o[v][i][5]);
+              o[v][i][6] = fmaf(p, y.z, o[v][i][6]); o[v][i][7] = fmaf(p, y.w, o[v][i][7]);
+            }
+          }
+        }
+      }
+    }
+    // ---- whole: the rows' outputs; else this CTA's part of them
+    const bool whole = it.first && it.last;
+    if (it.first && !it.last && t == 0) a.split[blockIdx.x] = make_int4(it.parts, it.s, it.g, it.rt);
+    const size_t pb = (static_cast<size_t>(blockIdx.x) * 2 + (it.first ? 1 : 0)) * TT_BM;
+    if (!whole && t < pairs) { a.part_ml[(pb + t) * 2] = s_m[t]; a.part_ml[(pb + t) * 2 + 1] = s_l[t]; }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = ty * 4 + i, f = it.rt * TT_BM + row, h = it.g * rep + f % rep, r = sg.r0 + f / rep;
+      if (row >= pairs) continue;
+      float scale = 1.f;
+      if (whole) {
+        float l = s_l[row], c = 1.f;
+        if (a.sink) {
+          const float m = fmaxf(s_m[row], a.sink[h]);
+          c = expf(s_m[row] - m);
+          l = l * c + expf(a.sink[h] - m);
+        }
+        scale = l > 0.f ? ta_head_factor<T>(a, r, h) * c / l : 0.f;
+        if (l != l) scale = l;
+      }
+#pragma unroll
+      for (int v = 0; v < VC; ++v)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int col = v * 128 + half * 64 + tx * 4;
+          if (col >= V) continue;
+          const float4 x = make_float4(o[v][i][half * 4] * scale, o[v][i][half * 4 + 1] * scale, o[v][i][half * 4 + 2] * scale, o[v][i][half * 4 + 3] * scale);
+          if (whole) stf4(static_cast<T*>(a.out) + static_cast<size_t>(r) * a.ldo + static_cast<size_t>(h) * a.ho + col, x);
+          else *reinterpret_cast<float4*>(a.part_o + (pb + row) * V + col) = x;
+        }
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ merge
+// grid (ctas, row groups); 256 threads, `wpr` warps per row.  Parts in ascending order within a warp, warps in ascending order.
+template <typename T, int BM>
+__global__ void __launch_bounds__(256)
+tree_merge_kernel(const __grid_constant__ TreeAttn a, int wpr) {
+  __shared__ float4 s_o[8][128];
+  __shared__ float s_ml[8][2];
+  pdl_wait();
+  pdl_trigger();
+  const int t = threadIdx.x, warp = t >> 5, lane = t & 31, c = blockIdx.x, V4 = a.V >> 2, rep = a.H / a.G;
+  if (a.zero_rest && blockIdx.y == 0)
+    for (int r = a.starts[a.S] + c; r < a.R; r += gridDim.x)
+      for (int i = t; i < a.H * V4; i += 256) {
+        const int h = i / V4;
+        stf4(static_cast<T*>(a.out) + static_cast<size_t>(r) * a.ldo + static_cast<size_t>(h) * a.ho + (i - h * V4) * 4, make_float4(0.f, 0.f, 0.f, 0.f));
+      }
+  const int4 sp = a.split[c];
+  if (sp.x <= 1) return;
+  const TreeSeg sg = ta_segment<BM>(a, sp.y);
+  const int rpb = 8 / wpr, sub = warp % wpr, row = blockIdx.y * rpb + warp / wpr, f = sp.w * BM + row;
+  if (static_cast<int>(blockIdx.y) * rpb >= min(BM, sg.n * rep - sp.w * BM)) return;
+  const bool on = row < BM && f < sg.n * rep;
+  // part 0 lies behind the others' in its CTA's pair, see TreeAttn
+  auto part = [&](int i) { return (static_cast<size_t>(c + i) * 2 + (i == 0 ? 1 : 0)) * BM + row; };
+  float m = -INFINITY, l = 0.f;
+  if (on)
+    for (int i = sub; i < sp.x; i += wpr) m = fmaxf(m, a.part_ml[part(i) * 2]);
+  float4 o[4] = {};
+  const float ref = m == -INFINITY ? 0.f : m;
+  if (on)
+    for (int i0 = sub; i0 < sp.x; i0 += 4 * wpr) {           // four parts in flight
+      float4 x[4][4];
+      float w[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + u * wpr;
+        w[u] = 0.f;
+        if (i >= sp.x) continue;
+        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + part(i) * 2);
+        w[u] = expf(ml.x - ref);
+        l = fmaf(w[u], ml.y, l);
+#pragma unroll
+        for (int v = 0; v < 4; ++v)
+          if (lane + v * 32 < V4) x[u][v] = __ldcg(reinterpret_cast<const float4*>(a.part_o + part(i) * a.V) + lane + v * 32);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (w[u] != 0.f)
+#pragma unroll
+          for (int v = 0; v < 4; ++v)
+            if (lane + v * 32 < V4) {
+              o[v].x = fmaf(w[u], x[u][v].x, o[v].x); o[v].y = fmaf(w[u], x[u][v].y, o[v].y);
+              o[v].z = fmaf(w[u], x[u][v].z, o[v].z); o[v].w = fmaf(w[u], x[u][v].w, o[v].w);
+            }
+    }
+  if (wpr > 1) {
+    if (lane == 0) { s_ml[warp][0] = m; s_ml[warp][1] = l; }
+#pragma unroll
+    for (int v = 0; v < 4; ++v)
+      if (lane + v * 32 < V4) s_o[warp][lane + v * 32] = o[v];
+    __syncthreads();
+    if (sub) return;
+    for (int i = 1; i < wpr; ++i) m = fmaxf(m, s_ml[warp + i][0]);
+    const float r2 = m == -INFINITY ? 0.f : m, c0 = expf(s_ml[warp][0] - r2);
+    l *= c0;
+#pragma unroll
+    for (int v = 0; v < 4; ++v) { o[v].x *= c0; o[v].y *= c0; o[v].z *= c0; o[v].w *= c0; }
+    for (int i = 1; i < wpr; ++i) {
+      const float ci = expf(s_ml[warp + i][0] - r2);
+      if (ci == 0.f) continue;
+      l = fmaf(ci, s_ml[warp + i][1], l);
+#pragma unroll
+      for (int v = 0; v < 4; ++v)
+        if (lane + v * 32 < V4) {
+          const float4 x = s_o[warp + i][lane + v * 32];
+          o[v].x = fmaf(ci, x.x, o[v].x); o[v].y = fmaf(ci, x.y, o[v].y); o[v].z = fmaf(ci, x.z, o[v].z); o[v].w = fmaf(ci, x.w, o[v].w);
+        }
+    }
+  }
+  if (!on) return;
+  const int h = sp.z * rep + f % rep, r = sg.r0 + f / rep;
+  float k = 1.f;
+  if (a.sink) {
+    const float M = fmaxf(m, a.sink[h]);
+    k = expf(m - M);
+    l = l * k + expf(a.sink[h] - M);
+  }
+  float scale = l > 0.f ? ta_head_factor<T>(a, r, h) * k / l : 0.f;
+  if (l != l) scale = l;
+#pragma unroll
+  for (int v = 0; v < 4; ++v)
+    if (lane + v * 32 < V4)
+      stf4(static_cast<T*>(a.out) + static_cast<size_t>(r) * a.ldo + static_cast<size_t>(h) * a.ho + (lane + v * 32) * 4,
+           make_float4(o[v].x * scale, o[v].y * scale, o[v].z * scale, o[v].w * scale));
+}
+
+constexpr int TA_SMEM = 220 * 1024;
+
+template <typename T, int VC>
+static int launch_tile(const TreeAttn& a, cudaStream_t s) {
+  auto kern = tree_tile_kernel<T, VC>;
+  const int smem = (TT_BM * ((a.D + 63) / 64 * 64 + 4) + TA_PAGE * (TT_LDK + TT_LDV) + TT_BM * TT_LDS) * 4;
+  if (smem > TA_SMEM) return -6;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, TA_SMEM) != cudaSuccess) return -4;
+  spark_launch_pdl(kern, dim3(a.ctas), dim3(TT_THREADS), smem, s, dim3(1, 1, 1), a);
+  return spark_launch_rc("spark_tree_attn");
+}
+template <typename T>
+static int launch_tiles(const TreeAttn& a, cudaStream_t s) {
+  const int rc = a.V <= 128 ? launch_tile<T, 1>(a, s) : a.V <= 256 ? launch_tile<T, 2>(a, s) : launch_tile<T, 4>(a, s);
+  if (rc) return rc;
+  const int wpr = 8;
+  spark_launch_pdl(tree_merge_kernel<T, TT_BM>, dim3(a.ctas, TT_BM * wpr / 8), dim3(256), 0, s, dim3(1, 1, 1), a, wpr);
+  return spark_launch_rc("spark_tree_attn");
+}
+
+}  // namespace spark
+
+using namespace spark;
+
+extern "C" int spark_tree_attn(const TreeAttn* a, int f32, cudaStream_t s) {
+  if (a->S <= 0 || a->R <= 0) return 0;
+  if (a->H <= 0 || a->G <= 0 || a->H % a->G || a->D <= 0 || a->V <= 0 || ((a->D | a->V) & 7) || a->D > 512 || a->V > 512 || a->ctas <= 0 ||
+      a->min_tiles <= 0 || (a->bias && a->bias_n <= 0) || a->page_ld <= 0 || ((a->ldq | a->hq | a->ldo | a->ho) & 3)) return -5;
+  return f32 ? launch_tiles<float>(*a, s) : launch_tiles<__nv_bfloat16>(*a, s);
+}

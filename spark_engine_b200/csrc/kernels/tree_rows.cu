@@ -1,0 +1,365 @@
+// Rows of a verification round over paged caches (64-token pages), from request lengths that live on the device:
+//
+//   block_tables  a request's pages follow its length: pages go back on a stack and come off it
+//   slot_maps     request, index, position, cache row and ancestors of every row of the round
+//   path_conv     short causal convolution along a drafted tree's paths, keys and values into their pages
+//   commit_paths  the accepted path's cache rows of all layers together, the convolutions' states along it
+//
+// Row r of request s has index j = r - starts[s].  It is written to the cache at the request's token len_s + j, whatever its depth in the
+// tree; its position is len_s + depth.  What a table or a path gives is checked before it is used as an address: a bad entry sets the status
+// word and the row is skipped.
+#include "../common/rows.cuh"
+
+namespace spark {
+
+constexpr int TREE_PAGE = 64;
+
+// Exclusive prefix of v over the block's 1024 threads, and the sum; `sh`: 33 ints.  Every thread calls it.
+__device__ __forceinline__ int block_prefix(int v, int* sh, int& total) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = blockDim.x >> 5;
+  int x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  if (lane == 31) sh[w] = x;
+  __syncthreads();
+  if (w == 0) {
+    int s = lane < nw ? sh[lane] : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += y;
+    }
+    sh[lane] = s;
+  }
+  __syncthreads();
+  const int before = w ? sh[w - 1] : 0;
+  total = sh[nw - 1];
+  __syncthreads();
+  return before + x - v;
+}
+
+// ------------------------------------------------------------------------------------------------ block tables
+struct BlockTables {
+  const int* lengths;                    // [S] tokens a request needs room for; negative: the request is left as it is
+  int *tables, *held;                    // [S, ld] pages in position order, -1 behind the held ones; [S]
+  int *free, *n_free;                    // stack of free pages: free[0 .. n_free)
+  int *room, *status;                    // [S] tokens a request has room for afterwards
+  int S, ld, cap;                        // cap: entries of `free`
+};
+
+// One CTA, a warp per request in turn.  Pages go back first, the last request's last page first, then requests take theirs in order, each
+// from the top of the stack: giving back what was just taken restores the stack.  A request whose pages are not all there gets none, nor
+// does one behind it that needs any.
+__global__ void __launch_bounds__(1024)
+block_tables_kernel(const __grid_constant__ BlockTables a) {
+  __shared__ int sh[33], s_have[1024], s_need[1024], s_off[1024];
+  pdl_wait();
+  pdl_trigger();
+  const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+  const int nf = min(max(*a.n_free, 0), a.cap);
+  auto load = [&](int s, int& have, int& need) {
+    have = need = 0;
+    if (s >= a.S) return;
+    const int len = a.lengths[s];
+    have = min(max(a.held[s], 0), a.ld);
+    need = len < 0 ? have : len / TREE_PAGE + (len % TREE_PAGE != 0);
+    if (need > a.ld) { set_status(a.status, ST_BOUNDS, s, len, a.ld); need = a.ld; }
+  };
+  int total = 0;                                             // pages given back
+  for (int s0 = 0; s0 < a.S; s0 += 1024) {
+    int have, need, n;
+    load(s0 + t, have, need);
+    block_prefix(max(have - need, 0), sh, n);
+    total += n;
+  }
+  int done = 0;
+  for (int s0 = 0; s0 < a.S && total > 0; s0 += 1024) {
+    int n;
+    load(s0 + t, s_have[t], s_need[t]);
+    s_off[t] = done + block_prefix(max(s_have[t] - s_need[t], 0), sh, n);
+    done += n;
+    __syncthreads();
+    for (int i = warp; i < min(1024, a.S - s0); i += 32) {
+      int* row = a.tables + static_cast<size_t>(s0 + i) * a.ld;
+      for (int p = s_need[i] + lane; p < s_have[i]; p += 32) {
+        const int to = nf + total - 1 - (s_off[i] + p - s_need[i]);
+        if (to < a.cap) a.free[to] = row[p];
+        else set_status(a.status, ST_BOUNDS, s0 + i, to, a.cap);
+        row[p] = -1;
+      }
+    }
+    __syncthreads();
+  }
+  const int top = min(nf + total, a.cap);
+  int asked = 0, used = 0;
+  for (int s0 = 0; s0 < a.S; s0 += 1024) {
+    int n, m;
+    load(s0 + t, s_have[t], s_need[t]);
+    const int want = max(s_need[t] - s_have[t], 0), off = asked + block_prefix(want, sh, n);
+    const bool ok = off + want <= top;
+    block_prefix(ok ? want : 0, sh, m);
+    asked = min(asked + n, 1 << 30);
+    used += m;
+    s_off[t] = off;
+    if (!ok) s_need[t] = min(s_need[t], s_have[t]);
+    if (s0 + t < a.S) { a.held[s0 + t] = s_need[t]; a.room[s0 + t] = s_need[t] * TREE_PAGE; }
+    __syncthreads();
+    for (int i = warp; i < min(1024, a.S - s0); i += 32) {
+      int* row = a.tables + static_cast<size_t>(s0 + i) * a.ld;
+      for (int p = s_have[i] + lane; p < s_need[i]; p += 32) row[p] = a.free[top - 1 - (s_off[i] + p - s_have[i])];
+    }
+    __syncthreads();
+  }
+  if (t == 0) *a.n_free = top - used;
+}
+
+// ------------------------------------------------------------------------------------------------ row maps
+struct SlotMaps {
+  const int *lengths, *counts, *tables, *slots, *parents;    // slots (optional): a request's row of the tables; parents (trees): [R]
+  int *starts, *slot, *index, *pos, *anc;                    // [S + 1], [R] each, [R, words]
+  long long* cache_row;                                      // [R]
+  int* status;
+  int S, R, ld, n_slots, nodes, words;
+};
+
+constexpr int MAP_THREADS = 256;
+
+// grid: rows.  Every CTA forms the prefix of all counts (a few hundred numbers) instead of waiting for another launch that does.
+__global__ void __launch_bounds__(MAP_THREADS)
+slot_maps_kernel(const __grid_constant__ SlotMaps a) {
+  extern __shared__ int s_start[];                           // [S + 1]
+  __shared__ int sh[33];
+  pdl_wait();
+  pdl_trigger();
+  const int t = threadIdx.x;
+  int base = 0;
+  for (int s0 = 0; s0 < a.S; s0 += MAP_THREADS) {
+    int n;
+    const int c = s0 + t < a.S ? min(max(a.counts[s0 + t], 0), a.R) : 0;
+    const int b = min(base + block_prefix(c, sh, n), a.R);
+    if (s0 + t < a.S) s_start[s0 + t] = b;
+    if (base + n > a.R && t == 0 && blockIdx.x == 0) set_status(a.status, ST_BOUNDS, s0, base + n, a.R);
+    base = min(base + n, a.R);
+  }
+  if (t == 0) s_start[a.S] = base;
+  __syncthreads();
+  if (blockIdx.x == 0)
+    for (int s = t; s <= a.S; s += MAP_THREADS) a.starts[s] = s_start[s];
+  for (int r = blockIdx.x * MAP_THREADS + t; r < a.R; r += gridDim.x * MAP_THREADS) {
+    int slot = -1, j = -1, pos = -1;
+    long long row = -1;
+    if (r < base) {
+      int lo = 0, hi = a.S;                                  // the last request that starts at or before r (and is not empty)
+      while (hi - lo > 1) { const int m = (lo + hi) >> 1; if (s_start[m] <= r) lo = m; else hi = m; }
+      const int r0 = s_start[lo], len = max(a.lengths[lo], 0);
+      slot = a.slots ? a.slots[lo] : lo;
+      j = r - r0;
+      int depth = j;
+      if (a.words) {
+        if (j >= a.nodes) set_status(a.status, ST_BOUNDS, r, j, a.nodes);
+        depth = -1;
+        int* out = a.anc + static_cast<size_t>(r) * a.words;
+        uint32_t bits = 0;
+        int word = j >> 5;
+        for (int w = word + 1; w < a.words; ++w) out[w] = 0;
+        for (int at = j; at >= 0;) {                         // every step goes to a lower index
+          for (; word > (at >> 5); --word) { if (word < a.words) out[word] = bits; bits = 0; }
+          bits |= 1u << (at & 31);
+          ++depth;
+          int p = a.parents ? a.parents[r0 + at] : at - 1;
+          if (p >= at || p < -1) { set_status(a.status, ST_BAD_ARGUMENT, r0 + at, p, at); p = -1; }
+          at = p;
+        }
+        for (; word >= 0; --word) { if (word < a.words) out[word] = bits; bits = 0; }
+      }
+      pos = len + depth;
+      const long long tok = static_cast<long long>(len) + j;
+      const bool ok = slot >= 0 && slot < a.n_slots && tok / TREE_PAGE < a.ld;
+      const int page = ok ? a.tables[static_cast<size_t>(slot) * a.ld + tok / TREE_PAGE] : -1;
+      if (page >= 0) row = static_cast<long long>(page) * TREE_PAGE + tok % TREE_PAGE;
+      else set_status(a.status, ST_BOUNDS, r, static_cast<int>(tok), slot);
+    } else if (a.words) {
+      for (int w = 0; w < a.words; ++w) a.anc[static_cast<size_t>(r) * a.words + w] = 0;
+    }
+    a.slot[r] = slot; a.index[r] = j; a.pos[r] = pos; a.cache_row[r] = row;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ convolution along paths
+struct PathConv {
+  const void* x; const float* w; const void* tail;           // [R, ldx]; [taps, C]; [slots, taps - 1, C]
+  void *q, *k, *v;                                           // q [R, nq]
+  const int *slot, *index, *parents;                         // parents null: chains
+  const long long* cache_row;
+  int* status;
+  long long k_page, k_tok, v_page, v_tok, cache_rows;        // strides in elements
+  int ldx, R, C, taps, nq, nk, n_slots;
+};
+
+constexpr int PC_ROWS = 4;
+
+// grid (row groups, channel blocks); 128 threads x 16 bytes of channels.
+template <typename T, int TAPS>
+__global__ void __launch_bounds__(128)
+path_conv_kernel(const __grid_constant__ PathConv a) {
+  constexpr int VEC = 16 / sizeof(T);
+  pdl_wait();
+  pdl_trigger();
+  const int taps = TAPS > 0 ? TAPS : a.taps;
+  const int c0 = (blockIdx.y * 128 + threadIdx.x) * VEC;
+  if (c0 >= a.C) return;
+  for (int i = 0; i < PC_ROWS; ++i) {
+    const int r = blockIdx.x * PC_ROWS + i;
+    if (r >= a.R) return;
+    const int slot = a.slot[r];
+    if (slot < 0) continue;                                  // a row behind the last request
+    const int j = a.index[r], r0 = r - j;
+    float y[VEC] = {};
+    int at = j, back = 0;
+    for (int tp = taps - 1; tp >= 0; --tp) {                 // the row, its ancestors, then the sequence's past
+      const T* src;
+      if (at >= 0) {
+        src = static_cast<const T*>(a.x) + static_cast<size_t>(r0 + at) * a.ldx + c0;
+        if (tp) {
+          const int p = a.parents ? a.parents[r0 + at] : at - 1;
+          at = p < at ? p : -1;
+        }
+      } else {
+        ++back;
+        src = static_cast<const T*>(a.tail) + (static_cast<size_t>(min(slot, a.n_slots - 1)) * (taps - 1) + (taps - 1 - back)) * a.C + c0;
+      }
+#pragma unroll
+      for (int e = 0; e < VEC; e += 4) {
+        const float4 u = ldf4(src + e), w = *reinterpret_cast<const float4*>(a.w + static_cast<size_t>(tp) * a.C + c0 + e);
+        y[e] = fmaf(w.x, u.x, y[e]); y[e + 1] = fmaf(w.y, u.y, y[e + 1]);
+        y[e + 2] = fmaf(w.z, u.z, y[e + 2]); y[e + 3] = fmaf(w.w, u.w, y[e + 3]);
+      }
+    }
+    T* dst;
+    if (c0 < a.nq) dst = static_cast<T*>(a.q) + static_cast<size_t>(r) * a.nq + c0;
+    else {
+      const long long row = a.cache_row[r];
+      if (row < 0 || row >= a.cache_rows) {
+        set_status(a.status, ST_BOUNDS, r, static_cast<int>(row), slot);
+        continue;
+      }
+      const long long page = row / TREE_PAGE, tok = row % TREE_PAGE;
+      dst = c0 < a.nq + a.nk ? static_cast<T*>(a.k) + page * a.k_page + tok * a.k_tok + (c0 - a.nq)
+                             : static_cast<T*>(a.v) + page * a.v_page + tok * a.v_tok + (c0 - a.nq - a.nk);
+    }
+#pragma unroll
+    for (int e = 0; e < VEC; e += 4) stf4(dst + e, make_float4(y[e], y[e + 1], y[e + 2], y[e + 3]));
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ commit
+struct CommitJob {
+  char* base;                            // a cache, or the tail of a convolution
+  const char* x;                         // null: a cache; else the rows behind the tail
+  long long page, tok;                   // bytes: strides of a cache's pages and tokens, or of a slot's entries (tok) and of x's rows (page)
+  int bytes, extent, kept, pad;          // bytes of a row (multiple of 16); pages of the cache, or slots of the tail; a slot's entries
+};
+constexpr int COMMIT_JOBS = 64;
+struct CommitPaths {
+  CommitJob job[COMMIT_JOBS];
+  const int *path, *n_path, *starts, *lengths, *slots, *tables;
+  int* status;
+  int S, P, ld, n_slots;
+};
+
+// grid (requests, column blocks, jobs); 128 threads x 16 bytes.  A path is ascending, so row i is written after row path[i] >= i was read,
+// and no later row of the path lies at or below i: every thread moves its columns in order and in place.
+__global__ void __launch_bounds__(128)
+commit_paths_kernel(const __grid_constant__ CommitPaths a) {
+  extern __shared__ int s_path[];                            // [P], then [P] source and [P] target rows of the cache
+  pdl_wait();
+  pdl_trigger();
+  const CommitJob& jb = a.job[blockIdx.z];
+  const int s = blockIdx.x, t = threadIdx.x, n = min(a.n_path[s], a.P), count = a.starts[s + 1] - a.starts[s];
+  if (n <= 0) return;
+  const int slot = a.slots ? a.slots[s] : s, len = max(a.lengths[s], 0);
+  bool ok = slot >= 0 && slot < a.n_slots;
+  int* src = s_path + a.P;
+  int* dst = src + a.P;
+  for (int i = t; i < n; i += 128) {
+    const int p = a.path[static_cast<size_t>(s) * a.P + i];
+    if (p < i || p >= count || (i > 0 && p <= a.path[static_cast<size_t>(s) * a.P + i - 1])) ok = false;
+    s_path[i] = p;
+  }
+  ok = __syncthreads_and(ok);
+  if (ok && !jb.x) {
+    for (int i = t; i < n; i += 128) {
+      const int from = len + s_path[i], to = len + i;
+      const int pf = from / TREE_PAGE < a.ld ? a.tables[static_cast<size_t>(slot) * a.ld + from / TREE_PAGE] : -1;
+      const int pt = to / TREE_PAGE < a.ld ? a.tables[static_cast<size_t>(slot) * a.ld + to / TREE_PAGE] : -1;
+      if (pf < 0 || pt < 0 || pf >= jb.extent || pt >= jb.extent) ok = false;
+      src[i] = pf * TREE_PAGE + from % TREE_PAGE;
+      dst[i] = pt * TREE_PAGE + to % TREE_PAGE;
+    }
+  } else if (ok && slot >= jb.extent) ok = false;
+  ok = __syncthreads_and(ok);
+  if (!ok) {
+    if (t == 0) set_status(a.status, ST_BOUNDS, s, slot, n);
+    return;
+  }
+  const int col = (blockIdx.y * 128 + t) * 16;
+  if (col >= jb.bytes) return;
+  if (jb.x) {
+    char* tail = jb.base + static_cast<long long>(slot) * jb.kept * jb.tok + col;
+    for (int e = 0; e < jb.kept; ++e) {                       // ascending: an entry is read before any later one is written
+      const int at = n - jb.kept + e;
+      const char* p = at >= 0 ? jb.x + static_cast<long long>(a.starts[s] + s_path[at]) * jb.page + col : tail + (jb.kept + at) * jb.tok;
+      *reinterpret_cast<uint4*>(tail + e * jb.tok) = *reinterpret_cast<const uint4*>(p);
+    }
+    return;
+  }
+  for (int i = 0; i < n; ++i) {
+    if (src[i] == dst[i]) continue;
+    const uint4 v = *reinterpret_cast<const uint4*>(jb.base + (src[i] / TREE_PAGE) * jb.page + (src[i] % TREE_PAGE) * jb.tok + col);
+    *reinterpret_cast<uint4*>(jb.base + (dst[i] / TREE_PAGE) * jb.page + (dst[i] % TREE_PAGE) * jb.tok + col) = v;
+  }
+}
+
+}  // namespace spark
+
+using namespace spark;
+
+extern "C" int spark_block_tables(const BlockTables* a, cudaStream_t s) {
+  if (a->S <= 0) return 0;
+  if (a->ld <= 0 || a->cap < 0 || static_cast<long long>(a->S) * a->ld > (1 << 24)) return -5;
+  spark_launch_pdl(block_tables_kernel, dim3(1), dim3(1024), 0, s, dim3(1, 1, 1), *a);
+  return spark_launch_rc(__func__);
+}
+
+extern "C" int spark_slot_maps(const SlotMaps* a, cudaStream_t s) {
+  if (a->S <= 0 || a->S > 8192 || a->R < 0 || a->R > (1 << 22) || a->ld <= 0 || a->words < 0 || a->nodes > a->words * 32) return -5;
+  const int blocks = (a->R + MAP_THREADS - 1) / MAP_THREADS;
+  spark_launch_pdl(slot_maps_kernel, dim3(blocks < 1 ? 1 : (blocks > 1184 ? 1184 : blocks)), dim3(MAP_THREADS), (a->S + 1) * 4, s, dim3(1, 1, 1), *a);
+  return spark_launch_rc(__func__);
+}
+
+extern "C" int spark_path_conv(const PathConv* a, int f32, cudaStream_t s) {
+  if (a->R <= 0) return 0;
+  if (a->taps < 1 || ((a->C | a->nq | a->nk | a->ldx) & 7) || a->nq + a->nk > a->C || a->n_slots <= 0) return -5;
+  const int vec = f32 ? 4 : 8;
+  const dim3 grid((a->R + PC_ROWS - 1) / PC_ROWS, (a->C / vec + 127) / 128);
+  if (grid.y > 65535) return -5;
+#define SPARK_PATH(T, TAPS) spark_launch_pdl(path_conv_kernel<T, TAPS>, grid, dim3(128), 0, s, dim3(1, 1, 1), *a)
+  if (f32) { if (a->taps == 4) SPARK_PATH(float, 4); else SPARK_PATH(float, 0); }
+  else { if (a->taps == 4) SPARK_PATH(__nv_bfloat16, 4); else SPARK_PATH(__nv_bfloat16, 0); }
+#undef SPARK_PATH
+  return spark_launch_rc(__func__);
+}
+
+// `most`: bytes of the widest job's row.
+extern "C" int spark_commit_paths(const CommitPaths* a, int jobs, int most, cudaStream_t s) {
+  if (a->S <= 0 || jobs <= 0 || a->P <= 0) return 0;
+  if (jobs > COMMIT_JOBS || a->P > 4096 || a->ld <= 0 || (most & 15) || most <= 0) return -5;
+  for (int i = 0; i < jobs; ++i)
+    if (a->job[i].extent > (1 << 24) || (a->job[i].bytes & 15) || a->job[i].bytes > most) return -5;
+  spark_launch_pdl(commit_paths_kernel, dim3(a->S, (most / 16 + 127) / 128, jobs), dim3(128), a->P * 12, s, dim3(1, 1, 1), *a);
+  return spark_launch_rc(__func__);
+}

@@ -600,3 +600,7 @@ def latent_mixer(mixer, proj, plan, cat):
     if use_kernels(proj):
         return block_ops().latent_mixer(mixer, proj, plan, cat)
     return None
+
+
+# ----------------------------------------------------------------------------- drafted trees over paged caches
+from .tree import RowMaps, block_tables, commit_paths, path_conv, slot_maps, tree_attention  # noqa: E402, F401
