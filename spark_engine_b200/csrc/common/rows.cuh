@@ -46,6 +46,18 @@ __device__ __forceinline__ float log_sigmoid_decay(float x, float inv_tau) {
   return fmaxf((fminf(x, 0.f) - log1pf(expf(-fabsf(x)))) * inv_tau, -105.f);
 }
 
+// tanh to fp32 accuracy in the sense of the soft cap: the Taylor polynomial near 0 (where the quotient form would cancel),
+// 1 - 2 / (exp(2z) + 1) elsewhere (absolute error of a few 2^-23).  The polynomial gives tanh(z) / z.
+constexpr float CAP_NEAR = 0.25f;
+__device__ __forceinline__ float tanh_over_z(float z) {
+  const float s = z * z;
+  return fmaf(s, fmaf(s, fmaf(s, fmaf(s, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f);
+}
+__device__ __forceinline__ float cap_tanh(float z) {
+  const float near = z * tanh_over_z(z), far = 1.f - __fdividef(2.f, 1.f + __expf(2.f * fminf(z, 40.f)));
+  return fabsf(z) < CAP_NEAR ? near : far;
+}
+
 // Sum over the block in a fixed order; every thread gets the same bits.  sh: >= 32 floats.
 __device__ __forceinline__ float block_sum_all(float v, float* sh) {
   v = warp_sum(v);

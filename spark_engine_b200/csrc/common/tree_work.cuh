@@ -1,6 +1,6 @@
 // What the kernels of tree attention share: arguments, the division of the work, visibility, the merge of split rows.
 //
-// The (row, head) pairs of a request and a key / value head are numbered node by node and cut into tiles of BM; a tile's keys are the pages
+// The (row, head) pairs of a request and a key / value head are numbered node by node and cut into tiles of `bm`; a tile's keys are the pages
 // from the first one that any of its rows can see to the request's last node.  All (request, head, tile) items together are `total` pages,
 // and CTA c of the grid takes the same number of consecutive ones as every other: lengths may differ as they like, the host needs to know
 // none of them, and a captured launch may be replayed with others.  An item that ends in another CTA than it began leaves partial results
@@ -20,11 +20,11 @@ struct TreeAttn {
   const uint32_t* anc;                   // [R, words] (null: rows see the rows before them)
   const float *bias, *slopes, *sink;     // [H, bias_n], [H], [H]
   const void* gate;                      // [R, H], rows ldg apart
-  float *part_o, *part_ml;               // [ctas][2][BM][V], [ctas][2][BM][2]: of a tile begun before the CTA, of one that goes on behind it
+  float *part_o, *part_ml;               // [ctas][2][bm][V], [ctas][2][bm][2]: of a tile begun before the CTA, of one that goes on behind it
   int4* split;                           // [ctas]: parts of the item that begins in this CTA and ends in another (0: none), request, head, tile
   int* status;
   long long k_page, k_tok, v_page, v_tok;                    // strides in elements
-  int S, R, words, page_ld, n_slots, n_pages, H, G, D, V, ldq, hq, ldo, ho, ldg, bias_n, window, chunk, ctas, min_tiles, zero_rest;
+  int S, R, words, page_ld, n_slots, n_pages, H, G, D, V, ldq, hq, ldo, ho, ldg, bias_n, window, chunk, bm, ctas, min_tiles, zero_rest;
   float scale, cap, out_scale;
 };
 
@@ -35,7 +35,6 @@ __device__ __forceinline__ int ta_first_visible(const TreeAttn& a, int p) {
 struct TreeSeg {                         // a request's share of the work
   int r0, n, len, j0, nt, rts;           // first row, rows, committed tokens, first page, pages, row tiles
 };
-template <int BM>
 __device__ __forceinline__ TreeSeg ta_segment(const TreeAttn& a, int s) {
   TreeSeg t;
   t.r0 = a.starts[s];
@@ -43,7 +42,7 @@ __device__ __forceinline__ TreeSeg ta_segment(const TreeAttn& a, int s) {
   t.len = max(a.lengths[s], 0);
   t.j0 = ta_first_visible(a, t.len) / TA_PAGE;
   t.nt = (t.len + t.n + TA_PAGE - 1) / TA_PAGE - t.j0;
-  t.rts = t.n > 0 ? (t.n * (a.H / a.G) + BM - 1) / BM : 0;
+  t.rts = t.n > 0 ? (t.n * (a.H / a.G) + a.bm - 1) / a.bm : 0;
   return t;
 }
 __device__ __forceinline__ long long ta_tiles(const TreeAttn& a, const TreeSeg& t) { return static_cast<long long>(a.G) * t.rts * t.nt; }
@@ -73,11 +72,11 @@ __device__ __forceinline__ long long ta_prefix(long long v, long long* sh, long 
 }
 
 struct TreeRange { long long rem, count, per; int s; };       // pages into request s, pages of this CTA, pages of every CTA
-template <int NT, int BM>
+template <int NT>
 __device__ __forceinline__ TreeRange ta_range(const TreeAttn& a, long long* sh) {      // sh: [NT / 32 + 2]
   const int each = (a.S + NT - 1) / NT, s0 = threadIdx.x * each;                       // a thread's requests
   long long mine = 0, total;
-  for (int s = s0; s < min(s0 + each, a.S); ++s) mine += ta_tiles(a, ta_segment<BM>(a, s));
+  for (int s = s0; s < min(s0 + each, a.S); ++s) mine += ta_tiles(a, ta_segment(a, s));
   long long before = ta_prefix<NT>(mine, sh, total);
   TreeRange r;
   r.per = (total + a.ctas - 1) / a.ctas;
@@ -87,7 +86,7 @@ __device__ __forceinline__ TreeRange ta_range(const TreeAttn& a, long long* sh) 
   long long* found = sh + NT / 32;
   if (r.count > 0 && before <= begin && begin < before + mine) {
     for (int s = s0;; ++s) {
-      const long long n = ta_tiles(a, ta_segment<BM>(a, s));
+      const long long n = ta_tiles(a, ta_segment(a, s));
       if (begin < before + n) { found[0] = s; found[1] = begin - before; break; }
       before += n;
     }
@@ -105,13 +104,12 @@ struct TreeItem {                        // a row tile of one key / value head a
   int parts;                             // CTAs that share it (known to the one it begins in)
 };
 // The next item of the range; false at its end.
-template <int BM>
 __device__ __forceinline__ bool ta_next(const TreeAttn& a, TreeRange& r, TreeItem& it) {
   if (r.count <= 0) return false;
-  it.seg = ta_segment<BM>(a, r.s);
+  it.seg = ta_segment(a, r.s);
   while (r.rem >= ta_tiles(a, it.seg)) {                     // (the range ends with the last request's tiles)
     r.rem -= ta_tiles(a, it.seg);
-    it.seg = ta_segment<BM>(a, ++r.s);
+    it.seg = ta_segment(a, ++r.s);
   }
   const int nt = it.seg.nt, i = static_cast<int>(r.rem / nt), off = static_cast<int>(r.rem - static_cast<long long>(i) * nt);
   it.s = r.s;

@@ -37,6 +37,21 @@ int make_tmap_bf16(CUtensorMap* m, const void* base, uint64_t rows, uint64_t K, 
   return r == CUDA_SUCCESS ? 0 : -3;
 }
 
+// A bf16 cache [pages, 64 tokens, G heads, D] with strides in elements; box = 64 channels of one head of a whole page, 128-byte swizzle.
+// Channels from D on are zero-filled.
+int make_tmap_page(CUtensorMap* m, const void* base, uint64_t pages, uint64_t G, uint64_t D, uint64_t tok, uint64_t page) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return -1;
+  if ((reinterpret_cast<uintptr_t>(base) & 15) || ((D | tok | page) & 7)) return -2;
+  cuuint64_t dims[4] = {D, G, 64, pages};
+  cuuint64_t strides[3] = {D * 2, tok * 2, page * 2};
+  cuuint32_t box[4] = {64, 1, 64, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : -3;
+}
+
 static int num_sms() {
   static int n = 0;
   if (!n) { int dev; cudaGetDevice(&dev); cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev); }

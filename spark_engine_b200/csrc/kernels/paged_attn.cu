@@ -45,18 +45,6 @@ __device__ __forceinline__ float head_factor(const PagedAttn& a, int pr, int h) 
   return a.gate ? a.out_scale * sigmoid_f(ldf(static_cast<const T*>(a.gate) + static_cast<size_t>(pr) * a.ldg + h)) : a.out_scale;
 }
 
-// tanh to fp32 accuracy in the sense of the soft cap: the Taylor polynomial near 0 (where the quotient form would cancel),
-// 1 - 2 / (exp(2z) + 1) elsewhere (absolute error of a few 2^-23).  The polynomial gives tanh(z) / z.
-constexpr float CAP_NEAR = 0.25f;
-__device__ __forceinline__ float tanh_over_z(float z) {
-  const float s = z * z;
-  return fmaf(s, fmaf(s, fmaf(s, fmaf(s, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f);
-}
-__device__ __forceinline__ float cap_tanh(float z) {
-  const float near = z * tanh_over_z(z), far = 1.f - __fdividef(2.f, 1.f + __expf(2.f * fminf(z, 40.f)));
-  return fabsf(z) < CAP_NEAR ? near : far;
-}
-
 // ------------------------------------------------------------------------------------------------ short convolution
 struct ConvPrep {
   const void* proj; const float* w;      // [rows, ldp]; [taps, C]

@@ -29,10 +29,10 @@ tree_tile_kernel(const __grid_constant__ TreeAttn a) {
   const int t = threadIdx.x, ty = t >> 4, tx = t & 15;
   pdl_wait();
   pdl_trigger();
-  TreeRange range = ta_range<TT_THREADS, TT_BM>(a, sh);
+  TreeRange range = ta_range<TT_THREADS>(a, sh);
   if (t == 0) a.split[blockIdx.x] = make_int4(0, 0, 0, 0);
   TreeItem it;
-  while (ta_next<TT_BM>(a, range, it)) {
+  while (ta_next(a, range, it)) {
     const TreeSeg& sg = it.seg;
     const int slot = a.slots ? a.slots[it.s] : it.s, pairs = min(TT_BM, sg.n * rep - it.rt * TT_BM);
     __syncthreads();
@@ -200,7 +200,7 @@ tree_tile_kernel(const __grid_constant__ TreeAttn a) {
 
 // ------------------------------------------------------------------------------------------------ merge
 // grid (ctas, row groups); 256 threads, `wpr` warps per row.  Parts in ascending order within a warp, warps in ascending order.
-template <typename T, int BM>
+template <typename T>
 __global__ void __launch_bounds__(256)
 tree_merge_kernel(const __grid_constant__ TreeAttn a, int wpr) {
   __shared__ float4 s_o[8][128];
@@ -216,12 +216,12 @@ tree_merge_kernel(const __grid_constant__ TreeAttn a, int wpr) {
       }
   const int4 sp = a.split[c];
   if (sp.x <= 1) return;
-  const TreeSeg sg = ta_segment<BM>(a, sp.y);
-  const int rpb = 8 / wpr, sub = warp % wpr, row = blockIdx.y * rpb + warp / wpr, f = sp.w * BM + row;
-  if (static_cast<int>(blockIdx.y) * rpb >= min(BM, sg.n * rep - sp.w * BM)) return;
-  const bool on = row < BM && f < sg.n * rep;
+  const TreeSeg sg = ta_segment(a, sp.y);
+  const int rpb = 8 / wpr, sub = warp % wpr, row = blockIdx.y * rpb + warp / wpr, f = sp.w * a.bm + row;
+  if (static_cast<int>(blockIdx.y) * rpb >= min(a.bm, sg.n * rep - sp.w * a.bm)) return;
+  const bool on = row < a.bm && f < sg.n * rep;
   // part 0 lies behind the others' in its CTA's pair, see TreeAttn
-  auto part = [&](int i) { return (static_cast<size_t>(c + i) * 2 + (i == 0 ? 1 : 0)) * BM + row; };
+  auto part = [&](int i) { return (static_cast<size_t>(c + i) * 2 + (i == 0 ? 1 : 0)) * a.bm + row; };
   float m = -INFINITY, l = 0.f;
   if (on)
     for (int i = sub; i < sp.x; i += wpr) m = fmaxf(m, a.part_ml[part(i) * 2]);
@@ -307,20 +307,25 @@ static int launch_tile(const TreeAttn& a, cudaStream_t s) {
 }
 template <typename T>
 static int launch_tiles(const TreeAttn& a, cudaStream_t s) {
-  const int rc = a.V <= 128 ? launch_tile<T, 1>(a, s) : a.V <= 256 ? launch_tile<T, 2>(a, s) : launch_tile<T, 4>(a, s);
-  if (rc) return rc;
-  const int wpr = 8;
-  spark_launch_pdl(tree_merge_kernel<T, TT_BM>, dim3(a.ctas, TT_BM * wpr / 8), dim3(256), 0, s, dim3(1, 1, 1), a, wpr);
-  return spark_launch_rc("spark_tree_attn");
+  return a.V <= 128 ? launch_tile<T, 1>(a, s) : a.V <= 256 ? launch_tile<T, 2>(a, s) : launch_tile<T, 4>(a, s);
 }
+
+int launch_tree_tc(const TreeAttn& a, cudaStream_t s);       // tree_attn_tc.cu
 
 }  // namespace spark
 
 using namespace spark;
 
-extern "C" int spark_tree_attn(const TreeAttn* a, int f32, cudaStream_t s) {
+// tc: the tensor-core kernel (bf16, head widths of up to 256; bm 128 or 256), else the FP32 units (bm 32).
+extern "C" int spark_tree_attn(const TreeAttn* a, int f32, int tc, cudaStream_t s) {
   if (a->S <= 0 || a->R <= 0) return 0;
   if (a->H <= 0 || a->G <= 0 || a->H % a->G || a->D <= 0 || a->V <= 0 || ((a->D | a->V) & 7) || a->D > 512 || a->V > 512 || a->ctas <= 0 ||
       a->min_tiles <= 0 || (a->bias && a->bias_n <= 0) || a->page_ld <= 0 || ((a->ldq | a->hq | a->ldo | a->ho) & 3)) return -5;
-  return f32 ? launch_tiles<float>(*a, s) : launch_tiles<__nv_bfloat16>(*a, s);
+  if (tc ? f32 || (a->bm != 128 && a->bm != 256) : a->bm != TT_BM) return -5;
+  if (const int rc = tc ? launch_tree_tc(*a, s) : f32 ? launch_tiles<float>(*a, s) : launch_tiles<__nv_bfloat16>(*a, s)) return rc;
+  const int wpr = 8;
+  const dim3 grid(a->ctas, a->bm * wpr / 8);
+  if (f32) spark_launch_pdl(tree_merge_kernel<float>, grid, dim3(256), 0, s, dim3(1, 1, 1), *a, wpr);
+  else spark_launch_pdl(tree_merge_kernel<__nv_bfloat16>, grid, dim3(256), 0, s, dim3(1, 1, 1), *a, wpr);
+  return spark_launch_rc("spark_tree_attn");
 }

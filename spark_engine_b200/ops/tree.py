@@ -57,12 +57,12 @@ class _CommitPaths(C.Structure):
 class _TreeAttn(C.Structure):
     _fields_ = _struct((_p, "q k v out starts lengths slots pos pages anc bias slopes sink gate part_o part_ml split status"),
                        (_l, "k_page k_tok v_page v_tok"),
-                       (_i, "S R words page_ld n_slots n_pages H G D V ldq hq ldo ho ldg bias_n window chunk ctas min_tiles zero_rest"),
+                       (_i, "S R words page_ld n_slots n_pages H G D V ldq hq ldo ho ldg bias_n window chunk bm ctas min_tiles zero_rest"),
                        (_f, "scale cap out_scale"))
 
 
 _SIGS = {"spark_block_tables": [_p, _p], "spark_slot_maps": [_p, _p], "spark_path_conv": [_p, _i, _p], "spark_commit_paths": [_p, _i, _i, _p],
-         "spark_tree_attn": [_p, _i, _p]}
+         "spark_tree_attn": [_p, _i, _i, _p]}
 _bound = None
 
 
@@ -360,7 +360,13 @@ def tree_attention(q, k, v, maps: RowMaps, scale: float, softcap: float = 0.0, b
     q = _rows16(q)
     cu = _cu()
     sms = torch.cuda.get_device_properties(dev).multi_processor_count
-    ctas, bm = 3 * sms, 32
+    # tensor cores: one tile of 128 (node, head) rows per CTA and two CTAs per SM, or two tiles that share the keys (trees of more rows)
+    tc = dt == torch.bfloat16 and max(D, V) <= 256
+    if tc:
+        bm = 256 if max(D, V) <= 128 and min(maps.nodes or R, R) * (H // G) > 128 else 128
+        ctas = sms if bm == 256 or max(D, V) > 128 else 2 * sms
+    else:
+        bm, ctas = 32, 3 * sms
     part_o = torch.empty(ctas * 2 * bm * V, dtype=torch.float32, device=dev)
     part_ml = torch.empty(ctas * 2 * bm * 2, dtype=torch.float32, device=dev)
     split = torch.empty(ctas * 4, dtype=torch.int32, device=dev)
@@ -369,8 +375,8 @@ def tree_attention(q, k, v, maps: RowMaps, scale: float, softcap: float = 0.0, b
                   P(sink), P(gate), P(part_o), P(part_ml), P(split), P(cu.status_word(dev)), kp, kt, vp, vt, maps.lengths.shape[0], R,
                   maps.anc.shape[1] if maps.anc is not None else 0, maps.tables.shape[1], maps.tables.shape[0], k.shape[0], H, G, D, V, q.stride(0),
                   q.stride(1), out.stride(0), out.stride(1), gate.stride(0) if gate is not None else 0, bias.shape[1] if bias is not None else 0, window,
-                  chunk, ctas, 1, int(fresh), scale, softcap, out_scale)
-    _call("spark_tree_attn", dev, C.byref(a), int(dt == torch.float32))
+                  chunk, bm, ctas, 1, int(fresh), scale, softcap, out_scale)
+    _call("spark_tree_attn", dev, C.byref(a), int(dt == torch.float32), int(tc))
     return out
 
 
