@@ -21,10 +21,10 @@ struct TreeAttn {
   const float *bias, *slopes, *sink;     // [H, bias_n], [H], [H]
   const void* gate;                      // [R, H], rows ldg apart
   float *part_o, *part_ml;               // [ctas][2][bm][V], [ctas][2][bm][2]: of a tile begun before the CTA, of one that goes on behind it
-  int4* split;                           // [ctas]: parts of the item that begins in this CTA and ends in another (0: none), request, head, tile
+  int4* split;                           // [ctas]: the item that begins in this CTA and ends in another, see ta_split
   int* status;
   long long k_page, k_tok, v_page, v_tok;                    // strides in elements
-  int S, R, words, page_ld, n_slots, n_pages, H, G, D, V, ldq, hq, ldo, ho, ldg, bias_n, window, chunk, bm, ctas, min_tiles, zero_rest;
+  int S, R, words, page_ld, n_slots, n_pages, H, G, D, V, ldq, hq, ldo, ho, ldg, bias_n, window, chunk, bm, sms, ctas, min_tiles, zero_rest;
   float scale, cap, out_scale;
 };
 
@@ -123,6 +123,12 @@ __device__ __forceinline__ bool ta_next(const TreeAttn& a, TreeRange& r, TreeIte
   r.count -= it.nj;
   r.rem += it.nj;
   return true;
+}
+
+// What the second launch needs of an item: (parts, first row of the request, head, first pair and pairs of the tile).
+__device__ __forceinline__ int4 ta_split(const TreeAttn& a, const TreeItem& it) {
+  const int pairs = it.seg.n * (a.H / a.G) - it.rt * a.bm;
+  return make_int4(it.parts | (pairs < a.bm ? pairs : a.bm) << 16, it.seg.r0, it.g, it.rt * a.bm);
 }
 
 template <typename T>

@@ -166,7 +166,7 @@ tree_tile_kernel(const __grid_constant__ TreeAttn a) {
     }
     // ---- whole: the rows' outputs; else this CTA's part of them
     const bool whole = it.first && it.last;
-    if (it.first && !it.last && t == 0) a.split[blockIdx.x] = make_int4(it.parts, it.s, it.g, it.rt);
+    if (it.first && !it.last && t == 0) a.split[blockIdx.x] = ta_split(a, it);
     const size_t pb = (static_cast<size_t>(blockIdx.x) * 2 + (it.first ? 1 : 0)) * TT_BM;
     if (!whole && t < pairs) { a.part_ml[(pb + t) * 2] = s_m[t]; a.part_ml[(pb + t) * 2 + 1] = s_l[t]; }
 #pragma unroll
@@ -199,99 +199,132 @@ tree_tile_kernel(const __grid_constant__ TreeAttn a) {
 }
 
 // ------------------------------------------------------------------------------------------------ merge
-// grid (ctas, row groups); 256 threads, `wpr` warps per row.  Parts in ascending order within a warp, warps in ascending order.
+constexpr int TM_THREADS = 256, TM_WARPS = TM_THREADS / 32, TM_MAX_CTAS = 1024;
+
+// Every CTA makes the list of the split items' rows (a row per item that begins in one CTA of the first launch and ends in another) and
+// takes its share of them; the fewer there are, the more warps join one row.  Parts are added in ascending order within a warp, warps in
+// ascending order.
 template <typename T>
-__global__ void __launch_bounds__(256)
-tree_merge_kernel(const __grid_constant__ TreeAttn a, int wpr) {
-  __shared__ float4 s_o[8][128];
-  __shared__ float s_ml[8][2];
+__global__ void __launch_bounds__(TM_THREADS)
+tree_merge_kernel(const __grid_constant__ TreeAttn a) {
+  __shared__ long long sh[TM_WARPS + 2];
+  __shared__ int s_first[TM_MAX_CTAS + 1];                   // rows of the items in front of CTA c's
+  __shared__ float4 s_o[TM_WARPS][128];
+  __shared__ float s_ml[TM_WARPS][2];
   pdl_wait();
   pdl_trigger();
-  const int t = threadIdx.x, warp = t >> 5, lane = t & 31, c = blockIdx.x, V4 = a.V >> 2, rep = a.H / a.G;
-  if (a.zero_rest && blockIdx.y == 0)
-    for (int r = a.starts[a.S] + c; r < a.R; r += gridDim.x)
-      for (int i = t; i < a.H * V4; i += 256) {
+  const int t = threadIdx.x, warp = t >> 5, lane = t & 31, V4 = a.V >> 2, rep = a.H / a.G;
+  if (a.zero_rest)
+    for (int r = a.starts[a.S] + blockIdx.x; r < a.R; r += gridDim.x)
+      for (int i = t; i < a.H * V4; i += TM_THREADS) {
         const int h = i / V4;
         stf4(static_cast<T*>(a.out) + static_cast<size_t>(r) * a.ldo + static_cast<size_t>(h) * a.ho + (i - h * V4) * 4, make_float4(0.f, 0.f, 0.f, 0.f));
       }
-  const int4 sp = a.split[c];
-  if (sp.x <= 1) return;
-  const TreeSeg sg = ta_segment(a, sp.y);
-  const int rpb = 8 / wpr, sub = warp % wpr, row = blockIdx.y * rpb + warp / wpr, f = sp.w * a.bm + row;
-  if (static_cast<int>(blockIdx.y) * rpb >= min(a.bm, sg.n * rep - sp.w * a.bm)) return;
-  const bool on = row < a.bm && f < sg.n * rep;
-  // part 0 lies behind the others' in its CTA's pair, see TreeAttn
-  auto part = [&](int i) { return (static_cast<size_t>(c + i) * 2 + (i == 0 ? 1 : 0)) * a.bm + row; };
-  float m = -INFINITY, l = 0.f;
-  if (on)
-    for (int i = sub; i < sp.x; i += wpr) m = fmaxf(m, a.part_ml[part(i) * 2]);
-  float4 o[4] = {};
-  const float ref = m == -INFINITY ? 0.f : m;
-  if (on)
-    for (int i0 = sub; i0 < sp.x; i0 += 4 * wpr) {           // four parts in flight
+  const int each = (a.ctas + TM_THREADS - 1) / TM_THREADS;   // up to four
+  int n[4], mine = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int c = t * each + i;
+    n[i] = i < each && c < a.ctas ? a.split[c].x >> 16 : 0;
+    mine += n[i];
+  }
+  long long total;
+  int before = static_cast<int>(ta_prefix<TM_THREADS>(mine, sh, total));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (i < each && t * each + i < a.ctas) s_first[t * each + i] = before;
+    before += n[i];
+  }
+  const int rows = static_cast<int>(total);
+  if (t == 0) s_first[a.ctas] = rows;
+  __syncthreads();
+  int wpr = TM_WARPS;
+  while (wpr > 1 && rows * wpr > static_cast<int>(gridDim.x) * TM_WARPS) wpr >>= 1;
+  const int rpb = TM_WARPS / wpr, sub = warp & (wpr - 1);
+  for (int task0 = blockIdx.x * rpb; task0 < rows; task0 += gridDim.x * rpb) {
+    const int task = task0 + warp / wpr;
+    const bool on = task < rows;
+    int lo = 0, hi = a.ctas;                                 // the last CTA whose rows begin at or before the task
+    while (hi - lo > 1) { const int m = (lo + hi) >> 1; if (s_first[m] <= task) lo = m; else hi = m; }
+    const int c = lo, row = on ? task - s_first[lo] : 0;
+    const int4 sp = a.split[c];
+    const int parts = on ? sp.x & 0xffff : 0;
+    // part 0 lies behind the others' in its CTA's pair, see TreeAttn
+    auto part = [&](int i) { return (static_cast<size_t>(c + i) * 2 + (i == 0 ? 1 : 0)) * a.bm + row; };
+    float m = -INFINITY, l = 0.f;
+    float4 o[4] = {};
+    for (int i0 = sub; i0 < parts; i0 += 4 * wpr) {          // four parts in flight
       float4 x[4][4];
-      float w[4];
+      float2 ml[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const int i = i0 + u * wpr;
-        w[u] = 0.f;
-        if (i >= sp.x) continue;
-        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + part(i) * 2);
-        w[u] = expf(ml.x - ref);
-        l = fmaf(w[u], ml.y, l);
+        ml[u] = i < parts ? __ldcg(reinterpret_cast<const float2*>(a.part_ml + part(i) * 2)) : make_float2(-INFINITY, 0.f);
 #pragma unroll
         for (int v = 0; v < 4; ++v)
-          if (lane + v * 32 < V4) x[u][v] = __ldcg(reinterpret_cast<const float4*>(a.part_o + part(i) * a.V) + lane + v * 32);
+          if (i < parts && lane + v * 32 < V4) x[u][v] = __ldcg(reinterpret_cast<const float4*>(a.part_o + part(i) * a.V) + lane + v * 32);
       }
+      const float top = fmaxf(m, fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x))), ref = top == -INFINITY ? 0.f : top;
+      const float k = expf(m - ref);
+      m = top;
+      l *= k;
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
-        if (w[u] != 0.f)
+      for (int v = 0; v < 4; ++v) { o[v].x *= k; o[v].y *= k; o[v].z *= k; o[v].w *= k; }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float w = expf(ml[u].x - ref);
+        if (w == 0.f) continue;
+        l = fmaf(w, ml[u].y, l);
+#pragma unroll
+        for (int v = 0; v < 4; ++v)
+          if (lane + v * 32 < V4) {
+            o[v].x = fmaf(w, x[u][v].x, o[v].x); o[v].y = fmaf(w, x[u][v].y, o[v].y);
+            o[v].z = fmaf(w, x[u][v].z, o[v].z); o[v].w = fmaf(w, x[u][v].w, o[v].w);
+          }
+      }
+    }
+    if (wpr > 1) {
+      __syncthreads();                                       // (the task before has been read)
+      if (lane == 0) { s_ml[warp][0] = m; s_ml[warp][1] = l; }
+#pragma unroll
+      for (int v = 0; v < 4; ++v)
+        if (lane + v * 32 < V4) s_o[warp][lane + v * 32] = o[v];
+      __syncthreads();
+      if (sub == 0) {
+        for (int i = 1; i < wpr; ++i) m = fmaxf(m, s_ml[warp + i][0]);
+        const float ref = m == -INFINITY ? 0.f : m, c0 = expf(s_ml[warp][0] - ref);
+        l *= c0;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) { o[v].x *= c0; o[v].y *= c0; o[v].z *= c0; o[v].w *= c0; }
+        for (int i = 1; i < wpr; ++i) {
+          const float w = expf(s_ml[warp + i][0] - ref);
+          if (w == 0.f) continue;
+          l = fmaf(w, s_ml[warp + i][1], l);
 #pragma unroll
           for (int v = 0; v < 4; ++v)
             if (lane + v * 32 < V4) {
-              o[v].x = fmaf(w[u], x[u][v].x, o[v].x); o[v].y = fmaf(w[u], x[u][v].y, o[v].y);
-              o[v].z = fmaf(w[u], x[u][v].z, o[v].z); o[v].w = fmaf(w[u], x[u][v].w, o[v].w);
+              const float4 y = s_o[warp + i][lane + v * 32];
+              o[v].x = fmaf(w, y.x, o[v].x); o[v].y = fmaf(w, y.y, o[v].y); o[v].z = fmaf(w, y.z, o[v].z); o[v].w = fmaf(w, y.w, o[v].w);
             }
+        }
+      }
     }
-  if (wpr > 1) {
-    if (lane == 0) { s_ml[warp][0] = m; s_ml[warp][1] = l; }
+    if (!on || sub) continue;
+    const int f = sp.w + row, h = sp.z * rep + f % rep, r = sp.y + f / rep;
+    float k = 1.f;
+    if (a.sink) {
+      const float M = fmaxf(m, a.sink[h]);
+      k = expf(m - M);
+      l = l * k + expf(a.sink[h] - M);
+    }
+    float scale = l > 0.f ? ta_head_factor<T>(a, r, h) * k / l : 0.f;
+    if (l != l) scale = l;
 #pragma unroll
     for (int v = 0; v < 4; ++v)
-      if (lane + v * 32 < V4) s_o[warp][lane + v * 32] = o[v];
-    __syncthreads();
-    if (sub) return;
-    for (int i = 1; i < wpr; ++i) m = fmaxf(m, s_ml[warp + i][0]);
-    const float r2 = m == -INFINITY ? 0.f : m, c0 = expf(s_ml[warp][0] - r2);
-    l *= c0;
-#pragma unroll
-    for (int v = 0; v < 4; ++v) { o[v].x *= c0; o[v].y *= c0; o[v].z *= c0; o[v].w *= c0; }
-    for (int i = 1; i < wpr; ++i) {
-      const float ci = expf(s_ml[warp + i][0] - r2);
-      if (ci == 0.f) continue;
-      l = fmaf(ci, s_ml[warp + i][1], l);
-#pragma unroll
-      for (int v = 0; v < 4; ++v)
-        if (lane + v * 32 < V4) {
-          const float4 x = s_o[warp + i][lane + v * 32];
-          o[v].x = fmaf(ci, x.x, o[v].x); o[v].y = fmaf(ci, x.y, o[v].y); o[v].z = fmaf(ci, x.z, o[v].z); o[v].w = fmaf(ci, x.w, o[v].w);
-        }
-    }
+      if (lane + v * 32 < V4)
+        stf4(static_cast<T*>(a.out) + static_cast<size_t>(r) * a.ldo + static_cast<size_t>(h) * a.ho + (lane + v * 32) * 4,
+             make_float4(o[v].x * scale, o[v].y * scale, o[v].z * scale, o[v].w * scale));
   }
-  if (!on) return;
-  const int h = sp.z * rep + f % rep, r = sg.r0 + f / rep;
-  float k = 1.f;
-  if (a.sink) {
-    const float M = fmaxf(m, a.sink[h]);
-    k = expf(m - M);
-    l = l * k + expf(a.sink[h] - M);
-  }
-  float scale = l > 0.f ? ta_head_factor<T>(a, r, h) * k / l : 0.f;
-  if (l != l) scale = l;
-#pragma unroll
-  for (int v = 0; v < 4; ++v)
-    if (lane + v * 32 < V4)
-      stf4(static_cast<T*>(a.out) + static_cast<size_t>(r) * a.ldo + static_cast<size_t>(h) * a.ho + (lane + v * 32) * 4,
-           make_float4(o[v].x * scale, o[v].y * scale, o[v].z * scale, o[v].w * scale));
 }
 
 constexpr int TA_SMEM = 220 * 1024;
@@ -319,13 +352,12 @@ using namespace spark;
 // tc: the tensor-core kernel (bf16, head widths of up to 256; bm 128 or 256), else the FP32 units (bm 32).
 extern "C" int spark_tree_attn(const TreeAttn* a, int f32, int tc, cudaStream_t s) {
   if (a->S <= 0 || a->R <= 0) return 0;
-  if (a->H <= 0 || a->G <= 0 || a->H % a->G || a->D <= 0 || a->V <= 0 || ((a->D | a->V) & 7) || a->D > 512 || a->V > 512 || a->ctas <= 0 ||
+  if (a->H <= 0 || a->G <= 0 || a->H % a->G || a->D <= 0 || a->V <= 0 || ((a->D | a->V) & 7) || a->D > 512 || a->V > 512 || a->ctas <= 0 || a->ctas > TM_MAX_CTAS || a->sms <= 0 ||
       a->min_tiles <= 0 || (a->bias && a->bias_n <= 0) || a->page_ld <= 0 || ((a->ldq | a->hq | a->ldo | a->ho) & 3)) return -5;
   if (tc ? f32 || (a->bm != 128 && a->bm != 256) : a->bm != TT_BM) return -5;
   if (const int rc = tc ? launch_tree_tc(*a, s) : f32 ? launch_tiles<float>(*a, s) : launch_tiles<__nv_bfloat16>(*a, s)) return rc;
-  const int wpr = 8;
-  const dim3 grid(a->ctas, a->bm * wpr / 8);
-  if (f32) spark_launch_pdl(tree_merge_kernel<float>, grid, dim3(256), 0, s, dim3(1, 1, 1), *a, wpr);
-  else spark_launch_pdl(tree_merge_kernel<__nv_bfloat16>, grid, dim3(256), 0, s, dim3(1, 1, 1), *a, wpr);
+  const dim3 grid(2 * a->sms);
+  if (f32) spark_launch_pdl(tree_merge_kernel<float>, grid, dim3(TM_THREADS), 0, s, dim3(1, 1, 1), *a);
+  else spark_launch_pdl(tree_merge_kernel<__nv_bfloat16>, grid, dim3(TM_THREADS), 0, s, dim3(1, 1, 1), *a);
   return spark_launch_rc("spark_tree_attn");
 }

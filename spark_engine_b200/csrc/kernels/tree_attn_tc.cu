@@ -7,9 +7,9 @@
 // Weights enter the product as two bf16 terms (2^-17 of a weight is lost), so that the reference of the exponentials may lag behind the
 // maximum: the accumulator is rescaled only when a row's maximum outgrew its reference by 2^8.
 //
-// A page that not every row sees whole (the tree itself, the edge of a window or chunk) is masked by 64 bits per row.  Its values are looked
+// A page that not every row sees whole (the tree itself, the edge of a window or chunk) is masked by 64 bits per row.  Warp 1 looks its values
 // over first: rows that hold no token of the request are zeroed, and where a value is not finite, 0 * value would spoil the rows that do not
-// see it, so it is added by hand for the rows that do and zeroed in front of the product.
+// see it, so the softmax warps add it by hand for the rows that do and zero it in front of the product.
 #include "../common/tree_work.cuh"
 
 namespace spark {
@@ -21,8 +21,9 @@ constexpr float TC_LAG = 8.f;                                // log2
 template <int DC, int NQ> struct Tc {
   static constexpr bool QT = DC == 256;                      // queries in tensor memory: shared memory has no room for them beside the ring
   static constexpr int SLOT = TA_PAGE * DC * 2, Q_BYTES = QT ? 0 : 128 * DC * 2;
-  static constexpr int SLOTS = DC == 256 ? 6 : DC == 128 ? (NQ == 2 ? 9 : 4) : (NQ == 2 ? 16 : 8);
-  static constexpr int SMEM = NQ * Q_BYTES + SLOTS * SLOT + 1024 + 1024;
+  static constexpr int SLOTS = DC == 256 ? 5 : DC == 128 ? (NQ == 2 ? 9 : 4) : (NQ == 2 ? 16 : 8);
+  static constexpr int STAGE = QT ? 32768 : Q_BYTES;         // of a tile's results on their way out, over its queries where those are there
+  static constexpr int SMEM = NQ * STAGE + SLOTS * SLOT + 1024 + 1024;
   // per tile: two buffers of scores / weights of 64 columns, the accumulator
   static constexpr int TILE_COLS = 128 + DC, Q_COL = 128 + DC;
   static constexpr int COLS = QT || NQ == 2 ? 512 : 256;
@@ -43,8 +44,29 @@ __device__ __forceinline__ uint64_t tc_desc_nmajor(uint32_t addr, uint32_t chunk
   return static_cast<uint64_t>((addr & 0x3FFFF) >> 4) | static_cast<uint64_t>(chunk >> 4) << 16 | static_cast<uint64_t>(1024 >> 4) << 32 |
          static_cast<uint64_t>(1) << 46 | static_cast<uint64_t>(2) << 61;
 }
-__device__ __forceinline__ bool tc_odd(uint32_t w) {         // one of two bf16 is not finite
-  return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
+__device__ __forceinline__ float tc_ex2(float x) {          // relative error 2^-22, results below 2^-126 are 0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// two fp32 at a time
+__device__ __forceinline__ uint64_t tc_two(float x, float y) { return static_cast<uint64_t>(__float_as_uint(y)) << 32 | __float_as_uint(x); }
+__device__ __forceinline__ float tc_lo(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v)); }
+__device__ __forceinline__ float tc_hi(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
+__device__ __forceinline__ uint64_t tc_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t tc_add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t tc_mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
 }
 // All softmax warps of the item (4 or 8): a barrier whose wait ends.
 __device__ __forceinline__ bool tc_sync(uint64_t* bar, uint32_t& phase) {
@@ -91,17 +113,18 @@ template <int DC, int NQ, bool FEAT>
 __global__ void __launch_bounds__(Tc<DC, NQ>::THREADS, Tc<DC, NQ>::PER_SM)
 tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ TreeAttn a) {
   using L = Tc<DC, NQ>;
-  constexpr int CH = DC / 64, SLOT = L::SLOT, SLOTS = L::SLOTS, KV_CHUNK = TA_PAGE * 128, Q_CHUNK = 128 * 128, NT = L::THREADS;
+  constexpr int SLOT = L::SLOT, SLOTS = L::SLOTS, KV_CHUNK = TA_PAGE * 128, Q_CHUNK = 128 * 128, NT = L::THREADS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* ring = smem + NQ * L::Q_BYTES;
+  uint8_t* ring = smem + NQ * L::STAGE;
   uint64_t* full = reinterpret_cast<uint64_t*>(ring + SLOTS * SLOT);
   uint64_t* empty = full + SLOTS;
   uint64_t* q_full = empty + SLOTS;                          // [NQ]
   uint64_t* s_full = q_full + NQ;                            // [NQ][2] from here on
   uint64_t* p_full = s_full + 2 * NQ;
   uint64_t* o_full = p_full + 2 * NQ;
-  uint64_t* v_sync = o_full + 2 * NQ;                        // [NQ]: of 4 and of 8 softmax warps
+  uint64_t* v_seen = o_full + 2 * NQ;                        // [NQ]: warp 1 has looked over a masked page's values
+  uint64_t* v_sync = v_seen + NQ;                            // [NQ]: of 4 and of 8 softmax warps
   long long* sh = reinterpret_cast<long long*>(v_sync + NQ); // [NT / 32 + 2]
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(sh + NT / 32 + 2);
   uint32_t* odd_rows = tmem_ptr + 1;                         // [2]: tokens of a masked page with a value that is not finite
@@ -109,9 +132,8 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV);
     for (int s = 0; s < SLOTS; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-    for (int s = 0; s < NQ; ++s) { mbar_init(&q_full[s], 4); mbar_init(&v_sync[s], 4 * (s + 1)); }
+    for (int s = 0; s < NQ; ++s) { mbar_init(&q_full[s], 4); mbar_init(&v_seen[s], 1); mbar_init(&v_sync[s], 4 * (s + 1)); }
     for (int s = 0; s < 2 * NQ; ++s) { mbar_init(&s_full[s], 1); mbar_init(&p_full[s], 4); mbar_init(&o_full[s], 1); }
-    odd_rows[0] = odd_rows[1] = 0u;
     fence_barrier_init();
   }
   if (warp == 1) { tmem_alloc<L::COLS>(tmem_ptr); tmem_relinquish(); }
@@ -160,8 +182,9 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     // ------------------------------------------------------------ MMA issuer (the whole warp walks, one elected lane issues)
     const int ksteps = (a.D + 15) / 16, vn = (a.V + 15) / 16 * 16;
     const uint32_t id_s = make_idesc(1, 1, 128, TA_PAGE), id_o = make_idesc(1, 1, 128, vn) | (1u << 16);
-    const uint32_t qs = __shfl_sync(0xffffffffu, smem_u32(smem), 0), rs = qs + NQ * L::Q_BYTES, tm = __shfl_sync(0xffffffffu, tmem, 0);
+    const uint32_t qs = __shfl_sync(0xffffffffu, smem_u32(smem), 0), rs = qs + NQ * L::STAGE, tm = __shfl_sync(0xffffffffu, tmem, 0);
     TcCount c;
+    const int vunits = (a.V + 63) / 64 * 8;
     int n[NQ] = {}, items[NQ] = {};                          // pages and items of each tile so far
     while (ok && ta_next(a, range, it)) {
       const int pairs = it.seg.n * rep - it.rt * a.bm, act = NQ == 2 && pairs > 128 ? 2 : 1;
@@ -172,6 +195,8 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
           ++items[q];
         }
       if (!ok) { set_status(a.status, ST_TIMEOUT_MBAR_FULL, blockIdx.x, it.s, -2); break; }
+      const int slot = a.slots ? a.slots[it.s] : it.s, edge = ta_first_visible(a, it.seg.len + it.seg.n - 1);
+      uint32_t there = 0u;                                   // pages of the current 32 that the table leads to
       for (int j = -1; j < it.nj && ok; ++j) {
         if (j + 1 < it.nj) {
           ok = __all_sync(0xffffffffu, mbar_wait(&full[c.slot], c.ph));
@@ -188,7 +213,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
               for (int k = 0; k < ksteps; ++k) {
                 const uint64_t kd = make_smem_desc_sw128(rs + c.slot * SLOT + (k >> 2) * KV_CHUNK) + 2 * (k & 3);
                 if (L::QT) umma_f16_ts(d, tm + L::Q_COL + k * 8, kd, id_s, k != 0);
-                else umma_f16(d, make_smem_desc_sw128(qs + q * L::Q_BYTES + (k >> 2) * Q_CHUNK) + 2 * (k & 3), kd, id_s, k != 0);
+                else umma_f16(d, make_smem_desc_sw128(qs + q * L::STAGE + (k >> 2) * Q_CHUNK) + 2 * (k & 3), kd, id_s, k != 0);
               }
               umma_commit(&s_full[q * 2 + b]);
             }
@@ -200,7 +225,37 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
           tc_step<SLOTS>(c);
         }
         if (j < 0) continue;
+        if ((j & 31) == 0) there = __ballot_sync(0xffffffffu, j + lane < it.nj && ta_page(a, slot, it.j + j + lane) >= 0);
         ok = __all_sync(0xffffffffu, mbar_wait(&full[c.slot], c.ph));
+        const int tok0 = (it.j + j) * TA_PAGE;
+        if (ok && (tok0 + TA_PAGE > it.seg.len || tok0 < edge || !((there >> (j & 31)) & 1u))) {
+          // ---- a masked page's values: tokens that are not the request's are zeroed, the others with a value that is not finite noted
+          const int valid = (there >> (j & 31)) & 1u ? min(TA_PAGE, it.seg.len + it.seg.n - tok0) : 0;
+          uint32_t odd[2];
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const int tok = half * 32 + lane;
+            uint8_t* vrow = ring + c.slot * SLOT + tok * 128;
+            uint32_t most = 0u;                              // largest exponents of the row's even and odd columns
+            for (int u = 0; u < vunits; ++u) {
+              uint4* x = reinterpret_cast<uint4*>(vrow + (u >> 3) * KV_CHUNK + (((u & 7) ^ (tok & 7)) * 16));
+              if (tok >= valid) *x = make_uint4(0u, 0u, 0u, 0u);
+              else {
+                const uint4 v = *x;
+                most = __vmaxu2(__vmaxu2(most, v.x & 0x7f807f80u), __vmaxu2(v.y & 0x7f807f80u, __vmaxu2(v.z & 0x7f807f80u, v.w & 0x7f807f80u)));
+              }
+            }
+            odd[half] = __ballot_sync(0xffffffffu, (most & 0xffffu) == 0x7f80u || (most >> 16) == 0x7f80u);
+          }
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) {
+            odd_rows[0] = odd[0]; odd_rows[1] = odd[1];
+#pragma unroll
+            for (int q = 0; q < NQ; ++q)
+              if (q < act) mbar_arrive(&v_seen[q]);
+          }
+        }
 #pragma unroll
         for (int q = 0; q < NQ; ++q) {
           if (q >= act) continue;
@@ -234,14 +289,14 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     const int q = NQ == 2 ? (warp - 2) >> 2 : 0, quad = warp & 3, row = quad * 32 + lane;
     const uint32_t t_lane = tmem + (static_cast<uint32_t>(quad * 32) << 16) + q * L::TILE_COLS;
     const int vn = (a.V + 15) / 16 * 16, vn_units = (a.V + 63) / 64 * 8;
-    uint32_t sync_phase[NQ] = {};
+    uint32_t sync_phase[NQ] = {}, seen_phase = 0u;
     int n = 0, seq = 0;                                      // pages of this tile so far; position of the item in the ring's sequence
     while (ok && ta_next(a, range, it)) {
       const TreeSeg& sg = it.seg;
-      const int all = sg.n * rep - it.rt * a.bm, pairs = min(128, all - q * 128);      // rows of this tile
+      const int all = sg.n * rep - it.rt * a.bm, pairs = min(128, all - q * 128);        // rows of this tile
       const int seq0 = seq;
       seq += 2 * it.nj;
-      if (it.first && !it.last && threadIdx.x == 64) a.split[blockIdx.x] = make_int4(it.parts, it.s, it.g, it.rt);
+      if (it.first && !it.last && threadIdx.x == 64) a.split[blockIdx.x] = ta_split(a, it);
       if (pairs <= 0) continue;
       const bool both = NQ == 2 && all > 128;
       uint64_t* sync = &v_sync[both ? NQ - 1 : 0];
@@ -266,7 +321,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
 #pragma unroll 8
           for (int u = 0; u < DC / 8; ++u) {
             const uint4 v = u < units ? __ldg(src + u) : make_uint4(0u, 0u, 0u, 0u);
-            *reinterpret_cast<uint4*>(smem + q * L::Q_BYTES + (u >> 3) * Q_CHUNK + row * 128 + (((u & 7) ^ (row & 7)) * 16)) = v;
+            *reinterpret_cast<uint4*>(smem + q * L::STAGE + (u >> 3) * Q_CHUNK + row * 128 + (((u & 7) ^ (row & 7)) * 16)) = v;
           }
         }
         uint32_t z[32];
@@ -282,62 +337,83 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       float ref = -INFINITY, l = 0.f;                        // of the exponentials (FEAT: natural, else log2), and their sum
       const float c1 = FEAT ? 1.f : a.scale * TA_LOG2E;
       const int edge = ta_first_visible(a, sg.len + sg.n - 1);         // from here on every row sees committed tokens
+      uint32_t there = 0u;                                   // pages of the current 32 that the table leads to
       for (int j = 0; j < it.nj; ++j, ++n) {
         const int b = n & 1, tok0 = (it.j + j) * TA_PAGE;
-        const bool page = ta_page(a, slot, it.j + j) >= 0, whole = tok0 + TA_PAGE <= sg.len && tok0 >= edge && page;
+        if ((j & 31) == 0) there = __ballot_sync(0xffffffffu, j + lane < it.nj && ta_page(a, slot, it.j + j + lane) >= 0);
+        const bool page = (there >> (j & 31)) & 1u, whole = tok0 + TA_PAGE <= sg.len && tok0 >= edge && page;
+        uint64_t seen = ~0ull;
+        int at_lo = 0, at_hi = 0;                              // FEAT: positions of the page's tokens `lane` and 32 + lane
+        if (!whole && !idle) {
+          seen = page ? tc_mask(a, sg, tok0, node, p) : 0ull;
+          if (FEAT && tok0 + TA_PAGE > sg.len) {
+            const int n0 = tok0 + lane - sg.len, n1 = n0 + 32;
+            at_lo = n0 < 0 ? tok0 + lane : (n0 < sg.n ? a.pos[sg.r0 + n0] : p);
+            at_hi = n1 < 0 ? tok0 + lane + 32 : (n1 < sg.n ? a.pos[sg.r0 + n1] : p);
+          }
+        }
         ok = __all_sync(0xffffffffu, mbar_wait(&s_full[q * 2 + b], (n >> 1) & 1));
         if (!ok) { set_status(a.status, ST_TIMEOUT_TMEM_FULL, blockIdx.x, it.s, j); break; }
         tc_fence_after();
-        uint64_t seen = ~0ull;
         float s[64];
         if (!idle) {
-          uint32_t raw[2][32];
-          tmem_ld_32x32(t_lane + b * 64, raw[0]);
-          tmem_ld_32x32(t_lane + b * 64 + 32, raw[1]);
-          tmem_ld_wait();
+          {
+            uint32_t raw[2][32];
+            tmem_ld_32x32(t_lane + b * 64, raw[0]);
+            tmem_ld_32x32(t_lane + b * 64 + 32, raw[1]);
+            tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 64; ++i) s[i] = __uint_as_float(raw[i >> 5][i & 31]);
-          if (!whole) seen = page ? tc_mask(a, sg, tok0, node, p) : 0ull;
+            for (int i = 0; i < 64; ++i) s[i] = __uint_as_float(raw[i >> 5][i & 31]);
+          }
           if (FEAT) {
 #pragma unroll
             for (int i = 0; i < 64; ++i) s[i] *= a.scale;
             if (a.cap > 0.f) {
               const float icap = 1.f / a.cap;
+              float big = 0.f;                               // scores far below the cap need no exponential
 #pragma unroll
-              for (int i = 0; i < 64; ++i) s[i] = a.cap * cap_tanh(s[i] * icap);
+              for (int i = 0; i < 64; ++i) big = fmaxf(big, fabsf(s[i]));
+              if (__any_sync(0xffffffffu, big * icap >= CAP_NEAR)) {
+#pragma unroll
+                for (int i = 0; i < 64; ++i) s[i] = a.cap * cap_tanh(s[i] * icap);
+              } else {
+#pragma unroll
+                for (int i = 0; i < 64; ++i) s[i] *= tanh_over_z(s[i] * icap);
+              }
             }
             const int d0 = p - tok0;                         // distance of the page's token 0, were it committed
+            const bool nodes = tok0 + TA_PAGE > sg.len;
             if (a.bias) {
               const float* bh = a.bias + static_cast<size_t>(h) * a.bias_n;
-              if (tok0 + TA_PAGE <= sg.len && __all_sync(0xffffffffu, d0 - 63 >= a.bias_n - 1)) {
+              if (!nodes && __all_sync(0xffffffffu, d0 - 63 >= a.bias_n - 1)) {
                 const float far = __ldg(bh + a.bias_n - 1);
 #pragma unroll
                 for (int i = 0; i < 64; ++i) s[i] += far;
               } else {
 #pragma unroll
                 for (int i = 0; i < 64; ++i) {
-                  const int nd = tok0 + i - sg.len, d = nd < 0 ? d0 - i : (nd < sg.n ? p - __ldg(a.pos + sg.r0 + nd) : 0);
+                  const int d = nodes ? p - __shfl_sync(0xffffffffu, i < 32 ? at_lo : at_hi, i & 31) : d0 - i;
                   s[i] += __ldg(bh + min(max(d, 0), a.bias_n - 1));
                 }
               }
             }
             if (a.slopes) {
               const float sl = __ldg(a.slopes + h);
-              if (tok0 + TA_PAGE <= sg.len) {
+              if (nodes) {
 #pragma unroll
-                for (int i = 0; i < 64; ++i) s[i] -= sl * static_cast<float>(d0 - i);
+                for (int i = 0; i < 64; ++i) s[i] -= sl * static_cast<float>(p - __shfl_sync(0xffffffffu, i < 32 ? at_lo : at_hi, i & 31));
               } else {
+                // (near tokens, the ones that weigh, have a small d0: nothing is lost by taking the products apart)
+                const float s0 = sl * static_cast<float>(d0);
 #pragma unroll
-                for (int i = 0; i < 64; ++i) {
-                  const int nd = tok0 + i - sg.len, d = nd < 0 ? d0 - i : (nd < sg.n ? p - __ldg(a.pos + sg.r0 + nd) : 0);
-                  s[i] -= sl * static_cast<float>(d);
-                }
+                for (int i = 0; i < 64; ++i) s[i] = fmaf(sl, static_cast<float>(i), s[i] - s0);
               }
             }
           }
           if (!whole) {
+            const uint32_t m0 = static_cast<uint32_t>(seen), m1 = static_cast<uint32_t>(seen >> 32);
 #pragma unroll
-            for (int i = 0; i < 64; ++i) s[i] = (seen >> i) & 1ull ? s[i] : -INFINITY;
+            for (int i = 0; i < 64; ++i) s[i] = ((i < 32 ? m0 : m1) >> (i & 31)) & 1u ? s[i] : -INFINITY;
           }
           // ---- weights
           float mx[4] = {s[0], s[1], s[2], s[3]};
@@ -346,58 +422,57 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
           const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c1;
           const float lag = FEAT ? TC_LAG * TA_LN2 : TC_LAG;
           const bool grow = ref == -INFINITY ? top > -INFINITY : top > ref + lag;
-          const float c = ref == -INFINITY ? 1.f : exp2f(FEAT ? (ref - top) * TA_LOG2E : ref - top);
           const bool rescale = grow && ref != -INFINITY;
-          if (grow) { if (rescale) l *= c; ref = top; }
+          const float c = rescale ? exp2f(FEAT ? (ref - top) * TA_LOG2E : ref - top) : 1.f;
+          if (grow) { l *= c; ref = top; }
           const float r = ref == -INFINITY ? 0.f : ref;
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
-          uint32_t hi[32], lo[32];
+          const uint64_t c2 = FEAT ? tc_two(TA_LOG2E, TA_LOG2E) : tc_two(c1, c1), r2 = tc_two(-r, -r), one = tc_two(-1.f, -1.f);
+          uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const float e0 = exp2f(FEAT ? (s[2 * i] - r) * TA_LOG2E : fmaf(s[2 * i], c1, -r));
-            const float e1 = exp2f(FEAT ? (s[2 * i + 1] - r) * TA_LOG2E : fmaf(s[2 * i + 1], c1, -r));
-            sum[i & 1] += e0; sum[2 + (i & 1)] += e1;
-            hi[i] = tc_pack(e0, e1);
-            lo[i] = tc_pack(e0 - __uint_as_float(hi[i] << 16), e1 - __uint_as_float(hi[i] & 0xffff0000u));
+          for (int part = 0; part < 2; ++part) {
+            uint32_t hi[16], lo[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const uint64_t x = tc_two(s[part * 32 + 2 * i], s[part * 32 + 2 * i + 1]);
+              const uint64_t z = FEAT ? tc_mul2(tc_add2(x, r2), c2) : tc_fma2(x, c2, r2);
+              const uint64_t e = tc_two(tc_ex2(tc_lo(z)), tc_ex2(tc_hi(z)));
+              sum[i & 1] = tc_add2(sum[i & 1], e);
+              hi[i] = tc_pack(tc_lo(e), tc_hi(e));
+              const uint64_t d = tc_fma2(tc_two(__uint_as_float(hi[i] << 16), __uint_as_float(hi[i] & 0xffff0000u)), one, e);
+              lo[i] = tc_pack(tc_lo(d), tc_hi(d));
+            }
+            tmem_st_32x16(t_lane + b * 64 + part * 16, hi);
+            tmem_st_32x16(t_lane + b * 64 + 32 + part * 16, lo);
           }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-          tmem_st_32x32(t_lane + b * 64, hi);
-          tmem_st_32x32(t_lane + b * 64 + 32, lo);
+          sum[0] = tc_add2(sum[0], sum[1]);
+          l += tc_lo(sum[0]) + tc_hi(sum[0]);
           if (__any_sync(0xffffffffu, rescale)) {            // the product before has to be done
             ok = __all_sync(0xffffffffu, mbar_wait(&o_full[q * 2 + (b ^ 1)], ((n - 1) >> 1) & 1));
             if (!ok) { set_status(a.status, ST_TIMEOUT_TMEM_FULL, blockIdx.x, it.s, j); break; }
             tc_fence_after();
-            const float k = rescale ? c : 1.f;
+            const uint64_t k2 = tc_two(c, c);
 #pragma unroll 1
             for (int cc = 0; cc < vn; cc += 32) {
               uint32_t o[32];
               tmem_ld_32x32(t_lane + 128 + cc, o);
               tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * k);
+              for (int i = 0; i < 32; i += 2) {
+                const uint64_t v = tc_mul2(static_cast<uint64_t>(o[i + 1]) << 32 | o[i], k2);
+                o[i] = static_cast<uint32_t>(v); o[i + 1] = static_cast<uint32_t>(v >> 32);
+              }
               tmem_st_32x32(t_lane + 128 + cc, o);
             }
           }
         }
         if (!whole) {
-          // ---- the page's values: tokens that are not the request's are zeroed, values that are not finite taken out
-          const int i = seq0 + (j < it.nj - 1 ? 2 * j + 2 : 2 * j + 1), vs = i % SLOTS;
-          ok = __all_sync(0xffffffffu, mbar_wait(&full[vs], (i / SLOTS) & 1));
-          if (!ok) { set_status(a.status, ST_TIMEOUT_MBAR_FULL, blockIdx.x, it.s, j); break; }
-          const int tok = row & 63, half = both ? q * 2 + (row >> 6) : row >> 6, parts = both ? 4 : 2;
-          const bool there = tok0 + tok < sg.len + sg.n && page;
-          uint8_t* vrow = ring + vs * SLOT + tok * 128;
-          bool odd = false;
-          for (int u = half; u < vn_units; u += parts) {
-            uint4* x = reinterpret_cast<uint4*>(vrow + (u >> 3) * KV_CHUNK + (((u & 7) ^ (tok & 7)) * 16));
-            if (!there) *x = make_uint4(0u, 0u, 0u, 0u);
-            else { const uint4 v = *x; odd |= tc_odd(v.x) | tc_odd(v.y) | tc_odd(v.z) | tc_odd(v.w); }
-          }
-          if (odd) atomicOr(&odd_rows[tok >> 5], 1u << (tok & 31));
-          ok = tc_sync(sync, sync_ph);
+          ok = __all_sync(0xffffffffu, mbar_wait(&v_seen[q], seen_phase));
+          seen_phase ^= 1u;
           if (!ok) { set_status(a.status, ST_TIMEOUT_MBAR_FULL, blockIdx.x, it.s, j); break; }
           const uint64_t bad = odd_rows[0] | static_cast<uint64_t>(odd_rows[1]) << 32;
           if (bad) {                                         // (rare)
+            const int i = seq0 + (j < it.nj - 1 ? 2 * j + 2 : 2 * j + 1);        // the values' place in the ring's sequence
+            uint8_t* vals = ring + i % SLOTS * SLOT;
             if (j > 0) {
               ok = __all_sync(0xffffffffu, mbar_wait(&o_full[q * 2 + (b ^ 1)], ((n - 1) >> 1) & 1));
               if (!ok) { set_status(a.status, ST_TIMEOUT_TMEM_FULL, blockIdx.x, it.s, j); break; }
@@ -415,11 +490,11 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
                 float x = -INFINITY;
 #pragma unroll
                 for (int e = 0; e < 64; ++e) x = e == k ? s[e] : x;
-                const float w = (seen >> k) & 1ull ? exp2f(FEAT ? (x - r) * TA_LOG2E : fmaf(x, c1, -r)) : 0.f;
+                const float w = (seen >> k) & 1ull ? tc_ex2(FEAT ? (x - r) * TA_LOG2E : fmaf(x, c1, -r)) : 0.f;
 #pragma unroll
                 for (int e = 0; e < 32; ++e) {
                   const int col = cc + e, u = col >> 3;
-                  const uint16_t v = *reinterpret_cast<const uint16_t*>(ring + vs * SLOT + (u >> 3) * KV_CHUNK + k * 128 + (((u & 7) ^ (k & 7)) * 16) + (col & 7) * 2);
+                  const uint16_t v = *reinterpret_cast<const uint16_t*>(vals + (u >> 3) * KV_CHUNK + k * 128 + (((u & 7) ^ (k & 7)) * 16) + (col & 7) * 2);
                   if ((v & 0x7f80u) == 0x7f80u && w != 0.f) o[e] = __float_as_uint(fmaf(w, __uint_as_float(static_cast<uint32_t>(v) << 16), __uint_as_float(o[e])));
                 }
               }
@@ -427,16 +502,16 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
             }
             ok = tc_sync(sync, sync_ph);                     // everyone has read them
             if (!ok) { set_status(a.status, ST_TIMEOUT_MBAR_FULL, blockIdx.x, it.s, j); break; }
-            if (row + q * 128 == 0) { odd_rows[0] = 0u; odd_rows[1] = 0u; }
-            for (int u = half; u < vn_units; u += parts) {
-              uint16_t* x = reinterpret_cast<uint16_t*>(vrow + (u >> 3) * KV_CHUNK + (((u & 7) ^ (tok & 7)) * 16));
+            const int tok = row & 63, parts = both ? 4 : 2;
+            for (int u = q * 2 * both + (row >> 6); u < vn_units; u += parts) {
+              uint16_t* x = reinterpret_cast<uint16_t*>(vals + (u >> 3) * KV_CHUNK + tok * 128 + (((u & 7) ^ (tok & 7)) * 16));
               for (int e = 0; e < 8; ++e)
                 if ((x[e] & 0x7f80u) == 0x7f80u) x[e] = 0;
             }
+            fence_proxy_async();
+            ok = tc_sync(sync, sync_ph);
+            if (!ok) { set_status(a.status, ST_TIMEOUT_MBAR_FULL, blockIdx.x, it.s, j); break; }
           }
-          fence_proxy_async();
-          ok = tc_sync(sync, sync_ph);                       // the values are clean, and the marks are read
-          if (!ok) { set_status(a.status, ST_TIMEOUT_MBAR_FULL, blockIdx.x, it.s, j); break; }
         }
         tmem_st_wait();
         tc_fence_before();
@@ -444,7 +519,8 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         if (lane == 0) mbar_arrive(&p_full[q * 2 + b]);
       }
       if (!ok) break;
-      // ---- the rows' outputs, or this CTA's part of them
+      // ---- the rows' outputs, or this CTA's part of them: 32 rows of a warp pass shared memory (its own queries', which are used up) in
+      // blocks of columns, so that a row's columns are written together
       ok = __all_sync(0xffffffffu, mbar_wait(&o_full[q * 2 + ((n - 1) & 1)], ((n - 1) >> 1) & 1));
       if (!ok) { set_status(a.status, ST_TIMEOUT_TMEM_FULL, blockIdx.x, it.s, it.nj); break; }
       tc_fence_after();
@@ -452,7 +528,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       const bool done = it.first && it.last;
       float m = ref;
       if (!FEAT && m != -INFINITY) m *= TA_LN2;
-      const size_t pb = (static_cast<size_t>(blockIdx.x) * 2 + (it.first ? 1 : 0)) * a.bm + q * 128 + row;
+      const size_t pb = (static_cast<size_t>(blockIdx.x) * 2 + (it.first ? 1 : 0)) * a.bm + q * 128;
       float k = 1.f;
       if (done) {
         if (a.sink) {
@@ -463,30 +539,34 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         k = l > 0.f ? ta_head_factor<__nv_bfloat16>(a, pr, h) * k / l : 0.f;
         if (l != l) k = l;
       } else if (row < pairs) {
-        a.part_ml[pb * 2] = m;
-        a.part_ml[pb * 2 + 1] = l;
+        *reinterpret_cast<float2*>(a.part_ml + (pb + row) * 2) = make_float2(m, l);
       }
+      constexpr int BC = L::STAGE / (128 * 4);               // columns of a block: 32 or 64
+      uint8_t* mine = smem + q * L::STAGE + quad * 32 * 128;           // 32 columns of the warp's rows, the next 32 Q_CHUNK behind them
+      const size_t oo = done ? static_cast<size_t>(pr) * a.ldo + static_cast<size_t>(h) * a.ho : 0;
 #pragma unroll 1
-      for (int cc = 0; cc < vn; cc += 32) {
-        uint32_t o[32];
-        tmem_ld_32x32(t_lane + 128 + cc, o);
-        tmem_ld_wait();
-        if (row < pairs) {
-          if (done) {
-            uint4* dst = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + static_cast<size_t>(pr) * a.ldo + static_cast<size_t>(h) * a.ho + cc);
+      for (int cc = 0; cc < vn; cc += BC) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              if (cc + i * 8 >= a.V) break;
-              uint32_t w[4];
+        for (int x = 0; x < BC; x += 32) {
+          uint32_t o[32];
+          tmem_ld_32x32(t_lane + 128 + min(cc + x, DC - 32), o);
+          tmem_ld_wait();
 #pragma unroll
-              for (int e = 0; e < 4; ++e) w[e] = tc_pack(__uint_as_float(o[i * 8 + 2 * e]) * k, __uint_as_float(o[i * 8 + 2 * e + 1]) * k);
-              dst[i] = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-          } else {
-            uint4* dst = reinterpret_cast<uint4*>(a.part_o + pb * a.V + cc);
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if (cc + i * 4 < a.V) dst[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          for (int i = 0; i < 8; ++i)
+            *reinterpret_cast<float4*>(mine + x / 32 * Q_CHUNK + lane * 128 + ((i ^ (lane & 7)) * 16)) =
+                make_float4(__uint_as_float(o[4 * i]) * k, __uint_as_float(o[4 * i + 1]) * k, __uint_as_float(o[4 * i + 2]) * k, __uint_as_float(o[4 * i + 3]) * k);
+        }
+        __syncwarp();
+        constexpr int TR = 128 / BC;                         // rows of an instruction
+        const int unit = lane % (BC / 4), col = cc + unit * 4;
+#pragma unroll 4
+        for (int r0 = 0; r0 < 32; r0 += TR) {
+          const int rr = r0 + lane / (BC / 4);
+          const size_t dst = __shfl_sync(0xffffffffu, oo, rr);
+          const float4 v = *reinterpret_cast<const float4*>(mine + unit / 8 * Q_CHUNK + rr * 128 + (((unit & 7) ^ (rr & 7)) * 16));
+          if (quad * 32 + rr < pairs && col < a.V) {
+            if (done) stf4(static_cast<__nv_bfloat16*>(a.out) + dst + col, v);
+            else *reinterpret_cast<float4*>(a.part_o + (pb + quad * 32 + rr) * a.V + col) = v;
           }
         }
         __syncwarp();

@@ -57,7 +57,7 @@ class _CommitPaths(C.Structure):
 class _TreeAttn(C.Structure):
     _fields_ = _struct((_p, "q k v out starts lengths slots pos pages anc bias slopes sink gate part_o part_ml split status"),
                        (_l, "k_page k_tok v_page v_tok"),
-                       (_i, "S R words page_ld n_slots n_pages H G D V ldq hq ldo ho ldg bias_n window chunk bm ctas min_tiles zero_rest"),
+                       (_i, "S R words page_ld n_slots n_pages H G D V ldq hq ldo ho ldg bias_n window chunk bm sms ctas min_tiles zero_rest"),
                        (_f, "scale cap out_scale"))
 
 
@@ -375,7 +375,7 @@ def tree_attention(q, k, v, maps: RowMaps, scale: float, softcap: float = 0.0, b
                   P(sink), P(gate), P(part_o), P(part_ml), P(split), P(cu.status_word(dev)), kp, kt, vp, vt, maps.lengths.shape[0], R,
                   maps.anc.shape[1] if maps.anc is not None else 0, maps.tables.shape[1], maps.tables.shape[0], k.shape[0], H, G, D, V, q.stride(0),
                   q.stride(1), out.stride(0), out.stride(1), gate.stride(0) if gate is not None else 0, bias.shape[1] if bias is not None else 0, window,
-                  chunk, bm, ctas, 1, int(fresh), scale, softcap, out_scale)
+                  chunk, bm, sms, ctas, 1, int(fresh), scale, softcap, out_scale)
     _call("spark_tree_attn", dev, C.byref(a), int(dt == torch.float32), int(tc))
     return out
 
