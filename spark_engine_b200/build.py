@@ -3,6 +3,7 @@
   libspark_kernels.so : every .cu under csrc/kernels, compiled for sm_100a only
   libspark_kernels_<family>.so : the part of it one model family needs (`kernel_library`)
   _runtime*.so        : C++ host runtime (KV pool, scheduler core, prefix-cache I/O, ...) as a pybind11 module
+  _tree*.so           : checks and launches of the tree verification ops on torch tensors
 
 Usage: `python -m spark_engine_b200.build [--force]`.
 """
@@ -92,6 +93,21 @@ def build_runtime(force=False) -> str:
     return out
 
 
+def build_tree(force=False) -> str:
+    os.makedirs(LIBDIR, exist_ok=True)
+    out = os.path.join(LIBDIR, "_tree" + sysconfig.get_config_var("EXT_SUFFIX"))
+    src = os.path.join(CSRC, "bindings", "tree_ops.cpp")
+    if force or _newer([src, os.path.join(CSRC, "common", "tree_args.h")], out):
+        import torch
+        from torch.utils import cpp_extension as ext
+        inc = [os.path.join(CSRC, "common"), *ext.include_paths("cuda"), sysconfig.get_paths()["include"]]
+        lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+        _run(["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-DTORCH_EXTENSION_NAME=_tree", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+             + ["-isystem" + i if "torch" in i else "-I" + i for i in inc] + [src, "-o", out, "-L" + lib, "-Wl,-rpath," + lib]
+             + ["-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10_cuda", "-lc10"])
+    return out
+
+
 def build_race_stress(sanitizer: str = "thread", force=False) -> str:
     """The host runtime's concurrency stress driver (csrc/runtime/stress/race_stress.cpp) linked against the runtime
     sources with -fsanitize=<sanitizer> ("thread", or "address,undefined"); returns the executable's path.  It needs
@@ -107,7 +123,11 @@ def build_race_stress(sanitizer: str = "thread", force=False) -> str:
 
 
 def build_all(force=False, verbose=False):
-    return build_kernels(force, verbose), build_runtime(force)
+    with cf.ThreadPoolExecutor(max_workers=1) as ex:
+        tree = ex.submit(build_tree, force)
+        out = build_kernels(force, verbose), build_runtime(force)
+        tree.result()
+    return out
 
 
 if __name__ == "__main__":

@@ -3,30 +3,17 @@
 // The (row, head) pairs of a request and a key / value head are numbered node by node and cut into tiles of `bm`; a tile's keys are the pages
 // from the first one that any of its rows can see to the request's last node.  All (request, head, tile) items together are `total` pages,
 // and CTA c of the grid takes the same number of consecutive ones as every other: lengths may differ as they like, the host needs to know
-// none of them, and a captured launch may be replayed with others.  An item that ends in another CTA than it began leaves partial results
-// (sums, maxima) that a second launch joins in ascending order.
+// none of them, and a captured launch may be replayed with others.  To begin an item costs as much as `extra` pages (queries in, results out):
+// it counts as that many more, in front of its own, so that a CTA which ends one item and begins another is not the last to finish.  An item
+// that ends in another CTA than it began leaves partial results (sums, maxima) that a second launch joins in ascending order.
 #pragma once
 #include "rows.cuh"
+#include "tree_args.h"
 
 namespace spark {
 
-constexpr int TA_PAGE = 64;
+constexpr int TA_PAGE = TREE_PAGE;
 constexpr float TA_LOG2E = 1.4426950408889634f, TA_LN2 = 0.6931471805599453f;
-
-struct TreeAttn {
-  const void *q, *k, *v;                 // q [R, H, D] (rows ldq, heads hq apart); caches of pages of 64 tokens of G heads
-  void* out;                             // [R, H, V] (rows ldo, heads ho apart)
-  const int *starts, *lengths, *slots, *pos, *pages;
-  const uint32_t* anc;                   // [R, words] (null: rows see the rows before them)
-  const float *bias, *slopes, *sink;     // [H, bias_n], [H], [H]
-  const void* gate;                      // [R, H], rows ldg apart
-  float *part_o, *part_ml;               // [ctas][2][bm][V], [ctas][2][bm][2]: of a tile begun before the CTA, of one that goes on behind it
-  int4* split;                           // [ctas]: the item that begins in this CTA and ends in another, see ta_split
-  int* status;
-  long long k_page, k_tok, v_page, v_tok;                    // strides in elements
-  int S, R, words, page_ld, n_slots, n_pages, H, G, D, V, ldq, hq, ldo, ho, ldg, bias_n, window, chunk, bm, sms, ctas, min_tiles, zero_rest;
-  float scale, cap, out_scale;
-};
 
 __device__ __forceinline__ int ta_first_visible(const TreeAttn& a, int p) {
   return a.chunk > 0 ? p / a.chunk * a.chunk : (a.window > 0 ? max(p - a.window + 1, 0) : 0);
@@ -45,7 +32,7 @@ __device__ __forceinline__ TreeSeg ta_segment(const TreeAttn& a, int s) {
   t.rts = t.n > 0 ? (t.n * (a.H / a.G) + a.bm - 1) / a.bm : 0;
   return t;
 }
-__device__ __forceinline__ long long ta_tiles(const TreeAttn& a, const TreeSeg& t) { return static_cast<long long>(a.G) * t.rts * t.nt; }
+__device__ __forceinline__ long long ta_tiles(const TreeAttn& a, const TreeSeg& t) { return static_cast<long long>(a.G) * t.rts * (t.nt + a.extra); }
 
 // Exclusive prefix over the block; every thread calls it.  sh: [NT / 32].
 template <int NT>
@@ -105,31 +92,38 @@ struct TreeItem {                        // a row tile of one key / value head a
 };
 // The next item of the range; false at its end.
 __device__ __forceinline__ bool ta_next(const TreeAttn& a, TreeRange& r, TreeItem& it) {
-  if (r.count <= 0) return false;
-  it.seg = ta_segment(a, r.s);
-  while (r.rem >= ta_tiles(a, it.seg)) {                     // (the range ends with the last request's tiles)
-    r.rem -= ta_tiles(a, it.seg);
-    it.seg = ta_segment(a, ++r.s);
+  while (r.count > 0) {
+    it.seg = ta_segment(a, r.s);
+    while (r.rem >= ta_tiles(a, it.seg)) {                   // (the range ends with the last request's tiles)
+      r.rem -= ta_tiles(a, it.seg);
+      it.seg = ta_segment(a, ++r.s);
+    }
+    const int nt = it.seg.nt, all = nt + a.extra, i = static_cast<int>(r.rem / all), at = static_cast<int>(r.rem - static_cast<long long>(i) * all);
+    const int take = r.count < all - at ? static_cast<int>(r.count) : all - at;
+    const int off = at > a.extra ? at - a.extra : 0, end = at + take - a.extra;
+    r.count -= take;
+    r.rem += take;
+    if (end <= off) continue;                                // the range ends in front of the item's first page
+    it.s = r.s;
+    it.g = i / it.seg.rts;
+    it.rt = i - it.g * it.seg.rts;
+    it.j = it.seg.j0 + off;
+    it.nj = end - off;
+    it.first = off == 0;
+    it.last = end == nt;
+    it.parts = 1 + static_cast<int>((nt - end + r.per - 1) / r.per);
+    return true;
   }
-  const int nt = it.seg.nt, i = static_cast<int>(r.rem / nt), off = static_cast<int>(r.rem - static_cast<long long>(i) * nt);
-  it.s = r.s;
-  it.g = i / it.seg.rts;
-  it.rt = i - it.g * it.seg.rts;
-  it.j = it.seg.j0 + off;
-  it.nj = r.count < nt - off ? static_cast<int>(r.count) : nt - off;
-  it.first = off == 0;
-  it.last = off + it.nj == nt;
-  it.parts = 1 + static_cast<int>((nt - off - it.nj + r.per - 1) / r.per);
-  r.count -= it.nj;
-  r.rem += it.nj;
-  return true;
+  return false;
 }
-
 // What the second launch needs of an item: (parts, first row of the request, head, first pair and pairs of the tile).
 __device__ __forceinline__ int4 ta_split(const TreeAttn& a, const TreeItem& it) {
   const int pairs = it.seg.n * (a.H / a.G) - it.rt * a.bm;
   return make_int4(it.parts | (pairs < a.bm ? pairs : a.bm) << 16, it.seg.r0, it.g, it.rt * a.bm);
 }
+
+__device__ __forceinline__ void ta_set_split(const TreeAttn& a, int4 v) { reinterpret_cast<int4*>(a.split)[blockIdx.x] = v; }
+__device__ __forceinline__ int4 ta_get_split(const TreeAttn& a, int c) { return __ldcg(reinterpret_cast<const int4*>(a.split) + c); }
 
 template <typename T>
 __device__ __forceinline__ float ta_head_factor(const TreeAttn& a, int row, int h) {

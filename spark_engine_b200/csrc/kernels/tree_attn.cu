@@ -30,7 +30,7 @@ tree_tile_kernel(const __grid_constant__ TreeAttn a) {
   pdl_wait();
   pdl_trigger();
   TreeRange range = ta_range<TT_THREADS>(a, sh);
-  if (t == 0) a.split[blockIdx.x] = make_int4(0, 0, 0, 0);
+  if (t == 0) ta_set_split(a, make_int4(0, 0, 0, 0));
   TreeItem it;
   while (ta_next(a, range, it)) {
     const TreeSeg& sg = it.seg;
@@ -166,7 +166,7 @@ tree_tile_kernel(const __grid_constant__ TreeAttn a) {
     }
     // ---- whole: the rows' outputs; else this CTA's part of them
     const bool whole = it.first && it.last;
-    if (it.first && !it.last && t == 0) a.split[blockIdx.x] = ta_split(a, it);
+    if (it.first && !it.last && t == 0) ta_set_split(a, ta_split(a, it));
     const size_t pb = (static_cast<size_t>(blockIdx.x) * 2 + (it.first ? 1 : 0)) * TT_BM;
     if (!whole && t < pairs) { a.part_ml[(pb + t) * 2] = s_m[t]; a.part_ml[(pb + t) * 2 + 1] = s_l[t]; }
 #pragma unroll
@@ -225,7 +225,7 @@ tree_merge_kernel(const __grid_constant__ TreeAttn a) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int c = t * each + i;
-    n[i] = i < each && c < a.ctas ? a.split[c].x >> 16 : 0;
+    n[i] = i < each && c < a.ctas ? ta_get_split(a, c).x >> 16 : 0;
     mine += n[i];
   }
   long long total;
@@ -247,7 +247,7 @@ tree_merge_kernel(const __grid_constant__ TreeAttn a) {
     int lo = 0, hi = a.ctas;                                 // the last CTA whose rows begin at or before the task
     while (hi - lo > 1) { const int m = (lo + hi) >> 1; if (s_first[m] <= task) lo = m; else hi = m; }
     const int c = lo, row = on ? task - s_first[lo] : 0;
-    const int4 sp = a.split[c];
+    const int4 sp = ta_get_split(a, c);
     const int parts = on ? sp.x & 0xffff : 0;
     // part 0 lies behind the others' in its CTA's pair, see TreeAttn
     auto part = [&](int i) { return (static_cast<size_t>(c + i) * 2 + (i == 0 ? 1 : 0)) * a.bm + row; };

@@ -1,8 +1,9 @@
 // Tree attention on tcgen05 (bf16 caches): the tiles of tree_attn.cu with 128 (node, head) rows per accumulator, a page of keys per step.
 //   warp 0      TMA: pages of keys and values into a ring of slots in the order the products use them (K0 K1 V0 K2 V1 ..)
 //   warp 1      issues S = Q K^T one page ahead of O += P V (P in tensor memory, over the scores that it was made from)
-//   warps 2 ..  softmax, one row per thread: 64 scores are one tensor-memory load, statistics stay in the thread
-// NQ = 2: two tiles of 128 rows with their own softmax warps share the keys in shared memory (large trees: a page is read once for 256 rows).
+//   the others  softmax, one row per thread: 64 scores are one tensor-memory load, statistics stay in the thread
+// NQ = 2: two tiles of 128 rows with their own issuing and softmax warps share the keys in shared memory (large trees: a page is read once for
+// 256 rows).  Each tile's products wait for its own softmax alone: with one issuing warp for both, a page took 2.0 us instead of ...
 //
 // Weights enter the product as two bf16 terms (2^-17 of a weight is lost), so that the reference of the exponentials may lag behind the
 // maximum: the accumulator is rescaled only when a row's maximum outgrew its reference by 2^8.
@@ -27,7 +28,7 @@ template <int DC, int NQ> struct Tc {
   // per tile: two buffers of scores / weights of 64 columns, the accumulator
   static constexpr int TILE_COLS = 128 + DC, Q_COL = 128 + DC;
   static constexpr int COLS = QT || NQ == 2 ? 512 : 256;
-  static constexpr int WARPS = 2 + 4 * NQ, THREADS = WARPS * 32, PER_SM = QT || NQ == 2 ? 1 : 2;
+  static constexpr int SOFTMAX = 1 + NQ, WARPS = SOFTMAX + 4 * NQ, THREADS = WARPS * 32, PER_SM = QT || NQ == 2 ? 1 : 2;
   static_assert(NQ * TILE_COLS + (QT ? DC / 2 : 0) <= COLS && SMEM <= 232448, "tensor memory, shared memory");
 };
 
@@ -127,11 +128,11 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
   uint64_t* v_sync = v_seen + NQ;                            // [NQ]: of 4 and of 8 softmax warps
   long long* sh = reinterpret_cast<long long*>(v_sync + NQ); // [NT / 32 + 2]
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(sh + NT / 32 + 2);
-  uint32_t* odd_rows = tmem_ptr + 1;                         // [2]: tokens of a masked page with a value that is not finite
+  uint32_t* odd_rows = tmem_ptr + 1;                         // [SLOTS][2]: tokens of a masked page with a value that is not finite
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV);
-    for (int s = 0; s < SLOTS; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    for (int s = 0; s < SLOTS; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], NQ); }
     for (int s = 0; s < NQ; ++s) { mbar_init(&q_full[s], 4); mbar_init(&v_seen[s], 1); mbar_init(&v_sync[s], 4 * (s + 1)); }
     for (int s = 0; s < 2 * NQ; ++s) { mbar_init(&s_full[s], 1); mbar_init(&p_full[s], 4); mbar_init(&o_full[s], 1); }
     fence_barrier_init();
@@ -144,7 +145,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
   pdl_wait();
   pdl_trigger();
   TreeRange range = ta_range<NT>(a, sh);
-  if (threadIdx.x == 64) a.split[blockIdx.x] = make_int4(0, 0, 0, 0);
+  if (threadIdx.x == L::SOFTMAX * 32) ta_set_split(a, make_int4(0, 0, 0, 0));
   const int rep = a.H / a.G;
   TreeItem it;
   bool ok = true;
@@ -178,57 +179,56 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         tc_step<SLOTS>(c);
       }
     }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------ MMA issuer (the whole warp walks, one elected lane issues)
-    const int ksteps = (a.D + 15) / 16, vn = (a.V + 15) / 16 * 16;
+  } else if (warp <= NQ) {
+    // ------------------------------------------------------------ MMA issuer of tile q (the whole warp walks, one elected lane issues)
+    const int q = warp - 1, ksteps = (a.D + 15) / 16, vn = (a.V + 15) / 16 * 16, vunits = (a.V + 63) / 64 * 8;
     const uint32_t id_s = make_idesc(1, 1, 128, TA_PAGE), id_o = make_idesc(1, 1, 128, vn) | (1u << 16);
-    const uint32_t qs = __shfl_sync(0xffffffffu, smem_u32(smem), 0), rs = qs + NQ * L::STAGE, tm = __shfl_sync(0xffffffffu, tmem, 0);
+    const uint32_t qs = __shfl_sync(0xffffffffu, smem_u32(smem), 0) + q * L::STAGE, rs = __shfl_sync(0xffffffffu, smem_u32(ring), 0);
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0) + q * L::TILE_COLS;
     TcCount c;
-    const int vunits = (a.V + 63) / 64 * 8;
-    int n[NQ] = {}, items[NQ] = {};                          // pages and items of each tile so far
+    int n = 0, items = 0;                                    // pages and items of the tile so far
     while (ok && ta_next(a, range, it)) {
       const int pairs = it.seg.n * rep - it.rt * a.bm, act = NQ == 2 && pairs > 128 ? 2 : 1;
-#pragma unroll
-      for (int q = 0; q < NQ; ++q)
-        if (q < act && ok) {
-          ok = __all_sync(0xffffffffu, mbar_wait(&q_full[q], items[q] & 1));
-          ++items[q];
-        }
-      if (!ok) { set_status(a.status, ST_TIMEOUT_MBAR_FULL, blockIdx.x, it.s, -2); break; }
       const int slot = a.slots ? a.slots[it.s] : it.s, edge = ta_first_visible(a, it.seg.len + it.seg.n - 1);
-      uint32_t there = 0u;                                   // pages of the current 32 that the table leads to
-      for (int j = -1; j < it.nj && ok; ++j) {
-        if (j + 1 < it.nj) {
+      if (q >= act) {                                        // no rows here: the slots are passed on
+        for (int i = 0; i < 2 * it.nj; ++i) {
           ok = __all_sync(0xffffffffu, mbar_wait(&full[c.slot], c.ph));
-#pragma unroll
-          for (int q = 0; q < NQ; ++q) {
-            if (q >= act) continue;
-            // the scores go where the weights of two pages back were: their product has to be done
-            const int b = (n[q] + j + 1) & 1;
-            if (ok && n[q] + j + 1 >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&o_full[q * 2 + b], ((n[q] + j - 1) >> 1) & 1));
-            if (!ok) break;
-            tc_fence_after();
-            if (elect_one()) {
-              const uint32_t d = tm + q * L::TILE_COLS + b * 64;
-              for (int k = 0; k < ksteps; ++k) {
-                const uint64_t kd = make_smem_desc_sw128(rs + c.slot * SLOT + (k >> 2) * KV_CHUNK) + 2 * (k & 3);
-                if (L::QT) umma_f16_ts(d, tm + L::Q_COL + k * 8, kd, id_s, k != 0);
-                else umma_f16(d, make_smem_desc_sw128(qs + q * L::STAGE + (k >> 2) * Q_CHUNK) + 2 * (k & 3), kd, id_s, k != 0);
-              }
-              umma_commit(&s_full[q * 2 + b]);
-            }
-            __syncwarp();
-          }
+          if (!ok) { set_status(a.status, ST_TIMEOUT_MBAR_FULL, blockIdx.x, it.s, i); break; }
+          if (lane == 0) mbar_arrive(&empty[c.slot]);
+          tc_step<SLOTS>(c);
+        }
+        continue;
+      }
+      uint32_t there = 0u;                                   // pages of the current 32 that the table leads to
+      ok = __all_sync(0xffffffffu, mbar_wait(&q_full[q], items & 1));
+      if (!ok) { set_status(a.status, ST_TIMEOUT_MBAR_FULL, blockIdx.x, it.s, -2); break; }
+      ++items;
+      for (int j = -1; j < it.nj; ++j) {
+        if (j + 1 < it.nj) {
+          const int t = n + j + 1, b = t & 1;
+          ok = __all_sync(0xffffffffu, mbar_wait(&full[c.slot], c.ph));
+          // the scores go where the weights of two pages back were: their product has to be done
+          if (ok && t >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&o_full[q * 2 + b], ((t - 2) >> 1) & 1));
           if (!ok) { set_status(a.status, ST_TIMEOUT_MBAR_FULL, blockIdx.x, it.s, j); break; }
-          if (elect_one()) umma_commit(&empty[c.slot]);
+          tc_fence_after();
+          if (elect_one()) {
+            const uint32_t d = tm + b * 64;
+            for (int k = 0; k < ksteps; ++k) {
+              const uint64_t kd = make_smem_desc_sw128(rs + c.slot * SLOT + (k >> 2) * KV_CHUNK) + 2 * (k & 3);
+              if (L::QT) umma_f16_ts(d, tm + L::Q_COL + k * 8, kd, id_s, k != 0);
+              else umma_f16(d, make_smem_desc_sw128(qs + (k >> 2) * Q_CHUNK) + 2 * (k & 3), kd, id_s, k != 0);
+            }
+            umma_commit(&s_full[q * 2 + b]);
+            umma_commit(&empty[c.slot]);
+          }
           __syncwarp();
           tc_step<SLOTS>(c);
         }
         if (j < 0) continue;
+        const int b = (n + j) & 1, tok0 = (it.j + j) * TA_PAGE;
         if ((j & 31) == 0) there = __ballot_sync(0xffffffffu, j + lane < it.nj && ta_page(a, slot, it.j + j + lane) >= 0);
         ok = __all_sync(0xffffffffu, mbar_wait(&full[c.slot], c.ph));
-        const int tok0 = (it.j + j) * TA_PAGE;
-        if (ok && (tok0 + TA_PAGE > it.seg.len || tok0 < edge || !((there >> (j & 31)) & 1u))) {
+        if (q == 0 && ok && (tok0 + TA_PAGE > it.seg.len || tok0 < edge || !((there >> (j & 31)) & 1u))) {
           // ---- a masked page's values: tokens that are not the request's are zeroed, the others with a value that is not finite noted
           const int valid = (there >> (j & 31)) & 1u ? min(TA_PAGE, it.seg.len + it.seg.n - tok0) : 0;
           uint32_t odd[2];
@@ -250,43 +250,31 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
           fence_proxy_async();
           __syncwarp();
           if (lane == 0) {
-            odd_rows[0] = odd[0]; odd_rows[1] = odd[1];
-#pragma unroll
-            for (int q = 0; q < NQ; ++q)
-              if (q < act) mbar_arrive(&v_seen[q]);
+            odd_rows[2 * c.slot] = odd[0]; odd_rows[2 * c.slot + 1] = odd[1];
+            for (int i = 0; i < act; ++i) mbar_arrive(&v_seen[i]);
           }
         }
-#pragma unroll
-        for (int q = 0; q < NQ; ++q) {
-          if (q >= act) continue;
-          const int b = (n[q] + j) & 1;
-          ok = ok && __all_sync(0xffffffffu, mbar_wait(&p_full[q * 2 + b], ((n[q] + j) >> 1) & 1));
-          if (!ok) break;
-          tc_fence_after();
-          if (elect_one()) {
-            const uint32_t base = tm + q * L::TILE_COLS;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const uint64_t vd = tc_desc_nmajor(rs + c.slot * SLOT + k * 2048, KV_CHUNK);
-              umma_f16_ts(base + 128, base + b * 64 + k * 8, vd, id_o, 1);
-              umma_f16_ts(base + 128, base + b * 64 + 32 + k * 8, vd, id_o, 1);
-            }
-            umma_commit(&o_full[q * 2 + b]);
-          }
-          __syncwarp();
-        }
+        ok = ok && __all_sync(0xffffffffu, mbar_wait(&p_full[q * 2 + b], ((n + j) >> 1) & 1));
         if (!ok) { set_status(a.status, ST_TIMEOUT_MBAR_FULL, blockIdx.x, it.s, j); break; }
-        if (elect_one()) umma_commit(&empty[c.slot]);
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint64_t vd = tc_desc_nmajor(rs + c.slot * SLOT + k * 2048, KV_CHUNK);
+            umma_f16_ts(tm + 128, tm + b * 64 + k * 8, vd, id_o, 1);
+            umma_f16_ts(tm + 128, tm + b * 64 + 32 + k * 8, vd, id_o, 1);
+          }
+          umma_commit(&o_full[q * 2 + b]);
+          umma_commit(&empty[c.slot]);
+        }
         __syncwarp();
         tc_step<SLOTS>(c);
       }
-#pragma unroll
-      for (int q = 0; q < NQ; ++q)
-        if (q < act) n[q] += it.nj;
+      n += it.nj;
     }
   } else {
     // ------------------------------------------------------------ softmax, one row per thread
-    const int q = NQ == 2 ? (warp - 2) >> 2 : 0, quad = warp & 3, row = quad * 32 + lane;
+    const int q = (warp - L::SOFTMAX) >> 2, quad = warp & 3, row = quad * 32 + lane;
     const uint32_t t_lane = tmem + (static_cast<uint32_t>(quad * 32) << 16) + q * L::TILE_COLS;
     const int vn = (a.V + 15) / 16 * 16, vn_units = (a.V + 63) / 64 * 8;
     uint32_t sync_phase[NQ] = {}, seen_phase = 0u;
@@ -296,7 +284,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       const int all = sg.n * rep - it.rt * a.bm, pairs = min(128, all - q * 128);        // rows of this tile
       const int seq0 = seq;
       seq += 2 * it.nj;
-      if (it.first && !it.last && threadIdx.x == 64) a.split[blockIdx.x] = ta_split(a, it);
+      if (it.first && !it.last && threadIdx.x == L::SOFTMAX * 32) ta_set_split(a, ta_split(a, it));
       if (pairs <= 0) continue;
       const bool both = NQ == 2 && all > 128;
       uint64_t* sync = &v_sync[both ? NQ - 1 : 0];
@@ -469,10 +457,10 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
           ok = __all_sync(0xffffffffu, mbar_wait(&v_seen[q], seen_phase));
           seen_phase ^= 1u;
           if (!ok) { set_status(a.status, ST_TIMEOUT_MBAR_FULL, blockIdx.x, it.s, j); break; }
-          const uint64_t bad = odd_rows[0] | static_cast<uint64_t>(odd_rows[1]) << 32;
+          const int vs = (seq0 + (j < it.nj - 1 ? 2 * j + 2 : 2 * j + 1)) % SLOTS;       // the values' place in the ring's sequence
+          const uint64_t bad = odd_rows[2 * vs] | static_cast<uint64_t>(odd_rows[2 * vs + 1]) << 32;
           if (bad) {                                         // (rare)
-            const int i = seq0 + (j < it.nj - 1 ? 2 * j + 2 : 2 * j + 1);        // the values' place in the ring's sequence
-            uint8_t* vals = ring + i % SLOTS * SLOT;
+            uint8_t* vals = ring + vs * SLOT;
             if (j > 0) {
               ok = __all_sync(0xffffffffu, mbar_wait(&o_full[q * 2 + (b ^ 1)], ((n - 1) >> 1) & 1));
               if (!ok) { set_status(a.status, ST_TIMEOUT_TMEM_FULL, blockIdx.x, it.s, j); break; }

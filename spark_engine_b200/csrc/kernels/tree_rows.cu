@@ -9,10 +9,9 @@
 // tree; its position is len_s + depth.  What a table or a path gives is checked before it is used as an address: a bad entry sets the status
 // word and the row is skipped.
 #include "../common/rows.cuh"
+#include "../common/tree_args.h"
 
 namespace spark {
-
-constexpr int TREE_PAGE = 64;
 
 // Exclusive prefix of v over the block's 1024 threads, and the sum; `sh`: 33 ints.  Every thread calls it.
 __device__ __forceinline__ int block_prefix(int v, int* sh, int& total) {
@@ -42,13 +41,6 @@ __device__ __forceinline__ int block_prefix(int v, int* sh, int& total) {
 }
 
 // ------------------------------------------------------------------------------------------------ block tables
-struct BlockTables {
-  const int* lengths;                    // [S] tokens a request needs room for; negative: the request is left as it is
-  int *tables, *held;                    // [S, ld] pages in position order, -1 behind the held ones; [S]
-  int *free, *n_free;                    // stack of free pages: free[0 .. n_free)
-  int *room, *status;                    // [S] tokens a request has room for afterwards
-  int S, ld, cap;                        // cap: entries of `free`
-};
 
 // One CTA, a warp per request in turn.  Pages go back first, the last request's last page first, then requests take theirs in order, each
 // from the top of the stack: giving back what was just taken restores the stack.  A request whose pages are not all there gets none, nor
@@ -117,13 +109,6 @@ block_tables_kernel(const __grid_constant__ BlockTables a) {
 }
 
 // ------------------------------------------------------------------------------------------------ row maps
-struct SlotMaps {
-  const int *lengths, *counts, *tables, *slots, *parents;    // slots (optional): a request's row of the tables; parents (trees): [R]
-  int *starts, *slot, *index, *pos, *anc;                    // [S + 1], [R] each, [R, words]
-  long long* cache_row;                                      // [R]
-  int* status;
-  int S, R, ld, n_slots, nodes, words;
-};
 
 constexpr int MAP_THREADS = 256;
 
@@ -189,15 +174,6 @@ slot_maps_kernel(const __grid_constant__ SlotMaps a) {
 }
 
 // ------------------------------------------------------------------------------------------------ convolution along paths
-struct PathConv {
-  const void* x; const float* w; const void* tail;           // [R, ldx]; [taps, C]; [slots, taps - 1, C]
-  void *q, *k, *v;                                           // q [R, nq]
-  const int *slot, *index, *parents;                         // parents null: chains
-  const long long* cache_row;
-  int* status;
-  long long k_page, k_tok, v_page, v_tok, cache_rows;        // strides in elements
-  int ldx, R, C, taps, nq, nk, n_slots;
-};
 
 constexpr int PC_ROWS = 4;
 
@@ -256,19 +232,6 @@ path_conv_kernel(const __grid_constant__ PathConv a) {
 }
 
 // ------------------------------------------------------------------------------------------------ commit
-struct CommitJob {
-  char* base;                            // a cache, or the tail of a convolution
-  const char* x;                         // null: a cache; else the rows behind the tail
-  long long page, tok;                   // bytes: strides of a cache's pages and tokens, or of a slot's entries (tok) and of x's rows (page)
-  int bytes, extent, kept, pad;          // bytes of a row (multiple of 16); pages of the cache, or slots of the tail; a slot's entries
-};
-constexpr int COMMIT_JOBS = 64;
-struct CommitPaths {
-  CommitJob job[COMMIT_JOBS];
-  const int *path, *n_path, *starts, *lengths, *slots, *tables;
-  int* status;
-  int S, P, ld, n_slots;
-};
 
 // grid (requests, column blocks, jobs); 128 threads x 16 bytes.  A path is ascending, so row i is written after row path[i] >= i was read,
 // and no later row of the path lies at or below i: every thread moves its columns in order and in place.

@@ -603,4 +603,4 @@ def latent_mixer(mixer, proj, plan, cat):
 
 
 # ----------------------------------------------------------------------------- drafted trees over paged caches
-from .tree import RowMaps, block_tables, commit_paths, path_conv, slot_maps, tree_attention  # noqa: E402, F401
+from .tree import block_tables, commit_paths, path_conv, slot_maps, tree_attention  # noqa: E402, F401
