@@ -204,13 +204,14 @@ constexpr int TM_THREADS = 256, TM_WARPS = TM_THREADS / 32, TM_MAX_CTAS = 1024;
 // Every CTA makes the list of the split items' rows (a row per item that begins in one CTA of the first launch and ends in another) and
 // takes its share of them; the fewer there are, the more warps join one row.  Parts are added in ascending order within a warp, warps in
 // ascending order.
-template <typename T>
+template <typename T, int VC>                                // VC: 128-column pieces of a row
 __global__ void __launch_bounds__(TM_THREADS)
 tree_merge_kernel(const __grid_constant__ TreeAttn a) {
   __shared__ long long sh[TM_WARPS + 2];
   __shared__ int s_first[TM_MAX_CTAS + 1];                   // rows of the items in front of CTA c's
-  __shared__ float4 s_o[TM_WARPS][128];
+  __shared__ float4 s_o[TM_WARPS][32 * VC];
   __shared__ float s_ml[TM_WARPS][2];
+  __shared__ int4 s_split[TM_MAX_CTAS];
   pdl_wait();
   pdl_trigger();
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31, V4 = a.V >> 2, rep = a.H / a.G;
@@ -225,7 +226,12 @@ tree_merge_kernel(const __grid_constant__ TreeAttn a) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int c = t * each + i;
-    n[i] = i < each && c < a.ctas ? ta_get_split(a, c).x >> 16 : 0;
+    n[i] = 0;
+    if (i < each && c < a.ctas) {
+      const int4 sp = ta_get_split(a, c);
+      s_split[c] = sp;
+      n[i] = sp.x >> 16;
+    }
     mine += n[i];
   }
   long long total;
@@ -247,21 +253,21 @@ tree_merge_kernel(const __grid_constant__ TreeAttn a) {
     int lo = 0, hi = a.ctas;                                 // the last CTA whose rows begin at or before the task
     while (hi - lo > 1) { const int m = (lo + hi) >> 1; if (s_first[m] <= task) lo = m; else hi = m; }
     const int c = lo, row = on ? task - s_first[lo] : 0;
-    const int4 sp = ta_get_split(a, c);
+    const int4 sp = s_split[c];
     const int parts = on ? sp.x & 0xffff : 0;
     // part 0 lies behind the others' in its CTA's pair, see TreeAttn
     auto part = [&](int i) { return (static_cast<size_t>(c + i) * 2 + (i == 0 ? 1 : 0)) * a.bm + row; };
     float m = -INFINITY, l = 0.f;
-    float4 o[4] = {};
+    float4 o[VC] = {};
     for (int i0 = sub; i0 < parts; i0 += 4 * wpr) {          // four parts in flight
-      float4 x[4][4];
+      float4 x[4][VC];
       float2 ml[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const int i = i0 + u * wpr;
         ml[u] = i < parts ? __ldcg(reinterpret_cast<const float2*>(a.part_ml + part(i) * 2)) : make_float2(-INFINITY, 0.f);
 #pragma unroll
-        for (int v = 0; v < 4; ++v)
+        for (int v = 0; v < VC; ++v)
           if (i < parts && lane + v * 32 < V4) x[u][v] = __ldcg(reinterpret_cast<const float4*>(a.part_o + part(i) * a.V) + lane + v * 32);
       }
       const float top = fmaxf(m, fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x))), ref = top == -INFINITY ? 0.f : top;
@@ -269,14 +275,14 @@ tree_merge_kernel(const __grid_constant__ TreeAttn a) {
       m = top;
       l *= k;
 #pragma unroll
-      for (int v = 0; v < 4; ++v) { o[v].x *= k; o[v].y *= k; o[v].z *= k; o[v].w *= k; }
+      for (int v = 0; v < VC; ++v) { o[v].x *= k; o[v].y *= k; o[v].z *= k; o[v].w *= k; }
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const float w = expf(ml[u].x - ref);
         if (w == 0.f) continue;
         l = fmaf(w, ml[u].y, l);
 #pragma unroll
-        for (int v = 0; v < 4; ++v)
+        for (int v = 0; v < VC; ++v)
           if (lane + v * 32 < V4) {
             o[v].x = fmaf(w, x[u][v].x, o[v].x); o[v].y = fmaf(w, x[u][v].y, o[v].y);
             o[v].z = fmaf(w, x[u][v].z, o[v].z); o[v].w = fmaf(w, x[u][v].w, o[v].w);
@@ -287,7 +293,7 @@ tree_merge_kernel(const __grid_constant__ TreeAttn a) {
       __syncthreads();                                       // (the task before has been read)
       if (lane == 0) { s_ml[warp][0] = m; s_ml[warp][1] = l; }
 #pragma unroll
-      for (int v = 0; v < 4; ++v)
+      for (int v = 0; v < VC; ++v)
         if (lane + v * 32 < V4) s_o[warp][lane + v * 32] = o[v];
       __syncthreads();
       if (sub == 0) {
@@ -295,13 +301,13 @@ tree_merge_kernel(const __grid_constant__ TreeAttn a) {
         const float ref = m == -INFINITY ? 0.f : m, c0 = expf(s_ml[warp][0] - ref);
         l *= c0;
 #pragma unroll
-        for (int v = 0; v < 4; ++v) { o[v].x *= c0; o[v].y *= c0; o[v].z *= c0; o[v].w *= c0; }
+        for (int v = 0; v < VC; ++v) { o[v].x *= c0; o[v].y *= c0; o[v].z *= c0; o[v].w *= c0; }
         for (int i = 1; i < wpr; ++i) {
           const float w = expf(s_ml[warp + i][0] - ref);
           if (w == 0.f) continue;
           l = fmaf(w, s_ml[warp + i][1], l);
 #pragma unroll
-          for (int v = 0; v < 4; ++v)
+          for (int v = 0; v < VC; ++v)
             if (lane + v * 32 < V4) {
               const float4 y = s_o[warp + i][lane + v * 32];
               o[v].x = fmaf(w, y.x, o[v].x); o[v].y = fmaf(w, y.y, o[v].y); o[v].z = fmaf(w, y.z, o[v].z); o[v].w = fmaf(w, y.w, o[v].w);
@@ -320,7 +326,7 @@ tree_merge_kernel(const __grid_constant__ TreeAttn a) {
     float scale = l > 0.f ? ta_head_factor<T>(a, r, h) * k / l : 0.f;
     if (l != l) scale = l;
 #pragma unroll
-    for (int v = 0; v < 4; ++v)
+    for (int v = 0; v < VC; ++v)
       if (lane + v * 32 < V4)
         stf4(static_cast<T*>(a.out) + static_cast<size_t>(r) * a.ldo + static_cast<size_t>(h) * a.ho + (lane + v * 32) * 4,
              make_float4(o[v].x * scale, o[v].y * scale, o[v].z * scale, o[v].w * scale));
@@ -356,8 +362,10 @@ extern "C" int spark_tree_attn(const TreeAttn* a, int f32, int tc, cudaStream_t 
       a->min_tiles <= 0 || (a->bias && a->bias_n <= 0) || a->page_ld <= 0 || ((a->ldq | a->hq | a->ldo | a->ho) & 3)) return -5;
   if (tc ? f32 || (a->bm != 128 && a->bm != 256) : a->bm != TT_BM) return -5;
   if (const int rc = tc ? launch_tree_tc(*a, s) : f32 ? launch_tiles<float>(*a, s) : launch_tiles<__nv_bfloat16>(*a, s)) return rc;
-  const dim3 grid(2 * a->sms);
-  if (f32) spark_launch_pdl(tree_merge_kernel<float>, grid, dim3(TM_THREADS), 0, s, dim3(1, 1, 1), *a);
-  else spark_launch_pdl(tree_merge_kernel<__nv_bfloat16>, grid, dim3(TM_THREADS), 0, s, dim3(1, 1, 1), *a);
+  // (narrow rows: more CTAs to an SM)
+  const dim3 grid((a->V <= 128 ? 4 : 2) * a->sms);
+  auto merge = f32 ? (a->V <= 128 ? tree_merge_kernel<float, 1> : a->V <= 256 ? tree_merge_kernel<float, 2> : tree_merge_kernel<float, 4>)
+                   : (a->V <= 128 ? tree_merge_kernel<__nv_bfloat16, 1> : a->V <= 256 ? tree_merge_kernel<__nv_bfloat16, 2> : tree_merge_kernel<__nv_bfloat16, 4>);
+  spark_launch_pdl(merge, grid, dim3(TM_THREADS), 0, s, dim3(1, 1, 1), *a);
   return spark_launch_rc("spark_tree_attn");
 }

@@ -1,6 +1,6 @@
 // Tree attention on tcgen05 (bf16 caches): the tiles of tree_attn.cu with 128 (node, head) rows per accumulator, a page of keys per step.
 //   warp 0      TMA: pages of keys and values into a ring of slots in the order the products use them (K0 K1 V0 K2 V1 ..)
-//   warp 1      issues S = Q K^T one page ahead of O += P V (P in tensor memory, over the scores that it was made from)
+//   warp 1      issues S = Q K^T one page ahead of O += P V (P in tensor memory): as soon as the softmax warps have loaded a page's scores
 //   the others  softmax, one row per thread: 64 scores are one tensor-memory load, statistics stay in the thread
 // NQ = 2: two tiles of 128 rows with their own issuing and softmax warps share the keys in shared memory (large trees: a page is read once for
 // 256 rows).  Each tile's products wait for its own softmax alone: with one issuing warp for both, a page took 2.0 us instead of ...
@@ -25,7 +25,7 @@ template <int DC, int NQ> struct Tc {
   static constexpr int SLOTS = DC == 256 ? 5 : DC == 128 ? (NQ == 2 ? 9 : 4) : (NQ == 2 ? 16 : 8);
   static constexpr int STAGE = QT ? 32768 : Q_BYTES;         // of a tile's results on their way out, over its queries where those are there
   static constexpr int SMEM = NQ * STAGE + SLOTS * SLOT + 1024 + 1024;
-  // per tile: two buffers of scores / weights of 64 columns, the accumulator
+  // per tile: scores, weights (high and low terms of 32 columns each), the accumulator
   static constexpr int TILE_COLS = 128 + DC, Q_COL = 128 + DC;
   static constexpr int COLS = QT || NQ == 2 ? 512 : 256;
   static constexpr int SOFTMAX = 1 + NQ, WARPS = SOFTMAX + 4 * NQ, THREADS = WARPS * 32, PER_SM = QT || NQ == 2 ? 1 : 2;
@@ -121,10 +121,11 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
   uint64_t* full = reinterpret_cast<uint64_t*>(ring + SLOTS * SLOT);
   uint64_t* empty = full + SLOTS;
   uint64_t* q_full = empty + SLOTS;                          // [NQ]
-  uint64_t* s_full = q_full + NQ;                            // [NQ][2] from here on
-  uint64_t* p_full = s_full + 2 * NQ;
-  uint64_t* o_full = p_full + 2 * NQ;
-  uint64_t* v_seen = o_full + 2 * NQ;                        // [NQ]: warp 1 has looked over a masked page's values
+  uint64_t* s_full = q_full + NQ;
+  uint64_t* s_read = s_full + NQ;
+  uint64_t* p_full = s_read + NQ;
+  uint64_t* o_full = p_full + NQ;
+  uint64_t* v_seen = o_full + NQ;                            // warp 1 has looked over a masked page's values
   uint64_t* v_sync = v_seen + NQ;                            // [NQ]: of 4 and of 8 softmax warps
   long long* sh = reinterpret_cast<long long*>(v_sync + NQ); // [NT / 32 + 2]
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(sh + NT / 32 + 2);
@@ -133,8 +134,10 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV);
     for (int s = 0; s < SLOTS; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], NQ); }
-    for (int s = 0; s < NQ; ++s) { mbar_init(&q_full[s], 4); mbar_init(&v_seen[s], 1); mbar_init(&v_sync[s], 4 * (s + 1)); }
-    for (int s = 0; s < 2 * NQ; ++s) { mbar_init(&s_full[s], 1); mbar_init(&p_full[s], 4); mbar_init(&o_full[s], 1); }
+    for (int s = 0; s < NQ; ++s) {
+      mbar_init(&q_full[s], 4); mbar_init(&s_full[s], 1); mbar_init(&s_read[s], 4); mbar_init(&p_full[s], 4); mbar_init(&o_full[s], 1);
+      mbar_init(&v_seen[s], 1); mbar_init(&v_sync[s], 4 * (s + 1));
+    }
     fence_barrier_init();
   }
   if (warp == 1) { tmem_alloc<L::COLS>(tmem_ptr); tmem_relinquish(); }
@@ -205,27 +208,24 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       ++items;
       for (int j = -1; j < it.nj; ++j) {
         if (j + 1 < it.nj) {
-          const int t = n + j + 1, b = t & 1;
-          ok = __all_sync(0xffffffffu, mbar_wait(&full[c.slot], c.ph));
-          // the scores go where the weights of two pages back were: their product has to be done
-          if (ok && t >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&o_full[q * 2 + b], ((t - 2) >> 1) & 1));
+          const int t = n + j + 1;
+          ok = __all_sync(0xffffffffu, mbar_wait(&full[c.slot], c.ph) && (t == 0 || mbar_wait(&s_read[q], (t - 1) & 1)));
           if (!ok) { set_status(a.status, ST_TIMEOUT_MBAR_FULL, blockIdx.x, it.s, j); break; }
           tc_fence_after();
           if (elect_one()) {
-            const uint32_t d = tm + b * 64;
             for (int k = 0; k < ksteps; ++k) {
               const uint64_t kd = make_smem_desc_sw128(rs + c.slot * SLOT + (k >> 2) * KV_CHUNK) + 2 * (k & 3);
-              if (L::QT) umma_f16_ts(d, tm + L::Q_COL + k * 8, kd, id_s, k != 0);
-              else umma_f16(d, make_smem_desc_sw128(qs + (k >> 2) * Q_CHUNK) + 2 * (k & 3), kd, id_s, k != 0);
+              if (L::QT) umma_f16_ts(tm, tm + L::Q_COL + k * 8, kd, id_s, k != 0);
+              else umma_f16(tm, make_smem_desc_sw128(qs + (k >> 2) * Q_CHUNK) + 2 * (k & 3), kd, id_s, k != 0);
             }
-            umma_commit(&s_full[q * 2 + b]);
+            umma_commit(&s_full[q]);
             umma_commit(&empty[c.slot]);
           }
           __syncwarp();
           tc_step<SLOTS>(c);
         }
         if (j < 0) continue;
-        const int b = (n + j) & 1, tok0 = (it.j + j) * TA_PAGE;
+        const int tok0 = (it.j + j) * TA_PAGE;
         if ((j & 31) == 0) there = __ballot_sync(0xffffffffu, j + lane < it.nj && ta_page(a, slot, it.j + j + lane) >= 0);
         ok = __all_sync(0xffffffffu, mbar_wait(&full[c.slot], c.ph));
         if (q == 0 && ok && (tok0 + TA_PAGE > it.seg.len || tok0 < edge || !((there >> (j & 31)) & 1u))) {
@@ -254,17 +254,17 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
             for (int i = 0; i < act; ++i) mbar_arrive(&v_seen[i]);
           }
         }
-        ok = ok && __all_sync(0xffffffffu, mbar_wait(&p_full[q * 2 + b], ((n + j) >> 1) & 1));
+        ok = ok && __all_sync(0xffffffffu, mbar_wait(&p_full[q], (n + j) & 1));
         if (!ok) { set_status(a.status, ST_TIMEOUT_MBAR_FULL, blockIdx.x, it.s, j); break; }
         tc_fence_after();
         if (elect_one()) {
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const uint64_t vd = tc_desc_nmajor(rs + c.slot * SLOT + k * 2048, KV_CHUNK);
-            umma_f16_ts(tm + 128, tm + b * 64 + k * 8, vd, id_o, 1);
-            umma_f16_ts(tm + 128, tm + b * 64 + 32 + k * 8, vd, id_o, 1);
+            umma_f16_ts(tm + 128, tm + 64 + k * 8, vd, id_o, 1);
+            umma_f16_ts(tm + 128, tm + 96 + k * 8, vd, id_o, 1);
           }
-          umma_commit(&o_full[q * 2 + b]);
+          umma_commit(&o_full[q]);
           umma_commit(&empty[c.slot]);
         }
         __syncwarp();
@@ -327,7 +327,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       const int edge = ta_first_visible(a, sg.len + sg.n - 1);         // from here on every row sees committed tokens
       uint32_t there = 0u;                                   // pages of the current 32 that the table leads to
       for (int j = 0; j < it.nj; ++j, ++n) {
-        const int b = n & 1, tok0 = (it.j + j) * TA_PAGE;
+        const int tok0 = (it.j + j) * TA_PAGE;
         if ((j & 31) == 0) there = __ballot_sync(0xffffffffu, j + lane < it.nj && ta_page(a, slot, it.j + j + lane) >= 0);
         const bool page = (there >> (j & 31)) & 1u, whole = tok0 + TA_PAGE <= sg.len && tok0 >= edge && page;
         uint64_t seen = ~0ull;
@@ -340,19 +340,26 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
             at_hi = n1 < 0 ? tok0 + lane + 32 : (n1 < sg.n ? a.pos[sg.r0 + n1] : p);
           }
         }
-        ok = __all_sync(0xffffffffu, mbar_wait(&s_full[q * 2 + b], (n >> 1) & 1));
+        ok = __all_sync(0xffffffffu, mbar_wait(&s_full[q], n & 1));
         if (!ok) { set_status(a.status, ST_TIMEOUT_TMEM_FULL, blockIdx.x, it.s, j); break; }
         tc_fence_after();
         float s[64];
-        if (!idle) {
+        if (idle) {                                          // (it waits as well: weights of two pages may not be announced in one phase)
+          if (lane == 0) mbar_arrive(&s_read[q]);
+          if (n > 0) ok = __all_sync(0xffffffffu, mbar_wait(&o_full[q], (n - 1) & 1));
+          if (!ok) { set_status(a.status, ST_TIMEOUT_TMEM_FULL, blockIdx.x, it.s, j); break; }
+        } else {
           {
             uint32_t raw[2][32];
-            tmem_ld_32x32(t_lane + b * 64, raw[0]);
-            tmem_ld_32x32(t_lane + b * 64 + 32, raw[1]);
+            tmem_ld_32x32(t_lane, raw[0]);
+            tmem_ld_32x32(t_lane + 32, raw[1]);
             tmem_ld_wait();
 #pragma unroll
             for (int i = 0; i < 64; ++i) s[i] = __uint_as_float(raw[i >> 5][i & 31]);
           }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s_read[q]);
           if (FEAT) {
 #pragma unroll
             for (int i = 0; i < 64; ++i) s[i] *= a.scale;
@@ -379,9 +386,20 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
                 for (int i = 0; i < 64; ++i) s[i] += far;
               } else {
 #pragma unroll
-                for (int i = 0; i < 64; ++i) {
-                  const int d = nodes ? p - __shfl_sync(0xffffffffu, i < 32 ? at_lo : at_hi, i & 31) : d0 - i;
-                  s[i] += __ldg(bh + min(max(d, 0), a.bias_n - 1));
+                for (int i0 = 0; i0 < 64; i0 += 16) {        // sixteen in flight
+                  float x[16];
+                  if (nodes) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                      const int d = p - __shfl_sync(0xffffffffu, i0 < 32 ? at_lo : at_hi, (i0 & 31) + i);
+                      x[i] = __ldg(bh + min(max(d, 0), a.bias_n - 1));
+                    }
+                  } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) x[i] = __ldg(bh + min(d0 - i0 - i, a.bias_n - 1));
+                  }
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) s[i0 + i] += x[i];
                 }
               }
             }
@@ -416,6 +434,12 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
           const float r = ref == -INFINITY ? 0.f : ref;
           const uint64_t c2 = FEAT ? tc_two(TA_LOG2E, TA_LOG2E) : tc_two(c1, c1), r2 = tc_two(-r, -r), one = tc_two(-1.f, -1.f);
           uint64_t sum[2] = {0ull, 0ull};
+          // the weights' place: the product before has read it
+          if (n > 0) {
+            ok = __all_sync(0xffffffffu, mbar_wait(&o_full[q], (n - 1) & 1));
+            if (!ok) { set_status(a.status, ST_TIMEOUT_TMEM_FULL, blockIdx.x, it.s, j); break; }
+            tc_fence_after();
+          }
 #pragma unroll
           for (int part = 0; part < 2; ++part) {
             uint32_t hi[16], lo[16];
@@ -429,15 +453,12 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
               const uint64_t d = tc_fma2(tc_two(__uint_as_float(hi[i] << 16), __uint_as_float(hi[i] & 0xffff0000u)), one, e);
               lo[i] = tc_pack(tc_lo(d), tc_hi(d));
             }
-            tmem_st_32x16(t_lane + b * 64 + part * 16, hi);
-            tmem_st_32x16(t_lane + b * 64 + 32 + part * 16, lo);
+            tmem_st_32x16(t_lane + 64 + part * 16, hi);
+            tmem_st_32x16(t_lane + 96 + part * 16, lo);
           }
           sum[0] = tc_add2(sum[0], sum[1]);
           l += tc_lo(sum[0]) + tc_hi(sum[0]);
-          if (__any_sync(0xffffffffu, rescale)) {            // the product before has to be done
-            ok = __all_sync(0xffffffffu, mbar_wait(&o_full[q * 2 + (b ^ 1)], ((n - 1) >> 1) & 1));
-            if (!ok) { set_status(a.status, ST_TIMEOUT_TMEM_FULL, blockIdx.x, it.s, j); break; }
-            tc_fence_after();
+          if (__any_sync(0xffffffffu, rescale)) {
             const uint64_t k2 = tc_two(c, c);
 #pragma unroll 1
             for (int cc = 0; cc < vn; cc += 32) {
@@ -461,11 +482,6 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
           const uint64_t bad = odd_rows[2 * vs] | static_cast<uint64_t>(odd_rows[2 * vs + 1]) << 32;
           if (bad) {                                         // (rare)
             uint8_t* vals = ring + vs * SLOT;
-            if (j > 0) {
-              ok = __all_sync(0xffffffffu, mbar_wait(&o_full[q * 2 + (b ^ 1)], ((n - 1) >> 1) & 1));
-              if (!ok) { set_status(a.status, ST_TIMEOUT_TMEM_FULL, blockIdx.x, it.s, j); break; }
-            }
-            tc_fence_after();
             const float r = ref == -INFINITY ? 0.f : ref;
 #pragma unroll 1
             for (int cc = 0; cc < vn && !idle; cc += 32) {
@@ -504,12 +520,12 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[q * 2 + b]);
+        if (lane == 0) mbar_arrive(&p_full[q]);
       }
       if (!ok) break;
       // ---- the rows' outputs, or this CTA's part of them: 32 rows of a warp pass shared memory (its own queries', which are used up) in
       // blocks of columns, so that a row's columns are written together
-      ok = __all_sync(0xffffffffu, mbar_wait(&o_full[q * 2 + ((n - 1) & 1)], ((n - 1) >> 1) & 1));
+      ok = __all_sync(0xffffffffu, mbar_wait(&o_full[q], (n - 1) & 1));
       if (!ok) { set_status(a.status, ST_TIMEOUT_TMEM_FULL, blockIdx.x, it.s, it.nj); break; }
       tc_fence_after();
       if (idle) { tc_fence_before(); continue; }
