@@ -5,8 +5,11 @@
 // NQ = 2: two tiles of 128 rows with their own issuing and softmax warps share the keys in shared memory (large trees: a page is read once for
 // 256 rows).  Each tile's products wait for its own softmax alone: with one issuing warp for both, a page took 2.0 us instead of ...
 //
-// Weights enter the product as two bf16 terms (2^-17 of a weight is lost), so that the reference of the exponentials may lag behind the
-// maximum: the accumulator is rescaled only when a row's maximum outgrew its reference by 2^8.
+// Weights are exponentials against a reference that may lag behind the maximum: the accumulator is rescaled only when a row's maximum outgrew
+// its reference by 2^8.  They enter the product as two bf16 terms (2^-17 of a weight is lost) where reading the keys takes longer than the
+// products (NQ = 1), and as one (half a step of bf16 each, at random, less than the step that the outputs are rounded to) where it does not:
+// for 256 rows the second term would be a third of all products.  One-term weights have two places, so that a page's weights need not wait
+// for the product of the page before.
 //
 // A page that not every row sees whole (the tree itself, the edge of a window or chunk) is masked by 64 bits per row.  Warp 1 looks its values
 // over first: rows that hold no token of the request are zeroed, and where a value is not finite, 0 * value would spoil the rows that do not
@@ -25,7 +28,8 @@ template <int DC, int NQ> struct Tc {
   static constexpr int SLOTS = DC == 256 ? 5 : DC == 128 ? (NQ == 2 ? 9 : 4) : (NQ == 2 ? 16 : 8);
   static constexpr int STAGE = QT ? 32768 : Q_BYTES;         // of a tile's results on their way out, over its queries where those are there
   static constexpr int SMEM = NQ * STAGE + SLOTS * SLOT + 1024 + 1024;
-  // per tile: scores, weights (high and low terms of 32 columns each), the accumulator
+  static constexpr bool TWO = NQ == 1;
+  // per tile: scores, weights (high and low terms of 32 columns each, or two places for high ones), the accumulator
   static constexpr int TILE_COLS = 128 + DC, Q_COL = 128 + DC;
   static constexpr int COLS = QT || NQ == 2 ? 512 : 256;
   static constexpr int SOFTMAX = 1 + NQ, WARPS = SOFTMAX + 4 * NQ, THREADS = WARPS * 32, PER_SM = QT || NQ == 2 ? 1 : 2;
@@ -124,8 +128,8 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
   uint64_t* s_full = q_full + NQ;
   uint64_t* s_read = s_full + NQ;
   uint64_t* p_full = s_read + NQ;
-  uint64_t* o_full = p_full + NQ;
-  uint64_t* v_seen = o_full + NQ;                            // warp 1 has looked over a masked page's values
+  uint64_t* o_full = p_full + 2 * NQ;                        // ([NQ][2] like p_full)
+  uint64_t* v_seen = o_full + 2 * NQ;                        // warp 1 has looked over a masked page's values
   uint64_t* v_sync = v_seen + NQ;                            // [NQ]: of 4 and of 8 softmax warps
   long long* sh = reinterpret_cast<long long*>(v_sync + NQ); // [NT / 32 + 2]
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(sh + NT / 32 + 2);
@@ -135,9 +139,10 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV);
     for (int s = 0; s < SLOTS; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], NQ); }
     for (int s = 0; s < NQ; ++s) {
-      mbar_init(&q_full[s], 4); mbar_init(&s_full[s], 1); mbar_init(&s_read[s], 4); mbar_init(&p_full[s], 4); mbar_init(&o_full[s], 1);
+      mbar_init(&q_full[s], 4); mbar_init(&s_full[s], 1); mbar_init(&s_read[s], 4);
       mbar_init(&v_seen[s], 1); mbar_init(&v_sync[s], 4 * (s + 1));
     }
+    for (int s = 0; s < 2 * NQ; ++s) { mbar_init(&p_full[s], 4); mbar_init(&o_full[s], 1); }
     fence_barrier_init();
   }
   if (warp == 1) { tmem_alloc<L::COLS>(tmem_ptr); tmem_relinquish(); }
@@ -152,6 +157,8 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
   const int rep = a.H / a.G;
   TreeItem it;
   bool ok = true;
+  const auto place = [](int n) { return L::TWO ? 0 : n & 1; };         // barrier and phase of page n's weights
+  const auto phase = [](int n) { return static_cast<uint32_t>(L::TWO ? n & 1 : (n >> 1) & 1); };
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
@@ -213,10 +220,13 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
           if (!ok) { set_status(a.status, ST_TIMEOUT_MBAR_FULL, blockIdx.x, it.s, j); break; }
           tc_fence_after();
           if (elect_one()) {
-            for (int k = 0; k < ksteps; ++k) {
-              const uint64_t kd = make_smem_desc_sw128(rs + c.slot * SLOT + (k >> 2) * KV_CHUNK) + 2 * (k & 3);
-              if (L::QT) umma_f16_ts(tm, tm + L::Q_COL + k * 8, kd, id_s, k != 0);
-              else umma_f16(tm, make_smem_desc_sw128(qs + (k >> 2) * Q_CHUNK) + 2 * (k & 3), kd, id_s, k != 0);
+            const uint64_t kd = make_smem_desc_sw128(rs + c.slot * SLOT), qd = make_smem_desc_sw128(qs);
+#pragma unroll
+            for (int k = 0; k < DC / 16; ++k) {
+              if (k >= ksteps) break;
+              const uint64_t kk = kd + (k >> 2) * (KV_CHUNK >> 4) + 2 * (k & 3);
+              if (L::QT) umma_f16_ts(tm, tm + L::Q_COL + k * 8, kk, id_s, k != 0);
+              else umma_f16(tm, qd + (k >> 2) * (Q_CHUNK >> 4) + 2 * (k & 3), kk, id_s, k != 0);
             }
             umma_commit(&s_full[q]);
             umma_commit(&empty[c.slot]);
@@ -254,17 +264,18 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
             for (int i = 0; i < act; ++i) mbar_arrive(&v_seen[i]);
           }
         }
-        ok = ok && __all_sync(0xffffffffu, mbar_wait(&p_full[q], (n + j) & 1));
+        ok = ok && __all_sync(0xffffffffu, mbar_wait(&p_full[q * 2 + place(n + j)], phase(n + j)));
         if (!ok) { set_status(a.status, ST_TIMEOUT_MBAR_FULL, blockIdx.x, it.s, j); break; }
         tc_fence_after();
         if (elect_one()) {
+          const uint64_t vd = tc_desc_nmajor(rs + c.slot * SLOT, KV_CHUNK);
+          const uint32_t w = tm + 64 + place(n + j) * 32;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const uint64_t vd = tc_desc_nmajor(rs + c.slot * SLOT + k * 2048, KV_CHUNK);
-            umma_f16_ts(tm + 128, tm + 64 + k * 8, vd, id_o, 1);
-            umma_f16_ts(tm + 128, tm + 96 + k * 8, vd, id_o, 1);
+            umma_f16_ts(tm + 128, w + k * 8, vd + k * 128, id_o, 1);
+            if (L::TWO) umma_f16_ts(tm + 128, w + 32 + k * 8, vd + k * 128, id_o, 1);
           }
-          umma_commit(&o_full[q]);
+          umma_commit(&o_full[q * 2 + place(n + j)]);
           umma_commit(&empty[c.slot]);
         }
         __syncwarp();
@@ -277,6 +288,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     const int q = (warp - L::SOFTMAX) >> 2, quad = warp & 3, row = quad * 32 + lane;
     const uint32_t t_lane = tmem + (static_cast<uint32_t>(quad * 32) << 16) + q * L::TILE_COLS;
     const int vn = (a.V + 15) / 16 * 16, vn_units = (a.V + 63) / 64 * 8;
+    constexpr int BACK = L::TWO ? 1 : 2;                     // pages back that had this page's place of the weights
     uint32_t sync_phase[NQ] = {}, seen_phase = 0u;
     int n = 0, seq = 0;                                      // pages of this tile so far; position of the item in the ring's sequence
     while (ok && ta_next(a, range, it)) {
@@ -346,7 +358,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         float s[64];
         if (idle) {                                          // (it waits as well: weights of two pages may not be announced in one phase)
           if (lane == 0) mbar_arrive(&s_read[q]);
-          if (n > 0) ok = __all_sync(0xffffffffu, mbar_wait(&o_full[q], (n - 1) & 1));
+          if (n >= BACK) ok = __all_sync(0xffffffffu, mbar_wait(&o_full[q * 2 + place(n - BACK)], phase(n - BACK)));
           if (!ok) { set_status(a.status, ST_TIMEOUT_TMEM_FULL, blockIdx.x, it.s, j); break; }
         } else {
           {
@@ -434,9 +446,8 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
           const float r = ref == -INFINITY ? 0.f : ref;
           const uint64_t c2 = FEAT ? tc_two(TA_LOG2E, TA_LOG2E) : tc_two(c1, c1), r2 = tc_two(-r, -r), one = tc_two(-1.f, -1.f);
           uint64_t sum[2] = {0ull, 0ull};
-          // the weights' place: the product before has read it
-          if (n > 0) {
-            ok = __all_sync(0xffffffffu, mbar_wait(&o_full[q], (n - 1) & 1));
+          if (n >= BACK) {                                   // the weights' place: the product has read it
+            ok = __all_sync(0xffffffffu, mbar_wait(&o_full[q * 2 + place(n - BACK)], phase(n - BACK)));
             if (!ok) { set_status(a.status, ST_TIMEOUT_TMEM_FULL, blockIdx.x, it.s, j); break; }
             tc_fence_after();
           }
@@ -450,15 +461,22 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
               const uint64_t e = tc_two(tc_ex2(tc_lo(z)), tc_ex2(tc_hi(z)));
               sum[i & 1] = tc_add2(sum[i & 1], e);
               hi[i] = tc_pack(tc_lo(e), tc_hi(e));
-              const uint64_t d = tc_fma2(tc_two(__uint_as_float(hi[i] << 16), __uint_as_float(hi[i] & 0xffff0000u)), one, e);
-              lo[i] = tc_pack(tc_lo(d), tc_hi(d));
+              if (L::TWO) {
+                const uint64_t d = tc_fma2(tc_two(__uint_as_float(hi[i] << 16), __uint_as_float(hi[i] & 0xffff0000u)), one, e);
+                lo[i] = tc_pack(tc_lo(d), tc_hi(d));
+              }
             }
-            tmem_st_32x16(t_lane + 64 + part * 16, hi);
-            tmem_st_32x16(t_lane + 96 + part * 16, lo);
+            tmem_st_32x16(t_lane + 64 + place(n) * 32 + part * 16, hi);
+            if (L::TWO) tmem_st_32x16(t_lane + 96 + part * 16, lo);
           }
           sum[0] = tc_add2(sum[0], sum[1]);
           l += tc_lo(sum[0]) + tc_hi(sum[0]);
           if (__any_sync(0xffffffffu, rescale)) {
+            if (!L::TWO) {                                   // (with two terms the product before has been waited for)
+              ok = __all_sync(0xffffffffu, mbar_wait(&o_full[q * 2 + place(n - 1)], phase(n - 1)));
+              if (!ok) { set_status(a.status, ST_TIMEOUT_TMEM_FULL, blockIdx.x, it.s, j); break; }
+              tc_fence_after();
+            }
             const uint64_t k2 = tc_two(c, c);
 #pragma unroll 1
             for (int cc = 0; cc < vn; cc += 32) {
@@ -482,6 +500,11 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
           const uint64_t bad = odd_rows[2 * vs] | static_cast<uint64_t>(odd_rows[2 * vs + 1]) << 32;
           if (bad) {                                         // (rare)
             uint8_t* vals = ring + vs * SLOT;
+            if (!L::TWO && n > 0) {
+              ok = __all_sync(0xffffffffu, mbar_wait(&o_full[q * 2 + place(n - 1)], phase(n - 1)));
+              if (!ok) { set_status(a.status, ST_TIMEOUT_TMEM_FULL, blockIdx.x, it.s, j); break; }
+              tc_fence_after();
+            }
             const float r = ref == -INFINITY ? 0.f : ref;
 #pragma unroll 1
             for (int cc = 0; cc < vn && !idle; cc += 32) {
@@ -520,12 +543,12 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[q]);
+        if (lane == 0) mbar_arrive(&p_full[q * 2 + place(n)]);
       }
       if (!ok) break;
       // ---- the rows' outputs, or this CTA's part of them: 32 rows of a warp pass shared memory (its own queries', which are used up) in
       // blocks of columns, so that a row's columns are written together
-      ok = __all_sync(0xffffffffu, mbar_wait(&o_full[q], (n - 1) & 1));
+      ok = __all_sync(0xffffffffu, mbar_wait(&o_full[q * 2 + place(n - 1)], phase(n - 1)));
       if (!ok) { set_status(a.status, ST_TIMEOUT_TMEM_FULL, blockIdx.x, it.s, it.nj); break; }
       tc_fence_after();
       if (idle) { tc_fence_before(); continue; }

@@ -12,7 +12,7 @@ pytestmark = pytest.mark.gpu
 DEV = "cuda"
 BF16, F32 = torch.bfloat16, torch.float32
 DTYPES = [F32, BF16]
-WEIGHTS = {F32: 0.0, BF16: 2.0 ** -16}       # half step of a weight: two bf16 terms
+WEIGHTS = {F32: 0.0, BF16: U.half_step(BF16)}          # of a weight: one or two bf16 terms enter the product
 
 
 @pytest.fixture(autouse=True)
