@@ -5,8 +5,9 @@
 // NQ = 2: two tiles of 128 rows with their own issuing and softmax warps share the keys in shared memory (large trees: a page is read once for
 // 256 rows).  Each tile's products wait for its own softmax alone: with one issuing warp for both, a page took 2.0 us instead of ...
 //
-// Weights are exponentials against a reference that may lag behind the maximum: the accumulator is rescaled only when a row's maximum outgrew
-// its reference by 2^8.  They enter the product as two bf16 terms (2^-17 of a weight is lost) where reading the keys takes longer than the
+// Weights are exponentials against a reference that may lag far behind the maximum: the maximum of the first page that a row sees, renewed
+// (and the accumulator rescaled) only when a page's weights add up to more than 2^40; fp32 sums and bf16 weights lose nothing by a common
+// factor.  So most pages need no maximum.  Weights enter the product as two bf16 terms (2^-17 of a weight is lost) where reading the keys takes longer than the
 // products (NQ = 1), and as one (half a step of bf16 each, at random, less than the step that the outputs are rounded to) where it does not:
 // for 256 rows the second term would be a third of all products.  One-term weights have two places, so that a page's weights need not wait
 // for the product of the page before.
@@ -20,7 +21,7 @@ namespace spark {
 
 int make_tmap_page(CUtensorMap* m, const void* base, uint64_t pages, uint64_t G, uint64_t D, uint64_t tok, uint64_t page);
 
-constexpr float TC_LAG = 8.f;                                // log2
+constexpr float TC_MOST = 1099511627776.f;                   // 2^40
 
 template <int DC, int NQ> struct Tc {
   static constexpr bool QT = DC == 256;                      // queries in tensor memory: shared memory has no room for them beside the ring
@@ -334,6 +335,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         __syncwarp();
         if (lane == 0) mbar_arrive(&q_full[q]);
       }
+      bool fresh = true;                                     // some row of the warp has no reference yet
       float ref = -INFINITY, l = 0.f;                        // of the exponentials (FEAT: natural, else log2), and their sum
       const float c1 = FEAT ? 1.f : a.scale * TA_LOG2E;
       const int edge = ta_first_visible(a, sg.len + sg.n - 1);         // from here on every row sees committed tokens
@@ -434,44 +436,58 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
             for (int i = 0; i < 64; ++i) s[i] = ((i < 32 ? m0 : m1) >> (i & 31)) & 1u ? s[i] : -INFINITY;
           }
           // ---- weights
-          float mx[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-          for (int i = 4; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
-          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c1;
-          const float lag = FEAT ? TC_LAG * TA_LN2 : TC_LAG;
-          const bool grow = ref == -INFINITY ? top > -INFINITY : top > ref + lag;
-          const bool rescale = grow && ref != -INFINITY;
-          const float c = rescale ? exp2f(FEAT ? (ref - top) * TA_LOG2E : ref - top) : 1.f;
-          if (grow) { l *= c; ref = top; }
-          const float r = ref == -INFINITY ? 0.f : ref;
-          const uint64_t c2 = FEAT ? tc_two(TA_LOG2E, TA_LOG2E) : tc_two(c1, c1), r2 = tc_two(-r, -r), one = tc_two(-1.f, -1.f);
-          uint64_t sum[2] = {0ull, 0ull};
+          const uint64_t c2 = FEAT ? tc_two(TA_LOG2E, TA_LOG2E) : tc_two(c1, c1);
+          bool renew = fresh, rescale = false;
+          float c = 1.f, page_sum;
           if (n >= BACK) {                                   // the weights' place: the product has read it
             ok = __all_sync(0xffffffffu, mbar_wait(&o_full[q * 2 + place(n - BACK)], phase(n - BACK)));
             if (!ok) { set_status(a.status, ST_TIMEOUT_TMEM_FULL, blockIdx.x, it.s, j); break; }
             tc_fence_after();
           }
+#pragma unroll 1
+          while (true) {
+            if (renew) {
+              float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-          for (int part = 0; part < 2; ++part) {
-            uint32_t hi[16], lo[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const uint64_t x = tc_two(s[part * 32 + 2 * i], s[part * 32 + 2 * i + 1]);
-              const uint64_t z = FEAT ? tc_mul2(tc_add2(x, r2), c2) : tc_fma2(x, c2, r2);
-              const uint64_t e = tc_two(tc_ex2(tc_lo(z)), tc_ex2(tc_hi(z)));
-              sum[i & 1] = tc_add2(sum[i & 1], e);
-              hi[i] = tc_pack(tc_lo(e), tc_hi(e));
-              if (L::TWO) {
-                const uint64_t d = tc_fma2(tc_two(__uint_as_float(hi[i] << 16), __uint_as_float(hi[i] & 0xffff0000u)), one, e);
-                lo[i] = tc_pack(tc_lo(d), tc_hi(d));
+              for (int i = 4; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
+              const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c1;
+              if (ref == -INFINITY) ref = top;
+              else if (top > ref) {
+                rescale = true;
+                c = exp2f(FEAT ? (ref - top) * TA_LOG2E : ref - top);
+                l *= c;
+                ref = top;
               }
+              fresh = __any_sync(0xffffffffu, ref == -INFINITY);       // rows that have seen nothing yet
             }
-            tmem_st_32x16(t_lane + 64 + place(n) * 32 + part * 16, hi);
-            if (L::TWO) tmem_st_32x16(t_lane + 96 + part * 16, lo);
+            const float r = ref == -INFINITY ? 0.f : ref;
+            const uint64_t r2 = tc_two(-r, -r), one = tc_two(-1.f, -1.f);
+            uint64_t sum[2] = {0ull, 0ull};
+#pragma unroll
+            for (int part = 0; part < 2; ++part) {
+              uint32_t hi[16], lo[16];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const uint64_t x = tc_two(s[part * 32 + 2 * i], s[part * 32 + 2 * i + 1]);
+                const uint64_t z = FEAT ? tc_mul2(tc_add2(x, r2), c2) : tc_fma2(x, c2, r2);
+                const uint64_t e = tc_two(tc_ex2(tc_lo(z)), tc_ex2(tc_hi(z)));
+                sum[i & 1] = tc_add2(sum[i & 1], e);
+                hi[i] = tc_pack(tc_lo(e), tc_hi(e));
+                if (L::TWO) {
+                  const uint64_t d = tc_fma2(tc_two(__uint_as_float(hi[i] << 16), __uint_as_float(hi[i] & 0xffff0000u)), one, e);
+                  lo[i] = tc_pack(tc_lo(d), tc_hi(d));
+                }
+              }
+              tmem_st_32x16(t_lane + 64 + place(n) * 32 + part * 16, hi);
+              if (L::TWO) tmem_st_32x16(t_lane + 96 + part * 16, lo);
+            }
+            sum[0] = tc_add2(sum[0], sum[1]);
+            page_sum = tc_lo(sum[0]) + tc_hi(sum[0]);
+            if (renew || !__any_sync(0xffffffffu, !(page_sum < TC_MOST))) break;
+            renew = true;
           }
-          sum[0] = tc_add2(sum[0], sum[1]);
-          l += tc_lo(sum[0]) + tc_hi(sum[0]);
-          if (__any_sync(0xffffffffu, rescale)) {
+          l += page_sum;
+          if (renew && __any_sync(0xffffffffu, rescale)) {
             if (!L::TWO) {                                   // (with two terms the product before has been waited for)
               ok = __all_sync(0xffffffffu, mbar_wait(&o_full[q * 2 + place(n - 1)], phase(n - 1)));
               if (!ok) { set_status(a.status, ST_TIMEOUT_TMEM_FULL, blockIdx.x, it.s, j); break; }
