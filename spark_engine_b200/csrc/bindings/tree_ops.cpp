@@ -139,12 +139,15 @@ std::shared_ptr<RowMaps> slot_maps(const Tensor& lengths, const Tensor& counts, 
   const auto opt = tables.options();
   auto m = std::make_shared<RowMaps>();
   m->lengths = lengths; m->counts = counts; m->tables = tables; m->slots = slots; m->parents = parents; m->nodes = nodes;
-  m->starts = at::empty({S + 1}, opt);
-  m->slot = at::empty({rows}, opt);
-  m->index = at::empty({rows}, opt);
-  m->pos = at::empty({rows}, opt);
+  // one allocation for what is int32: [anc | slot | index | pos | starts]
+  const int64_t na = rows * words;
+  Tensor all = at::empty({na + 3 * rows + S + 1}, opt);
+  if (words) m->anc = all.as_strided({rows, words}, {words, 1}, 0);
+  m->slot = all.as_strided({rows}, {1}, na);
+  m->index = all.as_strided({rows}, {1}, na + rows);
+  m->pos = all.as_strided({rows}, {1}, na + 2 * rows);
+  m->starts = all.as_strided({S + 1}, {1}, na + 3 * rows);
   m->cache_row = at::empty({rows}, opt.dtype(at::kLong));
-  if (words) m->anc = at::empty({rows, words}, opt);
   if (!run) return m;
   if (S == 0) {
     m->starts.zero_();
@@ -170,7 +173,7 @@ Tensor path_conv(Tensor x, const Tensor& w, const Tensor& tail, const RowMaps& m
   NEED(w.dim() == 2 && w.size(0) > 0 && w.size(1) == C && w.scalar_type() == at::kFloat && w.device() == dev && w.is_contiguous() && aligned(w),
        "w must be fp32 [taps, channels]");
   const int64_t taps = w.size(0);
-  NEED(taps <= 1024, "at most 1024 taps");
+  NEED(taps <= 32, "at most 32 taps");
   NEED(tail.dim() == 3 && tail.size(1) == taps - 1 && tail.size(2) == C && tail.scalar_type() == dt && tail.device() == dev && tail.is_contiguous() && aligned(tail),
        "tail must be [slots, taps - 1, channels] in the rows' type");
   NEED(tail.size(0) == m.tables.size(0), "tail and tables must have the same slots");
@@ -234,7 +237,10 @@ Tensor tree_attention(Tensor q, const Tensor& k, const Tensor& v, const RowMaps&
   const int64_t most = (m.nodes ? std::min(m.nodes, R) : R) * (H / G);
   const int bm = !tc ? 32 : !wide && most > 128 ? 256 : 128;
   const int ctas = std::min(1024, on.dev.sms * (!tc ? 3 : bm == 256 || wide ? 1 : 2));
-  const int extra = !tc ? 0 : 6;
+  // What beginning an item costs, in pages (us of a call, extra 0 / 3 / 6 / 10 / 15: four requests of 16k tokens, heads of 256: 61.3 / 57.5 / 55.2 /
+  // 49.4 / 48.5; eight windows of 1024, heads of 128 with slopes: 37.2 / 32.1 / 31.7 / 31.5 / 34.6; ragged, soft cap and bias, whose pages take
+  // longer: 45.6 / 41.5 / 45.0 / 45.1 / 52.0)
+  const int extra = !tc ? 0 : wide ? 10 : softcap > 0 || bias || slopes ? 4 : 6;
   const int64_t no = static_cast<int64_t>(ctas) * 2 * bm * V, nm = static_cast<int64_t>(ctas) * 2 * bm * 2;
   Tensor ws = at::empty({no + nm + ctas * 4}, q.options().dtype(at::kFloat));
   float* part = static_cast<float*>(ws.data_ptr());

@@ -38,7 +38,7 @@ struct CommitJob {
   long long page, tok;                   // bytes: strides of a cache's pages and tokens, or of a slot's entries (tok) and of x's rows (page)
   int bytes, extent, kept, pad;          // bytes of a row (multiple of 16); pages of the cache, or slots of the tail; a slot's entries
 };
-constexpr int COMMIT_JOBS = 64;
+constexpr int COMMIT_JOBS = 128;
 struct CommitPaths {
   CommitJob job[COMMIT_JOBS];
   const int *path, *n_path, *starts, *lengths, *slots, *tables;

@@ -86,24 +86,26 @@ __device__ __forceinline__ bool tc_sync(uint64_t* bar, uint32_t& phase) {
 struct TcCount { int slot = 0; uint32_t ph = 0; };
 template <int N> __device__ __forceinline__ void tc_step(TcCount& c) { if (++c.slot == N) { c.slot = 0; c.ph ^= 1; } }
 
-// Which of the 64 tokens of page j row `node` (position p) sees.
-__device__ __forceinline__ uint64_t tc_mask(const TreeAttn& a, const TreeSeg& sg, int tok0, int node, int p) {
+// Bits b .. b + 63 of a row's ancestors.
+__device__ __forceinline__ uint64_t tc_ancestors(const TreeAttn& a, const TreeSeg& sg, int node, int b) {
+  if (a.anc) {
+    const uint32_t* w = a.anc + static_cast<size_t>(sg.r0 + node) * a.words;
+    const int k = b >> 5, sh = b & 31;
+    const uint64_t w0 = k < a.words ? w[k] : 0u, w1 = k + 1 < a.words ? w[k + 1] : 0u, w2 = k + 2 < a.words ? w[k + 2] : 0u;
+    const uint64_t t = (w0 | w1 << 32) >> sh;
+    return sh ? t | w2 << (64 - sh) : t;
+  }
+  const int n = node - b + 1;
+  return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1;
+}
+// Which of the 64 tokens from tok0 on row `node` (position p) sees; near: its ancestors 0 .. 63.
+__device__ __forceinline__ uint64_t tc_mask(const TreeAttn& a, const TreeSeg& sg, int tok0, int node, int p, uint64_t near) {
   const int first = ta_first_visible(a, p), i0 = tok0 - sg.len;        // the page's token 0 is node i0
   const int lo = min(max(first - tok0, 0), 64), hi = min(max(-i0, 0), 64);
   uint64_t m = hi > lo ? (hi == 64 ? ~0ull : (1ull << hi) - 1) & ~(lo == 0 ? 0ull : (1ull << lo) - 1) : 0ull;
   if (hi == 64) return m;
-  uint64_t t = 0;                                            // bit b: node max(i0, 0) + b
-  const int b0 = max(i0, 0);
-  if (a.anc) {
-    const uint32_t* w = a.anc + static_cast<size_t>(sg.r0 + node) * a.words;
-    const int k = b0 >> 5, sh = b0 & 31;
-    const uint64_t w0 = k < a.words ? w[k] : 0u, w1 = k + 1 < a.words ? w[k + 1] : 0u, w2 = k + 2 < a.words ? w[k + 2] : 0u;
-    t = (w0 | w1 << 32) >> sh;
-    if (sh) t |= w2 << (64 - sh);
-  } else {
-    const int n = node - b0 + 1;
-    t = n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1;
-  }
+  const int b0 = max(i0, 0);                                 // bit b of t: node b0 + b
+  uint64_t t = b0 == 0 ? near : sg.n <= 64 ? (b0 < 64 ? near >> b0 : 0ull) : tc_ancestors(a, sg, node, b0);
   const int left = sg.n - b0;                                // nodes there are
   if (left < 64) t &= left <= 0 ? 0ull : (1ull << left) - 1;
   if (first > sg.len)                                        // ancestors outside the window or chunk
@@ -248,6 +250,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
             const int tok = half * 32 + lane;
             uint8_t* vrow = ring + c.slot * SLOT + tok * 128;
             uint32_t most = 0u;                              // largest exponents of the row's even and odd columns
+#pragma unroll 8
             for (int u = 0; u < vunits; ++u) {
               uint4* x = reinterpret_cast<uint4*>(vrow + (u >> 3) * KV_CHUNK + (((u & 7) ^ (tok & 7)) * 16));
               if (tok >= valid) *x = make_uint4(0u, 0u, 0u, 0u);
@@ -289,7 +292,6 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     const int q = (warp - L::SOFTMAX) >> 2, quad = warp & 3, row = quad * 32 + lane;
     const uint32_t t_lane = tmem + (static_cast<uint32_t>(quad * 32) << 16) + q * L::TILE_COLS;
     const int vn = (a.V + 15) / 16 * 16, vn_units = (a.V + 63) / 64 * 8;
-    constexpr int BACK = L::TWO ? 1 : 2;                     // pages back that had this page's place of the weights
     uint32_t sync_phase[NQ] = {}, seen_phase = 0u;
     int n = 0, seq = 0;                                      // pages of this tile so far; position of the item in the ring's sequence
     while (ok && ta_next(a, range, it)) {
@@ -305,6 +307,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       const int f = it.rt * a.bm + q * 128 + min(row, pairs - 1), node = f / rep, h = it.g * rep + f - node * rep, pr = sg.r0 + node;
       const bool idle = quad * 32 >= pairs;                  // a warp without rows keeps the pace and computes nothing
       const int p = a.pos[pr], slot = a.slots ? a.slots[it.s] : it.s;
+      const uint64_t near = tc_ancestors(a, sg, node, 0);    // (asked for long before the tree's page)
       {                                                      // the row's query; columns from D on are zero
         const uint4* src = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) + static_cast<size_t>(pr) * a.ldq + static_cast<size_t>(h) * a.hq);
         const int units = row < pairs ? a.D / 8 : 0;
@@ -347,7 +350,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         uint64_t seen = ~0ull;
         int at_lo = 0, at_hi = 0;                              // FEAT: positions of the page's tokens `lane` and 32 + lane
         if (!whole && !idle) {
-          seen = page ? tc_mask(a, sg, tok0, node, p) : 0ull;
+          seen = page ? tc_mask(a, sg, tok0, node, p, near) : 0ull;
           if (FEAT && tok0 + TA_PAGE > sg.len) {
             const int n0 = tok0 + lane - sg.len, n1 = n0 + 32;
             at_lo = n0 < 0 ? tok0 + lane : (n0 < sg.n ? a.pos[sg.r0 + n0] : p);
@@ -360,7 +363,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         float s[64];
         if (idle) {                                          // (it waits as well: weights of two pages may not be announced in one phase)
           if (lane == 0) mbar_arrive(&s_read[q]);
-          if (n >= BACK) ok = __all_sync(0xffffffffu, mbar_wait(&o_full[q * 2 + place(n - BACK)], phase(n - BACK)));
+          if (L::TWO && n > 0) ok = __all_sync(0xffffffffu, mbar_wait(&o_full[q * 2], phase(n - 1)));
           if (!ok) { set_status(a.status, ST_TIMEOUT_TMEM_FULL, blockIdx.x, it.s, j); break; }
         } else {
           {
@@ -439,8 +442,9 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
           const uint64_t c2 = FEAT ? tc_two(TA_LOG2E, TA_LOG2E) : tc_two(c1, c1);
           bool renew = fresh, rescale = false;
           float c = 1.f, page_sum;
-          if (n >= BACK) {                                   // the weights' place: the product has read it
-            ok = __all_sync(0xffffffffu, mbar_wait(&o_full[q * 2 + place(n - BACK)], phase(n - BACK)));
+          // the weights' place: the product has read it (of two places: scores are announced behind the product of two pages back)
+          if (L::TWO && n > 0) {
+            ok = __all_sync(0xffffffffu, mbar_wait(&o_full[q * 2], phase(n - 1)));
             if (!ok) { set_status(a.status, ST_TIMEOUT_TMEM_FULL, blockIdx.x, it.s, j); break; }
             tc_fence_after();
           }

@@ -175,59 +175,174 @@ slot_maps_kernel(const __grid_constant__ SlotMaps a) {
 
 // ------------------------------------------------------------------------------------------------ convolution along paths
 
-constexpr int PC_ROWS = 4;
+constexpr int PC_ROWS = 64, PC_FAR = 64, PC_THREADS = 256, PC_UNITS = 16;     // rows of a tile and brought in beside them; 16-byte pieces of its channels
+constexpr int PC_STAGES = 3, PC_PER_SM = 2;
 
-// grid (row groups, channel blocks); 128 threads x 16 bytes of channels.
+__device__ __forceinline__ void pc_copy(void* d, const void* s) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(d)), "l"(s) : "memory");
+}
+
+// channels of a 16-byte piece
+__device__ __forceinline__ void pc_split(const uint4& u, float (&f)[8], __nv_bfloat16) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+}
+__device__ __forceinline__ void pc_split(const uint4& u, float (&f)[4], float) {
+  f[0] = __uint_as_float(u.x); f[1] = __uint_as_float(u.y); f[2] = __uint_as_float(u.z); f[3] = __uint_as_float(u.w);
+}
+__device__ __forceinline__ uint4 pc_join(const float (&f)[8], __nv_bfloat16) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 b = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t*>(&b);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ uint4 pc_join(const float (&f)[4], float) {
+  return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+}
+
+// grid (groups of `per` channel tiles, row tiles).  A tile's rows are brought to shared memory once and every row takes its taps from there;
+// so are up to PC_FAR rows that lie elsewhere (ancestors in front of the tile, the sequences' past).  The paths are
+// followed once for all channel tiles of a CTA, and the next two tiles' rows are on their way while one is computed.  Instructions bound it before
+// the bytes do: what depends on the row alone is formed once, and the common loop has no branches (nobody's rows take a row of zeros).
 template <typename T, int TAPS>
-__global__ void __launch_bounds__(128)
-path_conv_kernel(const __grid_constant__ PathConv a) {
-  constexpr int VEC = 16 / sizeof(T);
+__global__ void __launch_bounds__(PC_THREADS, PC_PER_SM)
+path_conv_kernel(const __grid_constant__ PathConv a, int per) {
+  constexpr int VEC = 16 / sizeof(T), STEP = PC_THREADS / PC_UNITS, ZERO = (PC_ROWS + PC_FAR) * PC_UNITS;
+  extern __shared__ __align__(16) uint4 s_x[];               // [PC_STAGES][PC_ROWS + PC_FAR + 1][PC_UNITS]
+  constexpr int BUF = ZERO + PC_UNITS, LAST = PC_STAGES - 1;
+  __shared__ const T* s_far[PC_FAR];                         // channel 0 of the rows brought in
+  __shared__ int s_fars, s_left;                             // rows that lie elsewhere; some tap found no place
+  __shared__ int s_before[PC_ROWS], s_past[PC_ROWS];         // places: of the rows in front of the tile; of the past of the request that begins here
+  __shared__ long long s_k[PC_ROWS], s_v[PC_ROWS];           // places of the results in the caches (-1: none)
+  __shared__ int s_slot[PC_ROWS], s_parent[PC_ROWS];
+  int* s_src = reinterpret_cast<int*>(s_x + PC_STAGES * BUF);        // [PC_ROWS][taps, 3 padded to 4]: a tap's place in s_x; else as `elsewhere` takes it
   pdl_wait();
   pdl_trigger();
-  const int taps = TAPS > 0 ? TAPS : a.taps;
-  const int c0 = (blockIdx.y * 128 + threadIdx.x) * VEC;
-  if (c0 >= a.C) return;
-  for (int i = 0; i < PC_ROWS; ++i) {
-    const int r = blockIdx.x * PC_ROWS + i;
-    if (r >= a.R) return;
-    const int slot = a.slot[r];
-    if (slot < 0) continue;                                  // a row behind the last request
-    const int j = a.index[r], r0 = r - j;
-    float y[VEC] = {};
+  const int taps = TAPS > 0 ? TAPS : a.taps, ld = taps == 3 ? 4 : taps, t = threadIdx.x, unit = t % PC_UNITS, b0 = blockIdx.y * PC_ROWS;
+  const int n = min(PC_ROWS, a.R - b0), tile0 = blockIdx.x * per;
+  // -1 - a flat row, or -2^30 - e: the e-th newest entry of the slot's tail
+  auto elsewhere = [&](int s, int slot) {
+    return s < -(1 << 30) ? static_cast<const T*>(a.tail) + ((static_cast<size_t>(min(slot, a.n_slots - 1)) + 1) * (taps - 1) + (s + (1 << 30))) * a.C
+                          : static_cast<const T*>(a.x) + static_cast<size_t>(-1 - s) * a.ldx;
+  };
+  auto load = [&](int i) {                                   // rows of channel tile tile0 + i
+    const int c = ((tile0 + i) * PC_UNITS + unit) * VEC;
+    if (i < per && c < a.C)
+#pragma unroll
+      for (int r = t / PC_UNITS; r < PC_ROWS; r += STEP)
+        if (r < n) pc_copy(s_x + (i % PC_STAGES) * BUF + r * PC_UNITS + unit, static_cast<const T*>(a.x) + static_cast<size_t>(b0 + r) * a.ldx + c);
+  };
+  auto load_far = [&](int i) {
+    const int c = ((tile0 + i) * PC_UNITS + unit) * VEC;
+    if (i < per && c < a.C)
+      for (int r = t / PC_UNITS; r < min(s_fars, PC_FAR); r += STEP) pc_copy(s_x + (i % PC_STAGES) * BUF + (PC_ROWS + r) * PC_UNITS + unit, s_far[r] + c);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int i = 0; i < LAST; ++i) load(i);
+  if (t < PC_STAGES * PC_UNITS) s_x[t / PC_UNITS * BUF + ZERO + unit] = make_uint4(0u, 0u, 0u, 0u);
+  for (int r = t; r < PC_ROWS * ld; r += PC_THREADS) s_src[r] = ZERO;
+  int j = 0;
+  if (t == 0) s_fars = s_left = 0;
+  if (t < PC_ROWS) s_before[t] = -1;
+  if (t < n) {
+    j = a.index[b0 + t];
+    s_parent[t] = a.parents ? a.parents[b0 + t] : j - 1;
+    const int slot = s_slot[t] = a.slot[b0 + t];
+    const long long row = a.cache_row[b0 + t];
+    const bool ok = slot >= 0 && row >= 0 && row < a.cache_rows;
+    if (slot >= 0 && !ok) set_status(a.status, ST_BOUNDS, b0 + t, static_cast<int>(row), slot);
+    s_k[t] = ok ? row / TREE_PAGE * a.k_page + row % TREE_PAGE * a.k_tok : -1;
+    s_v[t] = ok ? row / TREE_PAGE * a.v_page + row % TREE_PAGE * a.v_tok : -1;
+  }
+  __syncthreads();
+  const bool live = t < n && s_slot[t] >= 0;
+  const int r0 = b0 + t - j, head = max(r0 - b0, 0);         // the request's first row, and its first one in the tile
+  if (live) {                                                // the row, its ancestors, then the sequence's past
+    if (t == head) {
+      const int f = s_past[t] = atomicAdd(&s_fars, taps - 1);
+      for (int e = 1; e < taps; ++e)
+        if (f + e - 1 < PC_FAR) s_far[f + e - 1] = elsewhere(-(1 << 30) - e, s_slot[t]);
+    }
     int at = j, back = 0;
-    for (int tp = taps - 1; tp >= 0; --tp) {                 // the row, its ancestors, then the sequence's past
-      const T* src;
-      if (at >= 0) {
-        src = static_cast<const T*>(a.x) + static_cast<size_t>(r0 + at) * a.ldx + c0;
-        if (tp) {
-          const int p = a.parents ? a.parents[r0 + at] : at - 1;
-          at = p < at ? p : -1;
+    for (int tp = taps - 1; tp >= 0; --tp) {
+      const int x = at >= 0 ? (r0 + at >= b0 ? (r0 + at - b0) * PC_UNITS : -1 - (r0 + at)) : -(1 << 30) - ++back;
+      s_src[t * ld + tp] = x;
+      if (x < 0 && x >= -(1 << 30) && -1 - x >= b0 - PC_ROWS && atomicCAS(&s_before[-1 - x - (b0 - PC_ROWS)], -1, -2) == -1) {
+        const int f = atomicAdd(&s_fars, 1);
+        if (f < PC_FAR) s_far[f] = elsewhere(x, 0);
+        s_before[-1 - x - (b0 - PC_ROWS)] = f;
+      }
+      if (tp && at >= 0) {
+        const int p = r0 + at >= b0 ? s_parent[r0 + at - b0] : a.parents ? a.parents[r0 + at] : at - 1;
+        at = p < at ? p : -1;
+      }
+    }
+  }
+  __syncthreads();
+  if (live)
+    for (int tp = 0; tp < taps; ++tp) {
+      const int x = s_src[t * ld + tp];
+      if (x >= 0) continue;
+      const int f = x < -(1 << 30) ? s_past[head] - x - (1 << 30) - 1 : -1 - x >= b0 - PC_ROWS ? s_before[-1 - x - (b0 - PC_ROWS)] : PC_FAR;
+      if (f < PC_FAR) s_src[t * ld + tp] = (PC_ROWS + f) * PC_UNITS;
+      else s_left = 1;
+    }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < LAST; ++i) load_far(i);                // (the first group has the rows of both)
+  const bool near = !s_left;                                 // every tap is in shared memory
+  for (int i = 0; i < per; ++i) {
+    const int c0 = ((tile0 + i) * PC_UNITS + unit) * VEC;
+    float w[TAPS > 0 ? TAPS : 1][VEC];
+    if (TAPS > 0 && c0 < a.C)
+#pragma unroll
+      for (int tp = 0; tp < TAPS; ++tp)
+#pragma unroll
+        for (int e = 0; e < VEC; e += 4) *reinterpret_cast<float4*>(&w[tp][e]) = *reinterpret_cast<const float4*>(a.w + static_cast<size_t>(tp) * a.C + c0 + e);
+    asm volatile("cp.async.wait_group %0;" ::"n"(LAST - 1) : "memory");
+    __syncthreads();                                         // tile i is there, and tile i - 1 is used up
+    load(i + LAST);
+    load_far(i + LAST);
+    const uint4* xs = s_x + (i % PC_STAGES) * BUF + unit;
+    const bool isq = c0 < a.nq, isk = c0 < a.nq + a.nk;
+    T* base = isq ? static_cast<T*>(a.q) + static_cast<size_t>(b0) * a.nq + c0 : isk ? static_cast<T*>(a.k) + (c0 - a.nq) : static_cast<T*>(a.v) + (c0 - a.nq - a.nk);
+    auto store = [&](int r, const float (&y)[VEC]) {
+      const long long to = isq ? static_cast<long long>(r) * a.nq : isk ? s_k[r] : s_v[r];
+      if (to >= 0) *reinterpret_cast<uint4*>(base + to) = pc_join(y, T());
+    };
+    if (c0 >= a.C) continue;
+    if (TAPS > 0 && near) {
+#pragma unroll
+      for (int k = 0; k < PC_ROWS / STEP; ++k) {
+        const int r = t / PC_UNITS + k * STEP;
+        float y[VEC] = {};
+#pragma unroll
+        for (int tp = 0; tp < TAPS; ++tp) {
+          float f[VEC];
+          pc_split(xs[s_src[r * (TAPS == 3 ? 4 : TAPS) + tp]], f, T());
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) y[e] = fmaf(w[tp][e], f[e], y[e]);
         }
-      } else {
-        ++back;
-        src = static_cast<const T*>(a.tail) + (static_cast<size_t>(min(slot, a.n_slots - 1)) * (taps - 1) + (taps - 1 - back)) * a.C + c0;
+        if (r < n) store(r, y);
       }
+    } else {
+      for (int r = t / PC_UNITS; r < n; r += STEP) {
+        float y[VEC] = {};
+        for (int tp = 0; tp < taps; ++tp) {
+          const int s = s_src[r * ld + tp];
+          float f[VEC];
+          pc_split(s >= 0 ? xs[s] : *reinterpret_cast<const uint4*>(elsewhere(s, s_slot[r]) + c0), f, T());
 #pragma unroll
-      for (int e = 0; e < VEC; e += 4) {
-        const float4 u = ldf4(src + e), w = *reinterpret_cast<const float4*>(a.w + static_cast<size_t>(tp) * a.C + c0 + e);
-        y[e] = fmaf(w.x, u.x, y[e]); y[e + 1] = fmaf(w.y, u.y, y[e + 1]);
-        y[e + 2] = fmaf(w.z, u.z, y[e + 2]); y[e + 3] = fmaf(w.w, u.w, y[e + 3]);
+          for (int e = 0; e < VEC; ++e) y[e] = fmaf(a.w[static_cast<size_t>(tp) * a.C + c0 + e], f[e], y[e]);
+        }
+        store(r, y);
       }
     }
-    T* dst;
-    if (c0 < a.nq) dst = static_cast<T*>(a.q) + static_cast<size_t>(r) * a.nq + c0;
-    else {
-      const long long row = a.cache_row[r];
-      if (row < 0 || row >= a.cache_rows) {
-        set_status(a.status, ST_BOUNDS, r, static_cast<int>(row), slot);
-        continue;
-      }
-      const long long page = row / TREE_PAGE, tok = row % TREE_PAGE;
-      dst = c0 < a.nq + a.nk ? static_cast<T*>(a.k) + page * a.k_page + tok * a.k_tok + (c0 - a.nq)
-                             : static_cast<T*>(a.v) + page * a.v_page + tok * a.v_tok + (c0 - a.nq - a.nk);
-    }
-#pragma unroll
-    for (int e = 0; e < VEC; e += 4) stf4(dst + e, make_float4(y[e], y[e + 1], y[e + 2], y[e + 3]));
   }
 }
 
@@ -307,12 +422,34 @@ extern "C" int spark_slot_maps(const SlotMaps* a, cudaStream_t s) {
 extern "C" int spark_path_conv(const PathConv* a, int f32, cudaStream_t s) {
   if (a->R <= 0) return 0;
   if (a->taps < 1 || ((a->C | a->nq | a->nk | a->ldx) & 7) || a->nq + a->nk > a->C || a->n_slots <= 0) return -5;
-  const int vec = f32 ? 4 : 8;
-  const dim3 grid((a->R + PC_ROWS - 1) / PC_ROWS, (a->C / vec + 127) / 128);
-  if (grid.y > 65535) return -5;
-#define SPARK_PATH(T, TAPS) spark_launch_pdl(path_conv_kernel<T, TAPS>, grid, dim3(128), 0, s, dim3(1, 1, 1), *a)
-  if (f32) { if (a->taps == 4) SPARK_PATH(float, 4); else SPARK_PATH(float, 0); }
-  else { if (a->taps == 4) SPARK_PATH(__nv_bfloat16, 4); else SPARK_PATH(__nv_bfloat16, 0); }
+  const int cols = PC_UNITS * (f32 ? 4 : 8), smem = PC_STAGES * (PC_ROWS + PC_FAR + 1) * PC_UNITS * 16 + PC_ROWS * (a->taps == 3 ? 4 : a->taps) * 4;
+  const int tiles = (a->C + cols - 1) / cols, rows = (a->R + PC_ROWS - 1) / PC_ROWS;
+  int dev = 0, sms = 148;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return -4;
+  // channel tiles per CTA: the least of rounds x (tiles + 2 for the start)
+  int per = 1;
+  long long best = 1ll << 60;
+  for (int p = 1; p <= 16 && p <= tiles; ++p) {
+    const long long ctas = static_cast<long long>((tiles + p - 1) / p) * rows, cost = (ctas + PC_PER_SM * sms - 1) / (PC_PER_SM * sms) * (p + 2);
+    if (cost < best) { best = cost; per = p; }
+  }
+  const dim3 grid((tiles + per - 1) / per, rows);
+  if (rows > 65535 || a->taps > 32) return -5;
+#define SPARK_PATH(T, TAPS)                                                                                                     \
+  {                                                                                                                             \
+    if (cudaFuncSetAttribute(path_conv_kernel<T, TAPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -4; \
+    spark_launch_pdl(path_conv_kernel<T, TAPS>, grid, dim3(PC_THREADS), smem, s, dim3(1, 1, 1), *a, per);                        \
+  }
+#define SPARK_PATH_T(T)               \
+  switch (a->taps) {                  \
+    case 1: SPARK_PATH(T, 1) break;   \
+    case 2: SPARK_PATH(T, 2) break;   \
+    case 3: SPARK_PATH(T, 3) break;   \
+    case 4: SPARK_PATH(T, 4) break;   \
+    default: SPARK_PATH(T, 0)         \
+  }
+  if (f32) { SPARK_PATH_T(float) } else { SPARK_PATH_T(__nv_bfloat16) }
+#undef SPARK_PATH_T
 #undef SPARK_PATH
   return spark_launch_rc(__func__);
 }
