@@ -920,6 +920,8 @@ class Model:
         from the segment's first row (always accepted: it is the last sampled token)."""
         plan = self._pending_plan
         assert plan is not None, "commit() without a pending verify"
+        if plan.is_tree and self.page:
+            self._commit_trees(plan, accepted)
         for mix in self.stateful(drafter=False):
             mix.commit(accepted)
             if plan.is_tree and hasattr(mix, "compact"):
@@ -929,6 +931,17 @@ class Model:
             self.seqs[s.slot].length = s.pos0 + len(rows)
         self._pending_plan = None
 
+    def _commit_trees(self, plan: Plan, accepted: List[List[int]]):
+        """The accepted paths' rows of all paged layers at once: cache rows move together, convolution tails advance."""
+        width = max(1, max(len(rows) for rows in accepted))
+        i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=self.device)
+        caches, tails = [], []
+        for _, mix, _ in self.layers:
+            c, t = mix.pending_tree()
+            caches += c
+            tails += t
+        ops.commit_paths(plan.maps, i32([rows + [0] * (width - len(rows)) for rows in accepted]), i32([len(rows) for rows in accepted]), caches, tails)
+
     # -- MTP drafter ------------------------------------------------------------------------
     @torch.no_grad()
     def sparse_ctx_limit(self) -> Optional[int]:
@@ -936,8 +949,8 @@ class Model:
         block; latent attention: top-k pools x pool), or None when no layer selects.  Up to here dense visibility of the
         committed context (what tree-verification rows use) equals what a decode row sees."""
         lim = None
-        if self.cfg.layer_specs:             # their states and pages verify chains only
-            return 0
+        if self.cfg.layer_specs:             # recurrent states and input convolutions verify chains only
+            return None if all(getattr(mix, "takes_trees", False) for _, mix, _ in self.layers) and not self.convs else 0
         for _, mix, _ in self.layers:
             c = getattr(mix, "c", None)
             if isinstance(mix, AttnMixer) and c.sparse_topk_blocks:

@@ -4,7 +4,9 @@ chunks or a window; a sink may enter the denominator, a gate per head may scale 
 
 The cache holds the finished keys and values (heads padded to 16) in pages shared by all slots, or is another layer's
 (`source`).  With convolutions a slot's state is the last `taps - 1` projected rows (`tail`).  Verify rows (`commit=False`) write
-their cache rows in place past the committed length and leave the tail alone; `commit_rows` advances it by the accepted prefix."""
+their cache rows in place past the committed length and leave the tail alone; `commit_rows` advances it by the accepted prefix.  Layers
+with convolutions verify drafted trees too: every node is convolved along its path and written behind the committed tokens in the order
+of the rows, and `Model.commit` moves the accepted path's rows together in all layers at once."""
 from __future__ import annotations
 
 import math
@@ -16,7 +18,7 @@ from ..config import ModelConfig, PagedGqaConfig
 from ..oracle import layers as L
 from .layout import pad
 from .parallel_mixers import PendingRows
-from .plan import Plan
+from .plan import Plan, tree_maps
 
 
 class PagedGqaMixer(PendingRows):
@@ -40,6 +42,12 @@ class PagedGqaMixer(PendingRows):
         if c.slopes:
             self.slopes = torch.tensor([2.0 ** (-8 * (h + 1) / c.n_heads) for h in range(c.n_heads)], dtype=torch.float32, device=device)
 
+    @property
+    def takes_trees(self) -> bool:
+        """Rows are stored by their place in the round, not by their position (norms and rotations go by the position), in a cache of the
+        layer's own."""
+        return bool(self.c.conv_k) and self.source is None and not self.c.gated and max(self.Dp, self.Vp) <= 512
+
     def reset(self, slot: int):
         if self.tail is not None:
             self.tail[slot].zero_()
@@ -52,8 +60,21 @@ class PagedGqaMixer(PendingRows):
 
     def attend(self, proj, plan: Plan, commit: bool, out=None):
         """Heads' outputs [R, heads * padded value width] of the projected rows (into `out` if given)."""
+        if plan.is_tree:
+            assert not commit, "a tree's rows are committed by their accepted path"
+            return self._tree(proj, plan, out)
         o = ops.paged_gqa(self, proj, plan, commit, out)
         return o if o is not None else self._rows(proj, plan, commit, out)
+
+    def _tree(self, proj, plan, out):
+        assert self.takes_trees, "paged attention without convolutions verifies chains"
+        c, w, m = self.c, self.w, tree_maps(plan, self.pages)
+        k, v = self.k.unflatten(2, (c.n_kv_heads, self.Dp)), self.v.unflatten(2, (c.n_kv_heads, self.Vp))
+        q = ops.path_conv(proj, w["conv_t"], self.tail, m, self.nq, k, v)
+        o = ops.tree_attention(q.unflatten(1, (self.H, self.Dp)), k, v, m, c.scale, softcap=c.softcap, bias=w.get("dist_bias"), slopes=self.slopes,
+                               sink=w.get("sink"), window=c.window, chunk=c.chunk, out_scale=self.out_scale,
+                               out=None if out is None else out.unflatten(1, (self.H, self.Vp)))
+        return o.flatten(1) if out is None else out
 
     def commit_rows(self, args, plan, n_rows):
         proj, = args
@@ -137,8 +158,11 @@ class PagedGqaMixer(PendingRows):
             out[sl] = (o * self.out_scale).reshape(s.n, H * V).to(out.dtype)
         return out
 
-    def compact(self, seqs, seg, rows):
-        assert rows == list(range(len(rows))), "paged attention rows verify chains"
+    def pending_tree(self):
+        """(caches, (rows, tail) of the convolutions) that wait for a tree's accepted path; nothing waits any more."""
+        (proj,), _ = self.pending
+        self.pending = None
+        return [self.k, self.v], [(proj, self.tail)]
 
     def state_tensors(self):
         d = {} if self.source is not None else {"k": self.k, "v": self.v}

@@ -34,6 +34,7 @@ class Plan:
     has_media: bool = False                   # some ids are salted media placeholders (outside the vocabulary)
     mm_rows: Optional[list] = None            # multimodal: [(first row, tensor [n, hidden])] written over the embedding
                                               # rows of salted placeholder ids (multimodal/canvas.py)
+    maps: Optional[object] = None             # trees over a paged cache: ops.RowMaps of the rows (`tree_maps`)
 
     @property
     def rows(self) -> int:
@@ -93,3 +94,14 @@ def plan_device_arrays(p: Plan, device) -> dict:
     return {"row_slot": row_slot.to(device), "row_j": row_j.to(device), "row_r0": row_r0.to(device),
             "row_pos0": row_pos0.to(device), "seg": seg.to(device), "pos32": p.pos.to(torch.int32),
             "ids32": p.ids.to(torch.int32)}
+
+
+def tree_maps(p: Plan, tables: torch.Tensor):
+    """Maps of the plan's rows over the page table `tables`, made once for all layers: trees as they are, other segments as chains."""
+    if p.maps is None:
+        from .. import ops
+        i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=tables.device)
+        parents = [q for s in p.segs for q in (s.parents if s.parents is not None else range(-1, s.n - 1))]
+        p.maps = ops.slot_maps(i32([s.pos0 for s in p.segs]), i32([s.n for s in p.segs]), tables, p.rows, slots=i32([s.slot for s in p.segs]),
+                               parents=i32(parents), nodes=max(s.n for s in p.segs))
+    return p.maps

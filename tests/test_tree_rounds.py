@@ -1,0 +1,125 @@
+"""Drafted trees over paged caches in whole models: every node's logits are those of its path, accepted paths are committed, speculative rounds
+are lossless (CPU; on a B200 in bf16 and 32-bit)."""
+import debisun_util as U
+import pytest
+import torch
+
+from spark_engine_b200.models.plan import make_plan
+from spark_engine_b200.spec.decoder import SpecDecoder
+from spark_engine_b200.spec.tree import Node
+
+CONFIGS = {
+    "mixed layers": U.MIXED,
+    "dense": dict(layers=[U.layer(U.dense()), U.layer(U.dense(), heads=8, kv_heads=2, dim=64, vdim=32, conv=2, chunk=64)]),
+    "one tap": dict(layers=[U.layer(U.dense(), conv=1, chunk=1000), U.layer(conv=7)]),
+}
+TREE = [-1, 0, 0, 1, 1, 2, 3, 6, 4, -1, 9, 5]          # the last sampled token, drafts below it, and one more root with a draft of its own
+
+
+def setup(name):
+    cfg = U.config(**CONFIGS[name])
+    return cfg, U.tensors(cfg)
+
+
+def path(parents, j):
+    line = []
+    while j >= 0:
+        line.append(j)
+        j = parents[j]
+    return line[::-1]
+
+
+def check_nodes_and_commits(name, device, dtype, agree):
+    cfg, T = setup(name)
+    g = torch.Generator().manual_seed(3)
+    tok = lambda n: torch.randint(0, cfg["vocab"], (n,), generator=g).tolist()
+    m = U.framework(cfg, T, device, dtype)
+    assert m.sparse_ctx_limit() is None
+    prompts = {2: tok(61), 0: tok(130)}
+    for slot, p in prompts.items():
+        m.forward(make_plan([(slot, p, 0)], device=device, all_logits=False))
+    said = dict(prompts)
+    for rnd, accepted in enumerate((([0, 1, 3, 6], [0]), ([0, 2, 5, 11], [0, 1, 4, 8]), ([9, 10], []))):
+        trees = [tok(len(TREE)), tok(9)]
+        plan = make_plan([(s, t, len(said[s])) for s, t in zip(said, trees)], device=device, parents=[TREE, TREE[:9]])
+        got = m.forward(plan, commit=False).float().cpu()
+        for seg, t, par in zip(plan.segs, trees, (TREE, TREE[:9])):
+            for j in range(rnd % 2, seg.n, 2):
+                line = path(par, j)
+                want = U.oracle_logits(cfg, T, said[seg.slot] + [t[i] for i in line])[-1]
+                agree(got[seg.r0 + j: seg.r0 + j + 1], want.unsqueeze(0), cfg)
+        m.commit([list(a) for a in accepted])
+        for s, t, a in zip(list(said), trees, accepted):
+            said[s] = said[s] + [t[j] for j in a]
+        assert [m.seqs[s].length for s in said] == [len(x) for x in said.values()]
+    # what was committed is what a chain would have left: rows of both sequences go on behind it, and a chain's rows are verified again
+    nxt = {s: tok(3) for s in said}
+    plan = make_plan([(s, nxt[s], len(said[s])) for s in said], device=device)
+    got = m.forward(plan, commit=False).float().cpu()
+    for seg in plan.segs:
+        agree(got[seg.r0: seg.r0 + 3], U.oracle_logits(cfg, T, said[seg.slot] + nxt[seg.slot])[-3:], cfg)
+    m.commit([[0, 1], [0]])
+
+
+def check_rounds(name, device, dtype):
+    """Rounds over trees emit what plain greedy decoding of the same model does, in fewer rounds."""
+    cfg, T = setup(name)
+    prompt = U.prompt(70, cfg["vocab"])
+    ref = SpecDecoder(U.framework(cfg, T, device, dtype), lambda s, d: ([], []), depth=0).generate([prompt], 16)[0]
+    m = U.framework(cfg, T, device, dtype)
+    sd = SpecDecoder(m, lambda s, d: ([], []), depth=0)
+    seq = sd.start(1, prompt)
+    rounds = 0
+    while len(seq.generated) < 16:
+        n = len(seq.generated)
+        nodes, parent = [], -1
+        for t in ref[n: n + 4]:                          # a wrong draft in front of every right one, and one below it
+            nodes.append(Node(parent, (t + 1) % cfg["vocab"]))
+            nodes.append(Node(parent, t))
+            nodes.append(Node(len(nodes) - 2, t))
+            parent = len(nodes) - 2
+        sd.round_tree([seq], [nodes], budgets=[16 - n])
+        rounds += 1
+    return ref, seq, rounds
+
+
+def close(got, want, cfg):
+    assert U.error(got, want) < 3e-5
+
+
+@pytest.mark.parametrize("name", list(CONFIGS))
+def test_nodes_see_their_paths(name):
+    check_nodes_and_commits(name, "cpu", torch.float32, close)
+
+
+@pytest.mark.parametrize("name", list(CONFIGS))
+def test_tree_rounds_are_lossless(name):
+    ref, seq, rounds = check_rounds(name, "cpu", torch.float32)
+    assert seq.generated[:16] == ref and rounds <= 5 and seq.accepted >= 10
+
+
+def test_models_with_other_layers_verify_chains():
+    import zapolorn_util as Z
+    cfg = Z.config(**Z.MIXED) if not isinstance(Z.MIXED, list) else Z.config(Z.MIXED)
+    assert Z.framework(cfg, Z.tensors(cfg)).sparse_ctx_limit() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("name", list(CONFIGS))
+def test_nodes_see_their_paths_on_the_device(name, dtype):
+    """bf16 of models with experts: rows whose choice of experts is close may differ by an expert (see test_debisun_gpu); the dense ones are held."""
+    def agree(got, want, cfg):
+        if dtype == torch.float32:
+            assert U.error(got, want) < 3e-5
+        elif name != "mixed layers":
+            assert U.error(got, want) < 3e-2 * len(cfg["layers"]) ** 0.5
+        assert torch.isfinite(got).all()
+    check_nodes_and_commits(name, "cuda", dtype, agree)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", list(CONFIGS))
+def test_tree_rounds_are_lossless_on_the_device(name):
+    ref, seq, rounds = check_rounds(name, "cuda", torch.float32)
+    assert seq.generated[:16] == ref and rounds <= 5 and seq.accepted >= 10
