@@ -241,6 +241,8 @@ Tensor tree_attention(Tensor q, const Tensor& k, const Tensor& v, const RowMaps&
   // 49.4 / 48.5; eight windows of 1024, heads of 128 with slopes: 37.2 / 32.1 / 31.7 / 31.5 / 34.6; ragged, soft cap and bias, whose pages take
   // longer: 45.6 / 41.5 / 45.0 / 45.1 / 52.0)
   const int extra = !tc ? 0 : wide ? 10 : softcap > 0 || bias || slopes ? 4 : 6;
+  const int64_t work = G * (R * (H / G) / bm + S) * (m.tables.size(1) + extra);
+  NEED(work < 1ll << 31, "a round of ", R, " rows over tables of ", m.tables.size(1), " pages is more than one call takes");
   const int64_t no = static_cast<int64_t>(ctas) * 2 * bm * V, nm = static_cast<int64_t>(ctas) * 2 * bm * 2;
   Tensor ws = at::empty({no + nm + ctas * 4}, q.options().dtype(at::kFloat));
   float* part = static_cast<float*>(ws.data_ptr());
@@ -251,7 +253,12 @@ Tensor tree_attention(Tensor q, const Tensor& k, const Tensor& v, const RowMaps&
   a.S = i(S); a.R = i(R); a.words = m.anc ? i(m.anc->size(1)) : 0; a.page_ld = i(m.tables.size(1)); a.n_slots = i(m.tables.size(0)); a.n_pages = i(k.size(0));
   a.H = i(H); a.G = i(G); a.D = i(D); a.V = i(V); a.ldq = i(q.stride(0)); a.hq = i(q.stride(1)); a.ldo = i(out.stride(0)); a.ho = i(out.stride(1));
   a.ldg = gate ? i(gate->stride(0)) : 0; a.bias_n = bias ? i(bias->size(1)) : 0; a.window = i(window); a.chunk = i(chunk);
-  a.bm = bm; a.sms = on.dev.sms; a.ctas = ctas; a.min_tiles = 1; a.extra = extra; a.zero_rest = !given;
+  if (chunk) {
+    a.chunk_shift = 31;
+    while (1ll << (a.chunk_shift - 31) < chunk) ++a.chunk_shift;
+    a.chunk_mul = static_cast<unsigned>(((static_cast<unsigned __int128>(1) << a.chunk_shift) + chunk - 1) / chunk);
+  }
+  a.bm_log = bm == 32 ? 5 : bm == 128 ? 7 : 8; a.sms = on.dev.sms; a.ctas = ctas; a.min_tiles = 1; a.extra = extra; a.zero_rest = !given;
   a.scale = static_cast<float>(scale); a.cap = static_cast<float>(softcap); a.out_scale = static_cast<float>(out_scale);
   on.launch(e_attn, &a, static_cast<int>(dt == at::kFloat), static_cast<int>(tc));
   return out;

@@ -18,7 +18,7 @@ template <typename T, int VC>
 __global__ void __launch_bounds__(TT_THREADS)
 tree_tile_kernel(const __grid_constant__ TreeAttn a) {
   extern __shared__ __align__(16) float smem_tt[];
-  __shared__ long long sh[TT_THREADS / 32 + 2];
+  __shared__ TreeItem s_item;
   __shared__ float s_m[TT_BM], s_l[TT_BM], s_f[TT_BM];
   __shared__ int s_pos[TT_BM], s_first[TT_BM], s_at[TA_PAGE];
   const int D = a.D, V = a.V, LDQ = (D + 63) / 64 * 64 + 4, rep = a.H / a.G;
@@ -29,12 +29,21 @@ tree_tile_kernel(const __grid_constant__ TreeAttn a) {
   const int t = threadIdx.x, ty = t >> 4, tx = t & 15;
   pdl_wait();
   pdl_trigger();
-  TreeRange range = ta_range<TT_THREADS>(a, sh);
+  TreeRange range;
+  if (t < 32) range = ta_range(a);
   if (t == 0) ta_set_split(a, make_int4(0, 0, 0, 0));
-  TreeItem it;
-  while (ta_next(a, range, it)) {
-    const TreeSeg& sg = it.seg;
-    const int slot = a.slots ? a.slots[it.s] : it.s, pairs = min(TT_BM, sg.n * rep - it.rt * TT_BM);
+#pragma unroll 1
+  while (true) {
+    if (t < 32) {
+      TreeItem next;
+      ta_next(a, range, next);
+      if (t == 0) s_item = next;
+    }
+    __syncthreads();
+    const TreeItem it = s_item;
+    if (it.nj == 0) break;
+    const TreeItem& sg = it;
+    const int slot = it.slot, pairs = min(TT_BM, sg.n * rep - it.rt * TT_BM);
     __syncthreads();
     for (int i = t; i < TT_BM * (LDQ / 4); i += TT_THREADS) {
       const int row = i / (LDQ / 4), c = (i - row * (LDQ / 4)) * 4, f = it.rt * TT_BM + row;
@@ -207,7 +216,7 @@ constexpr int TM_THREADS = 256, TM_WARPS = TM_THREADS / 32, TM_MAX_CTAS = 1024;
 template <typename T, int VC>                                // VC: 128-column pieces of a row
 __global__ void __launch_bounds__(TM_THREADS)
 tree_merge_kernel(const __grid_constant__ TreeAttn a) {
-  __shared__ long long sh[TM_WARPS + 2];
+  __shared__ int sh[TM_WARPS];
   __shared__ int s_first[TM_MAX_CTAS + 1];                   // rows of the items in front of CTA c's
   __shared__ float4 s_o[TM_WARPS][32 * VC];
   __shared__ float s_ml[TM_WARPS][2];
@@ -234,14 +243,13 @@ tree_merge_kernel(const __grid_constant__ TreeAttn a) {
     }
     mine += n[i];
   }
-  long long total;
-  int before = static_cast<int>(ta_prefix<TM_THREADS>(mine, sh, total));
+  int rows;
+  int before = ta_prefix<TM_THREADS>(mine, sh, rows);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if (i < each && t * each + i < a.ctas) s_first[t * each + i] = before;
     before += n[i];
   }
-  const int rows = static_cast<int>(total);
   if (t == 0) s_first[a.ctas] = rows;
   __syncthreads();
   int wpr = TM_WARPS;
@@ -256,7 +264,7 @@ tree_merge_kernel(const __grid_constant__ TreeAttn a) {
     const int4 sp = s_split[c];
     const int parts = on ? sp.x & 0xffff : 0;
     // part 0 lies behind the others' in its CTA's pair, see TreeAttn
-    auto part = [&](int i) { return (static_cast<size_t>(c + i) * 2 + (i == 0 ? 1 : 0)) * a.bm + row; };
+    auto part = [&](int i) { return ((static_cast<size_t>(c + i) * 2 + (i == 0 ? 1 : 0)) << a.bm_log) + row; };
     float m = -INFINITY, l = 0.f;
     float4 o[VC] = {};
     for (int i0 = sub; i0 < parts; i0 += 4 * wpr) {          // four parts in flight
@@ -355,12 +363,12 @@ int launch_tree_tc(const TreeAttn& a, cudaStream_t s);       // tree_attn_tc.cu
 
 using namespace spark;
 
-// tc: the tensor-core kernel (bf16, head widths of up to 256; bm 128 or 256), else the FP32 units (bm 32).
+// tc: the tensor-core kernel (bf16, head widths of up to 256; tiles of 128 or 256 rows), else the FP32 units (tiles of 32).
 extern "C" int spark_tree_attn(const TreeAttn* a, int f32, int tc, cudaStream_t s) {
   if (a->S <= 0 || a->R <= 0) return 0;
   if (a->H <= 0 || a->G <= 0 || a->H % a->G || a->D <= 0 || a->V <= 0 || ((a->D | a->V) & 7) || a->D > 512 || a->V > 512 || a->ctas <= 0 || a->ctas > TM_MAX_CTAS || a->sms <= 0 ||
       a->min_tiles <= 0 || (a->bias && a->bias_n <= 0) || a->page_ld <= 0 || ((a->ldq | a->hq | a->ldo | a->ho) & 3)) return -5;
-  if (tc ? f32 || (a->bm != 128 && a->bm != 256) : a->bm != TT_BM) return -5;
+  if (tc ? f32 || (a->bm_log != 7 && a->bm_log != 8) : 1 << a->bm_log != TT_BM) return -5;
   if (const int rc = tc ? launch_tree_tc(*a, s) : f32 ? launch_tiles<float>(*a, s) : launch_tiles<__nv_bfloat16>(*a, s)) return rc;
   // (narrow rows: more CTAs to an SM)
   const dim3 grid((a->V <= 128 ? 4 : 2) * a->sms);

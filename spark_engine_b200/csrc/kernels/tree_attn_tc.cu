@@ -1,5 +1,6 @@
 // Tree attention on tcgen05 (bf16 caches): the tiles of tree_attn.cu with 128 (node, head) rows per accumulator, a page of keys per step.
-//   warp 0      TMA: pages of keys and values into a ring of slots in the order the products use them (K0 K1 V0 K2 V1 ..)
+//   warp 0      finds this CTA's items and announces them; TMA: pages of keys and values into a ring of slots in the order the products use
+//               them (K0 K1 V0 K2 V1 ..)
 //   warp 1      issues S = Q K^T one page ahead of O += P V (P in tensor memory): as soon as the softmax warps have loaded a page's scores
 //   the others  softmax, one row per thread: 64 scores are one tensor-memory load, statistics stay in the thread
 // NQ = 2: two tiles of 128 rows with their own issuing and softmax warps share the keys in shared memory (large trees: a page is read once for
@@ -22,21 +23,33 @@ namespace spark {
 int make_tmap_page(CUtensorMap* m, const void* base, uint64_t pages, uint64_t G, uint64_t D, uint64_t tok, uint64_t page);
 
 constexpr float TC_MOST = 1099511627776.f;                   // 2^40
+// Items announced at a time: an item has two slots of the ring at least, so that the one whose place is taken again has been read long ago.
+constexpr int TC_ITEMS = 16;
 
 template <int DC, int NQ> struct Tc {
   static constexpr bool QT = DC == 256;                      // queries in tensor memory: shared memory has no room for them beside the ring
   static constexpr int SLOT = TA_PAGE * DC * 2, Q_BYTES = QT ? 0 : 128 * DC * 2;
-  static constexpr int SLOTS = DC == 256 ? 5 : DC == 128 ? (NQ == 2 ? 9 : 4) : (NQ == 2 ? 16 : 8);
-  static constexpr int STAGE = QT ? 32768 : Q_BYTES;         // of a tile's results on their way out, over its queries where those are there
-  static constexpr int SMEM = NQ * STAGE + SLOTS * SLOT + 1024 + 1024;
+  static constexpr int SLOTS = DC == 256 ? 6 : DC == 128 ? (NQ == 2 ? 9 : 4) : (NQ == 2 ? 16 : 8);
+  static constexpr int SMEM = NQ * Q_BYTES + SLOTS * SLOT + 1024 + 1024;
   static constexpr bool TWO = NQ == 1;
   // per tile: scores, weights (high and low terms of 32 columns each, or two places for high ones), the accumulator
   static constexpr int TILE_COLS = 128 + DC, Q_COL = 128 + DC;
   static constexpr int COLS = QT || NQ == 2 ? 512 : 256;
   static constexpr int SOFTMAX = 1 + NQ, WARPS = SOFTMAX + 4 * NQ, THREADS = WARPS * 32, PER_SM = QT || NQ == 2 ? 1 : 2;
+  static_assert(2 * TC_ITEMS > SLOTS, "an item's place");
   static_assert(NQ * TILE_COLS + (QT ? DC / 2 : 0) <= COLS && SMEM <= 232448, "tensor memory, shared memory");
 };
 
+__device__ __forceinline__ uint32_t tc_ld1(uint32_t taddr) {
+  uint32_t r;
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr) : "memory");
+  tmem_ld_wait();
+  return r;
+}
+__device__ __forceinline__ void tc_st1(uint32_t taddr, uint32_t v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(taddr), "r"(v) : "memory");
+  tmem_st_wait();
+}
 __device__ __forceinline__ void tc_load_page(void* dst, const CUtensorMap* m, uint64_t* bar, int c, int head, int page) {
   asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
                ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(c), "r"(head), "r"(0), "r"(page) : "memory");
@@ -53,6 +66,11 @@ __device__ __forceinline__ uint64_t tc_desc_nmajor(uint32_t addr, uint32_t chunk
 __device__ __forceinline__ float tc_ex2(float x) {          // relative error 2^-22, results below 2^-126 are 0
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float tc_rcp(float x) {          // relative error 2^-23
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 // two fp32 at a time
@@ -74,11 +92,24 @@ __device__ __forceinline__ uint64_t tc_mul2(uint64_t a, uint64_t b) {
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
+// A wait that ends: each try may suspend the thread for 20 us, a hundred thousand of them are two seconds.
+__device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity) {
+  uint32_t ok = 0;
+#pragma unroll 1
+  for (int i = 0; i < 100000 && !ok; ++i)
+    asm volatile(
+        "{\n"
+        ".reg .pred P;\n"
+        "mbarrier.try_wait.parity.shared::cta.b64 P, [%1], %2, 20000;\n"
+        "selp.u32 %0, 1, 0, P;\n"
+        "}\n" : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+  return __all_sync(0xffffffffu, ok);
+}
 // All softmax warps of the item (4 or 8): a barrier whose wait ends.
 __device__ __forceinline__ bool tc_sync(uint64_t* bar, uint32_t& phase) {
   __syncwarp();
   if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
-  const bool ok = __all_sync(0xffffffffu, mbar_wait(bar, phase));
+  const bool ok = tc_wait(bar, phase);
   phase ^= 1u;
   return ok;
 }
@@ -87,7 +118,7 @@ struct TcCount { int slot = 0; uint32_t ph = 0; };
 template <int N> __device__ __forceinline__ void tc_step(TcCount& c) { if (++c.slot == N) { c.slot = 0; c.ph ^= 1; } }
 
 // Bits b .. b + 63 of a row's ancestors.
-__device__ __forceinline__ uint64_t tc_ancestors(const TreeAttn& a, const TreeSeg& sg, int node, int b) {
+__device__ __forceinline__ uint64_t tc_ancestors(const TreeAttn& a, const TreeItem& sg, int node, int b) {
   if (a.anc) {
     const uint32_t* w = a.anc + static_cast<size_t>(sg.r0 + node) * a.words;
     const int k = b >> 5, sh = b & 31;
@@ -99,7 +130,7 @@ __device__ __forceinline__ uint64_t tc_ancestors(const TreeAttn& a, const TreeSe
   return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1;
 }
 // Which of the 64 tokens from tok0 on row `node` (position p) sees; near: its ancestors 0 .. 63.
-__device__ __forceinline__ uint64_t tc_mask(const TreeAttn& a, const TreeSeg& sg, int tok0, int node, int p, uint64_t near) {
+__device__ __forceinline__ uint64_t tc_mask(const TreeAttn& a, const TreeItem& sg, int tok0, int node, int p, uint64_t near) {
   const int first = ta_first_visible(a, p), i0 = tok0 - sg.len;        // the page's token 0 is node i0
   const int lo = min(max(first - tok0, 0), 64), hi = min(max(-i0, 0), 64);
   uint64_t m = hi > lo ? (hi == 64 ? ~0ull : (1ull << hi) - 1) & ~(lo == 0 ? 0ull : (1ull << lo) - 1) : 0ull;
@@ -121,10 +152,10 @@ template <int DC, int NQ, bool FEAT>
 __global__ void __launch_bounds__(Tc<DC, NQ>::THREADS, Tc<DC, NQ>::PER_SM)
 tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ TreeAttn a) {
   using L = Tc<DC, NQ>;
-  constexpr int SLOT = L::SLOT, SLOTS = L::SLOTS, KV_CHUNK = TA_PAGE * 128, Q_CHUNK = 128 * 128, NT = L::THREADS;
+  constexpr int SLOT = L::SLOT, SLOTS = L::SLOTS, KV_CHUNK = TA_PAGE * 128, Q_CHUNK = 128 * 128;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* ring = smem + NQ * L::STAGE;
+  uint8_t* ring = smem + NQ * L::Q_BYTES;
   uint64_t* full = reinterpret_cast<uint64_t*>(ring + SLOTS * SLOT);
   uint64_t* empty = full + SLOTS;
   uint64_t* q_full = empty + SLOTS;                          // [NQ]
@@ -134,8 +165,9 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
   uint64_t* o_full = p_full + 2 * NQ;                        // ([NQ][2] like p_full)
   uint64_t* v_seen = o_full + 2 * NQ;                        // warp 1 has looked over a masked page's values
   uint64_t* v_sync = v_seen + NQ;                            // [NQ]: of 4 and of 8 softmax warps
-  long long* sh = reinterpret_cast<long long*>(v_sync + NQ); // [NT / 32 + 2]
-  uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(sh + NT / 32 + 2);
+  uint64_t* item_full = v_sync + NQ;                         // [TC_ITEMS]
+  TreeItem* items = reinterpret_cast<TreeItem*>((reinterpret_cast<uintptr_t>(item_full + TC_ITEMS) + 15) & ~uintptr_t(15));     // [TC_ITEMS]
+  uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(items + TC_ITEMS);
   uint32_t* odd_rows = tmem_ptr + 1;                         // [SLOTS][2]: tokens of a masked page with a value that is not finite
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -146,6 +178,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       mbar_init(&v_seen[s], 1); mbar_init(&v_sync[s], 4 * (s + 1));
     }
     for (int s = 0; s < 2 * NQ; ++s) { mbar_init(&p_full[s], 4); mbar_init(&o_full[s], 1); }
+    for (int s = 0; s < TC_ITEMS; ++s) mbar_init(&item_full[s], 1);
     fence_barrier_init();
   }
   if (warp == 1) { tmem_alloc<L::COLS>(tmem_ptr); tmem_relinquish(); }
@@ -155,37 +188,53 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
   const uint32_t tmem = *tmem_ptr;
   pdl_wait();
   pdl_trigger();
-  TreeRange range = ta_range<NT>(a, sh);
   if (threadIdx.x == L::SOFTMAX * 32) ta_set_split(a, make_int4(0, 0, 0, 0));
   const int rep = a.H / a.G;
-  TreeItem it;
   bool ok = true;
+  int why = ST_OK;                                           // what a wait that ran out waited for
   const auto place = [](int n) { return L::TWO ? 0 : n & 1; };         // barrier and phase of page n's weights
+  const auto announced = [&](int k, TreeItem& it) {                     // item k of this CTA; nj = 0: there is none, or the wait for it ran out
+    const bool there = tc_wait(&item_full[k % TC_ITEMS], (k / TC_ITEMS) & 1);
+    it = items[k % TC_ITEMS];
+    if (!there) { why = ST_TIMEOUT_MBAR_FULL; it.nj = 0; }
+    return it.nj > 0;
+  };
   const auto phase = [](int n) { return static_cast<uint32_t>(L::TWO ? n & 1 : (n >> 1) & 1); };
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
     TcCount c;
     const int kch = (a.D + 63) / 64, vch = (a.V + 63) / 64;
-    while (ok && ta_next(a, range, it)) {
-      const int slot = a.slots ? a.slots[it.s] : it.s;
+    TreeRange range = ta_range(a);
+#pragma unroll 1
+    for (int k = 0; ok; ++k) {
+      TreeItem it;
+      ta_next(a, range, it);
+      if (lane == 0) {
+        items[k % TC_ITEMS] = it;
+        mbar_arrive(&item_full[k % TC_ITEMS]);
+      }
+      if (it.nj == 0) break;
+      const int slot = it.slot;
       int page = 0, page_v = 0;                              // of tile (lane) of the current 32: keys run one tile ahead of values
+#pragma unroll 1
       for (int i = 0; i < 2 * it.nj; ++i) {
         const bool is_v = i == 2 * it.nj - 1 || (i >= 2 && !(i & 1));
         const int j = i == 0 ? 0 : i == 2 * it.nj - 1 ? it.nj - 1 : is_v ? i / 2 - 1 : (i + 1) / 2;
         if ((j & 31) == 0) {
           int p = j + lane < it.nj ? ta_page(a, slot, it.j + j + lane) : 0;
           if (p < 0) {
-            if (!is_v) set_status(a.status, ST_BOUNDS, it.seg.r0, (it.j + j + lane) * TA_PAGE, slot);
+            if (!is_v) set_status(a.status, ST_BOUNDS, it.r0, (it.j + j + lane) * TA_PAGE, slot);
             p = 0;                                           // some page: its tokens are masked
           }
           if (is_v) page_v = p; else page = p;
         }
-        ok = __all_sync(0xffffffffu, mbar_wait(&empty[c.slot], c.ph ^ 1));
-        if (!ok) { set_status(a.status, ST_TIMEOUT_MBAR_EMPTY, blockIdx.x, it.s, i); break; }
+        ok = tc_wait(&empty[c.slot], c.ph ^ 1);
+        if (!ok) { why = ST_TIMEOUT_MBAR_EMPTY; break; }
         const int pg = __shfl_sync(0xffffffffu, is_v ? page_v : page, j & 31), ch = is_v ? vch : kch;
         if (lane == 0) {
           mbar_arrive_expect_tx(&full[c.slot], ch * KV_CHUNK);
+#pragma unroll 1
           for (int x = 0; x < ch; ++x) tc_load_page(ring + c.slot * SLOT + x * KV_CHUNK, is_v ? &tmV : &tmK, &full[c.slot], x * 64, it.g, pg);
         }
         __syncwarp();
@@ -196,31 +245,34 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     // ------------------------------------------------------------ MMA issuer of tile q (the whole warp walks, one elected lane issues)
     const int q = warp - 1, ksteps = (a.D + 15) / 16, vn = (a.V + 15) / 16 * 16, vunits = (a.V + 63) / 64 * 8;
     const uint32_t id_s = make_idesc(1, 1, 128, TA_PAGE), id_o = make_idesc(1, 1, 128, vn) | (1u << 16);
-    const uint32_t qs = __shfl_sync(0xffffffffu, smem_u32(smem), 0) + q * L::STAGE, rs = __shfl_sync(0xffffffffu, smem_u32(ring), 0);
+    const uint32_t qs = __shfl_sync(0xffffffffu, smem_u32(smem), 0) + q * L::Q_BYTES, rs = __shfl_sync(0xffffffffu, smem_u32(ring), 0);
     const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0) + q * L::TILE_COLS;
     TcCount c;
-    int n = 0, items = 0;                                    // pages and items of the tile so far
-    while (ok && ta_next(a, range, it)) {
-      const int pairs = it.seg.n * rep - it.rt * a.bm, act = NQ == 2 && pairs > 128 ? 2 : 1;
-      const int slot = a.slots ? a.slots[it.s] : it.s, edge = ta_first_visible(a, it.seg.len + it.seg.n - 1);
+    int n = 0, own = 0;                                      // pages and items of the tile so far
+    TreeItem it;
+#pragma unroll 1
+    for (int k = 0; ok && announced(k, it); ++k) {
+      const int pairs = it.n * rep - (it.rt << a.bm_log), act = NQ == 2 && pairs > 128 ? 2 : 1;
       if (q >= act) {                                        // no rows here: the slots are passed on
+#pragma unroll 1
         for (int i = 0; i < 2 * it.nj; ++i) {
-          ok = __all_sync(0xffffffffu, mbar_wait(&full[c.slot], c.ph));
-          if (!ok) { set_status(a.status, ST_TIMEOUT_MBAR_FULL, blockIdx.x, it.s, i); break; }
+          ok = tc_wait(&full[c.slot], c.ph);
+          if (!ok) { why = ST_TIMEOUT_MBAR_FULL; break; }
           if (lane == 0) mbar_arrive(&empty[c.slot]);
           tc_step<SLOTS>(c);
         }
         continue;
       }
       uint32_t there = 0u;                                   // pages of the current 32 that the table leads to
-      ok = __all_sync(0xffffffffu, mbar_wait(&q_full[q], items & 1));
-      if (!ok) { set_status(a.status, ST_TIMEOUT_MBAR_FULL, blockIdx.x, it.s, -2); break; }
-      ++items;
+      ok = tc_wait(&q_full[q], own & 1);
+      if (!ok) { why = ST_TIMEOUT_MBAR_FULL; break; }
+      ++own;
+#pragma unroll 1
       for (int j = -1; j < it.nj; ++j) {
         if (j + 1 < it.nj) {
           const int t = n + j + 1;
-          ok = __all_sync(0xffffffffu, mbar_wait(&full[c.slot], c.ph) && (t == 0 || mbar_wait(&s_read[q], (t - 1) & 1)));
-          if (!ok) { set_status(a.status, ST_TIMEOUT_MBAR_FULL, blockIdx.x, it.s, j); break; }
+          ok = tc_wait(&full[c.slot], c.ph) && (t == 0 || tc_wait(&s_read[q], (t - 1) & 1));
+          if (!ok) { why = ST_TIMEOUT_MBAR_FULL; break; }
           tc_fence_after();
           if (elect_one()) {
             const uint64_t kd = make_smem_desc_sw128(rs + c.slot * SLOT), qd = make_smem_desc_sw128(qs);
@@ -239,18 +291,18 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         }
         if (j < 0) continue;
         const int tok0 = (it.j + j) * TA_PAGE;
-        if ((j & 31) == 0) there = __ballot_sync(0xffffffffu, j + lane < it.nj && ta_page(a, slot, it.j + j + lane) >= 0);
-        ok = __all_sync(0xffffffffu, mbar_wait(&full[c.slot], c.ph));
-        if (q == 0 && ok && (tok0 + TA_PAGE > it.seg.len || tok0 < edge || !((there >> (j & 31)) & 1u))) {
+        if ((j & 31) == 0) there = __ballot_sync(0xffffffffu, j + lane < it.nj && ta_page(a, it.slot, it.j + j + lane) >= 0);
+        ok = tc_wait(&full[c.slot], c.ph);
+        if (q == 0 && ok && (tok0 + TA_PAGE > it.len || tok0 < it.edge || !((there >> (j & 31)) & 1u))) {
           // ---- a masked page's values: tokens that are not the request's are zeroed, the others with a value that is not finite noted
-          const int valid = (there >> (j & 31)) & 1u ? min(TA_PAGE, it.seg.len + it.seg.n - tok0) : 0;
+          const int valid = (there >> (j & 31)) & 1u ? min(TA_PAGE, it.len + it.n - tok0) : 0;
           uint32_t odd[2];
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             const int tok = half * 32 + lane;
             uint8_t* vrow = ring + c.slot * SLOT + tok * 128;
             uint32_t most = 0u;                              // largest exponents of the row's even and odd columns
-#pragma unroll 8
+#pragma unroll 4
             for (int u = 0; u < vunits; ++u) {
               uint4* x = reinterpret_cast<uint4*>(vrow + (u >> 3) * KV_CHUNK + (((u & 7) ^ (tok & 7)) * 16));
               if (tok >= valid) *x = make_uint4(0u, 0u, 0u, 0u);
@@ -268,8 +320,8 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
             for (int i = 0; i < act; ++i) mbar_arrive(&v_seen[i]);
           }
         }
-        ok = ok && __all_sync(0xffffffffu, mbar_wait(&p_full[q * 2 + place(n + j)], phase(n + j)));
-        if (!ok) { set_status(a.status, ST_TIMEOUT_MBAR_FULL, blockIdx.x, it.s, j); break; }
+        ok = ok && tc_wait(&p_full[q * 2 + place(n + j)], phase(n + j));
+        if (!ok) { why = ST_TIMEOUT_MBAR_FULL; break; }
         tc_fence_after();
         if (elect_one()) {
           const uint64_t vd = tc_desc_nmajor(rs + c.slot * SLOT, KV_CHUNK);
@@ -294,9 +346,11 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     const int vn = (a.V + 15) / 16 * 16, vn_units = (a.V + 63) / 64 * 8;
     uint32_t sync_phase[NQ] = {}, seen_phase = 0u;
     int n = 0, seq = 0;                                      // pages of this tile so far; position of the item in the ring's sequence
-    while (ok && ta_next(a, range, it)) {
-      const TreeSeg& sg = it.seg;
-      const int all = sg.n * rep - it.rt * a.bm, pairs = min(128, all - q * 128);        // rows of this tile
+    TreeItem sg;
+#pragma unroll 1
+    for (int i = 0; ok && announced(i, sg); ++i) {
+      const TreeItem& it = sg;
+      const int all = sg.n * rep - (it.rt << a.bm_log), pairs = min(128, all - q * 128);        // rows of this tile
       const int seq0 = seq;
       seq += 2 * it.nj;
       if (it.first && !it.last && threadIdx.x == L::SOFTMAX * 32) ta_set_split(a, ta_split(a, it));
@@ -304,9 +358,9 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       const bool both = NQ == 2 && all > 128;
       uint64_t* sync = &v_sync[both ? NQ - 1 : 0];
       uint32_t& sync_ph = sync_phase[both ? NQ - 1 : 0];
-      const int f = it.rt * a.bm + q * 128 + min(row, pairs - 1), node = f / rep, h = it.g * rep + f - node * rep, pr = sg.r0 + node;
+      const int f = (it.rt << a.bm_log) + q * 128 + min(row, pairs - 1), node = f / rep, h = it.g * rep + f - node * rep, pr = sg.r0 + node;
       const bool idle = quad * 32 >= pairs;                  // a warp without rows keeps the pace and computes nothing
-      const int p = a.pos[pr], slot = a.slots ? a.slots[it.s] : it.s;
+      const int p = a.pos[pr];
       const uint64_t near = tc_ancestors(a, sg, node, 0);    // (asked for long before the tree's page)
       {                                                      // the row's query; columns from D on are zero
         const uint4* src = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) + static_cast<size_t>(pr) * a.ldq + static_cast<size_t>(h) * a.hq);
@@ -325,7 +379,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
 #pragma unroll 8
           for (int u = 0; u < DC / 8; ++u) {
             const uint4 v = u < units ? __ldg(src + u) : make_uint4(0u, 0u, 0u, 0u);
-            *reinterpret_cast<uint4*>(smem + q * L::STAGE + (u >> 3) * Q_CHUNK + row * 128 + (((u & 7) ^ (row & 7)) * 16)) = v;
+            *reinterpret_cast<uint4*>(smem + q * L::Q_BYTES + (u >> 3) * Q_CHUNK + row * 128 + (((u & 7) ^ (row & 7)) * 16)) = v;
           }
         }
         uint32_t z[32];
@@ -341,30 +395,30 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       bool fresh = true;                                     // some row of the warp has no reference yet
       float ref = -INFINITY, l = 0.f;                        // of the exponentials (FEAT: natural, else log2), and their sum
       const float c1 = FEAT ? 1.f : a.scale * TA_LOG2E;
-      const int edge = ta_first_visible(a, sg.len + sg.n - 1);         // from here on every row sees committed tokens
       uint32_t there = 0u;                                   // pages of the current 32 that the table leads to
+#pragma unroll 1
       for (int j = 0; j < it.nj; ++j, ++n) {
         const int tok0 = (it.j + j) * TA_PAGE;
-        if ((j & 31) == 0) there = __ballot_sync(0xffffffffu, j + lane < it.nj && ta_page(a, slot, it.j + j + lane) >= 0);
-        const bool page = (there >> (j & 31)) & 1u, whole = tok0 + TA_PAGE <= sg.len && tok0 >= edge && page;
+        if ((j & 31) == 0) there = __ballot_sync(0xffffffffu, j + lane < it.nj && ta_page(a, it.slot, it.j + j + lane) >= 0);
+        const bool page = (there >> (j & 31)) & 1u, whole = tok0 + TA_PAGE <= sg.len && tok0 >= it.edge && page;
         uint64_t seen = ~0ull;
-        int at_lo = 0, at_hi = 0;                              // FEAT: positions of the page's tokens `lane` and 32 + lane
+        int at_lo = tok0 + lane, at_hi = at_lo + 32;           // FEAT: positions of the page's tokens `lane` and 32 + lane
         if (!whole && !idle) {
           seen = page ? tc_mask(a, sg, tok0, node, p, near) : 0ull;
           if (FEAT && tok0 + TA_PAGE > sg.len) {
             const int n0 = tok0 + lane - sg.len, n1 = n0 + 32;
-            at_lo = n0 < 0 ? tok0 + lane : (n0 < sg.n ? a.pos[sg.r0 + n0] : p);
-            at_hi = n1 < 0 ? tok0 + lane + 32 : (n1 < sg.n ? a.pos[sg.r0 + n1] : p);
+            if (n0 >= 0) at_lo = n0 < sg.n ? a.pos[sg.r0 + n0] : p;
+            if (n1 >= 0) at_hi = n1 < sg.n ? a.pos[sg.r0 + n1] : p;
           }
         }
-        ok = __all_sync(0xffffffffu, mbar_wait(&s_full[q], n & 1));
-        if (!ok) { set_status(a.status, ST_TIMEOUT_TMEM_FULL, blockIdx.x, it.s, j); break; }
+        ok = tc_wait(&s_full[q], n & 1);
+        if (!ok) { why = ST_TIMEOUT_TMEM_FULL; break; }
         tc_fence_after();
         float s[64];
         if (idle) {                                          // (it waits as well: weights of two pages may not be announced in one phase)
           if (lane == 0) mbar_arrive(&s_read[q]);
-          if (L::TWO && n > 0) ok = __all_sync(0xffffffffu, mbar_wait(&o_full[q * 2], phase(n - 1)));
-          if (!ok) { set_status(a.status, ST_TIMEOUT_TMEM_FULL, blockIdx.x, it.s, j); break; }
+          if (L::TWO && n > 0) ok = tc_wait(&o_full[q * 2], phase(n - 1));
+          if (!ok) { why = ST_TIMEOUT_TMEM_FULL; break; }
         } else {
           {
             uint32_t raw[2][32];
@@ -387,7 +441,10 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
               for (int i = 0; i < 64; ++i) big = fmaxf(big, fabsf(s[i]));
               if (__any_sync(0xffffffffu, big * icap >= CAP_NEAR)) {
 #pragma unroll
-                for (int i = 0; i < 64; ++i) s[i] = a.cap * cap_tanh(s[i] * icap);
+                for (int i = 0; i < 64; ++i) {               // (cap_tanh with the approximate instructions)
+                  const float z = s[i] * icap, e = tc_ex2(fminf(z, 40.f) * (2.f * TA_LOG2E));
+                  s[i] = fabsf(z) < CAP_NEAR ? s[i] * tanh_over_z(z) : a.cap - 2.f * a.cap * tc_rcp(1.f + e);
+                }
               } else {
 #pragma unroll
                 for (int i = 0; i < 64; ++i) s[i] *= tanh_over_z(s[i] * icap);
@@ -405,15 +462,10 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
 #pragma unroll
                 for (int i0 = 0; i0 < 64; i0 += 16) {        // sixteen in flight
                   float x[16];
-                  if (nodes) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                      const int d = p - __shfl_sync(0xffffffffu, i0 < 32 ? at_lo : at_hi, (i0 & 31) + i);
-                      x[i] = __ldg(bh + min(max(d, 0), a.bias_n - 1));
-                    }
-                  } else {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) x[i] = __ldg(bh + min(d0 - i0 - i, a.bias_n - 1));
+                  for (int i = 0; i < 16; ++i) {
+                    const int d = p - __shfl_sync(0xffffffffu, i0 < 32 ? at_lo : at_hi, (i0 & 31) + i);
+                    x[i] = __ldg(bh + min(max(d, 0), a.bias_n - 1));
                   }
 #pragma unroll
                   for (int i = 0; i < 16; ++i) s[i0 + i] += x[i];
@@ -444,8 +496,8 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
           float c = 1.f, page_sum;
           // the weights' place: the product has read it (of two places: scores are announced behind the product of two pages back)
           if (L::TWO && n > 0) {
-            ok = __all_sync(0xffffffffu, mbar_wait(&o_full[q * 2], phase(n - 1)));
-            if (!ok) { set_status(a.status, ST_TIMEOUT_TMEM_FULL, blockIdx.x, it.s, j); break; }
+            ok = tc_wait(&o_full[q * 2], phase(n - 1));
+            if (!ok) { why = ST_TIMEOUT_TMEM_FULL; break; }
             tc_fence_after();
           }
 #pragma unroll 1
@@ -493,8 +545,8 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
           l += page_sum;
           if (renew && __any_sync(0xffffffffu, rescale)) {
             if (!L::TWO) {                                   // (with two terms the product before has been waited for)
-              ok = __all_sync(0xffffffffu, mbar_wait(&o_full[q * 2 + place(n - 1)], phase(n - 1)));
-              if (!ok) { set_status(a.status, ST_TIMEOUT_TMEM_FULL, blockIdx.x, it.s, j); break; }
+              ok = tc_wait(&o_full[q * 2 + place(n - 1)], phase(n - 1));
+              if (!ok) { why = ST_TIMEOUT_TMEM_FULL; break; }
               tc_fence_after();
             }
             const uint64_t k2 = tc_two(c, c);
@@ -513,42 +565,36 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
           }
         }
         if (!whole) {
-          ok = __all_sync(0xffffffffu, mbar_wait(&v_seen[q], seen_phase));
+          ok = tc_wait(&v_seen[q], seen_phase);
           seen_phase ^= 1u;
-          if (!ok) { set_status(a.status, ST_TIMEOUT_MBAR_FULL, blockIdx.x, it.s, j); break; }
+          if (!ok) { why = ST_TIMEOUT_MBAR_FULL; break; }
           const int vs = (seq0 + (j < it.nj - 1 ? 2 * j + 2 : 2 * j + 1)) % SLOTS;       // the values' place in the ring's sequence
           const uint64_t bad = odd_rows[2 * vs] | static_cast<uint64_t>(odd_rows[2 * vs + 1]) << 32;
           if (bad) {                                         // (rare)
             uint8_t* vals = ring + vs * SLOT;
             if (!L::TWO && n > 0) {
-              ok = __all_sync(0xffffffffu, mbar_wait(&o_full[q * 2 + place(n - 1)], phase(n - 1)));
-              if (!ok) { set_status(a.status, ST_TIMEOUT_TMEM_FULL, blockIdx.x, it.s, j); break; }
+              ok = tc_wait(&o_full[q * 2 + place(n - 1)], phase(n - 1));
+              if (!ok) { why = ST_TIMEOUT_TMEM_FULL; break; }
               tc_fence_after();
             }
-            const float r = ref == -INFINITY ? 0.f : ref;
+            if (!idle) {                                     // (the weights are there already; which are 0 is all that matters)
+              tmem_st_wait();
 #pragma unroll 1
-            for (int cc = 0; cc < vn && !idle; cc += 32) {
-              uint32_t o[32];
-              tmem_ld_32x32(t_lane + 128 + cc, o);
-              tmem_ld_wait();
+              for (uint64_t left = bad; left; left &= left - 1) {
+                const int k = __ffsll(left) - 1;
+                const uint32_t pair = tc_ld1(t_lane + 64 + place(n) * 32 + k / 2);
+                const float w = __uint_as_float(k & 1 ? pair & 0xffff0000u : pair << 16);
 #pragma unroll 1
-              for (int k = 0; k < 64; ++k) {
-                if (!((bad >> k) & 1ull)) continue;
-                float x = -INFINITY;
-#pragma unroll
-                for (int e = 0; e < 64; ++e) x = e == k ? s[e] : x;
-                const float w = (seen >> k) & 1ull ? tc_ex2(FEAT ? (x - r) * TA_LOG2E : fmaf(x, c1, -r)) : 0.f;
-#pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                  const int col = cc + e, u = col >> 3;
-                  const uint16_t v = *reinterpret_cast<const uint16_t*>(vals + (u >> 3) * KV_CHUNK + k * 128 + (((u & 7) ^ (k & 7)) * 16) + (col & 7) * 2);
-                  if ((v & 0x7f80u) == 0x7f80u && w != 0.f) o[e] = __float_as_uint(fmaf(w, __uint_as_float(static_cast<uint32_t>(v) << 16), __uint_as_float(o[e])));
+                for (int col = 0; col < vn; ++col) {
+                  const uint32_t v = *reinterpret_cast<const uint16_t*>(vals + (col >> 6) * KV_CHUNK + k * 128 + (((col >> 3 & 7) ^ (k & 7)) * 16) + (col & 7) * 2);
+                  if ((v & 0x7f80u) != 0x7f80u) continue;    // (the same for the whole warp)
+                  const float o = __uint_as_float(tc_ld1(t_lane + 128 + col));
+                  tc_st1(t_lane + 128 + col, __float_as_uint(w != 0.f ? fmaf(w, __uint_as_float(v << 16), o) : o));
                 }
               }
-              tmem_st_32x32(t_lane + 128 + cc, o);
             }
             ok = tc_sync(sync, sync_ph);                     // everyone has read them
-            if (!ok) { set_status(a.status, ST_TIMEOUT_MBAR_FULL, blockIdx.x, it.s, j); break; }
+            if (!ok) { why = ST_TIMEOUT_MBAR_FULL; break; }
             const int tok = row & 63, parts = both ? 4 : 2;
             for (int u = q * 2 * both + (row >> 6); u < vn_units; u += parts) {
               uint16_t* x = reinterpret_cast<uint16_t*>(vals + (u >> 3) * KV_CHUNK + tok * 128 + (((u & 7) ^ (tok & 7)) * 16));
@@ -557,7 +603,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
             }
             fence_proxy_async();
             ok = tc_sync(sync, sync_ph);
-            if (!ok) { set_status(a.status, ST_TIMEOUT_MBAR_FULL, blockIdx.x, it.s, j); break; }
+            if (!ok) { why = ST_TIMEOUT_MBAR_FULL; break; }
           }
         }
         tmem_st_wait();
@@ -566,54 +612,47 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         if (lane == 0) mbar_arrive(&p_full[q * 2 + place(n)]);
       }
       if (!ok) break;
-      // ---- the rows' outputs, or this CTA's part of them: 32 rows of a warp pass shared memory (its own queries', which are used up) in
-      // blocks of columns, so that a row's columns are written together
-      ok = __all_sync(0xffffffffu, mbar_wait(&o_full[q * 2 + place(n - 1)], phase(n - 1)));
-      if (!ok) { set_status(a.status, ST_TIMEOUT_TMEM_FULL, blockIdx.x, it.s, it.nj); break; }
+      // ---- the rows' outputs, or this CTA's part of them
+      ok = tc_wait(&o_full[q * 2 + place(n - 1)], phase(n - 1));
+      if (!ok) { why = ST_TIMEOUT_TMEM_FULL; break; }
       tc_fence_after();
       if (idle) { tc_fence_before(); continue; }
       const bool done = it.first && it.last;
       float m = ref;
       if (!FEAT && m != -INFINITY) m *= TA_LN2;
-      const size_t pb = (static_cast<size_t>(blockIdx.x) * 2 + (it.first ? 1 : 0)) * a.bm + q * 128;
+      const size_t pb = ((static_cast<size_t>(blockIdx.x) * 2 + (it.first ? 1 : 0)) << a.bm_log) + q * 128 + row;
       float k = 1.f;
       if (done) {
         if (a.sink) {
           const float M = fmaxf(m, a.sink[h]);
-          k = expf(m - M);
-          l = l * k + expf(a.sink[h] - M);
+          k = __expf(m - M);
+          l = l * k + __expf(a.sink[h] - M);
         }
         k = l > 0.f ? ta_head_factor<__nv_bfloat16>(a, pr, h) * k / l : 0.f;
         if (l != l) k = l;
       } else if (row < pairs) {
-        *reinterpret_cast<float2*>(a.part_ml + (pb + row) * 2) = make_float2(m, l);
+        *reinterpret_cast<float2*>(a.part_ml + pb * 2) = make_float2(m, l);
       }
-      constexpr int BC = L::STAGE / (128 * 4);               // columns of a block: 32 or 64
-      uint8_t* mine = smem + q * L::STAGE + quad * 32 * 128;           // 32 columns of the warp's rows, the next 32 Q_CHUNK behind them
-      const size_t oo = done ? static_cast<size_t>(pr) * a.ldo + static_cast<size_t>(h) * a.ho : 0;
+      __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + static_cast<size_t>(pr) * a.ldo + static_cast<size_t>(h) * a.ho;
+      float* part = a.part_o + pb * a.V;
 #pragma unroll 1
-      for (int cc = 0; cc < vn; cc += BC) {
+      for (int cc = 0; cc < vn; cc += 32) {
+        uint32_t o[32];
+        tmem_ld_32x32(t_lane + 128 + cc, o);
+        tmem_ld_wait();
+        if (row < pairs) {
 #pragma unroll
-        for (int x = 0; x < BC; x += 32) {
-          uint32_t o[32];
-          tmem_ld_32x32(t_lane + 128 + min(cc + x, DC - 32), o);
-          tmem_ld_wait();
+          for (int i = 0; i < 4; ++i) {
+            if (cc + i * 8 >= a.V) break;
+            if (done) {
+              uint32_t w[4];
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            *reinterpret_cast<float4*>(mine + x / 32 * Q_CHUNK + lane * 128 + ((i ^ (lane & 7)) * 16)) =
-                make_float4(__uint_as_float(o[4 * i]) * k, __uint_as_float(o[4 * i + 1]) * k, __uint_as_float(o[4 * i + 2]) * k, __uint_as_float(o[4 * i + 3]) * k);
-        }
-        __syncwarp();
-        constexpr int TR = 128 / BC;                         // rows of an instruction
-        const int unit = lane % (BC / 4), col = cc + unit * 4;
-#pragma unroll 4
-        for (int r0 = 0; r0 < 32; r0 += TR) {
-          const int rr = r0 + lane / (BC / 4);
-          const size_t dst = __shfl_sync(0xffffffffu, oo, rr);
-          const float4 v = *reinterpret_cast<const float4*>(mine + unit / 8 * Q_CHUNK + rr * 128 + (((unit & 7) ^ (rr & 7)) * 16));
-          if (quad * 32 + rr < pairs && col < a.V) {
-            if (done) stf4(static_cast<__nv_bfloat16*>(a.out) + dst + col, v);
-            else *reinterpret_cast<float4*>(a.part_o + (pb + quad * 32 + rr) * a.V + col) = v;
+              for (int e = 0; e < 4; ++e) w[e] = tc_pack(__uint_as_float(o[i * 8 + 2 * e]) * k, __uint_as_float(o[i * 8 + 2 * e + 1]) * k);
+              *reinterpret_cast<uint4*>(out + cc + i * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+            } else {
+              *reinterpret_cast<uint4*>(part + cc + i * 8) = make_uint4(o[i * 8], o[i * 8 + 1], o[i * 8 + 2], o[i * 8 + 3]);
+              *reinterpret_cast<uint4*>(part + cc + i * 8 + 4) = make_uint4(o[i * 8 + 4], o[i * 8 + 5], o[i * 8 + 6], o[i * 8 + 7]);
+            }
           }
         }
         __syncwarp();
@@ -621,6 +660,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       tc_fence_before();
     }
   }
+  if (why != ST_OK && lane == 0) set_status(a.status, why, blockIdx.x, warp);
   tc_fence_before();
   __syncthreads();
   if (warp == 1) { tc_fence_after(); tmem_dealloc<L::COLS>(tmem); }
@@ -641,13 +681,13 @@ static int launch_tc_feat(const CUtensorMap& tk, const CUtensorMap& tv, const Tr
 
 int launch_tree_tc(const TreeAttn& a, cudaStream_t s) {
   const int w = a.D > a.V ? a.D : a.V;
-  if (w > 256 || ((a.ldq | a.hq | a.ldo | a.ho) & 7) || (a.bm == 256 && w > 128)) return -5;
+  if (w > 256 || ((a.ldq | a.hq | a.ldo | a.ho) & 7) || (a.bm_log == 8 && w > 128)) return -5;
   CUtensorMap tk, tv;
   if (const int r = make_tmap_page(&tk, a.k, a.n_pages, a.G, a.D, a.k_tok, a.k_page)) return r;
   if (const int r = make_tmap_page(&tv, a.v, a.n_pages, a.G, a.V, a.v_tok, a.v_page)) return r;
   if (w > 128) return launch_tc_feat<256, 1>(tk, tv, a, s);
-  if (w > 64) return a.bm == 256 ? launch_tc_feat<128, 2>(tk, tv, a, s) : launch_tc_feat<128, 1>(tk, tv, a, s);
-  return a.bm == 256 ? launch_tc_feat<64, 2>(tk, tv, a, s) : launch_tc_feat<64, 1>(tk, tv, a, s);
+  if (w > 64) return a.bm_log == 8 ? launch_tc_feat<128, 2>(tk, tv, a, s) : launch_tc_feat<128, 1>(tk, tv, a, s);
+  return a.bm_log == 8 ? launch_tc_feat<64, 2>(tk, tv, a, s) : launch_tc_feat<64, 1>(tk, tv, a, s);
 }
 
 }  // namespace spark
