@@ -40,7 +40,7 @@ def _run(cmd):
 
 # kernel sources of families that need only part of the library
 FAMILY_SOURCES = {"vabunex": ("block_rows", "elementwise", "gemm", "gemm_simt", "gemv", "latent", "linear_state", "mla"),
-                  "debisun": ("block_rows", "elementwise", "gemm", "gemm_simt", "gemv", "moe", "paged_attn", "tree_attn", "tree_rows"),
+                  "debisun": ("block_rows", "elementwise", "gemm", "gemm_simt", "gemv", "moe", "paged_attn", "tree_attn", "tree_attn_tc", "tree_rows"),
                   "zapolorn": ("block_rows", "elementwise", "gemm", "gemm_simt", "gemv", "linear_state", "moe", "paged_attn"),
                   "zakusun": ("block_rows", "elementwise", "gemm", "gemm_simt", "gemv", "latent", "mla", "moe", "row_tiles")}
 

@@ -208,6 +208,9 @@ tree_tile_kernel(const __grid_constant__ TreeAttn a) {
 }
 
 // ------------------------------------------------------------------------------------------------ merge
+// exponential of the outputs' accuracy
+template <typename T> __device__ __forceinline__ float tm_exp(float x) { return sizeof(T) == 2 ? __expf(x) : expf(x); }
+
 constexpr int TM_THREADS = 256, TM_WARPS = TM_THREADS / 32, TM_MAX_CTAS = 1024;
 
 // Every CTA makes the list of the split items' rows (a row per item that begins in one CTA of the first launch and ends in another) and
@@ -224,12 +227,7 @@ tree_merge_kernel(const __grid_constant__ TreeAttn a) {
   pdl_wait();
   pdl_trigger();
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31, V4 = a.V >> 2, rep = a.H / a.G;
-  if (a.zero_rest)
-    for (int r = a.starts[a.S] + blockIdx.x; r < a.R; r += gridDim.x)
-      for (int i = t; i < a.H * V4; i += TM_THREADS) {
-        const int h = i / V4;
-        stf4(static_cast<T*>(a.out) + static_cast<size_t>(r) * a.ldo + static_cast<size_t>(h) * a.ho + (i - h * V4) * 4, make_float4(0.f, 0.f, 0.f, 0.f));
-      }
+  const int end = a.zero_rest ? a.starts[a.S] : a.R;         // rows of the requests
   const int each = (a.ctas + TM_THREADS - 1) / TM_THREADS;   // up to four
   int n[4], mine = 0;
 #pragma unroll
@@ -252,13 +250,15 @@ tree_merge_kernel(const __grid_constant__ TreeAttn a) {
   }
   if (t == 0) s_first[a.ctas] = rows;
   __syncthreads();
-  int wpr = TM_WARPS;
-  while (wpr > 1 && rows * wpr > static_cast<int>(gridDim.x) * TM_WARPS) wpr >>= 1;
-  const int rpb = TM_WARPS / wpr, sub = warp & (wpr - 1);
+  int lw = 3;                                                // log2 of the warps that join one row
+  while (lw > 0 && rows << lw > static_cast<int>(gridDim.x) * TM_WARPS) --lw;
+  const int wpr = 1 << lw, rpb = TM_WARPS >> lw, sub = warp & (wpr - 1);
+#pragma unroll 1
   for (int task0 = blockIdx.x * rpb; task0 < rows; task0 += gridDim.x * rpb) {
-    const int task = task0 + warp / wpr;
+    const int task = task0 + (warp >> lw);
     const bool on = task < rows;
     int lo = 0, hi = a.ctas;                                 // the last CTA whose rows begin at or before the task
+#pragma unroll 1
     while (hi - lo > 1) { const int m = (lo + hi) >> 1; if (s_first[m] <= task) lo = m; else hi = m; }
     const int c = lo, row = on ? task - s_first[lo] : 0;
     const int4 sp = s_split[c];
@@ -267,6 +267,7 @@ tree_merge_kernel(const __grid_constant__ TreeAttn a) {
     auto part = [&](int i) { return ((static_cast<size_t>(c + i) * 2 + (i == 0 ? 1 : 0)) << a.bm_log) + row; };
     float m = -INFINITY, l = 0.f;
     float4 o[VC] = {};
+#pragma unroll 1
     for (int i0 = sub; i0 < parts; i0 += 4 * wpr) {          // four parts in flight
       float4 x[4][VC];
       float2 ml[4];
@@ -279,15 +280,15 @@ tree_merge_kernel(const __grid_constant__ TreeAttn a) {
           if (i < parts && lane + v * 32 < V4) x[u][v] = __ldcg(reinterpret_cast<const float4*>(a.part_o + part(i) * a.V) + lane + v * 32);
       }
       const float top = fmaxf(m, fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x))), ref = top == -INFINITY ? 0.f : top;
-      const float k = expf(m - ref);
+      const float k = tm_exp<T>(m - ref);
       m = top;
       l *= k;
 #pragma unroll
       for (int v = 0; v < VC; ++v) { o[v].x *= k; o[v].y *= k; o[v].z *= k; o[v].w *= k; }
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        const float w = expf(ml[u].x - ref);
-        if (w == 0.f) continue;
+        const float w = tm_exp<T>(ml[u].x - ref);
+        if (w == 0.f && ml[u].y == ml[u].y) continue;        // (a part of NaN scores alone stays)
         l = fmaf(w, ml[u].y, l);
 #pragma unroll
         for (int v = 0; v < VC; ++v)
@@ -306,13 +307,14 @@ tree_merge_kernel(const __grid_constant__ TreeAttn a) {
       __syncthreads();
       if (sub == 0) {
         for (int i = 1; i < wpr; ++i) m = fmaxf(m, s_ml[warp + i][0]);
-        const float ref = m == -INFINITY ? 0.f : m, c0 = expf(s_ml[warp][0] - ref);
+        const float ref = m == -INFINITY ? 0.f : m, c0 = tm_exp<T>(s_ml[warp][0] - ref);
         l *= c0;
 #pragma unroll
         for (int v = 0; v < VC; ++v) { o[v].x *= c0; o[v].y *= c0; o[v].z *= c0; o[v].w *= c0; }
+#pragma unroll 1
         for (int i = 1; i < wpr; ++i) {
-          const float w = expf(s_ml[warp + i][0] - ref);
-          if (w == 0.f) continue;
+          const float w = tm_exp<T>(s_ml[warp + i][0] - ref);
+          if (w == 0.f && s_ml[warp + i][1] == s_ml[warp + i][1]) continue;
           l = fmaf(w, s_ml[warp + i][1], l);
 #pragma unroll
           for (int v = 0; v < VC; ++v)
@@ -328,8 +330,8 @@ tree_merge_kernel(const __grid_constant__ TreeAttn a) {
     float k = 1.f;
     if (a.sink) {
       const float M = fmaxf(m, a.sink[h]);
-      k = expf(m - M);
-      l = l * k + expf(a.sink[h] - M);
+      k = tm_exp<T>(m - M);
+      l = l * k + tm_exp<T>(a.sink[h] - M);
     }
     float scale = l > 0.f ? ta_head_factor<T>(a, r, h) * k / l : 0.f;
     if (l != l) scale = l;
@@ -339,6 +341,13 @@ tree_merge_kernel(const __grid_constant__ TreeAttn a) {
         stf4(static_cast<T*>(a.out) + static_cast<size_t>(r) * a.ldo + static_cast<size_t>(h) * a.ho + (lane + v * 32) * 4,
              make_float4(o[v].x * scale, o[v].y * scale, o[v].z * scale, o[v].w * scale));
   }
+#pragma unroll 1
+  for (int r = end + blockIdx.x; r < a.R; r += gridDim.x)
+#pragma unroll 1
+    for (int i = t; i < a.H * V4; i += TM_THREADS) {
+      const int h = i / V4;
+      stf4(static_cast<T*>(a.out) + static_cast<size_t>(r) * a.ldo + static_cast<size_t>(h) * a.ho + (i - h * V4) * 4, make_float4(0.f, 0.f, 0.f, 0.f));
+    }
 }
 
 constexpr int TA_SMEM = 220 * 1024;

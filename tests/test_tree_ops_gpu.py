@@ -133,6 +133,21 @@ def test_rows_that_see_nothing_are_zero(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("length", [70, 9000])         # one CTA to a request's keys, and many
+def test_what_is_not_a_number_shows(length, dtype):
+    r = U.Round([length, length], [9, 9], device=DEV)
+    q, k, v = r.randn(r.R, 4, 64, dtype=dtype), r.randn(r.n_pages, 64, 2, 64, dtype=dtype), r.randn(r.n_pages, 64, 2, 64, dtype=dtype)
+    maps = ops.slot_maps(**r.inputs())
+    clean = ops.tree_attention(q, k, v, maps, 0.125)
+    q[3, 1] = float("nan")                             # every score of the row
+    got = ops.tree_attention(q, k, v, maps, 0.125)
+    assert got[3, 1].isnan().all()
+    got[3, 1] = clean[3, 1]
+    # rows beside it may be held against another reference: 2^-17 of a weight and half a step of the output on either side
+    assert ((got - clean).abs().float() <= 2 * U.half_step(dtype) * clean.abs().float() + 2.0 ** -16 * v.abs().max().float()).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_missing_pages_are_not_read(dtype):
     r = U.Round([300], [5], device=DEV)
     q, k, v = r.randn(r.R, 4, 64, dtype=dtype), r.randn(r.n_pages, 64, 2, 64, dtype=dtype), r.randn(r.n_pages, 64, 2, 64, dtype=dtype)
