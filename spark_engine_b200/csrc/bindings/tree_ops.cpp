@@ -235,8 +235,8 @@ Tensor tree_attention(Tensor q, const Tensor& k, const Tensor& v, const RowMaps&
   // the keys, one CTA per SM.  Heads wider than 128 leave room for one tile and one CTA.
   const bool tc = dt == at::kBFloat16 && D <= 256 && V <= 256, wide = D > 128 || V > 128;
   const int64_t most = (m.nodes ? std::min(m.nodes, R) : R) * (H / G);
-  const int bm = !tc ? 32 : !wide && most > 128 ? 256 : 128;
-  const int ctas = std::min(1024, on.dev.sms * (!tc ? 3 : bm == 256 || wide ? 1 : 2));
+  const int bm = !tc ? 64 : !wide && most > 128 ? 256 : 128;
+  const int ctas = std::min(1024, on.dev.sms * (bm == 256 || wide ? 1 : 2));
   // What beginning an item costs, in pages (us of a call, extra 0 / 3 / 6 / 10 / 15: four requests of 16k tokens, heads of 256: 61.3 / 57.5 / 55.2 /
   // 49.4 / 48.5; eight windows of 1024, heads of 128 with slopes: 37.2 / 32.1 / 31.7 / 31.5 / 34.6; ragged, soft cap and bias, whose pages take
   // longer: 45.6 / 41.5 / 45.0 / 45.1 / 52.0)
@@ -258,7 +258,7 @@ Tensor tree_attention(Tensor q, const Tensor& k, const Tensor& v, const RowMaps&
     while (1ll << (a.chunk_shift - 31) < chunk) ++a.chunk_shift;
     a.chunk_mul = static_cast<unsigned>(((static_cast<unsigned __int128>(1) << a.chunk_shift) + chunk - 1) / chunk);
   }
-  a.bm_log = bm == 32 ? 5 : bm == 128 ? 7 : 8; a.sms = on.dev.sms; a.ctas = ctas; a.min_tiles = 1; a.extra = extra; a.zero_rest = !given;
+  a.bm_log = bm == 64 ? 6 : bm == 128 ? 7 : 8; a.sms = on.dev.sms; a.ctas = ctas; a.min_tiles = 1; a.extra = extra; a.zero_rest = !given;
   a.scale = static_cast<float>(scale); a.cap = static_cast<float>(softcap); a.out_scale = static_cast<float>(out_scale);
   on.launch(e_attn, &a, static_cast<int>(dt == at::kFloat), static_cast<int>(tc));
   return out;

@@ -15,6 +15,26 @@ namespace spark {
 constexpr int TA_PAGE = TREE_PAGE;
 constexpr float TA_LOG2E = 1.4426950408889634f, TA_LN2 = 0.6931471805599453f;
 
+// two fp32 at a time
+__device__ __forceinline__ uint64_t ta_two(float x, float y) { return static_cast<uint64_t>(__float_as_uint(y)) << 32 | __float_as_uint(x); }
+__device__ __forceinline__ float ta_lo(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v)); }
+__device__ __forceinline__ float ta_hi(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
+__device__ __forceinline__ uint64_t ta_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t ta_add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t ta_mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
 __device__ __forceinline__ int ta_first_visible(const TreeAttn& a, int p) {
   // (p / chunk as a product: chunk_mul = ceil(2^chunk_shift / chunk) is exact for all p below 2^31)
   return a.chunk > 0 ? static_cast<int>(static_cast<unsigned long long>(p) * a.chunk_mul >> a.chunk_shift) * a.chunk : (a.window > 0 ? max(p - a.window + 1, 0) : 0);

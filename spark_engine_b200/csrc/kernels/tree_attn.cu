@@ -11,22 +11,222 @@
 namespace spark {
 
 // ------------------------------------------------------------------------------------------------ FP32 units
-constexpr int TT_BM = 32, TT_THREADS = 128, TT_LDK = 68, TT_LDV = 132, TT_LDS = 68;
+constexpr int TT_BM = 64, TT_THREADS = 256, TT_STAGES = 3, TT_LD = 68, TT_PIECE = TA_PAGE * TT_LD;
 
-// Scores: four rows x four keys per thread over 64-wide pieces of the head; outputs: four rows x eight columns per 128-wide piece of V.
-template <typename T, int VC>
-__global__ void __launch_bounds__(TT_THREADS)
+template <int N>                                             // bytes
+__device__ __forceinline__ void tt_copy(void* d, const void* s) {
+  if (N == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(d)), "l"(s) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(d)), "l"(s) : "memory");
+}
+
+// One item, 16 * MR rows: thread (ty, tx) has rows ty + 16 i; of a page's scores keys tx + 16 e, of the outputs four columns in every 64.  Keys and
+// values pass in pieces of 64 tokens x 64 channels (VP: pieces of a value), two of them on their way while one is worked on.
+template <typename T, int VP, int MR>
+__device__ __forceinline__ void tt_item(const TreeAttn& a, const TreeItem& it, T* ring, float* Qs, float* Ss, int* s_pos, int* s_first, int* s_at) {
+  const int t = threadIdx.x, ty = t >> 4, tx = t & 15, D = a.D, V = a.V, LDQ = (D + 63) / 64 * 64 + 4, rep = a.H / a.G;
+  const int f0 = it.rt * TT_BM, pairs = min(16 * MR, it.n * rep - f0), kc = (D + 63) >> 6, vc = (V + 63) >> 6;
+  int lj = 0, lc = 0, stage = 0;                             // the piece to be asked for next
+  int lpage = ta_page(a, it.slot, it.j), npage = it.nj > 1 ? ta_page(a, it.slot, it.j + 1) : -1;
+  auto load = [&](int to) {
+    if (lj < it.nj) {
+      const bool is_v = lc >= kc;
+      const int c = (is_v ? lc - kc : lc) * 64 + tx * 4, valid = lpage < 0 ? 0 : min(TA_PAGE, it.len + it.n - (it.j + lj) * TA_PAGE);
+      const T* src = is_v ? static_cast<const T*>(a.v) + max(lpage, 0) * a.v_page + static_cast<size_t>(it.g) * V
+                          : static_cast<const T*>(a.k) + max(lpage, 0) * a.k_page + static_cast<size_t>(it.g) * D;
+      const int64_t tok = is_v ? a.v_tok : a.k_tok;
+      if (c < (is_v ? V : D))
+#pragma unroll
+        for (int row = ty; row < TA_PAGE; row += 16)
+          if (row < valid) tt_copy<4 * sizeof(T)>(ring + to * TT_PIECE + row * TT_LD + tx * 4, src + row * tok + c);
+      if (++lc == kc + vc) {
+        lc = 0;
+        ++lj;
+        lpage = npage;
+        npage = lj + 1 < it.nj ? ta_page(a, it.slot, it.j + lj + 1) : -1;
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  auto next = [&]() {                                        // the piece that has come; everyone is done with the one before
+    asm volatile("cp.async.wait_group %0;" ::"n"(TT_STAGES - 2) : "memory");
+    __syncthreads();
+    const int now = stage;
+    stage = stage == TT_STAGES - 1 ? 0 : stage + 1;
+    load(now == 0 ? TT_STAGES - 1 : now - 1);
+    return ring + now * TT_PIECE;
+  };
+#pragma unroll
+  for (int i = 0; i < TT_STAGES - 1; ++i) load(i);
+  for (int row = ty; row < 16 * MR; row += 16)
+    for (int c = tx * 4; c < D; c += 64)
+      *reinterpret_cast<float4*>(Qs + row * LDQ + c) = row < pairs ? ldf4(static_cast<const T*>(a.q) + static_cast<size_t>(it.r0 + (f0 + row) / rep) * a.ldq + static_cast<size_t>(it.g * rep + (f0 + row) % rep) * a.hq + c)
+                                                                  : make_float4(0.f, 0.f, 0.f, 0.f);
+  if (t < 16 * MR) {
+    const int p = t < pairs ? a.pos[it.r0 + (f0 + t) / rep] : 0;
+    s_pos[t] = p;
+    s_first[t] = ta_first_visible(a, p);
+  }
+  uint64_t o[VP][MR][2] = {};                                // columns in pairs
+  float m[MR], l[MR];                                        // maximum, and this thread's share of the sum
+#pragma unroll
+  for (int i = 0; i < MR; ++i) { m[i] = -INFINITY; l[i] = 0.f; }
+#pragma unroll 1
+  for (int j = it.j; j < it.j + it.nj; ++j) {
+    const int page = ta_page(a, it.slot, j), tok0 = j * TA_PAGE;
+    const bool whole = page >= 0 && tok0 >= it.edge && tok0 + TA_PAGE <= it.len;
+    if (page < 0 && t == 0) set_status(a.status, ST_BOUNDS, it.r0, tok0, it.slot);
+    if (t < TA_PAGE) {
+      const int node = tok0 + t - it.len;
+      s_at[t] = node < 0 ? tok0 + t : (node < it.n ? a.pos[it.r0 + node] : 0);
+    }
+    // ---- scores: even and odd channels apart
+    uint64_t s2[MR][4] = {};
+#pragma unroll 1
+    for (int d0 = 0; d0 < D; d0 += 64) {
+      const T* kp = next() + tx * TT_LD;
+      const float* qp = Qs + ty * LDQ + d0;
+      const int width = min(64, D - d0);
+#pragma unroll 2
+      for (int c = 0; c < width; c += 4) {
+        ulonglong2 q[MR];
+#pragma unroll
+        for (int i = 0; i < MR; ++i) q[i] = *reinterpret_cast<const ulonglong2*>(qp + 16 * i * LDQ + c);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float4 k = ldf4(kp + 16 * e * TT_LD + c);
+          const uint64_t k0 = ta_two(k.x, k.y), k1 = ta_two(k.z, k.w);
+#pragma unroll
+          for (int i = 0; i < MR; ++i) s2[i][e] = ta_fma2(q[i].y, k1, ta_fma2(q[i].x, k0, s2[i][e]));
+        }
+      }
+    }
+    float s[MR][4];
+#pragma unroll
+    for (int i = 0; i < MR; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[i][e] = (ta_lo(s2[i][e]) + ta_hi(s2[i][e])) * a.scale;
+    if (a.cap > 0.f)
+#pragma unroll
+      for (int i = 0; i < MR; ++i)
+#pragma unroll 1
+        for (int e = 0; e < 4; ++e) {
+          const float x = e == 0 ? s[i][0] : e == 1 ? s[i][1] : e == 2 ? s[i][2] : s[i][3], y = a.cap * tanhf(x / a.cap);
+#pragma unroll
+          for (int z = 0; z < 4; ++z) s[i][z] = z == e ? y : s[i][z];
+        }
+    if (!whole || a.bias || a.slopes) {
+      const int valid = page < 0 ? 0 : min(TA_PAGE, it.len + it.n - tok0);
+#pragma unroll
+      for (int i = 0; i < MR; ++i) {
+        const int row = ty + 16 * i, f = f0 + min(row, pairs - 1), node = f / rep, h = it.g * rep + f - node * rep, p = s_pos[row], first = s_first[row];
+        const uint32_t* anc = a.anc ? a.anc + static_cast<size_t>(it.r0 + node) * a.words : nullptr;
+        const float slope = a.slopes ? a.slopes[h] : 0.f;
+        const float* bias = a.bias ? a.bias + static_cast<size_t>(h) * a.bias_n : nullptr;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int key = tx + 16 * e, at = s_at[key], kn = tok0 + key - it.len;
+          if (bias) s[i][e] += bias[min(max(p - at, 0), a.bias_n - 1)];
+          if (a.slopes) s[i][e] -= slope * static_cast<float>(p - at);
+          bool on = whole || (key < valid && at >= first);
+          if (on && kn >= 0) on = anc ? (kn >> 5) < a.words && (anc[kn >> 5] >> (kn & 31)) & 1u : kn <= node;
+          if (!on) s[i][e] = -INFINITY;
+        }
+      }
+    }
+    // ---- weights
+#pragma unroll
+    for (int i = 0; i < MR; ++i) {
+      float top = fmaxf(fmaxf(fmaxf(s[i][0], s[i][1]), fmaxf(s[i][2], s[i][3])), m[i]);
+#pragma unroll
+      for (int x = 1; x < 16; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+      const float ref = top == -INFINITY ? 0.f : top;
+      if (__any_sync(0xffffffffu, top != m[i])) {
+        const float k = expf(m[i] - ref);
+        const uint64_t k2 = ta_two(k, k);
+        l[i] *= k;
+#pragma unroll
+        for (int v = 0; v < VP; ++v) { o[v][i][0] = ta_mul2(o[v][i][0], k2); o[v][i][1] = ta_mul2(o[v][i][1], k2); }
+        m[i] = top;
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float w = expf(s[i][e] - ref);
+        l[i] += w;
+        Ss[(ty + 16 * i) * TT_LD + tx + 16 * e] = w;
+      }
+    }
+    __syncwarp();                                            // (a row's weights stay in its warp)
+#pragma unroll
+    for (int v = 0; v < VP; ++v) {
+      if (v >= vc) break;
+      const T* vp = next() + tx * 4;
+#pragma unroll 1
+      for (int k0 = 0; k0 < TA_PAGE; k0 += 4) {
+        float4 w[MR];
+#pragma unroll
+        for (int i = 0; i < MR; ++i) w[i] = *reinterpret_cast<const float4*>(Ss + (ty + 16 * i) * TT_LD + k0);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float4 x = ldf4(vp + (k0 + k) * TT_LD);
+          const uint64_t x0 = ta_two(x.x, x.y), x1 = ta_two(x.z, x.w);
+#pragma unroll
+          for (int i = 0; i < MR; ++i) {
+            const float y = k == 0 ? w[i].x : k == 1 ? w[i].y : k == 2 ? w[i].z : w[i].w;
+            const uint64_t y2 = ta_two(y, y);
+            if (whole || y != 0.f) {                         // what a row does not see stays out of it, whatever it holds
+              o[v][i][0] = ta_fma2(y2, x0, o[v][i][0]);
+              o[v][i][1] = ta_fma2(y2, x1, o[v][i][1]);
+            }
+          }
+        }
+      }
+    }
+  }
+  // ---- whole: the rows' outputs; else this CTA's part of them
+  const bool done = it.first && it.last;
+  if (it.first && !it.last && t == 0) ta_set_split(a, ta_split(a, it));
+  const size_t pb = (static_cast<size_t>(blockIdx.x) * 2 + (it.first ? 1 : 0)) * TT_BM;
+#pragma unroll
+  for (int i = 0; i < MR; ++i) {
+    const int row = ty + 16 * i, f = f0 + row, h = it.g * rep + f % rep, r = it.r0 + f / rep;
+    float sum = l[i], scale = 1.f;
+#pragma unroll
+    for (int x = 1; x < 16; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+    if (row >= pairs) continue;
+    if (done) {
+      float c = 1.f;
+      if (a.sink) {
+        const float top = fmaxf(m[i], a.sink[h]);
+        c = expf(m[i] - top);
+        sum = sum * c + expf(a.sink[h] - top);
+      }
+      scale = sum > 0.f ? ta_head_factor<T>(a, r, h) * c / sum : 0.f;
+      if (sum != sum) scale = sum;
+    } else if (tx == 0) {
+      a.part_ml[(pb + row) * 2] = m[i];
+      a.part_ml[(pb + row) * 2 + 1] = sum;
+    }
+#pragma unroll
+    for (int v = 0; v < VP; ++v) {
+      const int col = v * 64 + tx * 4;
+      if (col >= V) continue;
+      const float4 x = make_float4(ta_lo(o[v][i][0]) * scale, ta_hi(o[v][i][0]) * scale, ta_lo(o[v][i][1]) * scale, ta_hi(o[v][i][1]) * scale);
+      if (done) stf4(static_cast<T*>(a.out) + static_cast<size_t>(r) * a.ldo + static_cast<size_t>(h) * a.ho + col, x);
+      else *reinterpret_cast<float4*>(a.part_o + (pb + row) * V + col) = x;
+    }
+  }
+}
+
+template <typename T, int VP>
+__global__ void __launch_bounds__(TT_THREADS, VP <= 2 ? 2 : 1)
 tree_tile_kernel(const __grid_constant__ TreeAttn a) {
   extern __shared__ __align__(16) float smem_tt[];
   __shared__ TreeItem s_item;
-  __shared__ float s_m[TT_BM], s_l[TT_BM], s_f[TT_BM];
   __shared__ int s_pos[TT_BM], s_first[TT_BM], s_at[TA_PAGE];
-  const int D = a.D, V = a.V, LDQ = (D + 63) / 64 * 64 + 4, rep = a.H / a.G;
-  float* Qs = smem_tt;                                       // [32][LDQ]
-  float* Ks = Qs + TT_BM * LDQ;                              // [64][68]
-  float* Vs = Ks + TA_PAGE * TT_LDK;                         // [64][132]
-  float* Ss = Vs + TA_PAGE * TT_LDV;                         // [32][68]
-  const int t = threadIdx.x, ty = t >> 4, tx = t & 15;
+  float* Qs = smem_tt;                                       // [64][D + 4]
+  float* Ss = Qs + TT_BM * ((a.D + 63) / 64 * 64 + 4);       // [64][68]
+  T* ring = reinterpret_cast<T*>(Ss + TT_BM * TT_LD);        // [3][64][68]
+  const int t = threadIdx.x;
   pdl_wait();
   pdl_trigger();
   TreeRange range;
@@ -39,171 +239,13 @@ tree_tile_kernel(const __grid_constant__ TreeAttn a) {
       ta_next(a, range, next);
       if (t == 0) s_item = next;
     }
-    __syncthreads();
+    __syncthreads();                                         // (everyone is done with the item before)
     const TreeItem it = s_item;
     if (it.nj == 0) break;
-    const TreeItem& sg = it;
-    const int slot = it.slot, pairs = min(TT_BM, sg.n * rep - it.rt * TT_BM);
-    __syncthreads();
-    for (int i = t; i < TT_BM * (LDQ / 4); i += TT_THREADS) {
-      const int row = i / (LDQ / 4), c = (i - row * (LDQ / 4)) * 4, f = it.rt * TT_BM + row;
-      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (row < pairs && c < D) x = ldf4(static_cast<const T*>(a.q) + static_cast<size_t>(sg.r0 + f / rep) * a.ldq + static_cast<size_t>(it.g * rep + f % rep) * a.hq + c);
-      *reinterpret_cast<float4*>(Qs + row * LDQ + c) = x;
-    }
-    if (t < TT_BM) {
-      const int p = t < pairs ? a.pos[sg.r0 + (it.rt * TT_BM + t) / rep] : 0;
-      s_pos[t] = p;
-      s_first[t] = ta_first_visible(a, p);
-      s_m[t] = -INFINITY;
-      s_l[t] = 0.f;
-    }
-    float o[VC][4][8] = {};
-    for (int j = it.j; j < it.j + it.nj; ++j) {
-      const int page = ta_page(a, slot, j), tok0 = j * TA_PAGE;
-      if (page < 0 && t == 0) set_status(a.status, ST_BOUNDS, sg.r0, tok0, slot);
-      const int valid = page < 0 ? 0 : min(TA_PAGE, sg.len + sg.n - tok0);
-      const T* kp = static_cast<const T*>(a.k) + max(page, 0) * a.k_page + static_cast<size_t>(it.g) * D;
-      const T* vp = static_cast<const T*>(a.v) + max(page, 0) * a.v_page + static_cast<size_t>(it.g) * V;
-      if (t < TA_PAGE) {
-        const int node = tok0 + t - sg.len;
-        s_at[t] = node < 0 ? tok0 + t : (node < sg.n ? a.pos[sg.r0 + node] : 0);
-      }
-      float s[4][4] = {};
-      for (int d0 = 0; d0 < D; d0 += 64) {
-        __syncthreads();
-        for (int i = t; i < TA_PAGE * 16; i += TT_THREADS) {
-          const int row = i >> 4, c = (i & 15) * 4;
-          float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (row < valid && d0 + c < D) x = ldf4(kp + row * a.k_tok + d0 + c);
-          *reinterpret_cast<float4*>(Ks + row * TT_LDK + c) = x;
-        }
-        __syncthreads();
-#pragma unroll 4
-        for (int c = 0; c < 64; c += 4) {
-          float4 q[4], k[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) q[i] = *reinterpret_cast<const float4*>(Qs + (ty * 4 + i) * LDQ + d0 + c);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) k[i] = *reinterpret_cast<const float4*>(Ks + (tx + 16 * i) * TT_LDK + c);
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              s[i][e] = fmaf(q[i].x, k[e].x, fmaf(q[i].y, k[e].y, fmaf(q[i].z, k[e].z, fmaf(q[i].w, k[e].w, s[i][e]))));
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = ty * 4 + i, f = it.rt * TT_BM + row, h = it.g * rep + f % rep, node = f / rep;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int key = tx + 16 * e, kn = tok0 + key - sg.len;
-          bool on = row < pairs && key < valid && s_at[key] >= s_first[row];
-          if (on && kn >= 0) on = a.anc ? (kn >> 5) < a.words && (a.anc[static_cast<size_t>(sg.r0 + node) * a.words + (kn >> 5)] >> (kn & 31)) & 1u : kn <= node;
-          float x = -INFINITY;
-          if (on) {
-            const int dist = s_pos[row] - s_at[key];
-            x = s[i][e] * a.scale;
-            if (a.cap > 0.f) x = a.cap * tanhf(x / a.cap);
-            if (a.bias) x += a.bias[static_cast<size_t>(h) * a.bias_n + min(max(dist, 0), a.bias_n - 1)];
-            if (a.slopes) x -= a.slopes[h] * static_cast<float>(dist);
-          }
-          Ss[row * TT_LDS + key] = x;
-        }
-      }
-      __syncthreads();
-      {                                                      // statistics: four threads per row
-        const int row = t >> 2, c = t & 3;
-        float* sr = Ss + row * TT_LDS + c;
-        float mx = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sr[4 * i]);
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float m0 = s_m[row], m = fmaxf(m0, mx), ref = m == -INFINITY ? 0.f : m;
-        float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float e = expf(sr[4 * i] - ref);
-          sr[4 * i] = e;
-          sum += e;
-        }
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        __syncwarp();
-        if (c == 0) {
-          const float f = expf(m0 - ref);
-          s_f[row] = f;
-          s_m[row] = m;
-          s_l[row] = s_l[row] * f + sum;
-        }
-      }
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float f = s_f[ty * 4 + i];
-#pragma unroll
-        for (int v = 0; v < VC; ++v)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) o[v][i][e] *= f;
-      }
-#pragma unroll
-      for (int v = 0; v < VC; ++v) {
-        if (v) __syncthreads();
-        for (int i = t; i < TA_PAGE * 32; i += TT_THREADS) {
-          const int row = i >> 5, c = (i & 31) * 4;
-          float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (row < valid && v * 128 + c < V) x = ldf4(vp + row * a.v_tok + v * 128 + c);
-          *reinterpret_cast<float4*>(Vs + row * TT_LDV + c) = x;
-        }
-        __syncthreads();
-        for (int k = 0; k < TA_PAGE; ++k) {
-          const float4 x = *reinterpret_cast<const float4*>(Vs + k * TT_LDV + tx * 4), y = *reinterpret_cast<const float4*>(Vs + k * TT_LDV + 64 + tx * 4);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float p = Ss[(ty * 4 + i) * TT_LDS + k];
-            if (p != 0.f) {                                  // what a row does not see stays out of it, whatever it holds
-              o[v][i][0] = fmaf(p, x.x, o[v][i][0]); o[v][i][1] = fmaf(p, x.y, o[v][i][1]);
-              o[v][i][2] = fmaf(p, x.z, o[v][i][2]); o[v][i][3] = fmaf(p, x.w, o[v][i][3]);
-              o[v][i][4] = fmaf(p, y.x, o[v][i][4]); o[v][i][5] = fmaf(p, y.y, o[v][i][5]);
-              o[v][i][6] = fmaf(p, y.z, o[v][i][6]); o[v][i][7] = fmaf(p, y.w, o[v][i][7]);
-            }
-          }
-        }
-      }
-    }
-    // ---- whole: the rows' outputs; else this CTA's part of them
-    const bool whole = it.first && it.last;
-    if (it.first && !it.last && t == 0) ta_set_split(a, ta_split(a, it));
-    const size_t pb = (static_cast<size_t>(blockIdx.x) * 2 + (it.first ? 1 : 0)) * TT_BM;
-    if (!whole && t < pairs) { a.part_ml[(pb + t) * 2] = s_m[t]; a.part_ml[(pb + t) * 2 + 1] = s_l[t]; }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = ty * 4 + i, f = it.rt * TT_BM + row, h = it.g * rep + f % rep, r = sg.r0 + f / rep;
-      if (row >= pairs) continue;
-      float scale = 1.f;
-      if (whole) {
-        float l = s_l[row], c = 1.f;
-        if (a.sink) {
-          const float m = fmaxf(s_m[row], a.sink[h]);
-          c = expf(s_m[row] - m);
-          l = l * c + expf(a.sink[h] - m);
-        }
-        scale = l > 0.f ? ta_head_factor<T>(a, r, h) * c / l : 0.f;
-        if (l != l) scale = l;
-      }
-#pragma unroll
-      for (int v = 0; v < VC; ++v)
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int col = v * 128 + half * 64 + tx * 4;
-          if (col >= V) continue;
-          const float4 x = make_float4(o[v][i][half * 4] * scale, o[v][i][half * 4 + 1] * scale, o[v][i][half * 4 + 2] * scale, o[v][i][half * 4 + 3] * scale);
-          if (whole) stf4(static_cast<T*>(a.out) + static_cast<size_t>(r) * a.ldo + static_cast<size_t>(h) * a.ho + col, x);
-          else *reinterpret_cast<float4*>(a.part_o + (pb + row) * V + col) = x;
-        }
-    }
+    const int pairs = it.n * (a.H / a.G) - it.rt * TT_BM;
+    if (pairs <= 16) tt_item<T, VP, 1>(a, it, ring, Qs, Ss, s_pos, s_first, s_at);
+    else if (pairs <= 32) tt_item<T, VP, 2>(a, it, ring, Qs, Ss, s_pos, s_first, s_at);
+    else tt_item<T, VP, 4>(a, it, ring, Qs, Ss, s_pos, s_first, s_at);
   }
 }
 
@@ -352,10 +394,10 @@ tree_merge_kernel(const __grid_constant__ TreeAttn a) {
 
 constexpr int TA_SMEM = 220 * 1024;
 
-template <typename T, int VC>
+template <typename T, int VP>
 static int launch_tile(const TreeAttn& a, cudaStream_t s) {
-  auto kern = tree_tile_kernel<T, VC>;
-  const int smem = (TT_BM * ((a.D + 63) / 64 * 64 + 4) + TA_PAGE * (TT_LDK + TT_LDV) + TT_BM * TT_LDS) * 4;
+  auto kern = tree_tile_kernel<T, VP>;
+  const int smem = (TT_BM * ((a.D + 63) / 64 * 64 + 4) + TT_BM * TT_LD) * 4 + TT_STAGES * TT_PIECE * static_cast<int>(sizeof(T));
   if (smem > TA_SMEM) return -6;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, TA_SMEM) != cudaSuccess) return -4;
   spark_launch_pdl(kern, dim3(a.ctas), dim3(TT_THREADS), smem, s, dim3(1, 1, 1), a);
@@ -363,7 +405,7 @@ static int launch_tile(const TreeAttn& a, cudaStream_t s) {
 }
 template <typename T>
 static int launch_tiles(const TreeAttn& a, cudaStream_t s) {
-  return a.V <= 128 ? launch_tile<T, 1>(a, s) : a.V <= 256 ? launch_tile<T, 2>(a, s) : launch_tile<T, 4>(a, s);
+  return a.V <= 128 ? launch_tile<T, 2>(a, s) : a.V <= 256 ? launch_tile<T, 4>(a, s) : launch_tile<T, 8>(a, s);
 }
 
 int launch_tree_tc(const TreeAttn& a, cudaStream_t s);       // tree_attn_tc.cu
@@ -372,7 +414,7 @@ int launch_tree_tc(const TreeAttn& a, cudaStream_t s);       // tree_attn_tc.cu
 
 using namespace spark;
 
-// tc: the tensor-core kernel (bf16, head widths of up to 256; tiles of 128 or 256 rows), else the FP32 units (tiles of 32).
+// tc: the tensor-core kernel (bf16, head widths of up to 256; tiles of 128 or 256 rows), else the FP32 units (tiles of 64).
 extern "C" int spark_tree_attn(const TreeAttn* a, int f32, int tc, cudaStream_t s) {
   if (a->S <= 0 || a->R <= 0) return 0;
   if (a->H <= 0 || a->G <= 0 || a->H % a->G || a->D <= 0 || a->V <= 0 || ((a->D | a->V) & 7) || a->D > 512 || a->V > 512 || a->ctas <= 0 || a->ctas > TM_MAX_CTAS || a->sms <= 0 ||

@@ -73,25 +73,6 @@ __device__ __forceinline__ float tc_rcp(float x) {          // relative error 2^
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// two fp32 at a time
-__device__ __forceinline__ uint64_t tc_two(float x, float y) { return static_cast<uint64_t>(__float_as_uint(y)) << 32 | __float_as_uint(x); }
-__device__ __forceinline__ float tc_lo(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v)); }
-__device__ __forceinline__ float tc_hi(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
-__device__ __forceinline__ uint64_t tc_fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t tc_add2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ uint64_t tc_mul2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
 // A wait that ends: each try may suspend the thread for 20 us, a hundred thousand of them are two seconds.
 __device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity) {
   uint32_t ok = 0;
@@ -491,7 +472,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
             for (int i = 0; i < 64; ++i) s[i] = ((i < 32 ? m0 : m1) >> (i & 31)) & 1u ? s[i] : -INFINITY;
           }
           // ---- weights
-          const uint64_t c2 = FEAT ? tc_two(TA_LOG2E, TA_LOG2E) : tc_two(c1, c1);
+          const uint64_t c2 = FEAT ? ta_two(TA_LOG2E, TA_LOG2E) : ta_two(c1, c1);
           bool renew = fresh, rescale = false;
           float c = 1.f, page_sum;
           // the weights' place: the product has read it (of two places: scores are announced behind the product of two pages back)
@@ -517,28 +498,28 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
               fresh = __any_sync(0xffffffffu, ref == -INFINITY);       // rows that have seen nothing yet
             }
             const float r = ref == -INFINITY ? 0.f : ref;
-            const uint64_t r2 = tc_two(-r, -r), one = tc_two(-1.f, -1.f);
+            const uint64_t r2 = ta_two(-r, -r), one = ta_two(-1.f, -1.f);
             uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
             for (int part = 0; part < 2; ++part) {
               uint32_t hi[16], lo[16];
 #pragma unroll
               for (int i = 0; i < 16; ++i) {
-                const uint64_t x = tc_two(s[part * 32 + 2 * i], s[part * 32 + 2 * i + 1]);
-                const uint64_t z = FEAT ? tc_mul2(tc_add2(x, r2), c2) : tc_fma2(x, c2, r2);
-                const uint64_t e = tc_two(tc_ex2(tc_lo(z)), tc_ex2(tc_hi(z)));
-                sum[i & 1] = tc_add2(sum[i & 1], e);
-                hi[i] = tc_pack(tc_lo(e), tc_hi(e));
+                const uint64_t x = ta_two(s[part * 32 + 2 * i], s[part * 32 + 2 * i + 1]);
+                const uint64_t z = FEAT ? ta_mul2(ta_add2(x, r2), c2) : ta_fma2(x, c2, r2);
+                const uint64_t e = ta_two(tc_ex2(ta_lo(z)), tc_ex2(ta_hi(z)));
+                sum[i & 1] = ta_add2(sum[i & 1], e);
+                hi[i] = tc_pack(ta_lo(e), ta_hi(e));
                 if (L::TWO) {
-                  const uint64_t d = tc_fma2(tc_two(__uint_as_float(hi[i] << 16), __uint_as_float(hi[i] & 0xffff0000u)), one, e);
-                  lo[i] = tc_pack(tc_lo(d), tc_hi(d));
+                  const uint64_t d = ta_fma2(ta_two(__uint_as_float(hi[i] << 16), __uint_as_float(hi[i] & 0xffff0000u)), one, e);
+                  lo[i] = tc_pack(ta_lo(d), ta_hi(d));
                 }
               }
               tmem_st_32x16(t_lane + 64 + place(n) * 32 + part * 16, hi);
               if (L::TWO) tmem_st_32x16(t_lane + 96 + part * 16, lo);
             }
-            sum[0] = tc_add2(sum[0], sum[1]);
-            page_sum = tc_lo(sum[0]) + tc_hi(sum[0]);
+            sum[0] = ta_add2(sum[0], sum[1]);
+            page_sum = ta_lo(sum[0]) + ta_hi(sum[0]);
             if (renew || !__any_sync(0xffffffffu, !(page_sum < TC_MOST))) break;
             renew = true;
           }
@@ -549,7 +530,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
               if (!ok) { why = ST_TIMEOUT_TMEM_FULL; break; }
               tc_fence_after();
             }
-            const uint64_t k2 = tc_two(c, c);
+            const uint64_t k2 = ta_two(c, c);
 #pragma unroll 1
             for (int cc = 0; cc < vn; cc += 32) {
               uint32_t o[32];
@@ -557,7 +538,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
               tmem_ld_wait();
 #pragma unroll
               for (int i = 0; i < 32; i += 2) {
-                const uint64_t v = tc_mul2(static_cast<uint64_t>(o[i + 1]) << 32 | o[i], k2);
+                const uint64_t v = ta_mul2(static_cast<uint64_t>(o[i + 1]) << 32 | o[i], k2);
                 o[i] = static_cast<uint32_t>(v); o[i + 1] = static_cast<uint32_t>(v >> 32);
               }
               tmem_st_32x32(t_lane + 128 + cc, o);
