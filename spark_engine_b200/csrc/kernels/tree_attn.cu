@@ -8,10 +8,12 @@
 //   tree_merge   joins the parts of items that several CTAs share, and zeroes the rows behind the last request
 #include "../common/tree_work.cuh"
 
+#include <type_traits>
+
 namespace spark {
 
 // ------------------------------------------------------------------------------------------------ FP32 units
-constexpr int TT_BM = 64, TT_THREADS = 256, TT_STAGES = 3, TT_LD = 68, TT_PIECE = TA_PAGE * TT_LD;
+constexpr int TT_BM = 64, TT_THREADS = 256, TT_WARPS = TT_THREADS / 32, TT_STAGES = 3, TT_LD = 68, TT_PIECE = TA_PAGE * TT_LD;
 
 template <int N>                                             // bytes
 __device__ __forceinline__ void tt_copy(void* d, const void* s) {
@@ -19,26 +21,58 @@ __device__ __forceinline__ void tt_copy(void* d, const void* s) {
   else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(d)), "l"(s) : "memory");
 }
 
-// One item, 16 * MR rows: thread (ty, tx) has rows ty + 16 i; of a page's scores keys tx + 16 e, of the outputs four columns in every 64.  Keys and
-// values pass in pieces of 64 tokens x 64 channels (VP: pieces of a value), two of them on their way while one is worked on.
-template <typename T, int VP, int MR>
+// 2 or 4 columns
+template <typename T>
+__device__ __forceinline__ void tt_load(float (&x)[4], const T* p) {
+  const float4 v = ldf4(p);
+  x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+}
+__device__ __forceinline__ void tt_load(float (&x)[2], const float* p) {
+  const float2 v = *reinterpret_cast<const float2*>(p);
+  x[0] = v.x; x[1] = v.y;
+}
+__device__ __forceinline__ void tt_load(float (&x)[2], const __nv_bfloat16* p) {
+  const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(p));
+  x[0] = v.x; x[1] = v.y;
+}
+template <typename T>
+__device__ __forceinline__ void tt_store(T* p, const float (&x)[4], float k) { stf4(p, make_float4(x[0] * k, x[1] * k, x[2] * k, x[3] * k)); }
+__device__ __forceinline__ void tt_store(float* p, const float (&x)[2], float k) { *reinterpret_cast<float2*>(p) = make_float2(x[0] * k, x[1] * k); }
+__device__ __forceinline__ void tt_store(__nv_bfloat16* p, const float (&x)[2], float k) {
+  *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(x[0] * k, x[1] * k);
+}
+
+// One item, 8 * MR rows: a warp has rows warp + 8 i, so that what is read of a row is the same for all lanes (one shared-memory cycle instead of
+// four); a lane has keys lane + 32 e of a page's scores and CW neighbouring columns in every 32 CW of the outputs.  Keys pass in pieces of 64
+// tokens x 64 channels, values in pieces of 4096 (128 channels, or 64 where there are no more), two of them on their way while one is worked on.
+template <typename T, int VP, int CW, int MR>
 __device__ __forceinline__ void tt_item(const TreeAttn& a, const TreeItem& it, T* ring, float* Qs, float* Ss, int* s_pos, int* s_first, int* s_at) {
-  const int t = threadIdx.x, ty = t >> 4, tx = t & 15, D = a.D, V = a.V, LDQ = (D + 63) / 64 * 64 + 4, rep = a.H / a.G;
-  const int f0 = it.rt * TT_BM, pairs = min(16 * MR, it.n * rep - f0), kc = (D + 63) >> 6, vc = (V + 63) >> 6;
+  constexpr int VW = 32 * CW, VT = 4096 / VW;                // channels and tokens of a piece of values
+  const int t = threadIdx.x, warp = t >> 5, lane = t & 31, D = a.D, V = a.V, LDQ = (D + 63) / 64 * 64, rep = a.H / a.G;
+  const int f0 = it.rt * TT_BM, pairs = min(TT_WARPS * MR, it.n * rep - f0), kc = (D + 63) >> 6, vc = (V + VW - 1) / VW;
   int lj = 0, lc = 0, stage = 0;                             // the piece to be asked for next
   int lpage = ta_page(a, it.slot, it.j), npage = it.nj > 1 ? ta_page(a, it.slot, it.j + 1) : -1;
   auto load = [&](int to) {
     if (lj < it.nj) {
-      const bool is_v = lc >= kc;
-      const int c = (is_v ? lc - kc : lc) * 64 + tx * 4, valid = lpage < 0 ? 0 : min(TA_PAGE, it.len + it.n - (it.j + lj) * TA_PAGE);
-      const T* src = is_v ? static_cast<const T*>(a.v) + max(lpage, 0) * a.v_page + static_cast<size_t>(it.g) * V
-                          : static_cast<const T*>(a.k) + max(lpage, 0) * a.k_page + static_cast<size_t>(it.g) * D;
-      const int64_t tok = is_v ? a.v_tok : a.k_tok;
-      if (c < (is_v ? V : D))
+      const int valid = lpage < 0 ? 0 : min(TA_PAGE, it.len + it.n - (it.j + lj) * TA_PAGE);
+      T* dst = ring + to * TT_PIECE;
+      if (lc < kc) {
+        const int c = lc * 64 + (t & 15) * 4;
+        const T* src = static_cast<const T*>(a.k) + max(lpage, 0) * a.k_page + static_cast<size_t>(it.g) * D + c;
+        if (c < D)
 #pragma unroll
-        for (int row = ty; row < TA_PAGE; row += 16)
-          if (row < valid) tt_copy<4 * sizeof(T)>(ring + to * TT_PIECE + row * TT_LD + tx * 4, src + row * tok + c);
-      if (++lc == kc + vc) {
+          for (int row = t >> 4; row < TA_PAGE; row += 16)
+            if (row < valid) tt_copy<4 * sizeof(T)>(dst + row * TT_LD + (t & 15) * 4, src + row * a.k_tok);
+      } else {
+        constexpr int UNITS = VW / 4;                        // per token
+        const int x = lc - kc, u = t % UNITS, c = x / (TA_PAGE / VT) * VW + u * 4, tok0 = x % (TA_PAGE / VT) * VT;
+        const T* src = static_cast<const T*>(a.v) + max(lpage, 0) * a.v_page + static_cast<size_t>(it.g) * V + c;
+        if (c < V)
+#pragma unroll
+          for (int row = t / UNITS; row < VT; row += TT_THREADS / UNITS)
+            if (tok0 + row < valid) tt_copy<4 * sizeof(T)>(dst + row * VW + u * 4, src + (tok0 + row) * a.v_tok);
+      }
+      if (++lc == kc + vc * (TA_PAGE / VT)) {
         lc = 0;
         ++lj;
         lpage = npage;
@@ -57,16 +91,18 @@ __device__ __forceinline__ void tt_item(const TreeAttn& a, const TreeItem& it, T
   };
 #pragma unroll
   for (int i = 0; i < TT_STAGES - 1; ++i) load(i);
-  for (int row = ty; row < 16 * MR; row += 16)
-    for (int c = tx * 4; c < D; c += 64)
+#pragma unroll 1
+  for (int row = t >> 4; row < TT_WARPS * MR; row += 16)
+#pragma unroll 1
+    for (int c = (t & 15) * 4; c < D; c += 64)
       *reinterpret_cast<float4*>(Qs + row * LDQ + c) = row < pairs ? ldf4(static_cast<const T*>(a.q) + static_cast<size_t>(it.r0 + (f0 + row) / rep) * a.ldq + static_cast<size_t>(it.g * rep + (f0 + row) % rep) * a.hq + c)
                                                                   : make_float4(0.f, 0.f, 0.f, 0.f);
-  if (t < 16 * MR) {
+  if (t < TT_WARPS * MR) {
     const int p = t < pairs ? a.pos[it.r0 + (f0 + t) / rep] : 0;
     s_pos[t] = p;
     s_first[t] = ta_first_visible(a, p);
   }
-  uint64_t o[VP][MR][2] = {};                                // columns in pairs
+  float o[VP][MR][CW] = {};
   float m[MR], l[MR];                                        // maximum, and this thread's share of the sum
 #pragma unroll
   for (int i = 0; i < MR; ++i) { m[i] = -INFINITY; l[i] = 0.f; }
@@ -80,51 +116,48 @@ __device__ __forceinline__ void tt_item(const TreeAttn& a, const TreeItem& it, T
       s_at[t] = node < 0 ? tok0 + t : (node < it.n ? a.pos[it.r0 + node] : 0);
     }
     // ---- scores: even and odd channels apart
-    uint64_t s2[MR][4] = {};
+    uint64_t s2[MR][2] = {};
 #pragma unroll 1
     for (int d0 = 0; d0 < D; d0 += 64) {
-      const T* kp = next() + tx * TT_LD;
-      const float* qp = Qs + ty * LDQ + d0;
+      const T* kp = next() + lane * TT_LD;
+      const float* qp = Qs + warp * LDQ + d0;
       const int width = min(64, D - d0);
 #pragma unroll 2
       for (int c = 0; c < width; c += 4) {
         ulonglong2 q[MR];
 #pragma unroll
-        for (int i = 0; i < MR; ++i) q[i] = *reinterpret_cast<const ulonglong2*>(qp + 16 * i * LDQ + c);
+        for (int i = 0; i < MR; ++i) q[i] = *reinterpret_cast<const ulonglong2*>(qp + TT_WARPS * i * LDQ + c);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float4 k = ldf4(kp + 16 * e * TT_LD + c);
+        for (int e = 0; e < 2; ++e) {
+          const float4 k = ldf4(kp + 32 * e * TT_LD + c);
           const uint64_t k0 = ta_two(k.x, k.y), k1 = ta_two(k.z, k.w);
 #pragma unroll
           for (int i = 0; i < MR; ++i) s2[i][e] = ta_fma2(q[i].y, k1, ta_fma2(q[i].x, k0, s2[i][e]));
         }
       }
     }
-    float s[MR][4];
+    float s[MR][2];
 #pragma unroll
     for (int i = 0; i < MR; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[i][e] = (ta_lo(s2[i][e]) + ta_hi(s2[i][e])) * a.scale;
+      for (int e = 0; e < 2; ++e) s[i][e] = (ta_lo(s2[i][e]) + ta_hi(s2[i][e])) * a.scale;
     if (a.cap > 0.f)
 #pragma unroll
-      for (int i = 0; i < MR; ++i)
-#pragma unroll 1
-        for (int e = 0; e < 4; ++e) {
-          const float x = e == 0 ? s[i][0] : e == 1 ? s[i][1] : e == 2 ? s[i][2] : s[i][3], y = a.cap * tanhf(x / a.cap);
-#pragma unroll
-          for (int z = 0; z < 4; ++z) s[i][z] = z == e ? y : s[i][z];
-        }
+      for (int i = 0; i < MR; ++i) {
+        s[i][0] = a.cap * tanhf(s[i][0] / a.cap);
+        s[i][1] = a.cap * tanhf(s[i][1] / a.cap);
+      }
     if (!whole || a.bias || a.slopes) {
       const int valid = page < 0 ? 0 : min(TA_PAGE, it.len + it.n - tok0);
 #pragma unroll
       for (int i = 0; i < MR; ++i) {
-        const int row = ty + 16 * i, f = f0 + min(row, pairs - 1), node = f / rep, h = it.g * rep + f - node * rep, p = s_pos[row], first = s_first[row];
+        const int row = warp + TT_WARPS * i, f = f0 + min(row, pairs - 1), node = f / rep, h = it.g * rep + f - node * rep, p = s_pos[row], first = s_first[row];
         const uint32_t* anc = a.anc ? a.anc + static_cast<size_t>(it.r0 + node) * a.words : nullptr;
         const float slope = a.slopes ? a.slopes[h] : 0.f;
         const float* bias = a.bias ? a.bias + static_cast<size_t>(h) * a.bias_n : nullptr;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int key = tx + 16 * e, at = s_at[key], kn = tok0 + key - it.len;
+        for (int e = 0; e < 2; ++e) {
+          const int key = lane + 32 * e, at = s_at[key], kn = tok0 + key - it.len;
           if (bias) s[i][e] += bias[min(max(p - at, 0), a.bias_n - 1)];
           if (a.slopes) s[i][e] -= slope * static_cast<float>(p - at);
           bool on = whole || (key < valid && at >= first);
@@ -136,48 +169,58 @@ __device__ __forceinline__ void tt_item(const TreeAttn& a, const TreeItem& it, T
     // ---- weights
 #pragma unroll
     for (int i = 0; i < MR; ++i) {
-      float top = fmaxf(fmaxf(fmaxf(s[i][0], s[i][1]), fmaxf(s[i][2], s[i][3])), m[i]);
+      float top = fmaxf(fmaxf(s[i][0], s[i][1]), m[i]);
 #pragma unroll
-      for (int x = 1; x < 16; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+      for (int x = 1; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
       const float ref = top == -INFINITY ? 0.f : top;
-      if (__any_sync(0xffffffffu, top != m[i])) {
+      if (top != m[i]) {                                     // (the same for the whole warp)
         const float k = expf(m[i] - ref);
-        const uint64_t k2 = ta_two(k, k);
         l[i] *= k;
 #pragma unroll
-        for (int v = 0; v < VP; ++v) { o[v][i][0] = ta_mul2(o[v][i][0], k2); o[v][i][1] = ta_mul2(o[v][i][1], k2); }
+        for (int v = 0; v < VP; ++v)
+#pragma unroll
+          for (int x = 0; x < CW; ++x) o[v][i][x] *= k;
         m[i] = top;
       }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
+      for (int e = 0; e < 2; ++e) {
         const float w = expf(s[i][e] - ref);
         l[i] += w;
-        Ss[(ty + 16 * i) * TT_LD + tx + 16 * e] = w;
+        Ss[(warp + TT_WARPS * i) * TA_PAGE + lane + 32 * e] = w;
       }
     }
     __syncwarp();                                            // (a row's weights stay in its warp)
 #pragma unroll
     for (int v = 0; v < VP; ++v) {
       if (v >= vc) break;
-      const T* vp = next() + tx * 4;
 #pragma unroll 1
-      for (int k0 = 0; k0 < TA_PAGE; k0 += 4) {
-        float4 w[MR];
+      for (int tk = 0; tk < TA_PAGE; tk += VT) {
+        const T* vp = next() + lane * CW;
+        const float* wp = Ss + warp * TA_PAGE + tk;
+        auto add = [&](int k0, auto seen) {                  // four tokens
+          float4 w[MR];
 #pragma unroll
-        for (int i = 0; i < MR; ++i) w[i] = *reinterpret_cast<const float4*>(Ss + (ty + 16 * i) * TT_LD + k0);
+          for (int i = 0; i < MR; ++i) w[i] = *reinterpret_cast<const float4*>(wp + TT_WARPS * i * TA_PAGE + k0);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float4 x = ldf4(vp + (k0 + k) * TT_LD);
-          const uint64_t x0 = ta_two(x.x, x.y), x1 = ta_two(x.z, x.w);
+          for (int k = 0; k < 4; ++k) {
+            float x[CW];
+            tt_load(x, vp + (k0 + k) * VW);
 #pragma unroll
-          for (int i = 0; i < MR; ++i) {
-            const float y = k == 0 ? w[i].x : k == 1 ? w[i].y : k == 2 ? w[i].z : w[i].w;
-            const uint64_t y2 = ta_two(y, y);
-            if (whole || y != 0.f) {                         // what a row does not see stays out of it, whatever it holds
-              o[v][i][0] = ta_fma2(y2, x0, o[v][i][0]);
-              o[v][i][1] = ta_fma2(y2, x1, o[v][i][1]);
+            for (int i = 0; i < MR; ++i) {
+              const float y = k == 0 ? w[i].x : k == 1 ? w[i].y : k == 2 ? w[i].z : w[i].w;
+              if (decltype(seen)::value || y != 0.f) {       // what a row does not see stays out of it, whatever it holds
+#pragma unroll
+                for (int z = 0; z < CW; ++z) o[v][i][z] = fmaf(y, x[z], o[v][i][z]);
+              }
             }
           }
+        };
+        if (whole) {
+#pragma unroll 2
+          for (int k0 = 0; k0 < VT; k0 += 4) add(k0, std::true_type());
+        } else {
+#pragma unroll 1
+          for (int k0 = 0; k0 < VT; k0 += 4) add(k0, std::false_type());
         }
       }
     }
@@ -188,10 +231,10 @@ __device__ __forceinline__ void tt_item(const TreeAttn& a, const TreeItem& it, T
   const size_t pb = (static_cast<size_t>(blockIdx.x) * 2 + (it.first ? 1 : 0)) * TT_BM;
 #pragma unroll
   for (int i = 0; i < MR; ++i) {
-    const int row = ty + 16 * i, f = f0 + row, h = it.g * rep + f % rep, r = it.r0 + f / rep;
+    const int row = warp + TT_WARPS * i, f = f0 + row, h = it.g * rep + f % rep, r = it.r0 + f / rep;
     float sum = l[i], scale = 1.f;
 #pragma unroll
-    for (int x = 1; x < 16; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+    for (int x = 1; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
     if (row >= pairs) continue;
     if (done) {
       float c = 1.f;
@@ -202,30 +245,31 @@ __device__ __forceinline__ void tt_item(const TreeAttn& a, const TreeItem& it, T
       }
       scale = sum > 0.f ? ta_head_factor<T>(a, r, h) * c / sum : 0.f;
       if (sum != sum) scale = sum;
-    } else if (tx == 0) {
+    } else if (lane == 0) {
       a.part_ml[(pb + row) * 2] = m[i];
       a.part_ml[(pb + row) * 2 + 1] = sum;
     }
 #pragma unroll
     for (int v = 0; v < VP; ++v) {
-      const int col = v * 64 + tx * 4;
+      const int col = v * VW + lane * CW;
       if (col >= V) continue;
-      const float4 x = make_float4(ta_lo(o[v][i][0]) * scale, ta_hi(o[v][i][0]) * scale, ta_lo(o[v][i][1]) * scale, ta_hi(o[v][i][1]) * scale);
-      if (done) stf4(static_cast<T*>(a.out) + static_cast<size_t>(r) * a.ldo + static_cast<size_t>(h) * a.ho + col, x);
-      else *reinterpret_cast<float4*>(a.part_o + (pb + row) * V + col) = x;
+      T* out = static_cast<T*>(a.out) + static_cast<size_t>(r) * a.ldo + static_cast<size_t>(h) * a.ho + col;
+      float* part = a.part_o + (pb + row) * V + col;
+      if (done) tt_store(out, o[v][i], scale);
+      else tt_store(part, o[v][i], 1.f);
     }
   }
 }
 
-template <typename T, int VP>
-__global__ void __launch_bounds__(TT_THREADS, VP <= 2 ? 2 : 1)
+template <typename T, int VP, int CW>
+__global__ void __launch_bounds__(TT_THREADS, VP == 1 ? 2 : 1)
 tree_tile_kernel(const __grid_constant__ TreeAttn a) {
   extern __shared__ __align__(16) float smem_tt[];
   __shared__ TreeItem s_item;
   __shared__ int s_pos[TT_BM], s_first[TT_BM], s_at[TA_PAGE];
-  float* Qs = smem_tt;                                       // [64][D + 4]
-  float* Ss = Qs + TT_BM * ((a.D + 63) / 64 * 64 + 4);       // [64][68]
-  T* ring = reinterpret_cast<T*>(Ss + TT_BM * TT_LD);        // [3][64][68]
+  float* Qs = smem_tt;                                       // [64][D, in 64s]
+  float* Ss = Qs + TT_BM * ((a.D + 63) / 64 * 64);           // [64][64]
+  T* ring = reinterpret_cast<T*>(Ss + TT_BM * TA_PAGE);      // [3][64][68]
   const int t = threadIdx.x;
   pdl_wait();
   pdl_trigger();
@@ -243,9 +287,10 @@ tree_tile_kernel(const __grid_constant__ TreeAttn a) {
     const TreeItem it = s_item;
     if (it.nj == 0) break;
     const int pairs = it.n * (a.H / a.G) - it.rt * TT_BM;
-    if (pairs <= 16) tt_item<T, VP, 1>(a, it, ring, Qs, Ss, s_pos, s_first, s_at);
-    else if (pairs <= 32) tt_item<T, VP, 2>(a, it, ring, Qs, Ss, s_pos, s_first, s_at);
-    else tt_item<T, VP, 4>(a, it, ring, Qs, Ss, s_pos, s_first, s_at);
+    if (pairs <= 8) tt_item<T, VP, CW, 1>(a, it, ring, Qs, Ss, s_pos, s_first, s_at);
+    else if (pairs <= 16) tt_item<T, VP, CW, 2>(a, it, ring, Qs, Ss, s_pos, s_first, s_at);
+    else if (pairs <= 32) tt_item<T, VP, CW, 4>(a, it, ring, Qs, Ss, s_pos, s_first, s_at);
+    else tt_item<T, VP, CW, 8>(a, it, ring, Qs, Ss, s_pos, s_first, s_at);
   }
 }
 
@@ -394,10 +439,10 @@ tree_merge_kernel(const __grid_constant__ TreeAttn a) {
 
 constexpr int TA_SMEM = 220 * 1024;
 
-template <typename T, int VP>
+template <typename T, int VP, int CW>
 static int launch_tile(const TreeAttn& a, cudaStream_t s) {
-  auto kern = tree_tile_kernel<T, VP>;
-  const int smem = (TT_BM * ((a.D + 63) / 64 * 64 + 4) + TT_BM * TT_LD) * 4 + TT_STAGES * TT_PIECE * static_cast<int>(sizeof(T));
+  auto kern = tree_tile_kernel<T, VP, CW>;
+  const int smem = (TT_BM * ((a.D + 63) / 64 * 64) + TT_BM * TA_PAGE) * 4 + TT_STAGES * TT_PIECE * static_cast<int>(sizeof(T));
   if (smem > TA_SMEM) return -6;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, TA_SMEM) != cudaSuccess) return -4;
   spark_launch_pdl(kern, dim3(a.ctas), dim3(TT_THREADS), smem, s, dim3(1, 1, 1), a);
@@ -405,7 +450,7 @@ static int launch_tile(const TreeAttn& a, cudaStream_t s) {
 }
 template <typename T>
 static int launch_tiles(const TreeAttn& a, cudaStream_t s) {
-  return a.V <= 128 ? launch_tile<T, 2>(a, s) : a.V <= 256 ? launch_tile<T, 4>(a, s) : launch_tile<T, 8>(a, s);
+  return a.V <= 64 ? launch_tile<T, 1, 2>(a, s) : a.V <= 128 ? launch_tile<T, 1, 4>(a, s) : a.V <= 256 ? launch_tile<T, 2, 4>(a, s) : launch_tile<T, 4, 4>(a, s);
 }
 
 int launch_tree_tc(const TreeAttn& a, cudaStream_t s);       // tree_attn_tc.cu
