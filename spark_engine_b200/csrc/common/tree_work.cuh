@@ -173,4 +173,34 @@ __device__ __forceinline__ int ta_page(const TreeAttn& a, int slot, int j) {
   return p < a.n_pages ? p : -1;
 }
 
+// Bits b .. b + 63 of a row's ancestors.
+__device__ __forceinline__ uint64_t ta_ancestors(const TreeAttn& a, const TreeItem& sg, int node, int b) {
+  if (a.anc) {
+    const uint32_t* w = a.anc + static_cast<size_t>(sg.r0 + node) * a.words;
+    const int k = b >> 5, sh = b & 31;
+    const uint64_t w0 = k < a.words ? w[k] : 0u, w1 = k + 1 < a.words ? w[k + 1] : 0u, w2 = k + 2 < a.words ? w[k + 2] : 0u;
+    const uint64_t t = (w0 | w1 << 32) >> sh;
+    return sh ? t | w2 << (64 - sh) : t;
+  }
+  const int n = node - b + 1;
+  return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1;
+}
+// Which of the 64 tokens from tok0 on row `node` (position p) sees; near: its ancestors 0 .. 63.
+__device__ __forceinline__ uint64_t ta_mask(const TreeAttn& a, const TreeItem& sg, int tok0, int node, int p, uint64_t near) {
+  const int first = ta_first_visible(a, p), i0 = tok0 - sg.len;        // the page's token 0 is node i0
+  const int lo = min(max(first - tok0, 0), 64), hi = min(max(-i0, 0), 64);
+  uint64_t m = hi > lo ? (hi == 64 ? ~0ull : (1ull << hi) - 1) & ~(lo == 0 ? 0ull : (1ull << lo) - 1) : 0ull;
+  if (hi == 64) return m;
+  const int b0 = max(i0, 0);                                 // bit b of t: node b0 + b
+  uint64_t t = b0 == 0 ? near : sg.n <= 64 ? (b0 < 64 ? near >> b0 : 0ull) : ta_ancestors(a, sg, node, b0);
+  const int left = sg.n - b0;                                // nodes there are
+  if (left < 64) t &= left <= 0 ? 0ull : (1ull << left) - 1;
+  if (first > sg.len)                                        // ancestors outside the window or chunk
+    for (uint64_t x = t; x; x &= x - 1) {
+      const int b = __ffsll(x) - 1;
+      if (a.pos[sg.r0 + b0 + b] < first) t &= ~(1ull << b);
+    }
+  return m | t << hi;
+}
+
 }  // namespace spark

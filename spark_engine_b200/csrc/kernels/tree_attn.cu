@@ -42,11 +42,13 @@ __device__ __forceinline__ void tt_store(__nv_bfloat16* p, const float (&x)[2], 
   *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(x[0] * k, x[1] * k);
 }
 
+struct TtRows { uint64_t seen[TT_BM]; int pos[TT_BM], head[TT_BM], at[TA_PAGE]; };    // of a row: tokens of the page it sees, position, head
+
 // One item, 8 * MR rows: a warp has rows warp + 8 i, so that what is read of a row is the same for all lanes (one shared-memory cycle instead of
 // four); a lane has keys lane + 32 e of a page's scores and CW neighbouring columns in every 32 CW of the outputs.  Keys pass in pieces of 64
 // tokens x 64 channels, values in pieces of 4096 (128 channels, or 64 where there are no more), two of them on their way while one is worked on.
 template <typename T, int VP, int CW, int MR>
-__device__ __forceinline__ void tt_item(const TreeAttn& a, const TreeItem& it, T* ring, float* Qs, float* Ss, int* s_pos, int* s_first, int* s_at) {
+__device__ __forceinline__ void tt_item(const TreeAttn& a, const TreeItem& it, T* ring, float* Qs, float* Ss, TtRows& rows) {
   constexpr int VW = 32 * CW, VT = 4096 / VW;                // channels and tokens of a piece of values
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31, D = a.D, V = a.V, LDQ = (D + 63) / 64 * 64, rep = a.H / a.G;
   const int f0 = it.rt * TT_BM, pairs = min(TT_WARPS * MR, it.n * rep - f0), kc = (D + 63) >> 6, vc = (V + VW - 1) / VW;
@@ -89,31 +91,36 @@ __device__ __forceinline__ void tt_item(const TreeAttn& a, const TreeItem& it, T
     load(now == 0 ? TT_STAGES - 1 : now - 1);
     return ring + now * TT_PIECE;
   };
-#pragma unroll
-  for (int i = 0; i < TT_STAGES - 1; ++i) load(i);
+  int node = 0, pos = 0;                                     // of row t
+  uint64_t near = 0ull;
+  if (t < TT_WARPS * MR) {
+    const int f = f0 + min(t, pairs - 1);
+    node = f / rep;
+    pos = rows.pos[t] = a.pos[it.r0 + node];
+    rows.head[t] = it.g * rep + f - node * rep;
+    near = ta_ancestors(a, it, node, 0);
+  }
 #pragma unroll 1
-  for (int row = t >> 4; row < TT_WARPS * MR; row += 16)
+  for (int row = t >> 4; row < pairs; row += 16) {
+    const T* src = static_cast<const T*>(a.q) + static_cast<size_t>(it.r0 + (f0 + row) / rep) * a.ldq + static_cast<size_t>(it.g * rep + (f0 + row) % rep) * a.hq;
 #pragma unroll 1
     for (int c = (t & 15) * 4; c < D; c += 64)
-      *reinterpret_cast<float4*>(Qs + row * LDQ + c) = row < pairs ? ldf4(static_cast<const T*>(a.q) + static_cast<size_t>(it.r0 + (f0 + row) / rep) * a.ldq + static_cast<size_t>(it.g * rep + (f0 + row) % rep) * a.hq + c)
-                                                                  : make_float4(0.f, 0.f, 0.f, 0.f);
-  if (t < TT_WARPS * MR) {
-    const int p = t < pairs ? a.pos[it.r0 + (f0 + t) / rep] : 0;
-    s_pos[t] = p;
-    s_first[t] = ta_first_visible(a, p);
+      if (sizeof(T) == 4) tt_copy<16>(Qs + row * LDQ + c, src + c);
+      else *reinterpret_cast<float4*>(Qs + row * LDQ + c) = ldf4(src + c);
   }
+#pragma unroll 1
+  for (int i = 0; i < TT_STAGES - 1; ++i) load(i);
   float o[VP][MR][CW] = {};
-  float m[MR], l[MR];                                        // maximum, and this thread's share of the sum
-#pragma unroll
-  for (int i = 0; i < MR; ++i) { m[i] = -INFINITY; l[i] = 0.f; }
+  float m = -INFINITY, l = 0.f;                              // of the row warp + 8 lane: maximum and sum
 #pragma unroll 1
   for (int j = it.j; j < it.j + it.nj; ++j) {
     const int page = ta_page(a, it.slot, j), tok0 = j * TA_PAGE;
     const bool whole = page >= 0 && tok0 >= it.edge && tok0 + TA_PAGE <= it.len;
     if (page < 0 && t == 0) set_status(a.status, ST_BOUNDS, it.r0, tok0, it.slot);
-    if (t < TA_PAGE) {
-      const int node = tok0 + t - it.len;
-      s_at[t] = node < 0 ? tok0 + t : (node < it.n ? a.pos[it.r0 + node] : 0);
+    if (!whole && t < TT_WARPS * MR) rows.seen[t] = page >= 0 ? ta_mask(a, it, tok0, node, pos, near) : 0ull;
+    if ((a.bias || a.slopes) && t >= TT_THREADS - TA_PAGE) {
+      const int x = t - (TT_THREADS - TA_PAGE), n = tok0 + x - it.len;
+      rows.at[x] = n < 0 ? tok0 + x : n < it.n ? a.pos[it.r0 + n] : 0;
     }
     // ---- scores: even and odd channels apart
     uint64_t s2[MR][2] = {};
@@ -136,59 +143,57 @@ __device__ __forceinline__ void tt_item(const TreeAttn& a, const TreeItem& it, T
         }
       }
     }
-    float s[MR][2];
+    float* sw = Ss + warp * TA_PAGE;
 #pragma unroll
     for (int i = 0; i < MR; ++i)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) s[i][e] = (ta_lo(s2[i][e]) + ta_hi(s2[i][e])) * a.scale;
-    if (a.cap > 0.f)
+      for (int e = 0; e < 2; ++e) sw[i * TT_WARPS * TA_PAGE + lane + 32 * e] = (ta_lo(s2[i][e]) + ta_hi(s2[i][e])) * a.scale;
+    // ---- weights, row by row (little code: in short calls the first run of every instruction is what takes time)
+    float k = 1.f;                                           // of the row warp + 8 lane: what its outputs shrink by
+#pragma unroll 1
+    for (int i = 0, row = warp; row < pairs; ++i, row += TT_WARPS) {
+      float* sr = Ss + row * TA_PAGE + lane;
+      float x[2];
+      const int h = rows.head[row], p = rows.pos[row];
+      const uint64_t seen = whole ? ~0ull : rows.seen[row];
 #pragma unroll
-      for (int i = 0; i < MR; ++i) {
-        s[i][0] = a.cap * tanhf(s[i][0] / a.cap);
-        s[i][1] = a.cap * tanhf(s[i][1] / a.cap);
-      }
-    if (!whole || a.bias || a.slopes) {
-      const int valid = page < 0 ? 0 : min(TA_PAGE, it.len + it.n - tok0);
-#pragma unroll
-      for (int i = 0; i < MR; ++i) {
-        const int row = warp + TT_WARPS * i, f = f0 + min(row, pairs - 1), node = f / rep, h = it.g * rep + f - node * rep, p = s_pos[row], first = s_first[row];
-        const uint32_t* anc = a.anc ? a.anc + static_cast<size_t>(it.r0 + node) * a.words : nullptr;
-        const float slope = a.slopes ? a.slopes[h] : 0.f;
-        const float* bias = a.bias ? a.bias + static_cast<size_t>(h) * a.bias_n : nullptr;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int key = lane + 32 * e, at = s_at[key], kn = tok0 + key - it.len;
-          if (bias) s[i][e] += bias[min(max(p - at, 0), a.bias_n - 1)];
-          if (a.slopes) s[i][e] -= slope * static_cast<float>(p - at);
-          bool on = whole || (key < valid && at >= first);
-          if (on && kn >= 0) on = anc ? (kn >> 5) < a.words && (anc[kn >> 5] >> (kn & 31)) & 1u : kn <= node;
-          if (!on) s[i][e] = -INFINITY;
+      for (int e = 0; e < 2; ++e) {
+        x[e] = sr[32 * e];
+        if (a.cap > 0.f) x[e] = a.cap * tanhf(x[e] / a.cap);
+        if (a.bias || a.slopes) {
+          const int dist = p - rows.at[lane + 32 * e];
+          if (a.bias) x[e] += a.bias[static_cast<size_t>(h) * a.bias_n + min(max(dist, 0), a.bias_n - 1)];
+          if (a.slopes) x[e] -= a.slopes[h] * static_cast<float>(dist);
         }
+        if (!(seen >> (lane + 32 * e) & 1ull)) x[e] = -INFINITY;
+      }
+      const float m0 = __shfl_sync(0xffffffffu, m, i);
+      float top = fmaxf(fmaxf(x[0], x[1]), m0);
+#pragma unroll
+      for (int z = 1; z < 32; z <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, z));
+      const float ref = top == -INFINITY ? 0.f : top;
+      x[0] = expf(x[0] - ref);
+      x[1] = expf(x[1] - ref);
+      sr[0] = x[0];
+      sr[32] = x[1];
+      float sum = x[0] + x[1];
+#pragma unroll
+      for (int z = 1; z < 32; z <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, z);
+      if (lane == i) {
+        k = expf(m0 - ref);
+        l = l * k + sum;
+        m = top;
       }
     }
-    // ---- weights
+    if (__any_sync(0xffffffffu, k != 1.f))
 #pragma unroll
-    for (int i = 0; i < MR; ++i) {
-      float top = fmaxf(fmaxf(s[i][0], s[i][1]), m[i]);
-#pragma unroll
-      for (int x = 1; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-      const float ref = top == -INFINITY ? 0.f : top;
-      if (top != m[i]) {                                     // (the same for the whole warp)
-        const float k = expf(m[i] - ref);
-        l[i] *= k;
+      for (int i = 0; i < MR; ++i) {
+        const float ki = __shfl_sync(0xffffffffu, k, i);
 #pragma unroll
         for (int v = 0; v < VP; ++v)
 #pragma unroll
-          for (int x = 0; x < CW; ++x) o[v][i][x] *= k;
-        m[i] = top;
+          for (int x = 0; x < CW; ++x) o[v][i][x] *= ki;
       }
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float w = expf(s[i][e] - ref);
-        l[i] += w;
-        Ss[(warp + TT_WARPS * i) * TA_PAGE + lane + 32 * e] = w;
-      }
-    }
     __syncwarp();                                            // (a row's weights stay in its warp)
 #pragma unroll
     for (int v = 0; v < VP; ++v) {
@@ -229,33 +234,36 @@ __device__ __forceinline__ void tt_item(const TreeAttn& a, const TreeItem& it, T
   const bool done = it.first && it.last;
   if (it.first && !it.last && t == 0) ta_set_split(a, ta_split(a, it));
   const size_t pb = (static_cast<size_t>(blockIdx.x) * 2 + (it.first ? 1 : 0)) * TT_BM;
-#pragma unroll
-  for (int i = 0; i < MR; ++i) {
-    const int row = warp + TT_WARPS * i, f = f0 + row, h = it.g * rep + f % rep, r = it.r0 + f / rep;
-    float sum = l[i], scale = 1.f;
-#pragma unroll
-    for (int x = 1; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-    if (row >= pairs) continue;
+  float scale = 1.f;                                         // of the row warp + 8 lane
+  const int mine = warp + TT_WARPS * lane;
+  if (lane < MR && mine < pairs) {
     if (done) {
+      const int h = rows.head[mine];
       float c = 1.f;
       if (a.sink) {
-        const float top = fmaxf(m[i], a.sink[h]);
-        c = expf(m[i] - top);
-        sum = sum * c + expf(a.sink[h] - top);
+        const float top = fmaxf(m, a.sink[h]);
+        c = expf(m - top);
+        l = l * c + expf(a.sink[h] - top);
       }
-      scale = sum > 0.f ? ta_head_factor<T>(a, r, h) * c / sum : 0.f;
-      if (sum != sum) scale = sum;
-    } else if (lane == 0) {
-      a.part_ml[(pb + row) * 2] = m[i];
-      a.part_ml[(pb + row) * 2 + 1] = sum;
+      scale = l > 0.f ? ta_head_factor<T>(a, it.r0 + (f0 + mine) / rep, h) * c / l : 0.f;
+      if (l != l) scale = l;
+    } else {
+      *reinterpret_cast<float2*>(a.part_ml + (pb + mine) * 2) = make_float2(m, l);
     }
+  }
+#pragma unroll
+  for (int i = 0; i < MR; ++i) {
+    const int row = warp + TT_WARPS * i;
+    if (row >= pairs) break;
+    const int h = rows.head[row], r = it.r0 + (f0 + row) / rep;
+    const float by = __shfl_sync(0xffffffffu, scale, i);
 #pragma unroll
     for (int v = 0; v < VP; ++v) {
       const int col = v * VW + lane * CW;
       if (col >= V) continue;
       T* out = static_cast<T*>(a.out) + static_cast<size_t>(r) * a.ldo + static_cast<size_t>(h) * a.ho + col;
       float* part = a.part_o + (pb + row) * V + col;
-      if (done) tt_store(out, o[v][i], scale);
+      if (done) tt_store(out, o[v][i], by);
       else tt_store(part, o[v][i], 1.f);
     }
   }
@@ -266,7 +274,7 @@ __global__ void __launch_bounds__(TT_THREADS, VP == 1 ? 2 : 1)
 tree_tile_kernel(const __grid_constant__ TreeAttn a) {
   extern __shared__ __align__(16) float smem_tt[];
   __shared__ TreeItem s_item;
-  __shared__ int s_pos[TT_BM], s_first[TT_BM], s_at[TA_PAGE];
+  __shared__ TtRows rows;
   float* Qs = smem_tt;                                       // [64][D, in 64s]
   float* Ss = Qs + TT_BM * ((a.D + 63) / 64 * 64);           // [64][64]
   T* ring = reinterpret_cast<T*>(Ss + TT_BM * TA_PAGE);      // [3][64][68]
@@ -287,10 +295,10 @@ tree_tile_kernel(const __grid_constant__ TreeAttn a) {
     const TreeItem it = s_item;
     if (it.nj == 0) break;
     const int pairs = it.n * (a.H / a.G) - it.rt * TT_BM;
-    if (pairs <= 8) tt_item<T, VP, CW, 1>(a, it, ring, Qs, Ss, s_pos, s_first, s_at);
-    else if (pairs <= 16) tt_item<T, VP, CW, 2>(a, it, ring, Qs, Ss, s_pos, s_first, s_at);
-    else if (pairs <= 32) tt_item<T, VP, CW, 4>(a, it, ring, Qs, Ss, s_pos, s_first, s_at);
-    else tt_item<T, VP, CW, 8>(a, it, ring, Qs, Ss, s_pos, s_first, s_at);
+    if (pairs <= 8) tt_item<T, VP, CW, 1>(a, it, ring, Qs, Ss, rows);
+    else if (pairs <= 16) tt_item<T, VP, CW, 2>(a, it, ring, Qs, Ss, rows);
+    else if (pairs <= 32) tt_item<T, VP, CW, 4>(a, it, ring, Qs, Ss, rows);
+    else tt_item<T, VP, CW, 8>(a, it, ring, Qs, Ss, rows);
   }
 }
 

@@ -98,36 +98,6 @@ __device__ __forceinline__ bool tc_sync(uint64_t* bar, uint32_t& phase) {
 struct TcCount { int slot = 0; uint32_t ph = 0; };
 template <int N> __device__ __forceinline__ void tc_step(TcCount& c) { if (++c.slot == N) { c.slot = 0; c.ph ^= 1; } }
 
-// Bits b .. b + 63 of a row's ancestors.
-__device__ __forceinline__ uint64_t tc_ancestors(const TreeAttn& a, const TreeItem& sg, int node, int b) {
-  if (a.anc) {
-    const uint32_t* w = a.anc + static_cast<size_t>(sg.r0 + node) * a.words;
-    const int k = b >> 5, sh = b & 31;
-    const uint64_t w0 = k < a.words ? w[k] : 0u, w1 = k + 1 < a.words ? w[k + 1] : 0u, w2 = k + 2 < a.words ? w[k + 2] : 0u;
-    const uint64_t t = (w0 | w1 << 32) >> sh;
-    return sh ? t | w2 << (64 - sh) : t;
-  }
-  const int n = node - b + 1;
-  return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1;
-}
-// Which of the 64 tokens from tok0 on row `node` (position p) sees; near: its ancestors 0 .. 63.
-__device__ __forceinline__ uint64_t tc_mask(const TreeAttn& a, const TreeItem& sg, int tok0, int node, int p, uint64_t near) {
-  const int first = ta_first_visible(a, p), i0 = tok0 - sg.len;        // the page's token 0 is node i0
-  const int lo = min(max(first - tok0, 0), 64), hi = min(max(-i0, 0), 64);
-  uint64_t m = hi > lo ? (hi == 64 ? ~0ull : (1ull << hi) - 1) & ~(lo == 0 ? 0ull : (1ull << lo) - 1) : 0ull;
-  if (hi == 64) return m;
-  const int b0 = max(i0, 0);                                 // bit b of t: node b0 + b
-  uint64_t t = b0 == 0 ? near : sg.n <= 64 ? (b0 < 64 ? near >> b0 : 0ull) : tc_ancestors(a, sg, node, b0);
-  const int left = sg.n - b0;                                // nodes there are
-  if (left < 64) t &= left <= 0 ? 0ull : (1ull << left) - 1;
-  if (first > sg.len)                                        // ancestors outside the window or chunk
-    for (uint64_t x = t; x; x &= x - 1) {
-      const int b = __ffsll(x) - 1;
-      if (a.pos[sg.r0 + b0 + b] < first) t &= ~(1ull << b);
-    }
-  return m | t << hi;
-}
-
 // grid: a.ctas.  FEAT: soft cap, distance bias or slopes, or a scale that is not positive (the scaled scores are then masked, not the products).
 template <int DC, int NQ, bool FEAT>
 __global__ void __launch_bounds__(Tc<DC, NQ>::THREADS, Tc<DC, NQ>::PER_SM)
@@ -342,7 +312,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       const int f = (it.rt << a.bm_log) + q * 128 + min(row, pairs - 1), node = f / rep, h = it.g * rep + f - node * rep, pr = sg.r0 + node;
       const bool idle = quad * 32 >= pairs;                  // a warp without rows keeps the pace and computes nothing
       const int p = a.pos[pr];
-      const uint64_t near = tc_ancestors(a, sg, node, 0);    // (asked for long before the tree's page)
+      const uint64_t near = ta_ancestors(a, sg, node, 0);    // (asked for long before the tree's page)
       {                                                      // the row's query; columns from D on are zero
         const uint4* src = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) + static_cast<size_t>(pr) * a.ldq + static_cast<size_t>(h) * a.hq);
         const int units = row < pairs ? a.D / 8 : 0;
@@ -385,7 +355,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         uint64_t seen = ~0ull;
         int at_lo = tok0 + lane, at_hi = at_lo + 32;           // FEAT: positions of the page's tokens `lane` and 32 + lane
         if (!whole && !idle) {
-          seen = page ? tc_mask(a, sg, tok0, node, p, near) : 0ull;
+          seen = page ? ta_mask(a, sg, tok0, node, p, near) : 0ull;
           if (FEAT && tok0 + TA_PAGE > sg.len) {
             const int n0 = tok0 + lane - sg.len, n1 = n0 + 32;
             if (n0 >= 0) at_lo = n0 < sg.n ? a.pos[sg.r0 + n0] : p;
