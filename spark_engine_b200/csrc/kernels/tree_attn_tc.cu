@@ -4,18 +4,24 @@
 //   warp 1      issues S = Q K^T one page ahead of O += P V (P in tensor memory): as soon as the softmax warps have loaded a page's scores
 //   the others  softmax, one row per thread: 64 scores are one tensor-memory load, statistics stay in the thread
 // NQ = 2: two tiles of 128 rows with their own issuing and softmax warps share the keys in shared memory (large trees: a page is read once for
-// 256 rows).  Each tile's products wait for its own softmax alone: with one issuing warp for both, a page took 2.0 us instead of ...
+// 256 rows); each tile's products wait for its own softmax alone.
 //
 // Weights are exponentials against a reference that may lag far behind the maximum: the maximum of the first page that a row sees, renewed
 // (and the accumulator rescaled) only when a page's weights add up to more than 2^40; fp32 sums and bf16 weights lose nothing by a common
-// factor.  So most pages need no maximum.  Weights enter the product as two bf16 terms (2^-17 of a weight is lost) where reading the keys takes longer than the
-// products (NQ = 1), and as one (half a step of bf16 each, at random, less than the step that the outputs are rounded to) where it does not:
-// for 256 rows the second term would be a third of all products.  One-term weights have two places, so that a page's weights need not wait
-// for the product of the page before.
+// factor.  So most pages need no maximum.  Weights enter the product as two bf16 terms (2^-17 of a weight is lost) where reading the keys
+// takes longer than the products (NQ = 1), and as one (half a step of bf16 each, at random, less than the step that the outputs are rounded to)
+// where it does not: for 256 rows the second term would be a third of all products.  One-term weights have two places, so that a page's
+// weights need not wait for the product of the page before.
 //
 // A page that not every row sees whole (the tree itself, the edge of a window or chunk) is masked by 64 bits per row.  Warp 1 looks its values
 // over first: rows that hold no token of the request are zeroed, and where a value is not finite, 0 * value would spoil the rows that do not
 // see it, so the softmax warps add it by hand for the rows that do and zero it in front of the product.
+//
+// What bounds it (kernel time, inputs from HBM): few rows over long caches stream at 6.1 TB/s between the first page and the last, about 8 us
+// after the launch (four requests of 16 nodes over 16k tokens, two heads of 256 of 8 each: 132 MB in 41 us); 256 rows are bound by the products and
+// the exponentials of a page, 1024 clocks each, which overlap in part (64 requests of 64 nodes over 4k tokens, 8 heads of 128 of 4 each: 272 GFLOP
+// in 308 us).  Short calls are the latency of what is done once: 10 us for 8 nodes over 900 tokens.  What did not pay: the two tiles' softmax
+// in turn (412 us instead of 363), results through shared memory (no change), an earlier start of the second launch (no change).
 #include "../common/tree_work.cuh"
 
 namespace spark {

