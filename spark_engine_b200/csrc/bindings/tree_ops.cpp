@@ -72,6 +72,11 @@ void need_tables(const Tensor& t) {
 int* ip(const Tensor& t) { return t.numel() ? static_cast<int*>(t.data_ptr()) : nullptr; }
 int* ip(const Opt& t) { return t ? ip(*t) : nullptr; }
 int64_t quantum(const Tensor& t) { return 16 / t.element_size(); }
+bool strides_fit(const Tensor& t) {               // the kernels take strides of rows and heads in 32 bits
+  for (const int64_t s : t.strides())
+    if (s >= 1ll << 31) return false;
+  return true;
+}
 bool aligned(const Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0; }
 
 struct Cache { int64_t page, tok, width; };      // strides and a token's channels, in elements
@@ -84,9 +89,10 @@ Cache need_cache(const char* name, const Tensor& t, at::ScalarType dtype, const 
     want *= t.size(i);
   }
   const int64_t e = quantum(t);
-  NEED(want > 0 && want % e == 0 && t.stride(0) % e == 0 && t.stride(1) % e == 0 && t.stride(1) >= want && aligned(t), name, ": tokens must start on 16 bytes");
+  NEED(want > 0 && want % e == 0 && (t.size(0) < 2 || t.stride(0) % e == 0) && t.stride(1) % e == 0 && t.stride(1) >= want && aligned(t), name, ": tokens must start on 16 bytes");
   NEED(t.size(0) <= 1 << 24, name, " has more than 2^24 pages");
-  return {t.stride(0), t.stride(1), want};
+  NEED(t.size(0) < 2 || t.stride(0) >= want, name, ": pages must not overlap");
+  return {t.size(0) < 2 ? spark::TREE_PAGE * t.stride(1) : t.stride(0), t.stride(1), want};
 }
 bool is_act(at::ScalarType t) { return t == at::kBFloat16 || t == at::kFloat; }
 
@@ -181,9 +187,11 @@ Tensor path_conv(Tensor x, const Tensor& w, const Tensor& tail, const RowMaps& m
   NEED(k.size(0) == v.size(0), "k and v must have the same pages");
   NEED(nq >= 0 && nq + kc.width + vc.width == C, "a row's ", C, " channels are not ", nq, " of queries, ", kc.width, " of keys and ", vc.width, " of values");
   NEED(nq % 8 == 0 && kc.width % 8 == 0 && C % 8 == 0, "channels must be multiples of 8");
+  NEED(R <= 65535 * 64, "at most 65535 tiles of 64 rows");
   Tensor q = at::empty({R, nq}, x.options());
   if (!run || R == 0) return q;
-  if (x.stride(1) != 1 || x.stride(0) % 8 || !aligned(x)) x = x.contiguous();
+  NEED(k.size(0) > 0, "caches without pages");
+  if (x.stride(1) != 1 || x.stride(0) % 8 || !aligned(x) || !strides_fit(x)) x = x.contiguous();
   const On on(x);
   spark::PathConv a{x.data_ptr(), static_cast<float*>(w.data_ptr()), tail.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), ip(m.slot), ip(m.index),
                     ip(m.parents), static_cast<long long*>(m.cache_row.data_ptr()), on.dev.status, kc.page, kc.tok, vc.page, vc.tok,
@@ -211,6 +219,7 @@ Tensor tree_attention(Tensor q, const Tensor& k, const Tensor& v, const RowMaps&
        "caches must be [pages, ", spark::TREE_PAGE, ", heads, channels], keys as wide as queries");
   const int64_t G = k.size(2), V = v.size(3);
   NEED(H > 0 && H % G == 0, "query heads must be a multiple of the key / value heads");
+  NEED(R * H < 1ll << 31, "at most 2^31 rows of heads");
   NEED(D % 8 == 0 && V % 8 == 0 && D <= MAX_HEAD && V <= MAX_HEAD, "head widths must be multiples of 8 up to ", MAX_HEAD);
   NEED(R == m.rows() && m.slot.device() == dev, "the maps are another round's");
   NEED(window >= 0 && chunk >= 0 && !(window && chunk) && window < 1ll << 31 && chunk < 1ll << 31, "either a window or a chunk");
@@ -218,18 +227,20 @@ Tensor tree_attention(Tensor q, const Tensor& k, const Tensor& v, const RowMaps&
   need_heads("bias", bias, 2, H, dev);
   need_heads("slopes", slopes, 1, H, dev);
   need_heads("sink", sink, 1, H, dev);
-  NEED(!gate || (gate->dim() == 2 && gate->size(0) == R && gate->size(1) == H && gate->scalar_type() == dt && gate->device() == dev && gate->stride(1) == 1),
+  NEED(!gate || (gate->dim() == 2 && gate->size(0) == R && gate->size(1) == H && gate->scalar_type() == dt && gate->device() == dev && gate->stride(1) == 1 && strides_fit(*gate)),
        "gate must be [rows, heads] in the queries' type");
   const int64_t e = quantum(q);
   if (given)
     NEED(given->dim() == 3 && given->size(0) == R && given->size(1) == H && given->size(2) == V && given->scalar_type() == dt && given->device() == dev &&
-             given->stride(2) == 1 && given->stride(0) % e == 0 && given->stride(1) % e == 0 && aligned(*given),
-         "out must be [rows, heads, value channels] in the queries' type, heads on 16 bytes");
+             given->stride(2) == 1 && given->stride(0) % e == 0 && given->stride(1) % e == 0 && aligned(*given) && strides_fit(*given) &&
+             (H < 2 || given->stride(1) >= V) && (R < 2 || given->stride(0) >= V),
+         "out must be [rows, heads, value channels] in the queries' type, heads apart and on 16 bytes");
   Tensor out = given ? *given : at::empty({R, H, V}, q.options());
   if (!run || R == 0) return out;
   const int64_t S = m.lengths.size(0);
   if (S == 0) return given ? out : out.zero_();
-  if (q.stride(2) != 1 || q.stride(0) % e || q.stride(1) % e || !aligned(q)) q = q.contiguous();
+  NEED(k.size(0) > 0, "caches without pages");
+  if (q.stride(2) != 1 || q.stride(0) % e || q.stride(1) % e || !aligned(q) || !strides_fit(q)) q = q.contiguous();
   const On on(q);
   // Tensor cores: tiles of 128 (node, head) rows, two CTAs per SM; or, where a request may have more of them, two tiles per CTA that share
   // the keys, one CTA per SM.  Heads wider than 128 leave room for one tile and one CTA.

@@ -48,9 +48,11 @@ static __device__ __noinline__ TreeSeg ta_segment(const TreeAttn& a, int s) {
   TreeSeg t;
   t.r0 = a.starts[s];
   t.n = a.starts[s + 1] - t.r0;
-  t.len = max(a.lengths[s], 0);
-  t.j0 = ta_first_visible(a, t.len) / TA_PAGE;
-  t.nt = (t.len + t.n + TA_PAGE - 1) / TA_PAGE - t.j0;
+  const int most = a.page_ld * TA_PAGE;                      // (what lies behind the table's last page is not there)
+  t.len = min(max(a.lengths[s], 0), most);
+  if (t.n > 0 && t.len + t.n > most) set_status(a.status, ST_BOUNDS, t.r0, t.len + t.n, most);
+  t.j0 = min(ta_first_visible(a, t.len) / TA_PAGE, a.page_ld - 1);
+  t.nt = max(min((t.len + t.n + TA_PAGE - 1) / TA_PAGE, a.page_ld) - t.j0, 1);
   t.rts = t.n > 0 ? (t.n * (a.H / a.G) + (1 << a.bm_log) - 1) >> a.bm_log : 0;
   return t;
 }
@@ -163,6 +165,15 @@ __device__ __forceinline__ int4 ta_split(const TreeAttn& a, const TreeItem& it) 
 __device__ __forceinline__ void ta_set_split(const TreeAttn& a, int4 v) { reinterpret_cast<int4*>(a.split)[blockIdx.x] = v; }
 __device__ __forceinline__ int4 ta_get_split(const TreeAttn& a, int c) { return __ldcg(reinterpret_cast<const int4*>(a.split) + c); }
 
+// exponential of the outputs' accuracy
+template <typename T> __device__ __forceinline__ float ta_exp(float x) { return sizeof(T) == 2 ? __expf(x) : expf(x); }
+// The sum of a row (against its maximum m) with a sink; what its outputs shrink by.
+template <typename T>
+__device__ __forceinline__ float ta_sink(float sink, float m, float& l) {
+  const float top = fmaxf(m, sink), ref = top == -INFINITY ? 0.f : top, k = ta_exp<T>(m - ref);
+  l = l * k + ta_exp<T>(sink - ref);
+  return k;
+}
 template <typename T>
 __device__ __forceinline__ float ta_head_factor(const TreeAttn& a, int row, int h) {
   return a.gate ? a.out_scale * sigmoid_f(ldf(static_cast<const T*>(a.gate) + static_cast<size_t>(row) * a.ldg + h)) : a.out_scale;

@@ -242,12 +242,7 @@ __device__ __forceinline__ void tt_item(const TreeAttn& a, const TreeItem& it, T
   if (lane < MR && mine < pairs) {
     if (done) {
       const int h = rows.head[mine];
-      float c = 1.f;
-      if (a.sink) {
-        const float top = fmaxf(m, a.sink[h]);
-        c = expf(m - top);
-        l = l * c + expf(a.sink[h] - top);
-      }
+      const float c = a.sink ? ta_sink<T>(a.sink[h], m, l) : 1.f;
       scale = l > 0.f ? ta_head_factor<T>(a, it.r0 + (f0 + mine) / rep, h) * c / l : 0.f;
       if (l != l) scale = l;
     } else {
@@ -306,9 +301,6 @@ tree_tile_kernel(const __grid_constant__ TreeAttn a) {
 }
 
 // ------------------------------------------------------------------------------------------------ merge
-// exponential of the outputs' accuracy
-template <typename T> __device__ __forceinline__ float tm_exp(float x) { return sizeof(T) == 2 ? __expf(x) : expf(x); }
-
 constexpr int TM_THREADS = 256, TM_WARPS = TM_THREADS / 32, TM_MAX_CTAS = 1024;
 
 // Every CTA makes the list of the split items' rows (a row per item that begins in one CTA of the first launch and ends in another) and
@@ -379,14 +371,14 @@ tree_merge_kernel(const __grid_constant__ TreeAttn a) {
           if (i < parts && lane + v * 32 < V4) x[u][v] = __ldcg(reinterpret_cast<const float4*>(a.part_o + part(i) * a.V) + lane + v * 32);
       }
       const float top = fmaxf(m, fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x))), ref = top == -INFINITY ? 0.f : top;
-      const float k = tm_exp<T>(m - ref);
+      const float k = ta_exp<T>(m - ref);
       m = top;
       l *= k;
 #pragma unroll
       for (int v = 0; v < VC; ++v) { o[v].x *= k; o[v].y *= k; o[v].z *= k; o[v].w *= k; }
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        const float w = tm_exp<T>(ml[u].x - ref);
+        const float w = ta_exp<T>(ml[u].x - ref);
         if (w == 0.f && ml[u].y == ml[u].y) continue;        // (a part of NaN scores alone stays)
         l = fmaf(w, ml[u].y, l);
 #pragma unroll
@@ -406,13 +398,13 @@ tree_merge_kernel(const __grid_constant__ TreeAttn a) {
       __syncthreads();
       if (sub == 0) {
         for (int i = 1; i < wpr; ++i) m = fmaxf(m, s_ml[warp + i][0]);
-        const float ref = m == -INFINITY ? 0.f : m, c0 = tm_exp<T>(s_ml[warp][0] - ref);
+        const float ref = m == -INFINITY ? 0.f : m, c0 = ta_exp<T>(s_ml[warp][0] - ref);
         l *= c0;
 #pragma unroll
         for (int v = 0; v < VC; ++v) { o[v].x *= c0; o[v].y *= c0; o[v].z *= c0; o[v].w *= c0; }
 #pragma unroll 1
         for (int i = 1; i < wpr; ++i) {
-          const float w = tm_exp<T>(s_ml[warp + i][0] - ref);
+          const float w = ta_exp<T>(s_ml[warp + i][0] - ref);
           if (w == 0.f && s_ml[warp + i][1] == s_ml[warp + i][1]) continue;
           l = fmaf(w, s_ml[warp + i][1], l);
 #pragma unroll
@@ -426,12 +418,7 @@ tree_merge_kernel(const __grid_constant__ TreeAttn a) {
     }
     if (!on || sub) continue;
     const int f = sp.w + row, h = sp.z * rep + f % rep, r = sp.y + f / rep;
-    float k = 1.f;
-    if (a.sink) {
-      const float M = fmaxf(m, a.sink[h]);
-      k = tm_exp<T>(m - M);
-      l = l * k + tm_exp<T>(a.sink[h] - M);
-    }
+    const float k = a.sink ? ta_sink<T>(a.sink[h], m, l) : 1.f;
     float scale = l > 0.f ? ta_head_factor<T>(a, r, h) * k / l : 0.f;
     if (l != l) scale = l;
 #pragma unroll

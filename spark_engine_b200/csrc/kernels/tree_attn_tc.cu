@@ -580,11 +580,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       const size_t pb = ((static_cast<size_t>(blockIdx.x) * 2 + (it.first ? 1 : 0)) << a.bm_log) + q * 128 + row;
       float k = 1.f;
       if (done) {
-        if (a.sink) {
-          const float M = fmaxf(m, a.sink[h]);
-          k = __expf(m - M);
-          l = l * k + __expf(a.sink[h] - M);
-        }
+        if (a.sink) k = ta_sink<__nv_bfloat16>(a.sink[h], m, l);
         k = l > 0.f ? ta_head_factor<__nv_bfloat16>(a, pr, h) * k / l : 0.f;
         if (l != l) k = l;
       } else if (row < pairs) {

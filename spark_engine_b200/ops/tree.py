@@ -5,6 +5,8 @@ A round's rows are the requests' rows one after another: request s brings counts
 request's token lengths[s] + j.  In a tree, parents[row] is the parent's index within the request (-1: hangs off the committed tokens),
 below the row's own; a row's position is lengths[s] plus its depth, and it sees the committed tokens, its ancestors and itself.  Without
 parents the rows are chains.  Lengths, counts, parents, tables and paths live on the device: a captured round may be replayed with others.
+The maps refer to lengths, tables, slots and parents, which have to stay as they are until the round is committed; requests of one round
+have different slots, and pages that only one of them writes to.
 
 The calls neither wait for the device nor read from it.  What they can only find out there (a missing page, a parent behind its child, a
 path that does not ascend) skips the row, or the request in `commit_paths`, and sets the device status word."""
@@ -268,7 +270,8 @@ def _plain_attention(q, k, v, maps, scale, softcap, bias, slopes, sink, window, 
 def commit_paths(maps: "RowMaps", path, n_path, caches: Sequence[torch.Tensor], tails: Sequence[Tuple[torch.Tensor, torch.Tensor]] = ()):
     """Keep the accepted rows of every request: path [S, P] int32, its first n_path[s] entries the accepted rows' indices in ascending order
     (0: nothing happens to the request).  In every cache [pages, 64, ...] row path[i] of the request moves to its token length + i, and each
-    tail [slots, kept, C] of `tails` = [(x [R, C], tail), ...] becomes the last `kept` of (tail, accepted rows of x)."""
+    tail [slots, kept, C] of `tails` = [(x [R, C], tail), ...] becomes the last `kept` of (tail, accepted rows of x).  No two of the
+    caches and tails may share memory."""
     run = _kernels(maps.tables)
     calls = _native().commit_paths(maps, path, n_path, caches, tails, run)
     if run:

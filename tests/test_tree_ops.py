@@ -245,6 +245,30 @@ def test_attention_refuses(over):
         ops.tree_attention(**_args(**over))
 
 
+@pytest.mark.parametrize("over", [
+    dict(out=lambda d: torch.zeros(5, 1, 8).expand(5, 4, 8)), dict(out=lambda d: torch.zeros(1, 4, 8).expand(5, 4, 8)),
+    dict(k=lambda d: d["k"][:1].expand_as(d["k"])), dict(v=lambda d: d["v"][:1].expand_as(d["v"])),
+])
+def test_attention_refuses_memory_that_overlaps(over):
+    with pytest.raises(ValueError):
+        ops.tree_attention(**_args(**over))
+
+
+def check_sink_of_nothing(device, dtype):
+    """A sink may be -inf: a row that sees nothing is still zero."""
+    r = U.Round([0, 70], [3, 2], device=device)
+    q, k, v = r.randn(r.R, 4, 64, dtype=dtype), r.randn(r.n_pages, 64, 2, 64, dtype=dtype), r.randn(r.n_pages, 64, 2, 64, dtype=dtype)
+    m = ops.slot_maps(**r.inputs())
+    want = ops.tree_attention(q, k, v, m, 0.1)
+    m.anc[1].zero_()
+    got = ops.tree_attention(q, k, v, m, 0.1, sink=torch.full((4,), -float("inf"), device=device))
+    assert not got[1].any() and torch.equal(got[[0, 2, 3, 4]], want[[0, 2, 3, 4]])
+
+
+def test_sink_of_nothing():
+    check_sink_of_nothing("cpu", torch.float32)
+
+
 def test_maps_and_tables_refuse():
     r = U.Round([70, 9], [5, 6])
     good = r.inputs()

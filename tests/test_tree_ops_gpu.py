@@ -105,6 +105,13 @@ def test_attention_of_sizes(name, dtype):
     T.check_attention(U.Round(**r, device=DEV), *heads, dtype, {}, rounded=WEIGHTS[dtype])
 
 
+@pytest.mark.parametrize("nodes", [1, 4, 10, 17, 45])     # of 3 query heads: tiles of 8, 16, 32 and 64 rows, and two of them
+@pytest.mark.parametrize("D,V", [(64, 48), (136, 128), (40, 256), (264, 512), (512, 64)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_attention_of_tiles(D, V, nodes, dtype):
+    T.check_attention(U.Round([150, 64], [nodes, 2], device=DEV), 6, 2, D, V, dtype, {}, rounded=WEIGHTS[dtype])
+
+
 @pytest.mark.parametrize("layout", ["plain", "interleaved"])
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("name", list(T.FEATURES))
@@ -158,6 +165,26 @@ def test_missing_pages_are_not_read(dtype):
         assert torch.equal(ops.tree_attention(q, k, v, m, 0.1, window=70), want)          # outside the window
         assert torch.isfinite(ops.tree_attention(q, k, v, m, 0.1)).all()
         expect_status()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_sink_of_nothing(dtype):
+    T.check_sink_of_nothing(DEV, dtype)
+
+
+@pytest.mark.parametrize("length", [200, 1 << 20, (1 << 31) - 1])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_lengths_beyond_the_table(dtype, length):
+    r = U.Round([150, 90], [6, 4], device=DEV)
+    q, k, v = r.randn(r.R, 4, 64, dtype=dtype), r.randn(r.n_pages, 64, 2, 64, dtype=dtype), r.randn(r.n_pages, 64, 2, 64, dtype=dtype)
+    want = ops.tree_attention(q, k, v, ops.slot_maps(**r.inputs()), 0.1)
+    d = r.inputs()
+    d["lengths"] = torch.tensor([length, 90], dtype=torch.int32, device=DEV)          # the table has three pages
+    m = ops.slot_maps(**d)
+    expect_status()
+    got = ops.tree_attention(q, k, v, m, 0.1)
+    expect_status()
+    assert torch.isfinite(got).all() and torch.equal(got[6:], want[6:])
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
