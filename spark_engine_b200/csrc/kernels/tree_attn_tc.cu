@@ -29,20 +29,19 @@ namespace spark {
 int make_tmap_page(CUtensorMap* m, const void* base, uint64_t pages, uint64_t G, uint64_t D, uint64_t tok, uint64_t page);
 
 constexpr float TC_MOST = 1099511627776.f;                   // 2^40
-// Items announced at a time: an item has two slots of the ring at least, so that the one whose place is taken again has been read long ago.
-constexpr int TC_ITEMS = 16;
+constexpr int TC_ITEMS = 16;                                 // items announced at a time
 
 template <int DC, int NQ> struct Tc {
   static constexpr bool QT = DC == 256;                      // queries in tensor memory: shared memory has no room for them beside the ring
   static constexpr int SLOT = TA_PAGE * DC * 2, Q_BYTES = QT ? 0 : 128 * DC * 2;
   static constexpr int SLOTS = DC == 256 ? 6 : DC == 128 ? (NQ == 2 ? 9 : 4) : (NQ == 2 ? 16 : 8);
-  static constexpr int SMEM = NQ * Q_BYTES + SLOTS * SLOT + 1024 + 1024;
+  static constexpr int BARS = 2 * SLOTS + 10 * NQ + 2 * TC_ITEMS;
+  static constexpr int SMEM = 1024 + NQ * Q_BYTES + SLOTS * SLOT + BARS * 8 + 16 + TC_ITEMS * static_cast<int>(sizeof(TreeItem)) + 4 + SLOTS * 8;
   static constexpr bool TWO = NQ == 1;
   // per tile: scores, weights (high and low terms of 32 columns each, or two places for high ones), the accumulator
   static constexpr int TILE_COLS = 128 + DC, Q_COL = 128 + DC;
   static constexpr int COLS = QT || NQ == 2 ? 512 : 256;
   static constexpr int SOFTMAX = 1 + NQ, WARPS = SOFTMAX + 4 * NQ, THREADS = WARPS * 32, PER_SM = QT || NQ == 2 ? 1 : 2;
-  static_assert(2 * TC_ITEMS > SLOTS, "an item's place");
   static_assert(NQ * TILE_COLS + (QT ? DC / 2 : 0) <= COLS && SMEM <= 232448, "tensor memory, shared memory");
 };
 
@@ -121,9 +120,11 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
   uint64_t* p_full = s_read + NQ;
   uint64_t* o_full = p_full + 2 * NQ;                        // ([NQ][2] like p_full)
   uint64_t* v_seen = o_full + 2 * NQ;                        // warp 1 has looked over a masked page's values
-  uint64_t* v_sync = v_seen + NQ;                            // [NQ]: of 4 and of 8 softmax warps
+  uint64_t* v_read = v_seen + NQ;                            // the tile's softmax warps know of it (tile 1 may be masked pages behind tile 0)
+  uint64_t* v_sync = v_read + NQ;                            // [NQ]: of 4 and of 8 softmax warps
   uint64_t* item_full = v_sync + NQ;                         // [TC_ITEMS]
-  TreeItem* items = reinterpret_cast<TreeItem*>((reinterpret_cast<uintptr_t>(item_full + TC_ITEMS) + 15) & ~uintptr_t(15));     // [TC_ITEMS]
+  uint64_t* item_read = item_full + TC_ITEMS;                // [TC_ITEMS]: by every warp but the producer
+  TreeItem* items = reinterpret_cast<TreeItem*>((reinterpret_cast<uintptr_t>(ring + SLOTS * SLOT + L::BARS * 8) + 15) & ~uintptr_t(15));      // [TC_ITEMS]
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(items + TC_ITEMS);
   uint32_t* odd_rows = tmem_ptr + 1;                         // [SLOTS][2]: tokens of a masked page with a value that is not finite
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -132,10 +133,10 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     for (int s = 0; s < SLOTS; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], NQ); }
     for (int s = 0; s < NQ; ++s) {
       mbar_init(&q_full[s], 4); mbar_init(&s_full[s], 1); mbar_init(&s_read[s], 4);
-      mbar_init(&v_seen[s], 1); mbar_init(&v_sync[s], 4 * (s + 1));
+      mbar_init(&v_seen[s], 1); mbar_init(&v_read[s], 4); mbar_init(&v_sync[s], 4 * (s + 1));
     }
     for (int s = 0; s < 2 * NQ; ++s) { mbar_init(&p_full[s], 4); mbar_init(&o_full[s], 1); }
-    for (int s = 0; s < TC_ITEMS; ++s) mbar_init(&item_full[s], 1);
+    for (int s = 0; s < TC_ITEMS; ++s) { mbar_init(&item_full[s], 1); mbar_init(&item_read[s], L::WARPS - 1); }
     fence_barrier_init();
   }
   if (warp == 1) { tmem_alloc<L::COLS>(tmem_ptr); tmem_relinquish(); }
@@ -153,6 +154,8 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
   const auto announced = [&](int k, TreeItem& it) {                     // item k of this CTA; nj = 0: there is none, or the wait for it ran out
     const bool there = tc_wait(&item_full[k % TC_ITEMS], (k / TC_ITEMS) & 1);
     it = items[k % TC_ITEMS];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&item_read[k % TC_ITEMS]);
     if (!there) { why = ST_TIMEOUT_MBAR_FULL; it.nj = 0; }
     return it.nj > 0;
   };
@@ -167,6 +170,8 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     for (int k = 0; ok; ++k) {
       TreeItem it;
       ta_next(a, range, it);
+      if (k >= TC_ITEMS) ok = tc_wait(&item_read[k % TC_ITEMS], (k / TC_ITEMS - 1) & 1);
+      if (!ok) { why = ST_TIMEOUT_MBAR_EMPTY; break; }
       if (lane == 0) {
         items[k % TC_ITEMS] = it;
         mbar_arrive(&item_full[k % TC_ITEMS]);
@@ -206,6 +211,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0) + q * L::TILE_COLS;
     TcCount c;
     int n = 0, own = 0;                                      // pages and items of the tile so far
+    int shown[NQ] = {};                                      // masked pages announced to the tiles
     TreeItem it;
 #pragma unroll 1
     for (int k = 0; ok && announced(k, it); ++k) {
@@ -272,10 +278,14 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
           }
           fence_proxy_async();
           __syncwarp();
-          if (lane == 0) {
-            odd_rows[2 * c.slot] = odd[0]; odd_rows[2 * c.slot + 1] = odd[1];
-            for (int i = 0; i < act; ++i) mbar_arrive(&v_seen[i]);
-          }
+          if (lane == 0) { odd_rows[2 * c.slot] = odd[0]; odd_rows[2 * c.slot + 1] = odd[1]; }
+#pragma unroll
+          for (int i = 0; i < NQ; ++i)
+            if (i < act) {
+              if (shown[i] > 0) ok = ok && tc_wait(&v_read[i], (shown[i] - 1) & 1);
+              if (lane == 0) mbar_arrive(&v_seen[i]);
+              ++shown[i];
+            }
         }
         ok = ok && tc_wait(&p_full[q * 2 + place(n + j)], phase(n + j));
         if (!ok) { why = ST_TIMEOUT_MBAR_FULL; break; }
@@ -525,6 +535,8 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
           ok = tc_wait(&v_seen[q], seen_phase);
           seen_phase ^= 1u;
           if (!ok) { why = ST_TIMEOUT_MBAR_FULL; break; }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&v_read[q]);
           const int vs = (seq0 + (j < it.nj - 1 ? 2 * j + 2 : 2 * j + 1)) % SLOTS;       // the values' place in the ring's sequence
           const uint64_t bad = odd_rows[2 * vs] | static_cast<uint64_t>(odd_rows[2 * vs + 1]) << 32;
           if (bad) {                                         // (rare)

@@ -112,6 +112,24 @@ def test_attention_of_tiles(D, V, nodes, dtype):
     T.check_attention(U.Round([150, 64], [nodes, 2], device=DEV), 6, 2, D, V, dtype, {}, rounded=WEIGHTS[dtype])
 
 
+@pytest.mark.parametrize("D,f", [(64, {}), (64, dict(window=300)), (128, dict(softcap=3.0)), (128, dict(slopes=True, chunk=256)), (64, dict(bias=40))])
+def test_large_trees_again_and_again(D, f):
+    """Two tiles of a request's rows share its keys and run apart, through pages (ends of windows, trees over a page's end) that not every
+    row sees whole."""
+    rs = np.random.RandomState(5)
+    r = U.Round(rs.randint(900, 1100, 40), rs.randint(33, 65, 40), device=DEV)
+    T.check_attention(r, 16, 4, D, D, BF16, f, rounded=WEIGHTS[BF16])
+    q, k, v, m = r.randn(r.R, 16, D, dtype=BF16), r.randn(r.n_pages, 64, 4, D, dtype=BF16), r.randn(r.n_pages, 64, 4, D, dtype=BF16), ops.slot_maps(**r.inputs())
+    opt = {n: x for n, x in f.items() if n in ("softcap", "window", "chunk")}
+    if "bias" in f:
+        opt["bias"] = r.randn(16, f["bias"])
+    if "slopes" in f:
+        opt["slopes"] = torch.linspace(0.01, 0.5, 16, device=DEV)
+    first = ops.tree_attention(q, k, v, m, D ** -0.5, **opt)
+    for _ in range(40):
+        assert torch.equal(ops.tree_attention(q, k, v, m, D ** -0.5, **opt), first)
+
+
 @pytest.mark.parametrize("layout", ["plain", "interleaved"])
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("name", list(T.FEATURES))
