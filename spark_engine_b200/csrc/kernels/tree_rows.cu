@@ -178,7 +178,7 @@ slot_maps_kernel(const __grid_constant__ SlotMaps a) {
 // ------------------------------------------------------------------------------------------------ convolution along paths
 
 constexpr int PC_ROWS = 64, PC_FAR = 64, PC_THREADS = 256, PC_UNITS = 16;     // rows of a tile and brought in beside them; 16-byte pieces of its channels
-constexpr int PC_STAGES = 3, PC_PER_SM = 2;
+constexpr int PC_STAGES = 2, PC_PER_SM = 3;                    // (three stages leave room for two CTAs: 38.2 us instead of 35.6)
 
 __device__ __forceinline__ void pc_copy(void* d, const void* s) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(d)), "l"(s) : "memory");
@@ -208,9 +208,10 @@ __device__ __forceinline__ uint4 pc_join(const float (&f)[4], float) {
 
 // grid (groups of `per` channel tiles, row tiles).  A tile's rows are brought to shared memory once and every row takes its taps from there;
 // so are up to PC_FAR rows that lie elsewhere (ancestors in front of the tile, the sequences' past).  The paths are
-// followed once for all channel tiles of a CTA, and the next two tiles' rows are on their way while one is computed.  Instructions bound it before
-// the bytes do: what depends on the row alone is formed once, and the common loop has no branches (nobody's rows take a row of zeros).  5.2 us for 50 rows of 2560 channels, 39 us for 5000 rows of 6144 (126 MB, 3.2 TB/s; 52 with the taps'
-// places looked up per tile, 87 with every tap loaded from memory).
+// followed once for all channel tiles of a CTA, and the next tile's rows are on their way while one is computed.  Instructions bound it before
+// the bytes do: what depends on the row alone is formed once, and the common loop has no branches (nobody's rows take a row of zeros).
+// 5.2 us for 50 rows of 2560 channels, 36 us for 5000 rows of 6144 (126 MB, 3.5 TB/s; 52 with the taps' places looked up per tile, 87 with every
+// tap loaded from memory; two products per instruction: no change).
 template <typename T, int TAPS>
 __global__ void __launch_bounds__(PC_THREADS, PC_PER_SM)
 path_conv_kernel(const __grid_constant__ PathConv a, int per) {
