@@ -247,7 +247,7 @@ Tensor tree_attention(Tensor q, const Tensor& k, const Tensor& v, const RowMaps&
   const bool tc = dt == at::kBFloat16 && D <= 256 && V <= 256, wide = D > 128 || V > 128;
   const int64_t most = (m.nodes ? std::min(m.nodes, R) : R) * (H / G);
   const int bm = !tc ? 64 : !wide && most > 128 ? 256 : 128;
-  const int ctas = std::min(1024, on.dev.sms * (bm == 256 || wide ? 1 : 2));
+  const int ctas = std::min(512, on.dev.sms * (bm == 256 || wide ? 1 : 2));
   // What beginning an item costs, in pages (us of a call, extra 0 / 3 / 6 / 10 / 15: four requests of 16k tokens, heads of 256: 61.3 / 57.5 / 55.2 /
   // 49.4 / 48.5; eight windows of 1024, heads of 128 with slopes: 37.2 / 32.1 / 31.7 / 31.5 / 34.6; ragged, soft cap and bias, whose pages take
   // longer: 45.6 / 41.5 / 45.0 / 45.1 / 52.0)

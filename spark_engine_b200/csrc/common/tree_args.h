@@ -53,7 +53,7 @@ struct TreeAttn {
   const uint32_t* anc;                   // [R, words] (null: rows see the rows before them)
   const float *bias, *slopes, *sink;     // [H, bias_n], [H], [H]
   const void* gate;                      // [R, H], rows ldg apart
-  float *part_o, *part_ml;               // [ctas][2][bm][V], [ctas][2][bm][2]: of a tile begun before the CTA, of one that goes on behind it
+  float *part_o, *part_ml;               // [ctas][2][V / 8][bm][8], [ctas][2][bm][2]: of a tile begun before the CTA, of one that goes on behind it
   int* split;                            // [ctas]: the item that begins in this CTA and ends in another, see ta_split
   int* status;
   long long k_page, k_tok, v_page, v_tok;                    // strides in elements

@@ -162,6 +162,12 @@ __device__ __forceinline__ int4 ta_split(const TreeAttn& a, const TreeItem& it) 
   return make_int4(it.parts | min(pairs, bm) << 16, it.r0, it.g, it.rt * bm);
 }
 
+// Columns 8 c8 .. + 8 of a row of part p: the rows of a part lie side by side, 32 bytes each, so that threads that have a row each write whole
+// lines (with rows one behind the other 64 requests of 64 nodes took 336 us instead of 322, windows of 1024 31 instead of 26.5).
+__device__ __forceinline__ float* ta_part(const TreeAttn& a, size_t p, int row, int c8) {
+  return a.part_o + (p << a.bm_log) * a.V + ((static_cast<size_t>(c8) << a.bm_log) + row) * 8;
+}
+
 __device__ __forceinline__ void ta_set_split(const TreeAttn& a, int4 v) { reinterpret_cast<int4*>(a.split)[blockIdx.x] = v; }
 __device__ __forceinline__ int4 ta_get_split(const TreeAttn& a, int c) { return __ldcg(reinterpret_cast<const int4*>(a.split) + c); }
 

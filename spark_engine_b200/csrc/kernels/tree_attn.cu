@@ -260,7 +260,7 @@ __device__ __forceinline__ void tt_item(const TreeAttn& a, const TreeItem& it, T
       const int col = v * VW + lane * CW;
       if (col >= V) continue;
       T* out = static_cast<T*>(a.out) + static_cast<size_t>(r) * a.ldo + static_cast<size_t>(h) * a.ho + col;
-      float* part = a.part_o + (pb + row) * V + col;
+      float* part = ta_part(a, static_cast<size_t>(blockIdx.x) * 2 + (it.first ? 1 : 0), row, col >> 3) + (col & 7);
       if (done) tt_store(out, o[v][i], by);
       else tt_store(part, o[v][i], 1.f);
     }
@@ -301,116 +301,123 @@ tree_tile_kernel(const __grid_constant__ TreeAttn a) {
 }
 
 // ------------------------------------------------------------------------------------------------ merge
-constexpr int TM_THREADS = 256, TM_WARPS = TM_THREADS / 32, TM_MAX_CTAS = 1024;
+constexpr int TM_MAX_CTAS = 512;
 
-// Every CTA makes the list of the split items' rows (a row per item that begins in one CTA of the first launch and ends in another) and
-// takes its share of them; the fewer there are, the more warps join one row.  Parts are added in ascending order within a warp, warps in
-// ascending order.  5 to 9 us behind the first launch, most of it the way to the first part; 20 us for the 39 MB that 148 CTAs with tiles of
-// 256 rows leave (2, 6 and 8 CTAs per SM instead of 4: the same within the noise, 8 slower in short calls).
-template <typename T, int VC>                                // VC: 128-column pieces of a row
-__global__ void __launch_bounds__(TM_THREADS)
+// Every CTA makes the list of the split items' rows (four of an item that begins in one CTA of the first launch and ends in another are a task)
+// and takes its share of them; the fewer there are, the more warps join one task.  Parts are added in ascending order within a warp, warps in
+// ascending order.  A lane has 4 columns in every 32 of one of the four rows, so that loads are whole lines of the parts' layout (ta_part).
+// 5 to 6 us behind the first launch, most of it the way to the first part (8 for rows of 256); 12 us for the 39 MB that 148 CTAs with tiles of
+// 256 rows leave (a row per warp: 20).
+template <typename T, int VC, int THREADS>                   // VC: 32-column pieces of a row
+__global__ void __launch_bounds__(THREADS)
 tree_merge_kernel(const __grid_constant__ TreeAttn a) {
-  __shared__ int sh[TM_WARPS];
-  __shared__ int s_first[TM_MAX_CTAS + 1];                   // rows of the items in front of CTA c's
-  __shared__ float4 s_o[TM_WARPS][32 * VC];
-  __shared__ float s_ml[TM_WARPS][2];
+  constexpr int WARPS = THREADS / 32, EACH = TM_MAX_CTAS / THREADS, FLIGHT = VC <= 4 ? 4 : VC <= 8 ? 2 : 1;        // parts in flight
+  __shared__ int sh[WARPS];
+  __shared__ int s_first[TM_MAX_CTAS + 1];                   // tasks of the items in front of CTA c's
+  __shared__ float4 s_o[WARPS][32 * VC];
+  __shared__ float2 s_ml[WARPS][32];
   __shared__ int4 s_split[TM_MAX_CTAS];
   pdl_wait();
   pdl_trigger();
-  const int t = threadIdx.x, warp = t >> 5, lane = t & 31, V4 = a.V >> 2, rep = a.H / a.G;
+  const int t = threadIdx.x, warp = t >> 5, lane = t & 31, V8 = a.V >> 3, V4 = a.V >> 2, rep = a.H / a.G;
+  const int half = lane & 1, of4 = lane >> 1 & 3, c8 = lane >> 3;
   const int end = a.zero_rest ? a.starts[a.S] : a.R;         // rows of the requests
-  const int each = (a.ctas + TM_THREADS - 1) / TM_THREADS;   // up to four
-  int n[4], mine = 0;
+  const int each = (a.ctas + THREADS - 1) / THREADS;
+  int n[EACH], mine = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < EACH; ++i) {
     const int c = t * each + i;
     n[i] = 0;
     if (i < each && c < a.ctas) {
       const int4 sp = ta_get_split(a, c);
       s_split[c] = sp;
-      n[i] = sp.x >> 16;
+      n[i] = ((sp.x >> 16) + 3) >> 2;
     }
     mine += n[i];
   }
-  int rows;
-  int before = ta_prefix<TM_THREADS>(mine, sh, rows);
+  int tasks;
+  int before = ta_prefix<THREADS>(mine, sh, tasks);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < EACH; ++i) {
     if (i < each && t * each + i < a.ctas) s_first[t * each + i] = before;
     before += n[i];
   }
-  if (t == 0) s_first[a.ctas] = rows;
   __syncthreads();
-  int lw = 3;                                                // log2 of the warps that join one row
-  while (lw > 0 && rows << lw > static_cast<int>(gridDim.x) * TM_WARPS) --lw;
-  const int wpr = 1 << lw, rpb = TM_WARPS >> lw, sub = warp & (wpr - 1);
+  int lw = 31 - __clz(WARPS);                                // log2 of the warps that join one task
+  while (lw > 0 && tasks << lw > static_cast<int>(gridDim.x) * WARPS) --lw;
+  const int wpt = 1 << lw, tpb = WARPS >> lw, sub = warp & (wpt - 1);
 #pragma unroll 1
-  for (int task0 = blockIdx.x * rpb; task0 < rows; task0 += gridDim.x * rpb) {
+  for (int task0 = blockIdx.x * tpb; task0 < tasks; task0 += gridDim.x * tpb) {
     const int task = task0 + (warp >> lw);
-    const bool on = task < rows;
-    int lo = 0, hi = a.ctas;                                 // the last CTA whose rows begin at or before the task
+    int lo = 0, hi = a.ctas;                                 // the last CTA whose tasks begin at or before this one
 #pragma unroll 1
     while (hi - lo > 1) { const int m = (lo + hi) >> 1; if (s_first[m] <= task) lo = m; else hi = m; }
-    const int c = lo, row = on ? task - s_first[lo] : 0;
-    const int4 sp = s_split[c];
+    const int4 sp = s_split[lo];
+    const int row = (task - s_first[lo]) * 4 + of4;
+    const bool on = task < tasks && row < sp.x >> 16;
     const int parts = on ? sp.x & 0xffff : 0;
     // part 0 lies behind the others' in its CTA's pair, see TreeAttn
-    auto part = [&](int i) { return ((static_cast<size_t>(c + i) * 2 + (i == 0 ? 1 : 0)) << a.bm_log) + row; };
+    auto part = [&](int i) { return static_cast<size_t>(lo + i) * 2 + (i == 0 ? 1 : 0); };
     float m = -INFINITY, l = 0.f;
     float4 o[VC] = {};
 #pragma unroll 1
-    for (int i0 = sub; i0 < parts; i0 += 4 * wpr) {          // four parts in flight
-      float4 x[4][VC];
-      float2 ml[4];
+    for (int i0 = sub; i0 < parts; i0 += FLIGHT * wpt) {
+      float4 x[FLIGHT][VC];
+      float2 ml[FLIGHT];
+      float top = m;
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int i = i0 + u * wpr;
-        ml[u] = i < parts ? __ldcg(reinterpret_cast<const float2*>(a.part_ml + part(i) * 2)) : make_float2(-INFINITY, 0.f);
+      for (int u = 0; u < FLIGHT; ++u) {
+        const int i = i0 + u * wpt;
+        ml[u] = i < parts ? __ldcg(reinterpret_cast<const float2*>(a.part_ml) + (part(i) << a.bm_log) + row) : make_float2(-INFINITY, 0.f);
 #pragma unroll
         for (int v = 0; v < VC; ++v)
-          if (i < parts && lane + v * 32 < V4) x[u][v] = __ldcg(reinterpret_cast<const float4*>(a.part_o + part(i) * a.V) + lane + v * 32);
+          if (i < parts && v * 4 + c8 < V8) x[u][v] = __ldcg(reinterpret_cast<const float4*>(ta_part(a, part(i), row, v * 4 + c8)) + half);
       }
-      const float top = fmaxf(m, fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x))), ref = top == -INFINITY ? 0.f : top;
-      const float k = ta_exp<T>(m - ref);
+#pragma unroll
+      for (int u = 0; u < FLIGHT; ++u) top = fmaxf(top, ml[u].x);
+      const float ref = top == -INFINITY ? 0.f : top, k = ta_exp<T>(m - ref);
       m = top;
       l *= k;
 #pragma unroll
       for (int v = 0; v < VC; ++v) { o[v].x *= k; o[v].y *= k; o[v].z *= k; o[v].w *= k; }
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < FLIGHT; ++u) {
         const float w = ta_exp<T>(ml[u].x - ref);
         if (w == 0.f && ml[u].y == ml[u].y) continue;        // (a part of NaN scores alone stays)
         l = fmaf(w, ml[u].y, l);
 #pragma unroll
         for (int v = 0; v < VC; ++v)
-          if (lane + v * 32 < V4) {
+          if (v * 4 + c8 < V8) {
             o[v].x = fmaf(w, x[u][v].x, o[v].x); o[v].y = fmaf(w, x[u][v].y, o[v].y);
             o[v].z = fmaf(w, x[u][v].z, o[v].z); o[v].w = fmaf(w, x[u][v].w, o[v].w);
           }
       }
     }
-    if (wpr > 1) {
+    if (wpt > 1) {
       __syncthreads();                                       // (the task before has been read)
-      if (lane == 0) { s_ml[warp][0] = m; s_ml[warp][1] = l; }
+      s_ml[warp][lane] = make_float2(m, l);
 #pragma unroll
       for (int v = 0; v < VC; ++v)
-        if (lane + v * 32 < V4) s_o[warp][lane + v * 32] = o[v];
+        if (v * 4 + c8 < V8) s_o[warp][v * 32 + lane] = o[v];
       __syncthreads();
       if (sub == 0) {
-        for (int i = 1; i < wpr; ++i) m = fmaxf(m, s_ml[warp + i][0]);
-        const float ref = m == -INFINITY ? 0.f : m, c0 = ta_exp<T>(s_ml[warp][0] - ref);
-        l *= c0;
-#pragma unroll
-        for (int v = 0; v < VC; ++v) { o[v].x *= c0; o[v].y *= c0; o[v].z *= c0; o[v].w *= c0; }
+        const float m0 = m;
 #pragma unroll 1
-        for (int i = 1; i < wpr; ++i) {
-          const float w = ta_exp<T>(s_ml[warp + i][0] - ref);
-          if (w == 0.f && s_ml[warp + i][1] == s_ml[warp + i][1]) continue;
-          l = fmaf(w, s_ml[warp + i][1], l);
+        for (int i = 1; i < wpt; ++i) m = fmaxf(m, s_ml[warp + i][lane].x);
+        const float ref = m == -INFINITY ? 0.f : m, k = ta_exp<T>(m0 - ref);
+        l *= k;
+#pragma unroll
+        for (int v = 0; v < VC; ++v) { o[v].x *= k; o[v].y *= k; o[v].z *= k; o[v].w *= k; }
+#pragma unroll 1
+        for (int i = 1; i < wpt; ++i) {
+          const float2 ml = s_ml[warp + i][lane];
+          const float w = ta_exp<T>(ml.x - ref);
+          if (w == 0.f && ml.y == ml.y) continue;
+          l = fmaf(w, ml.y, l);
 #pragma unroll
           for (int v = 0; v < VC; ++v)
-            if (lane + v * 32 < V4) {
-              const float4 y = s_o[warp + i][lane + v * 32];
+            if (v * 4 + c8 < V8) {
+              const float4 y = s_o[warp + i][v * 32 + lane];
               o[v].x = fmaf(w, y.x, o[v].x); o[v].y = fmaf(w, y.y, o[v].y); o[v].z = fmaf(w, y.z, o[v].z); o[v].w = fmaf(w, y.w, o[v].w);
             }
         }
@@ -421,19 +428,29 @@ tree_merge_kernel(const __grid_constant__ TreeAttn a) {
     const float k = a.sink ? ta_sink<T>(a.sink[h], m, l) : 1.f;
     float scale = l > 0.f ? ta_head_factor<T>(a, r, h) * k / l : 0.f;
     if (l != l) scale = l;
+    T* out = static_cast<T*>(a.out) + static_cast<size_t>(r) * a.ldo + static_cast<size_t>(h) * a.ho + c8 * 8 + half * 4;
 #pragma unroll
     for (int v = 0; v < VC; ++v)
-      if (lane + v * 32 < V4)
-        stf4(static_cast<T*>(a.out) + static_cast<size_t>(r) * a.ldo + static_cast<size_t>(h) * a.ho + (lane + v * 32) * 4,
-             make_float4(o[v].x * scale, o[v].y * scale, o[v].z * scale, o[v].w * scale));
+      if (v * 4 + c8 < V8) stf4(out + v * 32, make_float4(o[v].x * scale, o[v].y * scale, o[v].z * scale, o[v].w * scale));
   }
 #pragma unroll 1
   for (int r = end + blockIdx.x; r < a.R; r += gridDim.x)
 #pragma unroll 1
-    for (int i = t; i < a.H * V4; i += TM_THREADS) {
+    for (int i = t; i < a.H * V4; i += THREADS) {
       const int h = i / V4;
       stf4(static_cast<T*>(a.out) + static_cast<size_t>(r) * a.ldo + static_cast<size_t>(h) * a.ho + (i - h * V4) * 4, make_float4(0.f, 0.f, 0.f, 0.f));
     }
+}
+template <typename T, int VC, int THREADS>
+static void launch_merge(const TreeAttn& a, cudaStream_t s) {
+  // (narrow rows: more CTAs to an SM)
+  spark_launch_pdl(tree_merge_kernel<T, VC, THREADS>, dim3((VC <= 4 ? 2 : 1) * a.sms), dim3(THREADS), 0, s, dim3(1, 1, 1), a);
+}
+template <typename T>
+static void launch_merges(const TreeAttn& a, cudaStream_t s) {
+  if (a.V <= 128) launch_merge<T, 4, 256>(a, s);
+  else if (a.V <= 256) launch_merge<T, 8, 256>(a, s);
+  else launch_merge<T, 16, 128>(a, s);
 }
 
 constexpr int TA_SMEM = 220 * 1024;
@@ -465,10 +482,7 @@ extern "C" int spark_tree_attn(const TreeAttn* a, int f32, int tc, cudaStream_t 
       a->min_tiles <= 0 || (a->bias && a->bias_n <= 0) || a->page_ld <= 0 || ((a->ldq | a->hq | a->ldo | a->ho) & 3)) return -5;
   if (tc ? f32 || (a->bm_log != 7 && a->bm_log != 8) : 1 << a->bm_log != TT_BM) return -5;
   if (const int rc = tc ? launch_tree_tc(*a, s) : f32 ? launch_tiles<float>(*a, s) : launch_tiles<__nv_bfloat16>(*a, s)) return rc;
-  // (narrow rows: more CTAs to an SM)
-  const dim3 grid((a->V <= 128 ? 4 : 2) * a->sms);
-  auto merge = f32 ? (a->V <= 128 ? tree_merge_kernel<float, 1> : a->V <= 256 ? tree_merge_kernel<float, 2> : tree_merge_kernel<float, 4>)
-                   : (a->V <= 128 ? tree_merge_kernel<__nv_bfloat16, 1> : a->V <= 256 ? tree_merge_kernel<__nv_bfloat16, 2> : tree_merge_kernel<__nv_bfloat16, 4>);
-  spark_launch_pdl(merge, grid, dim3(TM_THREADS), 0, s, dim3(1, 1, 1), *a);
+  if (f32) launch_merges<float>(*a, s);
+  else launch_merges<__nv_bfloat16>(*a, s);
   return spark_launch_rc("spark_tree_attn");
 }

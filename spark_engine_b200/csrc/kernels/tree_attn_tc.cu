@@ -599,7 +599,6 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         *reinterpret_cast<float2*>(a.part_ml + pb * 2) = make_float2(m, l);
       }
       __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + static_cast<size_t>(pr) * a.ldo + static_cast<size_t>(h) * a.ho;
-      float* part = a.part_o + pb * a.V;
 #pragma unroll 1
       for (int cc = 0; cc < vn; cc += 32) {
         uint32_t o[32];
@@ -615,8 +614,9 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
               for (int e = 0; e < 4; ++e) w[e] = tc_pack(__uint_as_float(o[i * 8 + 2 * e]) * k, __uint_as_float(o[i * 8 + 2 * e + 1]) * k);
               *reinterpret_cast<uint4*>(out + cc + i * 8) = make_uint4(w[0], w[1], w[2], w[3]);
             } else {
-              *reinterpret_cast<uint4*>(part + cc + i * 8) = make_uint4(o[i * 8], o[i * 8 + 1], o[i * 8 + 2], o[i * 8 + 3]);
-              *reinterpret_cast<uint4*>(part + cc + i * 8 + 4) = make_uint4(o[i * 8 + 4], o[i * 8 + 5], o[i * 8 + 6], o[i * 8 + 7]);
+              uint4* part = reinterpret_cast<uint4*>(ta_part(a, static_cast<size_t>(blockIdx.x) * 2 + (it.first ? 1 : 0), q * 128 + row, (cc >> 3) + i));
+              part[0] = make_uint4(o[i * 8], o[i * 8 + 1], o[i * 8 + 2], o[i * 8 + 3]);
+              part[1] = make_uint4(o[i * 8 + 4], o[i * 8 + 5], o[i * 8 + 6], o[i * 8 + 7]);
             }
           }
         }
