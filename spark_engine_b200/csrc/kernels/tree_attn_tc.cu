@@ -73,6 +73,7 @@ __device__ __forceinline__ float tc_ex2(float x) {          // relative error 2^
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ void tc_set(float (&s)[64], int i, uint64_t v) { s[i] = ta_lo(v); s[i + 1] = ta_hi(v); }
 __device__ __forceinline__ float tc_rcp(float x) {          // relative error 2^-23
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -399,8 +400,9 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
           __syncwarp();
           if (lane == 0) mbar_arrive(&s_read[q]);
           if (FEAT) {
+            const uint64_t scale2 = ta_two(a.scale, a.scale);
 #pragma unroll
-            for (int i = 0; i < 64; ++i) s[i] *= a.scale;
+            for (int i = 0; i < 64; i += 2) tc_set(s, i, ta_mul2(ta_two(s[i], s[i + 1]), scale2));
             if (a.cap > 0.f) {
               const float icap = 1.f / a.cap;
               float big = 0.f;                               // scores far below the cap need no exponential
@@ -413,8 +415,14 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
                   s[i] = fabsf(z) < CAP_NEAR ? s[i] * tanh_over_z(z) : a.cap - 2.f * a.cap * tc_rcp(1.f + e);
                 }
               } else {
+                const uint64_t icap2 = ta_two(icap, icap);
 #pragma unroll
-                for (int i = 0; i < 64; ++i) s[i] *= tanh_over_z(s[i] * icap);
+                for (int i = 0; i < 64; i += 2) {            // (tanh_over_z, two at a time)
+                  const uint64_t x = ta_two(s[i], s[i + 1]), z = ta_mul2(x, icap2), zz = ta_mul2(z, z);
+                  uint64_t y = ta_two(62.f / 2835.f, 62.f / 2835.f);
+                  for (const float c : {-17.f / 315.f, 2.f / 15.f, -1.f / 3.f, 1.f}) y = ta_fma2(zz, y, ta_two(c, c));
+                  tc_set(s, i, ta_mul2(x, y));
+                }
               }
             }
             const int d0 = p - tok0;                         // distance of the page's token 0, were it committed
@@ -425,6 +433,10 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
                 const float far = __ldg(bh + a.bias_n - 1);
 #pragma unroll
                 for (int i = 0; i < 64; ++i) s[i] += far;
+              } else if (!nodes && __all_sync(0xffffffffu, d0 >= 63 && d0 < a.bias_n)) {           // (within the table: 31.5 -> 29.4 us of a ragged round)
+                const float* near_to = bh + d0;
+#pragma unroll
+                for (int i = 0; i < 64; ++i) s[i] += __ldg(near_to - i);
               } else {
 #pragma unroll
                 for (int i0 = 0; i0 < 64; i0 += 16) {        // sixteen in flight
@@ -446,9 +458,11 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
                 for (int i = 0; i < 64; ++i) s[i] -= sl * static_cast<float>(p - __shfl_sync(0xffffffffu, i < 32 ? at_lo : at_hi, i & 31));
               } else {
                 // (near tokens, the ones that weigh, have a small d0: nothing is lost by taking the products apart)
-                const float s0 = sl * static_cast<float>(d0);
+                const float s0 = -sl * static_cast<float>(d0);
+                const uint64_t s2 = ta_two(s0, s0), sl2 = ta_two(sl, sl);
 #pragma unroll
-                for (int i = 0; i < 64; ++i) s[i] = fmaf(sl, static_cast<float>(i), s[i] - s0);
+                for (int i = 0; i < 64; i += 2)
+                  tc_set(s, i, ta_fma2(sl2, ta_two(static_cast<float>(i), static_cast<float>(i + 1)), ta_add2(ta_two(s[i], s[i + 1]), s2)));
               }
             }
           }
