@@ -400,30 +400,31 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
           __syncwarp();
           if (lane == 0) mbar_arrive(&s_read[q]);
           if (FEAT) {
-            const uint64_t scale2 = ta_two(a.scale, a.scale);
-#pragma unroll
-            for (int i = 0; i < 64; i += 2) tc_set(s, i, ta_mul2(ta_two(s[i], s[i + 1]), scale2));
             if (a.cap > 0.f) {
-              const float icap = 1.f / a.cap;
-              float big = 0.f;                               // scores far below the cap need no exponential
+              const float to_z = a.scale / a.cap;
+              float big[4] = {};                             // scores far below the cap need no exponential
 #pragma unroll
-              for (int i = 0; i < 64; ++i) big = fmaxf(big, fabsf(s[i]));
-              if (__any_sync(0xffffffffu, big * icap >= CAP_NEAR)) {
+              for (int i = 0; i < 64; ++i) big[i & 3] = fmaxf(big[i & 3], fabsf(s[i]));
+              if (__any_sync(0xffffffffu, fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3])) * fabsf(to_z) >= CAP_NEAR)) {
 #pragma unroll
                 for (int i = 0; i < 64; ++i) {               // (cap_tanh with the approximate instructions)
-                  const float z = s[i] * icap, e = tc_ex2(fminf(z, 40.f) * (2.f * TA_LOG2E));
-                  s[i] = fabsf(z) < CAP_NEAR ? s[i] * tanh_over_z(z) : a.cap - 2.f * a.cap * tc_rcp(1.f + e);
+                  const float z = s[i] * to_z, e = tc_ex2(fminf(z, 40.f) * (2.f * TA_LOG2E));
+                  s[i] = a.cap * (fabsf(z) < CAP_NEAR ? z * tanh_over_z(z) : fmaf(-2.f, tc_rcp(1.f + e), 1.f));
                 }
               } else {
-                const uint64_t icap2 = ta_two(icap, icap);
+                const uint64_t to_z2 = ta_two(to_z, to_z);
 #pragma unroll
-                for (int i = 0; i < 64; i += 2) {            // (tanh_over_z, two at a time)
-                  const uint64_t x = ta_two(s[i], s[i + 1]), z = ta_mul2(x, icap2), zz = ta_mul2(z, z);
-                  uint64_t y = ta_two(62.f / 2835.f, 62.f / 2835.f);
-                  for (const float c : {-17.f / 315.f, 2.f / 15.f, -1.f / 3.f, 1.f}) y = ta_fma2(zz, y, ta_two(c, c));
+                for (int i = 0; i < 64; i += 2) {            // (scale * tanh_over_z, two at a time)
+                  const uint64_t x = ta_two(s[i], s[i + 1]), z = ta_mul2(x, to_z2), zz = ta_mul2(z, z);
+                  uint64_t y = ta_two(62.f / 2835.f * a.scale, 62.f / 2835.f * a.scale);
+                  for (const float c : {-17.f / 315.f, 2.f / 15.f, -1.f / 3.f, 1.f}) y = ta_fma2(zz, y, ta_two(c * a.scale, c * a.scale));
                   tc_set(s, i, ta_mul2(x, y));
                 }
               }
+            } else {
+              const uint64_t scale2 = ta_two(a.scale, a.scale);
+#pragma unroll
+              for (int i = 0; i < 64; i += 2) tc_set(s, i, ta_mul2(ta_two(s[i], s[i + 1]), scale2));
             }
             const int d0 = p - tok0;                         // distance of the page's token 0, were it committed
             const bool nodes = tok0 + TA_PAGE > sg.len;
@@ -487,7 +488,9 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
               float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
               for (int i = 4; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
-              const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c1;
+              float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c1;
+              if (FEAT && a.slopes)                          // nearer pages weigh more by as much as is known: room for 2^86 of it
+                top += fminf(fmaxf(__ldg(a.slopes + h) * static_cast<float>(p - tok0 - 63), 0.f), 60.f);
               if (ref == -INFINITY) ref = top;
               else if (top > ref) {
                 rescale = true;
