@@ -248,9 +248,9 @@ Tensor tree_attention(Tensor q, const Tensor& k, const Tensor& v, const RowMaps&
   const int64_t most = (m.nodes ? std::min(m.nodes, R) : R) * (H / G);
   const int bm = !tc ? 64 : !wide && most > 128 ? 256 : 128;
   const int ctas = std::min(512, on.dev.sms * (bm == 256 || wide ? 1 : 2));
-  // What beginning an item costs, in pages (us of a call, extra 0 / 3 / 6 / 10 / 15: four requests of 16k tokens, heads of 256: 61.3 / 57.5 / 55.2 /
-  // 49.4 / 48.5; eight windows of 1024, heads of 128 with slopes: 37.2 / 32.1 / 31.7 / 31.5 / 34.6; ragged, soft cap and bias, whose pages take
-  // longer: 45.6 / 41.5 / 45.0 / 45.1 / 52.0)
+  // What beginning an item costs, in pages (us of a call: four requests of 16k tokens, heads of 256, with 5 / 8 / 10 / 14 / 20: 51.7 / 46.1 / 45.1 /
+  // 44.7 / 44.9; a ragged round with soft cap and bias, whose pages take longer, with 2 / 3 / 4 / 6 / 8: 28.5 / 28.6 / 28.6 / 30.8 / 31.0; 64 requests
+  // of 64 nodes with 3 / 4 / 8 / 10 / 12: 322 / 322 / 320 / 321 / 320; the FP32 units' pages are long)
   const int extra = !tc ? 0 : wide ? 10 : softcap > 0 || bias || slopes ? 4 : 6;
   const int64_t work = G * (R * (H / G) / bm + S) * (m.tables.size(1) + extra);
   NEED(work < 1ll << 31, "a round of ", R, " rows over tables of ", m.tables.size(1), " pages is more than one call takes");
