@@ -44,12 +44,12 @@ __device__ __forceinline__ void tt_store(__nv_bfloat16* p, const float (&x)[2], 
 
 struct TtRows { uint64_t seen[TT_BM]; int pos[TT_BM], head[TT_BM], at[TA_PAGE]; };    // of a row: tokens of the page it sees, position, head
 
-// One item, 8 * MR rows: a warp has rows warp + 8 i, so that what is read of a row is the same for all lanes (one shared-memory cycle instead of
-// four: LDS.128 of 32 lanes that share 16 addresses); a lane has keys lane + 32 e of a page's scores and CW neighbouring columns in every 32 CW of the outputs.  Keys pass in pieces of 64
-// tokens x 64 channels, values in pieces of 4096 (128 channels, or 64 where there are no more), two of them on their way while one is worked on.  The
-// FP32 units and the instructions that feed them bound it: one request of 64 nodes, 12 heads of 128 over 39k tokens runs at 27 TFLOP/s (with 4 x 4
-// scores and outputs per thread 23, with copies waited for where they are needed 14), a single row over 30k tokens at 1.8 TB/s; 5 to 11 nodes
-// over 2k tokens are 24 us of latency (35 with the rows' softmax unrolled: every instruction's first run waits for memory).
+// One item, 8 * MR rows: a warp has rows warp + 8 i, so that what is read of a row is the same for all lanes (one shared-memory cycle instead
+// of four); a lane has keys lane + 32 e of a page's scores and CW neighbouring columns in every 32 CW of the outputs.  Keys pass in pieces of
+// 64 tokens x 64 channels, values in pieces of 4096 (128 channels, or 64 where there are no more), two of them on their way while one is worked
+// on.  The FP32 units and the instructions that feed them bound it: one request of 64 nodes, 12 heads of 128 over 39k tokens runs at 27 TFLOP/s
+// (with 4 x 4 scores and outputs per thread 23, with copies waited for where they are needed 14), a single row over 30k tokens at 1.8 TB/s; 5 to
+// 11 nodes over 2k tokens are 24 us of latency (35 with the rows' softmax unrolled: every instruction's first run waits for memory).
 template <typename T, int VP, int CW, int MR>
 __device__ __forceinline__ void tt_item(const TreeAttn& a, const TreeItem& it, T* ring, float* Qs, float* Ss, TtRows& rows) {
   constexpr int VW = 32 * CW, VT = 4096 / VW;                // channels and tokens of a piece of values

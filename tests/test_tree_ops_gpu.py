@@ -130,6 +130,21 @@ def test_large_trees_again_and_again(D, f):
         assert torch.equal(ops.tree_attention(q, k, v, m, D ** -0.5, **opt), first)
 
 
+@pytest.mark.parametrize("sharp", [1.0, 40.0])
+@pytest.mark.parametrize("window", [0, 333])
+@pytest.mark.parametrize("rep", [4, 32])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_steep_slopes(dtype, rep, window, sharp):
+    """Slopes that outweigh the scores within a page and others that do not, towards the nearest token and away from it, with and without sinks."""
+    r = U.Round([700, 1500, 3], [9, 7, 2], device=DEV)
+    q, k, v = r.randn(r.R, 2 * rep, 64, dtype=dtype) * sharp, r.randn(r.n_pages, 64, 2, 64, dtype=dtype), r.randn(r.n_pages, 64, 2, 64, dtype=dtype)
+    slopes = torch.tensor([[3.0, 0.7, 0.3, -0.2, 0.05, -1.5, 0.0, 0.01][h % 8] for h in range(2 * rep)], device=DEV)
+    m = ops.slot_maps(**r.inputs())
+    for sink in (None, torch.linspace(-90, 30, 2 * rep, device=DEV)):
+        got = ops.tree_attention(q, k, v, m, 0.125, slopes=slopes, sink=sink, window=window)
+        U.close(got, *U.want_attention(r, q, k, v, 0.125, slopes=slopes, sink=sink, window=window, rounded=WEIGHTS[dtype]), dtype)
+
+
 @pytest.mark.parametrize("layout", ["plain", "interleaved"])
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("name", list(T.FEATURES))

@@ -113,7 +113,7 @@ def want_attention(r, q, k, v, scale, softcap=0.0, bias=None, slopes=None, sink=
                 x = x + bias[h].double()[dist.clamp(0, bias.shape[1] - 1)]
             if slopes is not None:
                 x = x - slopes[h].double() * dist
-                e = e + slopes[h].double() * dist.abs() * 4 * u
+                e = e + (slopes[h].double() * dist).abs() * 4 * u
             x = x.masked_fill(~seen, -math.inf)
             usual = x.abs() < 1e30
             e = 2 * e.masked_fill(~seen, 0).amax(1) + 4 * u * x.masked_fill(~usual, 0).abs().amax(1)
