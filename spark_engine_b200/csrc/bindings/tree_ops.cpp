@@ -146,6 +146,7 @@ std::shared_ptr<RowMaps> slot_maps(const Tensor& lengths, const Tensor& counts, 
   auto m = std::make_shared<RowMaps>();
   m->lengths = lengths; m->counts = counts; m->tables = tables; m->slots = slots; m->parents = parents; m->nodes = nodes;
   // one allocation for what is int32: [anc | slot | index | pos | starts]
+  const at::AutoDispatchBelowADInplaceOrView plain;      // (integers: nobody differentiates them)
   const int64_t na = rows * words;
   Tensor all = at::empty({na + 3 * rows + S + 1}, opt);
   if (words) m->anc = all.as_strided({rows, words}, {words, 1}, 0);
@@ -326,7 +327,7 @@ int64_t commit_paths(const RowMaps& m, const Tensor& path, const Tensor& n_path,
 
 PYBIND11_MODULE(_tree, mod) {
   mod.doc() = "spark_engine_b200: verification of drafted trees over paged caches (checks and launches)";
-  mod.def("bind_entry", &bind_entry).def("bind_device", &bind_device).def("knows_device", &knows_device);
+  mod.def("bind_entry", &bind_entry).def("bind_device", &bind_device);
   py::class_<RowMaps, std::shared_ptr<RowMaps>>(mod, "RowMaps",
       "Where a round's rows belong (int32 unless said otherwise; -1 for rows behind the last request): slot [R] row of the tables, index [R]\n"
       "within the request, pos [R], cache_row [R] int64 (page * 64 + token; -1 too where the table has no page), starts [S + 1] first row of\n"

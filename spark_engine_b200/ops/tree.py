@@ -27,6 +27,7 @@ PAGE = 64
 _ENTRIES = {"spark_block_tables": 1, "spark_slot_maps": 1, "spark_path_conv": 1, "spark_commit_paths": 1, "spark_tree_attn": 2}     # kernels of a call
 _mod = None
 _bound = None
+_known = set()                                     # devices that the bindings know
 
 
 def _native():
@@ -46,19 +47,24 @@ def _native():
 
 def _kernels(t: torch.Tensor) -> bool:
     """Whether the kernels run on this tensor; the bindings then know them and its device."""
-    global _bound
     if not use_kernels(t):
         return False
-    mod, index = _mod or _native(), t.get_device()
-    cu = cuda_ops()
-    dll = cu.lib()
-    if _bound is not dll:
+    index = t.get_device()
+    if index not in _known:
+        _bind(index)
+    return True
+
+
+def _bind(index: int):
+    global _bound
+    mod, cu = _native(), cuda_ops()
+    if _bound is None:
+        dll = cu.lib()
         for name in _ENTRIES:
             mod.bind_entry(name, ctypes.cast(getattr(dll._dll, name), ctypes.c_void_p).value)
         _bound = dll
-    if not mod.knows_device(index):
-        mod.bind_device(index, cu.status_word(t.device).data_ptr(), torch.cuda.get_device_properties(index).multi_processor_count)
-    return True
+    mod.bind_device(index, cu.status_word(torch.device("cuda", index)).data_ptr(), torch.cuda.get_device_properties(index).multi_processor_count)
+    _known.add(index)
 
 
 def _count(name: str, calls: int = 1):
