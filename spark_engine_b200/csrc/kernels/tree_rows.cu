@@ -354,7 +354,8 @@ path_conv_kernel(const __grid_constant__ PathConv a, int per) {
 
 // grid (requests, column blocks, jobs); 128 threads x 16 bytes.  A path is ascending, so row i is written after row path[i] >= i was read,
 // and no later row of the path lies at or below i: every thread moves its columns in order and in place.  One launch for all layers: 6 us for 12,
-// 31 to 35 us for 24 of 64 requests (142 MB in rows of 2 KB, 4.0 to 4.7 TB/s; with 4 or 8 rows read before any is written, the same).
+// 31 to 35 us for 24 of 64 requests (142 MB in rows of 2 KB, 4.0 to 4.7 TB/s; with 4 or 8 rows read before any is written the same,
+// with two or four layers per CTA 34 and 37).
 __global__ void __launch_bounds__(128)
 commit_paths_kernel(const __grid_constant__ CommitPaths a) {
   extern __shared__ int s_path[];                            // [P], then [P] source and [P] target rows of the cache
