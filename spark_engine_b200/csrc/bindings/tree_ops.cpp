@@ -244,7 +244,9 @@ Tensor tree_attention(Tensor q, const Tensor& k, const Tensor& v, const RowMaps&
   if (q.stride(2) != 1 || q.stride(0) % e || q.stride(1) % e || !aligned(q) || !strides_fit(q)) q = q.contiguous();
   const On on(q);
   // Tensor cores: tiles of 128 (node, head) rows, two CTAs per SM; or, where a request may have more of them, two tiles per CTA that share
-  // the keys, one CTA per SM.  Heads wider than 128 leave room for one tile and one CTA.
+  // the keys, one CTA per SM.  Heads wider than 128 leave room for one tile and one CTA.  One tile / two (us of a call, 64 requests over 4k tokens, 32
+  // query heads on 8 of 128): 20 nodes (80 rows) 220 / 236, 32 nodes (128 rows) 240 / 244, 40 nodes (160 rows) 423 / 310, 64 nodes (256 rows) 465 /
+  // 328; 8 requests of 32 nodes 50 / 46.
   const bool tc = dt == at::kBFloat16 && D <= 256 && V <= 256, wide = D > 128 || V > 128;
   const int64_t most = (m.nodes ? std::min(m.nodes, R) : R) * (H / G);
   const int bm = !tc ? 64 : !wide && most > 128 ? 256 : 128;
@@ -270,7 +272,7 @@ Tensor tree_attention(Tensor q, const Tensor& k, const Tensor& v, const RowMaps&
     while (1ll << (a.chunk_shift - 31) < chunk) ++a.chunk_shift;
     a.chunk_mul = static_cast<unsigned>(((static_cast<unsigned __int128>(1) << a.chunk_shift) + chunk - 1) / chunk);
   }
-  a.bm_log = bm == 64 ? 6 : bm == 128 ? 7 : 8; a.sms = on.dev.sms; a.ctas = ctas; a.min_tiles = 1; a.extra = extra; a.zero_rest = !given;
+  a.bm_log = bm == 64 ? 6 : bm == 128 ? 7 : 8; a.sms = on.dev.sms; a.ctas = ctas; a.extra = extra; a.zero_rest = !given;
   a.scale = static_cast<float>(scale); a.cap = static_cast<float>(softcap); a.out_scale = static_cast<float>(out_scale);
   on.launch(e_attn, &a, static_cast<int>(dt == at::kFloat), static_cast<int>(tc));
   return out;

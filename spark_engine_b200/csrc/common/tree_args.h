@@ -57,7 +57,7 @@ struct TreeAttn {
   int* split;                            // [ctas]: the item that begins in this CTA and ends in another, see ta_split
   int* status;
   long long k_page, k_tok, v_page, v_tok;                    // strides in elements
-  int S, R, words, page_ld, n_slots, n_pages, H, G, D, V, ldq, hq, ldo, ho, ldg, bias_n, window, chunk, chunk_shift, bm_log, sms, ctas, min_tiles, extra, zero_rest;
+  int S, R, words, page_ld, n_slots, n_pages, H, G, D, V, ldq, hq, ldo, ho, ldg, bias_n, window, chunk, chunk_shift, bm_log, sms, ctas, extra, zero_rest;
   unsigned chunk_mul;
   float scale, cap, out_scale;
 };

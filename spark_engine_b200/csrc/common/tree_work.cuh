@@ -98,7 +98,7 @@ __device__ __forceinline__ TreeRange ta_range(const TreeAttn& a) {
   }
   const int total = __shfl_sync(0xffffffffu, x, 31);
   TreeRange r;
-  r.per = max(static_cast<int>((static_cast<unsigned>(total) + a.ctas - 1) / a.ctas), a.min_tiles);
+  r.per = max(static_cast<int>((static_cast<unsigned>(total) + a.ctas - 1) / a.ctas), 1);
   const long long begin = static_cast<long long>(r.per) * blockIdx.x;
   r.count = begin < total ? min(total - static_cast<int>(begin), r.per) : 0;
   if (r.count == 0) return r;

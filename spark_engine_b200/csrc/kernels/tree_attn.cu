@@ -479,7 +479,7 @@ using namespace spark;
 extern "C" int spark_tree_attn(const TreeAttn* a, int f32, int tc, cudaStream_t s) {
   if (a->S <= 0 || a->R <= 0) return 0;
   if (a->H <= 0 || a->G <= 0 || a->H % a->G || a->D <= 0 || a->V <= 0 || ((a->D | a->V) & 7) || a->D > 512 || a->V > 512 || a->ctas <= 0 || a->ctas > TM_MAX_CTAS || a->sms <= 0 ||
-      a->min_tiles <= 0 || (a->bias && a->bias_n <= 0) || a->page_ld <= 0 || ((a->ldq | a->hq | a->ldo | a->ho) & 3)) return -5;
+      (a->bias && a->bias_n <= 0) || a->page_ld <= 0 || ((a->ldq | a->hq | a->ldo | a->ho) & 3)) return -5;
   if (tc ? f32 || (a->bm_log != 7 && a->bm_log != 8) : 1 << a->bm_log != TT_BM) return -5;
   if (const int rc = tc ? launch_tree_tc(*a, s) : f32 ? launch_tiles<float>(*a, s) : launch_tiles<__nv_bfloat16>(*a, s)) return rc;
   if (f32) launch_merges<float>(*a, s);
