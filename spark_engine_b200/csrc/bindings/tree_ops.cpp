@@ -72,12 +72,27 @@ void need_tables(const Tensor& t) {
 int* ip(const Tensor& t) { return t.numel() ? static_cast<int*>(t.data_ptr()) : nullptr; }
 int* ip(const Opt& t) { return t ? ip(*t) : nullptr; }
 int64_t quantum(const Tensor& t) { return 16 / t.element_size(); }
+// Stride of dimension i; 0 where it has one entry, whose stride may be anything and means nothing.
+int64_t step(const Tensor& t, int64_t i) { return t.size(i) < 2 ? 0 : t.stride(i); }
 bool strides_fit(const Tensor& t) {               // the kernels take strides of rows and heads in 32 bits
-  for (const int64_t s : t.strides())
-    if (s >= 1ll << 31) return false;
+  for (int64_t i = 0; i < t.dim(); ++i)
+    if (step(t, i) >= 1ll << 31) return false;
   return true;
 }
 bool aligned(const Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0; }
+// Whether kernels can read t in pieces of 16 bytes: channels side by side, the others on multiples of `quantum` elements.
+bool in_pieces(const Tensor& t, int64_t quantum) {
+  bool ok = aligned(t) && strides_fit(t) && (t.size(-1) < 2 || t.stride(-1) == 1);
+  for (int64_t i = 0; i + 1 < t.dim(); ++i) ok = ok && step(t, i) % quantum == 0;
+  return ok;
+}
+// t, or a copy of it that they can.  (A new one: `contiguous` gives a contiguous tensor back wherever it starts.)
+Tensor pieces(const Tensor& t, int64_t quantum) {
+  if (in_pieces(t, quantum)) return t;
+  const Tensor c = t.clone(at::MemoryFormat::Contiguous);
+  NEED(in_pieces(c, quantum), "rows must be multiples of 16 bytes");
+  return c;
+}
 
 struct Cache { int64_t page, tok, width; };      // strides and a token's channels, in elements
 Cache need_cache(const char* name, const Tensor& t, at::ScalarType dtype, const at::Device& dev) {
@@ -192,11 +207,11 @@ Tensor path_conv(Tensor x, const Tensor& w, const Tensor& tail, const RowMaps& m
   Tensor q = at::empty({R, nq}, x.options());
   if (!run || R == 0) return q;
   NEED(k.size(0) > 0, "caches without pages");
-  if (x.stride(1) != 1 || x.stride(0) % 8 || !aligned(x) || !strides_fit(x)) x = x.contiguous();
+  x = pieces(x, 8);
   const On on(x);
   spark::PathConv a{x.data_ptr(), static_cast<float*>(w.data_ptr()), tail.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), ip(m.slot), ip(m.index),
                     ip(m.parents), static_cast<long long*>(m.cache_row.data_ptr()), on.dev.status, kc.page, kc.tok, vc.page, vc.tok,
-                    k.size(0) * spark::TREE_PAGE, static_cast<int>(x.stride(0)), static_cast<int>(R), static_cast<int>(C), static_cast<int>(taps),
+                    k.size(0) * spark::TREE_PAGE, static_cast<int>(step(x, 0)), static_cast<int>(R), static_cast<int>(C), static_cast<int>(taps),
                     static_cast<int>(nq), static_cast<int>(kc.width), static_cast<int>(tail.size(0))};
   on.launch(e_conv, &a, static_cast<int>(dt == at::kFloat));
   return q;
@@ -228,12 +243,12 @@ Tensor tree_attention(Tensor q, const Tensor& k, const Tensor& v, const RowMaps&
   need_heads("bias", bias, 2, H, dev);
   need_heads("slopes", slopes, 1, H, dev);
   need_heads("sink", sink, 1, H, dev);
-  NEED(!gate || (gate->dim() == 2 && gate->size(0) == R && gate->size(1) == H && gate->scalar_type() == dt && gate->device() == dev && gate->stride(1) == 1 && strides_fit(*gate)),
+  NEED(!gate || (gate->dim() == 2 && gate->size(0) == R && gate->size(1) == H && gate->scalar_type() == dt && gate->device() == dev && (H < 2 || gate->stride(1) == 1) && strides_fit(*gate)),
        "gate must be [rows, heads] in the queries' type");
   const int64_t e = quantum(q);
   if (given)
     NEED(given->dim() == 3 && given->size(0) == R && given->size(1) == H && given->size(2) == V && given->scalar_type() == dt && given->device() == dev &&
-             given->stride(2) == 1 && given->stride(0) % e == 0 && given->stride(1) % e == 0 && aligned(*given) && strides_fit(*given) &&
+             in_pieces(*given, e) &&
              (H < 2 || given->stride(1) >= V) && (R < 2 || given->stride(0) >= V),
          "out must be [rows, heads, value channels] in the queries' type, heads apart and on 16 bytes");
   Tensor out = given ? *given : at::empty({R, H, V}, q.options());
@@ -241,7 +256,7 @@ Tensor tree_attention(Tensor q, const Tensor& k, const Tensor& v, const RowMaps&
   const int64_t S = m.lengths.size(0);
   if (S == 0) return given ? out : out.zero_();
   NEED(k.size(0) > 0, "caches without pages");
-  if (q.stride(2) != 1 || q.stride(0) % e || q.stride(1) % e || !aligned(q) || !strides_fit(q)) q = q.contiguous();
+  q = pieces(q, e);
   const On on(q);
   // Tensor cores: tiles of 128 (node, head) rows, two CTAs per SM; or, where a request may have more of them, two tiles per CTA that share
   // the keys, one CTA per SM.  Heads wider than 128 leave room for one tile and one CTA.  One tile / two (us of a call, 64 requests over 4k tokens, 32
@@ -265,8 +280,8 @@ Tensor tree_attention(Tensor q, const Tensor& k, const Tensor& v, const RowMaps&
                     reinterpret_cast<int*>(part + no + nm), on.dev.status, kc.page, kc.tok, vc.page, vc.tok};
   const auto i = [](int64_t x) { return static_cast<int>(x); };
   a.S = i(S); a.R = i(R); a.words = m.anc ? i(m.anc->size(1)) : 0; a.page_ld = i(m.tables.size(1)); a.n_slots = i(m.tables.size(0)); a.n_pages = i(k.size(0));
-  a.H = i(H); a.G = i(G); a.D = i(D); a.V = i(V); a.ldq = i(q.stride(0)); a.hq = i(q.stride(1)); a.ldo = i(out.stride(0)); a.ho = i(out.stride(1));
-  a.ldg = gate ? i(gate->stride(0)) : 0; a.bias_n = bias ? i(bias->size(1)) : 0; a.window = i(window); a.chunk = i(chunk);
+  a.H = i(H); a.G = i(G); a.D = i(D); a.V = i(V); a.ldq = i(step(q, 0)); a.hq = i(step(q, 1)); a.ldo = i(step(out, 0)); a.ho = i(step(out, 1));
+  a.ldg = gate ? i(step(*gate, 0)) : 0; a.bias_n = bias ? i(bias->size(1)) : 0; a.window = i(window); a.chunk = i(chunk);
   if (chunk) {
     a.chunk_shift = 31;
     while (1ll << (a.chunk_shift - 31) < chunk) ++a.chunk_shift;
@@ -299,12 +314,12 @@ int64_t commit_paths(const RowMaps& m, const Tensor& path, const Tensor& n_path,
   for (const auto& [x, t] : tails) {
     NEED(t.dim() == 3 && t.is_contiguous() && t.size(0) == m.tables.size(0) && t.device() == dev && is_act(t.scalar_type()),
          "tails must be contiguous bf16 or fp32 tensors [slots, kept, channels] on ", dev);
-    NEED(x.dim() == 2 && x.size(0) == m.rows() && x.size(1) == t.size(2) && x.scalar_type() == t.scalar_type() && x.device() == dev && x.stride(1) == 1,
+    NEED(x.dim() == 2 && x.size(0) == m.rows() && x.size(1) == t.size(2) && x.scalar_type() == t.scalar_type() && x.device() == dev && (x.size(1) < 2 || x.stride(1) == 1),
          "the rows behind a tail must be [rows, channels] in its type");
     const int64_t e = t.element_size();
-    NEED(t.size(2) * e % 16 == 0 && x.stride(0) * e % 16 == 0 && aligned(x) && aligned(t), "rows and tails must start on 16 bytes");
+    NEED(t.size(2) * e % 16 == 0 && step(x, 0) * e % 16 == 0 && aligned(x) && aligned(t), "rows and tails must start on 16 bytes");
     if (t.numel() && x.numel())
-      jobs.push_back({static_cast<char*>(t.data_ptr()), static_cast<char*>(x.data_ptr()), x.stride(0) * e, t.size(2) * e, static_cast<int>(t.size(2) * e),
+      jobs.push_back({static_cast<char*>(t.data_ptr()), static_cast<char*>(x.data_ptr()), step(x, 0) * e, t.size(2) * e, static_cast<int>(t.size(2) * e),
                       static_cast<int>(t.size(0)), static_cast<int>(t.size(1)), 0});
   }
   std::vector<char*> seen;
@@ -329,7 +344,7 @@ int64_t commit_paths(const RowMaps& m, const Tensor& path, const Tensor& n_path,
 
 PYBIND11_MODULE(_tree, mod) {
   mod.doc() = "spark_engine_b200: verification of drafted trees over paged caches (checks and launches)";
-  mod.def("bind_entry", &bind_entry).def("bind_device", &bind_device);
+  mod.def("bind_entry", &bind_entry).def("bind_device", &bind_device).def("pieces", &pieces);
   py::class_<RowMaps, std::shared_ptr<RowMaps>>(mod, "RowMaps",
       "Where a round's rows belong (int32 unless said otherwise; -1 for rows behind the last request): slot [R] row of the tables, index [R]\n"
       "within the request, pos [R], cache_row [R] int64 (page * 64 + token; -1 too where the table has no page), starts [S + 1] first row of\n"

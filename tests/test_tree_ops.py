@@ -304,3 +304,31 @@ def test_convolution_and_commit_refuse():
                  (path, n, [k[:, :, :, :4].expand(-1, -1, -1, 4)[:, :, :, :3]], []), (path.flip(1), n, [k], []), (path + 4, n, [k], [])):
         with pytest.raises(ValueError):
             ops.commit_paths(m, *args)
+
+
+# ----------------------------------------------------------------------------- rows that start anywhere
+ANYWHERE = {                                         # of a buffer: rows that kernels cannot read 16 bytes at a time as they are
+    "contiguous, one element in": lambda b: b[1: 1 + 3 * 32].view(3, 32),
+    "contiguous, three elements in": lambda b: b[3: 3 + 3 * 32].view(3, 32),
+    "rows of an odd pitch": lambda b: b[: 4 * 37].view(4, 37)[:3, :32],
+    "one row of an odd pitch": lambda b: b[: 4 * 37].view(4, 37)[:1, :32],
+    "one row of an odd pitch, in the middle": lambda b: b[: 4 * 37].view(4, 37)[2:3, 3: 35],
+    "columns": lambda b: b[: 32 * 8].view(32, 8).t(),
+    "one value for all channels": lambda b: b[:3].view(3, 1).expand(3, 32),
+}
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("name", list(ANYWHERE))
+def test_rows_that_start_anywhere_are_made_readable(name, dtype):
+    """What the launches take: 16-byte starts, whatever a contiguous tensor's offset or a single row's stride."""
+    from spark_engine_b200.ops import tree
+    x = ANYWHERE[name](torch.arange(600, dtype=torch.float32).remainder(251).to(dtype))
+    y = tree._native().pieces(x, 8)
+    assert torch.equal(x, y) and y.data_ptr() % 16 == 0 and y.stride(1) == 1 and (y.shape[0] == 1 or y.stride(0) % 8 == 0)
+    heads = x.unflatten(1, (4, x.shape[1] // 4))
+    if x.shape[1] // 4 % 8 == 0:
+        y = tree._native().pieces(heads, 8)
+        assert torch.equal(heads, y) and y.data_ptr() % 16 == 0 and y.stride(2) == 1 and all(y.shape[i] == 1 or y.stride(i) % 8 == 0 for i in range(2))
+    good = torch.zeros(3, 40, dtype=dtype)[:, :32]
+    assert tree._native().pieces(good, 8).data_ptr() == good.data_ptr()

@@ -417,3 +417,52 @@ def test_empty_calls():
     m = ops.slot_maps(**r.inputs())
     assert m.slot.tolist() == [-1] * 4
     assert not ops.tree_attention(torch.ones(4, 2, 64, device=DEV), k, k.clone(), m, 0.1).any()
+
+
+def _anywhere(x, how):
+    """The rows x [R, C] again, where kernels cannot read them 16 bytes at a time."""
+    R, C = x.shape
+    if how == "contiguous, one element in":
+        b = x.new_zeros(R * C + 1)
+        y = b[1:].view(R, C)
+    else:                                            # one row, or rows, of an odd pitch
+        b = x.new_zeros(R + 1, C + 5)
+        y = b[:R, :C]
+    y.copy_(x)
+    return y
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [1, 2, 9])
+@pytest.mark.parametrize("how", ["contiguous, one element in", "an odd pitch"])
+def test_rows_that_start_anywhere(how, rows, dtype):
+    r = U.Round([70], [rows], device=DEV)
+    H, G, D, taps = 4, 2, 64, 3
+    C = (H + 2 * G) * D
+    m, k, v = ops.slot_maps(**r.inputs()), r.randn(r.n_pages, 64, G, D, dtype=dtype), r.randn(r.n_pages, 64, G, D, dtype=dtype)
+    x, w, tail = r.randn(rows, C, dtype=dtype), r.randn(taps, C), r.randn(1, taps - 1, C, dtype=dtype)
+    k2, v2 = k.clone(), v.clone()
+    want = ops.path_conv(x, w, tail, m, H * D, k, v)
+    got = ops.path_conv(_anywhere(x, how), w, tail, m, H * D, k2, v2)
+    assert torch.equal(got, want) and torch.equal(k, k2) and torch.equal(v, v2)
+    q = r.randn(rows, H * D, dtype=dtype)
+    want = ops.tree_attention(q.view(rows, H, D), k, v, m, 0.1)
+    assert torch.equal(ops.tree_attention(_anywhere(q, how).unflatten(1, (H, D)), k, v, m, 0.1), want)
+    one = q[:1].expand(rows, -1)                     # one row for all
+    assert torch.equal(ops.tree_attention(one.unflatten(1, (H, D)), k, v, m, 0.1), ops.tree_attention(one.contiguous().view(rows, H, D), k, v, m, 0.1))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_one_row_and_one_head_have_any_stride(dtype):
+    """Strides of dimensions with one entry mean nothing: outputs, gates and rows behind a tail."""
+    r = U.Round([70], [1], device=DEV)
+    m, k, v = ops.slot_maps(**r.inputs()), r.randn(r.n_pages, 64, 1, 64, dtype=dtype), r.randn(r.n_pages, 64, 1, 64, dtype=dtype)
+    q, gate = r.randn(1, 1, 64, dtype=dtype), r.randn(1, 1, dtype=dtype)
+    want = ops.tree_attention(q, k, v, m, 0.1, gate=gate)
+    out = torch.zeros(200, dtype=dtype, device=DEV).as_strided((1, 1, 64), (67, 5, 1))
+    got = ops.tree_attention(q, k, v, m, 0.1, gate=torch.zeros(9, dtype=dtype, device=DEV).as_strided((1, 1), (3, 7)).copy_(gate), out=out)
+    assert got.data_ptr() == out.data_ptr() and torch.equal(got, want)
+    x, tail = r.randn(1, 64, dtype=dtype), r.randn(1, 2, 64, dtype=dtype)
+    last = tail[0, 1].clone()
+    ops.commit_paths(m, r.i32([[0]]), r.i32([1]), [k], [(torch.cat((x, x), 1).as_strided((1, 64), (67, 1)), tail)])
+    assert torch.equal(tail[0], torch.stack((last, x[0])))
