@@ -376,12 +376,12 @@ commit_paths_kernel(const __grid_constant__ CommitPaths a) {
   ok = __syncthreads_and(ok);
   if (ok && !jb.x) {
     for (int i = t; i < n; i += 128) {
-      const int from = len + s_path[i], to = len + i;
+      const long long from = static_cast<long long>(len) + s_path[i], to = static_cast<long long>(len) + i;
       const int pf = from / TREE_PAGE < a.ld ? a.tables[static_cast<size_t>(slot) * a.ld + from / TREE_PAGE] : -1;
       const int pt = to / TREE_PAGE < a.ld ? a.tables[static_cast<size_t>(slot) * a.ld + to / TREE_PAGE] : -1;
       if (pf < 0 || pt < 0 || pf >= jb.extent || pt >= jb.extent) ok = false;
-      src[i] = pf * TREE_PAGE + from % TREE_PAGE;
-      dst[i] = pt * TREE_PAGE + to % TREE_PAGE;
+      src[i] = pf * TREE_PAGE + static_cast<int>(from % TREE_PAGE);
+      dst[i] = pt * TREE_PAGE + static_cast<int>(to % TREE_PAGE);
     }
   } else if (ok && slot >= jb.extent) ok = false;
   ok = __syncthreads_and(ok);

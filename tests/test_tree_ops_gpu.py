@@ -466,3 +466,19 @@ def test_one_row_and_one_head_have_any_stride(dtype):
     last = tail[0, 1].clone()
     ops.commit_paths(m, r.i32([[0]]), r.i32([1]), [k], [(torch.cat((x, x), 1).as_strided((1, 64), (67, 1)), tail)])
     assert torch.equal(tail[0], torch.stack((last, x[0])))
+
+
+@pytest.mark.parametrize("length", [200, 1 << 20, (1 << 31) - 1024, (1 << 31) - 2, (1 << 31) - 1])
+def test_commit_of_lengths_beyond_the_table(length):
+    """Token numbers are formed in 64 bits: the request is skipped, the one beside it is not."""
+    r = U.Round([150, 90], [6, 4], device=DEV)
+    good, k = ops.slot_maps(**r.inputs()), r.randn(r.n_pages, 64, 2, 8)
+    want = k.clone()
+    ops.commit_paths(good, r.i32([[0, 0, 0], [0, 2, 3]]), r.i32([0, 3]), [want])
+    d = r.inputs()
+    d["lengths"] = torch.tensor([length, 90], dtype=torch.int32, device=DEV)          # the table has three pages
+    m = ops.slot_maps(**d)
+    expect_status()
+    ops.commit_paths(m, r.i32([[0, 2, 5], [0, 2, 3]]), r.i32([3, 3]), [k])
+    expect_status()
+    assert torch.equal(k, want)
