@@ -304,12 +304,14 @@ int64_t commit_paths(const RowMaps& m, const Tensor& path, const Tensor& n_path,
   const int64_t P = path.size(1);
   NEED(P <= MAX_PATH, "paths of at most ", MAX_PATH, " rows");
   std::vector<spark::CommitJob> jobs;
+  int64_t pages = -1;
   jobs.reserve(caches.size() + tails.size());
   for (const Tensor& c : caches) {
     NEED(is_act(c.scalar_type()), "caches must be bf16 or fp32");
     const Cache x = need_cache("a cache", c, c.scalar_type(), dev);
     const int64_t e = c.element_size();
-    if (c.numel()) jobs.push_back({static_cast<char*>(c.data_ptr()), nullptr, x.page * e, x.tok * e, static_cast<int>(x.width * e), static_cast<int>(c.size(0)), 0, 0});
+    pages = pages < 0 ? c.size(0) : std::min(pages, c.size(0));
+    if (c.numel()) jobs.push_back({static_cast<char*>(c.data_ptr()), nullptr, x.page * e, x.tok * e, static_cast<int>(x.width * e), 0});
   }
   for (const auto& [x, t] : tails) {
     NEED(t.dim() == 3 && t.is_contiguous() && t.size(0) == m.tables.size(0) && t.device() == dev && is_act(t.scalar_type()),
@@ -320,7 +322,7 @@ int64_t commit_paths(const RowMaps& m, const Tensor& path, const Tensor& n_path,
     NEED(t.size(2) * e % 16 == 0 && step(x, 0) * e % 16 == 0 && aligned(x) && aligned(t), "rows and tails must start on 16 bytes");
     if (t.numel() && x.numel())
       jobs.push_back({static_cast<char*>(t.data_ptr()), static_cast<char*>(x.data_ptr()), step(x, 0) * e, t.size(2) * e, static_cast<int>(t.size(2) * e),
-                      static_cast<int>(t.size(0)), static_cast<int>(t.size(1)), 0});
+                      static_cast<int>(t.size(1))});
   }
   std::vector<char*> seen;
   for (const auto& j : jobs) seen.push_back(j.base);
@@ -331,7 +333,7 @@ int64_t commit_paths(const RowMaps& m, const Tensor& path, const Tensor& n_path,
   int64_t launches = 0;
   for (size_t at = 0; at < jobs.size(); at += spark::COMMIT_JOBS, ++launches) {
     spark::CommitPaths a{{}, ip(path), ip(n_path), ip(m.starts), ip(m.lengths), ip(m.slots), ip(m.tables), on.dev.status, static_cast<int>(S),
-                         static_cast<int>(P), static_cast<int>(m.tables.size(1)), static_cast<int>(m.tables.size(0))};
+                         static_cast<int>(P), static_cast<int>(m.tables.size(1)), static_cast<int>(m.tables.size(0)), static_cast<int>(pages)};
     const int n = static_cast<int>(std::min<size_t>(spark::COMMIT_JOBS, jobs.size() - at));
     int most = 0;
     for (int i = 0; i < n; ++i) { a.job[i] = jobs[at + i]; most = std::max(most, a.job[i].bytes); }

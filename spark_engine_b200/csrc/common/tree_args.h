@@ -36,14 +36,14 @@ struct CommitJob {
   char* base;                            // a cache, or the tail of a convolution
   const char* x;                         // null: a cache; else the rows behind the tail
   long long page, tok;                   // bytes: strides of a cache's pages and tokens, or of a slot's entries (tok) and of x's rows (page)
-  int bytes, extent, kept, pad;          // bytes of a row (multiple of 16); pages of the cache, or slots of the tail; a slot's entries
+  int bytes, kept;                       // bytes of a row (multiple of 16); a slot's entries
 };
 constexpr int COMMIT_JOBS = 128;
 struct CommitPaths {
   CommitJob job[COMMIT_JOBS];
   const int *path, *n_path, *starts, *lengths, *slots, *tables;
   int* status;
-  int S, P, ld, n_slots;
+  int S, P, ld, n_slots, pages;          // pages: of the caches of the whole call, the fewest (-1: it has none)
 };
 
 struct TreeAttn {

@@ -374,16 +374,16 @@ commit_paths_kernel(const __grid_constant__ CommitPaths a) {
     s_path[i] = p;
   }
   ok = __syncthreads_and(ok);
-  if (ok && !jb.x) {
+  // (the caches' rows are looked up for tails as well: all jobs of a request go ahead, or none does)
+  if (ok && a.pages >= 0)
     for (int i = t; i < n; i += 128) {
       const long long from = static_cast<long long>(len) + s_path[i], to = static_cast<long long>(len) + i;
       const int pf = from / TREE_PAGE < a.ld ? a.tables[static_cast<size_t>(slot) * a.ld + from / TREE_PAGE] : -1;
       const int pt = to / TREE_PAGE < a.ld ? a.tables[static_cast<size_t>(slot) * a.ld + to / TREE_PAGE] : -1;
-      if (pf < 0 || pt < 0 || pf >= jb.extent || pt >= jb.extent) ok = false;
+      if (pf < 0 || pt < 0 || pf >= a.pages || pt >= a.pages) ok = false;
       src[i] = pf * TREE_PAGE + static_cast<int>(from % TREE_PAGE);
       dst[i] = pt * TREE_PAGE + static_cast<int>(to % TREE_PAGE);
     }
-  } else if (ok && slot >= jb.extent) ok = false;
   ok = __syncthreads_and(ok);
   if (!ok) {
     if (t == 0) set_status(a.status, ST_BOUNDS, s, slot, n);
@@ -463,9 +463,9 @@ extern "C" int spark_path_conv(const PathConv* a, int f32, cudaStream_t s) {
 // `most`: bytes of the widest job's row.
 extern "C" int spark_commit_paths(const CommitPaths* a, int jobs, int most, cudaStream_t s) {
   if (a->S <= 0 || jobs <= 0 || a->P <= 0) return 0;
-  if (jobs > COMMIT_JOBS || a->P > 4096 || a->ld <= 0 || (most & 15) || most <= 0) return -5;
+  if (jobs > COMMIT_JOBS || a->P > 4096 || a->ld <= 0 || (most & 15) || most <= 0 || a->pages > (1 << 24)) return -5;
   for (int i = 0; i < jobs; ++i)
-    if (a->job[i].extent > (1 << 24) || (a->job[i].bytes & 15) || a->job[i].bytes > most) return -5;
+    if ((a->job[i].bytes & 15) || a->job[i].bytes > most || (!a->job[i].x && a->pages < 0)) return -5;
   spark_launch_pdl(commit_paths_kernel, dim3(a->S, (most / 16 + 127) / 128, jobs), dim3(128), a->P * 12, s, dim3(1, 1, 1), *a);
   return spark_launch_rc(__func__);
 }

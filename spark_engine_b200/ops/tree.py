@@ -276,8 +276,9 @@ def _plain_attention(q, k, v, maps, scale, softcap, bias, slopes, sink, window, 
 def commit_paths(maps: "RowMaps", path, n_path, caches: Sequence[torch.Tensor], tails: Sequence[Tuple[torch.Tensor, torch.Tensor]] = ()):
     """Keep the accepted rows of every request: path [S, P] int32, its first n_path[s] entries the accepted rows' indices in ascending order
     (0: nothing happens to the request).  In every cache [pages, 64, ...] row path[i] of the request moves to its token length + i, and each
-    tail [slots, kept, C] of `tails` = [(x [R, C], tail), ...] becomes the last `kept` of (tail, accepted rows of x).  No two of the
-    caches and tails may share memory."""
+    tail [slots, kept, C] of `tails` = [(x [R, C], tail), ...] becomes the last `kept` of (tail, accepted rows of x).  A request whose path
+    does not ascend, or whose accepted rows are not in pages that all caches of the call have, stays as it is in every cache and tail.  No
+    two of the caches and tails may share memory."""
     run = _kernels(maps.tables)
     calls = _native().commit_paths(maps, path, n_path, caches, tails, run)
     if run:

@@ -482,3 +482,33 @@ def test_commit_of_lengths_beyond_the_table(length):
     ops.commit_paths(m, r.i32([[0, 2, 5], [0, 2, 3]]), r.i32([3, 3]), [k])
     expect_status()
     assert torch.equal(k, want)
+
+
+@pytest.mark.parametrize("layers", [1, 70])            # one launch, and two
+def test_a_request_is_committed_everywhere_or_nowhere(layers):
+    """A missing page, or one that only some of the caches have: neither caches nor tails of the request change, those of the others do."""
+    for bad in (-1, "past the smallest cache", 1 << 30):
+        r = U.Round([60, 90, 126], [9, 6, 4], device=DEV, spare=4)
+        m = ops.slot_maps(**r.inputs())
+        caches = [r.randn(r.n_pages, 64, 2, 8) for _ in range(layers)] + [r.randn(r.n_pages, 64, 1, 16, dtype=BF16)]
+        tails = [(r.randn(r.R, 32), r.randn(3, 2, 32)) for _ in range(layers)]
+        path, n_path = r.i32([[0, 2, 4, 6, 8], [0, 2, 3, 3, 3], [0, 1, 3, 3, 3]]), r.i32([5, 3, 3])
+        want_c, want_t = [c.clone() for c in caches], [t.clone() for _, t in tails]
+        ops.commit_paths(m, path, r.i32([0, 3, 3]), want_c, [(x, t) for (x, _), t in zip(tails, want_t)])
+        if bad == "past the smallest cache":
+            most = r.table[1:].max() + 1
+            keep = max(most, r.table[0, 0] + 1)
+            if r.table[0, 1] < keep:                   # (the request's second page lies behind all others)
+                m.tables[0, 1] = int(keep)
+            caches.append(r.randn(int(keep), 64, 2, 8))
+            want_c.append(caches[-1].clone())
+            ops.commit_paths(m, path, r.i32([0, 3, 3]), want_c[-1:])
+        else:
+            m.tables[0, 1] = bad
+        ops.commit_paths(m, path, n_path, caches, tails)
+        expect_status()
+        assert all(torch.equal(a, b) for a, b in zip(caches, want_c)) and all(torch.equal(t, b) for (_, t), b in zip(tails, want_t))
+    m.tables[0, 1] = -1                              # without caches nothing depends on pages
+    x, t = tails[0]
+    ops.commit_paths(m, path, r.i32([5, 0, 0]), [], [(x, t)])
+    assert torch.equal(t[0], x[[6, 8]]) and torch.equal(t[1:], want_t[0][1:])
