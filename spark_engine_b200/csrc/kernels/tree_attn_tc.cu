@@ -35,7 +35,7 @@ template <int DC, int NQ> struct Tc {
   static constexpr bool QT = DC == 256;                      // queries in tensor memory: shared memory has no room for them beside the ring
   static constexpr int SLOT = TA_PAGE * DC * 2, Q_BYTES = QT ? 0 : 128 * DC * 2;
   static constexpr int SLOTS = DC == 256 ? 6 : DC == 128 ? (NQ == 2 ? 9 : 4) : (NQ == 2 ? 16 : 8);
-  static constexpr int BARS = 2 * SLOTS + 10 * NQ + 2 * TC_ITEMS;
+  static constexpr int BARS = 2 * SLOTS + 11 * NQ + 2 * TC_ITEMS;
   static constexpr int SMEM = 1024 + NQ * Q_BYTES + SLOTS * SLOT + BARS * 8 + 16 + TC_ITEMS * static_cast<int>(sizeof(TreeItem)) + 4 + SLOTS * 8;
   static constexpr bool TWO = NQ == 1;
   // per tile: scores, weights (high and low terms of 32 columns each, or two places for high ones), the accumulator
@@ -123,7 +123,8 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
   uint64_t* v_seen = o_full + 2 * NQ;                        // warp 1 has looked over a masked page's values
   uint64_t* v_read = v_seen + NQ;                            // the tile's softmax warps know of it (tile 1 may be masked pages behind tile 0)
   uint64_t* v_sync = v_read + NQ;                            // [NQ]: of 4 and of 8 softmax warps
-  uint64_t* item_full = v_sync + NQ;                         // [TC_ITEMS]
+  uint64_t* drained = v_sync + NQ;                           // [NQ]: the tile's products have all ended
+  uint64_t* item_full = drained + NQ;                        // [TC_ITEMS]
   uint64_t* item_read = item_full + TC_ITEMS;                // [TC_ITEMS]: by every warp but the producer
   TreeItem* items = reinterpret_cast<TreeItem*>((reinterpret_cast<uintptr_t>(ring + SLOTS * SLOT + L::BARS * 8) + 15) & ~uintptr_t(15));      // [TC_ITEMS]
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(items + TC_ITEMS);
@@ -134,7 +135,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     for (int s = 0; s < SLOTS; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], NQ); }
     for (int s = 0; s < NQ; ++s) {
       mbar_init(&q_full[s], 4); mbar_init(&s_full[s], 1); mbar_init(&s_read[s], 4);
-      mbar_init(&v_seen[s], 1); mbar_init(&v_read[s], 4); mbar_init(&v_sync[s], 4 * (s + 1));
+      mbar_init(&v_seen[s], 1); mbar_init(&v_read[s], 4); mbar_init(&v_sync[s], 4 * (s + 1)); mbar_init(&drained[s], 1);
     }
     for (int s = 0; s < 2 * NQ; ++s) { mbar_init(&p_full[s], 4); mbar_init(&o_full[s], 1); }
     for (int s = 0; s < TC_ITEMS; ++s) { mbar_init(&item_full[s], 1); mbar_init(&item_read[s], L::WARPS - 1); }
@@ -165,6 +166,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
   if (warp == 0) {
     // ------------------------------------------------------------ producer
     TcCount c;
+    int loads = 0;                                           // slots filled so far
     const int kch = (a.D + 63) / 64, vch = (a.V + 63) / 64;
     TreeRange range = ta_range(a);
 #pragma unroll 1
@@ -202,8 +204,15 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         }
         __syncwarp();
         tc_step<SLOTS>(c);
+        ++loads;
       }
     }
+    // no copy is on its way to shared memory when the CTA ends, whatever ended the loop
+    bool come = true;
+#pragma unroll 1
+    for (int s = 0; s < SLOTS && come; ++s)
+      if (s < c.slot || loads >= SLOTS) come = tc_wait(&full[s], s < c.slot ? c.ph : c.ph ^ 1);
+    if (!come) why = ST_TIMEOUT_MBAR_FULL;
   } else if (warp <= NQ) {
     // ------------------------------------------------------------ MMA issuer of tile q (the whole warp walks, one elected lane issues)
     const int q = warp - 1, ksteps = (a.D + 15) / 16, vn = (a.V + 15) / 16 * 16, vunits = (a.V + 63) / 64 * 8;
@@ -307,6 +316,10 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       }
       n += it.nj;
     }
+    // nor does a product read it, or write tensor memory
+    if (elect_one()) umma_commit(&drained[q]);
+    __syncwarp();
+    if (!tc_wait(&drained[q], 0)) why = ST_TIMEOUT_TMEM_FULL;
   } else {
     // ------------------------------------------------------------ softmax, one row per thread
     const int q = (warp - L::SOFTMAX) >> 2, quad = warp & 3, row = quad * 32 + lane;
