@@ -46,6 +46,13 @@ __device__ __forceinline__ float log_sigmoid_decay(float x, float inv_tau) {
   return fmaxf((fminf(x, 0.f) - log1pf(expf(-fabsf(x)))) * inv_tau, -105.f);
 }
 
+// The smaller of the two; NaN where either is (fminf gives the other one).
+__device__ __forceinline__ float min_or_nan(float x, float y) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+  return r;
+}
+
 // tanh to fp32 accuracy in the sense of the soft cap: the Taylor polynomial near 0 (where the quotient form would cancel),
 // 1 - 2 / (exp(2z) + 1) elsewhere (absolute error of a few 2^-23).  The polynomial gives tanh(z) / z.
 constexpr float CAP_NEAR = 0.25f;

@@ -420,8 +420,8 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
               for (int i = 0; i < 64; ++i) big[i & 3] = fmaxf(big[i & 3], fabsf(s[i]));
               if (__any_sync(0xffffffffu, fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3])) * fabsf(to_z) >= CAP_NEAR)) {
 #pragma unroll
-                for (int i = 0; i < 64; ++i) {               // (cap_tanh with the approximate instructions)
-                  const float z = s[i] * to_z, e = tc_ex2(fminf(z, 40.f) * (2.f * TA_LOG2E));
+                for (int i = 0; i < 64; ++i) {               // (cap_tanh with the approximate instructions; NaN stays NaN)
+                  const float z = s[i] * to_z, e = tc_ex2(min_or_nan(z, 40.f) * (2.f * TA_LOG2E));
                   s[i] = a.cap * (fabsf(z) < CAP_NEAR ? z * tanh_over_z(z) : fmaf(-2.f, tc_rcp(1.f + e), 1.f));
                 }
               } else {

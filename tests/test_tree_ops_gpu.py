@@ -512,3 +512,67 @@ def test_a_request_is_committed_everywhere_or_nowhere(layers):
     x, t = tails[0]
     ops.commit_paths(m, path, r.i32([5, 0, 0]), [], [(x, t)])
     assert torch.equal(t[0], x[[6, 8]]) and torch.equal(t[1:], want_t[0][1:])
+
+
+OPTIONS = {
+    "soft cap": dict(softcap=2.0), "soft cap and bias": dict(softcap=30.0, bias=100), "bias": dict(bias=100), "slopes": dict(slopes=True),
+    "soft cap, slopes, sink": dict(softcap=5.0, slopes=True, sink=True),
+}
+
+
+@pytest.mark.parametrize("name", list(OPTIONS))
+@pytest.mark.parametrize("near", [0.01, 3.0])          # scores far below the cap's bend, and past it
+@pytest.mark.parametrize("length", [70, 9000])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_what_is_not_a_number_shows_with_options(dtype, length, near, name):
+    """NaN in a query, in a visible key and in an option's table: the rows that it reaches are NaN, the others are as the definition has them."""
+    f = OPTIONS[name]
+    r = U.Round([length, length], [9, 9], device=DEV)
+    q, k, v = r.randn(r.R, 4, 64, dtype=dtype) * near, r.randn(r.n_pages, 64, 2, 64, dtype=dtype), r.randn(r.n_pages, 64, 2, 64, dtype=dtype)
+    opt = {"softcap": f["softcap"]} if "softcap" in f else {}
+    if "bias" in f:
+        opt["bias"] = r.randn(4, f["bias"])
+    if "slopes" in f:
+        opt["slopes"] = torch.linspace(0.001, 0.02, 4, device=DEV)
+    if "sink" in f:
+        opt["sink"] = r.randn(4)
+    m = ops.slot_maps(**r.inputs())
+    want, tol = U.want_attention(r, q, k, v, 0.125, rounded=WEIGHTS[dtype], **opt)
+
+    def check(rows, heads, q=q, k=k, opt=opt):
+        got = ops.tree_attention(q, k, v, m, 0.125, **opt)
+        hit = torch.zeros(r.R, 4, dtype=torch.bool)
+        hit[torch.tensor(rows)[:, None], torch.tensor(heads)] = True
+        assert torch.equal(got.isnan().all(-1).cpu(), hit) and torch.equal(got.isnan().any(-1).cpu(), hit)
+        U.close(got.cpu()[~hit], want[~hit], tol[~hit], dtype)
+
+    spoiled = q.clone()
+    spoiled[3, 1] = float("nan")
+    check([3], [1], q=spoiled)
+    for at, rows in ((5, list(range(9))), (length - 1, list(range(9))), (length + 4, [j for j in range(9) if r.anc[0][j, 4]])):
+        spoiled = k.clone()
+        spoiled.view(-1, 2, 64)[r.rows(0)[at], 1, 7] = float("nan")
+        check(rows, [2, 3], k=spoiled)
+    for n in ("bias", "slopes", "sink"):
+        if n in opt:
+            spoiled = opt[n].clone()
+            spoiled[2] = float("nan")
+            check(list(range(r.R)), [2], opt={**opt, n: spoiled})
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_infinite_scores_are_capped(dtype):
+    """Products past the largest number are scores of plus and minus the cap (held to 8 half steps of fp32, a weight to 16, the sums to one a token)."""
+    r = U.Round([300], [9], device=DEV)
+    q, k, v = r.randn(r.R, 4, 64, dtype=dtype), r.randn(r.n_pages, 64, 2, 64, dtype=dtype), r.randn(r.n_pages, 64, 2, 64, dtype=dtype)
+    q[:, :, 5], k[:, :, :, 5] = 3e38, 3e38 * torch.sign(k[:, :, :, 5].float()).to(dtype)
+    got = ops.tree_attention(q, k, v, ops.slot_maps(**r.inputs()), 1.0, softcap=3.0)
+    rows, seen = torch.tensor(r.rows(0), device=DEV), torch.ones(9, 309, dtype=torch.bool, device=DEV)
+    seen[:, 300:] = torch.tensor(r.anc[0], device=DEV)
+    want = torch.zeros(9, 4, 64, dtype=torch.float64, device=DEV)
+    tol = torch.zeros_like(want)
+    for h in range(4):
+        x = torch.where(seen, 3.0 * torch.sign(k.view(-1, 2, 64)[rows, h // 2, 5].double()), -torch.inf)
+        p, vv = torch.softmax(x, 1), v.view(-1, 2, 64)[rows, h // 2].double()
+        want[:, h], tol[:, h] = p @ vv, p @ vv.abs() * ((2 * 3 * 8 + 16 + 309) * 2.0 ** -24 + WEIGHTS[dtype])
+    U.close(got, want.cpu(), tol.cpu(), dtype)
