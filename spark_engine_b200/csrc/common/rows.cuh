@@ -54,14 +54,14 @@ __device__ __forceinline__ float min_or_nan(float x, float y) {
 }
 
 // tanh to fp32 accuracy in the sense of the soft cap: the Taylor polynomial near 0 (where the quotient form would cancel),
-// 1 - 2 / (exp(2z) + 1) elsewhere (absolute error of a few 2^-23).  The polynomial gives tanh(z) / z.
+// 1 - 2 / (exp(2z) + 1) elsewhere (absolute error of a few 2^-23; NaN of NaN).  The polynomial gives tanh(z) / z.
 constexpr float CAP_NEAR = 0.25f;
 __device__ __forceinline__ float tanh_over_z(float z) {
   const float s = z * z;
   return fmaf(s, fmaf(s, fmaf(s, fmaf(s, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f);
 }
 __device__ __forceinline__ float cap_tanh(float z) {
-  const float near = z * tanh_over_z(z), far = 1.f - __fdividef(2.f, 1.f + __expf(2.f * fminf(z, 40.f)));
+  const float near = z * tanh_over_z(z), far = 1.f - __fdividef(2.f, 1.f + __expf(2.f * min_or_nan(z, 40.f)));
   return fabsf(z) < CAP_NEAR ? near : far;
 }
 

@@ -281,3 +281,24 @@ def test_trace_runner(tmp_path):
     get = lambda i: torch.from_numpy(np.fromfile(tmp_path / f"{i}.f32", "<f4").reshape(-1, cfg["vocab"]))
     assert U.error(get(0), want[[0, 39]]) < 3e-5 and U.error(get(2), want[[69, 0]]) < 3e-5
     assert not (tmp_path / "1.f32").exists()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("large", [0.02, 4.0])         # scores far below the soft cap, and past it
+@pytest.mark.parametrize("rows", [40, 90])             # (rows of prompts)
+@pytest.mark.parametrize("dim,vdim", [(64, 64), (20, 36), (320, 272)])
+def test_what_is_not_a_number_shows_under_a_soft_cap(dim, vdim, rows, large, dtype):
+    cfg, T = _setup(dict(layers=[U.layer(heads=4, kv_heads=2, dim=dim, vdim=vdim, conv=1, softcap=2.0, chunk=1000, scale=0.3)]), 3)
+    m = U.framework(cfg, T, DEV, dtype)
+    toks = U.prompt(40 + rows, cfg["vocab"])
+    m.forward(make_plan([(0, toks, 0)], device=DEV, all_logits=False))
+    mix = m.layers[0][1]
+    g = torch.Generator().manual_seed(1)
+    proj = (torch.randn(rows, mix.columns, generator=g) * large).to(dtype).to(DEV)
+    plan = make_plan([(0, toks[40:], 40)], device=DEV)
+    assert torch.isfinite(mix.attend(proj, plan, False)).all()
+    proj[-1, mix.Dp: 2 * mix.Dp] = float("nan")        # the last row's second query head
+    got = mix.attend(proj, plan, False).view(rows, 4, -1)
+    hit = torch.zeros(rows, 4, dtype=torch.bool)
+    hit[-1, 1] = True
+    assert torch.equal(got.isnan().all(-1).cpu(), hit) and torch.equal(got.isnan().any(-1).cpu(), hit)
