@@ -8,8 +8,10 @@ parents the rows are chains.  Lengths, counts, parents, tables and paths live on
 The maps refer to lengths, tables, slots and parents, which have to stay as they are until the round is committed; requests of one round
 have different slots, and pages that only one of them writes to.
 
-The calls neither wait for the device nor read from it.  What they can only find out there (a missing page, a parent behind its child, a
-path that does not ascend) skips the row, or the request in `commit_paths`, and sets the device status word."""
+The calls neither wait for the device nor read from it.  What they can only find out there sets the device status word: what would be
+written to a missing page or read from one is left out, a row whose parent is not in front of it hangs off the committed tokens, and
+`commit_paths` skips a request whose path does not ascend or whose pages are missing.  The plain forms, for tensors on the host, leave missing
+pages out as well, and raise for such parents and commits before anything has changed."""
 from __future__ import annotations
 
 import ctypes
@@ -162,6 +164,17 @@ def _plain_maps(m):
     return m
 
 
+def _cache_rows(maps, slot: int, tokens, pages: int) -> torch.Tensor:
+    """Cache rows of a request's tokens; -1 where its table leads nowhere in a cache of `pages` pages."""
+    tables = maps.tables
+    t = torch.as_tensor(tokens, dtype=torch.long, device=tables.device)
+    if not 0 <= slot < tables.shape[0]:
+        return torch.full_like(t, -1)
+    page = tables[slot, (t // PAGE).clamp_max(tables.shape[1] - 1)].long()
+    there = (t // PAGE < tables.shape[1]) & (page >= 0) & (page < pages)
+    return torch.where(there, page * PAGE + t % PAGE, -1)
+
+
 # ----------------------------------------------------------------------------- convolution along paths
 def path_conv(x, w, tail, maps: "RowMaps", nq: int, k, v) -> torch.Tensor:
     """y_j = sum_t w[t] u_t over the row itself (t = taps - 1), its ancestors, then the request's past `tail` [slots, taps - 1, C] (newest
@@ -198,7 +211,7 @@ def _plain_conv(x, w, tail, maps, nq, k, v):
                 back += 1
                 u = tail[slot, taps - 1 - back]
             y[r] += w[t] * u.float()
-        if row >= 0:
+        if 0 <= row < k.shape[0] * PAGE:
             kf[row // PAGE, row % PAGE] = y[r, nq: nq + nk].to(k.dtype)
             vf[row // PAGE, row % PAGE] = y[r, nq + nk:].to(v.dtype)
     return y[:, :nq].to(x.dtype)
@@ -232,9 +245,11 @@ def _plain_attention(q, k, v, maps, scale, softcap, bias, slopes, sink, window, 
         r0, n = starts[s], starts[s + 1] - starts[s]
         if n == 0:
             continue
+        L = min(max(L, 0), maps.tables.shape[1] * PAGE)          # (what lies behind the table's last page is not there)
         t = torch.arange(L + n, device=q.device)
-        page = maps.tables[slot, t // PAGE].long()
-        kk, vv = kf[page.clamp_min(0), t % PAGE].float().view(-1, G, D), vf[page.clamp_min(0), t % PAGE].float().view(-1, G, V)
+        row = _cache_rows(maps, slot, t, k.shape[0])
+        page = row.clamp_min(0) // PAGE
+        kk, vv = kf[page, t % PAGE].float().view(-1, G, D), vf[page, t % PAGE].float().view(-1, G, V)
         pos, j = maps.pos[r0: r0 + n].long(), torch.arange(n, device=q.device)
         at = torch.cat((t[:L], pos))
         if maps.anc is not None:
@@ -242,7 +257,7 @@ def _plain_attention(q, k, v, maps, scale, softcap, bias, slopes, sink, window, 
         else:
             tree = j.unsqueeze(1) >= j
         dist = pos.unsqueeze(1) - at
-        seen = torch.cat((torch.ones(n, L, dtype=torch.bool, device=q.device), tree), 1) & (page >= 0)
+        seen = torch.cat((torch.ones(n, L, dtype=torch.bool, device=q.device), tree), 1) & (row >= 0)
         if window:
             seen &= dist < window
         if chunk:
@@ -289,16 +304,25 @@ def commit_paths(maps: "RowMaps", path, n_path, caches: Sequence[torch.Tensor], 
 
 def _plain_commit(maps, path, n_path, caches, tails):
     slots = maps.slots.tolist() if maps.slots is not None else range(maps.lengths.shape[0])
+    pages = min((c.shape[0] for c in caches), default=None)
+    todo = []
     for s, (slot, L, n) in enumerate(zip(slots, maps.lengths.tolist(), n_path.tolist())):
         rows = path[s, : max(n, 0)].tolist()
         count = int(maps.starts[s + 1] - maps.starts[s])
         _need(all(0 <= a < count for a in rows) and all(a < b for a, b in zip(rows, rows[1:])), "an accepted path must ascend within its request")
-        at = lambda j: (int(maps.tables[slot, (L + j) // PAGE]), (L + j) % PAGE)
+        if not rows:
+            continue
+        _need(0 <= slot < maps.tables.shape[0], "a request without a row of the tables")
+        src = dst = None
+        if pages is not None:
+            src, dst = (_cache_rows(maps, slot, [max(L, 0) + j for j in at], pages).tolist() for at in (rows, range(len(rows))))
+            _need(min(src + dst) >= 0, "an accepted row without a page")
+        todo.append((slot, int(maps.starts[s]), rows, src, dst))
+    for slot, r0, rows, src, dst in todo:            # (nothing has moved until all of them are known to be good)
         for c in caches:
             flat = _flat(c, int(math.prod(c.shape[2:])))
-            for i, j in enumerate(rows):
-                if i != j:
-                    flat[at(i)] = flat[at(j)]
+            for a, b in zip(src, dst):
+                if a != b:
+                    flat[b // PAGE, b % PAGE] = flat[a // PAGE, a % PAGE]
         for x, t in tails:
-            if rows:
-                t[slot] = torch.cat((t[slot], x[int(maps.starts[s]) + torch.tensor(rows, device=x.device)]))[len(rows):]
+            t[slot] = torch.cat((t[slot], x[r0 + torch.tensor(rows, device=x.device)]))[len(rows):]

@@ -332,3 +332,56 @@ def test_rows_that_start_anywhere_are_made_readable(name, dtype):
         assert torch.equal(heads, y) and y.data_ptr() % 16 == 0 and y.stride(2) == 1 and all(y.shape[i] == 1 or y.stride(i) % 8 == 0 for i in range(2))
     good = torch.zeros(3, 40, dtype=dtype)[:, :32]
     assert tree._native().pieces(good, 8).data_ptr() == good.data_ptr()
+
+
+# ----------------------------------------------------------------------------- tables that lead nowhere
+def _spoiled(bad):
+    """A request that crosses into a page that is not there, one beside it that is whole."""
+    r = U.Round([60, 90], [9, 6], spare=1)
+    r.table[0, 1] = r.n_pages if bad == "past the cache" else -1
+    d = r.inputs()
+    if bad == "past the table":
+        r.table[0, 1] = 0
+        d["tables"] = r.i32(r.table)
+        d["lengths"] = r.i32([126, 90])
+    if bad == "no row of the tables":
+        d["slots"] = r.i32([7, 1])
+    return r, ops.slot_maps(**d)
+
+
+@pytest.mark.parametrize("bad", ["missing", "past the cache", "past the table", "no row of the tables"])
+def test_commit_without_a_page_changes_nothing(bad):
+    r, m = _spoiled(bad)
+    caches, tail = [r.randn(r.n_pages, 64, 2, 8), r.randn(r.n_pages, 64, 1, 12)], (r.randn(r.R, 24), r.randn(2, 3, 24))
+    before = [c.clone() for c in caches] + [tail[1].clone()]
+    path = r.i32([[0, 1, 2, 5, 6, 8], [0, 2, 3, 9, 9, 9]])
+    with pytest.raises(ValueError):
+        ops.commit_paths(m, path, r.i32([6, 3]), caches, [tail])
+    assert all(torch.equal(a, b) for a, b in zip(before, caches + [tail[1]]))
+    ops.commit_paths(m, path, r.i32([0, 3]), caches, [tail])          # the other request alone
+    assert torch.equal(tail[1][0], before[2][0]) and torch.equal(tail[1][1], tail[0][[9, 11, 12]])
+
+
+@pytest.mark.parametrize("bad", ["missing", "past the cache", "past the table"])
+def test_rows_without_a_page_are_left_out(bad):
+    """Attention does not see what is not there, and the convolution writes nothing: no other page is read or written in its place."""
+    r, m = _spoiled(bad)
+    q, k, v = r.randn(r.R, 4, 16), r.randn(r.n_pages, 64, 2, 16), r.randn(r.n_pages, 64, 2, 8)
+    got = ops.tree_attention(q, k, v, m, 0.25)
+    good = U.Round([60, 90], [9, 6], spare=1)
+    there = ops.slot_maps(**good.inputs())
+    want = ops.tree_attention(q, k, v, there, 0.25)
+    assert torch.isfinite(got).all() and torch.equal(got[9:], want[9:])
+    if bad != "past the table":                      # tokens 0 .. 63 alone: nodes 0 .. 3 are in the first page
+        anc = there.anc.clone()
+        there.anc[:9] &= 15
+        assert torch.allclose(got[:9], ops.tree_attention(q, k, v, there, 0.25)[:9], rtol=1e-5, atol=1e-6)
+        there.anc.copy_(anc)
+    w, tail, x = r.randn(3, 40), r.randn(2, 2, 40), r.randn(r.R, 40)
+    k, v = r.randn(r.n_pages, 64, 2, 8), r.randn(r.n_pages, 64, 1, 8)
+    k0, k1 = k.clone(), k.clone()
+    out = ops.path_conv(x, w, tail, m, 16, k, v)
+    assert torch.equal(out, ops.path_conv(x, w, tail, there, 16, k1, v.clone()))
+    used = set(good.rows(1)[90:].tolist()) | (set(r.rows(0)[60:64].tolist()) if bad != "past the table" else set(r.table[0, 1] * 64 + np.arange(62, 64)))
+    changed = set(torch.nonzero((k != k0).flatten(2).any(2).flatten()).flatten().tolist())
+    assert changed == {int(t) for t in used}
