@@ -144,6 +144,7 @@ def _plain_maps(m):
     r, starts = 0, [0]
     slots = m.slots.tolist() if m.slots is not None else range(len(counts))
     for slot, L, n in zip(slots, m.lengths.tolist(), counts):
+        L = max(L, 0)
         par = m.parents[r: r + n].tolist() if m.parents is not None else [j - 1 for j in range(n)]
         _need(all(-1 <= p < j for j, p in enumerate(par)) and (m.parents is None or n <= m.nodes), "a tree's nodes must follow their parents")
         depth, anc = [], []

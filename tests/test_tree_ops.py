@@ -385,3 +385,13 @@ def test_rows_without_a_page_are_left_out(bad):
     used = set(good.rows(1)[90:].tolist()) | (set(r.rows(0)[60:64].tolist()) if bad != "past the table" else set(r.table[0, 1] * 64 + np.arange(62, 64)))
     changed = set(torch.nonzero((k != k0).flatten(2).any(2).flatten()).flatten().tolist())
     assert changed == {int(t) for t in used}
+
+
+def test_negative_lengths_are_zero():
+    r = U.Round([0, 70], [3, 4])
+    d = r.inputs()
+    want = ops.slot_maps(**d)
+    got = ops.slot_maps(**{**d, "lengths": r.i32([-1, 70])})
+    assert torch.equal(got.pos, want.pos) and torch.equal(got.cache_row, want.cache_row)
+    q, k, v = r.randn(r.R, 4, 16), r.randn(r.n_pages, 64, 2, 16), r.randn(r.n_pages, 64, 2, 8)
+    assert torch.equal(ops.tree_attention(q, k, v, got, 0.25), ops.tree_attention(q, k, v, want, 0.25))
