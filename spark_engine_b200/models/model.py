@@ -920,7 +920,7 @@ class Model:
         from the segment's first row (always accepted: it is the last sampled token)."""
         plan = self._pending_plan
         assert plan is not None, "commit() without a pending verify"
-        if plan.is_tree and self.page:
+        if plan.maps is not None:            # trees with branches over pages; chains are committed layer by layer
             self._commit_trees(plan, accepted)
         for mix in self.stateful(drafter=False):
             mix.commit(accepted)

@@ -60,7 +60,7 @@ class PagedGqaMixer(PendingRows):
 
     def attend(self, proj, plan: Plan, commit: bool, out=None):
         """Heads' outputs [R, heads * padded value width] of the projected rows (into `out` if given)."""
-        if plan.is_tree:
+        if plan.branches:
             assert not commit, "a tree's rows are committed by their accepted path"
             return self._tree(proj, plan, out)
         o = ops.paged_gqa(self, proj, plan, commit, out)
@@ -157,6 +157,10 @@ class PagedGqaMixer(PendingRows):
                 o = o * torch.sigmoid(proj[sl, self.columns: self.columns + H].float()).unsqueeze(-1)
             out[sl] = (o * self.out_scale).reshape(s.n, H * V).to(out.dtype)
         return out
+
+    def compact(self, seqs, seg, rows):
+        """(The rows of trees with branches have been moved in all layers at once, see `pending_tree`.)"""
+        assert self.takes_trees or rows == list(range(len(rows))), "paged attention rows verify chains"
 
     def pending_tree(self):
         """(caches, (rows, tail) of the convolutions) that wait for a tree's accepted path; nothing waits any more."""

@@ -34,7 +34,7 @@ class Plan:
     has_media: bool = False                   # some ids are salted media placeholders (outside the vocabulary)
     mm_rows: Optional[list] = None            # multimodal: [(first row, tensor [n, hidden])] written over the embedding
                                               # rows of salted placeholder ids (multimodal/canvas.py)
-    maps: Optional[object] = None             # trees over a paged cache: ops.RowMaps of the rows (`tree_maps`)
+    maps: Optional[object] = None             # trees over a paged cache: the rows' `ops.slot_maps` (`tree_maps`)
 
     @property
     def rows(self) -> int:
@@ -43,6 +43,11 @@ class Plan:
     @property
     def is_tree(self) -> bool:
         return any(s.parents is not None for s in self.segs)
+
+    @property
+    def branches(self) -> bool:
+        """Some segment is a tree that is not a chain."""
+        return any(s.parents is not None and any(p != j - 1 for j, p in enumerate(s.parents)) for s in self.segs)
 
 
 def depth_of(parents: List[int]) -> List[int]:

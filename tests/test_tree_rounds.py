@@ -123,3 +123,56 @@ def test_nodes_see_their_paths_on_the_device(name, dtype):
 def test_tree_rounds_are_lossless_on_the_device(name):
     ref, seq, rounds = check_rounds(name, "cuda", torch.float32)
     assert seq.generated[:16] == ref and rounds <= 5 and seq.accepted >= 10
+
+
+# ----------------------------------------------------------------------------- trees that are chains
+def _family(name):
+    import vabunex_util as VU
+    import zakusun_util as KU
+    import zapolorn_util as ZU
+    from test_vabunex import MIXED as vabunex
+    u, layers = {"debisun": (U, U.MIXED), "vabunex": (VU, vabunex), "zakusun": (KU, KU.MIXED), "zapolorn": (ZU, ZU.MIXED)}[name]
+    cfg = u.config(**layers)
+    return u, cfg, u.tensors(cfg)
+
+
+def check_chains(name, device):
+    """A plan whose trees are chains is verified and committed by every paged model as the plan without parents is."""
+    u, cfg, T = _family(name)
+    g = torch.Generator().manual_seed(4)
+    toks = {s: torch.randint(0, cfg["vocab"], (n,), generator=g).tolist() for s, n in ((1, 70), (2, 20))}
+    got = []
+    for parents in (None, [[-1, 0, 1, 2], [-1, 0]], [None, [-1, 0]]):
+        m = u.framework(cfg, T, device)
+        for s, t in toks.items():
+            m.forward(make_plan([(s, t[:-12], 0)], device=device, all_logits=False))
+        outs, at = [], {s: len(t) - 12 for s, t in toks.items()}
+        for accepted in ([[0, 1], [0]], [[0, 1, 2], [0, 1]], [[], [0]]):
+            plan = make_plan([(s, t[at[s]: at[s] + n], at[s]) for (s, t), n in zip(toks.items(), (4, 2))], device=device, parents=parents)
+            outs.append(m.forward(plan, commit=False).float().cpu())
+            m.commit([list(a) for a in accepted])
+            for s, a in zip(toks, accepted):
+                at[s] += len(a)
+            assert [m.seqs[s].length for s in toks] == list(at.values())
+        got.append(torch.cat(outs))
+    for x in got[1:]:
+        assert U.error(x, got[0]) < 1e-6
+
+
+@pytest.mark.parametrize("name", ["debisun", "vabunex", "zakusun", "zapolorn"])
+def test_trees_that_are_chains(name):
+    check_chains(name, "cpu")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["debisun", "vabunex", "zakusun", "zapolorn"])
+def test_trees_that_are_chains_on_the_device(name):
+    check_chains(name, "cuda")
+
+
+def test_branches_are_refused_where_rows_verify_chains():
+    u, cfg, T = _family("zapolorn")
+    m = u.framework(cfg, T)
+    m.forward(make_plan([(0, [1, 2, 3], 0)], all_logits=False))
+    with pytest.raises(AssertionError):
+        m.forward(make_plan([(0, [4, 5, 6], 3)], parents=[[-1, 0, 0]]), commit=False)
