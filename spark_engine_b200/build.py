@@ -15,6 +15,7 @@ import os
 import subprocess
 import sys
 import sysconfig
+import zlib
 
 ROOT = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(ROOT, "csrc")
@@ -49,11 +50,19 @@ def kernel_library(family: str) -> str:
     """Path of a kernel library that serves `family`, built if need be: the complete one when it is up to date, else one of
     the family's own sources (a first start compiles no more than the model needs; the objects are shared)."""
     build_runtime()
+    if "tree_attn" in FAMILY_SOURCES.get(family, ("tree_attn",)):
+        build_tree()                     # (it fills the kernels' argument structures: the two are built from one header)
     full = os.path.join(LIBDIR, "libspark_kernels.so")
-    srcs = glob.glob(os.path.join(CSRC, "kernels", "*.cu*")) + glob.glob(os.path.join(CSRC, "common", "*.cuh"))
+    srcs = [f for x in ("kernels/*.cu*", "common/*.cuh", "common/*.h") for f in glob.glob(os.path.join(CSRC, x))]
     if not _newer(srcs, full) or family not in FAMILY_SOURCES:
         return full if not _newer(srcs, full) else build_kernels()
     return build_kernels(family=family)
+
+
+def _tree_layout() -> list:
+    """The argument structures that kernels and `_tree` share, as a number that both carry and that is compared when they meet."""
+    with open(os.path.join(CSRC, "common", "tree_args.h"), "rb") as f:
+        return [f"-DSPARK_TREE_LAYOUT={zlib.crc32(f.read())}u"]
 
 
 def build_kernels(force=False, verbose=False, family=None) -> str:
@@ -68,7 +77,7 @@ def build_kernels(force=False, verbose=False, family=None) -> str:
         obj = os.path.join(LIBDIR, os.path.basename(cu)[:-3] + ".o")
         objs.append(obj)
         if force or _newer([cu] + headers, obj):
-            jobs.append([NVCC] + NVCC_FLAGS + (["-Xptxas", "-v"] if verbose else []) + ["-c", cu, "-o", obj])
+            jobs.append([NVCC] + NVCC_FLAGS + _tree_layout() + (["-Xptxas", "-v"] if verbose else []) + ["-c", cu, "-o", obj])
     with cf.ThreadPoolExecutor(max_workers=8) as ex:
         for log in ex.map(_run, jobs):
             if verbose and log:
@@ -103,6 +112,7 @@ def build_tree(force=False) -> str:
         inc = [os.path.join(CSRC, "common"), *ext.include_paths("cuda"), sysconfig.get_paths()["include"]]
         lib = os.path.join(os.path.dirname(torch.__file__), "lib")
         _run(["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-DTORCH_EXTENSION_NAME=_tree", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+             + _tree_layout()
              + ["-isystem" + i if "torch" in i else "-I" + i for i in inc] + [src, "-o", out, "-L" + lib, "-Wl,-rpath," + lib]
              + ["-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10_cuda", "-lc10"])
     return out

@@ -347,6 +347,7 @@ int64_t commit_paths(const RowMaps& m, const Tensor& path, const Tensor& n_path,
 PYBIND11_MODULE(_tree, mod) {
   mod.doc() = "spark_engine_b200: verification of drafted trees over paged caches (checks and launches)";
   mod.def("bind_entry", &bind_entry).def("bind_device", &bind_device).def("pieces", &pieces);
+  mod.def("layout", [] { return SPARK_TREE_LAYOUT; });
   py::class_<RowMaps, std::shared_ptr<RowMaps>>(mod, "RowMaps",
       "Where a round's rows belong (int32 unless said otherwise; -1 for rows behind the last request): slot [R] row of the tables, index [R]\n"
       "within the request, pos [R], cache_row [R] int64 (page * 64 + token; -1 too where the table has no page), starts [S + 1] first row of\n"

@@ -4,6 +4,11 @@
 
 namespace spark {
 
+// This file as a number (given by the build): the bindings launch only kernels that were compiled from the same one.
+#ifndef SPARK_TREE_LAYOUT
+#define SPARK_TREE_LAYOUT 0u
+#endif
+
 constexpr int TREE_PAGE = 64;
 
 struct BlockTables {

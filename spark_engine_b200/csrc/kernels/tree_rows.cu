@@ -411,6 +411,8 @@ commit_paths_kernel(const __grid_constant__ CommitPaths a) {
 
 using namespace spark;
 
+extern "C" unsigned spark_tree_layout() { return SPARK_TREE_LAYOUT; }
+
 extern "C" int spark_block_tables(const BlockTables* a, cudaStream_t s) {
   if (a->S <= 0) return 0;
   if (a->ld <= 0 || a->cap < 0 || static_cast<long long>(a->S) * a->ld > (1 << 24)) return -5;

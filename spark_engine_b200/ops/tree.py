@@ -15,10 +15,10 @@ pages out as well, and raise for such parents and commits before anything has ch
 from __future__ import annotations
 
 import ctypes
-import glob
 import importlib.util
 import math
 import os
+import sysconfig
 from typing import Sequence, Tuple
 
 import torch
@@ -36,12 +36,11 @@ def _native():
     """The bindings (`csrc/bindings/tree_ops.cpp`): checks of arguments, outputs, launches."""
     global _mod
     if _mod is None:
-        lib = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "_lib")
-        paths = glob.glob(os.path.join(lib, "_tree*.so"))
-        if not paths:
+        path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "_lib", "_tree" + sysconfig.get_config_var("EXT_SUFFIX"))
+        if not os.path.exists(path):
             from ..build import build_tree
-            paths = [build_tree()]
-        spec = importlib.util.spec_from_file_location("_tree", paths[0])
+            path = build_tree()
+        spec = importlib.util.spec_from_file_location("_tree", path)
         _mod = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(_mod)
     return _mod
@@ -57,11 +56,21 @@ def _kernels(t: torch.Tensor) -> bool:
     return True
 
 
+def _same_layout(mod, dll):
+    """The bindings fill structures that the kernels read: both have to come from one header."""
+    if not hasattr(dll, "spark_tree_layout"):
+        raise RuntimeError(f"{dll._name} has no tree kernels: run `python -m spark_engine_b200.build`")
+    dll.spark_tree_layout.restype = ctypes.c_uint
+    if dll.spark_tree_layout() != mod.layout():
+        raise RuntimeError(f"{dll._name} and {mod.__file__} were built from different sources: run `python -m spark_engine_b200.build`")
+
+
 def _bind(index: int):
     global _bound
     mod, cu = _native(), cuda_ops()
     if _bound is None:
         dll = cu.lib()
+        _same_layout(mod, dll._dll)
         for name in _ENTRIES:
             mod.bind_entry(name, ctypes.cast(getattr(dll._dll, name), ctypes.c_void_p).value)
         _bound = dll

@@ -395,3 +395,58 @@ def test_negative_lengths_are_zero():
     assert torch.equal(got.pos, want.pos) and torch.equal(got.cache_row, want.cache_row)
     q, k, v = r.randn(r.R, 4, 16), r.randn(r.n_pages, 64, 2, 16), r.randn(r.n_pages, 64, 2, 8)
     assert torch.equal(ops.tree_attention(q, k, v, got, 0.25), ops.tree_attention(q, k, v, want, 0.25))
+
+
+# ----------------------------------------------------------------------------- the two native parts
+def test_kernels_of_other_sources_are_refused():
+    """The bindings and the kernels share argument structures: what was built from another header is not launched."""
+    import ctypes
+
+    from spark_engine_b200 import build
+    from spark_engine_b200.ops import cuda, tree
+    mod = tree._native()
+    flag, = build._tree_layout()
+    assert f"={mod.layout()}u" in flag and mod.layout() != 0
+    assert mod.__file__.endswith(build.sysconfig.get_config_var("EXT_SUFFIX"))
+
+    class Fn:
+        def __init__(self, value):
+            self.value = value
+
+        def __call__(self):
+            return self.value
+
+    class Lib:
+        _name = "libother.so"
+
+    dll = Lib()
+    with pytest.raises(RuntimeError, match="no tree kernels"):
+        tree._same_layout(mod, dll)
+    dll.spark_tree_layout = Fn(mod.layout() ^ 1)
+    with pytest.raises(RuntimeError, match="different sources"):
+        tree._same_layout(mod, dll)
+    dll.spark_tree_layout = Fn(mod.layout())
+    tree._same_layout(mod, dll)
+    try:
+        real = ctypes.CDLL(cuda.LIB_PATH)
+    except OSError:
+        return
+    tree._same_layout(mod, real)
+
+
+def test_a_model_with_trees_builds_both_parts(monkeypatch):
+    """`kernel_library` keeps the bindings in step with the kernels, and a changed argument header makes the complete library stale."""
+    from spark_engine_b200 import build
+    called, seen = [], []
+    monkeypatch.setattr(build, "build_runtime", lambda: called.append("runtime"))
+    monkeypatch.setattr(build, "build_tree", lambda: called.append("tree"))
+    monkeypatch.setattr(build, "build_kernels", lambda **kw: called.append(kw.get("family", "all")))
+    monkeypatch.setattr(build, "_newer", lambda srcs, out: seen.extend(srcs) or True)
+    build.kernel_library("debisun")
+    assert called == ["runtime", "tree", "debisun"] and any(s.endswith("tree_args.h") for s in seen)
+    called.clear()
+    build.kernel_library("vabunex")
+    assert called == ["runtime", "vabunex"]
+    called.clear()
+    build.kernel_library("another family")
+    assert called == ["runtime", "tree", "all"]
