@@ -1,17 +1,18 @@
 // Tree attention on tcgen05 (bf16 caches): the tiles of tree_attn.cu with 128 (node, head) rows per accumulator, a page of keys per step.
 //   warp 0      finds this CTA's items and announces them; TMA: pages of keys and values into a ring of slots in the order the products use
 //               them (K0 K1 V0 K2 V1 ..)
-//   warp 1      issues S = Q K^T one page ahead of O += P V (P in tensor memory): as soon as the softmax warps have loaded a page's scores
+//   warp 1      issues S = Q K^T one page ahead of O += P V (P in tensor memory), into the place whose weights the product has read
 //   the others  softmax, one row per thread: 64 scores are one tensor-memory load, statistics stay in the thread
 // NQ = 2: two tiles of 128 rows with their own issuing and softmax warps share the keys in shared memory (large trees: a page is read once for
 // 256 rows); each tile's products wait for its own softmax alone.
 //
 // Weights are exponentials against a reference that may lag far behind the maximum: the maximum of the first page that a row sees, renewed
 // (and the accumulator rescaled) only when a page's weights add up to more than 2^40; fp32 sums and bf16 weights lose nothing by a common
-// factor.  So most pages need no maximum.  Weights enter the product as two bf16 terms (2^-17 of a weight is lost) where reading the keys
-// takes longer than the products (NQ = 1), and as one (half a step of bf16 each, at random, less than the step that the outputs are rounded to)
-// where it does not: for 256 rows the second term would be a third of all products.  One-term weights have two places, so that a page's
-// weights need not wait for the product of the page before.
+// factor.  So most pages need no maximum.  Weights enter the product as two bf16 terms (2^-17 of a weight is lost), as in all paged attention
+// here: what a round of drafts is verified with does not depend on how large their trees are.  (One term, half a step of bf16 per weight,
+// makes the error of 64 requests of 64 nodes over 4k tokens 1.4 times that of the rounded outputs, and the call 321 us instead of 378.)
+// A page's weights take the place of its scores, and two such places alternate, so that they need not wait for the product of the page
+// before (398 us with weights in one place beside the scores).
 //
 // A page that not every row sees whole (the tree itself, the edge of a window or chunk) is masked by 64 bits per row.  Warp 1 looks its values
 // over first: rows that hold no token of the request are zeroed, and where a value is not finite, 0 * value would spoil the rows that do not
@@ -37,8 +38,7 @@ template <int DC, int NQ> struct Tc {
   static constexpr int SLOTS = DC == 256 ? 6 : DC == 128 ? (NQ == 2 ? 9 : 4) : (NQ == 2 ? 16 : 8);
   static constexpr int BARS = 2 * SLOTS + 11 * NQ + 2 * TC_ITEMS;
   static constexpr int SMEM = 1024 + NQ * Q_BYTES + SLOTS * SLOT + BARS * 8 + 16 + TC_ITEMS * static_cast<int>(sizeof(TreeItem)) + 4 + SLOTS * 8;
-  static constexpr bool TWO = NQ == 1;
-  // per tile: scores, weights (high and low terms of 32 columns each, or two places for high ones), the accumulator
+  // per tile: two places of 64 columns, a page's scores and then its weights (high and low terms, 32 columns each), and the accumulator
   static constexpr int TILE_COLS = 128 + DC, Q_COL = 128 + DC;
   static constexpr int COLS = QT || NQ == 2 ? 512 : 256;
   static constexpr int SOFTMAX = 1 + NQ, WARPS = SOFTMAX + 4 * NQ, THREADS = WARPS * 32, PER_SM = QT || NQ == 2 ? 1 : 2;
@@ -116,10 +116,9 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
   uint64_t* full = reinterpret_cast<uint64_t*>(ring + SLOTS * SLOT);
   uint64_t* empty = full + SLOTS;
   uint64_t* q_full = empty + SLOTS;                          // [NQ]
-  uint64_t* s_full = q_full + NQ;
-  uint64_t* s_read = s_full + NQ;
-  uint64_t* p_full = s_read + NQ;
-  uint64_t* o_full = p_full + 2 * NQ;                        // ([NQ][2] like p_full)
+  uint64_t* s_full = q_full + NQ;                            // [NQ][2], like the next two: of the place
+  uint64_t* p_full = s_full + 2 * NQ;
+  uint64_t* o_full = p_full + 2 * NQ;
   uint64_t* v_seen = o_full + 2 * NQ;                        // warp 1 has looked over a masked page's values
   uint64_t* v_read = v_seen + NQ;                            // the tile's softmax warps know of it (tile 1 may be masked pages behind tile 0)
   uint64_t* v_sync = v_read + NQ;                            // [NQ]: of 4 and of 8 softmax warps
@@ -134,10 +133,10 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV);
     for (int s = 0; s < SLOTS; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], NQ); }
     for (int s = 0; s < NQ; ++s) {
-      mbar_init(&q_full[s], 4); mbar_init(&s_full[s], 1); mbar_init(&s_read[s], 4);
+      mbar_init(&q_full[s], 4);
       mbar_init(&v_seen[s], 1); mbar_init(&v_read[s], 4); mbar_init(&v_sync[s], 4 * (s + 1)); mbar_init(&drained[s], 1);
     }
-    for (int s = 0; s < 2 * NQ; ++s) { mbar_init(&p_full[s], 4); mbar_init(&o_full[s], 1); }
+    for (int s = 0; s < 2 * NQ; ++s) { mbar_init(&s_full[s], 1); mbar_init(&p_full[s], 4); mbar_init(&o_full[s], 1); }
     for (int s = 0; s < TC_ITEMS; ++s) { mbar_init(&item_full[s], 1); mbar_init(&item_read[s], L::WARPS - 1); }
     fence_barrier_init();
   }
@@ -152,7 +151,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
   const int rep = a.H / a.G;
   bool ok = true;
   int why = ST_OK;                                           // what a wait that ran out waited for
-  const auto place = [](int n) { return L::TWO ? 0 : n & 1; };         // barrier and phase of page n's weights
+  const auto place = [](int n) { return n & 1; };                       // of page n, and the phase of its barriers
   const auto announced = [&](int k, TreeItem& it) {                     // item k of this CTA; nj = 0: there is none, or the wait for it ran out
     const bool there = tc_wait(&item_full[k % TC_ITEMS], (k / TC_ITEMS) & 1);
     it = items[k % TC_ITEMS];
@@ -161,7 +160,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     if (!there) { why = ST_TIMEOUT_MBAR_FULL; it.nj = 0; }
     return it.nj > 0;
   };
-  const auto phase = [](int n) { return static_cast<uint32_t>(L::TWO ? n & 1 : (n >> 1) & 1); };
+  const auto phase = [](int n) { return static_cast<uint32_t>(n >> 1 & 1); };
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
@@ -244,7 +243,8 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       for (int j = -1; j < it.nj; ++j) {
         if (j + 1 < it.nj) {
           const int t = n + j + 1;
-          ok = tc_wait(&full[c.slot], c.ph) && (t == 0 || tc_wait(&s_read[q], (t - 1) & 1));
+          // (the weights of two pages back lie where the scores go: their product has read them, and all softmax warps these scores)
+          ok = tc_wait(&full[c.slot], c.ph) && (t < 2 || tc_wait(&o_full[q * 2 + place(t)], phase(t - 2)));
           if (!ok) { why = ST_TIMEOUT_MBAR_FULL; break; }
           tc_fence_after();
           if (elect_one()) {
@@ -253,10 +253,10 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
             for (int k = 0; k < DC / 16; ++k) {
               if (k >= ksteps) break;
               const uint64_t kk = kd + (k >> 2) * (KV_CHUNK >> 4) + 2 * (k & 3);
-              if (L::QT) umma_f16_ts(tm, tm + L::Q_COL + k * 8, kk, id_s, k != 0);
-              else umma_f16(tm, qd + (k >> 2) * (Q_CHUNK >> 4) + 2 * (k & 3), kk, id_s, k != 0);
+              if (L::QT) umma_f16_ts(tm + place(t) * 64, tm + L::Q_COL + k * 8, kk, id_s, k != 0);
+              else umma_f16(tm + place(t) * 64, qd + (k >> 2) * (Q_CHUNK >> 4) + 2 * (k & 3), kk, id_s, k != 0);
             }
-            umma_commit(&s_full[q]);
+            umma_commit(&s_full[q * 2 + place(t)]);
             umma_commit(&empty[c.slot]);
           }
           __syncwarp();
@@ -302,11 +302,11 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         tc_fence_after();
         if (elect_one()) {
           const uint64_t vd = tc_desc_nmajor(rs + c.slot * SLOT, KV_CHUNK);
-          const uint32_t w = tm + 64 + place(n + j) * 32;
+          const uint32_t w = tm + place(n + j) * 64;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             umma_f16_ts(tm + 128, w + k * 8, vd + k * 128, id_o, 1);
-            if (L::TWO) umma_f16_ts(tm + 128, w + 32 + k * 8, vd + k * 128, id_o, 1);
+            umma_f16_ts(tm + 128, w + 32 + k * 8, vd + k * 128, id_o, 1);
           }
           umma_commit(&o_full[q * 2 + place(n + j)]);
           umma_commit(&empty[c.slot]);
@@ -392,26 +392,20 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
             if (n1 >= 0) at_hi = n1 < sg.n ? a.pos[sg.r0 + n1] : p;
           }
         }
-        ok = tc_wait(&s_full[q], n & 1);
+        ok = tc_wait(&s_full[q * 2 + place(n)], phase(n));
         if (!ok) { why = ST_TIMEOUT_TMEM_FULL; break; }
         tc_fence_after();
         float s[64];
-        if (idle) {                                          // (it waits as well: weights of two pages may not be announced in one phase)
-          if (lane == 0) mbar_arrive(&s_read[q]);
-          if (L::TWO && n > 0) ok = tc_wait(&o_full[q * 2], phase(n - 1));
-          if (!ok) { why = ST_TIMEOUT_TMEM_FULL; break; }
-        } else {
+        const uint32_t t_page = t_lane + place(n) * 64;
+        if (!idle) {
           {
             uint32_t raw[2][32];
-            tmem_ld_32x32(t_lane, raw[0]);
-            tmem_ld_32x32(t_lane + 32, raw[1]);
+            tmem_ld_32x32(t_page, raw[0]);
+            tmem_ld_32x32(t_page + 32, raw[1]);
             tmem_ld_wait();
 #pragma unroll
             for (int i = 0; i < 64; ++i) s[i] = __uint_as_float(raw[i >> 5][i & 31]);
           }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&s_read[q]);
           if (FEAT) {
             if (a.cap > 0.f) {
               const float to_z = a.scale / a.cap;
@@ -489,12 +483,6 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
           const uint64_t c2 = FEAT ? ta_two(TA_LOG2E, TA_LOG2E) : ta_two(c1, c1);
           bool renew = fresh, rescale = false;
           float c = 1.f, page_sum;
-          // the weights' place: the product has read it (of two places: scores are announced behind the product of two pages back)
-          if (L::TWO && n > 0) {
-            ok = tc_wait(&o_full[q * 2], phase(n - 1));
-            if (!ok) { why = ST_TIMEOUT_TMEM_FULL; break; }
-            tc_fence_after();
-          }
 #pragma unroll 1
           while (true) {
             if (renew) {
@@ -526,13 +514,11 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
                 const uint64_t e = ta_two(tc_ex2(ta_lo(z)), tc_ex2(ta_hi(z)));
                 sum[i & 1] = ta_add2(sum[i & 1], e);
                 hi[i] = tc_pack(ta_lo(e), ta_hi(e));
-                if (L::TWO) {
-                  const uint64_t d = ta_fma2(ta_two(__uint_as_float(hi[i] << 16), __uint_as_float(hi[i] & 0xffff0000u)), one, e);
-                  lo[i] = tc_pack(ta_lo(d), ta_hi(d));
-                }
+                const uint64_t d = ta_fma2(ta_two(__uint_as_float(hi[i] << 16), __uint_as_float(hi[i] & 0xffff0000u)), one, e);
+                lo[i] = tc_pack(ta_lo(d), ta_hi(d));
               }
-              tmem_st_32x16(t_lane + 64 + place(n) * 32 + part * 16, hi);
-              if (L::TWO) tmem_st_32x16(t_lane + 96 + part * 16, lo);
+              tmem_st_32x16(t_page + part * 16, hi);         // (over the scores, which are in registers)
+              tmem_st_32x16(t_page + 32 + part * 16, lo);
             }
             sum[0] = ta_add2(sum[0], sum[1]);
             page_sum = ta_lo(sum[0]) + ta_hi(sum[0]);
@@ -541,11 +527,9 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
           }
           l += page_sum;
           if (renew && __any_sync(0xffffffffu, rescale)) {
-            if (!L::TWO) {                                   // (with two terms the product before has been waited for)
-              ok = tc_wait(&o_full[q * 2 + place(n - 1)], phase(n - 1));
-              if (!ok) { why = ST_TIMEOUT_TMEM_FULL; break; }
-              tc_fence_after();
-            }
+            ok = tc_wait(&o_full[q * 2 + place(n - 1)], phase(n - 1));
+            if (!ok) { why = ST_TIMEOUT_TMEM_FULL; break; }
+            tc_fence_after();
             const uint64_t k2 = ta_two(c, c);
 #pragma unroll 1
             for (int cc = 0; cc < vn; cc += 32) {
@@ -571,7 +555,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
           const uint64_t bad = odd_rows[2 * vs] | static_cast<uint64_t>(odd_rows[2 * vs + 1]) << 32;
           if (bad) {                                         // (rare)
             uint8_t* vals = ring + vs * SLOT;
-            if (!L::TWO && n > 0) {
+            if (n > 0) {
               ok = tc_wait(&o_full[q * 2 + place(n - 1)], phase(n - 1));
               if (!ok) { why = ST_TIMEOUT_TMEM_FULL; break; }
               tc_fence_after();
@@ -581,7 +565,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
 #pragma unroll 1
               for (uint64_t left = bad; left; left &= left - 1) {
                 const int k = __ffsll(left) - 1;
-                const uint32_t pair = tc_ld1(t_lane + 64 + place(n) * 32 + k / 2);
+                const uint32_t pair = tc_ld1(t_page + k / 2);
                 const float w = __uint_as_float(k & 1 ? pair & 0xffff0000u : pair << 16);
 #pragma unroll 1
                 for (int col = 0; col < vn; ++col) {

@@ -576,3 +576,14 @@ def test_infinite_scores_are_capped(dtype):
         p, vv = torch.softmax(x, 1), v.view(-1, 2, 64)[rows, h // 2].double()
         want[:, h], tol[:, h] = p @ vv, p @ vv.abs() * ((2 * 3 * 8 + 16 + 309) * 2.0 ** -24 + WEIGHTS[dtype])
     U.close(got, want.cpu(), tol.cpu(), dtype)
+
+
+@pytest.mark.parametrize("G,rep,D,V,nodes", [(2, 4, 64, 64, 7), (2, 4, 128, 128, 50), (1, 8, 64, 128, 60), (2, 2, 256, 256, 9), (1, 16, 96, 48, 33)])
+@pytest.mark.parametrize("f", [{}, dict(softcap=4.0)])
+def test_weights_keep_two_terms(G, rep, D, V, nodes, f):
+    """Scores near 0 and values of either sign: outputs that cancel show what the weights lose, which may be 2^-17 of each for any size of tree."""
+    r = U.Round([90, 40], [nodes, 3], device=DEV, seed=4)
+    q, k = r.randn(r.R, G * rep, D, dtype=BF16) * 0.05, r.randn(r.n_pages, 64, G, D, dtype=BF16)
+    v = torch.sign(r.randn(r.n_pages, 64, G, V)).to(BF16)
+    got = ops.tree_attention(q, k, v, ops.slot_maps(**r.inputs()), D ** -0.5, **f)
+    U.close(got, *U.want_attention(r, q, k, v, D ** -0.5, rounded=2.0 ** -17, **f), BF16)
