@@ -4,7 +4,9 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <cmath>
+#include <cstdlib>
 #include <sstream>
 #include <vector>
 
@@ -94,6 +96,16 @@ Tensor pieces(const Tensor& t, int64_t quantum) {
   return c;
 }
 
+// Whether n0 x n1 pieces of `width` elements, s0 and s1 apart, share no memory.
+bool apart(int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t width) {
+  if ((n0 > 1 && s0 < width) || (n1 > 1 && s1 < width)) return false;
+  if (n0 < 2 || n1 < 2 || s0 >= (n1 - 1) * s1 + width || s1 >= (n0 - 1) * s0 + width) return true;
+  for (int64_t d = 1; d < n1; ++d)               // piece (0, d) and its neighbours (r, 0), (r + 1, 0): any two that meet are that far apart
+    for (int64_t r = d * s1 / s0; r <= std::min(d * s1 / s0 + 1, n0 - 1); ++r)
+      if (std::abs(d * s1 - r * s0) < width) return false;
+  return true;
+}
+
 struct Cache { int64_t page, tok, width; };      // strides and a token's channels, in elements
 Cache need_cache(const char* name, const Tensor& t, at::ScalarType dtype, const at::Device& dev) {
   NEED(t.dim() >= 3 && t.size(1) == spark::TREE_PAGE && t.scalar_type() == dtype && t.device() == dev, name, " must be a cache [pages, ", spark::TREE_PAGE,
@@ -106,7 +118,7 @@ Cache need_cache(const char* name, const Tensor& t, at::ScalarType dtype, const 
   const int64_t e = quantum(t);
   NEED(want > 0 && want % e == 0 && (t.size(0) < 2 || t.stride(0) % e == 0) && t.stride(1) % e == 0 && t.stride(1) >= want && aligned(t), name, ": tokens must start on 16 bytes");
   NEED(t.size(0) <= 1 << 24, name, " has more than 2^24 pages");
-  NEED(t.size(0) < 2 || t.stride(0) >= want, name, ": pages must not overlap");
+  NEED(apart(t.size(0), t.stride(0), t.size(1), t.stride(1), want), name, ": pages must not overlap");
   return {t.size(0) < 2 ? spark::TREE_PAGE * t.stride(1) : t.stride(0), t.stride(1), want};
 }
 bool is_act(at::ScalarType t) { return t == at::kBFloat16 || t == at::kFloat; }
@@ -248,8 +260,7 @@ Tensor tree_attention(Tensor q, const Tensor& k, const Tensor& v, const RowMaps&
   const int64_t e = quantum(q);
   if (given)
     NEED(given->dim() == 3 && given->size(0) == R && given->size(1) == H && given->size(2) == V && given->scalar_type() == dt && given->device() == dev &&
-             in_pieces(*given, e) &&
-             (H < 2 || given->stride(1) >= V) && (R < 2 || given->stride(0) >= V),
+             in_pieces(*given, e) && apart(R, given->stride(0), H, given->stride(1), V),
          "out must be [rows, heads, value channels] in the queries' type, heads apart and on 16 bytes");
   Tensor out = given ? *given : at::empty({R, H, V}, q.options());
   if (!run || R == 0) return out;
@@ -346,7 +357,7 @@ int64_t commit_paths(const RowMaps& m, const Tensor& path, const Tensor& n_path,
 
 PYBIND11_MODULE(_tree, mod) {
   mod.doc() = "spark_engine_b200: verification of drafted trees over paged caches (checks and launches)";
-  mod.def("bind_entry", &bind_entry).def("bind_device", &bind_device).def("pieces", &pieces);
+  mod.def("bind_entry", &bind_entry).def("bind_device", &bind_device).def("pieces", &pieces).def("apart", &apart);
   mod.def("layout", [] { return SPARK_TREE_LAYOUT; });
   py::class_<RowMaps, std::shared_ptr<RowMaps>>(mod, "RowMaps",
       "Where a round's rows belong (int32 unless said otherwise; -1 for rows behind the last request): slot [R] row of the tables, index [R]\n"

@@ -450,3 +450,32 @@ def test_a_model_with_trees_builds_both_parts(monkeypatch):
     called.clear()
     build.kernel_library("another family")
     assert called == ["runtime", "tree", "all"]
+
+
+# ----------------------------------------------------------------------------- memory that overlaps itself
+def test_pieces_that_share_memory_are_known():
+    from spark_engine_b200.ops import tree
+    rs = np.random.RandomState(0)
+    for _ in range(3000):
+        n0, n1, w = int(rs.randint(1, 7)), int(rs.randint(1, 7)), int(rs.randint(1, 5))
+        s0, s1 = int(rs.randint(0, 30)), int(rs.randint(0, 30))
+        at = [a * s0 + b * s1 + c for a in range(n0) for b in range(n1) for c in range(w)]
+        assert tree._native().apart(n0, s0, n1, s1, w) == (len(set(at)) == len(at)), (n0, s0, n1, s1, w)
+
+
+def test_outputs_and_caches_that_overlap_themselves_are_refused():
+    d = _args()
+    ops.tree_attention(**d)
+    heads_on_rows = torch.zeros(200).as_strided((5, 4, 8), (8, 8, 1))           # head 1 of a row is head 0 of the next
+    with pytest.raises(ValueError):
+        ops.tree_attention(**d, out=heads_on_rows)
+    heads_first = torch.zeros(4, 5, 8).transpose(0, 1)                          # (rows within heads do not overlap)
+    assert torch.equal(ops.tree_attention(**d, out=heads_first), ops.tree_attention(**d))
+    pages = d["k"].shape[0]
+    sliding = torch.randn(pages * 64 * 32).as_strided((pages, 64, 2, 16), (32, 32, 16, 1))        # a page's token 1 is the next page's token 0
+    with pytest.raises(ValueError):
+        ops.tree_attention(**{**d, "k": sliding})
+    with pytest.raises(ValueError):
+        ops.commit_paths(d["maps"], torch.zeros(1, 1, dtype=torch.int32), torch.ones(1, dtype=torch.int32), [sliding])
+    tokens_first = torch.randn(64, pages, 2, 16).transpose(0, 1)
+    ops.tree_attention(**{**d, "k": tokens_first})

@@ -587,3 +587,19 @@ def test_weights_keep_two_terms(G, rep, D, V, nodes, f):
     v = torch.sign(r.randn(r.n_pages, 64, G, V)).to(BF16)
     got = ops.tree_attention(q, k, v, ops.slot_maps(**r.inputs()), D ** -0.5, **f)
     U.close(got, *U.want_attention(r, q, k, v, D ** -0.5, rounded=2.0 ** -17, **f), BF16)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_caches_and_outputs_in_any_order(dtype):
+    """Pages inside tokens, heads outside rows: what does not overlap is taken."""
+    r = U.Round([300, 63], [16, 3], device=DEV)
+    q, k, v, m = r.randn(r.R, 4, 64, dtype=dtype), r.randn(r.n_pages, 64, 2, 64, dtype=dtype), r.randn(r.n_pages, 64, 2, 64, dtype=dtype), ops.slot_maps(**r.inputs())
+    want = ops.tree_attention(q, k, v, m, 0.125)
+    turned = lambda t: t.transpose(0, 1).contiguous().transpose(0, 1)
+    out = torch.zeros(4, r.R, 64, dtype=dtype, device=DEV).transpose(0, 1)
+    assert torch.equal(ops.tree_attention(turned(q), turned(k), turned(v), m, 0.125, out=out), want) and torch.equal(out, want)
+    path, n = r.i32([[0, 3, 9], [0, 2, 2]]), r.i32([3, 2])
+    other = turned(k)
+    ops.commit_paths(m, path, n, [k])
+    ops.commit_paths(m, path, n, [other])
+    assert torch.equal(k, other)
