@@ -219,7 +219,7 @@ path_conv_kernel(const __grid_constant__ PathConv a, int per) {
   extern __shared__ __align__(16) uint4 s_x[];               // [PC_STAGES][PC_ROWS + PC_FAR + 1][PC_UNITS]
   constexpr int BUF = ZERO + PC_UNITS, LAST = PC_STAGES - 1;
   __shared__ const T* s_far[PC_FAR];                         // channel 0 of the rows brought in
-  __shared__ int s_fars, s_left;                             // rows that lie elsewhere; some tap found no place
+  __shared__ int s_fars, s_left, s_rest;                     // rows that lie elsewhere; some tap found no place; some row is nobody's
   __shared__ int s_before[PC_ROWS], s_past[PC_ROWS];         // places: of the rows in front of the tile; of the past of the request that begins here
   __shared__ long long s_k[PC_ROWS], s_v[PC_ROWS];           // places of the results in the caches (-1: none)
   __shared__ int s_slot[PC_ROWS], s_parent[PC_ROWS];
@@ -230,7 +230,7 @@ path_conv_kernel(const __grid_constant__ PathConv a, int per) {
   const int n = min(PC_ROWS, a.R - b0), tile0 = blockIdx.x * per;
   // -1 - a flat row, or -2^30 - e: the e-th newest entry of the slot's tail
   auto elsewhere = [&](int s, int slot) {
-    return s < -(1 << 30) ? static_cast<const T*>(a.tail) + ((static_cast<size_t>(min(slot, a.n_slots - 1)) + 1) * (taps - 1) + (s + (1 << 30))) * a.C
+    return s < -(1 << 30) ? static_cast<const T*>(a.tail) + ((static_cast<size_t>(slot) + 1) * (taps - 1) + (s + (1 << 30))) * a.C
                           : static_cast<const T*>(a.x) + static_cast<size_t>(-1 - s) * a.ldx;
   };
   auto load = [&](int i) {                                   // rows of channel tile tile0 + i
@@ -251,20 +251,22 @@ path_conv_kernel(const __grid_constant__ PathConv a, int per) {
   if (t < PC_STAGES * PC_UNITS) s_x[t / PC_UNITS * BUF + ZERO + unit] = make_uint4(0u, 0u, 0u, 0u);
   for (int r = t; r < PC_ROWS * ld; r += PC_THREADS) s_src[r] = ZERO;
   int j = 0;
-  if (t == 0) s_fars = s_left = 0;
+  if (t == 0) s_fars = s_left = s_rest = 0;
   if (t < PC_ROWS) s_before[t] = -1;
   if (t < n) {
     j = a.index[b0 + t];
     s_parent[t] = a.parents ? a.parents[b0 + t] : j - 1;
-    const int slot = s_slot[t] = a.slot[b0 + t];
+    const int slot = a.slot[b0 + t];
+    s_slot[t] = slot < a.n_slots ? slot : -1;
     const long long row = a.cache_row[b0 + t];
-    const bool ok = slot >= 0 && row >= 0 && row < a.cache_rows;
+    const bool ok = slot >= 0 && slot < a.n_slots && row >= 0 && row < a.cache_rows;
     if (slot >= 0 && !ok) set_status(a.status, ST_BOUNDS, b0 + t, static_cast<int>(row), slot);
     s_k[t] = ok ? row / TREE_PAGE * a.k_page + row % TREE_PAGE * a.k_tok : -1;
     s_v[t] = ok ? row / TREE_PAGE * a.v_page + row % TREE_PAGE * a.v_tok : -1;
   }
   __syncthreads();
   const bool live = t < n && s_slot[t] >= 0;
+  if (t < n && !live) s_rest = 1;
   const int r0 = b0 + t - j, head = max(r0 - b0, 0);         // the request's first row, and its first one in the tile
   if (live) {                                                // the row, its ancestors, then the sequence's past
     if (t == head) {
@@ -299,7 +301,7 @@ path_conv_kernel(const __grid_constant__ PathConv a, int per) {
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < LAST; ++i) load_far(i);                // (the first group has the rows of both)
-  const bool near = !s_left;                                 // every tap is in shared memory
+  const bool near = !s_left, rest = s_rest;                  // every tap is in shared memory
   for (int i = 0; i < per; ++i) {
     const int c0 = ((tile0 + i) * PC_UNITS + unit) * VEC;
     float w[TAPS > 0 ? TAPS : 1][VEC];
@@ -347,6 +349,9 @@ path_conv_kernel(const __grid_constant__ PathConv a, int per) {
         store(r, y);
       }
     }
+    if (rest && isq)                                         // (a weight that is not finite times their zeros is not 0; the same thread's stores)
+      for (int r = t / PC_UNITS; r < n; r += STEP)
+        if (s_slot[r] < 0) *reinterpret_cast<uint4*>(base + static_cast<long long>(r) * a.nq) = make_uint4(0u, 0u, 0u, 0u);
   }
 }
 

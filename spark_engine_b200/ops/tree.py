@@ -210,7 +210,7 @@ def _plain_conv(x, w, tail, maps, nq, k, v):
     kf, vf = _flat(k, nk), _flat(v, x.shape[1] - nq - nk)
     for r in range(x.shape[0]):
         slot, j, row = int(maps.slot[r]), int(maps.index[r]), int(maps.cache_row[r])
-        if slot < 0:
+        if not 0 <= slot < tail.shape[0]:
             continue
         at, back = j, 0
         for t in reversed(range(taps)):

@@ -479,3 +479,30 @@ def test_outputs_and_caches_that_overlap_themselves_are_refused():
         ops.commit_paths(d["maps"], torch.zeros(1, 1, dtype=torch.int32), torch.ones(1, dtype=torch.int32), [sliding])
     tokens_first = torch.randn(64, pages, 2, 16).transpose(0, 1)
     ops.tree_attention(**{**d, "k": tokens_first})
+
+
+def check_rest_of_convolution(device, dtype):
+    """Rows that are nobody's, behind the last request or of one without a row of the tables, are zeros whatever weights and rows hold."""
+    for lengths, counts, pad, slots in (([70, 3], [5, 9], 7, None), ([0], [1], 80, None), ([5, 9, 2], [3, 70, 2], 1, [0, 9, 1])):
+        r = U.Round(lengths, counts, device=device, pad=pad)
+        d = r.inputs()
+        if slots:
+            d["slots"] = r.i32(slots)
+        m = ops.slot_maps(**d)
+        w, x, tail = r.randn(3, 40), r.randn(r.R, 40, dtype=dtype), r.randn(len(lengths), 2, 40, dtype=dtype)
+        k, v = r.randn(r.n_pages, 64, 2, 8, dtype=dtype), r.randn(r.n_pages, 64, 1, 8, dtype=dtype)
+        want = ops.path_conv(x, w, tail, m, 16, k.clone(), v.clone())
+        w[0, 3], w[1, 5], w[2, 7] = float("inf"), float("nan"), -float("inf")
+        dead = torch.ones(r.R, dtype=torch.bool)
+        for s in range(len(lengths)):
+            if slots is None or slots[s] < r.table.shape[0]:
+                dead[r.starts[s]: r.starts[s + 1]] = False
+        x[dead.to(device)] = float("nan")
+        got = ops.path_conv(x, w, tail, m, 16, k, v)
+        assert not got[dead.to(device)].any() and bool(got[~dead.to(device)][:, [3, 5, 7]].isfinite().logical_not().all())
+        fine = [c for c in range(16) if c not in (3, 5, 7)]
+        assert torch.equal(got[:, fine], want[:, fine])
+
+
+def test_rest_of_convolution():
+    check_rest_of_convolution("cpu", torch.float32)

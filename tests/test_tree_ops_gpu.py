@@ -603,3 +603,9 @@ def test_caches_and_outputs_in_any_order(dtype):
     ops.commit_paths(m, path, n, [k])
     ops.commit_paths(m, path, n, [other])
     assert torch.equal(k, other)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rest_of_convolution(dtype):
+    T.check_rest_of_convolution(DEV, dtype)
+    expect_status()                                  # (a request without a row of the tables)
