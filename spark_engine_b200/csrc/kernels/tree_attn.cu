@@ -177,8 +177,8 @@ __device__ __forceinline__ void tt_item(const TreeAttn& a, const TreeItem& it, T
       const float ref = top == -INFINITY ? 0.f : top;
       x[0] = expf(x[0] - ref);
       x[1] = expf(x[1] - ref);
-      sr[0] = x[0];
-      sr[32] = x[1];
+      sr[0] = seen >> lane & 1ull ? x[0] : -0.f;             // (a weight of 0 counts: times infinity it is NaN)
+      sr[32] = seen >> (lane + 32) & 1ull ? x[1] : -0.f;
       float sum = x[0] + x[1];
 #pragma unroll
       for (int z = 1; z < 32; z <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, z);
@@ -216,7 +216,7 @@ __device__ __forceinline__ void tt_item(const TreeAttn& a, const TreeItem& it, T
 #pragma unroll
             for (int i = 0; i < MR; ++i) {
               const float y = k == 0 ? w[i].x : k == 1 ? w[i].y : k == 2 ? w[i].z : w[i].w;
-              if (decltype(seen)::value || y != 0.f) {       // what a row does not see stays out of it, whatever it holds
+              if (decltype(seen)::value || __float_as_uint(y) != 0x80000000u) {        // what a row does not see stays out of it, whatever it holds
 #pragma unroll
                 for (int z = 0; z < CW; ++z) o[v][i][z] = fmaf(y, x[z], o[v][i][z]);
               }
@@ -382,8 +382,8 @@ tree_merge_kernel(const __grid_constant__ TreeAttn a) {
       for (int v = 0; v < VC; ++v) { o[v].x *= k; o[v].y *= k; o[v].z *= k; o[v].w *= k; }
 #pragma unroll
       for (int u = 0; u < FLIGHT; ++u) {
-        const float w = ta_exp<T>(ml[u].x - ref);
-        if (w == 0.f && ml[u].y == ml[u].y) continue;        // (a part of NaN scores alone stays)
+        if (i0 + u * wpt >= parts) break;
+        const float w = ta_exp<T>(ml[u].x - ref);            // (a part counts where it is 0 too: it may hold what is not finite)
         l = fmaf(w, ml[u].y, l);
 #pragma unroll
         for (int v = 0; v < VC; ++v)
@@ -412,7 +412,6 @@ tree_merge_kernel(const __grid_constant__ TreeAttn a) {
         for (int i = 1; i < wpt; ++i) {
           const float2 ml = s_ml[warp + i][lane];
           const float w = ta_exp<T>(ml.x - ref);
-          if (w == 0.f && ml.y == ml.y) continue;
           l = fmaf(w, ml.y, l);
 #pragma unroll
           for (int v = 0; v < VC; ++v)

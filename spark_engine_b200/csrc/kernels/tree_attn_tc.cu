@@ -560,7 +560,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
               if (!ok) { why = ST_TIMEOUT_TMEM_FULL; break; }
               tc_fence_after();
             }
-            if (!idle) {                                     // (the weights are there already; which are 0 is all that matters)
+            if (!idle) {                                     // (the weights are there already; their high terms are enough)
               tmem_st_wait();
 #pragma unroll 1
               for (uint64_t left = bad; left; left &= left - 1) {
@@ -572,7 +572,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
                   const uint32_t v = *reinterpret_cast<const uint16_t*>(vals + (col >> 6) * KV_CHUNK + k * 128 + (((col >> 3 & 7) ^ (k & 7)) * 16) + (col & 7) * 2);
                   if ((v & 0x7f80u) != 0x7f80u) continue;    // (the same for the whole warp)
                   const float o = __uint_as_float(tc_ld1(t_lane + 128 + col));
-                  tc_st1(t_lane + 128 + col, __float_as_uint(w != 0.f ? fmaf(w, __uint_as_float(v << 16), o) : o));
+                  tc_st1(t_lane + 128 + col, __float_as_uint(seen >> k & 1ull ? fmaf(w, __uint_as_float(v << 16), o) : o));
                 }
               }
             }

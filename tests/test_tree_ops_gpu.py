@@ -609,3 +609,40 @@ def test_caches_and_outputs_in_any_order(dtype):
 def test_rest_of_convolution(dtype):
     T.check_rest_of_convolution(DEV, dtype)
     expect_status()                                  # (a request without a row of the tables)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("window", [0, 40])
+def test_visible_infinities_show_in_every_page(window, dtype):
+    """A visible token counts even where its weight is 0: an infinite value of it makes NaN, in pages that all rows see whole and in others."""
+    r = U.Round([200], [9], device=DEV, seed=7)
+    q, v = r.randn(r.R, 4, 64, dtype=dtype), r.randn(r.n_pages, 64, 2, 64, dtype=dtype)
+    k, m, bias = r.randn(r.n_pages, 64, 2, 64, dtype=dtype), ops.slot_maps(**r.inputs()), r.randn(4, 300)
+    for at in (10, 100, 150, 195, 204):              # pages seen whole, the edge of the window, the tree's own page
+        low = bias.clone()
+        dist = m.pos.long() - (at if at < 200 else int(m.pos[at - 200]))
+        low[:, dist.clamp(0, 299)] = -float("inf")
+        bad = v.clone()
+        bad.view(-1, 2, 64)[r.rows(0)[at], :, 3] = float("inf")
+        got = ops.tree_attention(q, k, bad, m, 0.125, bias=low, window=window)
+        seen = torch.tensor(r.anc[0][:, at - 200]) if at >= 200 else torch.ones(9, dtype=torch.bool)
+        if window:
+            seen &= (dist < window).cpu()
+        assert torch.equal(got[:, :, 3].isnan().all(1).cpu(), seen) and torch.equal(got[:, :, 3].isnan().any(1).cpu(), seen)
+        assert torch.isfinite(got[:, :, [2, 4, 63]]).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("low", [-200.0, -float("inf")])
+def test_visible_infinities_show_in_every_part(low, dtype):
+    """The same of a request whose pages many CTAs share: a part that weighs nothing beside the others."""
+    r = U.Round([9000], [5], device=DEV)
+    q, k, v = r.randn(r.R, 4, 64, dtype=dtype), r.randn(r.n_pages, 64, 2, 64, dtype=dtype), r.randn(r.n_pages, 64, 2, 64, dtype=dtype)
+    m, bias = ops.slot_maps(**r.inputs()), torch.zeros(4, 9100, device=DEV)
+    bias[:, 4000:6000] = low
+    assert torch.isfinite(ops.tree_attention(q, k, v, m, 0.125, bias=bias)).all()
+    v.view(-1, 2, 64)[r.rows(0)[4100], 1, 3] = float("inf")
+    got = ops.tree_attention(q, k, v, m, 0.125, bias=bias).isfinite().cpu()
+    want = torch.ones_like(got)
+    want[:, 2:, 3] = False
+    assert torch.equal(got, want)
