@@ -8,6 +8,7 @@
 #include <cmath>
 #include <cstdlib>
 #include <sstream>
+#include <utility>
 #include <vector>
 
 #include "tree_args.h"
@@ -21,9 +22,12 @@ namespace {
 // ------------------------------------------------------------------------------------------------ plumbing
 struct Entry {                                   // an entry point of the kernel library
   const char* name;
+  int kernels = 1;                               // of a call
   void* fn = nullptr;
 };
-Entry e_tables{"spark_block_tables"}, e_maps{"spark_slot_maps"}, e_conv{"spark_path_conv"}, e_commit{"spark_commit_paths"}, e_attn{"spark_tree_attn"};
+Entry e_tables{"spark_block_tables"}, e_maps{"spark_slot_maps"}, e_conv{"spark_path_conv"}, e_commit{"spark_commit_paths"}, e_attn{"spark_tree_attn", 2};
+int64_t launched = 0;                            // kernels since it was last asked for
+int64_t take_launched() { return std::exchange(launched, 0); }
 struct Device { int* status = nullptr; int sms = 0; };
 std::vector<Device> devices;
 
@@ -60,6 +64,7 @@ struct On {                                      // the tensors' device and its 
   void launch(const Entry& e, A... args) const {
     const int rc = reinterpret_cast<int (*)(A..., cudaStream_t)>(e.fn)(args..., stream);
     if (rc) throw std::runtime_error(std::string(e.name) + " failed with code " + std::to_string(rc));
+    launched += e.kernels;
   }
 };
 
@@ -305,8 +310,8 @@ Tensor tree_attention(Tensor q, const Tensor& k, const Tensor& v, const RowMaps&
 }
 
 // ------------------------------------------------------------------------------------------------ commit
-int64_t commit_paths(const RowMaps& m, const Tensor& path, const Tensor& n_path, const std::vector<Tensor>& caches,
-                     const std::vector<std::pair<Tensor, Tensor>>& tails, bool run) {
+void commit_paths(const RowMaps& m, const Tensor& path, const Tensor& n_path, const std::vector<Tensor>& caches,
+                  const std::vector<std::pair<Tensor, Tensor>>& tails, bool run) {
   const at::Device dev = m.tables.device();
   const int64_t S = m.lengths.size(0);
   NEED(path.scalar_type() == at::kInt && path.device() == dev && path.dim() == 2 && path.size(0) == S && path.is_contiguous(),
@@ -339,10 +344,9 @@ int64_t commit_paths(const RowMaps& m, const Tensor& path, const Tensor& n_path,
   for (const auto& j : jobs) seen.push_back(j.base);
   std::sort(seen.begin(), seen.end());
   NEED(std::adjacent_find(seen.begin(), seen.end()) == seen.end(), "a cache or tail is given twice");
-  if (!run || jobs.empty() || S == 0 || P == 0 || m.rows() == 0) return 0;
+  if (!run || jobs.empty() || S == 0 || P == 0 || m.rows() == 0) return;
   const On on(m.tables);
-  int64_t launches = 0;
-  for (size_t at = 0; at < jobs.size(); at += spark::COMMIT_JOBS, ++launches) {
+  for (size_t at = 0; at < jobs.size(); at += spark::COMMIT_JOBS) {
     spark::CommitPaths a{{}, ip(path), ip(n_path), ip(m.starts), ip(m.lengths), ip(m.slots), ip(m.tables), on.dev.status, static_cast<int>(S),
                          static_cast<int>(P), static_cast<int>(m.tables.size(1)), static_cast<int>(m.tables.size(0)), static_cast<int>(pages)};
     const int n = static_cast<int>(std::min<size_t>(spark::COMMIT_JOBS, jobs.size() - at));
@@ -350,14 +354,13 @@ int64_t commit_paths(const RowMaps& m, const Tensor& path, const Tensor& n_path,
     for (int i = 0; i < n; ++i) { a.job[i] = jobs[at + i]; most = std::max(most, a.job[i].bytes); }
     on.launch(e_commit, &a, n, most);
   }
-  return launches;
 }
 
 }  // namespace
 
 PYBIND11_MODULE(_tree, mod) {
   mod.doc() = "spark_engine_b200: verification of drafted trees over paged caches (checks and launches)";
-  mod.def("bind_entry", &bind_entry).def("bind_device", &bind_device).def("pieces", &pieces).def("apart", &apart);
+  mod.def("bind_entry", &bind_entry).def("bind_device", &bind_device).def("take_launched", &take_launched).def("pieces", &pieces).def("apart", &apart);
   mod.def("layout", [] { return SPARK_TREE_LAYOUT; });
   py::class_<RowMaps, std::shared_ptr<RowMaps>>(mod, "RowMaps",
       "Where a round's rows belong (int32 unless said otherwise; -1 for rows behind the last request): slot [R] row of the tables, index [R]\n"

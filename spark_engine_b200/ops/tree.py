@@ -26,7 +26,7 @@ import torch
 from . import cuda_ops, use_kernels
 
 PAGE = 64
-_ENTRIES = {"spark_block_tables": 1, "spark_slot_maps": 1, "spark_path_conv": 1, "spark_commit_paths": 1, "spark_tree_attn": 2}     # kernels of a call
+_ENTRIES = ("spark_block_tables", "spark_slot_maps", "spark_path_conv", "spark_commit_paths", "spark_tree_attn")
 _mod = None
 _bound = None
 _known = set()                                     # devices that the bindings know
@@ -78,8 +78,9 @@ def _bind(index: int):
     _known.add(index)
 
 
-def _count(name: str, calls: int = 1):
-    cuda_ops().add_launches(_ENTRIES[name] * calls)
+def _count():
+    """Counts the kernels that the last call launched (none where there is nothing to do)."""
+    cuda_ops().add_launches(_mod.take_launched())
 
 
 def _need(ok: bool, what: str):
@@ -103,7 +104,7 @@ def block_tables(lengths, tables, held, free, n_free) -> torch.Tensor:
     run = _kernels(tables)
     room = _native().block_tables(lengths, tables, held, free, n_free, run)
     if run:
-        _count("spark_block_tables")
+        _count()
         return room
     return _plain_tables(lengths, tables, held, free, n_free)
 
@@ -138,7 +139,7 @@ def slot_maps(lengths, counts, tables, rows: int, slots=None, parents=None, node
     run = _kernels(tables)
     m = _native().slot_maps(lengths, counts, tables, rows, slots, parents, nodes, run)
     if run:
-        _count("spark_slot_maps")
+        _count()
         return m
     return _plain_maps(m)
 
@@ -194,7 +195,7 @@ def path_conv(x, w, tail, maps: "RowMaps", nq: int, k, v) -> torch.Tensor:
     run = _kernels(x)
     q = _native().path_conv(x, w, tail, maps, nq, k, v, run)
     if run:
-        _count("spark_path_conv")
+        _count()
         return q
     return _plain_conv(x, w, tail, maps, nq, k, v)
 
@@ -239,7 +240,7 @@ def tree_attention(q, k, v, maps: "RowMaps", scale: float, softcap: float = 0.0,
     run = _kernels(q)
     o = _native().tree_attention(q, k, v, maps, scale, softcap, bias, slopes, sink, window, chunk, gate, out_scale, out, run)
     if run:
-        _count("spark_tree_attn")
+        _count()
         return o
     return _plain_attention(q, k, v, maps, scale, softcap, bias, slopes, sink, window, chunk, gate, out_scale, o, out is None)
 
@@ -305,9 +306,9 @@ def commit_paths(maps: "RowMaps", path, n_path, caches: Sequence[torch.Tensor], 
     does not ascend, or whose accepted rows are not in pages that all caches of the call have, stays as it is in every cache and tail.  No
     two of the caches and tails may share memory."""
     run = _kernels(maps.tables)
-    calls = _native().commit_paths(maps, path, n_path, caches, tails, run)
+    _native().commit_paths(maps, path, n_path, caches, tails, run)
     if run:
-        _count("spark_commit_paths", calls)
+        _count()
     else:
         _plain_commit(maps, path, n_path, caches, tails)
 

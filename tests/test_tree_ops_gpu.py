@@ -646,3 +646,27 @@ def test_visible_infinities_show_in_every_part(low, dtype):
     want = torch.ones_like(got)
     want[:, 2:, 3] = False
     assert torch.equal(got, want)
+
+
+def test_launches_are_counted_where_there_are_any():
+    cu = ops.cuda_ops()
+    r, none = U.Round([70, 9], [5, 6], device=DEV), U.Round([70, 3], [0, 0], device=DEV, trees=False)
+    k, v = r.randn(r.n_pages, 64, 1, 64), r.randn(r.n_pages, 64, 1, 64)
+    m, empty = ops.slot_maps(**r.inputs()), ops.slot_maps(**none.inputs())
+    i32 = r.i32
+
+    def counted(call):
+        cu.reset_launch_count()
+        call()
+        return cu.launch_count()
+    x, w, tail = r.randn(r.R, 256), r.randn(2, 256), r.randn(2, 1, 256)
+    assert counted(lambda: ops.slot_maps(**r.inputs())) == 1
+    assert counted(lambda: ops.path_conv(x, w, tail, m, 128, k, v)) == 1
+    assert counted(lambda: ops.path_conv(x[:0], w, tail, empty, 128, k, v)) == 0
+    assert counted(lambda: ops.tree_attention(r.randn(r.R, 2, 64), k, v, m, 0.1)) == 2
+    assert counted(lambda: ops.tree_attention(x[:0, :128].view(0, 2, 64), k, v, empty, 0.1)) == 0
+    assert counted(lambda: ops.commit_paths(m, i32([[0], [0]]), i32([1, 1]), [k, v])) == 1
+    assert counted(lambda: ops.commit_paths(m, i32([[0], [0]]), i32([1, 1]), [r.randn(r.n_pages, 64, 1, 8) for _ in range(130)])) == 2
+    assert counted(lambda: ops.commit_paths(m, i32([[0], [0]]), i32([1, 1]), [])) == 0
+    nobody = torch.zeros(0, dtype=torch.int32, device=DEV)
+    assert counted(lambda: ops.block_tables(nobody, torch.zeros(0, 3, dtype=torch.int32, device=DEV), nobody, nobody, i32([0]))) == 0
