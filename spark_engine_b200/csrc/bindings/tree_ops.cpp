@@ -241,6 +241,16 @@ void need_heads(const char* name, const Opt& t, int64_t dim, int64_t H, const at
 }
 float* fp(const Opt& t) { return t ? static_cast<float*>(t->data_ptr()) : nullptr; }
 
+// Rows of a tile on the tensor cores, for heads of up to 128 (wider ones leave room for one tile of 128 and one CTA per SM): 128 (node, head) rows, two
+// CTAs per SM; or, where requests have more of them, two such tiles per CTA that share the keys, one CTA per SM.  A request's rows are known by
+// `nodes`; of chains, which may be of any lengths, by the average.  One tile / two (us of a call, 32 query heads on 8 of 128 over 4k tokens): 64 requests
+// of trees of 8 nodes (32 rows) 200 / 265, 32 nodes (128 rows) 224 / 299, 33 nodes 384 / 339, 64 nodes (256 rows) 423 / 376; 8 requests of 32 nodes
+// 54 / 60, of 33 71 / 65; 64 chains of one row 196 / 253, of 64 rows 421 / 374, one of 500 beside 63 of one 244 / 395.
+int64_t tile_rows(int64_t R, int64_t S, int64_t nodes, int64_t rep) {
+  const int64_t rows = nodes ? std::min(nodes, R) : (R + S - 1) / S;
+  return rows * rep > 128 ? 256 : 128;
+}
+
 Tensor tree_attention(Tensor q, const Tensor& k, const Tensor& v, const RowMaps& m, double scale, double softcap, const Opt& bias, const Opt& slopes,
                       const Opt& sink, int64_t window, int64_t chunk, const Opt& gate, double out_scale, const Opt& given, bool run) {
   const auto dt = q.scalar_type();
@@ -274,13 +284,8 @@ Tensor tree_attention(Tensor q, const Tensor& k, const Tensor& v, const RowMaps&
   NEED(k.size(0) > 0, "caches without pages");
   q = pieces(q, e);
   const On on(q);
-  // Tensor cores: tiles of 128 (node, head) rows, two CTAs per SM; or, where a request may have more of them, two tiles per CTA that share
-  // the keys, one CTA per SM.  Heads wider than 128 leave room for one tile and one CTA.  One tile / two (us of a call, 64 requests over 4k tokens, 32
-  // query heads on 8 of 128): 20 nodes (80 rows) 220 / 236, 32 nodes (128 rows) 240 / 244, 40 nodes (160 rows) 423 / 310, 64 nodes (256 rows) 465 /
-  // 328; 8 requests of 32 nodes 50 / 46.
   const bool tc = dt == at::kBFloat16 && D <= 256 && V <= 256, wide = D > 128 || V > 128;
-  const int64_t most = (m.nodes ? std::min(m.nodes, R) : R) * (H / G);
-  const int bm = !tc ? 64 : !wide && most > 128 ? 256 : 128;
+  const int bm = !tc ? 64 : wide ? 128 : static_cast<int>(tile_rows(R, S, m.nodes, H / G));
   const int ctas = std::min(512, on.dev.sms * (bm == 256 || wide ? 1 : 2));
   // What beginning an item costs, in pages (us of a call: four requests of 16k tokens, heads of 256, with 5 / 8 / 10 / 14 / 20: 51.7 / 46.1 / 45.1 /
   // 44.7 / 44.9; a ragged round with soft cap and bias, whose pages take longer, with 2 / 3 / 4 / 6 / 8: 28.5 / 28.6 / 28.6 / 30.8 / 31.0; 64 requests
@@ -360,7 +365,7 @@ void commit_paths(const RowMaps& m, const Tensor& path, const Tensor& n_path, co
 
 PYBIND11_MODULE(_tree, mod) {
   mod.doc() = "spark_engine_b200: verification of drafted trees over paged caches (checks and launches)";
-  mod.def("bind_entry", &bind_entry).def("bind_device", &bind_device).def("take_launched", &take_launched).def("pieces", &pieces).def("apart", &apart);
+  mod.def("bind_entry", &bind_entry).def("bind_device", &bind_device).def("take_launched", &take_launched).def("pieces", &pieces).def("apart", &apart).def("tile_rows", &tile_rows);
   mod.def("layout", [] { return SPARK_TREE_LAYOUT; });
   py::class_<RowMaps, std::shared_ptr<RowMaps>>(mod, "RowMaps",
       "Where a round's rows belong (int32 unless said otherwise; -1 for rows behind the last request): slot [R] row of the tables, index [R]\n"

@@ -506,3 +506,11 @@ def check_rest_of_convolution(device, dtype):
 
 def test_rest_of_convolution():
     check_rest_of_convolution("cpu", torch.float32)
+
+
+def test_tiles_go_by_a_requests_rows():
+    """Not by those of all requests: chains of one row are no tree of many."""
+    from spark_engine_b200.ops import tree
+    tile = tree._native().tile_rows
+    assert tile(64, 64, 0, 4) == 128 and tile(64 * 32, 64, 0, 4) == 128 and tile(64 * 33, 64, 0, 4) == 256 and tile(500, 1, 0, 4) == 256
+    assert tile(64 * 32, 64, 32, 4) == 128 and tile(64 * 33, 64, 33, 4) == 256 and tile(9, 1, 64, 8) == 128 and tile(563, 64, 0, 4) == 128

@@ -670,3 +670,10 @@ def test_launches_are_counted_where_there_are_any():
     assert counted(lambda: ops.commit_paths(m, i32([[0], [0]]), i32([1, 1]), [])) == 0
     nobody = torch.zeros(0, dtype=torch.int32, device=DEV)
     assert counted(lambda: ops.block_tables(nobody, torch.zeros(0, 3, dtype=torch.int32, device=DEV), nobody, nobody, i32([0]))) == 0
+
+
+@pytest.mark.parametrize("counts", [[1] * 40, [1] * 39 + [150], [4, 200], [70]])
+def test_chains_of_any_lengths(counts):
+    r = U.Round(np.random.RandomState(2).randint(0, 700, len(counts)), counts, device=DEV, trees=False, pad=2)
+    T.check_attention(r, 16, 4, 64, 64, BF16, {}, rounded=WEIGHTS[BF16])
+    T.check_attention(r, 16, 4, 128, 64, BF16, dict(softcap=3.0, window=100), rounded=WEIGHTS[BF16])
