@@ -677,3 +677,21 @@ def test_chains_of_any_lengths(counts):
     r = U.Round(np.random.RandomState(2).randint(0, 700, len(counts)), counts, device=DEV, trees=False, pad=2)
     T.check_attention(r, 16, 4, 64, 64, BF16, {}, rounded=WEIGHTS[BF16])
     T.check_attention(r, 16, 4, 128, 64, BF16, dict(softcap=3.0, window=100), rounded=WEIGHTS[BF16])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads", [(8, 2), (16, 1)])
+def test_requests_alone_and_in_a_batch(heads, dtype):
+    """A request's outputs beside others, whose lengths move where its pages are divided, and by itself: both within the bounds of the definition."""
+    r = U.Round([900, 64, 2000, 1, 300], [12, 5, 30, 7, 9], device=DEV)
+    H, G = heads
+    q, k, v = r.randn(r.R, H, 64, dtype=dtype), r.randn(r.n_pages, 64, G, 64, dtype=dtype), r.randn(r.n_pages, 64, G, 64, dtype=dtype)
+    opt = dict(softcap=9.0, sink=r.randn(H))
+    want, tol = U.want_attention(r, q, k, v, 0.125, rounded=2.0 ** -17 if dtype == BF16 else 0.0, **opt)
+    d = r.inputs()
+    U.close(ops.tree_attention(q, k, v, ops.slot_maps(**d), 0.125, **opt), want, tol, dtype)
+    for s in range(5):
+        sl = slice(r.starts[s], r.starts[s + 1])
+        m = ops.slot_maps(d["lengths"][s: s + 1].clone(), d["counts"][s: s + 1].clone(), d["tables"], r.counts[s], slots=r.i32([s]),
+                          parents=d["parents"][sl].clone(), nodes=r.counts[s])
+        U.close(ops.tree_attention(q[sl], k, v, m, 0.125, **opt), want[sl], tol[sl], dtype)
