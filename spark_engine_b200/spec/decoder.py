@@ -137,6 +137,11 @@ class SpecDecoder:
             return P.rate_depth(confs, seq.table, self.cost, n_seqs, other_rows, self.depth)
         return min(len(confs), self.depth)
 
+    def _room(self, seq: SeqSpec) -> int:
+        """Drafts that the sequence's cache has rows for beside the last token's (near its end there are fewer than a round would verify)."""
+        q = self.m.seqs[seq.slot]
+        return max(0, q.kv_cap - q.length - 1)
+
     # ---------------------------------------------------------------------------------------------
     def _propose_graph(self, seqs: List[SeqSpec], L: List[int]):
         """All sequences' MTP chains in one captured replay; same proposals as `_draft` one by one."""
@@ -175,6 +180,7 @@ class SpecDecoder:
         drafts, draft_confs = [], []
         for s, (d, c) in zip(seqs, proposals):
             k = len(d) if given else self._choose(s, c, len(seqs), sum(1 + len(x) for x in drafts))
+            k = min(k, self._room(s))
             drafts.append(list(d[:k]))
             draft_confs.append(list(c[:k]))
         toks = [[s.last_token] + d for s, d in zip(seqs, drafts)]
@@ -255,6 +261,7 @@ class SpecDecoder:
         decode rows), so the round stays lossless.  Reference: engine-rs/src/speculative.rs,
         spec_probe.rs:254-460 (tree topologies), mla_latent.rs:472-773."""
         m = self.m
+        trees = [nodes[: self._room(s)] for s, nodes in zip(seqs, trees)]         # (parents come first: what is left is a tree)
         limit = m.sparse_ctx_limit()
         if limit is not None and any(m.seqs[s.slot].length + 1 + len(nodes) > limit for s, nodes in zip(seqs, trees)):
             props = []

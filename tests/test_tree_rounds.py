@@ -176,3 +176,25 @@ def test_branches_are_refused_where_rows_verify_chains():
     m.forward(make_plan([(0, [1, 2, 3], 0)], all_logits=False))
     with pytest.raises(AssertionError):
         m.forward(make_plan([(0, [4, 5, 6], 3)], parents=[[-1, 0, 0]]), commit=False)
+
+
+@pytest.mark.parametrize("kind", ["trees", "chains"])
+@pytest.mark.parametrize("extra", [3, 4, 7])
+def test_rounds_up_to_the_last_row(kind, extra):
+    """A sequence is generated to the end of its pages: drafts that its cache has no rows for are left out."""
+    from spark_engine_b200.cache.kv import KvManager
+    cfg, T = setup("dense")
+    prompt = U.prompt(64 - extra, cfg["vocab"])
+    want = SpecDecoder(U.framework(cfg, T), lambda s, d: ([], []), depth=0).generate([prompt], extra + 1)[0]
+    m = U.framework(cfg, T)
+    assert KvManager(m).assign(1, 64) and m.seqs[1].kv_cap == 64
+    sd = SpecDecoder(m, lambda s, d: ([1, 2, 3][:d], [0.9] * min(3, d)), depth=3)
+    seq = sd.start(1, prompt)
+    while len(seq.generated) < extra + 1:
+        left = [extra + 1 - len(seq.generated)]
+        if kind == "chains":
+            sd.round([seq], left)
+        else:
+            t = (want[len(seq.generated):] + [1])[0]
+            sd.round_tree([seq], [[Node(-1, (t + 1) % cfg["vocab"]), Node(-1, t), Node(0, 3), Node(1, 4), Node(2, 5)]], left)
+    assert seq.generated[: extra + 1] == want and m.seqs[1].length <= 64
