@@ -287,12 +287,13 @@ Tensor tree_attention(Tensor q, const Tensor& k, const Tensor& v, const RowMaps&
   const bool tc = dt == at::kBFloat16 && D <= 256 && V <= 256, wide = D > 128 || V > 128;
   const int bm = !tc ? 64 : wide ? 128 : static_cast<int>(tile_rows(R, S, m.nodes, H / G));
   const int ctas = std::min(512, on.dev.sms * (bm == 256 || wide ? 1 : 2));
-  // What beginning an item costs, in pages (us of a call: four requests of 16k tokens, heads of 256, with 5 / 8 / 10 / 14 / 20: 51.7 / 46.1 / 45.1 /
-  // 44.7 / 44.9; a ragged round with soft cap and bias, whose pages take longer, with 2 / 3 / 4 / 6 / 8: 28.5 / 28.6 / 28.6 / 30.8 / 31.0; 64 requests
-  // of 64 nodes with 3 / 4 / 8 / 10 / 12: 322 / 322 / 320 / 321 / 320; the FP32 units' pages are long)
+  // What beginning an item costs, in pages (us of a call: four requests of 16k tokens, heads of 256, with 5 / 8 / 10 / 14 / 20: 51.1 / 48.0 / 47.1 /
+  // 47.2 / 47.1; a ragged round with soft cap and bias, whose pages take longer, with 2 / 3 / 4 / 6 / 8: 30.6 / 30.3 / 30.1 / 32.4 / 32.4; windows of 1024
+  // and 64 requests of 64 nodes: 3 to 12 make no difference; the FP32 units' pages are long)
   const int extra = !tc ? 0 : wide ? 10 : softcap > 0 || bias || slopes ? 4 : 6;
   const int64_t work = G * (R * (H / G) / bm + S) * (m.tables.size(1) + extra);
   NEED(work < 1ll << 31, "a round of ", R, " rows over tables of ", m.tables.size(1), " pages is more than one call takes");
+  // (places for two parts per CTA, whatever the lengths turn out to be: 39 MB for values of 128, in bf16 calls of any size)
   const int64_t no = static_cast<int64_t>(ctas) * 2 * bm * V, nm = static_cast<int64_t>(ctas) * 2 * bm * 2;
   Tensor ws = at::empty({no + nm + ctas * 4}, q.options().dtype(at::kFloat));
   float* part = static_cast<float*>(ws.data_ptr());

@@ -48,7 +48,7 @@ struct TtRows { uint64_t seen[TT_BM]; int pos[TT_BM], head[TT_BM], at[TA_PAGE]; 
 // of four); a lane has keys lane + 32 e of a page's scores and CW neighbouring columns in every 32 CW of the outputs.  Keys pass in pieces of
 // 64 tokens x 64 channels, values in pieces of 4096 (128 channels, or 64 where there are no more), two of them on their way while one is worked
 // on.  The FP32 units and the instructions that feed them bound it: one request of 64 nodes, 12 heads of 128 over 39k tokens runs at 27 TFLOP/s
-// (with 4 x 4 scores and outputs per thread 23, with copies waited for where they are needed 14), a single row over 30k tokens at 1.8 TB/s; 5 to
+// (with 4 x 4 scores and outputs per thread 23, with copies waited for where they are needed 14), a single row over 30k tokens, 4 heads, at 1.5 TB/s; 5 to
 // 11 nodes over 2k tokens are 24 us of latency (35 with the rows' softmax unrolled: every instruction's first run waits for memory).
 template <typename T, int VP, int CW, int MR>
 __device__ __forceinline__ void tt_item(const TreeAttn& a, const TreeItem& it, T* ring, float* Qs, float* Ss, TtRows& rows) {

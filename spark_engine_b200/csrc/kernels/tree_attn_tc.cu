@@ -19,10 +19,11 @@
 // see it, so the softmax warps add it by hand for the rows that do and zero it in front of the product.
 //
 // What bounds it (kernel time, inputs from HBM): few rows over long caches stream at 6.1 TB/s between the first page and the last, about 8 us
-// after the launch (four requests of 16 nodes over 16k tokens, two heads of 256 of 8 each: 132 MB in 41 us); 256 rows are bound by the products and
-// the exponentials of a page, 1024 clocks each, which overlap in part (64 requests of 64 nodes over 4k tokens, 8 heads of 128 of 4 each: 272 GFLOP
-// in 310 us; at the 1560 MHz that 1000 W leave after seconds 370).  Short calls are the latency of what is done once: 10 us for 8 nodes over 900 tokens.  What did not pay: the two tiles' softmax
-// in turn (412 us instead of 363), results through shared memory (no change), an earlier start of the second launch (no change).
+// after the launch (four requests of 16 nodes over 16k tokens, two heads of 256 of 8 each: 132 MB in 41 us); 256 rows are bound by the products of
+// a page, 1536 clocks, and its exponentials, 1024, which overlap in part (64 requests of 64 nodes over 4k tokens, 8 heads of 128 of 4 each: 272 GFLOP
+// in 369 us, 450 at the clock that 1000 W leave after seconds; the tensor pipe is active in 53 % of the clocks, issue slots in 39 %).  Short calls
+// are the latency of what is done once: 10 us for 8 nodes over 900 tokens.  What did not pay (measured with weights of one term): the two tiles'
+// softmax in turn (412 us instead of 363), results through shared memory (no change), an earlier start of the second launch (no change).
 #include "../common/tree_work.cuh"
 
 namespace spark {

@@ -208,10 +208,13 @@ __device__ __forceinline__ uint4 pc_join(const float (&f)[4], float) {
 
 // grid (groups of `per` channel tiles, row tiles).  A tile's rows are brought to shared memory once and every row takes its taps from there;
 // so are up to PC_FAR rows that lie elsewhere (ancestors in front of the tile, the sequences' past).  The paths are
-// followed once for all channel tiles of a CTA, and the next tile's rows are on their way while one is computed.  Instructions bound it before
-// the bytes do: what depends on the row alone is formed once, and the common loop has no branches (nobody's rows take a row of zeros).
+// followed once for all channel tiles of a CTA, and the next tile's rows are on their way while one is computed.  The bytes do not bound it (a
+// quarter of DRAM's rate under the profiler): the shared-memory pipe is busy half of the time, issue slots 56 %, and the barrier per channel tile
+// holds up as many warps as the shared memory does.  So what depends on the row alone is formed once, and the common loop has no branches
+// (nobody's rows take a row of zeros).
 // 5.2 us for 50 rows of 2560 channels, 36 us for 5000 rows of 6144 (126 MB, 3.5 TB/s; 52 with the taps' places looked up per tile, 87 with every
-// tap loaded from memory; two products per instruction: no change).
+// tap loaded from memory; two products per instruction: no change).  Where more than PC_FAR rows lie elsewhere (four taps: the pasts of 22 requests
+// that begin in a tile), its taps are looked up one by one and some come from memory: 96 requests of one row take 16 us, of eight rows 14.
 template <typename T, int TAPS>
 __global__ void __launch_bounds__(PC_THREADS, PC_PER_SM)
 path_conv_kernel(const __grid_constant__ PathConv a, int per) {

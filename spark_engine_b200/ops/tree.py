@@ -8,6 +8,9 @@ parents the rows are chains.  Lengths, counts, parents, tables and paths live on
 The maps refer to lengths, tables, slots and parents, which have to stay as they are until the round is committed; requests of one round
 have different slots, and pages that only one of them writes to.
 
+`block_tables` is for callers that keep their free pages on the device as well; the engine's own pages are leased by the host's pool
+(`cache/kv.py`), whose tables `slot_maps` and the others read as they are.
+
 The calls neither wait for the device nor read from it.  What they can only find out there sets the device status word: what would be
 written to a missing page or read from one is left out, a row whose parent is not in front of it hangs off the committed tokens, and
 `commit_paths` skips a request whose path does not ascend or whose pages are missing.  The plain forms, for tensors on the host, leave missing
@@ -236,7 +239,11 @@ def tree_attention(q, k, v, maps: "RowMaps", scale: float, softcap: float = 0.0,
     (softcap * tanh(s / softcap)), get bias[h, min(distance, n - 1)] (fp32 [H, n]) or lose slopes[h] * distance; rows see the tokens of their
     own aligned `chunk` of positions or of the `window` positions that end at theirs.  sink fp32 [H] enters the denominators, gate [R, H]
     (logits, in q's type) and out_scale scale the outputs.  Into `out` [R, H, V] if given (rows behind the last request are left as they
-    were), else a new tensor (they are zero).  A row that sees nothing is zero; what a row does not see has no effect on it, whatever it holds."""
+    were), else a new tensor (they are zero).  A row that sees nothing is zero; what a row does not see has no effect on it, whatever it holds.
+
+    Scores, statistics and sums are fp32.  bf16 heads of up to 256 run on the tensor cores, where a weight enters the product as two bf16 terms
+    (2^-17 of it is lost); what fp32 and wider heads run on keeps weights in fp32.  A call takes a workspace from torch's allocator (39 MB for
+    values of 128 in bf16, however small the round), which a captured call keeps."""
     run = _kernels(q)
     o = _native().tree_attention(q, k, v, maps, scale, softcap, bias, slopes, sink, window, chunk, gate, out_scale, out, run)
     if run:
