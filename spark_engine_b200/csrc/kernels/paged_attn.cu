@@ -389,7 +389,7 @@ paged_decode_kernel(const __grid_constant__ PagedAttn a) {
     Ps[(PGA_HEADS + row) * 72 + lane] = __float2bfloat16(e0 - __bfloat162float(b0));
     Ps[(PGA_HEADS + row) * 72 + lane + 32] = __float2bfloat16(e1 - __bfloat162float(b1));
     if (lane == 0 && row < nh) {
-      a.part_ml[(pb + static_cast<size_t>(row) * a.nsplit) * 2] = m;
+      a.part_ml[(pb + static_cast<size_t>(row) * a.nsplit) * 2] = l == l ? m : l;        // (scores of NaN alone leave a maximum of -inf: no empty split)
       a.part_ml[(pb + static_cast<size_t>(row) * a.nsplit) * 2 + 1] = l;
     }
   }

@@ -302,3 +302,26 @@ def test_what_is_not_a_number_shows_under_a_soft_cap(dim, vdim, rows, large, dty
     hit = torch.zeros(rows, 4, dtype=torch.bool)
     hit[-1, 1] = True
     assert torch.equal(got.isnan().all(-1).cpu(), hit) and torch.equal(got.isnan().any(-1).cpu(), hit)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("softcap", [0.0, 2.0])
+@pytest.mark.parametrize("rows,past", [(1, 40), (4, 40), (1, 63), (3, 300)])
+@pytest.mark.parametrize("dim,vdim", [(64, 64), (20, 36), (320, 272)])
+def test_what_is_not_a_number_shows_in_decode_rows(dim, vdim, rows, past, softcap, dtype):
+    """A query of NaN, whose pages may have no other score, gives NaN and not the zeros of a row without keys."""
+    cfg, T = _setup(dict(layers=[U.layer(heads=4, kv_heads=2, dim=dim, vdim=vdim, conv=1, softcap=6.0, chunk=1000, scale=0.3)]), 3)
+    m = U.framework(cfg, T, DEV, dtype)
+    toks = U.prompt(past + rows, cfg["vocab"])
+    m.forward(make_plan([(0, toks, 0)], device=DEV, all_logits=False))
+    mix = m.layers[0][1]
+    mix.c.softcap = softcap
+    g = torch.Generator().manual_seed(1)
+    proj = (torch.randn(rows, mix.columns, generator=g) * 2).to(dtype).to(DEV)
+    plan = make_plan([(0, toks[past:], past)], device=DEV)
+    assert torch.isfinite(mix.attend(proj, plan, False)).all()
+    proj[-1, mix.Dp: 2 * mix.Dp] = float("nan")
+    got = mix.attend(proj, plan, False).view(rows, 4, -1)
+    hit = torch.zeros(rows, 4, dtype=torch.bool)
+    hit[-1, 1] = True
+    assert torch.equal(got.isnan().all(-1).cpu(), hit) and torch.equal(got.isnan().any(-1).cpu(), hit)
