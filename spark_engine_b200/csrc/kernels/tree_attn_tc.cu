@@ -12,7 +12,8 @@
 // here: what a round of drafts is verified with does not depend on how large their trees are.  (One term, half a step of bf16 per weight,
 // makes the error of 64 requests of 64 nodes over 4k tokens 1.4 times that of the rounded outputs, and the call 321 us instead of 378.)
 // A page's weights take the place of its scores, and two such places alternate, so that they need not wait for the product of the page
-// before (398 us with weights in one place beside the scores).
+// before (398 us with weights in one place beside the scores).  (A visible value of infinity times two terms, of either sign or 0, may be NaN where
+// the definition has infinity.)
 //
 // A page that not every row sees whole (the tree itself, the edge of a window or chunk) is masked by 64 bits per row.  Warp 1 looks its values
 // over first: rows that hold no token of the request are zeroed, and where a value is not finite, 0 * value would spoil the rows that do not

@@ -242,7 +242,7 @@ def tree_attention(q, k, v, maps: "RowMaps", scale: float, softcap: float = 0.0,
     were), else a new tensor (they are zero).  A row that sees nothing is zero; what a row does not see has no effect on it, whatever it holds.
 
     Scores, statistics and sums are fp32.  bf16 heads of up to 256 run on the tensor cores, where a weight enters the product as two bf16 terms
-    (2^-17 of it is lost); what fp32 and wider heads run on keeps weights in fp32.  A call takes a workspace from torch's allocator (39 MB for
+    (2^-17 of it is lost; infinite values that a row sees may give NaN for infinity); what fp32 and wider heads run on keeps weights in fp32.  A call takes a workspace from torch's allocator (39 MB for
     values of 128 in bf16, however small the round), which a captured call keeps."""
     run = _kernels(q)
     o = _native().tree_attention(q, k, v, maps, scale, softcap, bias, slopes, sink, window, chunk, gate, out_scale, out, run)
