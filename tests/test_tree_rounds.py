@@ -198,3 +198,52 @@ def test_rounds_up_to_the_last_row(kind, extra):
             t = (want[len(seq.generated):] + [1])[0]
             sd.round_tree([seq], [[Node(-1, (t + 1) % cfg["vocab"]), Node(-1, t), Node(0, 3), Node(1, 4), Node(2, 5)]], left)
     assert seq.generated[: extra + 1] == want and m.seqs[1].length <= 64
+
+
+# ----------------------------------------------------------------------------- the server
+class _Guesses:
+    """Candidates with the right token best or second best in turn: leaves beside the spine, and down it, are accepted and turned down."""
+
+    def __init__(self, server, texts, vocab):
+        self.server, self.texts, self.vocab = server, texts, vocab
+
+    def __call__(self, seq, depth):
+        return [], []
+
+    def candidates(self, seq):
+        from spark_engine_b200.spec.drafters import Candidates
+        i, n = self.server.by_slot[seq.slot].id, len(seq.generated)
+        right = (self.texts[i][n: n + 3] + [0, 0, 0])[:3]
+        ids = torch.tensor([[(t + 7 + a) % self.vocab if a != (n % 2, 0, 1)[j] else t for a in range(4)] for j, t in enumerate(right)])
+        return Candidates(ids=ids, unary=torch.tensor([[4.0, 3.0, 2.0, 1.0]] * 3), edges=torch.zeros(2, 4, 4), path=[0, 0, 0], conf=[0.9] * 3)
+
+
+def check_server(device):
+    """Requests through admission, shared rounds of trees, more requests than slots, prompts and ends at page borders, a continued conversation: the
+    text is that of plain decoding."""
+    from spark_engine_b200.config import EngineConfig
+    from spark_engine_b200.serving.worker import EngineServer
+    from test_vabunex import _serve
+    cfg, T = setup("dense")
+    mc = U.D.read_config(cfg)
+    es = EngineServer(mc, U.D.from_tensors(mc, T, device, torch.float32), EngineConfig(max_seqs=2, kv_tokens=1024, prefill_chunk=48, spec="lookup", spec_depth=3,
+                                                                                     spec_tree_widths="3,2,2", dtype="float32"), device=device)
+    prompts = {i: U.prompt(n, cfg["vocab"], n) for i, n in enumerate((41, 52, 116, 3, 128))}
+    texts = {i: U.oracle_greedy(cfg, T, p, 12) for i, p in prompts.items()}
+    es.spec.drafter = _Guesses(es, texts, cfg["vocab"])
+    done = _serve(es, [{"id": i, "prompt_ids": p, "max_new": 12} for i, p in prompts.items()])
+    for i in prompts:
+        assert done[i]["token_ids"] == texts[i], i
+    p = prompts[0] + done[0]["token_ids"] + [1, 2]
+    texts[9] = U.oracle_greedy(cfg, T, p, 9)
+    assert _serve(es, [{"id": 9, "prompt_ids": p, "max_new": 9}])[9]["token_ids"] == texts[9]
+    assert 0 < es.totals["accepted_drafts"] < es.totals["drafted_tokens"]
+
+
+def test_server_with_trees():
+    check_server("cpu")
+
+
+@pytest.mark.gpu
+def test_server_with_trees_on_the_device():
+    check_server("cuda")
