@@ -4,6 +4,7 @@
   libspark_kernels_<family>.so : the part of it one model family needs (`kernel_library`)
   _runtime*.so        : C++ host runtime (KV pool, scheduler core, prefix-cache I/O, ...) as a pybind11 module
   _tree*.so           : checks and launches of the tree verification ops on torch tensors
+  _sampling*.so       : the same for the ops between a round's logits and its tokens
 
 Usage: `python -m spark_engine_b200.build [--force]`.
 """
@@ -59,10 +60,18 @@ def kernel_library(family: str) -> str:
     return build_kernels(family=family)
 
 
+def _layout(header: str, flag: str) -> list:
+    """The argument structures that kernels and bindings share, as a number that both carry and that is compared when they meet."""
+    with open(os.path.join(CSRC, "common", header), "rb") as f:
+        return [f"-D{flag}={zlib.crc32(f.read())}u"]
+
+
 def _tree_layout() -> list:
-    """The argument structures that kernels and `_tree` share, as a number that both carry and that is compared when they meet."""
-    with open(os.path.join(CSRC, "common", "tree_args.h"), "rb") as f:
-        return [f"-DSPARK_TREE_LAYOUT={zlib.crc32(f.read())}u"]
+    return _layout("tree_args.h", "SPARK_TREE_LAYOUT")
+
+
+def _sampling_layout() -> list:
+    return _layout("sampling_args.h", "SPARK_SAMPLING_LAYOUT")
 
 
 def build_kernels(force=False, verbose=False, family=None) -> str:
@@ -77,7 +86,7 @@ def build_kernels(force=False, verbose=False, family=None) -> str:
         obj = os.path.join(LIBDIR, os.path.basename(cu)[:-3] + ".o")
         objs.append(obj)
         if force or _newer([cu] + headers, obj):
-            jobs.append([NVCC] + NVCC_FLAGS + _tree_layout() + (["-Xptxas", "-v"] if verbose else []) + ["-c", cu, "-o", obj])
+            jobs.append([NVCC] + NVCC_FLAGS + _tree_layout() + _sampling_layout() + (["-Xptxas", "-v"] if verbose else []) + ["-c", cu, "-o", obj])
     with cf.ThreadPoolExecutor(max_workers=8) as ex:
         for log in ex.map(_run, jobs):
             if verbose and log:
@@ -102,20 +111,28 @@ def build_runtime(force=False) -> str:
     return out
 
 
-def build_tree(force=False) -> str:
+def _build_bindings(name: str, source: str, header: str, layout: list, force: bool) -> str:
     os.makedirs(LIBDIR, exist_ok=True)
-    out = os.path.join(LIBDIR, "_tree" + sysconfig.get_config_var("EXT_SUFFIX"))
-    src = os.path.join(CSRC, "bindings", "tree_ops.cpp")
-    if force or _newer([src, os.path.join(CSRC, "common", "tree_args.h")], out):
+    out = os.path.join(LIBDIR, name + sysconfig.get_config_var("EXT_SUFFIX"))
+    src = os.path.join(CSRC, "bindings", source)
+    if force or _newer([src, os.path.join(CSRC, "bindings", "plumbing.h"), os.path.join(CSRC, "common", header)], out):
         import torch
         from torch.utils import cpp_extension as ext
         inc = [os.path.join(CSRC, "common"), *ext.include_paths("cuda"), sysconfig.get_paths()["include"]]
         lib = os.path.join(os.path.dirname(torch.__file__), "lib")
-        _run(["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-DTORCH_EXTENSION_NAME=_tree", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
-             + _tree_layout()
+        _run(["g++", "-O2", "-std=c++17", "-shared", "-fPIC", f"-DTORCH_EXTENSION_NAME={name}", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+             + layout
              + ["-isystem" + i if "torch" in i else "-I" + i for i in inc] + [src, "-o", out, "-L" + lib, "-Wl,-rpath," + lib]
              + ["-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10_cuda", "-lc10"])
     return out
+
+
+def build_tree(force=False) -> str:
+    return _build_bindings("_tree", "tree_ops.cpp", "tree_args.h", _tree_layout(), force)
+
+
+def build_sampling(force=False) -> str:
+    return _build_bindings("_sampling", "sampling_ops.cpp", "sampling_args.h", _sampling_layout(), force)
 
 
 def build_race_stress(sanitizer: str = "thread", force=False) -> str:
@@ -133,10 +150,11 @@ def build_race_stress(sanitizer: str = "thread", force=False) -> str:
 
 
 def build_all(force=False, verbose=False):
-    with cf.ThreadPoolExecutor(max_workers=1) as ex:
-        tree = ex.submit(build_tree, force)
+    with cf.ThreadPoolExecutor(max_workers=2) as ex:
+        bindings = [ex.submit(build_tree, force), ex.submit(build_sampling, force)]
         out = build_kernels(force, verbose), build_runtime(force)
-        tree.result()
+        for b in bindings:
+            b.result()
     return out
 
 

@@ -1,83 +1,26 @@
 // Device side of ops/tree.py: arguments checked, outputs and workspaces taken from torch's allocator, kernels launched on the tensors' device
 // and its current stream.  In C++ because a round makes these calls for every layer and the kernels take a few microseconds.
-#include <c10/cuda/CUDAGuard.h>
-#include <c10/cuda/CUDAStream.h>
-#include <torch/extension.h>
-
 #include <algorithm>
 #include <cmath>
 #include <cstdlib>
-#include <sstream>
-#include <utility>
-#include <vector>
 
+#include "plumbing.h"
 #include "tree_args.h"
-
-namespace py = pybind11;
-using at::Tensor;
-using Opt = std::optional<Tensor>;
 
 namespace {
 
 // ------------------------------------------------------------------------------------------------ plumbing
-struct Entry {                                   // an entry point of the kernel library
-  const char* name;
-  int kernels = 1;                               // of a call
-  void* fn = nullptr;
-};
 Entry e_tables{"spark_block_tables"}, e_maps{"spark_slot_maps"}, e_conv{"spark_path_conv"}, e_commit{"spark_commit_paths"}, e_attn{"spark_tree_attn", 2};
-int64_t launched = 0;                            // kernels since it was last asked for
-int64_t take_launched() { return std::exchange(launched, 0); }
-struct Device { int* status = nullptr; int sms = 0; };
-std::vector<Device> devices;
 
 void bind_entry(const std::string& name, uintptr_t fn) {
   for (Entry* e : {&e_tables, &e_maps, &e_conv, &e_commit, &e_attn})
     if (name == e->name) { e->fn = reinterpret_cast<void*>(fn); return; }
   throw py::value_error("no entry " + name);
 }
-void bind_device(int index, uintptr_t status, int sms) {
-  if (static_cast<int>(devices.size()) <= index) devices.resize(index + 1);
-  devices[index] = {reinterpret_cast<int*>(status), sms};
-}
-bool knows_device(int index) { return index >= 0 && index < static_cast<int>(devices.size()) && devices[index].sms > 0; }
-
-template <class... A>
-[[noreturn]] void refuse(const A&... a) {
-  std::ostringstream s;
-  (s << ... << a);
-  throw py::value_error(s.str());
-}
-#define NEED(c, ...) do { if (!(c)) refuse(__VA_ARGS__); } while (0)
-
-struct On {                                      // the tensors' device and its current stream
-  c10::cuda::OptionalCUDAGuard guard;
-  Device dev;
-  cudaStream_t stream;
-  explicit On(const Tensor& t) {
-    NEED(t.is_cuda() && knows_device(t.get_device()), "no such device: ", t.device());
-    if (c10::cuda::current_device() != t.get_device()) guard.set_device(t.device());
-    dev = devices[t.get_device()];
-    stream = c10::cuda::getCurrentCUDAStream(t.get_device()).stream();
-  }
-  template <class... A>
-  void launch(const Entry& e, A... args) const {
-    const int rc = reinterpret_cast<int (*)(A..., cudaStream_t)>(e.fn)(args..., stream);
-    if (rc) throw std::runtime_error(std::string(e.name) + " failed with code " + std::to_string(rc));
-    launched += e.kernels;
-  }
-};
-
-void need_ints(const char* name, const Tensor& t, int64_t n, const at::Device& dev) {
-  NEED(t.scalar_type() == at::kInt && t.device() == dev && t.dim() == 1 && t.is_contiguous() && (n < 0 || t.size(0) == n), name,
-       " must be a contiguous int32 tensor", n < 0 ? "" : " of ", n < 0 ? "" : std::to_string(n), " on ", dev, ", not ", t.toString(), " ", t.sizes());
-}
 void need_tables(const Tensor& t) {
   NEED(t.scalar_type() == at::kInt && t.dim() == 2 && t.is_contiguous() && t.size(1) > 0, "tables must be a contiguous int32 tensor [slots, pages]");
   NEED(t.numel() <= 1 << 24, "tables of more than 2^24 entries");
 }
-int* ip(const Tensor& t) { return t.numel() ? static_cast<int*>(t.data_ptr()) : nullptr; }
-int* ip(const Opt& t) { return t ? ip(*t) : nullptr; }
 int64_t quantum(const Tensor& t) { return 16 / t.element_size(); }
 // Stride of dimension i; 0 where it has one entry, whose stride may be anything and means nothing.
 int64_t step(const Tensor& t, int64_t i) { return t.size(i) < 2 ? 0 : t.stride(i); }

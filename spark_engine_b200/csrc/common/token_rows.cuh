@@ -1,0 +1,134 @@
+// Logits of a row as the token kernels see them: their order, the adjustments that clients ask for, reductions over a cluster's CTAs.
+#pragma once
+#include <cooperative_groups.h>
+
+#include "rows.cuh"
+#include "sampling_args.h"
+
+namespace spark {
+
+namespace cg = cooperative_groups;
+
+__device__ __forceinline__ float logit(const float* p) { return *p; }
+__device__ __forceinline__ float logit(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+__device__ __forceinline__ float logit(const __half* p) { return __half2float(*p); }
+
+// What is not a number is no token, as -inf; zeros are equal whatever their sign.
+__device__ __forceinline__ float plain_logit(float z) { return z == z ? z + 0.f : -INFINITY; }
+
+// ------------------------------------------------------------------------------------------------ adjustments
+
+// A row's adjustments, for the columns that belong to ids offset .. offset + V.
+struct RowAdjust {
+  const int* counts = nullptr;                     // the row's, or null
+  const int *drafted = nullptr, *bias_ids = nullptr;
+  const float* bias = nullptr;
+  const uint32_t* allowed = nullptr;
+  float rep = 1.f, pres = 0.f, freq = 0.f;
+  int nd = 0, nb = 0;
+
+  __device__ __forceinline__ RowAdjust(const Adjustments& a, int r, int* status) {
+    const int slot = a.slots ? a.slots[r] : r;
+    if (slot >= 0) {
+      if (a.counts) {
+        if (slot < a.n_slots) counts = a.counts + slot * a.ld_counts;
+        else set_status(status, ST_BOUNDS, r, slot, a.n_slots);
+      }
+      if (a.repetition) rep = a.repetition[r];
+      if (a.presence) pres = a.presence[r];
+      if (a.frequency) freq = a.frequency[r];
+      if (a.drafted) { nd = a.n_drafted; drafted = a.drafted + static_cast<long long>(r) * nd; }
+    }
+    if (a.bias_ids) { nb = a.n_bias; bias_ids = a.bias_ids + static_cast<long long>(r) * nb; bias = a.bias + static_cast<long long>(r) * nb; }
+    if (a.allowed) allowed = a.allowed + static_cast<long long>(r) * a.words;
+  }
+  // Rounded after every step, as the definition is: products and differences are not contracted.
+  __device__ __forceinline__ float penalised(float z, int count, int more) const {
+    const int c = (count >> 1) + more;
+    if (count > 0 || more > 0) z = z > 0.f ? __fdiv_rn(z, rep) : __fmul_rn(z, rep);
+    z = __fsub_rn(z, __fmul_rn(freq, static_cast<float>(c)));
+    return __fsub_rn(z, c > 0 ? pres : 0.f);
+  }
+  __device__ __forceinline__ bool allows(int col) const { return !allowed || (allowed[col >> 5] >> (col & 31) & 1); }
+  // Column `col` with nothing drafted and no bias.
+  __device__ __forceinline__ float common(float z, int col) const {
+    z = penalised(z, counts ? counts[col] : 0, 0);
+    return allows(col) ? z : -INFINITY;
+  }
+  __device__ __forceinline__ int entries() const { return nd + nb; }
+  __device__ __forceinline__ int entry(int i) const { return i < nd ? drafted[i] : bias_ids[i - nd]; }
+  // Entry i's column from its logit, all of the lists' entries of its id counted; false where an entry before it is of the same id.  `ids`: the entries.
+  __device__ __forceinline__ bool listed(int i, const int* ids, int col, float z, float& y) const {
+    const int id = ids[i];
+    int more = 0;
+    for (int j = 0; j < nd; ++j) {
+      if (ids[j] != id) continue;
+      if (j < i) return false;
+      ++more;
+    }
+    y = penalised(z, counts ? counts[col] : 0, more);
+    for (int j = nd; j < nd + nb; ++j) {
+      if (ids[j] != id) continue;
+      if (j < i) return false;
+      y = __fadd_rn(y, bias[j - nd]);
+    }
+    if (!allows(col)) y = -INFINITY;
+    return true;
+  }
+};
+
+// ------------------------------------------------------------------------------------------------ reductions
+
+struct Best {                                      // the first of an order: value descending, id ascending
+  float v;
+  int id;
+};
+__device__ __forceinline__ Best first_of(Best a, Best b) { return b.v > a.v || (b.v == a.v && b.id < a.id) ? b : a; }
+constexpr int NO_ID = 0x7fffffff;
+
+template <class V>
+__device__ __forceinline__ V shfl_words(V v, int o) {
+  static_assert(sizeof(V) % 4 == 0, "words");
+  union { V v; int w[sizeof(V) / 4]; } a, b;
+  a.v = v;
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(V) / 4); ++i) b.w[i] = __shfl_xor_sync(0xffffffffu, a.w[i], o);
+  return b.v;
+}
+
+// Values of a row's cluster: each CTA's in its mailbox, one of two in turn, so that one barrier per reduction is enough.
+struct alignas(16) Mail { unsigned long long w[2]; };
+struct Mailboxes {
+  Mail box[2], warp[32];
+};
+struct Cluster {
+  cg::cluster_group g;
+  Mailboxes* mine;
+  int phase = 0, rank, size;
+  __device__ __forceinline__ explicit Cluster(Mailboxes* m) : g(cg::this_cluster()), mine(m), rank(static_cast<int>(g.block_rank())), size(static_cast<int>(g.num_blocks())) {}
+
+  // op over all threads of the cluster, in an order that is the same in every run; every thread gets it.
+  template <class V, class Op>
+  __device__ __forceinline__ V reduce(V v, V none, Op op) {
+    static_assert(sizeof(V) <= sizeof(Mail), "mailboxes");
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = blockDim.x >> 5;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v = op(v, shfl_words(v, o));
+    if (lane == 0) *reinterpret_cast<V*>(&mine->warp[w]) = v;
+    __syncthreads();
+    if (w == 0) {
+      v = lane < nw ? *reinterpret_cast<V*>(&mine->warp[lane]) : none;
+#pragma unroll
+      for (int o = 16; o; o >>= 1) v = op(v, shfl_words(v, o));
+      if (lane == 0) *reinterpret_cast<V*>(&mine->box[phase]) = v;
+    }
+    g.sync();
+    v = lane < size ? *reinterpret_cast<V*>(g.map_shared_rank(&mine->box[phase], lane)) : none;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v = op(v, shfl_words(v, o));
+    phase ^= 1;
+    return v;
+  }
+};
+
+}  // namespace spark
