@@ -13,8 +13,28 @@ __device__ __forceinline__ float logit(const float* p) { return *p; }
 __device__ __forceinline__ float logit(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 __device__ __forceinline__ float logit(const __half* p) { return __half2float(*p); }
 
-// What is not a number is no token, as -inf; zeros are equal whatever their sign.
-__device__ __forceinline__ float plain_logit(float z) { return z == z ? z + 0.f : -INFINITY; }
+// What is not a number is no token, as -inf.
+__device__ __forceinline__ float plain_logit(float z) { return fmaxf(z, -INFINITY); }
+
+template <class T> constexpr int LOGITS_16B = 16 / sizeof(T);
+__device__ __forceinline__ void unpack(const uint4& q, float (&f)[4]) {
+  f[0] = __uint_as_float(q.x); f[1] = __uint_as_float(q.y); f[2] = __uint_as_float(q.z); f[3] = __uint_as_float(q.w);
+}
+template <class H>
+__device__ __forceinline__ void unpack_halves(const uint4& q, float (&f)[8]) {
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const H* h = reinterpret_cast<const H*>(&w[i]);
+    f[2 * i] = logit(h);
+    f[2 * i + 1] = logit(h + 1);
+  }
+}
+template <class T>
+__device__ __forceinline__ void unpack_logits(const uint4& q, float (&f)[LOGITS_16B<T>]) {
+  if constexpr (sizeof(T) == 4) unpack(q, f);
+  else unpack_halves<T>(q, f);
+}
 
 // ------------------------------------------------------------------------------------------------ adjustments
 
@@ -96,6 +116,15 @@ __device__ __forceinline__ V shfl_words(V v, int o) {
   return b.v;
 }
 
+template <class V>
+__device__ __forceinline__ V bcast_words(V v) {    // lane 0's
+  union { V v; int w[sizeof(V) / 4]; } a, b;
+  a.v = v;
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(V) / 4); ++i) b.w[i] = __shfl_sync(0xffffffffu, a.w[i], 0);
+  return b.v;
+}
+
 // Values of a row's cluster: each CTA's in its mailbox, one of two in turn, so that one barrier per reduction is enough.
 struct alignas(16) Mail { unsigned long long w[2]; };
 struct Mailboxes {
@@ -107,9 +136,16 @@ struct Cluster {
   int phase = 0, rank, size;
   __device__ __forceinline__ explicit Cluster(Mailboxes* m) : g(cg::this_cluster()), mine(m), rank(static_cast<int>(g.block_rank())), size(static_cast<int>(g.num_blocks())) {}
 
-  // op over all threads of the cluster, in an order that is the same in every run; every thread gets it.
+  __device__ __forceinline__ void sync() {
+    if (size > 1) g.sync();
+    else __syncthreads();
+  }
+  template <class V>
+  __device__ __forceinline__ V* of(V* p, int r) { return g.map_shared_rank(p, r); }
+
+  // op over the block's threads; warp 0 gets it.
   template <class V, class Op>
-  __device__ __forceinline__ V reduce(V v, V none, Op op) {
+  __device__ __forceinline__ V block(V v, V none, Op op) {
     static_assert(sizeof(V) <= sizeof(Mail), "mailboxes");
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = blockDim.x >> 5;
 #pragma unroll
@@ -120,14 +156,21 @@ struct Cluster {
       v = lane < nw ? *reinterpret_cast<V*>(&mine->warp[lane]) : none;
 #pragma unroll
       for (int o = 16; o; o >>= 1) v = op(v, shfl_words(v, o));
-      if (lane == 0) *reinterpret_cast<V*>(&mine->box[phase]) = v;
     }
-    g.sync();
-    v = lane < size ? *reinterpret_cast<V*>(g.map_shared_rank(&mine->box[phase], lane)) : none;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) v = op(v, shfl_words(v, o));
-    phase ^= 1;
     return v;
+  }
+  // op over all threads of the cluster, in an order that is the same in every run; every thread gets it.
+  template <class V, class Op>
+  __device__ __forceinline__ V reduce(V v, V none, Op op) {
+    v = block(v, none, op);
+    if (threadIdx.x == 0) *reinterpret_cast<V*>(&mine->box[phase]) = v;
+    sync();
+    const int lane = threadIdx.x & 31;
+    v = lane < size ? *reinterpret_cast<V*>(size > 1 ? of(&mine->box[phase], lane) : &mine->box[phase]) : none;
+#pragma unroll
+    for (int o = 8; o; o >>= 1) v = op(v, shfl_words(v, o));       // (at most 16 CTAs; the lanes behind them hold nothing)
+    phase ^= 1;
+    return bcast_words(v);
   }
 };
 
