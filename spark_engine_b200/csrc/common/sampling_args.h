@@ -52,7 +52,6 @@ struct SampleRows {
   const float *top_p, *min_p;
   int *out, *status;
   int R, V, type, sms;
-  Adjustments a;
 };
 
 struct LogprobRows {

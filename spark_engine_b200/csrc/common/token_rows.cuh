@@ -116,19 +116,11 @@ __device__ __forceinline__ V shfl_words(V v, int o) {
   return b.v;
 }
 
-template <class V>
-__device__ __forceinline__ V bcast_words(V v) {    // lane 0's
-  union { V v; int w[sizeof(V) / 4]; } a, b;
-  a.v = v;
-#pragma unroll
-  for (int i = 0; i < static_cast<int>(sizeof(V) / 4); ++i) b.w[i] = __shfl_sync(0xffffffffu, a.w[i], 0);
-  return b.v;
-}
-
-// Values of a row's cluster: each CTA's in its mailbox, one of two in turn, so that one barrier per reduction is enough.
-struct alignas(16) Mail { unsigned long long w[2]; };
+// Values of a row's cluster.  A CTA writes its value to every CTA's boxes and all meet at a barrier: what is read then is near.  Two sets in turn, so that
+// one barrier per reduction is enough.
+struct alignas(16) Mail { unsigned long long w[4]; };
 struct Mailboxes {
-  Mail box[2], warp[32];
+  Mail box[2][16], warp[32];
 };
 struct Cluster {
   cg::cluster_group g;
@@ -163,14 +155,13 @@ struct Cluster {
   template <class V, class Op>
   __device__ __forceinline__ V reduce(V v, V none, Op op) {
     v = block(v, none, op);
-    if (threadIdx.x == 0) *reinterpret_cast<V*>(&mine->box[phase]) = v;
-    sync();
     const int lane = threadIdx.x & 31;
-    v = lane < size ? *reinterpret_cast<V*>(size > 1 ? of(&mine->box[phase], lane) : &mine->box[phase]) : none;
-#pragma unroll
-    for (int o = 8; o; o >>= 1) v = op(v, shfl_words(v, o));       // (at most 16 CTAs; the lanes behind them hold nothing)
+    if (threadIdx.x < size) *reinterpret_cast<V*>(size > 1 ? of(&mine->box[phase][rank], lane) : &mine->box[phase][0]) = v;
+    sync();
+    v = *reinterpret_cast<V*>(&mine->box[phase][0]);
+    for (int r = 1; r < size; ++r) v = op(v, *reinterpret_cast<V*>(&mine->box[phase][r]));
     phase ^= 1;
-    return bcast_words(v);
+    return v;
   }
 };
 

@@ -8,22 +8,21 @@
 //
 // What is kept is always a prefix of the order, given by its last token.
 //
-// A row lies in the shared memory of a cluster's CTAs: it is read once, whatever the passes over it.  The prefix is found among a few candidates where
-// there are few: the largest of every eight logits go to a histogram, whose first bins with k tokens (or top_p of the weight) in them hold what is kept,
-// since the other seven only add to it; what lies in these bins goes to a list, which one CTA sorts.  Where more are kept than the list takes, the k-th
-// token comes from a histogram of all, and for top_p a token is drawn first and its weight in front looked at then: a prefix of the order that ends in
-// front of a token drawn in vain holds all that is kept, and holds half as much on average.
+// A row is read once, by one CTA or, where there are few rows, by a cluster's; what stays of it in shared memory is the largest of every eight logits.
+// Their histogram's first bins with k tokens (or top_p of the weight) in them hold what is kept, since the other seven can only add to it; the groups that
+// reach into these bins are read again, and what of them lies there goes to a list, in which one CTA finds the prefix.  Where more are kept than the list
+// takes, the row is read again: the k-th token comes from a histogram of all, and for top_p a token is drawn first and the weight in front of it looked at
+// then: what lies in front of a token drawn in vain holds all that is kept, and half as much as before on average.
 #include "../common/token_rows.cuh"
 
 namespace spark {
 
 constexpr int ROW_THREADS = 512, ROW_WARPS = ROW_THREADS / 32;
-constexpr int ROW_BLOCK = 256;                     // logits that a warp takes at once, 8 per lane
-constexpr int ROW_SLICE_MAX = SAMPLE_MAX_V / 16;
-constexpr int ROW_PAD = ROW_BLOCK + 8;
+constexpr int CHUNK = 1024;                        // logits that a warp takes at once, 32 per lane
 constexpr int BINS = 1024;                         // of a sixteenth of a bit of weight; what weighs less than 2^-64 shares the last one
 constexpr float BINS_PER_BIT = 16.f;
 constexpr int LIST = 2048;
+constexpr int FEW = 256;                           // of the list: ordered by counting
 
 using u64 = unsigned long long;
 
@@ -41,234 +40,226 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ float max4(const float4& a) { return fmaxf(fmaxf(a.x, a.y), fmaxf(a.z, a.w)); }
+__device__ __forceinline__ float warp_highest(float v) {
+  const int b = __float_as_int(v);
+  const int m = __reduce_max_sync(0xffffffffu, b ^ (b >> 31 & 0x7fffffff));
+  return __int_as_float(m ^ (m >> 31 & 0x7fffffff));
+}
+__device__ __forceinline__ double pow2(float n) {  // 2^n for a whole n <= 0
+  return n < -1022.f ? 0.0 : __hiloint2double((1023 + static_cast<int>(n)) << 20, 0);
+}
 
 // A prefix of the order: its last token.
 struct Prefix { float z; int id; };
 __device__ __forceinline__ bool within(const Prefix& p, float z, int id) { return z > p.z || (z == p.z && id <= p.id); }
 constexpr float LOWEST = -3.402823466e38f;
+__device__ __forceinline__ float at_least(float z) { return fmaxf(z, LOWEST); }
+
+// Sum of 2^(z c) in units of 2^E, E whole: a change of units changes no bit.
+struct Mass { double s; float E; };
+__device__ __forceinline__ Mass add_mass(Mass a, Mass b) {
+  const float E = fmaxf(a.E, b.E);
+  return {(a.s ? a.s * pow2(a.E - E) : 0) + (b.s ? b.s * pow2(b.E - E) : 0), E};
+}
+constexpr Mass NO_MASS{0.0, LOWEST};
 
 struct RowShared {
   Mailboxes mail;
-  unsigned count[BINS], mass[BINS];
-  u64 list[LIST];
-  u64 warp[ROW_WARPS];
-  double dwarp[ROW_WARPS];
+  unsigned hist[BINS];
+  u64 list[LIST], weight[FEW], wsum[ROW_WARPS];
+  double dsum[ROW_WARPS];
+  float E[16];
   unsigned n_list, before, kept;
   int bin;
-  float z;
+  float z, local_E;
+  double log;
   Prefix cut;
   u64 total;
 };
 
 // ------------------------------------------------------------------------------------------------ a CTA's part of a row
 
-// This CTA's logits as fp32 in shared memory: z[j] is id first + j; -inf in front of them, behind them and up to whole blocks.
-struct Slice {
-  float* z;
-  int first, blocks;
+// Places j of a row from a 16-byte boundary on: id j + first at it; those in [lo, hi) are the row's.  Lane l of a warp has N = 16 bytes' logits of every
+// 32 * N: value i of its 32 in chunk k is place k * CHUNK + (i / N) * 32 N + l * N + i % N.
+template <class T>
+struct Row {
+  static constexpr int N = LOGITS_16B<T>;
+  const T* base;
+  int lo, hi, chunk0, chunks;                      // this CTA's chunks
 
-  template <class F>
-  __device__ __forceinline__ void quads(F f) const {          // f(four logits, id of the first)
-    const int lane = threadIdx.x & 31;
-    for (int k = threadIdx.x >> 5; k < blocks; k += ROW_WARPS) {
-      const int j = k * ROW_BLOCK + lane * 4;
-      const float4 a = *reinterpret_cast<const float4*>(z + j), b = *reinterpret_cast<const float4*>(z + j + 128);
-      f(a, first + j);
-      f(b, first + j + 128);
-    }
+  __device__ __forceinline__ Row(const T* x, int V, int rank, int per) {
+    lo = static_cast<int>(reinterpret_cast<uintptr_t>(x) / sizeof(T) % N);
+    hi = lo + V;
+    base = x - lo;
+    chunk0 = rank * per;
+    chunks = max(0, min(per, (hi + CHUNK - 1) / CHUNK - chunk0));
   }
-  template <class F>
-  __device__ __forceinline__ void each(F f) const {
-    quads([&](const float4& a, int id) { f(a.x, id); f(a.y, id + 1); f(a.z, id + 2); f(a.w, id + 3); });
-  }
-};
+  __device__ __forceinline__ int id(int j) const { return j - lo; }
+  __device__ __forceinline__ float one(int j) const { return j >= lo && j < hi ? plain_logit(logit(base + j)) : -INFINITY; }
+  static __device__ __forceinline__ int place(int chunk, int i, int lane) { return chunk * CHUNK + (i / N) * (32 * N) + lane * N + i % N; }
 
-// Columns [b, e) of a row, its best token seen on the way.  Whole 16 bytes are read as such wherever the row starts; their place in shared memory is
-// shifted as theirs in memory is.
-template <class T, bool ADJUSTED>
-__device__ __forceinline__ Slice load_slice(float* z, const T* x, int b, int e, const RowAdjust* adj, int* ids, Best& best) {
-  constexpr int N = LOGITS_16B<T>;
-  const int t = threadIdx.x, n = e - b;
-  const int shift = n ? static_cast<int>(reinterpret_cast<uintptr_t>(x + b) / sizeof(T) % N) : 0, end = shift + n;
-  const Slice s{z, b - shift, (end + ROW_BLOCK - 1) / ROW_BLOCK};
-  int entries = 0;
-  if constexpr (ADJUSTED) {
-    entries = adj->entries();
-    for (int i = t; i < entries; i += ROW_THREADS) ids[i] = adj->entry(i);
-  }
-  const auto one = [&](int j) {
-    float v = logit(x + b - shift + j);
-    if constexpr (ADJUSTED) v = adj->common(v, s.first + j);
-    z[j] = v = plain_logit(v);
-    best = first_of(best, Best{v, s.first + j});
-  };
-  const int v0 = shift ? 1 : 0, v1 = end / N;                  // whole vectors
-  if (t < N && t >= shift && shift && t < end) one(t);
-  if (t < N && v1 >= v0 && v1 * N + t < end) one(v1 * N + t);
-  if (t < shift) z[t] = -INFINITY;
-  for (int j = end + t; j < s.blocks * ROW_BLOCK; j += ROW_THREADS) z[j] = -INFINITY;
-  float top = -INFINITY;
-  int at = -1;
-  const uint4* src = reinterpret_cast<const uint4*>(x + b - shift);
-  const int* cnt = ADJUSTED && adj->counts ? adj->counts + s.first : nullptr;
-  const bool counts16 = (reinterpret_cast<uintptr_t>(cnt) & 15) == 0;
-  constexpr int U = 4;
-  for (int v = v0 + t; v < v1; v += U * ROW_THREADS) {
-    uint4 q[U];
+  __device__ __forceinline__ void load(int chunk, float (&v)[32]) const {
+    const int lane = threadIdx.x & 31, j0 = chunk * CHUNK;
+    if (j0 >= lo && j0 + CHUNK <= hi) {
+      uint4 q[32 / N];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (v + u * ROW_THREADS < v1) q[u] = __ldg(src + v + u * ROW_THREADS);
+      for (int i = 0; i < 32 / N; ++i) q[i] = __ldg(reinterpret_cast<const uint4*>(base + j0 + i * 32 * N) + lane);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int j = (v + u * ROW_THREADS) * N;
-      if (v + u * ROW_THREADS >= v1) break;
-      float f[N];
-      unpack_logits<T>(q[u], f);
-      if constexpr (ADJUSTED) {
-        int c[N] = {};
-        if (cnt && counts16) {
+      for (int i = 0; i < 32 / N; ++i) {
+        float f[N];
+        unpack_logits<T>(q[i], f);
 #pragma unroll
-          for (int i = 0; i < N; i += 4) *reinterpret_cast<int4*>(c + i) = __ldg(reinterpret_cast<const int4*>(cnt + j + i));
-        } else if (cnt) {
-#pragma unroll
-          for (int i = 0; i < N; ++i) c[i] = __ldg(cnt + j + i);
-        }
-        uint32_t bits = 0xffffffffu;
-        if (adj->allowed) {
-          const int col = s.first + j;
-          bits = __funnelshift_r(adj->allowed[col >> 5], adj->allowed[(col + N - 1) >> 5], col & 31);
-        }
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          f[i] = adj->penalised(f[i], c[i], 0);
-          if (!(bits >> i & 1)) f[i] = -INFINITY;
-        }
+        for (int e = 0; e < N; ++e) v[i * N + e] = plain_logit(f[e]);
       }
-      float m = -INFINITY;
+    } else {
 #pragma unroll
-      for (int i = 0; i < N; ++i) m = fmaxf(m, f[i] = plain_logit(f[i]));
-      if (m > top) { top = m; at = j; }
-#pragma unroll
-      for (int i = 0; i < N; i += 4) *reinterpret_cast<float4*>(z + j + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+      for (int i = 0; i < 32; ++i) v[i] = one(place(chunk, i, lane));
     }
   }
-  if (at >= 0) {
-    int i = 0;
-    while (i < N - 1 && z[at + i] != top) ++i;
-    best = first_of(best, Best{top, s.first + at + i});
-  }
-  if (entries) {                                               // drafted tokens and biases: their columns again
-    __syncthreads();
-    for (int i = t; i < entries; i += ROW_THREADS) {
-      const int col = ids[i];
-      float y;
-      if (col >= b && col < e && adj->listed(i, ids, col, logit(x + col), y)) z[col - s.first] = plain_logit(y);
+  // f(32 logits, chunk) for each of a warp's chunks that `wanted(chunk's number in the CTA)`.
+  template <class W, class F>
+  __device__ __forceinline__ void stream(W wanted, F f) const {
+    for (int k = threadIdx.x >> 5; k < chunks; k += ROW_WARPS) {
+      if (!wanted(k)) continue;
+      float v[32];
+      load(chunk0 + k, v);
+      f(v, k);
     }
-    __syncthreads();
-    best = Best{-INFINITY, NO_ID};
-    s.each([&](float v, int id) { best = first_of(best, Best{v, id}); });
   }
-  return s;
-}
-
-template <class F>
-__device__ __forceinline__ u64 row_count(const Slice& s, Cluster& c, F f) {
-  u64 n = 0;
-  s.each([&](float z, int id) { n += f(z, id); });
-  return c.reduce(n, u64{0}, [](u64 a, u64 b) { return a + b; });
-}
-__device__ __forceinline__ double row_total(Cluster& c, double v) { return c.reduce(v, 0.0, [](double a, double b) { return a + b; }); }
-
-// Weights relative to the best token's.  The difference comes first: it is exact or rounded by half a step, whatever the logits' size.
-struct Weights {
-  float top, c;                                    // c = log2(e) / T
-  __device__ __forceinline__ float bits(float z) const { return (z - top) * c; }
-  __device__ __forceinline__ float operator()(float z) const { return exp2_fast(bits(z)); }
-  __device__ __forceinline__ int bin(float z) const { return min(static_cast<int>(bits(z) * -BINS_PER_BIT), BINS - 1); }
 };
 
-// Weight of what `f` lets through; four at a time in fp32, 64 bits beyond.
-template <class F>
-__device__ __forceinline__ double row_mass(const Slice& s, Cluster& c, const Weights& w, F f) {
-  double sum = 0;
-  s.quads([&](const float4& a, int id) {
-    const float p = f(a.x, id) ? w(a.x) : 0.f, q = f(a.y, id + 1) ? w(a.y) : 0.f, r = f(a.z, id + 2) ? w(a.z) : 0.f, t = f(a.w, id + 3) ? w(a.w) : 0.f;
-    sum += (p + q) + (r + t);
-  });
-  return row_total(c, sum);
+// The largest logits of groups of 8 << shift values of a lane; group (k, q, lane) at (k * (4 >> shift) + q) * 32 + lane.
+struct Groups {
+  float* g;
+  int shift;
+  __device__ __forceinline__ void put(const float (&m)[4], int k) const {
+    const int lane = threadIdx.x & 31;
+    if (shift == 0) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) g[(k * 4 + q) * 32 + lane] = m[q];
+    } else if (shift == 1) {
+      g[k * 64 + lane] = fmaxf(m[0], m[1]);
+      g[k * 64 + 32 + lane] = fmaxf(m[2], m[3]);
+    } else {
+      g[k * 32 + lane] = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+    }
+  }
+  // Whether the chunk has a logit of `least` or more.
+  __device__ __forceinline__ bool reaches(int k, float least) const {
+    const int lane = threadIdx.x & 31;
+    float m = -INFINITY;
+    for (int q = 0; q < 4 >> shift; ++q) m = fmaxf(m, g[(k * (4 >> shift) + q) * 32 + lane]);
+    return __any_sync(0xffffffffu, m >= least);
+  }
+};
+
+__device__ __forceinline__ void max8(const float (&v)[32], float (&m)[4]) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    m[q] = v[8 * q];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) m[q] = fmaxf(m[q], v[8 * q + e]);
+  }
+}
+
+// A warp's best token so far: chunks come in the order of their ids, so that only larger logits replace it.
+template <class T>
+__device__ __forceinline__ void note_best(const Row<T>& row, const float (&v)[32], float mine, float highest, int chunk, Best& best) {
+  if (!(highest > best.v)) return;
+  int j = NO_ID;
+  if (mine == highest) {
+#pragma unroll
+    for (int i = 31; i >= 0; --i)
+      if (v[i] == highest) j = Row<T>::place(chunk, i, threadIdx.x & 31);
+  }
+  best = Best{highest, row.id(__reduce_min_sync(0xffffffffu, j))};
 }
 
 // ------------------------------------------------------------------------------------------------ histograms and lists
 
-__device__ __forceinline__ void clear_bins(RowShared& sh) {
-  for (int i = threadIdx.x; i < BINS; i += ROW_THREADS) sh.count[i] = sh.mass[i] = 0;
-}
-
-// The leader's: the first bin with which the cluster's bins hold `k` tokens, or `target` of weight (2^16 of a bin's best token's each); the last one
-// where they do not; with it the tokens in front of it.
-__device__ __forceinline__ void find_bin(RowShared& sh, Cluster& c, bool by_count, unsigned k, double target) {
-  const int t = threadIdx.x, lane = t & 31, w = t >> 5;
-  constexpr int PER = BINS / ROW_THREADS;
-  double v[PER], sum = 0;
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int b = t * PER + i;
-    unsigned n = 0;
-    double m = 0;
-    for (int r = 0; r < c.size; ++r) {
-      const RowShared* p = c.size > 1 ? c.of(&sh, r) : &sh;
-      if (by_count) n += p->count[b];
-      else m += p->mass[b];
-    }
-    v[i] = by_count ? static_cast<double>(n) : m * exp2f(b * (-1.f / BINS_PER_BIT));
-    sum += v[i];
+// Weights 2^((z - from) c - E).  `from` is 0, and the product exact and the difference rounded once, but for scores of 2^20 and more, in which that
+// would leave too few bits of the difference: they are seen from the best.
+struct Weights {
+  float c, E, from;
+  __device__ __forceinline__ float bits(float z) const { return fmaf(z - from, c, -E); }
+  __device__ __forceinline__ float operator()(float z) const { return exp2_fast(bits(z)); }
+  __device__ __forceinline__ int bin(float z) const { return max(0, min(static_cast<int>(bits(z) * -BINS_PER_BIT), BINS - 1)); }
+  // A logit a little below the bin's edge.
+  __device__ __forceinline__ float edge(int b) const {
+    if (b >= BINS - 1) return LOWEST;
+    const float y = E - (b + 1) * (1.f / BINS_PER_BIT), z = y / c;
+    return at_least(from + z - (fabsf(z) + fabsf(from)) * (1.f / 1048576) - (fabsf(E) + (b + 1)) * (1.f / 4194304) / c);
   }
-  double incl = sum;
+};
+
+// The first bin with which the bins of the cluster's CTAs hold `target` (tokens; or weight, in 2^16 of a bin's highest): the last one where they do not.
+// In units of 2^E; a CTA's bins are in units of its own.  Into sh.bin, with the tokens in front of it in sh.before.
+__device__ __forceinline__ void find_bin(RowShared& sh, Cluster& c, bool by_count, float E, double target) {
+  const int t = threadIdx.x, lane = t & 31, w = t >> 5;
+  static_assert(BINS == 2 * ROW_THREADS, "two bins per thread");
+  double v0 = 0, v1 = 0;
+  if (c.size == 1) {
+    v0 = sh.hist[2 * t];
+    v1 = sh.hist[2 * t + 1];
+  } else {
+#pragma unroll 8
+    for (int r = 0; r < c.size; ++r) {
+      const float d = (E - sh.E[r]) * BINS_PER_BIT;            // (a multiple of 16)
+      const int b = 2 * t - (d < 2.f * BINS ? static_cast<int>(d) : 2 * BINS);
+      const uint2 n = b >= 0 ? *reinterpret_cast<const uint2*>(c.of(sh.hist, r) + b) : make_uint2(0, 0);
+      v0 += n.x;
+      v1 += n.y;
+    }
+  }
+  if (!by_count) {
+    v0 *= exp2f(t * (-2.f / BINS_PER_BIT));
+    v1 *= exp2f((2 * t + 1) * (-1.f / BINS_PER_BIT));
+  }
+  double incl = v0 + v1;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const double y = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += y;
   }
-  if (lane == 31) sh.dwarp[w] = incl;
+  if (lane == 31) sh.dsum[w] = incl;
   if (t == 0) { sh.bin = BINS - 1; sh.before = 0; }
   __syncthreads();
-  double at = incl - sum;
-  for (int i = 0; i < w; ++i) at += sh.dwarp[i];
-  if (by_count) target = k;
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    if (at < target && at + v[i] >= target) { sh.bin = t * PER + i; sh.before = by_count ? static_cast<unsigned>(at) : 0; }
-    at += v[i];
-  }
+  double at = incl - (v0 + v1);
+  for (int i = 0; i < w; ++i) at += sh.dsum[i];
+  if (at < target && at + v0 >= target) { sh.bin = 2 * t; sh.before = static_cast<unsigned>(at); }
+  else if (at + v0 < target && at + v0 + v1 >= target) { sh.bin = 2 * t + 1; sh.before = static_cast<unsigned>(at + v0); }
+  __syncthreads();
 }
 
-// Tokens of the row that `f` lets through, into the leader's list; their number, which may be more than it takes.  Everyone has it.
-template <class F>
-__device__ __forceinline__ unsigned gather(RowShared& sh, const Slice& s, Cluster& c, float least, F f) {
-  s.quads([&](const float4& a, int id) {
-    if (!(max4(a) >= least)) return;
-    const float v[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (v[i] >= least && f(v[i], id + i)) {
-        const unsigned at = atomicAdd(&sh.n_list, 1u);
-        if (at < LIST) sh.list[at] = list_key(v[i], id + i);
-      }
-  });
-  c.sync();
-  unsigned n = 0;
-  for (int r = 0; r < c.size; ++r) n += c.size > 1 ? *c.of(&sh.n_list, r) : sh.n_list;
-  return n;
+__device__ __forceinline__ void to_list(RowShared& sh, float z, int id) {
+  const unsigned at = atomicAdd(&sh.n_list, 1u);
+  if (at < LIST) sh.list[at] = list_key(z, id);
 }
-__device__ __forceinline__ void collect(RowShared& sh, Cluster& c) {           // the leader's copy of the others' lists
-  unsigned at = sh.n_list;
-  for (int r = 1; r < c.size; ++r) {
-    const unsigned n = *c.of(&sh.n_list, r);
-    const u64* from = c.of(sh.list, r);
-    for (unsigned i = threadIdx.x; i < n; i += ROW_THREADS) sh.list[at + i] = from[i];
-    at += n;
+// The CTAs' lists behind the leader's own; how many they hold together, which everyone gets and which may be more than a list takes (nothing is moved then).
+__device__ __forceinline__ unsigned join_lists(RowShared& sh, Cluster& c) {
+  if (c.size == 1) {
+    __syncthreads();
+    return sh.n_list;
   }
+  __syncthreads();
+  const unsigned mine = sh.n_list;
+  struct Place { unsigned n, before; };
+  if (threadIdx.x < c.size) c.of(&sh.mail.box[c.phase][c.rank], threadIdx.x)->w[0] = mine;
+  c.sync();
+  unsigned n = 0, before = 0;
+  for (int r = 0; r < c.size; ++r) {
+    const unsigned m = static_cast<unsigned>(sh.mail.box[c.phase][r].w[0]);
+    before += r < c.rank ? m : 0;
+    n += m;
+  }
+  c.phase ^= 1;
+  if (n > LIST) return n;
+  if (c.rank) {
+    u64* to = c.of(sh.list, 0) + before;
+    for (unsigned i = threadIdx.x; i < mine; i += ROW_THREADS) to[i] = sh.list[i];
+  }
+  c.sync();
+  return n;
 }
 
 // list[0, n) in the row's order (descending keys; all differ).
@@ -288,6 +279,29 @@ __device__ __forceinline__ void sort_list(RowShared& sh, unsigned n) {
     }
 }
 
+// Up to FEW entries: how many of the list are in front of an entry, and their weight.  Threads share an entry; the first of them has it.
+struct Counted { u64 key, weight, before; unsigned rank; bool mine; };
+__device__ __forceinline__ Counted count_list(RowShared& sh, unsigned n, bool weights) {
+  int per = ROW_THREADS / 32;
+  while (per * n > ROW_THREADS) per /= 2;                      // (n <= 256: at least 2)
+  const unsigned at = threadIdx.x / per, part = threadIdx.x % per;
+  Counted e{0, 0, 0, 0, part == 0 && at < n};
+  if (at < n) {
+    e.key = sh.list[at];
+    for (unsigned j = part; j < n; j += per) {
+      const bool front = sh.list[j] > e.key;
+      e.rank += front;
+      if (weights && front) e.before += sh.weight[j];
+    }
+  }
+  for (int o = per / 2; o; o /= 2) {
+    e.rank += __shfl_xor_sync(0xffffffffu, e.rank, o);
+    e.before += __shfl_xor_sync(0xffffffffu, e.before, o);
+  }
+  if (at < n && weights) e.weight = sh.weight[at];
+  return e;
+}
+
 // ------------------------------------------------------------------------------------------------ draws
 
 __device__ __forceinline__ u64 mix64(u64 x) {
@@ -296,20 +310,22 @@ __device__ __forceinline__ u64 mix64(u64 x) {
   return x ^ (x >> 31);
 }
 
-struct Top2 { float a1; int id; float a2; int none; };         // the best score, its token, the second best score
+struct Top2 { float a1; int id; float a2, z; };                // the best score, its token, the second best score, the token's logit
+constexpr Top2 NO_TOP{-INFINITY, NO_ID, -INFINITY, -INFINITY};
 __device__ __forceinline__ Top2 best2(Top2 x, Top2 y) {
-  const bool first = x.a1 >= y.a1;
-  return first ? Top2{x.a1, x.id, fmaxf(x.a2, y.a1), 0} : Top2{y.a1, y.id, fmaxf(y.a2, x.a1), 0};
+  return x.a1 >= y.a1 ? Top2{x.a1, x.id, fmaxf(x.a2, y.a1), x.z} : Top2{y.a1, y.id, fmaxf(y.a2, x.a1), y.z};
 }
+struct Win { float v; int id; float z; int none; };
+__device__ __forceinline__ Win first_win(Win a, Win b) { return b.v > a.v || (b.v == a.v && b.id < a.id) ? b : a; }
 
 // A token's score is known from below and above at the price of a few fp32 operations: `margin` is more than twice what the rough one may be off.
 // Where the two best are further apart than that, the best is the best; else both are computed as the definition says.
 struct Race {
   float temp, c, margin;
   u64 key;
-  __device__ __forceinline__ Race(float T, float c_, float top, long long seed, long long pos)
-      : temp(T), c(c_), margin(1.f / 512 + (fabsf(top / T) + 64.f) * (1.f / 524288)),
-        key((static_cast<u64>(seed) * 0x9E3779B97F4A7C15ull) ^ (static_cast<u64>(pos + 1) * 0xBF58476D1CE4E5B9ull)) {}
+  __device__ __forceinline__ Race(float T, float c_, long long seed, long long pos)
+      : temp(T), c(c_), margin(0), key((static_cast<u64>(seed) * 0x9E3779B97F4A7C15ull) ^ (static_cast<u64>(pos + 1) * 0xBF58476D1CE4E5B9ull)) {}
+  __device__ __forceinline__ void scale(float top) { margin = 1.f / 512 + (fabsf(top / temp) + 64.f) * (1.f / 524288); }
   __device__ __forceinline__ u64 hash(int id) const { return mix64(static_cast<u64>(id) * 0x9E3779B97F4A7C15ull + key); }
   __device__ __forceinline__ float exact(float z, int id) const {
     const double u = (static_cast<double>(hash(id) >> 11) + 0.5) * (1.0 / 9007199254740992.0);
@@ -323,56 +339,70 @@ struct Race {
   }
 };
 
-__device__ __forceinline__ float warp_highest(float v) {
-  const int b = __float_as_int(v);
-  const int m = __reduce_max_sync(0xffffffffu, b ^ (b >> 31 & 0x7fffffff));
-  return __int_as_float(m ^ (m >> 31 & 0x7fffffff));
-}
-
-// The token that wins among those within `kept`.  -log u >= 1 - u, so that a score is at most z / T - log(1 - u): most tokens are out of the race by the
-// 32 upper bits of their hash, without a logarithm.
-__device__ __forceinline__ int draw_row(const Slice& s, Cluster& c, const Race& race, const Prefix& kept, const Best& top) {
-  Top2 m{-INFINITY, NO_ID, -INFINITY, 0};
-  float bound = race.rough(top.v, race.hash(top.id));          // (the best token is always kept)
-  float off = (race.margin - bound) * 1.4426950408889634f + 32.f;
-  s.quads([&](const float4& a, int id0) {
-    if (__all_sync(0xffffffffu, !(max4(a) >= kept.z))) return;
-    const float v[4] = {a.x, a.y, a.z, a.w};
+// A warp's race over the logits that come by.  -log u >= 1 - u, so that a score is at most z / T - log(1 - u): most tokens are out of it by the 32
+// upper bits of their hash, without a logarithm.
+struct Racer {
+  Top2 m = NO_TOP;
+  float bound, off;
+  __device__ __forceinline__ void raise(const Race& race, float b) {
+    bound = b;
+    off = (race.margin - bound) * 1.4426950408889634f + 32.f;
+  }
+  template <class T>
+  __device__ __forceinline__ void run(const Race& race, const Row<T>& row, const float (&v)[32], int chunk, const Prefix& kept) {
     bool more = false;
+    const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (!within(kept, v[i], id0 + i)) continue;
-      const u64 h = race.hash(id0 + i);
+    for (int i = 0; i < 32; ++i) {
+      const int id = row.id(Row<T>::place(chunk, i, lane));
+      if (!within(kept, v[i], id)) continue;
+      const u64 h = race.hash(id);
       if (static_cast<float>(static_cast<uint32_t>(~h >> 32)) > exp2_fast(fmaf(v[i], race.c, off))) continue;
       const float y = race.rough(v[i], h);
-      m = best2(m, Top2{y, id0 + i, -INFINITY, 0});
+      m = best2(m, Top2{y, id, -INFINITY, v[i]});
       more |= y > bound;
     }
-    if (__any_sync(0xffffffffu, more)) {
-      bound = fmaxf(bound, warp_highest(m.a1));
-      off = (race.margin - bound) * 1.4426950408889634f + 32.f;
+    if (__any_sync(0xffffffffu, more)) raise(race, fmaxf(bound, warp_highest(m.a1)));
+  }
+};
+
+// The winner among the tokens within `kept`, from the two best of a race.
+template <class T, class W>
+__device__ __forceinline__ Win settle(const Row<T>& row, Cluster& c, const Race& race, const Prefix& kept, Top2 m, W wanted) {
+  m = c.reduce(m, NO_TOP, best2);
+  if (m.a2 < m.a1 - race.margin) return Win{m.a1, m.id, m.z, 0};
+  Win b{-INFINITY, NO_ID, -INFINITY, 0};
+  const Win none = b;
+  row.stream(wanted, [&](const float (&v)[32], int k) {
+#pragma unroll 1
+    for (int i = 0; i < 32; ++i) {
+      const int j = Row<T>::place(row.chunk0 + k, i, threadIdx.x & 31), id = row.id(j);
+      const float z = row.one(j);
+      if (!within(kept, z, id) || race.rough(z, race.hash(id)) < m.a1 - race.margin) continue;
+      b = first_win(b, Win{race.exact(z, id), id, z, 0});
     }
   });
-  m = c.reduce(m, Top2{-INFINITY, NO_ID, -INFINITY, 0}, best2);
-  if (m.a2 < m.a1 - race.margin) return m.id;
-  Best b{-INFINITY, NO_ID};
-  s.each([&](float v, int id) {
-    if (!within(kept, v, id)) return;
-    const u64 h = race.hash(id);
-    if (race.rough(v, h) < m.a1 - race.margin) return;
-    b = first_of(b, Best{race.exact(v, id), id});
-  });
-  return c.reduce(b, Best{-INFINITY, NO_ID}, first_of).id;
+  return c.reduce(b, none, first_win);
 }
 
-// The leader's: the token that wins among the first n of its list.  Thread 0 has it.
+// The leader's: the winner among its candidates, of which a thread has one at most (`in`).  Thread 0 has it.
+__device__ __forceinline__ int draw_few(RowShared& sh, Cluster& c, const Race& race, u64 key, bool in) {
+  Top2 m = in ? Top2{race.rough(list_z(key), race.hash(list_id(key))), list_id(key), -INFINITY, 0} : NO_TOP;
+  m = c.block(m, NO_TOP, best2);
+  if (threadIdx.x == 0) sh.kept = m.a2 < m.a1 - race.margin;
+  __syncthreads();
+  if (sh.kept) return m.id;
+  Best b = in ? Best{race.exact(list_z(key), list_id(key)), list_id(key)} : Best{-INFINITY, NO_ID};
+  return c.block(b, Best{-INFINITY, NO_ID}, first_of).id;
+}
+// The same among the first n of its list.
 __device__ __forceinline__ int draw_list(RowShared& sh, Cluster& c, const Race& race, unsigned n) {
-  Top2 m{-INFINITY, NO_ID, -INFINITY, 0};
+  Top2 m = NO_TOP;
   for (unsigned i = threadIdx.x; i < n; i += ROW_THREADS) {
     const u64 k = sh.list[i];
     m = best2(m, Top2{race.rough(list_z(k), race.hash(list_id(k))), list_id(k), -INFINITY, 0});
   }
-  m = c.block(m, Top2{-INFINITY, NO_ID, -INFINITY, 0}, best2);
+  m = c.block(m, NO_TOP, best2);
   if (threadIdx.x == 0) sh.kept = m.a2 < m.a1 - race.margin;
   __syncthreads();
   if (sh.kept) return m.id;
@@ -386,303 +416,434 @@ __device__ __forceinline__ int draw_list(RowShared& sh, Cluster& c, const Race& 
 
 // ------------------------------------------------------------------------------------------------ the k-th token
 
+template <class T, class F>
+__device__ __forceinline__ u64 row_count(const Row<T>& row, Cluster& c, F f) {
+  u64 n = 0;
+  row.stream([](int) { return true; }, [&](const float (&v)[32], int k) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) n += f(v[i], row.id(Row<T>::place(row.chunk0 + k, i, threadIdx.x & 31))) ? 1 : 0;
+  });
+  return c.reduce(n, u64{0}, [](u64 a, u64 b) { return a + b; });
+}
+
 // By the bits of keys and ids, for the rare row in which more tokens than a list takes share a bin.
-__device__ __forceinline__ Prefix kth_by_bits(const Slice& s, Cluster& c, const Prefix& of, u64 k) {
-  if (row_count(s, c, [&](float z, int id) { return u64{within(of, z, id)}; }) <= k) return of;
+template <class T>
+__device__ __noinline__ Prefix kth_by_bits(const Row<T>& row, Cluster& c, const Prefix of, u64 k) {
+  if (row_count(row, c, [&](float z, int id) { return within(of, z, id); }) <= k) return of;
   uint32_t key = 0;
   for (int bit = 31; bit >= 0; --bit) {
     const uint32_t t = key | 1u << bit;
-    if (row_count(s, c, [&](float z, int id) { return u64{order_key(z) >= t && within(of, z, id)}; }) >= k) key = t;
+    if (row_count(row, c, [&](float z, int id) { return order_key(z) >= t && within(of, z, id); }) >= k) key = t;
   }
   const float v = key_order(key);
-  k -= row_count(s, c, [&](float z, int) { return u64{z > v}; });
+  k -= row_count(row, c, [&](float z, int) { return z > v; });
   int id = 0;
   for (int bit = 20; bit >= 0; --bit) {            // the largest id with less than k of these in front of it
     const int t = id | 1 << bit;
-    if (row_count(s, c, [&](float z, int i) { return u64{z == v && i < t && within(of, z, i)}; }) < k) id = t;
+    if (row_count(row, c, [&](float z, int i) { return z == v && i < t && within(of, z, i); }) < k) id = t;
   }
   return Prefix{v, id};
 }
 
-__device__ __forceinline__ Prefix kth_token(RowShared& sh, const Slice& s, Cluster& c, const Weights& w, const Prefix& of, unsigned k) {
+// The prefix of the first k tokens of `of` = (least logit, any id).
+template <class T>
+__device__ __forceinline__ Prefix kth_token(RowShared& sh, const Row<T>& row, const Groups& groups, Cluster& c, const Weights& w, const Prefix& of, unsigned k) {
   c.sync();                                        // (nobody reads the bins and lists of before any more)
-  clear_bins(sh);
+  for (int i = threadIdx.x; i < BINS; i += ROW_THREADS) sh.hist[i] = 0;
   if (threadIdx.x == 0) sh.n_list = 0;
+  if (threadIdx.x < 16) sh.E[threadIdx.x] = w.E;
   __syncthreads();
-  s.quads([&](const float4& a, int) {
-    const float v[4] = {a.x, a.y, a.z, a.w};
+  row.stream([&](int i) { return groups.reaches(i, of.z); }, [&](const float (&v)[32], int) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (v[i] >= of.z) atomicAdd(&sh.count[w.bin(v[i])], 1u);
+    for (int i = 0; i < 32; ++i)
+      if (v[i] >= of.z) atomicAdd(&sh.hist[w.bin(v[i])], 1u);
   });
   c.sync();
+  find_bin(sh, c, true, w.E, k);
+  const int bin = sh.bin;
+  const unsigned before = sh.before;               // (0 with the last bin where the row has fewer than k tokens)
+  row.stream([&](int i) { return groups.reaches(i, fmaxf(of.z, w.edge(bin))); }, [&](const float (&v)[32], int n) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (v[i] >= of.z && w.bin(v[i]) == bin) to_list(sh, v[i], row.id(Row<T>::place(row.chunk0 + n, i, threadIdx.x & 31)));
+  });
+  const unsigned n = join_lists(sh, c);
+  if (n > LIST) return kth_by_bits(row, c, of, k);
   if (c.rank == 0) {
-    find_bin(sh, c, true, k, 0);
-    __syncthreads();
-  }
-  c.sync();
-  const RowShared* lead = c.size > 1 ? c.of(&sh, 0) : &sh;
-  const int bin = lead->bin;
-  const unsigned before = lead->before;
-  // (the last bin's `before` is 0 where the row has fewer than k tokens)
-  const unsigned n = gather(sh, s, c, of.z, [&](float z, int) { return w.bin(z) == bin; });
-  if (n > LIST) return kth_by_bits(s, c, of, k);
-  if (c.rank == 0) {
-    collect(sh, c);
     sort_list(sh, n);
-    if (threadIdx.x == 0) {
-      const u64 last = k - before <= n ? sh.list[k - before - 1] : 0;
-      sh.cut = last ? Prefix{list_z(last), list_id(last)} : of;
-    }
+    const u64 last = k - before <= n ? sh.list[k - before - 1] : 0;
+    const Prefix cut = last ? Prefix{list_z(last), list_id(last)} : of;
+    if (threadIdx.x < c.size) (c.size > 1 ? c.of(&sh, threadIdx.x) : &sh)->cut = cut;
   }
   c.sync();
-  return lead->cut;
+  return sh.cut;
 }
 
 // ------------------------------------------------------------------------------------------------ kernels
 
-template <class T, bool ADJUSTED>
-__global__ void __launch_bounds__(ROW_THREADS)
-sample_kernel(const __grid_constant__ SampleRows a, int slice) {
-  extern __shared__ __align__(16) float z[];
+__device__ __forceinline__ Groups groups_at(float* smem, int chunks_per_cta) {
+  const int n = chunks_per_cta * 128;
+  return Groups{smem, n <= 20480 ? 0 : n <= 40960 ? 1 : 2};
+}
+static int group_bytes(int chunks_per_cta) {
+  const int n = chunks_per_cta * 128;
+  return 4 * (n <= 20480 ? n : n <= 40960 ? n / 2 : n / 4);
+}
+
+// The smallest logit that is not too improbable, decided in 64 bits.
+__device__ __forceinline__ float min_p_logit(float top, float temp, float mp) {
+  const double top64 = top, T64 = temp, least = log(static_cast<double>(mp));
+  const auto scaled = [&](float v) { return (static_cast<double>(v) - top64) / T64; };
+  float v = fminf(static_cast<float>(top64 + T64 * least), top);
+  for (int i = 0; i < 8 && scaled(v) >= least; ++i) v = nextafterf(v, -INFINITY);
+  for (int i = 0; i < 16 && scaled(v) < least; ++i) v = nextafterf(v, INFINITY);
+  return at_least(v);
+}
+
+template <class T>
+__global__ void __launch_bounds__(ROW_THREADS, 2)
+sample_kernel(const __grid_constant__ SampleRows a, int per) {
+  extern __shared__ __align__(16) float smem[];
   __shared__ RowShared sh;
   Cluster c(&sh.mail);
-  const int t = threadIdx.x, r = blockIdx.x / c.size, b = min(c.rank * slice, a.V), e = min(b + slice, a.V);
-  const T* x = static_cast<const T*>(a.x) + r * a.ldx;
-  Best top{-INFINITY, NO_ID};
-  Slice s;
-  if constexpr (ADJUSTED) {
-    const RowAdjust adj(a.a, r, a.status);
-    s = load_slice<T, true>(z, x, b, e, &adj, reinterpret_cast<int*>(sh.list), top);
-  } else {
-    s = load_slice<T, false>(z, x, b, e, nullptr, nullptr, top);
-  }
-  clear_bins(sh);
+  const int t = threadIdx.x, r = blockIdx.x / c.size;
+  const float temp = a.temps[r], mp = a.min_p ? a.min_p[r] : 0.f, p = a.top_p ? a.top_p[r] : 1.f;
+  const int asked = a.top_k ? a.top_k[r] : 0, k = asked < a.V ? asked : 0;
+  const Row<T> row(static_cast<const T*>(a.x) + r * a.ldx, a.V, c.rank, per);
+  const Groups groups = groups_at(smem, per);
+  const bool greedy = !(temp > 0.f) || k == 1 || p <= 0.f || mp > 1.f, by_p = p < 1.f, by_k = k > 0, by_min = mp > 0.f && isfinite(temp);
+  const bool all = !greedy && !by_p && !by_k && !by_min;
+  // (products of it with 0 and infinity are 0 and infinity)
+  const float scale = greedy ? 0.f : fmaxf(fminf(__fdiv_rn(1.4426950408889634f, temp), -LOWEST), 1e-44f);
+  const bool sums = !greedy && by_p && !by_k && !by_min;
+  Race race(temp, scale, a.seeds[r], a.positions[r]);
+  for (int i = t; i < BINS; i += ROW_THREADS) sh.hist[i] = 0;
   if (t == 0) sh.n_list = 0;
-  const float temp = a.temps[r];
-  float p = a.top_p ? a.top_p[r] : 1.f;
-  const float mp = a.min_p ? a.min_p[r] : 0.f;
-  int k = a.top_k ? a.top_k[r] : 0;
-  if (k >= a.V) k = 0;
-  top = c.reduce(top, Best{-INFINITY, NO_ID}, first_of);
+  const auto every = [](int) { return true; };
+
+  Best top{-INFINITY, NO_ID};
+  Mass mass = NO_MASS;
+  row.stream(every, [&](const float (&v)[32], int i) {
+    float m[4];
+    max8(v, m);
+    const float mine = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), highest = warp_highest(mine);
+    note_best(row, v, mine, highest, row.chunk0 + i, top);
+    if (!greedy && !all) groups.put(m, i);
+    if (sums && highest > -INFINITY) {             // the chunk's weight in units of its own: the same in every batch
+      const float E = ceilf(highest * scale);
+      float s = 0.f;
+#pragma unroll
+      for (int q = 0; q < 32; q += 4)
+        s += (exp2_fast(fmaf(v[q], scale, -E)) + exp2_fast(fmaf(v[q + 1], scale, -E))) + (exp2_fast(fmaf(v[q + 2], scale, -E)) + exp2_fast(fmaf(v[q + 3], scale, -E)));
+      mass = add_mass(mass, Mass{s, E});
+    }
+  });
+  if (!greedy && !all && !(by_min && !by_k && !by_p)) {        // the largest of every eight in bins, below the CTA's own best
+    const Best own = c.block(top, Best{-INFINITY, NO_ID}, first_of);
+    if (t == 0) sh.local_E = own.v > -INFINITY ? ceilf(own.v * scale) : LOWEST;
+    __syncthreads();
+    const Weights w{scale, sh.local_E, 0.f};
+    for (int i = t; i < row.chunks * (128 >> groups.shift); i += ROW_THREADS) {
+      const float m = groups.g[i];
+      if (!(m > -INFINITY)) continue;
+      const int bin = w.bin(m);
+      if (by_k) atomicAdd(&sh.hist[bin], 1u);
+      else atomicAdd(&sh.hist[bin], static_cast<unsigned>(fminf(exp2_fast(w.bits(m) + bin * (1.f / BINS_PER_BIT)) * 65536.f, 65536.f)));
+    }
+    if (t < c.size) (c.size > 1 ? c.of(&sh, t) : &sh)->E[c.rank] = w.E;
+    __syncthreads();
+  }
+  struct First { Best top; Mass mass; };
+  const First first = c.reduce(First{top, mass}, First{{-INFINITY, NO_ID}, NO_MASS}, [](First x, First y) { return First{first_of(x.top, y.top), add_mass(x.mass, y.mass)}; });
+  top = first.top;
   const bool lead = c.rank == 0 && t == 0;
-  // Greedy too: a best score that is not finite, beside which noise is nothing.
-  if (top.v == -INFINITY || !(temp > 0.f) || !isfinite(__fdiv_rn(top.v, temp)) || k == 1 || p <= 0.f || mp > 1.f) {
+  // Greedy too: a best score beside which noise is nothing.
+  if (greedy || top.v == -INFINITY || !(fabsf(__fdiv_rn(top.v, temp)) < 1073741824.f)) {
     if (lead) a.out[r] = top.v == -INFINITY ? -1 : top.id;
-    c.sync();                                      // (a CTA's mailbox stays until all have read it)
+    c.sync();                                      // (what a CTA's shared memory holds stays until all have read it)
     return;
   }
-  const Weights weight{top.v, fmaxf(fminf(__fdiv_rn(1.4426950408889634f, temp), -LOWEST), 1e-44f)};       // (products of it with 0 and infinity are 0 and infinity)
-  const Race race(temp, weight.c, top.v, a.seeds[r], a.positions[r]);
+  race.scale(top.v);
+  const bool far = !(fabsf(top.v * scale) < 1048576.f);
+  const Weights weight = far ? Weights{scale, 0.f, top.v} : Weights{scale, ceilf(top.v * scale), 0.f};
   Prefix kept{LOWEST, NO_ID};
-  if (mp > 0.f && isfinite(temp)) {                // the smallest logit that is not too improbable, decided in 64 bits
-    if (t == 0) {
-      const double top64 = top.v, T64 = temp, least = log(static_cast<double>(mp));
-      const auto scaled = [&](float v) { return (static_cast<double>(v) - top64) / T64; };
-      float v = fminf(static_cast<float>(top64 + T64 * least), top.v);
-      for (int i = 0; i < 8 && scaled(v) >= least; ++i) v = nextafterf(v, -INFINITY);
-      for (int i = 0; i < 16 && scaled(v) < least; ++i) v = nextafterf(v, INFINITY);
-      sh.z = v;
-    }
+  if (by_min) {
+    if (t == 0) sh.z = min_p_logit(top.v, temp, mp);
     __syncthreads();
-    kept.z = fmaxf(kept.z, sh.z);
+    kept.z = sh.z;
   }
-  if (k > 0 || p < 1.f) {
-    double all = 0;
+  const auto some = [&](int i) { return all || groups.reaches(i, kept.z); };
+  // Weight of what lies within a prefix, in units of 2^E.
+  const auto mass_of = [&](const Prefix& of) {
+    double s = 0;
+    row.stream([&](int i) { return groups.reaches(i, of.z); }, [&](const float (&v)[32], int i) {
+      float f = 0.f;
+#pragma unroll
+      for (int q = 0; q < 32; ++q) f += within(of, v[q], row.id(Row<T>::place(row.chunk0 + i, q, t & 31))) ? weight(v[q]) : 0.f;
+      s += f;
+    });
+    return c.reduce(s, 0.0, [](double x, double y) { return x + y; });
+  };
+  double total = sums && !far ? first.mass.s * pow2(first.mass.E - weight.E) : by_p && !by_k ? mass_of(kept) : 0;
+  if (by_k || by_p) {
     unsigned n = LIST + 1;
-    if (k <= LIST) {
-      // weight of the row, and the best of every eight in bins
-      const bool by_count = k > 0;
-      double sum = 0;
-      const int lane = t & 31;
-      for (int i = t >> 5; i < s.blocks; i += ROW_WARPS) {
-        const float4 u = *reinterpret_cast<const float4*>(z + i * ROW_BLOCK + lane * 4), v = *reinterpret_cast<const float4*>(z + i * ROW_BLOCK + 128 + lane * 4);
-        if (!by_count) {
-          const auto w = [&](float y) { return y >= kept.z ? weight(y) : 0.f; };
-          sum += (w(u.x) + w(u.y)) + (w(u.z) + w(u.w));
-          sum += (w(v.x) + w(v.y)) + (w(v.z) + w(v.w));
+    if (k <= LIST && !far) {
+      find_bin(sh, c, by_k, weight.E, by_k ? k : p * total * 65536.0 * (1 + 1.0 / 262144));
+      const float least = fmaxf(kept.z, weight.edge(sh.bin));
+      if (sh.bin < BINS - 1 || a.V <= LIST) {
+        for (int i = t; i < row.chunks * (128 >> groups.shift); i += ROW_THREADS) {
+          if (!(groups.g[i] >= least)) continue;
+          const int g = i >> 5, chunk = row.chunk0 + (g >> (2 - groups.shift)), q = (g & ((4 >> groups.shift) - 1)) * (8 << groups.shift);
+          for (int e = 0; e < 8 << groups.shift; ++e) {
+            const int j = Row<T>::place(chunk, q + e, i & 31);
+            const float z = row.one(j);
+            if (z >= least) to_list(sh, z, row.id(j));
+          }
         }
-        const float m = fmaxf(max4(u), max4(v));
-        if (m >= kept.z) {
-          const int bin = weight.bin(m);
-          if (by_count) atomicAdd(&sh.count[bin], 1u);
-          else atomicAdd(&sh.mass[bin], static_cast<unsigned>(fminf(exp2_fast(weight.bits(m) + bin * (1.f / BINS_PER_BIT)) * 65536.f, 65536.f)));
-        }
+        n = join_lists(sh, c);
       }
-      all = row_total(c, sum);
-      if (c.rank == 0) find_bin(sh, c, by_count, k, p * all * 65536.0 * (1 + 1.0 / 262144));
-      c.sync();
-      const int bin = c.size > 1 ? *c.of(&sh.bin, 0) : sh.bin;
-      float least = kept.z;                        // (a little below the bin's edge)
-      if (bin < BINS - 1) {
-        const float d = (bin + 1) / (BINS_PER_BIT * weight.c) * (1 + 1.f / 1048576);
-        least = fmaxf(least, top.v - d - fabsf(top.v) * (1.f / 4194304));
-      }
-      n = gather(sh, s, c, least, [](float, int) { return true; });
     }
     if (n <= LIST) {
-      if (c.rank == 0) collect(sh, c);
-      c.sync();
       if (c.rank) return;
-      sort_list(sh, n);
-      // weights in the row's order, in whole numbers of 2^-40: every token before the one that reaches top_p is kept
-      constexpr int PER = LIST / ROW_THREADS;
-      u64 w[PER], sum = 0;
+      // Weights in whole numbers of 2^-40: every token before the one that reaches top_p is kept.
+      const auto whole = [&](u64 key) { return __float2ull_rn(weight(list_z(key)) * 1099511627776.f); };
+      const unsigned n1 = by_k ? min(n, static_cast<unsigned>(k)) : n;
+      int token;
+      if (n <= FEW) {
+        if (by_p) {
+          if (t < n) sh.weight[t] = whole(sh.list[t]);
+          __syncthreads();
+        }
+        const Counted e = count_list(sh, n, by_p);
+        bool in = e.mine && e.rank < n1;
+        if (by_p) {
+          if (e.mine && e.rank + 1 == n1) sh.total = e.before + e.weight;
+          __syncthreads();
+          const double target = static_cast<double>(p) * (by_k ? static_cast<double>(sh.total) : total * 1099511627776.0);
+          in = in && (e.rank == 0 || static_cast<double>(e.before) < target);
+        }
+        token = draw_few(sh, c, race, e.key, in);
+      } else {
+        sort_list(sh, n);
+        unsigned m = n1;
+        if (by_p) {
+          constexpr int PER = LIST / ROW_THREADS;
+          u64 w[PER], sum = 0;
 #pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const unsigned at = t * PER + i;
-        w[i] = at < n && p < 1.f ? __float2ull_rn(weight(list_z(sh.list[at])) * 1099511627776.f) : 0;
-        sum += w[i];
+          for (int i = 0; i < PER; ++i) {
+            w[i] = t * PER + i < n ? whole(sh.list[t * PER + i]) : 0;
+            sum += w[i];
+          }
+          u64 before = sum;
+          const int lane = t & 31;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const u64 y = __shfl_up_sync(0xffffffffu, before, o);
+            if (lane >= o) before += y;
+          }
+          if (lane == 31) sh.wsum[t >> 5] = before;
+          if (t == 0) sh.kept = 0;
+          __syncthreads();
+          before -= sum;
+          for (int i = 0; i < t >> 5; ++i) before += sh.wsum[i];
+          u64 at = before;
+#pragma unroll
+          for (int i = 0; i < PER; ++i) {
+            at += w[i];
+            if (t * PER + i + 1 == n1) sh.total = at;
+          }
+          __syncthreads();
+          const double target = static_cast<double>(p) * (by_k ? static_cast<double>(sh.total) : total * 1099511627776.0);
+          unsigned mine = 0;
+          at = before;
+#pragma unroll
+          for (int i = 0; i < PER; ++i) {
+            const unsigned j = t * PER + i;
+            mine += j < n1 && (j == 0 || static_cast<double>(at) < target);
+            at += w[i];
+          }
+          if (mine) atomicAdd(&sh.kept, mine);
+          __syncthreads();
+          m = sh.kept;
+          __syncthreads();
+        }
+        token = draw_list(sh, c, race, m);
       }
-      const unsigned n1 = k > 0 ? min(n, static_cast<unsigned>(k)) : n;
-      unsigned m = n1;
-      if (p < 1.f) {
-        u64 incl = sum;
-        const int lane = t & 31;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const u64 y = __shfl_up_sync(0xffffffffu, incl, o);
-          if (lane >= o) incl += y;
-        }
-        if (lane == 31) sh.warp[t >> 5] = incl;
-        if (t == 0) sh.kept = 0;
-        __syncthreads();
-        u64 before = incl - sum;
-        for (int i = 0; i < t >> 5; ++i) before += sh.warp[i];
-        u64 at = before;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-          at += w[i];
-          if (t * PER + i + 1 == n1) sh.total = at;
-        }
-        __syncthreads();
-        const double target = static_cast<double>(p) * (k > 0 ? static_cast<double>(sh.total) : all * 1099511627776.0);
-        unsigned mine = 0;
-        at = before;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-          const unsigned j = t * PER + i;
-          mine += j < n1 && (j == 0 || static_cast<double>(at) < target);
-          at += w[i];
-        }
-        if (mine) atomicAdd(&sh.kept, mine);
-        __syncthreads();
-        m = sh.kept;
-        __syncthreads();
-      }
-      const int token = draw_list(sh, c, race, m);
       if (t == 0) a.out[r] = token;
       return;
     }
-    if (k > 0) {
-      kept = kth_token(sh, s, c, weight, kept, k);
-      if (p < 1.f) all = row_mass(s, c, weight, [&](float v, int id) { return within(kept, v, id); });
+    if (by_k) {
+      kept = kth_token(sh, row, groups, c, weight, kept, k);
+      if (by_p) total = mass_of(kept);
     }
-    const double target = p < 1.f ? p * all : 0;
-    int token;
-    for (;;) {
-      token = draw_row(s, c, race, kept, top);
-      if (p >= 1.f || token == top.id) break;
-      __syncthreads();
-      if (t == 0 && token >= b && token < e) sh.z = z[token - s.first];
-      c.sync();
-      const int owner = token / slice;
-      const float v = c.size > 1 ? *c.of(&sh.z, owner) : sh.z;
-      const Prefix front{v, token - 1};
-      if (row_mass(s, c, weight, [&](float y, int id) { return within(front, y, id); }) < target) break;
-      kept = front;
-    }
-    if (lead) a.out[r] = token;
-    c.sync();
-    return;
   }
-  const int token = draw_row(s, c, race, kept, top);
-  if (lead) a.out[r] = token;
+  // The best token is always kept.
+  const float start = race.rough(top.v, race.hash(top.id));
+  Racer racer;
+  racer.raise(race, start);
+  row.stream(some, [&](const float (&v)[32], int i) { racer.run(race, row, v, row.chunk0 + i, kept); });
+  Win win = settle(row, c, race, kept, racer.m, some);
+  const double target = by_p ? p * total : 0;
+  while (by_p && win.id != top.id) {               // what lies in front of it, and who wins there should that be too much
+    const Prefix front{win.z, win.id - 1};
+    const auto there = [&](int i) { return groups.reaches(i, front.z); };
+    Racer next;
+    next.raise(race, start);
+    double s = 0;
+    row.stream(there, [&](const float (&v)[32], int i) {
+      float f = 0.f;
+#pragma unroll
+      for (int q = 0; q < 32; ++q) f += within(front, v[q], row.id(Row<T>::place(row.chunk0 + i, q, t & 31))) ? weight(v[q]) : 0.f;
+      s += f;
+      next.run(race, row, v, row.chunk0 + i, front);
+    });
+    if (c.reduce(s, 0.0, [](double x, double y) { return x + y; }) < target) break;
+    win = settle(row, c, race, front, next.m, there);
+  }
+  if (lead) a.out[r] = win.id;
   c.sync();
 }
 
 template <class T>
-__global__ void __launch_bounds__(ROW_THREADS)
-logprob_kernel(const __grid_constant__ LogprobRows a, int slice) {
-  extern __shared__ __align__(16) float z[];
+__global__ void __launch_bounds__(ROW_THREADS, 2)
+logprob_kernel(const __grid_constant__ LogprobRows a, int per) {
+  extern __shared__ __align__(16) float smem[];
   __shared__ RowShared sh;
   Cluster c(&sh.mail);
-  const int tid = threadIdx.x, r = blockIdx.x / c.size, b = min(c.rank * slice, a.V), e = min(b + slice, a.V);
+  const int tid = threadIdx.x, r = blockIdx.x / c.size;
   const T* x = static_cast<const T*>(a.x) + r * a.ldx;
   const int t = a.tokens[r];
   const bool there = t >= 0 && t < a.V;
   const float zt = there ? plain_logit(logit(x + t)) : -INFINITY;
-  Best top{-INFINITY, NO_ID};
-  const Slice s = load_slice<T, false>(z, x, b, e, nullptr, nullptr, top);
-  clear_bins(sh);
-  if (tid == 0) sh.n_list = 0;
-  top = c.reduce(top, Best{-INFINITY, NO_ID}, first_of);
-  const bool listed = a.top > 1 && top.v > -INFINITY && top.v < INFINITY;
-  const Weights weight{top.v, 1.4426950408889634f};
-  const auto below = [&](float v) { return v == top.v ? 0.f : v - top.v; };       // (infinite logits: a limit)
-  struct Sums { double w; u64 before; };
-  Sums m{0, 0};
-  unsigned before = 0;
-  const int lane = tid & 31;
-  const float c2 = 1.4426950408889634f;
-  for (int i = tid >> 5; i < s.blocks; i += ROW_WARPS) {
-    const int j = i * ROW_BLOCK + lane * 4;
-    const float4 u = *reinterpret_cast<const float4*>(z + j), v = *reinterpret_cast<const float4*>(z + j + 128);
-    const float y[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
-    float w[8];
-#pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      const int id = s.first + j + (q & 3) + (q >> 2) * 128;
-      w[q] = exp2_fast(below(y[q]) * c2);
-      before += y[q] > zt || (y[q] == zt && id < t && id >= b && id < e);
-    }
-    m.w += (w[0] + w[1]) + (w[2] + w[3]);
-    m.w += (w[4] + w[5]) + (w[6] + w[7]);
-    if (listed) {
-      const float g = fmaxf(max4(u), max4(v));
-      if (g > -INFINITY) atomicAdd(&sh.count[weight.bin(g)], 1u);
-    }
+  const Row<T> row(x, a.V, c.rank, per);
+  const Groups groups = groups_at(smem, per);
+  if (a.top > 1) {
+    for (int i = tid; i < BINS; i += ROW_THREADS) sh.hist[i] = 0;
+    if (tid == 0) sh.n_list = 0;
   }
-  m.before = before;
-  m = c.reduce(m, Sums{0, 0}, [](Sums p, Sums q) { return Sums{p.w + q.w, p.before + q.before}; });
-  const double lse = log(m.w);
+  // log2(e) in two parts: z log2(e) - E as exact as its own size in fp32
+  constexpr float HI = 1.4426950408889634f, LO = static_cast<float>(1.4426950408889634 - static_cast<double>(HI));
+  Best top{-INFINITY, NO_ID};
+  Mass mass = NO_MASS;
+  unsigned before = 0;
+  const int tj = t + row.lo;
+  row.stream([](int) { return true; }, [&](const float (&v)[32], int i) {
+    const int chunk = row.chunk0 + i;
+    float m[4];
+    max8(v, m);
+    const float mine = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), highest = warp_highest(mine);
+    note_best(row, v, mine, highest, chunk, top);
+    if (a.top > 1) groups.put(m, i);
+    if (highest > -INFINITY && highest < INFINITY) {           // the chunk's sum in units of its own: the same in every batch
+      const float E = ceilf(highest * HI);
+      float s = 0.f;
+#pragma unroll
+      for (int q = 0; q < 32; q += 4) {
+        float w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = exp2_fast(fmaf(v[q + e], LO, fmaf(v[q + e], HI, -E)));
+        s += (w[0] + w[1]) + (w[2] + w[3]);
+      }
+      mass = add_mass(mass, Mass{s, E});
+    }
+    if (zt == -INFINITY || (chunk * CHUNK <= tj && tj < (chunk + 1) * CHUNK)) {
+#pragma unroll
+      for (int q = 0; q < 32; ++q) {
+        const int j = Row<T>::place(chunk, q, tid & 31);
+        before += v[q] > zt || (v[q] == zt && j < tj && j >= row.lo);
+      }
+    } else {                                                   // (equal ones are in front of it in the chunks in front of its own)
+      const float least = (chunk + 1) * CHUNK <= tj ? zt : nextafterf(zt, INFINITY);
+#pragma unroll
+      for (int q = 0; q < 32; ++q) before += v[q] >= least;
+    }
+  });
+  const bool listing = a.top > 1;
+  if (listing) {
+    const Best own = c.block(top, Best{-INFINITY, NO_ID}, first_of);
+    if (tid == 0) sh.local_E = own.v > -INFINITY ? ceilf(own.v * HI) : LOWEST;
+    __syncthreads();
+    const Weights w{HI, sh.local_E, 0.f};
+    for (int i = tid; i < row.chunks * (128 >> groups.shift); i += ROW_THREADS)
+      if (groups.g[i] > -INFINITY) atomicAdd(&sh.hist[w.bin(groups.g[i])], 1u);
+    if (tid < c.size) (c.size > 1 ? c.of(&sh, tid) : &sh)->E[c.rank] = w.E;
+    __syncthreads();
+  }
+  struct First { Best top; Mass mass; u64 before; };
+  const First first = c.reduce(First{top, mass, before}, First{{-INFINITY, NO_ID}, NO_MASS, 0},
+                               [](First p, First q) { return First{first_of(p.top, q.top), add_mass(p.mass, q.mass), p.before + q.before}; });
+  top = first.top;
   const bool lead = c.rank == 0 && tid == 0;
-  const auto lp = [&](float v) { return v == -INFINITY ? -INFINITY : static_cast<float>(static_cast<double>(below(v)) - lse); };
+  // log-probabilities: z - (E log 2 + log(sum)); seen from the best where logits are so large that this would leave too few bits of it, or infinite
+  const bool far = !(fabsf(top.v) < 1e6f);
+  double sum = first.mass.s;
+  if (far) {
+    sum = 0;
+    row.stream([](int) { return true; }, [&](const float (&v)[32], int) {
+      float f = 0.f;
+#pragma unroll
+      for (int q = 0; q < 32; ++q) f += v[q] == top.v ? 1.f : exp2_fast((v[q] - top.v) * HI);
+      sum += f;
+    });
+    sum = c.reduce(sum, 0.0, [](double p, double q) { return p + q; });
+  }
+  if (lead) sh.log = (far ? 0.0 : static_cast<double>(first.mass.E) * 0.69314718055994530942) + log(sum);
+  const auto lp = [&](float z) {
+    if (z == -INFINITY) return -INFINITY;
+    return static_cast<float>((far ? (z == top.v ? 0.0 : static_cast<double>(z) - top.v) : static_cast<double>(z)) - sh.log);
+  };
   int* ids = a.ids + static_cast<long long>(r) * a.top;
   float* lps = a.logprobs + static_cast<long long>(r) * a.top;
   if (lead) {
     a.logprob[r] = lp(zt);
-    a.rank[r] = there ? static_cast<int>(m.before) + 1 : 0;
+    a.rank[r] = there ? static_cast<int>(first.before) + 1 : 0;
     if (a.top == 1) {
       ids[0] = top.v == -INFINITY ? -1 : top.id;
       lps[0] = lp(top.v);
     }
   }
   if (a.top < 2) { c.sync(); return; }
-  if (listed) {
-    if (c.rank == 0) find_bin(sh, c, true, a.top, 0);
-    c.sync();
-    const int bin = c.size > 1 ? *c.of(&sh.bin, 0) : sh.bin;
-    float least = LOWEST;
-    if (bin < BINS - 1) least = top.v - (bin + 1) / (BINS_PER_BIT * weight.c) * (1 + 1.f / 1048576) - fabsf(top.v) * (1.f / 4194304);
-    const unsigned n = gather(sh, s, c, least, [](float, int) { return true; });
-    if (n <= LIST) {
-      if (c.rank == 0) collect(sh, c);
-      c.sync();
-      if (c.rank) return;
-      sort_list(sh, n);
-      for (unsigned i = tid; i < static_cast<unsigned>(a.top); i += ROW_THREADS) {
-        const float v = i < n ? list_z(sh.list[i]) : -INFINITY;
-        ids[i] = i < n ? list_id(sh.list[i]) : -1;
-        lps[i] = lp(v);
+  if (!far) {
+    const Weights w{HI, ceilf(top.v * HI), 0.f};
+    find_bin(sh, c, true, w.E, a.top);
+    unsigned n = LIST + 1;
+    if (sh.bin < BINS - 1 || a.V <= LIST) {
+      const float least = w.edge(sh.bin);
+      for (int i = tid; i < row.chunks * (128 >> groups.shift); i += ROW_THREADS) {
+        if (!(groups.g[i] >= least)) continue;
+        const int g = i >> 5, chunk = row.chunk0 + (g >> (2 - groups.shift)), q = (g & ((4 >> groups.shift) - 1)) * (8 << groups.shift);
+        for (int e = 0; e < 8 << groups.shift; ++e) {
+          const int j = Row<T>::place(chunk, q + e, i & 31);
+          const float z = row.one(j);
+          if (z >= least) to_list(sh, z, row.id(j));
+        }
       }
+      n = join_lists(sh, c);
+    }
+    if (n <= LIST) {
+      if (c.rank) return;
+      const auto put = [&](unsigned i, u64 key) { ids[i] = list_id(key); lps[i] = lp(list_z(key)); };
+      if (n <= FEW) {
+        const Counted e = count_list(sh, n, false);
+        if (e.mine && e.rank < a.top) put(e.rank, e.key);
+      } else {
+        sort_list(sh, n);
+        for (unsigned i = tid; i < min(n, static_cast<unsigned>(a.top)); i += ROW_THREADS) put(i, sh.list[i]);
+      }
+      for (unsigned i = n + tid; i < a.top; i += ROW_THREADS) { ids[i] = -1; lps[i] = -INFINITY; }
       return;
     }
   }
   Best last{INFINITY, -1};                         // one after the other: rows of nothing, of infinities, of very many equal logits
   for (int i = 0; i < a.top; ++i) {
     Best g{-INFINITY, NO_ID};
-    s.each([&](float v, int id) { if (v < last.v || (v == last.v && id > last.id)) g = first_of(g, Best{v, id}); });
+    row.stream([](int) { return true; }, [&](const float (&v)[32], int n) {
+#pragma unroll
+      for (int q = 0; q < 32; ++q) {
+        const int id = row.id(Row<T>::place(row.chunk0 + n, q, tid & 31));
+        if (v[q] < last.v || (v[q] == last.v && id > last.id)) g = first_of(g, Best{v[q], id});
+      }
+    });
     last = c.reduce(g, Best{-INFINITY, NO_ID}, first_of);
     if (lead) {
       ids[i] = last.v == -INFINITY ? -1 : last.id;
@@ -692,17 +853,16 @@ logprob_kernel(const __grid_constant__ LogprobRows a, int slice) {
   c.sync();
 }
 
-// CTAs of a row's cluster: enough to hold it, more where there are few rows.
-static int row_cluster(int R, int V, int sms) {
+// CTAs of a row's cluster: as many as there is room for, of four chunks each at least.
+static int row_cluster(int R, int chunks, int sms) {
   int c = 1;
-  while (c < 16 && (static_cast<long long>(c) * 20480 < V || (static_cast<long long>(R) * c * 2 <= sms && V / c > 4096))) c *= 2;
+  while (c < 16 && R * c * 2 <= 2 * sms && c * 4 < chunks) c *= 2;
   return c;
 }
 
 template <class A, class K>
 static int launch_rows(const char* name, K kern, const A& a, cudaStream_t s) {
-  const int c = row_cluster(a.R, a.V, a.sms), slice = ((a.V + c - 1) / c + ROW_BLOCK - 1) / ROW_BLOCK * ROW_BLOCK, bytes = (slice + ROW_PAD) * 4;
-  if (slice > ROW_SLICE_MAX) return -5;
+  const int chunks = (a.V + 8 + CHUNK - 1) / CHUNK, c = row_cluster(a.R, chunks, a.sms), per = (chunks + c - 1) / c, bytes = group_bytes(per);
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess ||
       cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return spark_launch_rc(name);
   cudaLaunchConfig_t cfg = {};
@@ -711,24 +871,19 @@ static int launch_rows(const char* name, K kern, const A& a, cudaStream_t s) {
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = c; attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr; cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, kern, a, slice) != cudaSuccess) return spark_launch_rc(name);
+  if (cudaLaunchKernelEx(&cfg, kern, a, per) != cudaSuccess) return spark_launch_rc(name);
   return spark_launch_rc(name);
-}
-
-template <bool ADJUSTED>
-static int sample_rows(const SampleRows& a, cudaStream_t s) {
-  if (a.type == LT_F32) return launch_rows("spark_sample_rows", sample_kernel<float, ADJUSTED>, a, s);
-  if (a.type == LT_BF16) return launch_rows("spark_sample_rows", sample_kernel<__nv_bfloat16, ADJUSTED>, a, s);
-  return launch_rows("spark_sample_rows", sample_kernel<__half, ADJUSTED>, a, s);
 }
 
 }  // namespace spark
 
 using namespace spark;
 
-extern "C" int spark_sample_rows(const SampleRows* a, int adjusted, cudaStream_t s) {
+extern "C" int spark_sample_rows(const SampleRows* a, cudaStream_t s) {
   if (a->R <= 0 || a->V <= 0) return 0;
-  return adjusted ? sample_rows<true>(*a, s) : sample_rows<false>(*a, s);
+  if (a->type == LT_F32) return launch_rows("spark_sample_rows", sample_kernel<float>, *a, s);
+  if (a->type == LT_BF16) return launch_rows("spark_sample_rows", sample_kernel<__nv_bfloat16>, *a, s);
+  return launch_rows("spark_sample_rows", sample_kernel<__half>, *a, s);
 }
 
 extern "C" int spark_logprob_rows(const LogprobRows* a, cudaStream_t s) {

@@ -62,7 +62,7 @@ def test_without_filters_it_is_the_token_of_perturbed_logits():
     assert np.array_equal(rows.draw(0.9), ops.argmax(x).cpu().numpy())
 
 
-@pytest.mark.parametrize("T", [1e-40, 1e-30, 1e-5, 1e6, float("inf")])
+@pytest.mark.parametrize("T", [1e-40, 1e-30, 1e-8, 1e-7, 1e-6, 1e-5, 1e6, float("inf")])
 def test_extreme_temperatures(T):
     for kind in ("flat", "equal"):
         rows = Rows(6, 3001, kind, seed=8, device="cuda")
