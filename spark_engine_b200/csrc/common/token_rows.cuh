@@ -126,7 +126,13 @@ struct Cluster {
   cg::cluster_group g;
   Mailboxes* mine;
   int phase = 0, rank, size;
-  __device__ __forceinline__ explicit Cluster(Mailboxes* m) : g(cg::this_cluster()), mine(m), rank(static_cast<int>(g.block_rank())), size(static_cast<int>(g.num_blocks())) {}
+  __device__ __forceinline__ explicit Cluster(Mailboxes* m) : g(cg::this_cluster()), mine(m), rank(static_cast<int>(g.block_rank())), size(static_cast<int>(g.num_blocks())) {
+    if (size > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  }
+  // Once, before anything is written to another CTA: all of them run.
+  __device__ __forceinline__ void ready() {
+    if (size > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+  }
 
   __device__ __forceinline__ void sync() {
     if (size > 1) g.sync();

@@ -9,10 +9,11 @@
 // What is kept is always a prefix of the order, given by its last token.
 //
 // A row is read once, by one CTA or, where there are few rows, by a cluster's; what stays of it in shared memory is the largest of every eight logits.
-// Their histogram's first bins with k tokens (or top_p of the weight) in them hold what is kept, since the other seven can only add to it; the groups that
-// reach into these bins are read again, and what of them lies there goes to a list, in which one CTA finds the prefix.  Where more are kept than the list
-// takes, the row is read again: the k-th token comes from a histogram of all, and for top_p a token is drawn first and the weight in front of it looked at
-// then: what lies in front of a token drawn in vain holds all that is kept, and half as much as before on average.
+// The largest that each thread has seen go to a histogram, whose first bins with k tokens (or top_p of the weight) in them hold what is kept, since all
+// others can only add to it; where they do not reach that far, the largest of every eight do.  The groups that come into these bins are read again,
+// and what of them lies there goes to a list, in which one CTA finds the prefix.  Where more are kept than the list takes, the row is read again: the k-th
+// token comes from a histogram of all, and for top_p a token is drawn first and the weight in front of it looked at then: what lies in front of a token
+// drawn in vain holds all that is kept, and half as much as before on average.
 #include "../common/token_rows.cuh"
 
 namespace spark {
@@ -55,23 +56,23 @@ __device__ __forceinline__ bool within(const Prefix& p, float z, int id) { retur
 constexpr float LOWEST = -3.402823466e38f;
 __device__ __forceinline__ float at_least(float z) { return fmaxf(z, LOWEST); }
 
-// Sum of 2^(z c) in units of 2^E, E whole: a change of units changes no bit.
-struct Mass { double s; float E; };
+// Sums of 2^(z c) in units of 2^E, E whole: a change of units changes no bit.  s: of all logits, g: of the largest of every eight.
+struct Mass { double s, g; float E; };
 __device__ __forceinline__ Mass add_mass(Mass a, Mass b) {
   const float E = fmaxf(a.E, b.E);
-  return {(a.s ? a.s * pow2(a.E - E) : 0) + (b.s ? b.s * pow2(b.E - E) : 0), E};
+  const double x = a.s ? pow2(a.E - E) : 0, y = b.s ? pow2(b.E - E) : 0;
+  return {a.s * x + b.s * y, a.g * x + b.g * y, E};
 }
-constexpr Mass NO_MASS{0.0, LOWEST};
+constexpr Mass NO_MASS{0.0, 0.0, LOWEST};
 
 struct RowShared {
   Mailboxes mail;
   unsigned hist[BINS];
   u64 list[LIST], weight[FEW], wsum[ROW_WARPS];
   double dsum[ROW_WARPS];
-  float E[16];
   unsigned n_list, before, kept;
   int bin;
-  float z, local_E;
+  float z;
   double log;
   Prefix cut;
   u64 total;
@@ -116,6 +117,25 @@ struct Row {
       for (int i = 0; i < 32; ++i) v[i] = one(place(chunk, i, lane));
     }
   }
+  // Eight values of a lane, from value 8 q of the chunk on.
+  __device__ __forceinline__ void load8(int chunk, int q, int lane, float (&v)[8]) const {
+    const int j0 = chunk * CHUNK;
+    if (j0 >= lo && j0 + CHUNK <= hi) {
+      uint4 w[8 / N];
+#pragma unroll
+      for (int i = 0; i < 8 / N; ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(base + j0 + (q * (8 / N) + i) * 32 * N) + lane);
+#pragma unroll
+      for (int i = 0; i < 8 / N; ++i) {
+        float f[N];
+        unpack_logits<T>(w[i], f);
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[i * N + e] = plain_logit(f[e]);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = one(place(chunk, 8 * q + e, lane));
+    }
+  }
   // f(32 logits, chunk) for each of a warp's chunks that `wanted(chunk's number in the CTA)`.
   template <class W, class F>
   __device__ __forceinline__ void stream(W wanted, F f) const {
@@ -143,6 +163,15 @@ struct Groups {
     } else {
       g[k * 32 + lane] = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
     }
+  }
+  // f(chunk's number, which eight of its lane's values) for a thread's own groups with a logit of `least` or more.
+  template <class F>
+  __device__ __forceinline__ void own(int chunks, float least, F f) const {
+    const int lane = threadIdx.x & 31, per = 4 >> shift;
+    for (int k = threadIdx.x >> 5; k < chunks; k += ROW_WARPS)
+      for (int q = 0; q < per; ++q)
+        if (g[(k * per + q) * 32 + lane] >= least)
+          for (int e = 0; e < 1 << shift; ++e) f(k, (q << shift) + e);
   }
   // Whether the chunk has a logit of `least` or more.
   __device__ __forceinline__ bool reaches(int k, float least) const {
@@ -192,28 +221,36 @@ struct Weights {
   }
 };
 
-// The first bin with which the bins of the cluster's CTAs hold `target` (tokens; or weight, in 2^16 of a bin's highest): the last one where they do not.
-// In units of 2^E; a CTA's bins are in units of its own.  Into sh.bin, with the tokens in front of it in sh.before.
-__device__ __forceinline__ void find_bin(RowShared& sh, Cluster& c, bool by_count, float E, double target) {
+__device__ __forceinline__ void clear_bins(RowShared& sh) {
+  for (int i = threadIdx.x; i < BINS; i += ROW_THREADS) sh.hist[i] = 0;
+}
+// A logit into its bin: as one, or as its weight in 2^-16 of the bin's highest (a little less at most).
+__device__ __forceinline__ void to_bin(RowShared& sh, const Weights& w, float z, bool by_count) {
+  const int bin = w.bin(z);
+  atomicAdd(&sh.hist[bin], by_count ? 1u : static_cast<unsigned>(fminf(exp2_fast(w.bits(z) + bin * (1.f / BINS_PER_BIT)) * 65536.f, 65536.f)));
+}
+// The first bin with which the bins (of the cluster's CTAs together, or this one's) hold `target`, tokens or weight: the last one where they do not.
+// Into sh.bin, with the tokens in front of it in sh.before.
+__device__ __forceinline__ void find_bin(RowShared& sh, Cluster& c, bool together, bool by_count, double target) {
   const int t = threadIdx.x, lane = t & 31, w = t >> 5;
   static_assert(BINS == 2 * ROW_THREADS, "two bins per thread");
   double v0 = 0, v1 = 0;
-  if (c.size == 1) {
+  if (!together || c.size == 1) {
     v0 = sh.hist[2 * t];
     v1 = sh.hist[2 * t + 1];
   } else {
-#pragma unroll 8
-    for (int r = 0; r < c.size; ++r) {
-      const float d = (E - sh.E[r]) * BINS_PER_BIT;            // (a multiple of 16)
-      const int b = 2 * t - (d < 2.f * BINS ? static_cast<int>(d) : 2 * BINS);
-      const uint2 n = b >= 0 ? *reinterpret_cast<const uint2*>(c.of(sh.hist, r) + b) : make_uint2(0, 0);
-      v0 += n.x;
-      v1 += n.y;
-    }
+    uint2 n[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+      if (r < c.size) n[r] = *reinterpret_cast<const uint2*>(c.of(sh.hist, r) + 2 * t);
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+      if (r < c.size) { v0 += n[r].x; v1 += n[r].y; }
   }
   if (!by_count) {
     v0 *= exp2f(t * (-2.f / BINS_PER_BIT));
     v1 *= exp2f((2 * t + 1) * (-1.f / BINS_PER_BIT));
+    target *= 65536.0;
   }
   double incl = v0 + v1;
 #pragma unroll
@@ -236,29 +273,45 @@ __device__ __forceinline__ void to_list(RowShared& sh, float z, int id) {
   if (at < LIST) sh.list[at] = list_key(z, id);
 }
 // The CTAs' lists behind the leader's own; how many they hold together, which everyone gets and which may be more than a list takes (nothing is moved then).
-__device__ __forceinline__ unsigned join_lists(RowShared& sh, Cluster& c) {
-  if (c.size == 1) {
-    __syncthreads();
-    return sh.n_list;
-  }
+// A CTA has a part of the leader's `inbox` to itself, so that entries and numbers travel together; only longer lists wait for the others' numbers.
+__device__ __forceinline__ unsigned join_lists(RowShared& sh, Cluster& c, u64* inbox) {
   __syncthreads();
   const unsigned mine = sh.n_list;
-  struct Place { unsigned n, before; };
-  if (threadIdx.x < c.size) c.of(&sh.mail.box[c.phase][c.rank], threadIdx.x)->w[0] = mine;
+  if (c.size == 1) return mine;
+  const unsigned part = LIST / c.size, t = threadIdx.x;
+  if (t < c.size) c.of(&sh.mail.box[c.phase][c.rank], t)->w[0] = mine;
+  if (c.rank && mine <= part) {
+    u64* to = c.of(inbox, 0) + c.rank * part;
+    for (unsigned i = t; i < mine; i += ROW_THREADS) to[i] = sh.list[i];
+  }
   c.sync();
-  unsigned n = 0, before = 0;
+  unsigned n = 0, before = 0, most = 0;
   for (int r = 0; r < c.size; ++r) {
     const unsigned m = static_cast<unsigned>(sh.mail.box[c.phase][r].w[0]);
     before += r < c.rank ? m : 0;
+    most = max(most, r ? m : 0);
     n += m;
   }
-  c.phase ^= 1;
-  if (n > LIST) return n;
-  if (c.rank) {
-    u64* to = c.of(sh.list, 0) + before;
-    for (unsigned i = threadIdx.x; i < mine; i += ROW_THREADS) to[i] = sh.list[i];
+  if (n <= LIST) {
+    if (most > part) {
+      if (c.rank && mine > part) {
+        u64* to = c.of(sh.list, 0) + before;
+        for (unsigned i = t; i < mine; i += ROW_THREADS) to[i] = sh.list[i];
+      }
+      c.sync();
+    }
+    if (c.rank == 0) {
+      unsigned at = mine;
+      for (int r = 1; r < c.size; ++r) {
+        const unsigned m = static_cast<unsigned>(sh.mail.box[c.phase][r].w[0]);
+        if (m <= part)
+          for (unsigned i = t; i < m; i += ROW_THREADS) sh.list[at + i] = inbox[r * part + i];
+        at += m;
+      }
+      __syncthreads();
+    }
   }
-  c.sync();
+  c.phase ^= 1;
   return n;
 }
 
@@ -321,11 +374,10 @@ __device__ __forceinline__ Win first_win(Win a, Win b) { return b.v > a.v || (b.
 // A token's score is known from below and above at the price of a few fp32 operations: `margin` is more than twice what the rough one may be off.
 // Where the two best are further apart than that, the best is the best; else both are computed as the definition says.
 struct Race {
-  float temp, c, margin;
+  float temp, c;
   u64 key;
   __device__ __forceinline__ Race(float T, float c_, long long seed, long long pos)
-      : temp(T), c(c_), margin(0), key((static_cast<u64>(seed) * 0x9E3779B97F4A7C15ull) ^ (static_cast<u64>(pos + 1) * 0xBF58476D1CE4E5B9ull)) {}
-  __device__ __forceinline__ void scale(float top) { margin = 1.f / 512 + (fabsf(top / temp) + 64.f) * (1.f / 524288); }
+      : temp(T), c(c_), key((static_cast<u64>(seed) * 0x9E3779B97F4A7C15ull) ^ (static_cast<u64>(pos + 1) * 0xBF58476D1CE4E5B9ull)) {}
   __device__ __forceinline__ u64 hash(int id) const { return mix64(static_cast<u64>(id) * 0x9E3779B97F4A7C15ull + key); }
   __device__ __forceinline__ float exact(float z, int id) const {
     const double u = (static_cast<double>(hash(id) >> 11) + 0.5) * (1.0 / 9007199254740992.0);
@@ -337,32 +389,47 @@ struct Race {
     const float L = q < 1.f / 256 ? q * (1.f + q * (0.5f + q * (1.f / 3))) : -__logf(q < 0.5f ? 1.f - q : (__ull2float_rn(h >> 11) + 0.5f) * (1.f / 9007199254740992.f));
     return __fdiv_rn(z, temp) - __logf(L);
   }
+  // (noise lies between -3.7 and 37.5: what comes near a score is z / T from not much further than that)
+  static __device__ __forceinline__ float margin(float score) { return 1.f / 512 + (fabsf(score) + 128.f) * (1.f / 524288); }
 };
 
 // A warp's race over the logits that come by.  -log u >= 1 - u, so that a score is at most z / T - log(1 - u): most tokens are out of it by the 32
 // upper bits of their hash, without a logarithm.
 struct Racer {
   Top2 m = NO_TOP;
-  float bound, off;
-  __device__ __forceinline__ void raise(const Race& race, float b) {
+  float bound = -INFINITY, off = 0.f;              // the best score so far, and what it takes to come near it
+  __device__ __forceinline__ void raise(float b) {
     bound = b;
-    off = (race.margin - bound) * 1.4426950408889634f + 32.f;
+    off = (Race::margin(b) - b) * 1.4426950408889634f + 32.f;
   }
+  // `mine`: the lane's largest logit.  The first chunk's 32 largest raise the bound before all others come.
   template <class T>
-  __device__ __forceinline__ void run(const Race& race, const Row<T>& row, const float (&v)[32], int chunk, const Prefix& kept) {
-    bool more = false;
+  __device__ __forceinline__ void run(const Race& race, const Row<T>& row, const float (&v)[32], float mine, int chunk, const Prefix& kept) {
     const int lane = threadIdx.x & 31;
+    if (bound == -INFINITY) {
+      int j = 0;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      const int id = row.id(Row<T>::place(chunk, i, lane));
-      if (!within(kept, v[i], id)) continue;
-      const u64 h = race.hash(id);
-      if (static_cast<float>(static_cast<uint32_t>(~h >> 32)) > exp2_fast(fmaf(v[i], race.c, off))) continue;
-      const float y = race.rough(v[i], h);
-      m = best2(m, Top2{y, id, -INFINITY, v[i]});
-      more |= y > bound;
+      for (int i = 31; i >= 0; --i)
+        if (v[i] == mine) j = Row<T>::place(chunk, i, lane);
+      const float b = warp_highest(within(kept, mine, row.id(j)) ? race.rough(mine, race.hash(row.id(j))) : -INFINITY);
+      if (b == -INFINITY) return;                  // (a lane without its largest logit has none)
+      raise(b);
     }
-    if (__any_sync(0xffffffffu, more)) raise(race, fmaxf(bound, warp_highest(m.a1)));
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      bool more = false;
+#pragma unroll
+      for (int i = 8 * g; i < 8 * g + 8; ++i) {
+        const int id = row.id(Row<T>::place(chunk, i, lane));
+        if (!within(kept, v[i], id)) continue;
+        const u64 h = race.hash(id);
+        if (static_cast<float>(static_cast<uint32_t>(~h >> 32)) > exp2_fast(fmaf(v[i], race.c, off))) continue;
+        const float y = race.rough(v[i], h);
+        m = best2(m, Top2{y, id, -INFINITY, v[i]});
+        more |= y > bound;
+      }
+      if (__any_sync(0xffffffffu, more)) raise(fmaxf(bound, warp_highest(m.a1)));
+    }
   }
 };
 
@@ -370,7 +437,7 @@ struct Racer {
 template <class T, class W>
 __device__ __forceinline__ Win settle(const Row<T>& row, Cluster& c, const Race& race, const Prefix& kept, Top2 m, W wanted) {
   m = c.reduce(m, NO_TOP, best2);
-  if (m.a2 < m.a1 - race.margin) return Win{m.a1, m.id, m.z, 0};
+  if (m.a2 < m.a1 - Race::margin(m.a1)) return Win{m.a1, m.id, m.z, 0};
   Win b{-INFINITY, NO_ID, -INFINITY, 0};
   const Win none = b;
   row.stream(wanted, [&](const float (&v)[32], int k) {
@@ -378,7 +445,7 @@ __device__ __forceinline__ Win settle(const Row<T>& row, Cluster& c, const Race&
     for (int i = 0; i < 32; ++i) {
       const int j = Row<T>::place(row.chunk0 + k, i, threadIdx.x & 31), id = row.id(j);
       const float z = row.one(j);
-      if (!within(kept, z, id) || race.rough(z, race.hash(id)) < m.a1 - race.margin) continue;
+      if (!within(kept, z, id) || race.rough(z, race.hash(id)) < m.a1 - Race::margin(m.a1)) continue;
       b = first_win(b, Win{race.exact(z, id), id, z, 0});
     }
   });
@@ -389,7 +456,7 @@ __device__ __forceinline__ Win settle(const Row<T>& row, Cluster& c, const Race&
 __device__ __forceinline__ int draw_few(RowShared& sh, Cluster& c, const Race& race, u64 key, bool in) {
   Top2 m = in ? Top2{race.rough(list_z(key), race.hash(list_id(key))), list_id(key), -INFINITY, 0} : NO_TOP;
   m = c.block(m, NO_TOP, best2);
-  if (threadIdx.x == 0) sh.kept = m.a2 < m.a1 - race.margin;
+  if (threadIdx.x == 0) sh.kept = m.a2 < m.a1 - Race::margin(m.a1);
   __syncthreads();
   if (sh.kept) return m.id;
   Best b = in ? Best{race.exact(list_z(key), list_id(key)), list_id(key)} : Best{-INFINITY, NO_ID};
@@ -403,7 +470,7 @@ __device__ __forceinline__ int draw_list(RowShared& sh, Cluster& c, const Race& 
     m = best2(m, Top2{race.rough(list_z(k), race.hash(list_id(k))), list_id(k), -INFINITY, 0});
   }
   m = c.block(m, NO_TOP, best2);
-  if (threadIdx.x == 0) sh.kept = m.a2 < m.a1 - race.margin;
+  if (threadIdx.x == 0) sh.kept = m.a2 < m.a1 - Race::margin(m.a1);
   __syncthreads();
   if (sh.kept) return m.id;
   Best b{-INFINITY, NO_ID};
@@ -447,11 +514,10 @@ __device__ __noinline__ Prefix kth_by_bits(const Row<T>& row, Cluster& c, const 
 
 // The prefix of the first k tokens of `of` = (least logit, any id).
 template <class T>
-__device__ __forceinline__ Prefix kth_token(RowShared& sh, const Row<T>& row, const Groups& groups, Cluster& c, const Weights& w, const Prefix& of, unsigned k) {
+__device__ __forceinline__ Prefix kth_token(RowShared& sh, const Row<T>& row, const Groups& groups, Cluster& c, const Weights& w, const Prefix& of, unsigned k, u64* inbox) {
   c.sync();                                        // (nobody reads the bins and lists of before any more)
-  for (int i = threadIdx.x; i < BINS; i += ROW_THREADS) sh.hist[i] = 0;
+  clear_bins(sh);
   if (threadIdx.x == 0) sh.n_list = 0;
-  if (threadIdx.x < 16) sh.E[threadIdx.x] = w.E;
   __syncthreads();
   row.stream([&](int i) { return groups.reaches(i, of.z); }, [&](const float (&v)[32], int) {
 #pragma unroll
@@ -459,7 +525,7 @@ __device__ __forceinline__ Prefix kth_token(RowShared& sh, const Row<T>& row, co
       if (v[i] >= of.z) atomicAdd(&sh.hist[w.bin(v[i])], 1u);
   });
   c.sync();
-  find_bin(sh, c, true, w.E, k);
+  find_bin(sh, c, true, true, k);
   const int bin = sh.bin;
   const unsigned before = sh.before;               // (0 with the last bin where the row has fewer than k tokens)
   row.stream([&](int i) { return groups.reaches(i, fmaxf(of.z, w.edge(bin))); }, [&](const float (&v)[32], int n) {
@@ -467,7 +533,7 @@ __device__ __forceinline__ Prefix kth_token(RowShared& sh, const Row<T>& row, co
     for (int i = 0; i < 32; ++i)
       if (v[i] >= of.z && w.bin(v[i]) == bin) to_list(sh, v[i], row.id(Row<T>::place(row.chunk0 + n, i, threadIdx.x & 31)));
   });
-  const unsigned n = join_lists(sh, c);
+  const unsigned n = join_lists(sh, c, inbox);
   if (n > LIST) return kth_by_bits(row, c, of, k);
   if (c.rank == 0) {
     sort_list(sh, n);
@@ -481,13 +547,53 @@ __device__ __forceinline__ Prefix kth_token(RowShared& sh, const Row<T>& row, co
 
 // ------------------------------------------------------------------------------------------------ kernels
 
-__device__ __forceinline__ Groups groups_at(float* smem, int chunks_per_cta) {
-  const int n = chunks_per_cta * 128;
-  return Groups{smem, n <= 20480 ? 0 : n <= 40960 ? 1 : 2};
+// Behind a CTA's groups: of a cluster, the largest logits of all its threads, and the leader's inbox.
+constexpr int CLUSTER_MAX = 8;
+struct Parts {
+  Groups groups;
+  float* maxima;
+  u64* inbox;
+};
+__host__ __device__ __forceinline__ int group_shift(int per) { return per <= 160 ? 0 : per <= 320 ? 1 : 2; }
+__device__ __forceinline__ Parts parts_of(float* smem, int per, int size) {
+  const int shift = group_shift(per);
+  float* maxima = smem + per * (128 >> shift);
+  return Parts{Groups{smem, shift}, maxima, reinterpret_cast<u64*>(maxima + size * ROW_THREADS)};
 }
-static int group_bytes(int chunks_per_cta) {
-  const int n = chunks_per_cta * 128;
-  return 4 * (n <= 20480 ? n : n <= 40960 ? n / 2 : n / 4);
+static int part_bytes(int per, int size) { return per * (128 >> group_shift(per)) * 4 + (size > 1 ? size * ROW_THREADS * 4 + LIST * 8 : 0); }
+
+// The bins below which the row's first tokens lie, from the largest logit of every thread.
+template <class T>
+__device__ __forceinline__ void bins_of_threads(RowShared& sh, Cluster& c, const float* maxima, float mine, const Weights& w, float least, bool by_count, double target) {
+  for (int r = 0; r < c.size; ++r) {
+    const float z = c.size > 1 ? maxima[r * ROW_THREADS + threadIdx.x] : mine;
+    if (z >= least) to_bin(sh, w, z, by_count);
+  }
+  __syncthreads();
+  find_bin(sh, c, false, by_count, target);
+}
+// The same from the groups' (the bins are of no use any more).
+__device__ __forceinline__ void bins_of_groups(RowShared& sh, Cluster& c, const Groups& groups, int chunks, const Weights& w, float least, bool by_count, double target) {
+  clear_bins(sh);
+  __syncthreads();
+  for (int i = threadIdx.x; i < chunks * (128 >> groups.shift); i += ROW_THREADS)
+    if (groups.g[i] >= least) to_bin(sh, w, groups.g[i], by_count);
+  c.sync();
+  find_bin(sh, c, true, by_count, target);
+}
+// What lies at `least` and above, in the leader's list.
+template <class T>
+__device__ __forceinline__ unsigned gather(RowShared& sh, Cluster& c, const Row<T>& row, const Parts& parts, float mine, float least) {
+  if (mine >= least)
+    parts.groups.own(row.chunks, least, [&](int k, int q) {
+      const int chunk = row.chunk0 + k, lane = threadIdx.x & 31;
+      float v[8];
+      row.load8(chunk, q, lane, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (v[e] >= least) to_list(sh, v[e], row.id(Row<T>::place(chunk, 8 * q + e, lane)));
+    });
+  return join_lists(sh, c, parts.inbox);
 }
 
 // The smallest logit that is not too improbable, decided in 64 bits.
@@ -505,54 +611,69 @@ __global__ void __launch_bounds__(ROW_THREADS, 2)
 sample_kernel(const __grid_constant__ SampleRows a, int per) {
   extern __shared__ __align__(16) float smem[];
   __shared__ RowShared sh;
+  pdl_wait();
+  pdl_trigger();
   Cluster c(&sh.mail);
   const int t = threadIdx.x, r = blockIdx.x / c.size;
   const float temp = a.temps[r], mp = a.min_p ? a.min_p[r] : 0.f, p = a.top_p ? a.top_p[r] : 1.f;
   const int asked = a.top_k ? a.top_k[r] : 0, k = asked < a.V ? asked : 0;
   const Row<T> row(static_cast<const T*>(a.x) + r * a.ldx, a.V, c.rank, per);
-  const Groups groups = groups_at(smem, per);
+  const Parts parts = parts_of(smem, per, c.size);
+  const Groups& groups = parts.groups;
   const bool greedy = !(temp > 0.f) || k == 1 || p <= 0.f || mp > 1.f, by_p = p < 1.f, by_k = k > 0, by_min = mp > 0.f && isfinite(temp);
   const bool all = !greedy && !by_p && !by_k && !by_min;
   // (products of it with 0 and infinity are 0 and infinity)
   const float scale = greedy ? 0.f : fmaxf(fminf(__fdiv_rn(1.4426950408889634f, temp), -LOWEST), 1e-44f);
   const bool sums = !greedy && by_p && !by_k && !by_min;
-  Race race(temp, scale, a.seeds[r], a.positions[r]);
-  for (int i = t; i < BINS; i += ROW_THREADS) sh.hist[i] = 0;
+  const Race race(temp, scale, a.seeds[r], a.positions[r]);
+  const Prefix whole_row{LOWEST, NO_ID};
+  clear_bins(sh);
   if (t == 0) sh.n_list = 0;
   const auto every = [](int) { return true; };
 
   Best top{-INFINITY, NO_ID};
   Mass mass = NO_MASS;
-  row.stream(every, [&](const float (&v)[32], int i) {
-    float m[4];
+  Racer racer;
+  float largest = -INFINITY;                       // of the thread
+  const auto look = [&](const float (&v)[32], float (&m)[4], int i, float& mine) {
     max8(v, m);
-    const float mine = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), highest = warp_highest(mine);
+    mine = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+    const float highest = warp_highest(mine);
     note_best(row, v, mine, highest, row.chunk0 + i, top);
-    if (!greedy && !all) groups.put(m, i);
-    if (sums && highest > -INFINITY) {             // the chunk's weight in units of its own: the same in every batch
-      const float E = ceilf(highest * scale);
-      float s = 0.f;
+    largest = fmaxf(largest, mine);
+    return highest;
+  };
+  if (all) {
+    row.stream(every, [&](const float (&v)[32], int i) {
+      float m[4], mine;
+      const float highest = look(v, m, i, mine);
+      if (highest > -INFINITY && highest < INFINITY) racer.run(race, row, v, mine, row.chunk0 + i, whole_row);
+    });
+  } else if (sums) {
+    row.stream(every, [&](const float (&v)[32], int i) {
+      float m[4], mine;
+      const float highest = look(v, m, i, mine);
+      groups.put(m, i);
+      if (!(highest > -INFINITY)) return;
+      const float E = ceilf(highest * scale);      // the chunk's weight in units of its own: the same in every batch
+      float s = 0.f, g = 0.f;
 #pragma unroll
       for (int q = 0; q < 32; q += 4)
         s += (exp2_fast(fmaf(v[q], scale, -E)) + exp2_fast(fmaf(v[q + 1], scale, -E))) + (exp2_fast(fmaf(v[q + 2], scale, -E)) + exp2_fast(fmaf(v[q + 3], scale, -E)));
-      mass = add_mass(mass, Mass{s, E});
-    }
-  });
-  if (!greedy && !all && !(by_min && !by_k && !by_p)) {        // the largest of every eight in bins, below the CTA's own best
-    const Best own = c.block(top, Best{-INFINITY, NO_ID}, first_of);
-    if (t == 0) sh.local_E = own.v > -INFINITY ? ceilf(own.v * scale) : LOWEST;
-    __syncthreads();
-    const Weights w{scale, sh.local_E, 0.f};
-    for (int i = t; i < row.chunks * (128 >> groups.shift); i += ROW_THREADS) {
-      const float m = groups.g[i];
-      if (!(m > -INFINITY)) continue;
-      const int bin = w.bin(m);
-      if (by_k) atomicAdd(&sh.hist[bin], 1u);
-      else atomicAdd(&sh.hist[bin], static_cast<unsigned>(fminf(exp2_fast(w.bits(m) + bin * (1.f / BINS_PER_BIT)) * 65536.f, 65536.f)));
-    }
-    if (t < c.size) (c.size > 1 ? c.of(&sh, t) : &sh)->E[c.rank] = w.E;
-    __syncthreads();
+#pragma unroll
+      for (int q = 0; q < 4; ++q) g += exp2_fast(fmaf(m[q], scale, -E));
+      mass = add_mass(mass, Mass{s, g, E});
+    });
+  } else {
+    row.stream(every, [&](const float (&v)[32], int i) {
+      float m[4], mine;
+      look(v, m, i, mine);
+      if (!greedy) groups.put(m, i);
+    });
   }
+  c.ready();
+  if (c.size > 1 && !greedy && !all)
+    for (int i = 0; i < c.size; ++i) c.of(parts.maxima, i)[c.rank * ROW_THREADS + t] = largest;
   struct First { Best top; Mass mass; };
   const First first = c.reduce(First{top, mass}, First{{-INFINITY, NO_ID}, NO_MASS}, [](First x, First y) { return First{first_of(x.top, y.top), add_mass(x.mass, y.mass)}; });
   top = first.top;
@@ -563,10 +684,9 @@ sample_kernel(const __grid_constant__ SampleRows a, int per) {
     c.sync();                                      // (what a CTA's shared memory holds stays until all have read it)
     return;
   }
-  race.scale(top.v);
   const bool far = !(fabsf(top.v * scale) < 1048576.f);
   const Weights weight = far ? Weights{scale, 0.f, top.v} : Weights{scale, ceilf(top.v * scale), 0.f};
-  Prefix kept{LOWEST, NO_ID};
+  Prefix kept = whole_row;
   if (by_min) {
     if (t == 0) sh.z = min_p_logit(top.v, temp, mp);
     __syncthreads();
@@ -588,20 +708,12 @@ sample_kernel(const __grid_constant__ SampleRows a, int per) {
   if (by_k || by_p) {
     unsigned n = LIST + 1;
     if (k <= LIST && !far) {
-      find_bin(sh, c, by_k, weight.E, by_k ? k : p * total * 65536.0 * (1 + 1.0 / 262144));
-      const float least = fmaxf(kept.z, weight.edge(sh.bin));
-      if (sh.bin < BINS - 1 || a.V <= LIST) {
-        for (int i = t; i < row.chunks * (128 >> groups.shift); i += ROW_THREADS) {
-          if (!(groups.g[i] >= least)) continue;
-          const int g = i >> 5, chunk = row.chunk0 + (g >> (2 - groups.shift)), q = (g & ((4 >> groups.shift) - 1)) * (8 << groups.shift);
-          for (int e = 0; e < 8 << groups.shift; ++e) {
-            const int j = Row<T>::place(chunk, q + e, i & 31);
-            const float z = row.one(j);
-            if (z >= least) to_list(sh, z, row.id(j));
-          }
-        }
-        n = join_lists(sh, c);
-      }
+      const double need = by_k ? k : p * total * (1 + 1.0 / 262144);
+      bins_of_threads<T>(sh, c, parts.maxima, largest, weight, kept.z, by_k, need);
+      // (the groups' largest may have the weight that the threads' have not, and they are more than these)
+      if (sh.bin == BINS - 1 && (by_k || by_min || first.mass.g * pow2(first.mass.E - weight.E) >= need))
+        bins_of_groups(sh, c, groups, row.chunks, weight, kept.z, by_k, need);
+      if (sh.bin < BINS - 1 || a.V <= LIST) n = gather(sh, c, row, parts, largest, fmaxf(kept.z, weight.edge(sh.bin)));
     }
     if (n <= LIST) {
       if (c.rank) return;
@@ -673,29 +785,29 @@ sample_kernel(const __grid_constant__ SampleRows a, int per) {
       return;
     }
     if (by_k) {
-      kept = kth_token(sh, row, groups, c, weight, kept, k);
+      kept = kth_token(sh, row, groups, c, weight, kept, k, parts.inbox);
       if (by_p) total = mass_of(kept);
     }
   }
-  // The best token is always kept.
-  const float start = race.rough(top.v, race.hash(top.id));
-  Racer racer;
-  racer.raise(race, start);
-  row.stream(some, [&](const float (&v)[32], int i) { racer.run(race, row, v, row.chunk0 + i, kept); });
+  const auto largest_of = [](const float (&v)[32]) {
+    float m[4];
+    max8(v, m);
+    return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+  };
+  if (!all) row.stream(some, [&](const float (&v)[32], int i) { racer.run(race, row, v, largest_of(v), row.chunk0 + i, kept); });
   Win win = settle(row, c, race, kept, racer.m, some);
   const double target = by_p ? p * total : 0;
   while (by_p && win.id != top.id) {               // what lies in front of it, and who wins there should that be too much
     const Prefix front{win.z, win.id - 1};
     const auto there = [&](int i) { return groups.reaches(i, front.z); };
     Racer next;
-    next.raise(race, start);
     double s = 0;
     row.stream(there, [&](const float (&v)[32], int i) {
       float f = 0.f;
 #pragma unroll
       for (int q = 0; q < 32; ++q) f += within(front, v[q], row.id(Row<T>::place(row.chunk0 + i, q, t & 31))) ? weight(v[q]) : 0.f;
       s += f;
-      next.run(race, row, v, row.chunk0 + i, front);
+      next.run(race, row, v, largest_of(v), row.chunk0 + i, front);
     });
     if (c.reduce(s, 0.0, [](double x, double y) { return x + y; }) < target) break;
     win = settle(row, c, race, front, next.m, there);
@@ -709,6 +821,8 @@ __global__ void __launch_bounds__(ROW_THREADS, 2)
 logprob_kernel(const __grid_constant__ LogprobRows a, int per) {
   extern __shared__ __align__(16) float smem[];
   __shared__ RowShared sh;
+  pdl_wait();
+  pdl_trigger();
   Cluster c(&sh.mail);
   const int tid = threadIdx.x, r = blockIdx.x / c.size;
   const T* x = static_cast<const T*>(a.x) + r * a.ldx;
@@ -716,9 +830,10 @@ logprob_kernel(const __grid_constant__ LogprobRows a, int per) {
   const bool there = t >= 0 && t < a.V;
   const float zt = there ? plain_logit(logit(x + t)) : -INFINITY;
   const Row<T> row(x, a.V, c.rank, per);
-  const Groups groups = groups_at(smem, per);
-  if (a.top > 1) {
-    for (int i = tid; i < BINS; i += ROW_THREADS) sh.hist[i] = 0;
+  const Parts parts = parts_of(smem, per, c.size);
+  const bool listing = a.top > 1;
+  if (listing) {
+    clear_bins(sh);
     if (tid == 0) sh.n_list = 0;
   }
   // log2(e) in two parts: z log2(e) - E as exact as its own size in fp32
@@ -726,6 +841,7 @@ logprob_kernel(const __grid_constant__ LogprobRows a, int per) {
   Best top{-INFINITY, NO_ID};
   Mass mass = NO_MASS;
   unsigned before = 0;
+  float largest = -INFINITY;                       // of the thread
   const int tj = t + row.lo;
   row.stream([](int) { return true; }, [&](const float (&v)[32], int i) {
     const int chunk = row.chunk0 + i;
@@ -733,7 +849,8 @@ logprob_kernel(const __grid_constant__ LogprobRows a, int per) {
     max8(v, m);
     const float mine = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), highest = warp_highest(mine);
     note_best(row, v, mine, highest, chunk, top);
-    if (a.top > 1) groups.put(m, i);
+    largest = fmaxf(largest, mine);
+    if (listing) parts.groups.put(m, i);
     if (highest > -INFINITY && highest < INFINITY) {           // the chunk's sum in units of its own: the same in every batch
       const float E = ceilf(highest * HI);
       float s = 0.f;
@@ -744,7 +861,7 @@ logprob_kernel(const __grid_constant__ LogprobRows a, int per) {
         for (int e = 0; e < 4; ++e) w[e] = exp2_fast(fmaf(v[q + e], LO, fmaf(v[q + e], HI, -E)));
         s += (w[0] + w[1]) + (w[2] + w[3]);
       }
-      mass = add_mass(mass, Mass{s, E});
+      mass = add_mass(mass, Mass{s, 0.0, E});
     }
     if (zt == -INFINITY || (chunk * CHUNK <= tj && tj < (chunk + 1) * CHUNK)) {
 #pragma unroll
@@ -758,25 +875,20 @@ logprob_kernel(const __grid_constant__ LogprobRows a, int per) {
       for (int q = 0; q < 32; ++q) before += v[q] >= least;
     }
   });
-  const bool listing = a.top > 1;
-  if (listing) {
-    const Best own = c.block(top, Best{-INFINITY, NO_ID}, first_of);
-    if (tid == 0) sh.local_E = own.v > -INFINITY ? ceilf(own.v * HI) : LOWEST;
-    __syncthreads();
-    const Weights w{HI, sh.local_E, 0.f};
-    for (int i = tid; i < row.chunks * (128 >> groups.shift); i += ROW_THREADS)
-      if (groups.g[i] > -INFINITY) atomicAdd(&sh.hist[w.bin(groups.g[i])], 1u);
-    if (tid < c.size) (c.size > 1 ? c.of(&sh, tid) : &sh)->E[c.rank] = w.E;
-    __syncthreads();
-  }
-  struct First { Best top; Mass mass; u64 before; };
-  const First first = c.reduce(First{top, mass, before}, First{{-INFINITY, NO_ID}, NO_MASS, 0},
-                               [](First p, First q) { return First{first_of(p.top, q.top), add_mass(p.mass, q.mass), p.before + q.before}; });
+  c.ready();
+  if (c.size > 1 && listing)
+    for (int i = 0; i < c.size; ++i) c.of(parts.maxima, i)[c.rank * ROW_THREADS + tid] = largest;
+  struct Sum { double s; float E; unsigned before; };
+  struct First { Best top; Sum sum; };
+  const First first = c.reduce(First{top, {mass.s, mass.E, before}}, First{{-INFINITY, NO_ID}, {0.0, LOWEST, 0}}, [](First p, First q) {
+    const Mass m = add_mass(Mass{p.sum.s, 0.0, p.sum.E}, Mass{q.sum.s, 0.0, q.sum.E});
+    return First{first_of(p.top, q.top), {m.s, m.E, p.sum.before + q.sum.before}};
+  });
   top = first.top;
   const bool lead = c.rank == 0 && tid == 0;
   // log-probabilities: z - (E log 2 + log(sum)); seen from the best where logits are so large that this would leave too few bits of it, or infinite
   const bool far = !(fabsf(top.v) < 1e6f);
-  double sum = first.mass.s;
+  double sum = first.sum.s;
   if (far) {
     sum = 0;
     row.stream([](int) { return true; }, [&](const float (&v)[32], int) {
@@ -787,7 +899,7 @@ logprob_kernel(const __grid_constant__ LogprobRows a, int per) {
     });
     sum = c.reduce(sum, 0.0, [](double p, double q) { return p + q; });
   }
-  if (lead) sh.log = (far ? 0.0 : static_cast<double>(first.mass.E) * 0.69314718055994530942) + log(sum);
+  if (lead) sh.log = (far ? 0.0 : static_cast<double>(first.sum.E) * 0.69314718055994530942) + log(sum);
   const auto lp = [&](float z) {
     if (z == -INFINITY) return -INFINITY;
     return static_cast<float>((far ? (z == top.v ? 0.0 : static_cast<double>(z) - top.v) : static_cast<double>(z)) - sh.log);
@@ -796,7 +908,7 @@ logprob_kernel(const __grid_constant__ LogprobRows a, int per) {
   float* lps = a.logprobs + static_cast<long long>(r) * a.top;
   if (lead) {
     a.logprob[r] = lp(zt);
-    a.rank[r] = there ? static_cast<int>(first.before) + 1 : 0;
+    a.rank[r] = there ? static_cast<int>(first.sum.before) + 1 : 0;
     if (a.top == 1) {
       ids[0] = top.v == -INFINITY ? -1 : top.id;
       lps[0] = lp(top.v);
@@ -805,21 +917,10 @@ logprob_kernel(const __grid_constant__ LogprobRows a, int per) {
   if (a.top < 2) { c.sync(); return; }
   if (!far) {
     const Weights w{HI, ceilf(top.v * HI), 0.f};
-    find_bin(sh, c, true, w.E, a.top);
+    bins_of_threads<T>(sh, c, parts.maxima, largest, w, LOWEST, true, a.top);
+    if (sh.bin == BINS - 1) bins_of_groups(sh, c, parts.groups, row.chunks, w, LOWEST, true, a.top);
     unsigned n = LIST + 1;
-    if (sh.bin < BINS - 1 || a.V <= LIST) {
-      const float least = w.edge(sh.bin);
-      for (int i = tid; i < row.chunks * (128 >> groups.shift); i += ROW_THREADS) {
-        if (!(groups.g[i] >= least)) continue;
-        const int g = i >> 5, chunk = row.chunk0 + (g >> (2 - groups.shift)), q = (g & ((4 >> groups.shift) - 1)) * (8 << groups.shift);
-        for (int e = 0; e < 8 << groups.shift; ++e) {
-          const int j = Row<T>::place(chunk, q + e, i & 31);
-          const float z = row.one(j);
-          if (z >= least) to_list(sh, z, row.id(j));
-        }
-      }
-      n = join_lists(sh, c);
-    }
+    if (sh.bin < BINS - 1 || a.V <= LIST) n = gather(sh, c, row, parts, largest, w.edge(sh.bin));
     if (n <= LIST) {
       if (c.rank) return;
       const auto put = [&](unsigned i, u64 key) { ids[i] = list_id(key); lps[i] = lp(list_z(key)); };
@@ -856,22 +957,15 @@ logprob_kernel(const __grid_constant__ LogprobRows a, int per) {
 // CTAs of a row's cluster: as many as there is room for, of four chunks each at least.
 static int row_cluster(int R, int chunks, int sms) {
   int c = 1;
-  while (c < 16 && R * c * 2 <= 2 * sms && c * 4 < chunks) c *= 2;
+  while (c < CLUSTER_MAX && R * c * 2 <= 2 * sms && c * 4 < chunks) c *= 2;
   return c;
 }
 
 template <class A, class K>
 static int launch_rows(const char* name, K kern, const A& a, cudaStream_t s) {
-  const int chunks = (a.V + 8 + CHUNK - 1) / CHUNK, c = row_cluster(a.R, chunks, a.sms), per = (chunks + c - 1) / c, bytes = group_bytes(per);
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess ||
-      cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return spark_launch_rc(name);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(a.R * c); cfg.blockDim = dim3(ROW_THREADS); cfg.dynamicSmemBytes = bytes; cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = c; attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr; cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, kern, a, per) != cudaSuccess) return spark_launch_rc(name);
+  const int chunks = (a.V + 8 + CHUNK - 1) / CHUNK, c = row_cluster(a.R, chunks, a.sms), per = (chunks + c - 1) / c, bytes = part_bytes(per, c);
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return spark_launch_rc(name);
+  spark_launch_pdl(kern, dim3(a.R * c), dim3(ROW_THREADS), bytes, s, dim3(c, 1, 1), a, per);
   return spark_launch_rc(name);
 }
 
