@@ -116,11 +116,20 @@ __device__ __forceinline__ V shfl_words(V v, int o) {
   return b.v;
 }
 
+template <class V>
+__device__ __forceinline__ V bcast_words(V v) {    // lane 0's
+  union { V v; int w[sizeof(V) / 4]; } a, b;
+  a.v = v;
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(V) / 4); ++i) b.w[i] = __shfl_sync(0xffffffffu, a.w[i], 0);
+  return b.v;
+}
+
 // Values of a row's cluster.  A CTA writes its value to every CTA's boxes and all meet at a barrier: what is read then is near.  Two sets in turn, so that
 // one barrier per reduction is enough.
 struct alignas(16) Mail { unsigned long long w[4]; };
 struct Mailboxes {
-  Mail box[2][16], warp[32];
+  Mail box[2][8], warp[16];
 };
 struct Cluster {
   cg::cluster_group g;
@@ -133,14 +142,23 @@ struct Cluster {
   __device__ __forceinline__ void ready() {
     if (size > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
   }
-
   __device__ __forceinline__ void sync() {
     if (size > 1) g.sync();
     else __syncthreads();
   }
   template <class V>
-  __device__ __forceinline__ V* of(V* p, int r) { return g.map_shared_rank(p, r); }
+  __device__ __forceinline__ V* of(V* p, int r) { return size > 1 ? g.map_shared_rank(p, r) : p; }
 
+  // Warp 0's value, which every CTA finds at its rank in `box` afterwards.
+  template <class V>
+  __device__ __forceinline__ const Mail* tell(V v) {
+    static_assert(sizeof(V) <= sizeof(Mail), "mailboxes");
+    if (threadIdx.x < size) *reinterpret_cast<V*>(of(&mine->box[phase][rank], threadIdx.x)) = v;
+    sync();
+    const Mail* b = mine->box[phase];
+    phase ^= 1;
+    return b;
+  }
   // op over the block's threads; warp 0 gets it.
   template <class V, class Op>
   __device__ __forceinline__ V block(V v, V none, Op op) {
@@ -153,20 +171,16 @@ struct Cluster {
     if (w == 0) {
       v = lane < nw ? *reinterpret_cast<V*>(&mine->warp[lane]) : none;
 #pragma unroll
-      for (int o = 16; o; o >>= 1) v = op(v, shfl_words(v, o));
+      for (int o = 8; o; o >>= 1) v = op(v, shfl_words(v, o));     // (at most 16 warps)
     }
     return v;
   }
   // op over all threads of the cluster, in an order that is the same in every run; every thread gets it.
   template <class V, class Op>
   __device__ __forceinline__ V reduce(V v, V none, Op op) {
-    v = block(v, none, op);
-    const int lane = threadIdx.x & 31;
-    if (threadIdx.x < size) *reinterpret_cast<V*>(size > 1 ? of(&mine->box[phase][rank], lane) : &mine->box[phase][0]) = v;
-    sync();
-    v = *reinterpret_cast<V*>(&mine->box[phase][0]);
-    for (int r = 1; r < size; ++r) v = op(v, *reinterpret_cast<V*>(&mine->box[phase][r]));
-    phase ^= 1;
+    const Mail* b = tell(bcast_words(block(v, none, op)));
+    v = *reinterpret_cast<const V*>(b);
+    for (int r = 1; r < size; ++r) v = op(v, *reinterpret_cast<const V*>(b + r));
     return v;
   }
 };

@@ -18,12 +18,12 @@
 
 namespace spark {
 
-constexpr int ROW_THREADS = 512, ROW_WARPS = ROW_THREADS / 32;
 constexpr int CHUNK = 1024;                        // logits that a warp takes at once, 32 per lane
 constexpr int BINS = 1024;                         // of a sixteenth of a bit of weight; what weighs less than 2^-64 shares the last one
 constexpr float BINS_PER_BIT = 16.f;
 constexpr int LIST = 2048;
-constexpr int FEW = 256;                           // of the list: ordered by counting
+constexpr int HITS = 512;
+constexpr int CLUSTER_MAX = 8;
 
 using u64 = unsigned long long;
 
@@ -46,6 +46,11 @@ __device__ __forceinline__ float warp_highest(float v) {
   const int m = __reduce_max_sync(0xffffffffu, b ^ (b >> 31 & 0x7fffffff));
   return __int_as_float(m ^ (m >> 31 & 0x7fffffff));
 }
+__device__ __forceinline__ double warp_total(double v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
 __device__ __forceinline__ double pow2(float n) {  // 2^n for a whole n <= 0
   return n < -1022.f ? 0.0 : __hiloint2double((1023 + static_cast<int>(n)) << 20, 0);
 }
@@ -54,23 +59,16 @@ __device__ __forceinline__ double pow2(float n) {  // 2^n for a whole n <= 0
 struct Prefix { float z; int id; };
 __device__ __forceinline__ bool within(const Prefix& p, float z, int id) { return z > p.z || (z == p.z && id <= p.id); }
 constexpr float LOWEST = -3.402823466e38f;
+__device__ __forceinline__ Prefix whole_row() { return Prefix{LOWEST, NO_ID}; }
 __device__ __forceinline__ float at_least(float z) { return fmaxf(z, LOWEST); }
 
-// Sums of 2^(z c) in units of 2^E, E whole: a change of units changes no bit.  s: of all logits, g: of the largest of every eight.
-struct Mass { double s, g; float E; };
-__device__ __forceinline__ Mass add_mass(Mass a, Mass b) {
-  const float E = fmaxf(a.E, b.E);
-  const double x = a.s ? pow2(a.E - E) : 0, y = b.s ? pow2(b.E - E) : 0;
-  return {a.s * x + b.s * y, a.g * x + b.g * y, E};
-}
-constexpr Mass NO_MASS{0.0, 0.0, LOWEST};
-
+template <int NT>
 struct RowShared {
   Mailboxes mail;
-  unsigned hist[BINS];
-  u64 list[LIST], weight[FEW], wsum[ROW_WARPS];
-  double dsum[ROW_WARPS];
-  unsigned n_list, before, kept;
+  unsigned hist[BINS], hits[HITS];
+  u64 list[LIST], weight[NT / 2], wsum[NT / 32];
+  float fsum[NT / 32];
+  unsigned n_list, n_hits, before, kept;
   int bin;
   float z;
   double log;
@@ -80,11 +78,24 @@ struct RowShared {
 
 // ------------------------------------------------------------------------------------------------ a CTA's part of a row
 
-// Places j of a row from a 16-byte boundary on: id j + first at it; those in [lo, hi) are the row's.  Lane l of a warp has N = 16 bytes' logits of every
-// 32 * N: value i of its 32 in chunk k is place k * CHUNK + (i / N) * 32 N + l * N + i % N.
+template <class T> __device__ __forceinline__ T no_logit();
+template <> __device__ __forceinline__ float no_logit<float>() { return -INFINITY; }
+template <> __device__ __forceinline__ __nv_bfloat16 no_logit<__nv_bfloat16>() { return __ushort_as_bfloat16(0xff80); }
+template <> __device__ __forceinline__ __half no_logit<__half>() { return __ushort_as_half(0xfc00); }
+
+// 16 bytes at the row's ends: -inf where they are not the row's.
 template <class T>
+__device__ __noinline__ uint4 edge_vector(const T* base, int j, int lo, int hi) {
+  alignas(16) T v[LOGITS_16B<T>];
+  for (int e = 0; e < LOGITS_16B<T>; ++e) v[e] = j + e >= lo && j + e < hi ? base[j + e] : no_logit<T>();
+  return *reinterpret_cast<const uint4*>(v);
+}
+
+// Places j of a row from a 16-byte boundary on: id j - lo; those in [lo, hi) are the row's.  Lane l of a warp has N = 16 bytes' logits of every
+// 32 * N: value i of its 32 in chunk k is place k * CHUNK + (i / N) * 32 N + l * N + i % N.
+template <class T, int NT>
 struct Row {
-  static constexpr int N = LOGITS_16B<T>;
+  static constexpr int N = LOGITS_16B<T>, WARPS = NT / 32;
   const T* base;
   int lo, hi, chunk0, chunks;                      // this CTA's chunks
 
@@ -99,51 +110,50 @@ struct Row {
   __device__ __forceinline__ float one(int j) const { return j >= lo && j < hi ? plain_logit(logit(base + j)) : -INFINITY; }
   static __device__ __forceinline__ int place(int chunk, int i, int lane) { return chunk * CHUNK + (i / N) * (32 * N) + lane * N + i % N; }
 
-  __device__ __forceinline__ void load(int chunk, float (&v)[32]) const {
-    const int lane = threadIdx.x & 31, j0 = chunk * CHUNK;
-    if (j0 >= lo && j0 + CHUNK <= hi) {
-      uint4 q[32 / N];
+  // A lane's values from value `from` on, M of them.
+  template <int M>
+  __device__ __forceinline__ void load(int chunk, int from, int lane, float (&v)[M]) const {
+    const int j0 = place(chunk, from, lane);
+    uint4 q[M / N];
+    if (chunk * CHUNK >= lo && chunk * CHUNK + CHUNK <= hi) {
 #pragma unroll
-      for (int i = 0; i < 32 / N; ++i) q[i] = __ldg(reinterpret_cast<const uint4*>(base + j0 + i * 32 * N) + lane);
-#pragma unroll
-      for (int i = 0; i < 32 / N; ++i) {
-        float f[N];
-        unpack_logits<T>(q[i], f);
-#pragma unroll
-        for (int e = 0; e < N; ++e) v[i * N + e] = plain_logit(f[e]);
-      }
+      for (int i = 0; i < M / N; ++i) q[i] = __ldg(reinterpret_cast<const uint4*>(base + j0 + i * 32 * N));
     } else {
 #pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = one(place(chunk, i, lane));
-    }
-  }
-  // Eight values of a lane, from value 8 q of the chunk on.
-  __device__ __forceinline__ void load8(int chunk, int q, int lane, float (&v)[8]) const {
-    const int j0 = chunk * CHUNK;
-    if (j0 >= lo && j0 + CHUNK <= hi) {
-      uint4 w[8 / N];
-#pragma unroll
-      for (int i = 0; i < 8 / N; ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(base + j0 + (q * (8 / N) + i) * 32 * N) + lane);
-#pragma unroll
-      for (int i = 0; i < 8 / N; ++i) {
-        float f[N];
-        unpack_logits<T>(w[i], f);
-#pragma unroll
-        for (int e = 0; e < N; ++e) v[i * N + e] = plain_logit(f[e]);
+      for (int i = 0; i < M / N; ++i) {
+        const int j = j0 + i * 32 * N;
+        if (j >= lo && j + N <= hi) q[i] = __ldg(reinterpret_cast<const uint4*>(base + j));
+        else q[i] = edge_vector(base, j, lo, hi);
       }
-    } else {
+    }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = one(place(chunk, 8 * q + e, lane));
+    for (int i = 0; i < M / N; ++i) {
+      float f[N];
+      unpack_logits<T>(q[i], f);
+#pragma unroll
+      for (int e = 0; e < N; ++e) v[i * N + e] = plain_logit(f[e]);
     }
   }
-  // f(32 logits, chunk) for each of a warp's chunks that `wanted(chunk's number in the CTA)`.
-  template <class W, class F>
-  __device__ __forceinline__ void stream(W wanted, F f) const {
-    for (int k = threadIdx.x >> 5; k < chunks; k += ROW_WARPS) {
-      if (!wanted(k)) continue;
+  // f(32 logits, chunk's number in the CTA) for each of a warp's chunks.
+  template <class F>
+  __device__ __forceinline__ void stream(F f) const {
+    for (int k = threadIdx.x >> 5; k < chunks; k += WARPS) {
       float v[32];
-      load(chunk0 + k, v);
+      load(chunk0 + k, 0, threadIdx.x & 31, v);
       f(v, k);
+    }
+  }
+  // f(8 logits, chunk's number, value of the first) for each of a warp's chunks that is `wanted`: less code, for what is read again.
+  template <class W, class F>
+  __device__ __forceinline__ void eights(W wanted, F f) const {
+    for (int k = threadIdx.x >> 5; k < chunks; k += WARPS) {
+      if (!wanted(k)) continue;
+#pragma unroll 1
+      for (int q = 0; q < 32; q += 8) {
+        float v[8];
+        load(chunk0 + k, q, threadIdx.x & 31, v);
+        f(v, k, q);
+      }
     }
   }
 };
@@ -164,15 +174,6 @@ struct Groups {
       g[k * 32 + lane] = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
     }
   }
-  // f(chunk's number, which eight of its lane's values) for a thread's own groups with a logit of `least` or more.
-  template <class F>
-  __device__ __forceinline__ void own(int chunks, float least, F f) const {
-    const int lane = threadIdx.x & 31, per = 4 >> shift;
-    for (int k = threadIdx.x >> 5; k < chunks; k += ROW_WARPS)
-      for (int q = 0; q < per; ++q)
-        if (g[(k * per + q) * 32 + lane] >= least)
-          for (int e = 0; e < 1 << shift; ++e) f(k, (q << shift) + e);
-  }
   // Whether the chunk has a logit of `least` or more.
   __device__ __forceinline__ bool reaches(int k, float least) const {
     const int lane = threadIdx.x & 31;
@@ -182,26 +183,97 @@ struct Groups {
   }
 };
 
-__device__ __forceinline__ void max8(const float (&v)[32], float (&m)[4]) {
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    m[q] = v[8 * q];
-#pragma unroll
-    for (int e = 1; e < 8; ++e) m[q] = fmaxf(m[q], v[8 * q + e]);
+// Behind a CTA's groups: of a cluster, the largest logits of all its threads, and the leader's inbox.
+template <int NT>
+struct Parts {
+  Groups groups;
+  float* maxima;
+  u64* inbox;
+  static __host__ __device__ __forceinline__ int shift_of(int per) { return per <= 160 ? 0 : per <= 320 ? 1 : 2; }
+  static __host__ int bytes(int per, int size) { return per * (128 >> shift_of(per)) * 4 + (size > 1 ? size * NT * 4 + LIST * 8 : 0); }
+  __device__ __forceinline__ Parts(float* smem, int per, int size) {
+    groups = Groups{smem, shift_of(per)};
+    maxima = smem + per * (128 >> groups.shift);
+    inbox = reinterpret_cast<u64*>(maxima + size * NT);
   }
+};
+
+__device__ __forceinline__ float max8(const float* v) {
+  float m = v[0];
+#pragma unroll
+  for (int e = 1; e < 8; ++e) m = fmaxf(m, v[e]);
+  return m;
 }
 
-// A warp's best token so far: chunks come in the order of their ids, so that only larger logits replace it.
-template <class T>
-__device__ __forceinline__ void note_best(const Row<T>& row, const float (&v)[32], float mine, float highest, int chunk, Best& best) {
-  if (!(highest > best.v)) return;
-  int j = NO_ID;
-  if (mine == highest) {
-#pragma unroll
-    for (int i = 31; i >= 0; --i)
-      if (v[i] == highest) j = Row<T>::place(chunk, i, threadIdx.x & 31);
+// What a thread has seen of the row: the best token and the units (its warp's), its own share of the sums of 2^(z c - E), E whole: a change of units changes
+// no bit, and in which batch a row is makes no difference.  s: of all logits, g: of the largest of every eight; n: a number.
+struct Seen {
+  Best top{-INFINITY, NO_ID};
+  float E = LOWEST;
+  unsigned n = 0;
+  double s = 0, g = 0;
+  __device__ __forceinline__ void add(double a, double b, float units) {
+    if (units > E) {
+      const double f = s ? pow2(E - units) : 0;    // (warps alike)
+      s *= f;
+      g *= f;
+      E = units;
+    }
+    const double f = pow2(units - E);
+    s += a * f;
+    g += b * f;
   }
-  best = Best{highest, row.id(__reduce_min_sync(0xffffffffu, j))};
+};
+// The largest of a lane's eights, of the lane, of the chunk; the warp's best token kept: chunks come in the order of their ids, so that only larger logits
+// replace it.
+template <class R>
+__device__ __forceinline__ float look(const R& row, const float (&v)[32], int k, float (&m)[4], float& mine, Best& best) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) m[q] = max8(v + 8 * q);
+  mine = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+  const float highest = warp_highest(mine);
+  if (highest > best.v) {
+    int j = NO_ID;
+    if (mine == highest) {
+#pragma unroll
+      for (int i = 31; i >= 0; --i)
+        if (v[i] == highest) j = R::place(row.chunk0 + k, i, threadIdx.x & 31);
+    }
+    best = Best{highest, row.id(__reduce_min_sync(0xffffffffu, j))};
+  }
+  return highest;
+}
+// Of the whole row.
+__device__ __forceinline__ Seen row_seen(Cluster& c, Seen m, bool sums, bool numbers) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = blockDim.x >> 5;
+  if (sums) { m.s = warp_total(m.s); m.g = warp_total(m.g); }
+  if (numbers) m.n = __reduce_add_sync(0xffffffffu, m.n);
+  if (lane == 0) *reinterpret_cast<Seen*>(&c.mine->warp[w]) = m;
+  __syncthreads();
+  const auto join = [&](const Mail* from, int n) {
+    const Seen x = lane < n ? *reinterpret_cast<const Seen*>(from + lane) : Seen{};
+    Seen y;
+    y.top.v = warp_highest(x.top.v);
+    y.top.id = __reduce_min_sync(0xffffffffu, x.top.v == y.top.v ? x.top.id : NO_ID);
+    if (sums) {
+      y.E = warp_highest(x.E);
+      const double f = x.s ? pow2(x.E - y.E) : 0;
+      y.s = x.s * f;
+      y.g = x.g * f;
+#pragma unroll
+      for (int o = 8; o; o >>= 1) {                // (at most 16 of them)
+        y.s += __shfl_xor_sync(0xffffffffu, y.s, o);
+        y.g += __shfl_xor_sync(0xffffffffu, y.g, o);
+      }
+      y.s = __shfl_sync(0xffffffffu, y.s, 0);
+      y.g = __shfl_sync(0xffffffffu, y.g, 0);
+    }
+    if (numbers) y.n = __reduce_add_sync(0xffffffffu, x.n);
+    return y;
+  };
+  if (w == 0) m = join(c.mine->warp, nw);
+  const Mail* b = c.tell(m);
+  return join(b, c.size);
 }
 
 // ------------------------------------------------------------------------------------------------ histograms and lists
@@ -221,122 +293,134 @@ struct Weights {
   }
 };
 
-__device__ __forceinline__ void clear_bins(RowShared& sh) {
-  for (int i = threadIdx.x; i < BINS; i += ROW_THREADS) sh.hist[i] = 0;
+template <int NT>
+__device__ __forceinline__ void clear_bins(RowShared<NT>& sh) {
+  for (int i = threadIdx.x; i < BINS; i += NT) sh.hist[i] = 0;
 }
 // A logit into its bin: as one, or as its weight in 2^-16 of the bin's highest (a little less at most).
-__device__ __forceinline__ void to_bin(RowShared& sh, const Weights& w, float z, bool by_count) {
+template <int NT>
+__device__ __forceinline__ void to_bin(RowShared<NT>& sh, const Weights& w, float z, bool by_count) {
   const int bin = w.bin(z);
   atomicAdd(&sh.hist[bin], by_count ? 1u : static_cast<unsigned>(fminf(exp2_fast(w.bits(z) + bin * (1.f / BINS_PER_BIT)) * 65536.f, 65536.f)));
 }
 // The first bin with which the bins (of the cluster's CTAs together, or this one's) hold `target`, tokens or weight: the last one where they do not.
-// Into sh.bin, with the tokens in front of it in sh.before.
-__device__ __forceinline__ void find_bin(RowShared& sh, Cluster& c, bool together, bool by_count, double target) {
+// Into sh.bin, with the tokens in front of it in sh.before.  (fp32: numbers of tokens are exact, weights are asked for with some to spare.)
+template <int NT>
+__device__ __forceinline__ void find_bin(RowShared<NT>& sh, Cluster& c, bool together, bool by_count, float target) {
   const int t = threadIdx.x, lane = t & 31, w = t >> 5;
-  static_assert(BINS == 2 * ROW_THREADS, "two bins per thread");
-  double v0 = 0, v1 = 0;
+  constexpr int PER = BINS / NT;
+  float v[PER], sum = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) v[i] = 0;
   if (!together || c.size == 1) {
-    v0 = sh.hist[2 * t];
-    v1 = sh.hist[2 * t + 1];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) v[i] = sh.hist[PER * t + i];
   } else {
-    uint2 n[8];
 #pragma unroll
-    for (int r = 0; r < 8; ++r)
-      if (r < c.size) n[r] = *reinterpret_cast<const uint2*>(c.of(sh.hist, r) + 2 * t);
+    for (int i = 0; i < PER; i += 2) {
+      uint2 n[CLUSTER_MAX];
 #pragma unroll
-    for (int r = 0; r < 8; ++r)
-      if (r < c.size) { v0 += n[r].x; v1 += n[r].y; }
+      for (int r = 0; r < CLUSTER_MAX; ++r)
+        if (r < c.size) n[r] = *reinterpret_cast<const uint2*>(c.of(sh.hist, r) + PER * t + i);
+#pragma unroll
+      for (int r = 0; r < CLUSTER_MAX; ++r)
+        if (r < c.size) { v[i] += n[r].x; v[i + 1] += n[r].y; }
+    }
   }
-  if (!by_count) {
-    v0 *= exp2f(t * (-2.f / BINS_PER_BIT));
-    v1 *= exp2f((2 * t + 1) * (-1.f / BINS_PER_BIT));
-    target *= 65536.0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    if (!by_count) v[i] *= exp2_fast((PER * t + i) * (-1.f / BINS_PER_BIT)) * (1.f / 65536);
+    sum += v[i];
   }
-  double incl = v0 + v1;
+  float incl = sum;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const double y = __shfl_up_sync(0xffffffffu, incl, o);
+    const float y = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += y;
   }
-  if (lane == 31) sh.dsum[w] = incl;
+  if (lane == 31) sh.fsum[w] = incl;
   if (t == 0) { sh.bin = BINS - 1; sh.before = 0; }
   __syncthreads();
-  double at = incl - (v0 + v1);
-  for (int i = 0; i < w; ++i) at += sh.dsum[i];
-  if (at < target && at + v0 >= target) { sh.bin = 2 * t; sh.before = static_cast<unsigned>(at); }
-  else if (at + v0 < target && at + v0 + v1 >= target) { sh.bin = 2 * t + 1; sh.before = static_cast<unsigned>(at + v0); }
+  float at = incl - sum;
+  for (int i = 0; i < w; ++i) at += sh.fsum[i];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {                  // (rounding may find two: the first counts)
+    if (at < target && at + v[i] >= target) { atomicMin(&sh.bin, PER * t + i); if (by_count) sh.before = static_cast<unsigned>(at); }
+    at += v[i];
+  }
   __syncthreads();
 }
 
-__device__ __forceinline__ void to_list(RowShared& sh, float z, int id) {
+template <int NT>
+__device__ __forceinline__ void to_list(RowShared<NT>& sh, float z, int id) {
   const unsigned at = atomicAdd(&sh.n_list, 1u);
   if (at < LIST) sh.list[at] = list_key(z, id);
 }
 // The CTAs' lists behind the leader's own; how many they hold together, which everyone gets and which may be more than a list takes (nothing is moved then).
 // A CTA has a part of the leader's `inbox` to itself, so that entries and numbers travel together; only longer lists wait for the others' numbers.
-__device__ __forceinline__ unsigned join_lists(RowShared& sh, Cluster& c, u64* inbox) {
+template <int NT>
+__device__ __forceinline__ unsigned join_lists(RowShared<NT>& sh, Cluster& c, u64* inbox) {
   __syncthreads();
   const unsigned mine = sh.n_list;
   if (c.size == 1) return mine;
   const unsigned part = LIST / c.size, t = threadIdx.x;
-  if (t < c.size) c.of(&sh.mail.box[c.phase][c.rank], t)->w[0] = mine;
   if (c.rank && mine <= part) {
     u64* to = c.of(inbox, 0) + c.rank * part;
-    for (unsigned i = t; i < mine; i += ROW_THREADS) to[i] = sh.list[i];
+    for (unsigned i = t; i < mine; i += NT) to[i] = sh.list[i];
   }
-  c.sync();
+  const Mail* box = c.tell(mine);
   unsigned n = 0, before = 0, most = 0;
   for (int r = 0; r < c.size; ++r) {
-    const unsigned m = static_cast<unsigned>(sh.mail.box[c.phase][r].w[0]);
+    const unsigned m = *reinterpret_cast<const unsigned*>(box + r);
     before += r < c.rank ? m : 0;
     most = max(most, r ? m : 0);
     n += m;
   }
-  if (n <= LIST) {
-    if (most > part) {
-      if (c.rank && mine > part) {
-        u64* to = c.of(sh.list, 0) + before;
-        for (unsigned i = t; i < mine; i += ROW_THREADS) to[i] = sh.list[i];
-      }
-      c.sync();
+  if (n > LIST) return n;
+  if (most > part) {
+    if (c.rank && mine > part) {
+      u64* to = c.of(sh.list, 0) + before;
+      for (unsigned i = t; i < mine; i += NT) to[i] = sh.list[i];
     }
-    if (c.rank == 0) {
-      unsigned at = mine;
-      for (int r = 1; r < c.size; ++r) {
-        const unsigned m = static_cast<unsigned>(sh.mail.box[c.phase][r].w[0]);
-        if (m <= part)
-          for (unsigned i = t; i < m; i += ROW_THREADS) sh.list[at + i] = inbox[r * part + i];
-        at += m;
-      }
-      __syncthreads();
-    }
+    c.sync();
   }
-  c.phase ^= 1;
+  if (c.rank == 0) {
+    unsigned at = mine;
+    for (int r = 1; r < c.size; ++r) {
+      const unsigned m = *reinterpret_cast<const unsigned*>(box + r);
+      if (m <= part)
+        for (unsigned i = t; i < m; i += NT) sh.list[at + i] = inbox[r * part + i];
+      at += m;
+    }
+    __syncthreads();
+  }
   return n;
 }
 
 // list[0, n) in the row's order (descending keys; all differ).
-__device__ __forceinline__ void sort_list(RowShared& sh, unsigned n) {
+template <int NT>
+__device__ __noinline__ void sort_list(u64* list, unsigned n) {
   unsigned m = 32;
   while (m < n) m *= 2;
-  for (unsigned i = n + threadIdx.x; i < m; i += ROW_THREADS) sh.list[i] = 0;
+  for (unsigned i = n + threadIdx.x; i < m; i += NT) list[i] = 0;
   __syncthreads();
   for (unsigned k = 2; k <= m; k *= 2)
     for (unsigned j = k / 2; j; j /= 2) {
-      for (unsigned p = threadIdx.x; p < m / 2; p += ROW_THREADS) {
+      for (unsigned p = threadIdx.x; p < m / 2; p += NT) {
         const unsigned a = 2 * p - (p & (j - 1)), b = a + j;
-        const u64 x = sh.list[a], y = sh.list[b];
-        if ((x < y) == ((a & k) == 0)) { sh.list[a] = y; sh.list[b] = x; }
+        const u64 x = list[a], y = list[b];
+        if ((x < y) == ((a & k) == 0)) { list[a] = y; list[b] = x; }
       }
       __syncthreads();
     }
 }
 
-// Up to FEW entries: how many of the list are in front of an entry, and their weight.  Threads share an entry; the first of them has it.
+// Up to NT / 2 entries: how many of the list are in front of an entry, and their weight.  Threads share an entry; the first of them has it.
 struct Counted { u64 key, weight, before; unsigned rank; bool mine; };
-__device__ __forceinline__ Counted count_list(RowShared& sh, unsigned n, bool weights) {
-  int per = ROW_THREADS / 32;
-  while (per * n > ROW_THREADS) per /= 2;                      // (n <= 256: at least 2)
+template <int NT>
+__device__ __forceinline__ Counted count_list(RowShared<NT>& sh, unsigned n, bool weights) {
+  int per = 16;
+  while (per * n > NT) per /= 2;
   const unsigned at = threadIdx.x / per, part = threadIdx.x % per;
   Counted e{0, 0, 0, 0, part == 0 && at < n};
   if (at < n) {
@@ -355,6 +439,54 @@ __device__ __forceinline__ Counted count_list(RowShared& sh, unsigned n, bool we
   return e;
 }
 
+// The bins below which the row's first tokens lie, from the largest logit of every thread.
+template <int NT>
+__device__ __forceinline__ void bins_of_threads(RowShared<NT>& sh, Cluster& c, const float* maxima, float mine, const Weights& w, float least, bool by_count, float target) {
+  for (int r = 0; r < c.size; ++r) {
+    const float z = c.size > 1 ? maxima[r * NT + threadIdx.x] : mine;
+    if (z >= least) to_bin(sh, w, z, by_count);
+  }
+  __syncthreads();
+  find_bin(sh, c, false, by_count, target);
+}
+// The same from the groups' (the bins are of no use any more).
+template <int NT>
+__device__ __noinline__ void bins_of_groups(RowShared<NT>& sh, Cluster& c, const Groups groups, int chunks, const Weights w, float least, bool by_count, float target) {
+  clear_bins(sh);
+  __syncthreads();
+  for (int i = threadIdx.x; i < chunks * (128 >> groups.shift); i += NT)
+    if (groups.g[i] >= least) to_bin(sh, w, groups.g[i], by_count);
+  c.sync();
+  find_bin(sh, c, true, by_count, target);
+}
+// What lies at `least` and above, in the leader's list.  First which groups of eight have any, then a thread for each of them.
+template <class T, int NT>
+__device__ __forceinline__ unsigned gather(RowShared<NT>& sh, Cluster& c, const Row<T, NT>& row, const Parts<NT>& parts, float mine, float least) {
+  const int lane = threadIdx.x & 31, shift = parts.groups.shift, per = 4 >> shift;
+  const auto read = [&](int i) {                   // group i
+    const int g = i >> 5, chunk = row.chunk0 + (g >> (2 - shift)), from = (g & (per - 1)) * (8 << shift);
+    for (int q = 0; q < 8 << shift; q += 8) {
+      float v[8];
+      row.load(chunk, from + q, i & 31, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (v[e] >= least) to_list(sh, v[e], row.id(Row<T, NT>::place(chunk, from + q + e, i & 31)));
+    }
+  };
+  if (mine >= least)
+    for (int k = threadIdx.x >> 5; k < row.chunks; k += NT / 32)
+      for (int q = 0; q < per; ++q) {
+        const int i = (k * per + q) * 32 + lane;
+        if (!(parts.groups.g[i] >= least)) continue;
+        const unsigned at = atomicAdd(&sh.n_hits, 1u);
+        if (at < HITS) sh.hits[at] = i;
+        else read(i);
+      }
+  __syncthreads();
+  for (unsigned h = threadIdx.x; h < min(sh.n_hits, static_cast<unsigned>(HITS)); h += NT) read(sh.hits[h]);
+  return join_lists(sh, c, parts.inbox);
+}
+
 // ------------------------------------------------------------------------------------------------ draws
 
 __device__ __forceinline__ u64 mix64(u64 x) {
@@ -364,7 +496,7 @@ __device__ __forceinline__ u64 mix64(u64 x) {
 }
 
 struct Top2 { float a1; int id; float a2, z; };                // the best score, its token, the second best score, the token's logit
-constexpr Top2 NO_TOP{-INFINITY, NO_ID, -INFINITY, -INFINITY};
+__device__ __forceinline__ Top2 no_top() { return Top2{-INFINITY, NO_ID, -INFINITY, -INFINITY}; }
 __device__ __forceinline__ Top2 best2(Top2 x, Top2 y) {
   return x.a1 >= y.a1 ? Top2{x.a1, x.id, fmaxf(x.a2, y.a1), x.z} : Top2{y.a1, y.id, fmaxf(y.a2, x.a1), y.z};
 }
@@ -376,15 +508,17 @@ __device__ __forceinline__ Win first_win(Win a, Win b) { return b.v > a.v || (b.
 struct Race {
   float temp, c;
   u64 key;
+  static constexpr u64 STEP = 0x9E3779B97F4A7C15ull;
   __device__ __forceinline__ Race(float T, float c_, long long seed, long long pos)
-      : temp(T), c(c_), key((static_cast<u64>(seed) * 0x9E3779B97F4A7C15ull) ^ (static_cast<u64>(pos + 1) * 0xBF58476D1CE4E5B9ull)) {}
-  __device__ __forceinline__ u64 hash(int id) const { return mix64(static_cast<u64>(id) * 0x9E3779B97F4A7C15ull + key); }
+      : temp(T), c(c_), key((static_cast<u64>(seed) * STEP) ^ (static_cast<u64>(pos + 1) * 0xBF58476D1CE4E5B9ull)) {}
+  __device__ __forceinline__ u64 hash(int id) const { return mix64(static_cast<u64>(id) * STEP + key); }
   __device__ __forceinline__ float exact(float z, int id) const {
     const double u = (static_cast<double>(hash(id) >> 11) + 0.5) * (1.0 / 9007199254740992.0);
     return __fadd_rn(__fdiv_rn(z, temp), static_cast<float>(-log(-log(u))));
   }
   // -log u from q = 1 - u where u is near 1 (to q^3 of it), from u where it is near 0; each to 2^-13 of itself.
-  __device__ __forceinline__ float rough(float z, u64 h) const {
+  __device__ __forceinline__ float rough(float z, int id) const {
+    const u64 h = hash(id);
     const float q = (__ull2float_rn(~h >> 11) + 0.5f) * (1.f / 9007199254740992.f);
     const float L = q < 1.f / 256 ? q * (1.f + q * (0.5f + q * (1.f / 3))) : -__logf(q < 0.5f ? 1.f - q : (__ull2float_rn(h >> 11) + 0.5f) * (1.f / 9007199254740992.f));
     return __fdiv_rn(z, temp) - __logf(L);
@@ -396,106 +530,123 @@ struct Race {
 // A warp's race over the logits that come by.  -log u >= 1 - u, so that a score is at most z / T - log(1 - u): most tokens are out of it by the 32
 // upper bits of their hash, without a logarithm.
 struct Racer {
-  Top2 m = NO_TOP;
+  Top2 m = no_top();
   float bound = -INFINITY, off = 0.f;              // the best score so far, and what it takes to come near it
   __device__ __forceinline__ void raise(float b) {
     bound = b;
     off = (Race::margin(b) - b) * 1.4426950408889634f + 32.f;
   }
-  // `mine`: the lane's largest logit.  The first chunk's 32 largest raise the bound before all others come.
-  template <class T>
-  __device__ __forceinline__ void run(const Race& race, const Row<T>& row, const float (&v)[32], float mine, int chunk, const Prefix& kept) {
-    const int lane = threadIdx.x & 31;
-    if (bound == -INFINITY) {
-      int j = 0;
+  // The lanes' largest logits raise the bound before all others come; false where none of them is within `kept`, and no other then.
+  template <int M, class R>
+  __device__ __forceinline__ bool begin(const Race& race, const R& row, const float (&v)[M], float mine, int chunk, int from, const Prefix& kept) {
+    int j = 0;
 #pragma unroll
-      for (int i = 31; i >= 0; --i)
-        if (v[i] == mine) j = Row<T>::place(chunk, i, lane);
-      const float b = warp_highest(within(kept, mine, row.id(j)) ? race.rough(mine, race.hash(row.id(j))) : -INFINITY);
-      if (b == -INFINITY) return;                  // (a lane without its largest logit has none)
-      raise(b);
+    for (int i = M - 1; i >= 0; --i)
+      if (v[i] == mine) j = R::place(chunk, from + i, threadIdx.x & 31);
+    const float b = warp_highest(within(kept, mine, row.id(j)) ? race.rough(mine, row.id(j)) : -INFINITY);
+    if (b == -INFINITY) return false;
+    raise(b);
+    return true;
+  }
+  // Eight values of the lane, from value `from` of the chunk on.
+  template <class R>
+  __device__ __forceinline__ void run(const Race& race, const R& row, const float* v, int chunk, int from, const Prefix& kept) {
+    const int j0 = R::place(chunk, from, threadIdx.x & 31), id0 = row.id(j0);
+    const u64 first = static_cast<u64>(static_cast<long long>(id0)) * Race::STEP + race.key;
+    unsigned near = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int d = i / R::N * (32 * R::N) + i % R::N;
+      u64 x = first + static_cast<u64>(d) * Race::STEP;
+      x = (x ^ (x >> 30)) * 0xBF58476D1CE4E5B9ull;
+      x = (x ^ (x >> 27)) * 0x94D049BB133111EBull;
+      const uint32_t hi = static_cast<uint32_t>(x >> 32), rest = ~(hi ^ (hi >> 31));
+      if (within(kept, v[i], id0 + d) && !(static_cast<float>(rest) > exp2_fast(fmaf(v[i], race.c, off)))) near |= 1u << i;
     }
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      bool more = false;
-#pragma unroll
-      for (int i = 8 * g; i < 8 * g + 8; ++i) {
-        const int id = row.id(Row<T>::place(chunk, i, lane));
-        if (!within(kept, v[i], id)) continue;
-        const u64 h = race.hash(id);
-        if (static_cast<float>(static_cast<uint32_t>(~h >> 32)) > exp2_fast(fmaf(v[i], race.c, off))) continue;
-        const float y = race.rough(v[i], h);
-        m = best2(m, Top2{y, id, -INFINITY, v[i]});
-        more |= y > bound;
-      }
-      if (__any_sync(0xffffffffu, more)) raise(fmaxf(bound, warp_highest(m.a1)));
+    bool more = false;
+    while (near) {
+      const int i = __ffs(near) - 1, j = j0 + i / R::N * (32 * R::N) + i % R::N;
+      near &= near - 1;
+      const float z = row.one(j), y = race.rough(z, row.id(j));
+      m = best2(m, Top2{y, row.id(j), -INFINITY, z});
+      more |= y > bound;
     }
+    if (__any_sync(0xffffffffu, more)) raise(fmaxf(bound, warp_highest(m.a1)));
   }
 };
 
-// The winner among the tokens within `kept`, from the two best of a race.
-template <class T, class W>
-__device__ __forceinline__ Win settle(const Row<T>& row, Cluster& c, const Race& race, const Prefix& kept, Top2 m, W wanted) {
-  m = c.reduce(m, NO_TOP, best2);
-  if (m.a2 < m.a1 - Race::margin(m.a1)) return Win{m.a1, m.id, m.z, 0};
-  Win b{-INFINITY, NO_ID, -INFINITY, 0};
-  const Win none = b;
-  row.stream(wanted, [&](const float (&v)[32], int k) {
-#pragma unroll 1
-    for (int i = 0; i < 32; ++i) {
-      const int j = Row<T>::place(row.chunk0 + k, i, threadIdx.x & 31), id = row.id(j);
-      const float z = row.one(j);
-      if (!within(kept, z, id) || race.rough(z, race.hash(id)) < m.a1 - Race::margin(m.a1)) continue;
-      b = first_win(b, Win{race.exact(z, id), id, z, 0});
-    }
+// A race over what lies within `front`, and the weight of that.
+struct Lap { Top2 m; double s; };
+template <class T, int NT>
+__device__ __noinline__ Lap lap(const Row<T, NT> row, const Groups groups, const Race race, const Weights w, const Prefix front) {
+  Racer racer;
+  double s = 0;
+  row.eights([&](int k) { return groups.reaches(k, front.z); }, [&](const float (&v)[8], int k, int q) {
+    const int chunk = row.chunk0 + k;
+    const float mine = max8(v);
+    if (__all_sync(0xffffffffu, !(mine >= front.z))) return;
+    float f[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = within(front, v[i], row.id(Row<T, NT>::place(chunk, q + i, threadIdx.x & 31))) ? w(v[i]) : 0.f;
+    s += ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
+    if (racer.bound > -INFINITY || racer.begin(race, row, v, mine, chunk, q, front)) racer.run(race, row, v, chunk, q, front);
   });
-  return c.reduce(b, none, first_win);
+  return Lap{racer.m, s};
+}
+__device__ __forceinline__ double row_total(Cluster& c, double s) {
+  return c.reduce(s, 0.0, [](double a, double b) { return a + b; });
 }
 
-// The leader's: the winner among its candidates, of which a thread has one at most (`in`).  Thread 0 has it.
-__device__ __forceinline__ int draw_few(RowShared& sh, Cluster& c, const Race& race, u64 key, bool in) {
-  Top2 m = in ? Top2{race.rough(list_z(key), race.hash(list_id(key))), list_id(key), -INFINITY, 0} : NO_TOP;
-  m = c.block(m, NO_TOP, best2);
-  if (threadIdx.x == 0) sh.kept = m.a2 < m.a1 - Race::margin(m.a1);
-  __syncthreads();
-  if (sh.kept) return m.id;
-  Best b = in ? Best{race.exact(list_z(key), list_id(key)), list_id(key)} : Best{-INFINITY, NO_ID};
-  return c.block(b, Best{-INFINITY, NO_ID}, first_of).id;
+// The winner among the tokens within `kept`, from the two best of a race.
+template <class T, int NT>
+__device__ __noinline__ Win photo_finish(const Row<T, NT> row, Cluster& c, const Race race, const Prefix kept, float best) {
+  Win b{-INFINITY, NO_ID, -INFINITY, 0};
+  row.eights([](int) { return true; }, [&](const float (&)[8], int k, int q) {
+#pragma unroll 1
+    for (int i = 0; i < 8; ++i) {
+      const int j = Row<T, NT>::place(row.chunk0 + k, q + i, threadIdx.x & 31), id = row.id(j);
+      const float z = row.one(j);
+      if (within(kept, z, id) && race.rough(z, id) >= best - Race::margin(best)) b = first_win(b, Win{race.exact(z, id), id, z, 0});
+    }
+  });
+  return c.reduce(b, Win{-INFINITY, NO_ID, -INFINITY, 0}, first_win);
 }
-// The same among the first n of its list.
-__device__ __forceinline__ int draw_list(RowShared& sh, Cluster& c, const Race& race, unsigned n) {
-  Top2 m = NO_TOP;
-  for (unsigned i = threadIdx.x; i < n; i += ROW_THREADS) {
-    const u64 k = sh.list[i];
-    m = best2(m, Top2{race.rough(list_z(k), race.hash(list_id(k))), list_id(k), -INFINITY, 0});
-  }
-  m = c.block(m, NO_TOP, best2);
+template <class T, int NT>
+__device__ __forceinline__ Win settle(const Row<T, NT>& row, Cluster& c, const Race& race, const Prefix& kept, Top2 m) {
+  m = c.reduce(m, no_top(), best2);
+  if (m.a2 < m.a1 - Race::margin(m.a1)) return Win{m.a1, m.id, m.z, 0};
+  return photo_finish(row, c, race, kept, m.a1);
+}
+
+// The leader's: the winner among what `each` gives (f(key) for the thread's candidates).  Thread 0 has it.
+template <int NT, class E>
+__device__ __forceinline__ int draw_listed(RowShared<NT>& sh, Cluster& c, const Race& race, E each) {
+  Top2 m = no_top();
+  each([&](u64 k) { m = best2(m, Top2{race.rough(list_z(k), list_id(k)), list_id(k), -INFINITY, 0}); });
+  m = c.block(m, no_top(), best2);
   if (threadIdx.x == 0) sh.kept = m.a2 < m.a1 - Race::margin(m.a1);
   __syncthreads();
   if (sh.kept) return m.id;
   Best b{-INFINITY, NO_ID};
-  for (unsigned i = threadIdx.x; i < n; i += ROW_THREADS) {
-    const u64 k = sh.list[i];
-    b = first_of(b, Best{race.exact(list_z(k), list_id(k)), list_id(k)});
-  }
+  each([&](u64 k) { b = first_of(b, Best{race.exact(list_z(k), list_id(k)), list_id(k)}); });
   return c.block(b, Best{-INFINITY, NO_ID}, first_of).id;
 }
 
 // ------------------------------------------------------------------------------------------------ the k-th token
 
-template <class T, class F>
-__device__ __forceinline__ u64 row_count(const Row<T>& row, Cluster& c, F f) {
+template <class T, int NT, class F>
+__device__ __forceinline__ u64 row_count(const Row<T, NT>& row, Cluster& c, F f) {
   u64 n = 0;
-  row.stream([](int) { return true; }, [&](const float (&v)[32], int k) {
+  row.eights([](int) { return true; }, [&](const float (&v)[8], int k, int q) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) n += f(v[i], row.id(Row<T>::place(row.chunk0 + k, i, threadIdx.x & 31))) ? 1 : 0;
+    for (int i = 0; i < 8; ++i) n += f(v[i], row.id(Row<T, NT>::place(row.chunk0 + k, q + i, threadIdx.x & 31))) ? 1 : 0;
   });
   return c.reduce(n, u64{0}, [](u64 a, u64 b) { return a + b; });
 }
 
 // By the bits of keys and ids, for the rare row in which more tokens than a list takes share a bin.
-template <class T>
-__device__ __noinline__ Prefix kth_by_bits(const Row<T>& row, Cluster& c, const Prefix of, u64 k) {
+template <class T, int NT>
+__device__ __noinline__ Prefix kth_by_bits(const Row<T, NT> row, Cluster& c, const Prefix of, u64 k) {
   if (row_count(row, c, [&](float z, int id) { return within(of, z, id); }) <= k) return of;
   uint32_t key = 0;
   for (int bit = 31; bit >= 0; --bit) {
@@ -513,33 +664,33 @@ __device__ __noinline__ Prefix kth_by_bits(const Row<T>& row, Cluster& c, const 
 }
 
 // The prefix of the first k tokens of `of` = (least logit, any id).
-template <class T>
-__device__ __forceinline__ Prefix kth_token(RowShared& sh, const Row<T>& row, const Groups& groups, Cluster& c, const Weights& w, const Prefix& of, unsigned k, u64* inbox) {
+template <class T, int NT>
+__device__ __noinline__ Prefix kth_token(RowShared<NT>& sh, const Row<T, NT> row, const Groups groups, Cluster& c, const Weights w, const Prefix of, unsigned k, u64* inbox) {
   c.sync();                                        // (nobody reads the bins and lists of before any more)
   clear_bins(sh);
   if (threadIdx.x == 0) sh.n_list = 0;
   __syncthreads();
-  row.stream([&](int i) { return groups.reaches(i, of.z); }, [&](const float (&v)[32], int) {
+  row.eights([&](int i) { return groups.reaches(i, of.z); }, [&](const float (&v)[8], int, int) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
+    for (int i = 0; i < 8; ++i)
       if (v[i] >= of.z) atomicAdd(&sh.hist[w.bin(v[i])], 1u);
   });
   c.sync();
   find_bin(sh, c, true, true, k);
   const int bin = sh.bin;
   const unsigned before = sh.before;               // (0 with the last bin where the row has fewer than k tokens)
-  row.stream([&](int i) { return groups.reaches(i, fmaxf(of.z, w.edge(bin))); }, [&](const float (&v)[32], int n) {
+  row.eights([&](int i) { return groups.reaches(i, fmaxf(of.z, w.edge(bin))); }, [&](const float (&v)[8], int n, int q) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (v[i] >= of.z && w.bin(v[i]) == bin) to_list(sh, v[i], row.id(Row<T>::place(row.chunk0 + n, i, threadIdx.x & 31)));
+    for (int i = 0; i < 8; ++i)
+      if (v[i] >= of.z && w.bin(v[i]) == bin) to_list(sh, v[i], row.id(Row<T, NT>::place(row.chunk0 + n, q + i, threadIdx.x & 31)));
   });
   const unsigned n = join_lists(sh, c, inbox);
   if (n > LIST) return kth_by_bits(row, c, of, k);
   if (c.rank == 0) {
-    sort_list(sh, n);
+    sort_list<NT>(sh.list, n);
     const u64 last = k - before <= n ? sh.list[k - before - 1] : 0;
     const Prefix cut = last ? Prefix{list_z(last), list_id(last)} : of;
-    if (threadIdx.x < c.size) (c.size > 1 ? c.of(&sh, threadIdx.x) : &sh)->cut = cut;
+    if (threadIdx.x < c.size) c.of(&sh, threadIdx.x)->cut = cut;
   }
   c.sync();
   return sh.cut;
@@ -547,57 +698,8 @@ __device__ __forceinline__ Prefix kth_token(RowShared& sh, const Row<T>& row, co
 
 // ------------------------------------------------------------------------------------------------ kernels
 
-// Behind a CTA's groups: of a cluster, the largest logits of all its threads, and the leader's inbox.
-constexpr int CLUSTER_MAX = 8;
-struct Parts {
-  Groups groups;
-  float* maxima;
-  u64* inbox;
-};
-__host__ __device__ __forceinline__ int group_shift(int per) { return per <= 160 ? 0 : per <= 320 ? 1 : 2; }
-__device__ __forceinline__ Parts parts_of(float* smem, int per, int size) {
-  const int shift = group_shift(per);
-  float* maxima = smem + per * (128 >> shift);
-  return Parts{Groups{smem, shift}, maxima, reinterpret_cast<u64*>(maxima + size * ROW_THREADS)};
-}
-static int part_bytes(int per, int size) { return per * (128 >> group_shift(per)) * 4 + (size > 1 ? size * ROW_THREADS * 4 + LIST * 8 : 0); }
-
-// The bins below which the row's first tokens lie, from the largest logit of every thread.
-template <class T>
-__device__ __forceinline__ void bins_of_threads(RowShared& sh, Cluster& c, const float* maxima, float mine, const Weights& w, float least, bool by_count, double target) {
-  for (int r = 0; r < c.size; ++r) {
-    const float z = c.size > 1 ? maxima[r * ROW_THREADS + threadIdx.x] : mine;
-    if (z >= least) to_bin(sh, w, z, by_count);
-  }
-  __syncthreads();
-  find_bin(sh, c, false, by_count, target);
-}
-// The same from the groups' (the bins are of no use any more).
-__device__ __forceinline__ void bins_of_groups(RowShared& sh, Cluster& c, const Groups& groups, int chunks, const Weights& w, float least, bool by_count, double target) {
-  clear_bins(sh);
-  __syncthreads();
-  for (int i = threadIdx.x; i < chunks * (128 >> groups.shift); i += ROW_THREADS)
-    if (groups.g[i] >= least) to_bin(sh, w, groups.g[i], by_count);
-  c.sync();
-  find_bin(sh, c, true, by_count, target);
-}
-// What lies at `least` and above, in the leader's list.
-template <class T>
-__device__ __forceinline__ unsigned gather(RowShared& sh, Cluster& c, const Row<T>& row, const Parts& parts, float mine, float least) {
-  if (mine >= least)
-    parts.groups.own(row.chunks, least, [&](int k, int q) {
-      const int chunk = row.chunk0 + k, lane = threadIdx.x & 31;
-      float v[8];
-      row.load8(chunk, q, lane, v);
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (v[e] >= least) to_list(sh, v[e], row.id(Row<T>::place(chunk, 8 * q + e, lane)));
-    });
-  return join_lists(sh, c, parts.inbox);
-}
-
 // The smallest logit that is not too improbable, decided in 64 bits.
-__device__ __forceinline__ float min_p_logit(float top, float temp, float mp) {
+__device__ __noinline__ float min_p_logit(float top, float temp, float mp) {
   const double top64 = top, T64 = temp, least = log(static_cast<double>(mp));
   const auto scaled = [&](float v) { return (static_cast<double>(v) - top64) / T64; };
   float v = fminf(static_cast<float>(top64 + T64 * least), top);
@@ -606,77 +708,69 @@ __device__ __forceinline__ float min_p_logit(float top, float temp, float mp) {
   return at_least(v);
 }
 
-template <class T>
-__global__ void __launch_bounds__(ROW_THREADS, 2)
+template <class T, int NT>
+__global__ void __launch_bounds__(NT, 1024 / NT)
 sample_kernel(const __grid_constant__ SampleRows a, int per) {
   extern __shared__ __align__(16) float smem[];
-  __shared__ RowShared sh;
+  __shared__ RowShared<NT> sh;
   pdl_wait();
   pdl_trigger();
   Cluster c(&sh.mail);
   const int t = threadIdx.x, r = blockIdx.x / c.size;
   const float temp = a.temps[r], mp = a.min_p ? a.min_p[r] : 0.f, p = a.top_p ? a.top_p[r] : 1.f;
   const int asked = a.top_k ? a.top_k[r] : 0, k = asked < a.V ? asked : 0;
-  const Row<T> row(static_cast<const T*>(a.x) + r * a.ldx, a.V, c.rank, per);
-  const Parts parts = parts_of(smem, per, c.size);
-  const Groups& groups = parts.groups;
+  const Row<T, NT> row(static_cast<const T*>(a.x) + r * a.ldx, a.V, c.rank, per);
+  const Parts<NT> parts(smem, per, c.size);
+  const Groups groups = parts.groups;
   const bool greedy = !(temp > 0.f) || k == 1 || p <= 0.f || mp > 1.f, by_p = p < 1.f, by_k = k > 0, by_min = mp > 0.f && isfinite(temp);
-  const bool all = !greedy && !by_p && !by_k && !by_min;
+  const bool all = !greedy && !by_p && !by_k && !by_min, sums = !greedy && by_p && !by_k && !by_min;
   // (products of it with 0 and infinity are 0 and infinity)
   const float scale = greedy ? 0.f : fmaxf(fminf(__fdiv_rn(1.4426950408889634f, temp), -LOWEST), 1e-44f);
-  const bool sums = !greedy && by_p && !by_k && !by_min;
   const Race race(temp, scale, a.seeds[r], a.positions[r]);
-  const Prefix whole_row{LOWEST, NO_ID};
   clear_bins(sh);
-  if (t == 0) sh.n_list = 0;
-  const auto every = [](int) { return true; };
+  if (t == 0) sh.n_list = sh.n_hits = 0;
 
-  Best top{-INFINITY, NO_ID};
-  Mass mass = NO_MASS;
+  Seen seen;
   Racer racer;
   float largest = -INFINITY;                       // of the thread
-  const auto look = [&](const float (&v)[32], float (&m)[4], int i, float& mine) {
-    max8(v, m);
-    mine = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-    const float highest = warp_highest(mine);
-    note_best(row, v, mine, highest, row.chunk0 + i, top);
-    largest = fmaxf(largest, mine);
-    return highest;
-  };
   if (all) {
-    row.stream(every, [&](const float (&v)[32], int i) {
+    row.stream([&](const float (&v)[32], int i) {
       float m[4], mine;
-      const float highest = look(v, m, i, mine);
-      if (highest > -INFINITY && highest < INFINITY) racer.run(race, row, v, mine, row.chunk0 + i, whole_row);
+      const float highest = look(row, v, i, m, mine, seen.top);
+      if (!(highest > -INFINITY && highest < INFINITY)) return;
+      if (racer.bound == -INFINITY) racer.begin(race, row, v, mine, row.chunk0 + i, 0, whole_row());
+#pragma unroll
+      for (int q = 0; q < 32; q += 8) racer.run(race, row, v + q, row.chunk0 + i, q, whole_row());
     });
   } else if (sums) {
-    row.stream(every, [&](const float (&v)[32], int i) {
+    row.stream([&](const float (&v)[32], int i) {
       float m[4], mine;
-      const float highest = look(v, m, i, mine);
+      const float highest = look(row, v, i, m, mine, seen.top);
+      largest = fmaxf(largest, mine);
       groups.put(m, i);
       if (!(highest > -INFINITY)) return;
-      const float E = ceilf(highest * scale);      // the chunk's weight in units of its own: the same in every batch
+      const float E = fmaxf(ceilf(highest * scale), -1e30f);     // the chunk's weight in units of its own
       float s = 0.f, g = 0.f;
 #pragma unroll
       for (int q = 0; q < 32; q += 4)
         s += (exp2_fast(fmaf(v[q], scale, -E)) + exp2_fast(fmaf(v[q + 1], scale, -E))) + (exp2_fast(fmaf(v[q + 2], scale, -E)) + exp2_fast(fmaf(v[q + 3], scale, -E)));
 #pragma unroll
       for (int q = 0; q < 4; ++q) g += exp2_fast(fmaf(m[q], scale, -E));
-      mass = add_mass(mass, Mass{s, g, E});
+      seen.add(s, g, E);
     });
   } else {
-    row.stream(every, [&](const float (&v)[32], int i) {
+    row.stream([&](const float (&v)[32], int i) {
       float m[4], mine;
-      look(v, m, i, mine);
+      look(row, v, i, m, mine, seen.top);
+      largest = fmaxf(largest, mine);
       if (!greedy) groups.put(m, i);
     });
   }
   c.ready();
   if (c.size > 1 && !greedy && !all)
-    for (int i = 0; i < c.size; ++i) c.of(parts.maxima, i)[c.rank * ROW_THREADS + t] = largest;
-  struct First { Best top; Mass mass; };
-  const First first = c.reduce(First{top, mass}, First{{-INFINITY, NO_ID}, NO_MASS}, [](First x, First y) { return First{first_of(x.top, y.top), add_mass(x.mass, y.mass)}; });
-  top = first.top;
+    for (int i = 0; i < c.size; ++i) c.of(parts.maxima, i)[c.rank * NT + t] = largest;
+  seen = row_seen(c, seen, sums, false);
+  const Best top = seen.top;
   const bool lead = c.rank == 0 && t == 0;
   // Greedy too: a best score beside which noise is nothing.
   if (greedy || top.v == -INFINITY || !(fabsf(__fdiv_rn(top.v, temp)) < 1073741824.f)) {
@@ -684,35 +778,30 @@ sample_kernel(const __grid_constant__ SampleRows a, int per) {
     c.sync();                                      // (what a CTA's shared memory holds stays until all have read it)
     return;
   }
+  if (all) {
+    const Win win = settle(row, c, race, whole_row(), racer.m);
+    if (lead) a.out[r] = win.id;
+    c.sync();
+    return;
+  }
   const bool far = !(fabsf(top.v * scale) < 1048576.f);
   const Weights weight = far ? Weights{scale, 0.f, top.v} : Weights{scale, ceilf(top.v * scale), 0.f};
-  Prefix kept = whole_row;
+  Prefix kept = whole_row();
   if (by_min) {
     if (t == 0) sh.z = min_p_logit(top.v, temp, mp);
     __syncthreads();
     kept.z = sh.z;
   }
-  const auto some = [&](int i) { return all || groups.reaches(i, kept.z); };
-  // Weight of what lies within a prefix, in units of 2^E.
-  const auto mass_of = [&](const Prefix& of) {
-    double s = 0;
-    row.stream([&](int i) { return groups.reaches(i, of.z); }, [&](const float (&v)[32], int i) {
-      float f = 0.f;
-#pragma unroll
-      for (int q = 0; q < 32; ++q) f += within(of, v[q], row.id(Row<T>::place(row.chunk0 + i, q, t & 31))) ? weight(v[q]) : 0.f;
-      s += f;
-    });
-    return c.reduce(s, 0.0, [](double x, double y) { return x + y; });
-  };
-  double total = sums && !far ? first.mass.s * pow2(first.mass.E - weight.E) : by_p && !by_k ? mass_of(kept) : 0;
+  double total = 0;
+  if (sums && !far) total = seen.s * pow2(seen.E - weight.E);
+  else if (by_p && !by_k) total = row_total(c, lap(row, groups, race, weight, kept).s);
   if (by_k || by_p) {
     unsigned n = LIST + 1;
     if (k <= LIST && !far) {
-      const double need = by_k ? k : p * total * (1 + 1.0 / 262144);
-      bins_of_threads<T>(sh, c, parts.maxima, largest, weight, kept.z, by_k, need);
+      const float need = by_k ? k : static_cast<float>(p * total * (1 + 1.0 / 262144));
+      bins_of_threads(sh, c, parts.maxima, largest, weight, kept.z, by_k, need);
       // (the groups' largest may have the weight that the threads' have not, and they are more than these)
-      if (sh.bin == BINS - 1 && (by_k || by_min || first.mass.g * pow2(first.mass.E - weight.E) >= need))
-        bins_of_groups(sh, c, groups, row.chunks, weight, kept.z, by_k, need);
+      if (sh.bin == BINS - 1 && (by_k || by_min || seen.g * pow2(seen.E - weight.E) >= need)) bins_of_groups(sh, c, groups, row.chunks, weight, kept.z, by_k, need);
       if (sh.bin < BINS - 1 || a.V <= LIST) n = gather(sh, c, row, parts, largest, fmaxf(kept.z, weight.edge(sh.bin)));
     }
     if (n <= LIST) {
@@ -721,7 +810,7 @@ sample_kernel(const __grid_constant__ SampleRows a, int per) {
       const auto whole = [&](u64 key) { return __float2ull_rn(weight(list_z(key)) * 1099511627776.f); };
       const unsigned n1 = by_k ? min(n, static_cast<unsigned>(k)) : n;
       int token;
-      if (n <= FEW) {
+      if (n <= NT / 2) {
         if (by_p) {
           if (t < n) sh.weight[t] = whole(sh.list[t]);
           __syncthreads();
@@ -734,18 +823,14 @@ sample_kernel(const __grid_constant__ SampleRows a, int per) {
           const double target = static_cast<double>(p) * (by_k ? static_cast<double>(sh.total) : total * 1099511627776.0);
           in = in && (e.rank == 0 || static_cast<double>(e.before) < target);
         }
-        token = draw_few(sh, c, race, e.key, in);
+        token = draw_listed(sh, c, race, [&](auto f) { if (in) f(e.key); });
       } else {
-        sort_list(sh, n);
+        sort_list<NT>(sh.list, n);
         unsigned m = n1;
         if (by_p) {
-          constexpr int PER = LIST / ROW_THREADS;
-          u64 w[PER], sum = 0;
-#pragma unroll
-          for (int i = 0; i < PER; ++i) {
-            w[i] = t * PER + i < n ? whole(sh.list[t * PER + i]) : 0;
-            sum += w[i];
-          }
+          constexpr int PER = LIST / NT;
+          u64 sum = 0;
+          for (int i = 0; i < PER; ++i) sum += t * PER + i < n ? whole(sh.list[t * PER + i]) : 0;
           u64 before = sum;
           const int lane = t & 31;
 #pragma unroll
@@ -759,100 +844,76 @@ sample_kernel(const __grid_constant__ SampleRows a, int per) {
           before -= sum;
           for (int i = 0; i < t >> 5; ++i) before += sh.wsum[i];
           u64 at = before;
-#pragma unroll
-          for (int i = 0; i < PER; ++i) {
-            at += w[i];
+          for (int i = 0; i < PER && t * PER + i < n1; ++i) {
+            at += whole(sh.list[t * PER + i]);
             if (t * PER + i + 1 == n1) sh.total = at;
           }
           __syncthreads();
           const double target = static_cast<double>(p) * (by_k ? static_cast<double>(sh.total) : total * 1099511627776.0);
           unsigned mine = 0;
           at = before;
-#pragma unroll
-          for (int i = 0; i < PER; ++i) {
-            const unsigned j = t * PER + i;
-            mine += j < n1 && (j == 0 || static_cast<double>(at) < target);
-            at += w[i];
+          for (int i = 0; i < PER && t * PER + i < n1; ++i) {
+            mine += t * PER + i == 0 || static_cast<double>(at) < target;
+            at += whole(sh.list[t * PER + i]);
           }
           if (mine) atomicAdd(&sh.kept, mine);
           __syncthreads();
           m = sh.kept;
           __syncthreads();
         }
-        token = draw_list(sh, c, race, m);
+        token = draw_listed(sh, c, race, [&](auto f) { for (unsigned i = t; i < m; i += NT) f(sh.list[i]); });
       }
       if (t == 0) a.out[r] = token;
       return;
     }
-    if (by_k) {
-      kept = kth_token(sh, row, groups, c, weight, kept, k, parts.inbox);
-      if (by_p) total = mass_of(kept);
-    }
+    if (by_k) kept = kth_token(sh, row, groups, c, weight, kept, k, parts.inbox);
   }
-  const auto largest_of = [](const float (&v)[32]) {
-    float m[4];
-    max8(v, m);
-    return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-  };
-  if (!all) row.stream(some, [&](const float (&v)[32], int i) { racer.run(race, row, v, largest_of(v), row.chunk0 + i, kept); });
-  Win win = settle(row, c, race, kept, racer.m, some);
-  const double target = by_p ? p * total : 0;
+  Lap l = lap(row, groups, race, weight, kept);
+  if (by_k && by_p) total = row_total(c, l.s);
+  Win win = settle(row, c, race, kept, l.m);
+  const double target = p * total;
   while (by_p && win.id != top.id) {               // what lies in front of it, and who wins there should that be too much
     const Prefix front{win.z, win.id - 1};
-    const auto there = [&](int i) { return groups.reaches(i, front.z); };
-    Racer next;
-    double s = 0;
-    row.stream(there, [&](const float (&v)[32], int i) {
-      float f = 0.f;
-#pragma unroll
-      for (int q = 0; q < 32; ++q) f += within(front, v[q], row.id(Row<T>::place(row.chunk0 + i, q, t & 31))) ? weight(v[q]) : 0.f;
-      s += f;
-      next.run(race, row, v, largest_of(v), row.chunk0 + i, front);
-    });
-    if (c.reduce(s, 0.0, [](double x, double y) { return x + y; }) < target) break;
-    win = settle(row, c, race, front, next.m, there);
+    l = lap(row, groups, race, weight, front);
+    if (row_total(c, l.s) < target) break;
+    win = settle(row, c, race, front, l.m);
   }
   if (lead) a.out[r] = win.id;
   c.sync();
 }
 
-template <class T>
-__global__ void __launch_bounds__(ROW_THREADS, 2)
+template <class T, int NT>
+__global__ void __launch_bounds__(NT, 1024 / NT)
 logprob_kernel(const __grid_constant__ LogprobRows a, int per) {
   extern __shared__ __align__(16) float smem[];
-  __shared__ RowShared sh;
+  __shared__ RowShared<NT> sh;
   pdl_wait();
   pdl_trigger();
   Cluster c(&sh.mail);
   const int tid = threadIdx.x, r = blockIdx.x / c.size;
   const T* x = static_cast<const T*>(a.x) + r * a.ldx;
   const int t = a.tokens[r];
-  const bool there = t >= 0 && t < a.V;
+  const bool there = t >= 0 && t < a.V, listing = a.top > 1;
   const float zt = there ? plain_logit(logit(x + t)) : -INFINITY;
-  const Row<T> row(x, a.V, c.rank, per);
-  const Parts parts = parts_of(smem, per, c.size);
-  const bool listing = a.top > 1;
+  const Row<T, NT> row(x, a.V, c.rank, per);
+  const Parts<NT> parts(smem, per, c.size);
   if (listing) {
     clear_bins(sh);
-    if (tid == 0) sh.n_list = 0;
+    if (tid == 0) sh.n_list = sh.n_hits = 0;
   }
   // log2(e) in two parts: z log2(e) - E as exact as its own size in fp32
   constexpr float HI = 1.4426950408889634f, LO = static_cast<float>(1.4426950408889634 - static_cast<double>(HI));
-  Best top{-INFINITY, NO_ID};
-  Mass mass = NO_MASS;
-  unsigned before = 0;
+  Seen seen;
   float largest = -INFINITY;                       // of the thread
   const int tj = t + row.lo;
-  row.stream([](int) { return true; }, [&](const float (&v)[32], int i) {
+  row.stream([&](const float (&v)[32], int i) {
     const int chunk = row.chunk0 + i;
-    float m[4];
-    max8(v, m);
-    const float mine = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), highest = warp_highest(mine);
-    note_best(row, v, mine, highest, chunk, top);
+    float m[4], mine;
+    const float highest = look(row, v, i, m, mine, seen.top);
     largest = fmaxf(largest, mine);
     if (listing) parts.groups.put(m, i);
-    if (highest > -INFINITY && highest < INFINITY) {           // the chunk's sum in units of its own: the same in every batch
-      const float E = ceilf(highest * HI);
+    if (highest > -INFINITY && highest < INFINITY) {           // the chunk's sum in units of its own
+      const float E = fmaxf(ceilf(highest * HI), -1e30f);
       float s = 0.f;
 #pragma unroll
       for (int q = 0; q < 32; q += 4) {
@@ -861,45 +922,40 @@ logprob_kernel(const __grid_constant__ LogprobRows a, int per) {
         for (int e = 0; e < 4; ++e) w[e] = exp2_fast(fmaf(v[q + e], LO, fmaf(v[q + e], HI, -E)));
         s += (w[0] + w[1]) + (w[2] + w[3]);
       }
-      mass = add_mass(mass, Mass{s, 0.0, E});
+      seen.add(s, 0.0, E);
     }
     if (zt == -INFINITY || (chunk * CHUNK <= tj && tj < (chunk + 1) * CHUNK)) {
 #pragma unroll
       for (int q = 0; q < 32; ++q) {
-        const int j = Row<T>::place(chunk, q, tid & 31);
-        before += v[q] > zt || (v[q] == zt && j < tj && j >= row.lo);
+        const int j = Row<T, NT>::place(chunk, q, tid & 31);
+        seen.n += v[q] > zt || (v[q] == zt && j < tj && j >= row.lo);
       }
     } else {                                                   // (equal ones are in front of it in the chunks in front of its own)
       const float least = (chunk + 1) * CHUNK <= tj ? zt : nextafterf(zt, INFINITY);
 #pragma unroll
-      for (int q = 0; q < 32; ++q) before += v[q] >= least;
+      for (int q = 0; q < 32; ++q) seen.n += v[q] >= least;
     }
   });
   c.ready();
   if (c.size > 1 && listing)
-    for (int i = 0; i < c.size; ++i) c.of(parts.maxima, i)[c.rank * ROW_THREADS + tid] = largest;
-  struct Sum { double s; float E; unsigned before; };
-  struct First { Best top; Sum sum; };
-  const First first = c.reduce(First{top, {mass.s, mass.E, before}}, First{{-INFINITY, NO_ID}, {0.0, LOWEST, 0}}, [](First p, First q) {
-    const Mass m = add_mass(Mass{p.sum.s, 0.0, p.sum.E}, Mass{q.sum.s, 0.0, q.sum.E});
-    return First{first_of(p.top, q.top), {m.s, m.E, p.sum.before + q.sum.before}};
-  });
-  top = first.top;
+    for (int i = 0; i < c.size; ++i) c.of(parts.maxima, i)[c.rank * NT + tid] = largest;
+  seen = row_seen(c, seen, true, true);
+  const Best top = seen.top;
   const bool lead = c.rank == 0 && tid == 0;
   // log-probabilities: z - (E log 2 + log(sum)); seen from the best where logits are so large that this would leave too few bits of it, or infinite
   const bool far = !(fabsf(top.v) < 1e6f);
-  double sum = first.sum.s;
+  double sum = seen.s;
   if (far) {
     sum = 0;
-    row.stream([](int) { return true; }, [&](const float (&v)[32], int) {
+    row.eights([](int) { return true; }, [&](const float (&v)[8], int, int) {
       float f = 0.f;
 #pragma unroll
-      for (int q = 0; q < 32; ++q) f += v[q] == top.v ? 1.f : exp2_fast((v[q] - top.v) * HI);
+      for (int q = 0; q < 8; ++q) f += v[q] == top.v ? 1.f : exp2_fast((v[q] - top.v) * HI);
       sum += f;
     });
-    sum = c.reduce(sum, 0.0, [](double p, double q) { return p + q; });
+    sum = row_total(c, sum);
   }
-  if (lead) sh.log = (far ? 0.0 : static_cast<double>(first.sum.E) * 0.69314718055994530942) + log(sum);
+  if (lead) sh.log = (far ? 0.0 : static_cast<double>(seen.E) * 0.69314718055994530942) + log(sum);
   const auto lp = [&](float z) {
     if (z == -INFINITY) return -INFINITY;
     return static_cast<float>((far ? (z == top.v ? 0.0 : static_cast<double>(z) - top.v) : static_cast<double>(z)) - sh.log);
@@ -908,7 +964,7 @@ logprob_kernel(const __grid_constant__ LogprobRows a, int per) {
   float* lps = a.logprobs + static_cast<long long>(r) * a.top;
   if (lead) {
     a.logprob[r] = lp(zt);
-    a.rank[r] = there ? static_cast<int>(first.sum.before) + 1 : 0;
+    a.rank[r] = there ? static_cast<int>(seen.n) + 1 : 0;
     if (a.top == 1) {
       ids[0] = top.v == -INFINITY ? -1 : top.id;
       lps[0] = lp(top.v);
@@ -917,32 +973,32 @@ logprob_kernel(const __grid_constant__ LogprobRows a, int per) {
   if (a.top < 2) { c.sync(); return; }
   if (!far) {
     const Weights w{HI, ceilf(top.v * HI), 0.f};
-    bins_of_threads<T>(sh, c, parts.maxima, largest, w, LOWEST, true, a.top);
+    bins_of_threads(sh, c, parts.maxima, largest, w, LOWEST, true, a.top);
     if (sh.bin == BINS - 1) bins_of_groups(sh, c, parts.groups, row.chunks, w, LOWEST, true, a.top);
     unsigned n = LIST + 1;
     if (sh.bin < BINS - 1 || a.V <= LIST) n = gather(sh, c, row, parts, largest, w.edge(sh.bin));
     if (n <= LIST) {
       if (c.rank) return;
       const auto put = [&](unsigned i, u64 key) { ids[i] = list_id(key); lps[i] = lp(list_z(key)); };
-      if (n <= FEW) {
+      if (n <= NT / 2) {
         const Counted e = count_list(sh, n, false);
-        if (e.mine && e.rank < a.top) put(e.rank, e.key);
+        if (e.mine && e.rank < static_cast<unsigned>(a.top)) put(e.rank, e.key);
       } else {
-        sort_list(sh, n);
-        for (unsigned i = tid; i < min(n, static_cast<unsigned>(a.top)); i += ROW_THREADS) put(i, sh.list[i]);
+        sort_list<NT>(sh.list, n);
+        for (unsigned i = tid; i < min(n, static_cast<unsigned>(a.top)); i += NT) put(i, sh.list[i]);
       }
-      for (unsigned i = n + tid; i < a.top; i += ROW_THREADS) { ids[i] = -1; lps[i] = -INFINITY; }
+      for (unsigned i = n + tid; i < static_cast<unsigned>(a.top); i += NT) { ids[i] = -1; lps[i] = -INFINITY; }
       return;
     }
   }
   Best last{INFINITY, -1};                         // one after the other: rows of nothing, of infinities, of very many equal logits
   for (int i = 0; i < a.top; ++i) {
     Best g{-INFINITY, NO_ID};
-    row.stream([](int) { return true; }, [&](const float (&v)[32], int n) {
+    row.eights([](int) { return true; }, [&](const float (&v)[8], int n, int q) {
 #pragma unroll
-      for (int q = 0; q < 32; ++q) {
-        const int id = row.id(Row<T>::place(row.chunk0 + n, q, tid & 31));
-        if (v[q] < last.v || (v[q] == last.v && id > last.id)) g = first_of(g, Best{v[q], id});
+      for (int e = 0; e < 8; ++e) {
+        const int id = row.id(Row<T, NT>::place(row.chunk0 + n, q + e, tid & 31));
+        if (v[e] < last.v || (v[e] == last.v && id > last.id)) g = first_of(g, Best{v[e], id});
       }
     });
     last = c.reduce(g, Best{-INFINITY, NO_ID}, first_of);
@@ -961,12 +1017,23 @@ static int row_cluster(int R, int chunks, int sms) {
   return c;
 }
 
-template <class A, class K>
-static int launch_rows(const char* name, K kern, const A& a, cudaStream_t s) {
-  const int chunks = (a.V + 8 + CHUNK - 1) / CHUNK, c = row_cluster(a.R, chunks, a.sms), per = (chunks + c - 1) / c, bytes = part_bytes(per, c);
+template <int NT, class A, class K>
+static int launch_rows(const char* name, K kern, const A& a, int chunks, cudaStream_t s) {
+  const int c = row_cluster(a.R, chunks, a.sms), per = (chunks + c - 1) / c, bytes = Parts<NT>::bytes(per, c);
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return spark_launch_rc(name);
-  spark_launch_pdl(kern, dim3(a.R * c), dim3(ROW_THREADS), bytes, s, dim3(c, 1, 1), a, per);
+  spark_launch_pdl(kern, dim3(a.R * c), dim3(NT), bytes, s, dim3(c, 1, 1), a, per);
   return spark_launch_rc(name);
+}
+// Rows of a few chunks take CTAs of four warps.
+template <class T>
+static int sample_rows(const SampleRows& a, cudaStream_t s) {
+  const int chunks = (a.V + 8 + CHUNK - 1) / CHUNK;
+  return chunks <= 8 ? launch_rows<128>("spark_sample_rows", sample_kernel<T, 128>, a, chunks, s) : launch_rows<512>("spark_sample_rows", sample_kernel<T, 512>, a, chunks, s);
+}
+template <class T>
+static int logprob_rows(const LogprobRows& a, cudaStream_t s) {
+  const int chunks = (a.V + 8 + CHUNK - 1) / CHUNK;
+  return chunks <= 8 ? launch_rows<128>("spark_logprob_rows", logprob_kernel<T, 128>, a, chunks, s) : launch_rows<512>("spark_logprob_rows", logprob_kernel<T, 512>, a, chunks, s);
 }
 
 }  // namespace spark
@@ -975,14 +1042,10 @@ using namespace spark;
 
 extern "C" int spark_sample_rows(const SampleRows* a, cudaStream_t s) {
   if (a->R <= 0 || a->V <= 0) return 0;
-  if (a->type == LT_F32) return launch_rows("spark_sample_rows", sample_kernel<float>, *a, s);
-  if (a->type == LT_BF16) return launch_rows("spark_sample_rows", sample_kernel<__nv_bfloat16>, *a, s);
-  return launch_rows("spark_sample_rows", sample_kernel<__half>, *a, s);
+  return a->type == LT_F32 ? sample_rows<float>(*a, s) : a->type == LT_BF16 ? sample_rows<__nv_bfloat16>(*a, s) : sample_rows<__half>(*a, s);
 }
 
 extern "C" int spark_logprob_rows(const LogprobRows* a, cudaStream_t s) {
   if (a->R <= 0 || a->V <= 0) return 0;
-  if (a->type == LT_F32) return launch_rows("spark_logprob_rows", logprob_kernel<float>, *a, s);
-  if (a->type == LT_BF16) return launch_rows("spark_logprob_rows", logprob_kernel<__nv_bfloat16>, *a, s);
-  return launch_rows("spark_logprob_rows", logprob_kernel<__half>, *a, s);
+  return a->type == LT_F32 ? logprob_rows<float>(*a, s) : a->type == LT_BF16 ? logprob_rows<__nv_bfloat16>(*a, s) : logprob_rows<__half>(*a, s);
 }

@@ -305,3 +305,26 @@ def test_strided_and_transposed_logits():
     one = torch.randn(1, 500, device="cuda").expand(40, 500)             # the same row again and again
     r = ops.token_logprobs(one, torch.arange(40, dtype=torch.int32, device="cuda"), 1)
     assert len(set(r.ids[:, 0].tolist())) == 1 and len(set(r.rank.tolist())) == 40
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("V", [700, 9000, 60000])
+def test_masks_of_the_lowest_value(V, dtype):
+    """Most of a row (whole stretches of it) masked by the type's lowest finite value, which is a token, if an improbable one."""
+    rows = Rows(6, V, "flat", TYPES[dtype], seed=V, device="cuda")
+    low = torch.finfo(TYPES[dtype]).min
+    x = rows.logits.clone()
+    x[:, V // 100: -5] = low
+    x[1] = low
+    x[2, 1:] = low
+    rows.logits, rows.z = x, x.float().cpu().numpy()
+    for s in (dict(), dict(top_k=30), dict(top_p=0.7), dict(min_p=0.05), dict(top_k=V - 1, top_p=0.9), dict(top_p=0.999, min_p=0.001)):
+        assert np.array_equal(rows.draw(0.8, **s), rows.want(0.8, **s)), s
+    t = rows.rs.randint(0, V, 6)
+    got = [y.cpu().numpy() for y in ops.token_logprobs(rows.logits, rows.t(t, torch.int32), 5)]
+    for r in range(6):
+        lp, rank, ids, lps = want_logprobs(rows.z[r], int(t[r]), 5)
+        assert got[1][r] == rank and got[2][r].tolist() == [int(i) for i in ids]
+        near(np.maximum(got[0][r: r + 1], -3e38), np.maximum([lp], -3e38))
+        near(np.maximum(got[3][r], -3e38), np.maximum(lps, -3e38))
+    _sound()
