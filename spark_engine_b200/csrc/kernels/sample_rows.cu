@@ -139,6 +139,8 @@ struct Row {
   __device__ __forceinline__ void stream(F f) const {
     for (int k = threadIdx.x >> 5; k < chunks; k += WARPS) {
       float v[32];
+      const int ahead = (chunk0 + k + 2 * WARPS) * CHUNK + (threadIdx.x & 31) * 32;         // (a lane: 128 bytes of fp32)
+      if (k + 2 * WARPS < chunks && ahead < hi) asm volatile("prefetch.global.L2 [%0];" ::"l"(base + ahead));
       load(chunk0 + k, 0, threadIdx.x & 31, v);
       f(v, k);
     }
@@ -561,13 +563,15 @@ struct Racer {
       x = (x ^ (x >> 30)) * 0xBF58476D1CE4E5B9ull;
       x = (x ^ (x >> 27)) * 0x94D049BB133111EBull;
       const uint32_t hi = static_cast<uint32_t>(x >> 32), rest = ~(hi ^ (hi >> 31));
-      if (within(kept, v[i], id0 + d) && !(static_cast<float>(rest) > exp2_fast(fmaf(v[i], race.c, off)))) near |= 1u << i;
+      if (v[i] >= kept.z && static_cast<float>(rest) <= exp2_fast(fmaf(v[i], race.c, off))) near |= 1u << i;
     }
     bool more = false;
     while (near) {
       const int i = __ffs(near) - 1, j = j0 + i / R::N * (32 * R::N) + i % R::N;
       near &= near - 1;
-      const float z = row.one(j), y = race.rough(z, row.id(j));
+      const float z = row.one(j);
+      if (!within(kept, z, row.id(j))) continue;
+      const float y = race.rough(z, row.id(j));
       m = best2(m, Top2{y, row.id(j), -INFINITY, z});
       more |= y > bound;
     }
@@ -577,7 +581,7 @@ struct Racer {
 
 // A race over what lies within `front`, and the weight of that.
 struct Lap { Top2 m; double s; };
-template <class T, int NT>
+template <bool RACE, bool MASS, class T, int NT>
 __device__ __noinline__ Lap lap(const Row<T, NT> row, const Groups groups, const Race race, const Weights w, const Prefix front) {
   Racer racer;
   double s = 0;
@@ -585,11 +589,22 @@ __device__ __noinline__ Lap lap(const Row<T, NT> row, const Groups groups, const
     const int chunk = row.chunk0 + k;
     const float mine = max8(v);
     if (__all_sync(0xffffffffu, !(mine >= front.z))) return;
-    float f[8];
+    if (MASS) {
+      float f[8];
+      bool last = false;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = within(front, v[i], row.id(Row<T, NT>::place(chunk, q + i, threadIdx.x & 31))) ? w(v[i]) : 0.f;
-    s += ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
-    if (racer.bound > -INFINITY || racer.begin(race, row, v, mine, chunk, q, front)) racer.run(race, row, v, chunk, q, front);
+      for (int i = 0; i < 8; ++i) {
+        f[i] = v[i] > front.z ? w(v[i]) : 0.f;
+        last |= v[i] == front.z;
+      }
+      if (last) {                                  // as the last token of it: by their ids
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (v[i] == front.z && row.id(Row<T, NT>::place(chunk, q + i, threadIdx.x & 31)) <= front.id) f[i] = w(v[i]);
+      }
+      s += ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
+    }
+    if (RACE && (racer.bound > -INFINITY || racer.begin(race, row, v, mine, chunk, q, front))) racer.run(race, row, v, chunk, q, front);
   });
   return Lap{racer.m, s};
 }
@@ -794,7 +809,7 @@ sample_kernel(const __grid_constant__ SampleRows a, int per) {
   }
   double total = 0;
   if (sums && !far) total = seen.s * pow2(seen.E - weight.E);
-  else if (by_p && !by_k) total = row_total(c, lap(row, groups, race, weight, kept).s);
+  else if (by_p && !by_k) total = row_total(c, lap<false, true>(row, groups, race, weight, kept).s);
   if (by_k || by_p) {
     unsigned n = LIST + 1;
     if (k <= LIST && !far) {
@@ -868,13 +883,13 @@ sample_kernel(const __grid_constant__ SampleRows a, int per) {
     }
     if (by_k) kept = kth_token(sh, row, groups, c, weight, kept, k, parts.inbox);
   }
-  Lap l = lap(row, groups, race, weight, kept);
+  Lap l = by_k && by_p ? lap<true, true>(row, groups, race, weight, kept) : lap<true, false>(row, groups, race, weight, kept);
   if (by_k && by_p) total = row_total(c, l.s);
   Win win = settle(row, c, race, kept, l.m);
   const double target = p * total;
   while (by_p && win.id != top.id) {               // what lies in front of it, and who wins there should that be too much
     const Prefix front{win.z, win.id - 1};
-    l = lap(row, groups, race, weight, front);
+    l = lap<true, true>(row, groups, race, weight, front);
     if (row_total(c, l.s) < target) break;
     win = settle(row, c, race, front, l.m);
   }

@@ -11,6 +11,8 @@ namespace spark {
 // Integer additions and the prompt's bit: the order of the atomics changes nothing.
 __global__ void __launch_bounds__(256)
 count_more_kernel(const __grid_constant__ CountTokens a) {
+  pdl_wait();
+  pdl_trigger();
   const int s = blockIdx.y, i = blockIdx.x * 256 + threadIdx.x;
   const int n = min(a.n[s], a.P);
   const int slot = a.slots ? a.slots[s] : s;
@@ -24,52 +26,126 @@ count_more_kernel(const __grid_constant__ CountTokens a) {
 }
 
 // A request's row is written whole: a CTA has a slice of the vocabulary in shared memory, marks it by the tokens that fall into it and writes it out.
-constexpr int COUNT_SLICE = 24576;
-__global__ void __launch_bounds__(512)
+constexpr int COUNT_SLICE = 24576, COUNT_THREADS = 1024;
+__global__ void __launch_bounds__(COUNT_THREADS)
 count_anew_kernel(const __grid_constant__ CountTokens a) {
   extern __shared__ __align__(16) int slice[];
-  const int s = blockIdx.y, b = blockIdx.x * COUNT_SLICE, len = min(COUNT_SLICE, a.V - b);
+  pdl_wait();
+  pdl_trigger();
+  const int s = blockIdx.y, b = blockIdx.x * COUNT_SLICE, len = min(COUNT_SLICE, a.V - b), t0 = threadIdx.x;
   const int slot = a.slots ? a.slots[s] : s;
   if (slot < 0) return;
   if (slot >= a.n_slots) { set_status(a.status, ST_BOUNDS, s, slot, a.n_slots); return; }
-  for (int i = threadIdx.x; i < len; i += 512) slice[i] = 0;
+  for (int i = t0; i < (len + 3) / 4; i += COUNT_THREADS) reinterpret_cast<int4*>(slice)[i] = make_int4(0, 0, 0, 0);
   __syncthreads();
   const int n = min(a.n[s], a.P);
   const int* tok = a.tokens + s * a.ld_tokens;
-  for (int i = threadIdx.x; i < n; i += 512) {
-    const int t = tok[i] - b;
-    if (t < 0 || t >= len) continue;
-    if (a.prompt) slice[t] = 1;
+  const auto mark = [&](int t) {
+    t -= b;
+    if (t < 0 || t >= len) return;
+    if (a.prompt) slice[t] = 1;                    // (whoever writes it)
     else atomicAdd(&slice[t], 2);
+  };
+  int done = 0;
+  if ((reinterpret_cast<uintptr_t>(tok) & 15) == 0) {
+    constexpr int U = 4;
+    const int whole = n / 4;
+    for (int i = t0; i < whole; i += U * COUNT_THREADS) {
+      int4 q[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) q[u] = i + u * COUNT_THREADS < whole ? __ldg(reinterpret_cast<const int4*>(tok) + i + u * COUNT_THREADS) : make_int4(-1, -1, -1, -1);
+#pragma unroll
+      for (int u = 0; u < U; ++u) { mark(q[u].x); mark(q[u].y); mark(q[u].z); mark(q[u].w); }
+    }
+    done = max(whole, 0) * 4;
   }
+  for (int i = done + t0; i < n; i += COUNT_THREADS) mark(__ldg(tok + i));
   __syncthreads();
   int* out = a.counts + slot * a.ld_counts + b;
-  for (int i = threadIdx.x; i < len; i += 512) out[i] = slice[i];
+  done = 0;
+  if ((reinterpret_cast<uintptr_t>(out) & 15) == 0) {
+    for (int i = t0; i < len / 4; i += COUNT_THREADS) reinterpret_cast<int4*>(out)[i] = reinterpret_cast<const int4*>(slice)[i];
+    done = len / 4 * 4;
+  }
+  for (int i = done + t0; i < len; i += COUNT_THREADS) out[i] = slice[i];
 }
 
 // ------------------------------------------------------------------------------------------------ adjustments
 
-constexpr int ADJUST_COLS = 4096;
+// Four columns of 16 or 8 bytes.
+__device__ __forceinline__ float4 four(const float* p) { return *reinterpret_cast<const float4*>(p); }
+template <class H>
+__device__ __forceinline__ float4 four(const H* p) {
+  const uint2 q = *reinterpret_cast<const uint2*>(p);
+  const H* a = reinterpret_cast<const H*>(&q.x);
+  const H* b = reinterpret_cast<const H*>(&q.y);
+  return make_float4(logit(a), logit(a + 1), logit(b), logit(b + 1));
+}
+
+// A CTA has ADJUST_COLS columns of a row: first all of them as if nothing were drafted and no bias given, then those in the lists again, by what they were.
+constexpr int ADJUST_THREADS = 256, ADJUST_COLS = ADJUST_THREADS * 16;
 template <class T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(ADJUST_THREADS)
 adjust_rows_kernel(const __grid_constant__ AdjustRows a) {
   extern __shared__ int ids[];                     // the lists' entries, then the logits of those in this CTA's columns
-  const int r = blockIdx.y, b = blockIdx.x * ADJUST_COLS, e = min(b + ADJUST_COLS, a.V);
+  pdl_wait();
+  pdl_trigger();
+  const int r = blockIdx.y, b = blockIdx.x * ADJUST_COLS, e = min(b + ADJUST_COLS, a.V), t = threadIdx.x;
   const RowAdjust adj(a.a, r, a.status);
   const T* x = static_cast<const T*>(a.x) + r * a.ldx;
   float* out = a.out + r * a.ldo;
   const int n = adj.entries();
   float* was = reinterpret_cast<float*>(ids + n);
-  for (int i = threadIdx.x; i < n; i += 256) {     // (read before they are written: `out` may be the logits)
+  bool mine = false;                               // whether any of the thread's entries is of these columns
+  for (int i = t; i < n; i += ADJUST_THREADS) {    // (read before they are written: `out` may be the logits)
     const int id = adj.entry(i), col = id < 0 ? -1 : id - a.offset;
     ids[i] = id;
-    if (col >= b && col < e) was[i] = logit(x + col);
+    if (col >= b && col < e) { was[i] = logit(x + col); mine = true; }
   }
+  const bool any = n && __syncthreads_or(mine);
+  const uintptr_t places = reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(adj.counts) | reinterpret_cast<uintptr_t>(x) * (4 / sizeof(T));
+  if ((places & 15) == 0) {
+    constexpr int U = ADJUST_COLS / ADJUST_THREADS / 4;
+    float4 z[U];
+    int4 c[U];
+    uint32_t bits[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int col = b + (u * ADJUST_THREADS + t) * 4;
+      if (col + 4 > e) continue;
+      z[u] = four(x + col);
+      c[u] = adj.counts ? __ldg(reinterpret_cast<const int4*>(adj.counts + col)) : make_int4(0, 0, 0, 0);
+      bits[u] = adj.allowed ? __ldg(adj.allowed + (col >> 5)) >> (col & 31) : 15u;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int col = b + (u * ADJUST_THREADS + t) * 4;
+      if (col + 4 > e) {
+        for (int i = col; i < e; ++i) out[i] = adj.common(logit(x + i), i);
+        continue;
+      }
+      float4 y = make_float4(adj.penalised(z[u].x, c[u].x, 0), adj.penalised(z[u].y, c[u].y, 0), adj.penalised(z[u].z, c[u].z, 0), adj.penalised(z[u].w, c[u].w, 0));
+      if (!(bits[u] & 1)) y.x = -INFINITY;
+      if (!(bits[u] & 2)) y.y = -INFINITY;
+      if (!(bits[u] & 4)) y.z = -INFINITY;
+      if (!(bits[u] & 8)) y.w = -INFINITY;
+      *reinterpret_cast<float4*>(out + col) = y;
+    }
+  } else {
+    constexpr int U = 4;
+    for (int col = b + t; col < e; col += U * ADJUST_THREADS) {
+      float z[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (col + u * ADJUST_THREADS < e) z[u] = logit(x + col + u * ADJUST_THREADS);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (col + u * ADJUST_THREADS < e) out[col + u * ADJUST_THREADS] = adj.common(z[u], col + u * ADJUST_THREADS);
+    }
+  }
+  if (!any) return;
   __syncthreads();
-  for (int col = b + threadIdx.x; col < e; col += 256) out[col] = adj.common(logit(x + col), col);
-  if (!n) return;
-  __syncthreads();
-  for (int i = threadIdx.x; i < n; i += 256) {
+  for (int i = t; i < n; i += ADJUST_THREADS) {
     const int col = ids[i] < 0 ? -1 : ids[i] - a.offset;
     float y;
     if (col >= b && col < e && adj.listed(i, ids, col, was[i], y)) out[col] = y;
@@ -87,19 +163,19 @@ extern "C" int spark_count_tokens(const CountTokens* a, cudaStream_t s) {
   if (a->reset) {
     constexpr int bytes = COUNT_SLICE * 4;
     if (cudaFuncSetAttribute(count_anew_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return spark_launch_rc("spark_count_tokens");
-    count_anew_kernel<<<dim3((a->V + COUNT_SLICE - 1) / COUNT_SLICE, a->S), 512, bytes, s>>>(*a);
+    spark_launch_pdl(count_anew_kernel, dim3((a->V + COUNT_SLICE - 1) / COUNT_SLICE, a->S), dim3(COUNT_THREADS), bytes, s, dim3(1, 1, 1), *a);
   } else if (a->P > 0) {
-    count_more_kernel<<<dim3((a->P + 255) / 256, a->S), 256, 0, s>>>(*a);
+    spark_launch_pdl(count_more_kernel, dim3((a->P + 255) / 256, a->S), dim3(256), 0, s, dim3(1, 1, 1), *a);
   }
   return spark_launch_rc("spark_count_tokens");
 }
 
 extern "C" int spark_adjust_rows(const AdjustRows* a, cudaStream_t s) {
   if (a->R <= 0 || a->V <= 0) return 0;
-  const dim3 grid((a->V + ADJUST_COLS - 1) / ADJUST_COLS, a->R);
+  const dim3 grid((a->V + ADJUST_COLS - 1) / ADJUST_COLS, a->R), block(ADJUST_THREADS), one(1, 1, 1);
   const int sm = (a->a.n_drafted + a->a.n_bias) * 8;
-  if (a->type == LT_F32) adjust_rows_kernel<float><<<grid, 256, sm, s>>>(*a);
-  else if (a->type == LT_BF16) adjust_rows_kernel<__nv_bfloat16><<<grid, 256, sm, s>>>(*a);
-  else adjust_rows_kernel<__half><<<grid, 256, sm, s>>>(*a);
+  if (a->type == LT_F32) spark_launch_pdl(adjust_rows_kernel<float>, grid, block, sm, s, one, *a);
+  else if (a->type == LT_BF16) spark_launch_pdl(adjust_rows_kernel<__nv_bfloat16>, grid, block, sm, s, one, *a);
+  else spark_launch_pdl(adjust_rows_kernel<__half>, grid, block, sm, s, one, *a);
   return spark_launch_rc("spark_adjust_rows");
 }
