@@ -69,7 +69,7 @@ struct RowShared {
   u64 list[LIST], weight[NT / 2], wsum[NT / 32];
   float fsum[NT / 32];
   unsigned n_list, n_hits, before, kept;
-  int bin;
+  int bin, score;
   float z;
   double log;
   Prefix cut;
@@ -475,14 +475,18 @@ __device__ __forceinline__ unsigned gather(RowShared<NT>& sh, Cluster& c, const 
         if (v[e] >= least) to_list(sh, v[e], row.id(Row<T, NT>::place(chunk, from + q + e, i & 31)));
     }
   };
-  if (mine >= least)
+  if (__any_sync(0xffffffffu, mine >= least))
     for (int k = threadIdx.x >> 5; k < row.chunks; k += NT / 32)
       for (int q = 0; q < per; ++q) {
         const int i = (k * per + q) * 32 + lane;
-        if (!(parts.groups.g[i] >= least)) continue;
-        const unsigned at = atomicAdd(&sh.n_hits, 1u);
-        if (at < HITS) sh.hits[at] = i;
-        else read(i);
+        const bool hit = parts.groups.g[i] >= least;
+        const unsigned who = __ballot_sync(0xffffffffu, hit);
+        if (!who) continue;
+        unsigned at = 0;
+        if (lane == 0) at = atomicAdd(&sh.n_hits, __popc(who));
+        at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1));
+        if (hit && at < HITS) sh.hits[at] = i;
+        else if (hit) read(i);
       }
   __syncthreads();
   for (unsigned h = threadIdx.x; h < min(sh.n_hits, static_cast<unsigned>(HITS)); h += NT) read(sh.hits[h]);
@@ -529,8 +533,13 @@ struct Race {
   static __device__ __forceinline__ float margin(float score) { return 1.f / 512 + (fabsf(score) + 128.f) * (1.f / 524288); }
 };
 
+// Scores as whole numbers of the same order.
+__device__ __forceinline__ int score_key(float v) { const int b = __float_as_int(v); return b ^ (b >> 31 & 0x7fffffff); }
+__device__ __forceinline__ float key_score(int k) { return __int_as_float(k ^ (k >> 31 & 0x7fffffff)); }
+
 // A warp's race over the logits that come by.  -log u >= 1 - u, so that a score is at most z / T - log(1 - u): most tokens are out of it by the 32
-// upper bits of their hash, without a logarithm.
+// upper bits of their hash, without a logarithm.  `shared`: the best score that any warp of the CTA knows of, which spares the others the look at tokens
+// that do not come near it; who wins does not depend on when they see it.
 struct Racer {
   Top2 m = no_top();
   float bound = -INFINITY, off = 0.f;              // the best score so far, and what it takes to come near it
@@ -538,9 +547,16 @@ struct Racer {
     bound = b;
     off = (Race::margin(b) - b) * 1.4426950408889634f + 32.f;
   }
+  __device__ __forceinline__ void tell(int* shared) const {
+    if ((threadIdx.x & 31) == 0) atomicMax(shared, score_key(bound));
+  }
+  __device__ __forceinline__ void hear(const int* shared) {
+    const float b = key_score(*static_cast<const volatile int*>(shared));
+    if (b > bound) raise(b);                       // (each lane for itself)
+  }
   // The lanes' largest logits raise the bound before all others come; false where none of them is within `kept`, and no other then.
   template <int M, class R>
-  __device__ __forceinline__ bool begin(const Race& race, const R& row, const float (&v)[M], float mine, int chunk, int from, const Prefix& kept) {
+  __device__ __forceinline__ bool begin(const Race& race, const R& row, const float (&v)[M], float mine, int chunk, int from, const Prefix& kept, int* shared) {
     int j = 0;
 #pragma unroll
     for (int i = M - 1; i >= 0; --i)
@@ -548,22 +564,25 @@ struct Racer {
     const float b = warp_highest(within(kept, mine, row.id(j)) ? race.rough(mine, row.id(j)) : -INFINITY);
     if (b == -INFINITY) return false;
     raise(b);
+    tell(shared);
     return true;
   }
-  // Eight values of the lane, from value `from` of the chunk on.
-  template <class R>
-  __device__ __forceinline__ void run(const Race& race, const R& row, const float* v, int chunk, int from, const Prefix& kept) {
+  // Eight values of the lane, from value `from` of the chunk on.  The hash's last step changes the lowest of its 32 upper bits at most: one is added to
+  // what may come near instead.
+  template <bool ALL, class R>
+  __device__ __forceinline__ void run(const Race& race, const R& row, const float* v, int chunk, int from, const Prefix& kept, int* shared) {
     const int j0 = R::place(chunk, from, threadIdx.x & 31), id0 = row.id(j0);
     const u64 first = static_cast<u64>(static_cast<long long>(id0)) * Race::STEP + race.key;
     unsigned near = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int d = i / R::N * (32 * R::N) + i % R::N;
-      u64 x = first + static_cast<u64>(d) * Race::STEP;
+      u64 x = first + static_cast<u64>(i / R::N * (32 * R::N) + i % R::N) * Race::STEP;
       x = (x ^ (x >> 30)) * 0xBF58476D1CE4E5B9ull;
-      x = (x ^ (x >> 27)) * 0x94D049BB133111EBull;
-      const uint32_t hi = static_cast<uint32_t>(x >> 32), rest = ~(hi ^ (hi >> 31));
-      if (v[i] >= kept.z && static_cast<float>(rest) <= exp2_fast(fmaf(v[i], race.c, off))) near |= 1u << i;
+      x ^= x >> 27;
+      const uint32_t lo = static_cast<uint32_t>(x), hi = static_cast<uint32_t>(x >> 32);
+      const uint32_t rest = ~(__umulhi(lo, 0x133111EBu) + lo * 0x94D049BBu + hi * 0x133111EBu);
+      const bool in = ALL || v[i] >= kept.z;
+      if (static_cast<float>(rest) <= exp2_fast(fmaf(v[i], race.c, off)) + 1.f && in) near |= 1u << i;
     }
     bool more = false;
     while (near) {
@@ -575,14 +594,18 @@ struct Racer {
       m = best2(m, Top2{y, row.id(j), -INFINITY, z});
       more |= y > bound;
     }
-    if (__any_sync(0xffffffffu, more)) raise(fmaxf(bound, warp_highest(m.a1)));
+    if (__any_sync(0xffffffffu, more)) {
+      raise(fmaxf(bound, warp_highest(m.a1)));
+      tell(shared);
+    }
+    hear(shared);
   }
 };
 
 // A race over what lies within `front`, and the weight of that.
 struct Lap { Top2 m; double s; };
 template <bool RACE, bool MASS, class T, int NT>
-__device__ __noinline__ Lap lap(const Row<T, NT> row, const Groups groups, const Race race, const Weights w, const Prefix front) {
+__device__ __noinline__ Lap lap(const Row<T, NT> row, const Groups groups, const Race race, const Weights w, const Prefix front, int* shared) {
   Racer racer;
   double s = 0;
   row.eights([&](int k) { return groups.reaches(k, front.z); }, [&](const float (&v)[8], int k, int q) {
@@ -604,7 +627,8 @@ __device__ __noinline__ Lap lap(const Row<T, NT> row, const Groups groups, const
       }
       s += ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
     }
-    if (RACE && (racer.bound > -INFINITY || racer.begin(race, row, v, mine, chunk, q, front))) racer.run(race, row, v, chunk, q, front);
+    if (RACE && (__any_sync(0xffffffffu, racer.bound > -INFINITY) || racer.begin(race, row, v, mine, chunk, q, front, shared)))
+      racer.template run<false>(race, row, v, chunk, q, front, shared);
   });
   return Lap{racer.m, s};
 }
@@ -682,14 +706,20 @@ __device__ __noinline__ Prefix kth_by_bits(const Row<T, NT> row, Cluster& c, con
 template <class T, int NT>
 __device__ __noinline__ Prefix kth_token(RowShared<NT>& sh, const Row<T, NT> row, const Groups groups, Cluster& c, const Weights w, const Prefix of, unsigned k, u64* inbox) {
   c.sync();                                        // (nobody reads the bins and lists of before any more)
-  clear_bins(sh);
+  // four sets of bins where the list will be, each for a fourth of the lanes: most tokens of a flat row fall into few bins
+  unsigned* sets = reinterpret_cast<unsigned*>(sh.list);
+  static_assert(4 * BINS * sizeof(unsigned) <= LIST * sizeof(u64), "sets of bins");
+  for (int i = threadIdx.x; i < 4 * BINS; i += NT) sets[i] = 0;
   if (threadIdx.x == 0) sh.n_list = 0;
   __syncthreads();
+  unsigned* mine = sets + (threadIdx.x & 3) * BINS;
   row.eights([&](int i) { return groups.reaches(i, of.z); }, [&](const float (&v)[8], int, int) {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (v[i] >= of.z) atomicAdd(&sh.hist[w.bin(v[i])], 1u);
+      if (v[i] >= of.z) atomicAdd(&mine[w.bin(v[i])], 1u);
   });
+  __syncthreads();
+  for (int i = threadIdx.x; i < BINS; i += NT) sh.hist[i] = (sets[i] + sets[BINS + i]) + (sets[2 * BINS + i] + sets[3 * BINS + i]);
   c.sync();
   find_bin(sh, c, true, true, k);
   const int bin = sh.bin;
@@ -743,7 +773,8 @@ sample_kernel(const __grid_constant__ SampleRows a, int per) {
   const float scale = greedy ? 0.f : fmaxf(fminf(__fdiv_rn(1.4426950408889634f, temp), -LOWEST), 1e-44f);
   const Race race(temp, scale, a.seeds[r], a.positions[r]);
   clear_bins(sh);
-  if (t == 0) sh.n_list = sh.n_hits = 0;
+  if (t == 0) { sh.n_list = sh.n_hits = 0; sh.score = score_key(-INFINITY); }
+  if (all) __syncthreads();
 
   Seen seen;
   Racer racer;
@@ -753,9 +784,9 @@ sample_kernel(const __grid_constant__ SampleRows a, int per) {
       float m[4], mine;
       const float highest = look(row, v, i, m, mine, seen.top);
       if (!(highest > -INFINITY && highest < INFINITY)) return;
-      if (racer.bound == -INFINITY) racer.begin(race, row, v, mine, row.chunk0 + i, 0, whole_row());
+      if (racer.bound == -INFINITY) racer.begin(race, row, v, mine, row.chunk0 + i, 0, whole_row(), &sh.score);
 #pragma unroll
-      for (int q = 0; q < 32; q += 8) racer.run(race, row, v + q, row.chunk0 + i, q, whole_row());
+      for (int q = 0; q < 32; q += 8) racer.template run<true>(race, row, v + q, row.chunk0 + i, q, whole_row(), &sh.score);
     });
   } else if (sums) {
     row.stream([&](const float (&v)[32], int i) {
@@ -809,7 +840,7 @@ sample_kernel(const __grid_constant__ SampleRows a, int per) {
   }
   double total = 0;
   if (sums && !far) total = seen.s * pow2(seen.E - weight.E);
-  else if (by_p && !by_k) total = row_total(c, lap<false, true>(row, groups, race, weight, kept).s);
+  else if (by_p && !by_k) total = row_total(c, lap<false, true>(row, groups, race, weight, kept, &sh.score).s);
   if (by_k || by_p) {
     unsigned n = LIST + 1;
     if (k <= LIST && !far) {
@@ -883,13 +914,15 @@ sample_kernel(const __grid_constant__ SampleRows a, int per) {
     }
     if (by_k) kept = kth_token(sh, row, groups, c, weight, kept, k, parts.inbox);
   }
-  Lap l = by_k && by_p ? lap<true, true>(row, groups, race, weight, kept) : lap<true, false>(row, groups, race, weight, kept);
+  Lap l = by_k && by_p ? lap<true, true>(row, groups, race, weight, kept, &sh.score) : lap<true, false>(row, groups, race, weight, kept, &sh.score);
   if (by_k && by_p) total = row_total(c, l.s);
   Win win = settle(row, c, race, kept, l.m);
   const double target = p * total;
   while (by_p && win.id != top.id) {               // what lies in front of it, and who wins there should that be too much
     const Prefix front{win.z, win.id - 1};
-    l = lap<true, true>(row, groups, race, weight, front);
+    if (t == 0) sh.score = score_key(-INFINITY);   // (all warps are past the last lap, and none begins the next before the barrier)
+    __syncthreads();
+    l = lap<true, true>(row, groups, race, weight, front, &sh.score);
     if (row_total(c, l.s) < target) break;
     win = settle(row, c, race, front, l.m);
   }
