@@ -134,18 +134,29 @@ struct Row {
       for (int e = 0; e < N; ++e) v[i * N + e] = plain_logit(f[e]);
     }
   }
-  // f(32 logits, chunk's number in the CTA) for each of a warp's chunks.
-  template <class F>
+  // f(32 logits, chunk's number in the CTA) for each of a warp's chunks; what it reads AHEAD chunks later is asked for.
+  template <int AHEAD, class F>
   __device__ __forceinline__ void stream(F f) const {
     for (int k = threadIdx.x >> 5; k < chunks; k += WARPS) {
       float v[32];
-      const int ahead = (chunk0 + k + 2 * WARPS) * CHUNK + (threadIdx.x & 31) * 32;         // (a lane: 128 bytes of fp32)
-      if (k + 2 * WARPS < chunks && ahead < hi) asm volatile("prefetch.global.L2 [%0];" ::"l"(base + ahead));
+      const int j = (chunk0 + k + AHEAD * WARPS) * CHUNK + (threadIdx.x & 31) * 32;          // (a lane: 128 bytes of fp32)
+      if (k + AHEAD * WARPS < chunks && j < hi) asm volatile("prefetch.global.L2 [%0];" ::"l"(base + j));
       load(chunk0 + k, 0, threadIdx.x & 31, v);
       f(v, k);
     }
   }
-  // f(8 logits, chunk's number, value of the first) for each of a warp's chunks that is `wanted`: less code, for what is read again.
+  // f(8 logits, chunk's number, value of the first) for each of a warp's chunks that is `wanted`.
+  template <class W, class F>
+  __device__ __forceinline__ void again(W wanted, F f) const {
+    for (int k = threadIdx.x >> 5; k < chunks; k += WARPS) {
+      if (!wanted(k)) continue;
+      float v[32];
+      load(chunk0 + k, 0, threadIdx.x & 31, v);
+#pragma unroll
+      for (int q = 0; q < 32; q += 8) f(v + q, k, q);
+    }
+  }
+  // The same in less code, for what hardly ever happens: it waits for memory four times a chunk.
   template <class W, class F>
   __device__ __forceinline__ void eights(W wanted, F f) const {
     for (int k = threadIdx.x >> 5; k < chunks; k += WARPS) {
@@ -417,6 +428,42 @@ __device__ __noinline__ void sort_list(u64* list, unsigned n) {
     }
 }
 
+// The m-th largest of list[0, n), from 1: by the bits in which its keys differ.
+template <int NT>
+__device__ __forceinline__ u64 nth_key(RowShared<NT>& sh, unsigned n, unsigned m) {
+  const int t = threadIdx.x, lane = t & 31, w = t >> 5;
+  constexpr int WARPS = NT / 32;
+  unsigned* part = sh.hits;                        // of each warp, two sets in turn
+  const u64 one = sh.list[0];
+  u64 d = 0;
+  for (unsigned i = t; i < n; i += NT) d |= sh.list[i] ^ one;
+  const auto joined = [&](unsigned x, int set, auto op) {
+    if (lane == 0) part[set * WARPS + w] = x;
+    __syncthreads();
+    return op(lane < WARPS ? part[set * WARPS + lane] : 0u);
+  };
+  const auto any = [](unsigned x) { return __reduce_or_sync(0xffffffffu, x); };
+  const auto sum = [](unsigned x) { return __reduce_add_sync(0xffffffffu, x); };
+  const uint32_t lo = joined(any(static_cast<uint32_t>(d)), 0, any), hi = joined(any(static_cast<uint32_t>(d >> 32)), 1, any);
+  u64 differ = static_cast<u64>(hi) << 32 | lo, key = one & ~differ, upper = 0;
+  unsigned front = 0, left = n;                    // keys above those that begin like `key`, and those
+  for (int set = 0; left > 1; set ^= 1) {
+    const u64 bit = 1ull << (63 - __clzll(differ)), with = key | bit;
+    differ ^= bit;
+    upper = ~(bit - 1);
+    unsigned c = 0;
+#pragma unroll 4
+    for (unsigned i = t; i < n; i += NT) c += (sh.list[i] & upper) == (with & upper);
+    c = joined(sum(c), set, sum);
+    if (front + c >= m) { key = with; left = c; }
+    else { front += c; left -= c; }
+  }
+  for (unsigned i = t; i < n; i += NT)
+    if ((sh.list[i] & upper) == (key & upper)) sh.total = sh.list[i];
+  __syncthreads();
+  return sh.total;
+}
+
 // Up to NT / 2 entries: how many of the list are in front of an entry, and their weight.  Threads share an entry; the first of them has it.
 struct Counted { u64 key, weight, before; unsigned rank; bool mine; };
 template <int NT>
@@ -537,6 +584,18 @@ struct Race {
 __device__ __forceinline__ int score_key(float v) { const int b = __float_as_int(v); return b ^ (b >> 31 & 0x7fffffff); }
 __device__ __forceinline__ float key_score(int k) { return __int_as_float(k ^ (k >> 31 & 0x7fffffff)); }
 
+// The values from place j0 on that `near` names: their scores among the best two.
+template <class R>
+__device__ __noinline__ Top2 look_at(const Race race, const R row, unsigned near, int j0, const Prefix kept, Top2 m) {
+  while (near) {
+    const int i = __ffs(near) - 1, j = j0 + i / R::N * (32 * R::N) + i % R::N;
+    near &= near - 1;
+    const float z = row.one(j);
+    if (within(kept, z, row.id(j))) m = best2(m, Top2{race.rough(z, row.id(j)), row.id(j), -INFINITY, z});
+  }
+  return m;
+}
+
 // A warp's race over the logits that come by.  -log u >= 1 - u, so that a score is at most z / T - log(1 - u): most tokens are out of it by the 32
 // upper bits of their hash, without a logarithm.  `shared`: the best score that any warp of the CTA knows of, which spares the others the look at tokens
 // that do not come near it; who wins does not depend on when they see it.
@@ -556,7 +615,7 @@ struct Racer {
   }
   // The lanes' largest logits raise the bound before all others come; false where none of them is within `kept`, and no other then.
   template <int M, class R>
-  __device__ __forceinline__ bool begin(const Race& race, const R& row, const float (&v)[M], float mine, int chunk, int from, const Prefix& kept, int* shared) {
+  __device__ __forceinline__ bool begin(const Race& race, const R& row, const float* v, float mine, int chunk, int from, const Prefix& kept, int* shared) {
     int j = 0;
 #pragma unroll
     for (int i = M - 1; i >= 0; --i)
@@ -585,14 +644,9 @@ struct Racer {
       if (static_cast<float>(rest) <= exp2_fast(fmaf(v[i], race.c, off)) + 1.f && in) near |= 1u << i;
     }
     bool more = false;
-    while (near) {
-      const int i = __ffs(near) - 1, j = j0 + i / R::N * (32 * R::N) + i % R::N;
-      near &= near - 1;
-      const float z = row.one(j);
-      if (!within(kept, z, row.id(j))) continue;
-      const float y = race.rough(z, row.id(j));
-      m = best2(m, Top2{y, row.id(j), -INFINITY, z});
-      more |= y > bound;
+    if (near) {
+      m = look_at(race, row, near, j0, kept, m);
+      more = m.a1 > bound;
     }
     if (__any_sync(0xffffffffu, more)) {
       raise(fmaxf(bound, warp_highest(m.a1)));
@@ -608,7 +662,7 @@ template <bool RACE, bool MASS, class T, int NT>
 __device__ __noinline__ Lap lap(const Row<T, NT> row, const Groups groups, const Race race, const Weights w, const Prefix front, int* shared) {
   Racer racer;
   double s = 0;
-  row.eights([&](int k) { return groups.reaches(k, front.z); }, [&](const float (&v)[8], int k, int q) {
+  row.again([&](int k) { return groups.reaches(k, front.z); }, [&](const float* v, int k, int q) {
     const int chunk = row.chunk0 + k;
     const float mine = max8(v);
     if (__all_sync(0xffffffffu, !(mine >= front.z))) return;
@@ -627,7 +681,7 @@ __device__ __noinline__ Lap lap(const Row<T, NT> row, const Groups groups, const
       }
       s += ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
     }
-    if (RACE && (__any_sync(0xffffffffu, racer.bound > -INFINITY) || racer.begin(race, row, v, mine, chunk, q, front, shared)))
+    if (RACE && (__any_sync(0xffffffffu, racer.bound > -INFINITY) || racer.template begin<8>(race, row, v, mine, chunk, q, front, shared)))
       racer.template run<false>(race, row, v, chunk, q, front, shared);
   });
   return Lap{racer.m, s};
@@ -713,7 +767,7 @@ __device__ __noinline__ Prefix kth_token(RowShared<NT>& sh, const Row<T, NT> row
   if (threadIdx.x == 0) sh.n_list = 0;
   __syncthreads();
   unsigned* mine = sets + (threadIdx.x & 3) * BINS;
-  row.eights([&](int i) { return groups.reaches(i, of.z); }, [&](const float (&v)[8], int, int) {
+  row.again([&](int i) { return groups.reaches(i, of.z); }, [&](const float* v, int, int) {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       if (v[i] >= of.z) atomicAdd(&mine[w.bin(v[i])], 1u);
@@ -724,7 +778,7 @@ __device__ __noinline__ Prefix kth_token(RowShared<NT>& sh, const Row<T, NT> row
   find_bin(sh, c, true, true, k);
   const int bin = sh.bin;
   const unsigned before = sh.before;               // (0 with the last bin where the row has fewer than k tokens)
-  row.eights([&](int i) { return groups.reaches(i, fmaxf(of.z, w.edge(bin))); }, [&](const float (&v)[8], int n, int q) {
+  row.again([&](int i) { return groups.reaches(i, fmaxf(of.z, w.edge(bin))); }, [&](const float* v, int n, int q) {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       if (v[i] >= of.z && w.bin(v[i]) == bin) to_list(sh, v[i], row.id(Row<T, NT>::place(row.chunk0 + n, q + i, threadIdx.x & 31)));
@@ -732,8 +786,7 @@ __device__ __noinline__ Prefix kth_token(RowShared<NT>& sh, const Row<T, NT> row
   const unsigned n = join_lists(sh, c, inbox);
   if (n > LIST) return kth_by_bits(row, c, of, k);
   if (c.rank == 0) {
-    sort_list<NT>(sh.list, n);
-    const u64 last = k - before <= n ? sh.list[k - before - 1] : 0;
+    const u64 last = k - before <= n ? nth_key(sh, n, k - before) : 0;
     const Prefix cut = last ? Prefix{list_z(last), list_id(last)} : of;
     if (threadIdx.x < c.size) c.of(&sh, threadIdx.x)->cut = cut;
   }
@@ -753,7 +806,7 @@ __device__ __noinline__ float min_p_logit(float top, float temp, float mp) {
   return at_least(v);
 }
 
-template <class T, int NT>
+template <class T, int NT, int AHEAD>
 __global__ void __launch_bounds__(NT, 1024 / NT)
 sample_kernel(const __grid_constant__ SampleRows a, int per) {
   extern __shared__ __align__(16) float smem[];
@@ -780,16 +833,16 @@ sample_kernel(const __grid_constant__ SampleRows a, int per) {
   Racer racer;
   float largest = -INFINITY;                       // of the thread
   if (all) {
-    row.stream([&](const float (&v)[32], int i) {
+    row.template stream<AHEAD>([&](const float (&v)[32], int i) {
       float m[4], mine;
       const float highest = look(row, v, i, m, mine, seen.top);
       if (!(highest > -INFINITY && highest < INFINITY)) return;
-      if (racer.bound == -INFINITY) racer.begin(race, row, v, mine, row.chunk0 + i, 0, whole_row(), &sh.score);
+      if (racer.bound == -INFINITY) racer.template begin<32>(race, row, v, mine, row.chunk0 + i, 0, whole_row(), &sh.score);
 #pragma unroll
       for (int q = 0; q < 32; q += 8) racer.template run<true>(race, row, v + q, row.chunk0 + i, q, whole_row(), &sh.score);
     });
   } else if (sums) {
-    row.stream([&](const float (&v)[32], int i) {
+    row.template stream<AHEAD>([&](const float (&v)[32], int i) {
       float m[4], mine;
       const float highest = look(row, v, i, m, mine, seen.top);
       largest = fmaxf(largest, mine);
@@ -805,7 +858,7 @@ sample_kernel(const __grid_constant__ SampleRows a, int per) {
       seen.add(s, g, E);
     });
   } else {
-    row.stream([&](const float (&v)[32], int i) {
+    row.template stream<AHEAD>([&](const float (&v)[32], int i) {
       float m[4], mine;
       look(row, v, i, m, mine, seen.top);
       largest = fmaxf(largest, mine);
@@ -914,23 +967,22 @@ sample_kernel(const __grid_constant__ SampleRows a, int per) {
     }
     if (by_k) kept = kth_token(sh, row, groups, c, weight, kept, k, parts.inbox);
   }
-  Lap l = by_k && by_p ? lap<true, true>(row, groups, race, weight, kept, &sh.score) : lap<true, false>(row, groups, race, weight, kept, &sh.score);
+  const Lap l = by_k && by_p ? lap<true, true>(row, groups, race, weight, kept, &sh.score) : lap<true, false>(row, groups, race, weight, kept, &sh.score);
   if (by_k && by_p) total = row_total(c, l.s);
   Win win = settle(row, c, race, kept, l.m);
   const double target = p * total;
-  while (by_p && win.id != top.id) {               // what lies in front of it, and who wins there should that be too much
+  while (by_p && win.id != top.id) {               // what lies in front of it; who wins there, should that be too much
     const Prefix front{win.z, win.id - 1};
-    if (t == 0) sh.score = score_key(-INFINITY);   // (all warps are past the last lap, and none begins the next before the barrier)
+    if (row_total(c, lap<false, true>(row, groups, race, weight, front, &sh.score).s) < target) break;
+    if (t == 0) sh.score = score_key(-INFINITY);   // (all warps are past the last race, and none begins the next before the barrier)
     __syncthreads();
-    l = lap<true, true>(row, groups, race, weight, front, &sh.score);
-    if (row_total(c, l.s) < target) break;
-    win = settle(row, c, race, front, l.m);
+    win = settle(row, c, race, front, lap<true, false>(row, groups, race, weight, front, &sh.score).m);
   }
   if (lead) a.out[r] = win.id;
   c.sync();
 }
 
-template <class T, int NT>
+template <class T, int NT, int AHEAD>
 __global__ void __launch_bounds__(NT, 1024 / NT)
 logprob_kernel(const __grid_constant__ LogprobRows a, int per) {
   extern __shared__ __align__(16) float smem[];
@@ -954,7 +1006,7 @@ logprob_kernel(const __grid_constant__ LogprobRows a, int per) {
   Seen seen;
   float largest = -INFINITY;                       // of the thread
   const int tj = t + row.lo;
-  row.stream([&](const float (&v)[32], int i) {
+  row.template stream<AHEAD>([&](const float (&v)[32], int i) {
     const int chunk = row.chunk0 + i;
     float m[4], mine;
     const float highest = look(row, v, i, m, mine, seen.top);
@@ -1066,23 +1118,22 @@ static int row_cluster(int R, int chunks, int sms) {
 }
 
 template <int NT, class A, class K>
-static int launch_rows(const char* name, K kern, const A& a, int chunks, cudaStream_t s) {
-  const int c = row_cluster(a.R, chunks, a.sms), per = (chunks + c - 1) / c, bytes = Parts<NT>::bytes(per, c);
+static int launch_rows(const char* name, K kern, const A& a, int chunks, int c, cudaStream_t s) {
+  const int per = (chunks + c - 1) / c, bytes = Parts<NT>::bytes(per, c);
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return spark_launch_rc(name);
   spark_launch_pdl(kern, dim3(a.R * c), dim3(NT), bytes, s, dim3(c, 1, 1), a, per);
   return spark_launch_rc(name);
 }
-// Rows of a few chunks take CTAs of four warps.
+// Rows of a few chunks take CTAs of four warps.  How far ahead others are asked for goes by whether all CTAs run at once: then one chunk (256 draws from
+// 152k 43.9 us, two chunks 47.9: the groups that are read again wait behind what was asked for), else two (1024 scored rows 101 us, one chunk 107).
+#define SPARK_ROWS(KERNEL, NAME)                                                                                        \
+  const int chunks = (a.V + 8 + CHUNK - 1) / CHUNK, c = row_cluster(a.R, chunks, a.sms);                                \
+  if (chunks <= 8) return launch_rows<128>(NAME, KERNEL<T, 128, 1>, a, chunks, c, s);                                   \
+  return a.R * c > 2 * a.sms ? launch_rows<512>(NAME, KERNEL<T, 512, 2>, a, chunks, c, s) : launch_rows<512>(NAME, KERNEL<T, 512, 1>, a, chunks, c, s)
 template <class T>
-static int sample_rows(const SampleRows& a, cudaStream_t s) {
-  const int chunks = (a.V + 8 + CHUNK - 1) / CHUNK;
-  return chunks <= 8 ? launch_rows<128>("spark_sample_rows", sample_kernel<T, 128>, a, chunks, s) : launch_rows<512>("spark_sample_rows", sample_kernel<T, 512>, a, chunks, s);
-}
+static int sample_rows(const SampleRows& a, cudaStream_t s) { SPARK_ROWS(sample_kernel, "spark_sample_rows"); }
 template <class T>
-static int logprob_rows(const LogprobRows& a, cudaStream_t s) {
-  const int chunks = (a.V + 8 + CHUNK - 1) / CHUNK;
-  return chunks <= 8 ? launch_rows<128>("spark_logprob_rows", logprob_kernel<T, 128>, a, chunks, s) : launch_rows<512>("spark_logprob_rows", logprob_kernel<T, 512>, a, chunks, s);
-}
+static int logprob_rows(const LogprobRows& a, cudaStream_t s) { SPARK_ROWS(logprob_kernel, "spark_logprob_rows"); }
 
 }  // namespace spark
 
