@@ -113,7 +113,7 @@ Tensor adjust_logits(const Tensor& given, const Adjust& a, int64_t offset, const
   Tensor y = out ? *out : at::empty({R, V}, x.options().dtype(at::kFloat));
   if (!run || R == 0) return y;
   const On on(x);
-  spark::AdjustRows arg{x.data_ptr(), ptr<float>(y), row_step(x), row_step(y), on.dev.status, static_cast<int>(R), static_cast<int>(V), type, static_cast<int>(offset), k};
+  spark::AdjustRows arg{x.data_ptr(), ptr<float>(y), row_step(x), row_step(y), on.dev.status, static_cast<int>(R), static_cast<int>(V), type, static_cast<int>(offset), on.dev.sms, k};
   on.launch(e_adjust, &arg);
   return y;
 }
@@ -156,16 +156,15 @@ Tensor sample_tokens(const Tensor& logits, const Tensor& temps, const Tensor& se
   const On on(x);
   spark::SampleRows arg{x.data_ptr(), row_step(x), ptr<float>(temps), ptr<long long>(seeds), ptr<long long>(positions), ptr<int>(top_k), ptr<float>(top_p),
                         ptr<float>(min_p), ptr<int>(out), on.dev.status, static_cast<int>(R), static_cast<int>(V), type, on.dev.sms};
+  Tensor z;
   if (a.any()) {                                 // (rows of whole 16 bytes)
     const int64_t ld = (V + 3) / 4 * 4;
-    Tensor z = at::empty({R, ld}, temps.options());
-    spark::AdjustRows first{x.data_ptr(), ptr<float>(z), row_step(x), ld, on.dev.status, static_cast<int>(R), static_cast<int>(V), type, 0, k};
+    z = at::empty({R, ld}, temps.options());
+    spark::AdjustRows first{x.data_ptr(), ptr<float>(z), row_step(x), ld, on.dev.status, static_cast<int>(R), static_cast<int>(V), type, 0, on.dev.sms, k};
     on.launch(e_adjust, &first);
     arg.x = z.data_ptr(); arg.ldx = ld; arg.type = spark::LT_F32;
-    on.launch(e_sample, &arg);
-  } else {
-    on.launch(e_sample, &arg);
   }
+  on.launch(e_sample, &arg);
   return out;
 }
 

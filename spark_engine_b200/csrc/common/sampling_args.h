@@ -39,7 +39,7 @@ struct AdjustRows {
   float* out;
   long long ldx, ldo;
   int* status;
-  int R, V, type, offset;
+  int R, V, type, offset, sms;
   Adjustments a;
 };
 

@@ -1110,11 +1110,13 @@ logprob_kernel(const __grid_constant__ LogprobRows a, int per) {
   c.sync();
 }
 
-// CTAs of a row's cluster: as many as there is room for, of four chunks each at least.
-static int row_cluster(int R, int chunks, int sms) {
+// CTAs of a row's cluster: as many as run at once, of four chunks each at least; draws take two while that is no more than twice as many, since a
+// row that keeps very many tokens holds the others up (256 draws of eight kinds from 152k logits 105 us, with one CTA each 148; without such rows 62
+// and 49.  1024 draws from 66k: 189 and 173).
+static int row_cluster(int R, int chunks, int sms, bool draws) {
   int c = 1;
   while (c < CLUSTER_MAX && R * c * 2 <= 2 * sms && c * 4 < chunks) c *= 2;
-  return c;
+  return c == 1 && draws && R <= 2 * sms && chunks > 16 ? 2 : c;
 }
 
 template <int NT, class A, class K>
@@ -1126,14 +1128,20 @@ static int launch_rows(const char* name, K kern, const A& a, int chunks, int c, 
 }
 // Rows of a few chunks take CTAs of four warps.  How far ahead others are asked for goes by whether all CTAs run at once: then one chunk (256 draws from
 // 152k 43.9 us, two chunks 47.9: the groups that are read again wait behind what was asked for), else two (1024 scored rows 101 us, one chunk 107).
-#define SPARK_ROWS(KERNEL, NAME)                                                                                        \
-  const int chunks = (a.V + 8 + CHUNK - 1) / CHUNK, c = row_cluster(a.R, chunks, a.sms);                                \
-  if (chunks <= 8) return launch_rows<128>(NAME, KERNEL<T, 128, 1>, a, chunks, c, s);                                   \
-  return a.R * c > 2 * a.sms ? launch_rows<512>(NAME, KERNEL<T, 512, 2>, a, chunks, c, s) : launch_rows<512>(NAME, KERNEL<T, 512, 1>, a, chunks, c, s)
 template <class T>
-static int sample_rows(const SampleRows& a, cudaStream_t s) { SPARK_ROWS(sample_kernel, "spark_sample_rows"); }
+static int sample_rows(const SampleRows& a, cudaStream_t s) {
+  const char* name = "spark_sample_rows";
+  const int chunks = (a.V + 8 + CHUNK - 1) / CHUNK, c = row_cluster(a.R, chunks, a.sms, true);
+  if (chunks <= 8) return launch_rows<128>(name, sample_kernel<T, 128, 1>, a, chunks, c, s);
+  return a.R * c > 2 * a.sms ? launch_rows<512>(name, sample_kernel<T, 512, 2>, a, chunks, c, s) : launch_rows<512>(name, sample_kernel<T, 512, 1>, a, chunks, c, s);
+}
 template <class T>
-static int logprob_rows(const LogprobRows& a, cudaStream_t s) { SPARK_ROWS(logprob_kernel, "spark_logprob_rows"); }
+static int logprob_rows(const LogprobRows& a, cudaStream_t s) {
+  const char* name = "spark_logprob_rows";
+  const int chunks = (a.V + 8 + CHUNK - 1) / CHUNK, c = row_cluster(a.R, chunks, a.sms, false);
+  if (chunks <= 8) return launch_rows<128>(name, logprob_kernel<T, 128, 1>, a, chunks, c, s);
+  return a.R * c > 2 * a.sms ? launch_rows<512>(name, logprob_kernel<T, 512, 2>, a, chunks, c, s) : launch_rows<512>(name, logprob_kernel<T, 512, 1>, a, chunks, c, s);
+}
 
 }  // namespace spark
 

@@ -82,65 +82,81 @@ __device__ __forceinline__ float4 four(const H* p) {
   return make_float4(logit(a), logit(a + 1), logit(b), logit(b + 1));
 }
 
-// A CTA has ADJUST_COLS columns of a row: first all of them as if nothing were drafted and no bias given, then those in the lists again, by what they were.
+// A CTA has some tiles of ADJUST_COLS columns of a row: first all of them as if nothing were drafted and no bias given, then those in the lists again,
+// by what they were.
 constexpr int ADJUST_THREADS = 256, ADJUST_COLS = ADJUST_THREADS * 16;
 template <class T>
 __global__ void __launch_bounds__(ADJUST_THREADS)
-adjust_rows_kernel(const __grid_constant__ AdjustRows a) {
+adjust_rows_kernel(const __grid_constant__ AdjustRows a, int tiles) {
   extern __shared__ int ids[];                     // the lists' entries, then the logits of those in this CTA's columns
   pdl_wait();
   pdl_trigger();
-  const int r = blockIdx.y, b = blockIdx.x * ADJUST_COLS, e = min(b + ADJUST_COLS, a.V), t = threadIdx.x;
-  const RowAdjust adj(a.a, r, a.status);
+  const int r = blockIdx.y, b = blockIdx.x * tiles * ADJUST_COLS, e = min(b + tiles * ADJUST_COLS, a.V), t = threadIdx.x;
   const T* x = static_cast<const T*>(a.x) + r * a.ldx;
   float* out = a.out + r * a.ldo;
+  const RowAdjust adj(a.a, r, a.status);
   const int n = adj.entries();
   float* was = reinterpret_cast<float*>(ids + n);
-  bool mine = false;                               // whether any of the thread's entries is of these columns
-  for (int i = t; i < n; i += ADJUST_THREADS) {    // (read before they are written: `out` may be the logits)
-    const int id = adj.entry(i), col = id < 0 ? -1 : id - a.offset;
-    ids[i] = id;
-    if (col >= b && col < e) { was[i] = logit(x + col); mine = true; }
+  bool any = false;                                // whether any entry is of these columns
+  if (n) {
+    for (int i = t; i < n; i += ADJUST_THREADS) {  // (read before they are written: `out` may be the logits)
+      const int id = adj.entry(i), col = id < 0 ? -1 : id - a.offset;
+      ids[i] = id;
+      if (col >= b && col < e) { was[i] = logit(x + col); any = true; }
+    }
+    any = __syncthreads_or(any);
   }
-  const bool any = n && __syncthreads_or(mine);
   const uintptr_t places = reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(adj.counts) | reinterpret_cast<uintptr_t>(x) * (4 / sizeof(T));
   if ((places & 15) == 0) {
     constexpr int U = ADJUST_COLS / ADJUST_THREADS / 4;
-    float4 z[U];
-    int4 c[U];
-    uint32_t bits[U];
+#pragma unroll 1
+    for (int at = b; at < e; at += ADJUST_COLS) {
+      float4 z[U];
+      int4 c[U];
+      uint32_t bits[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int col = b + (u * ADJUST_THREADS + t) * 4;
-      if (col + 4 > e) continue;
-      z[u] = four(x + col);
-      c[u] = adj.counts ? __ldg(reinterpret_cast<const int4*>(adj.counts + col)) : make_int4(0, 0, 0, 0);
-      bits[u] = adj.allowed ? __ldg(adj.allowed + (col >> 5)) >> (col & 31) : 15u;
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int col = b + (u * ADJUST_THREADS + t) * 4;
-      if (col + 4 > e) {
-        for (int i = col; i < e; ++i) out[i] = adj.common(logit(x + i), i);
-        continue;
+      for (int u = 0; u < U; ++u) {
+        const int col = at + (u * ADJUST_THREADS + t) * 4;
+        if (col + 4 > e) continue;
+        z[u] = four(x + col);
+        c[u] = adj.counts ? __ldg(reinterpret_cast<const int4*>(adj.counts + col)) : make_int4(0, 0, 0, 0);
+        bits[u] = adj.allowed ? __ldg(adj.allowed + (col >> 5)) >> (col & 31) : 15u;
       }
-      float4 y = make_float4(adj.penalised(z[u].x, c[u].x, 0), adj.penalised(z[u].y, c[u].y, 0), adj.penalised(z[u].z, c[u].z, 0), adj.penalised(z[u].w, c[u].w, 0));
-      if (!(bits[u] & 1)) y.x = -INFINITY;
-      if (!(bits[u] & 2)) y.y = -INFINITY;
-      if (!(bits[u] & 4)) y.z = -INFINITY;
-      if (!(bits[u] & 8)) y.w = -INFINITY;
-      *reinterpret_cast<float4*>(out + col) = y;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int col = at + (u * ADJUST_THREADS + t) * 4;
+        if (col + 4 > e) {
+          for (int i = col; i < e; ++i) out[i] = adj.common(logit(x + i), i);
+          continue;
+        }
+        float4 y = z[u];
+        if (c[u].x | c[u].y | c[u].z | c[u].w)
+          y = make_float4(adj.penalised(y.x, c[u].x, 0), adj.penalised(y.y, c[u].y, 0), adj.penalised(y.z, c[u].z, 0), adj.penalised(y.w, c[u].w, 0));
+        if (!(bits[u] & 1)) y.x = -INFINITY;
+        if (!(bits[u] & 2)) y.y = -INFINITY;
+        if (!(bits[u] & 4)) y.z = -INFINITY;
+        if (!(bits[u] & 8)) y.w = -INFINITY;
+        *reinterpret_cast<float4*>(out + col) = y;
+      }
     }
   } else {
-    constexpr int U = 4;
+    constexpr int U = 8;
     for (int col = b + t; col < e; col += U * ADJUST_THREADS) {
       float z[U];
+      int c[U];
+      uint32_t words[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (col + u * ADJUST_THREADS < e) z[u] = logit(x + col + u * ADJUST_THREADS);
+      for (int u = 0; u < U; ++u) {
+        const int at = min(col + u * ADJUST_THREADS, e - 1);
+        z[u] = logit(x + at);
+        c[u] = adj.counts ? __ldg(adj.counts + at) : 0;
+        words[u] = adj.allowed ? __ldg(adj.allowed + (at >> 5)) : ~0u;
+      }
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (col + u * ADJUST_THREADS < e) out[col + u * ADJUST_THREADS] = adj.common(z[u], col + u * ADJUST_THREADS);
+      for (int u = 0; u < U; ++u) {
+        const int at = col + u * ADJUST_THREADS;
+        if (at < e) out[at] = words[u] >> (at & 31) & 1 ? adj.penalised(z[u], c[u], 0) : -INFINITY;
+      }
     }
   }
   if (!any) return;
@@ -172,10 +188,12 @@ extern "C" int spark_count_tokens(const CountTokens* a, cudaStream_t s) {
 
 extern "C" int spark_adjust_rows(const AdjustRows* a, cudaStream_t s) {
   if (a->R <= 0 || a->V <= 0) return 0;
-  const dim3 grid((a->V + ADJUST_COLS - 1) / ADJUST_COLS, a->R), block(ADJUST_THREADS), one(1, 1, 1);
+  // Tiles per CTA: one where that fills the GPU no more than once, else four (their lists are read once for all of them).
+  const int all = (a->V + ADJUST_COLS - 1) / ADJUST_COLS, tiles = static_cast<long long>(all) * a->R <= 4ll * a->sms ? 1 : all < 4 ? all : 4;
+  const dim3 grid((all + tiles - 1) / tiles, a->R), block(ADJUST_THREADS), one(1, 1, 1);
   const int sm = (a->a.n_drafted + a->a.n_bias) * 8;
-  if (a->type == LT_F32) spark_launch_pdl(adjust_rows_kernel<float>, grid, block, sm, s, one, *a);
-  else if (a->type == LT_BF16) spark_launch_pdl(adjust_rows_kernel<__nv_bfloat16>, grid, block, sm, s, one, *a);
-  else spark_launch_pdl(adjust_rows_kernel<__half>, grid, block, sm, s, one, *a);
+  if (a->type == LT_F32) spark_launch_pdl(adjust_rows_kernel<float>, grid, block, sm, s, one, *a, tiles);
+  else if (a->type == LT_BF16) spark_launch_pdl(adjust_rows_kernel<__nv_bfloat16>, grid, block, sm, s, one, *a, tiles);
+  else spark_launch_pdl(adjust_rows_kernel<__half>, grid, block, sm, s, one, *a, tiles);
   return spark_launch_rc("spark_adjust_rows");
 }
