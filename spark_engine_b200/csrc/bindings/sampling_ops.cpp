@@ -1,5 +1,7 @@
 // Device side of ops/sampling.py: arguments checked, outputs taken from torch's allocator, kernels launched on the tensors' device and its current
 // stream.  In C++ because a round makes these calls between two forwards and the kernels take a few microseconds.
+#include <torch/csrc/autograd/python_variable.h>
+
 #include "plumbing.h"
 #include "sampling_args.h"
 
@@ -49,8 +51,19 @@ Tensor rows_of(const Tensor& t) {
 }
 
 // ------------------------------------------------------------------------------------------------ adjustments
-struct Adjust {
+struct Adjust {                                  // `Adjust` of ops/sampling.py
   Opt counts, slots, drafted, repetition, presence, frequency, bias_ids, bias, allowed;
+  explicit Adjust(const py::object& from) {
+    if (from.is_none()) return;
+    Opt* to[] = {&counts, &slots, &drafted, &repetition, &presence, &frequency, &bias_ids, &bias, &allowed};
+    NEED(py::isinstance<py::tuple>(from) && py::len(from) == 9, "adjustments are given as an `Adjust`");
+    for (int i = 0; i < 9; ++i) {
+      PyObject* o = PyTuple_GET_ITEM(from.ptr(), i);
+      if (o == Py_None) continue;
+      NEED(THPVariable_Check(o), "an `Adjust` holds tensors");
+      *to[i] = THPVariable_Unpack(o);
+    }
+  }
   bool any() const { return counts || drafted || repetition || presence || frequency || bias_ids || allowed; }
 };
 
@@ -94,7 +107,8 @@ std::pair<const char*, const char*> span(const Tensor& t) {
   return {p, p + (last + 1) * t.element_size()};
 }
 
-Tensor adjust_logits(const Tensor& given, const Adjust& a, int64_t offset, const Opt& out, bool run) {
+Tensor adjust_logits(const Tensor& given, const py::object& adjust, int64_t offset, const Opt& out, bool run) {
+  const Adjust a(adjust);
   const int type = type_of(given);
   const Tensor x = rows_of(given);
   const at::Device dev = x.device();
@@ -139,7 +153,8 @@ void count_tokens(const Tensor& counts, const Tensor& tokens, const Tensor& n, c
 
 // ------------------------------------------------------------------------------------------------ tokens
 Tensor sample_tokens(const Tensor& logits, const Tensor& temps, const Tensor& seeds, const Tensor& positions, const Opt& top_k, const Opt& top_p, const Opt& min_p,
-                     const Adjust& a, bool run) {
+                     const py::object& adjust, bool run) {
+  const Adjust a(adjust);
   const int type = type_of(logits);
   const Tensor x = rows_of(logits);
   const at::Device dev = x.device();
@@ -194,17 +209,5 @@ PYBIND11_MODULE(_sampling, mod) {
   mod.doc() = "spark_engine_b200: from logits to tokens (checks and launches)";
   mod.def("bind_entry", &bind_entry).def("bind_device", &bind_device).def("take_launched", &take_launched);
   mod.def("layout", [] { return SPARK_SAMPLING_LAYOUT; });
-  py::class_<Adjust>(mod, "Adjust",
-      "What a row's logits go through before a token is drawn; tensors on the logits' device, None: none of the kind.\n"
-      "counts int32 [slots, V]: 2 * times generated + (1 if in the prompt), see `count_tokens`; slots int32 [R]: a row's row of counts (None: its\n"
-      "number; negative: the row has no penalties); drafted int32 [R, n]: tokens on the way to the row that count as generated on top, negative:\n"
-      "none; repetition, presence, frequency fp32 [R]; bias_ids int32 and bias fp32 [R, n]: added to the logits of these ids, negative: none;\n"
-      "allowed int32 [R, (V + 31) / 32]: bit c % 32 of word c / 32 says whether column c may be drawn.")
-      .def(py::init([](Opt c, Opt s, Opt d, Opt r, Opt p, Opt f, Opt bi, Opt b, Opt al) { return Adjust{c, s, d, r, p, f, bi, b, al}; }), py::arg("counts") = py::none(), py::arg("slots") = py::none(), py::arg("drafted") = py::none(),
-           py::arg("repetition") = py::none(), py::arg("presence") = py::none(), py::arg("frequency") = py::none(), py::arg("bias_ids") = py::none(),
-           py::arg("bias") = py::none(), py::arg("allowed") = py::none())
-      .def_readonly("counts", &Adjust::counts).def_readonly("slots", &Adjust::slots).def_readonly("drafted", &Adjust::drafted)
-      .def_readonly("repetition", &Adjust::repetition).def_readonly("presence", &Adjust::presence).def_readonly("frequency", &Adjust::frequency)
-      .def_readonly("bias_ids", &Adjust::bias_ids).def_readonly("bias", &Adjust::bias).def_readonly("allowed", &Adjust::allowed);
   mod.def("count_tokens", &count_tokens).def("adjust_logits", &adjust_logits).def("sample_tokens", &sample_tokens).def("token_logprobs", &token_logprobs);
 }

@@ -75,26 +75,9 @@ struct RowAdjust {
     z = penalised(z, counts ? counts[col] : 0, 0);
     return allows(col) ? z : -INFINITY;
   }
+  // Entries of the lists: drafted tokens, then biases.
   __device__ __forceinline__ int entries() const { return nd + nb; }
   __device__ __forceinline__ int entry(int i) const { return i < nd ? drafted[i] : bias_ids[i - nd]; }
-  // Entry i's column from its logit, all of the lists' entries of its id counted; false where an entry before it is of the same id.  `ids`: the entries.
-  __device__ __forceinline__ bool listed(int i, const int* ids, int col, float z, float& y) const {
-    const int id = ids[i];
-    int more = 0;
-    for (int j = 0; j < nd; ++j) {
-      if (ids[j] != id) continue;
-      if (j < i) return false;
-      ++more;
-    }
-    y = penalised(z, counts ? counts[col] : 0, more);
-    for (int j = nd; j < nd + nb; ++j) {
-      if (ids[j] != id) continue;
-      if (j < i) return false;
-      y = __fadd_rn(y, bias[j - nd]);
-    }
-    if (!allows(col)) y = -INFINITY;
-    return true;
-  }
 };
 
 // ------------------------------------------------------------------------------------------------ reductions

@@ -86,9 +86,9 @@ __device__ __forceinline__ float4 four(const H* p) {
 // by what they were.
 constexpr int ADJUST_THREADS = 256, ADJUST_COLS = ADJUST_THREADS * 16;
 template <class T>
-__global__ void __launch_bounds__(ADJUST_THREADS)
+__global__ void __launch_bounds__(ADJUST_THREADS, 5)
 adjust_rows_kernel(const __grid_constant__ AdjustRows a, int tiles) {
-  extern __shared__ int ids[];                     // the lists' entries, then the logits of those in this CTA's columns
+  extern __shared__ int ids[];                     // the lists' entries, and of those in this CTA's columns what belongs to them
   pdl_wait();
   pdl_trigger();
   const int r = blockIdx.y, b = blockIdx.x * tiles * ADJUST_COLS, e = min(b + tiles * ADJUST_COLS, a.V), t = threadIdx.x;
@@ -96,13 +96,18 @@ adjust_rows_kernel(const __grid_constant__ AdjustRows a, int tiles) {
   float* out = a.out + r * a.ldo;
   const RowAdjust adj(a.a, r, a.status);
   const int n = adj.entries();
-  float* was = reinterpret_cast<float*>(ids + n);
+  float *was = reinterpret_cast<float*>(ids + n), *more = was + n;
+  int* count = ids + 3 * n;
   bool any = false;                                // whether any entry is of these columns
   if (n) {
     for (int i = t; i < n; i += ADJUST_THREADS) {  // (read before they are written: `out` may be the logits)
       const int id = adj.entry(i), col = id < 0 ? -1 : id - a.offset;
       ids[i] = id;
-      if (col >= b && col < e) { was[i] = logit(x + col); any = true; }
+      if (i >= adj.nd) more[i] = adj.bias[i - adj.nd];
+      if (col < b || col >= e) continue;
+      was[i] = logit(x + col);
+      count[i] = adj.allows(col) ? (adj.counts ? max(adj.counts[col], 0) : 0) : -1;
+      any = true;
     }
     any = __syncthreads_or(any);
   }
@@ -163,8 +168,15 @@ adjust_rows_kernel(const __grid_constant__ AdjustRows a, int tiles) {
   __syncthreads();
   for (int i = t; i < n; i += ADJUST_THREADS) {
     const int col = ids[i] < 0 ? -1 : ids[i] - a.offset;
-    float y;
-    if (col >= b && col < e && adj.listed(i, ids, col, was[i], y)) out[col] = y;
+    if (col < b || col >= e) continue;
+    // all entries of its id together; where one in front of it is of the same id, that one does it
+    int first = i, times = 0;
+    for (int j = 0; j < adj.nd; ++j)
+      if (ids[j] == ids[i]) { first = min(first, j); ++times; }
+    float y = adj.penalised(was[i], max(count[i], 0), times);
+    for (int j = adj.nd; j < n; ++j)
+      if (ids[j] == ids[i]) { first = min(first, j); y = __fadd_rn(y, more[j]); }
+    if (first == i) out[col] = count[i] < 0 ? -INFINITY : y;
   }
 }
 
@@ -191,7 +203,7 @@ extern "C" int spark_adjust_rows(const AdjustRows* a, cudaStream_t s) {
   // Tiles per CTA: one where that fills the GPU no more than once, else four (their lists are read once for all of them).
   const int all = (a->V + ADJUST_COLS - 1) / ADJUST_COLS, tiles = static_cast<long long>(all) * a->R <= 4ll * a->sms ? 1 : all < 4 ? all : 4;
   const dim3 grid((all + tiles - 1) / tiles, a->R), block(ADJUST_THREADS), one(1, 1, 1);
-  const int sm = (a->a.n_drafted + a->a.n_bias) * 8;
+  const int sm = (a->a.n_drafted + a->a.n_bias) * 16;
   if (a->type == LT_F32) spark_launch_pdl(adjust_rows_kernel<float>, grid, block, sm, s, one, *a, tiles);
   else if (a->type == LT_BF16) spark_launch_pdl(adjust_rows_kernel<__nv_bfloat16>, grid, block, sm, s, one, *a, tiles);
   else spark_launch_pdl(adjust_rows_kernel<__half>, grid, block, sm, s, one, *a, tiles);

@@ -646,6 +646,7 @@ class Model:
         self.kv_backing = kv_backing
         self.lcfg = tp.local_config(cfg) if tp is not None else cfg      # per-rank head counts
         self.n_slots, self.kv_tokens = n_slots, kv_tokens
+        self._counts = None                  # of the slots' tokens, see token_counts
         per = slot_tokens or kv_tokens // n_slots
         self.page = 0                        # > 0: caches are pages of this many tokens, found through `page_table`
         if cfg.layer_specs:
@@ -896,6 +897,61 @@ class Model:
 
     def sample(self, logits: torch.Tensor, temperature: float, seed: int, position: int) -> int:
         return self.sample_rows(logits, [temperature], [seed], [position])[0]
+
+    def draw_rows(self, logits: torch.Tensor, params, slots, positions, drafted=None) -> List[int]:
+        """One token per logits row by its request's `SamplingParams`: params[r], the request's slot, the position that the token takes and
+        drafted[r], the drafts on the way to the row, which penalties count as said.  Without filters these are `sample_rows`' tokens."""
+        if logits.dim() == 1:
+            logits = logits.unsqueeze(0)
+        if not any(p.filtered for p in params):
+            return self.sample_rows(logits, [p.temperature for p in params], [p.seed for p in params], positions)
+        if self.tp is not None:
+            logits = self.tp.gather_vocab(logits)
+        on = dict(device=logits.device, non_blocking=True)
+        f = torch.tensor([[p.temperature for p in params], [p.top_p for p in params], [p.min_p for p in params], [p.repetition for p in params],
+                          [p.presence for p in params], [p.frequency for p in params]], dtype=torch.float32).to(**on)
+        i = torch.tensor([[p.seed for p in params], list(positions)], dtype=torch.int64).to(**on)
+        ints = [[p.top_k for p in params], [s if p.counted else -1 for p, s in zip(params, slots)]]
+        n_draft = max((len(d) for d in drafted), default=0) if drafted is not None else 0
+        n_bias = max(len(p.bias) for p in params)
+        rows = [list(d) + [-1] * (n_draft - len(d)) for d in drafted] if n_draft else []
+        ids = [[t for t, _ in p.bias] + [-1] * (n_bias - len(p.bias)) for p in params] if n_bias else []
+        flat = torch.tensor(sum(ints, []) + sum(rows, []) + sum(ids, []), dtype=torch.int32).to(**on)
+        R = len(params)
+        adjust = None
+        if any(p.counted or p.bias for p in params):
+            counted = any(p.counted for p in params)
+            at = 2 * R + R * n_draft
+            adjust = ops.Adjust(counts=self.token_counts() if counted else None, slots=flat[R: 2 * R], drafted=flat[2 * R: at].view(R, n_draft) if n_draft else None,
+                                repetition=f[3], presence=f[4], frequency=f[5], bias_ids=flat[at:].view(R, n_bias) if n_bias else None,
+                                bias=torch.tensor([[b for _, b in p.bias] + [0.0] * (n_bias - len(p.bias)) for p in params], dtype=torch.float32).to(**on) if n_bias else None)
+        return ops.sample_tokens(logits, f[0], i[0], i[1], top_k=flat[:R], top_p=f[1], min_p=f[2], adjust=adjust).tolist()
+
+    def token_counts(self) -> torch.Tensor:
+        """Counts of the slots' tokens (`ops.count_tokens`), from the first request on that has penalties."""
+        if self._counts is None:
+            self._counts = torch.zeros(self.n_slots, self.cfg.vocab, dtype=torch.int32, device=self.device)
+        return self._counts
+
+    def count_prompt(self, slot: int, tokens):
+        """A new request's tokens in its slot."""
+        n = torch.tensor([slot, len(tokens)] + list(tokens), dtype=torch.int32).to(self.device, non_blocking=True)
+        ops.count_tokens(self.token_counts(), n[2:].unsqueeze(0), n[1:2], slots=n[:1], prompt=True, reset=True)
+
+    def count_answer(self, slots, tokens):
+        """Tokens that the slots' requests have said: a list for each."""
+        S, P = len(slots), max((len(t) for t in tokens), default=0)
+        if P:
+            n = torch.tensor(list(slots) + [len(t) for t in tokens] + sum((list(t) + [-1] * (P - len(t)) for t in tokens), []), dtype=torch.int32)
+            n = n.to(self.device, non_blocking=True)
+            ops.count_tokens(self.token_counts(), n[2 * S:].view(S, P), n[S: 2 * S], slots=n[:S])
+
+    def logprobs(self, logits: torch.Tensor, tokens, top: int):
+        """(log-probability, rank, [(id, log-probability) of the `top` most probable]) of a token per logits row."""
+        if self.tp is not None:
+            logits = self.tp.gather_vocab(logits)
+        r = ops.token_logprobs(logits, torch.tensor(list(tokens), dtype=torch.int32).to(logits.device, non_blocking=True), top)
+        return [(lp, rank, [(i, x) for i, x in zip(a, b) if i >= 0]) for lp, rank, a, b in zip(*(x.tolist() for x in r))]
 
     def token_prob(self, logits_row: torch.Tensor, token: int) -> float:
         """softmax(logits)[token] for one row; under vocabulary parallelism the maximum and the exponent sum are

@@ -607,11 +607,4 @@ from .tree import block_tables, commit_paths, path_conv, slot_maps, tree_attenti
 
 
 # ----------------------------------------------------------------------------- from logits to tokens
-from .sampling import Logprobs, adjust_logits, count_tokens, sample_tokens, token_logprobs  # noqa: E402, F401
-
-
-def __getattr__(name):
-    if name == "Adjust":                           # (of the bindings, loaded on first use)
-        from . import sampling
-        return sampling.Adjust
-    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+from .sampling import Adjust, Logprobs, adjust_logits, count_tokens, sample_tokens, token_logprobs  # noqa: E402, F401

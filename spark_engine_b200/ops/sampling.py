@@ -14,7 +14,7 @@ import importlib.util
 import math
 import os
 import sysconfig
-from typing import NamedTuple
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -77,20 +77,17 @@ def _count():
     cuda_ops().add_launches(_mod.take_launched())
 
 
-def __getattr__(name):
-    if name == "Adjust":
-        return _native().Adjust
-    raise AttributeError(name)
-
-
-_none = None
-
-
-def _nothing():
-    global _none
-    if _none is None:
-        _none = _native().Adjust()
-    return _none
+class Adjust(NamedTuple):
+    """What a row's logits go through before a token is drawn; tensors on the logits' device, None: none of the kind."""
+    counts: Optional[torch.Tensor] = None          # int32 [slots, V]: 2 * times generated + (1 if in the prompt), see `count_tokens`
+    slots: Optional[torch.Tensor] = None           # int32 [R]: a row's row of counts (None: its number; negative: the row has no penalties)
+    drafted: Optional[torch.Tensor] = None         # int32 [R, n]: tokens on the way to the row that count as generated on top, negative: none
+    repetition: Optional[torch.Tensor] = None      # fp32 [R]
+    presence: Optional[torch.Tensor] = None        # fp32 [R]
+    frequency: Optional[torch.Tensor] = None       # fp32 [R]
+    bias_ids: Optional[torch.Tensor] = None        # int32 [R, n]: ids whose logits get the biases (each of an id's), negative: none
+    bias: Optional[torch.Tensor] = None            # fp32 [R, n]
+    allowed: Optional[torch.Tensor] = None         # int32 [R, (V + 31) / 32]: bit c % 32 of word c / 32 says whether column c may be drawn
 
 
 # ----------------------------------------------------------------------------- counts
@@ -119,7 +116,7 @@ def count_tokens(counts, tokens, n, slots=None, prompt: bool = False, reset: boo
 
 
 # ----------------------------------------------------------------------------- adjustments
-def adjust_logits(logits, adjust: "Adjust", offset: int = 0, out=None) -> torch.Tensor:
+def adjust_logits(logits, adjust: Adjust, offset: int = 0, out=None) -> torch.Tensor:
     """fp32 logits [R, V] after a row's adjustments: of tokens that were generated (or drafted) or are in the prompt, z / repetition where z > 0, else
     z * repetition; minus frequency times the times generated, minus presence if generated; plus the biases of the id; -inf where not allowed.  Logits fp32,
     bf16 or fp16, of ids offset .. offset + V (counts and allowed words are of these columns, ids in the lists are the vocabulary's).  Into `out` if
@@ -165,7 +162,7 @@ def _plain_adjust(logits, a, offset: int = 0):
 
 
 # ----------------------------------------------------------------------------- tokens
-def sample_tokens(logits, temps, seeds, positions, top_k=None, top_p=None, min_p=None, adjust: "Adjust" = None) -> torch.Tensor:
+def sample_tokens(logits, temps, seeds, positions, top_k=None, top_p=None, min_p=None, adjust: Optional[Adjust] = None) -> torch.Tensor:
     """One token per row of logits [R, V] (fp32, bf16, fp16; after `adjust` if given): int32 [R], -1 where a row has none.  temps, top_p, min_p fp32 [R],
     top_k int32 [R], seeds and positions int64 [R].  Kept are the first top_k tokens of the row's order (<= 0: all); of these the ones at least min_p
     times as probable as the first (<= 0: all); of these the shortest run of the order that has top_p of their probability (>= 1: all; one at least).
@@ -174,7 +171,7 @@ def sample_tokens(logits, temps, seeds, positions, top_k=None, top_p=None, min_p
 
     Probabilities are summed in whole numbers of 2^-40 of the best token's: which token is the last one kept is the same in every batch."""
     run = _kernels(logits)
-    t = _native().sample_tokens(logits, temps, seeds, positions, top_k, top_p, min_p, adjust if adjust is not None else _nothing(), run)
+    t = _native().sample_tokens(logits, temps, seeds, positions, top_k, top_p, min_p, adjust, run)
     if run:
         _count()
         return t

@@ -169,6 +169,13 @@ class TPBase:
         uncombined expert outputs)."""
         return self.allreduce(ops.to_tensor(delta).float())
 
+    def gather_vocab(self, logits_local: torch.Tensor) -> torch.Tensor:
+        """Logits of the whole vocabulary on every rank (rows of a round whose draws look at all of it)."""
+        x = logits_local.contiguous()
+        parts = [torch.empty_like(x) for _ in range(self.world)]
+        dist.all_gather(parts, x, group=getattr(self, "group", None))
+        return torch.cat(parts, 1)
+
     def greedy(self, logits_local: torch.Tensor, vocab_local: int) -> torch.Tensor:
         """Global arg-max from vocabulary-parallel logits: (value, index) packets, ties -> lowest id."""
         val, idx = logits_local.max(-1)

@@ -68,7 +68,7 @@ class EngineClient:
         with self.lock:
             self.sock.sendall(proto.encode(msg))
 
-    def generate(self, prompt_ids: List[int], max_new: int, stop_ids: List[int], temperature: float, seed: int, mm=None):
+    def generate(self, prompt_ids: List[int], max_new: int, stop_ids: List[int], temperature: float, seed: int, mm=None, sampling=None):
         with self.lock:
             rid = self.next_id
             self.next_id += 1
@@ -77,6 +77,7 @@ class EngineClient:
                "temperature": temperature, "seed": seed}
         if mm:
             msg["mm"] = mm                      # canvas files + the prompt positions of their salted placeholder runs
+        msg.update(sampling or {})              # top_k, top_p, min_p, penalties, biases, log-probabilities (serving/protocol.py)
         self._send(msg)
         return rid, q
 
@@ -178,6 +179,55 @@ def parse_tool_calls(text: str):
     return _TOOL_RE.sub("", text).strip() if calls else text, calls
 
 
+def sampling_fields(body: dict, chat: bool) -> dict:
+    """What a request's body says about its draws beyond temperature and seed, in the fields of the line protocol; checks of ranges are the engine's."""
+    f = {k: body[k] for k in ("top_p", "top_k", "min_p", "presence_penalty", "frequency_penalty", "repetition_penalty") if body.get(k) is not None}
+    bias = body.get("logit_bias")
+    if bias:
+        if not isinstance(bias, dict):
+            raise ValueError("logit_bias must be an object of token ids")
+        f["logit_bias"] = [[int(t), b] for t, b in bias.items()]
+    if chat:
+        if body.get("logprobs"):
+            f["logprobs"] = body.get("top_logprobs") or 0
+        elif body.get("top_logprobs"):
+            raise ValueError("top_logprobs needs logprobs")
+    elif body.get("logprobs") is not None and body.get("logprobs") is not False:
+        f["logprobs"] = int(body["logprobs"])
+    return f
+
+
+class LogprobLog:
+    """Log-probabilities of an answer in the API's form; `take` gives those since it was last asked."""
+
+    def __init__(self, tok, chat: bool):
+        self.tok, self.chat, self.entries, self.taken, self.offset = tok, chat, [], 0, 0
+
+    def _text(self, i: int) -> str:
+        return self.tok.decode([i])
+
+    def feed(self, ids: List[int], got: List[list]):
+        for t, (lp, _, top) in zip(ids, got):
+            text = self._text(t)
+            raw = lambda s: list(s.encode())
+            if self.chat:
+                self.entries.append({"token": text, "logprob": lp, "bytes": raw(text),
+                                     "top_logprobs": [{"token": self._text(i), "logprob": x, "bytes": raw(self._text(i))} for i, x in top]})
+            else:
+                self.entries.append((text, lp, {self._text(i): x for i, x in top}, self.offset))
+                self.offset += len(text)
+
+    def form(self, entries) -> dict:
+        if self.chat:
+            return {"content": entries}
+        return {"tokens": [e[0] for e in entries], "token_logprobs": [e[1] for e in entries], "top_logprobs": [e[2] for e in entries],
+                "text_offset": [e[3] for e in entries]}
+
+    def take(self) -> dict:
+        new, self.taken = self.entries[self.taken:], len(self.entries)
+        return self.form(new)
+
+
 class App:
     def __init__(self, engine: EngineClient, tokenizer, model_name: str, max_new_default: int = 256, media: Optional[dict] = None):
         self.engine, self.tok, self.model_name, self.max_new_default = engine, tokenizer, model_name, max_new_default
@@ -213,8 +263,13 @@ class App:
         stops = [stops] if isinstance(stops, str) else list(stops)
         eos = getattr(self.tok, "eos_token_id", None)
         t0 = time.time()
+        sampling = sampling_fields(body, chat)
         rid, q = self.engine.generate(prompt_ids, max_new, [eos] if eos is not None else [], float(body.get("temperature", 0.0) or 0.0),
-                                      int(body.get("seed", 0) or 0), mm=mm)
+                                      int(body.get("seed", 0) or 0), mm=mm, **({"sampling": sampling} if sampling else {}))
+        lps = LogprobLog(self.tok, chat) if sampling.get("logprobs", -1) >= 0 else None
+        if lps is not None and write_event:
+            plain_event = write_event
+            write_event = lambda r, c: plain_event(r, c, lps.take())       # noqa: E731
         detok, ss, rs = IncrementalDetok(self.tok), StopStrings(stops), ReasoningSplit(chat)
         content, reasoning, itls, last_t, done, finish = "", "", [], None, None, "length"
         try:
@@ -234,6 +289,9 @@ class App:
                     if last_t is not None:
                         itls.append((now - last_t) / max(len(msg["delta"]), 1))
                     last_t = now
+                    if lps is not None:
+                        keep = [i for i, t in enumerate(msg["delta"]) if t != eos and i < len(msg.get("logprobs", ()))]
+                        lps.feed([msg["delta"][i] for i in keep], [msg["logprobs"][i] for i in keep])
                     text, hit = ss.feed(detok.feed([t for t in msg["delta"] if t != eos]))
                     r, c = rs.feed(text)
                     reasoning += r
@@ -259,7 +317,8 @@ class App:
         self.metrics.finish(dict(done, finish_reason=finish), time.time() - t0, itls)
         usage = {"prompt_tokens": len(prompt_ids), "completion_tokens": len(done.get("token_ids", [])),
                  "total_tokens": len(prompt_ids) + len(done.get("token_ids", []))}
-        return {"content": content, "reasoning": reasoning, "finish": finish, "usage": usage, "engine": done}
+        return {"content": content, "reasoning": reasoning, "finish": finish, "usage": usage, "engine": done,
+                "logprobs": None if lps is None else lps.form(lps.entries), "logprobs_left": lps.take() if lps is not None and lps.taken < len(lps.entries) else None}
 
 
 def make_handler(app: App):
@@ -337,6 +396,8 @@ def make_handler(app: App):
                     choice = {"index": 0, "message": msg, "finish_reason": "tool_calls" if calls else r["finish"]}
                 else:
                     choice = {"index": 0, "text": r["content"], "finish_reason": r["finish"]}
+                if r["logprobs"] is not None:
+                    choice["logprobs"] = r["logprobs"]
                 return self._json(200, {"id": cid, "object": obj, "created": created, "model": app.model_name,
                                         "choices": [choice], "usage": r["usage"]})
             self.send_response(200)
@@ -354,7 +415,7 @@ def make_handler(app: App):
                 except (BrokenPipeError, ConnectionResetError, OSError):
                     gone["v"] = True
 
-            def ev(reasoning, content):
+            def ev(reasoning, content, logprobs=None):
                 if chat:
                     d = {}
                     if reasoning:
@@ -364,6 +425,8 @@ def make_handler(app: App):
                     choice = {"index": 0, "delta": d, "finish_reason": None}
                 else:
                     choice = {"index": 0, "text": content, "finish_reason": None}
+                if logprobs is not None:
+                    choice["logprobs"] = logprobs
                 chunk(json.dumps({"id": cid, "object": obj + ".chunk", "created": created, "model": app.model_name, "choices": [choice]}))
             if chat:
                 chunk(json.dumps({"id": cid, "object": obj + ".chunk", "created": created, "model": app.model_name,
@@ -371,6 +434,8 @@ def make_handler(app: App):
             r = app.run(ids, body, chat, ev, lambda: gone["v"], mm=mm)
             last = {"index": 0, "finish_reason": r["finish"]}
             last["delta" if chat else "text"] = {} if chat else ""
+            if r["logprobs_left"] is not None:
+                last["logprobs"] = r["logprobs_left"]
             final = {"id": cid, "object": obj + ".chunk", "created": created, "model": app.model_name, "choices": [last]}
             if (body.get("stream_options") or {}).get("include_usage"):
                 final["usage"] = r["usage"]

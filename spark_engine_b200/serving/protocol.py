@@ -1,8 +1,9 @@
 """Engine <-> front-end line protocol: newline-delimited JSON over a Unix socket.
 
-Requests : {"id", "prompt_ids", "max_new", "stop_token_ids", "temperature", "seed"[, "mm"]}
+Requests : {"id", "prompt_ids", "max_new", "stop_token_ids", "temperature", "seed"[, "mm"][, "top_k", "top_p", "min_p", "repetition_penalty",
+            "presence_penalty", "frequency_penalty", "logit_bias": [[token, bias], ...], "logprobs": most probable tokens reported per token]}
            {"cancel": id}   {"id", "stats": true}   {"shutdown": true}
-Replies  : {"id", "queued": true}   {"id", "delta": [ids]}   {"id", "error": "..."}
+Replies  : {"id", "queued": true}   {"id", "delta": [ids][, "logprobs": [[log-probability, rank, [[id, log-probability], ...]], ...]]}   {"id", "error": "..."}
            {"id", "done": true, "token_ids", "queue_ms", "prefill_ms", "decode_ms", "prefix_hit_tokens", "rounds",
             "accepted_drafts", "drafted_tokens", "finish_reason"}
            {"id", "stats": {...}}
@@ -12,6 +13,8 @@ from __future__ import annotations
 
 import json
 from typing import Any, Dict, List
+
+from ..spec.params import refusal
 
 
 def encode(msg: Dict[str, Any]) -> bytes:
@@ -52,4 +55,4 @@ def validate_request(msg: Dict[str, Any], vocab: int, max_ctx: int) -> str:
         return "max_new must be a positive integer"
     if len(ids) + mn > max_ctx:
         return f"prompt ({len(ids)}) + max_new ({mn}) exceeds the context budget ({max_ctx})"
-    return ""
+    return refusal(msg, vocab)

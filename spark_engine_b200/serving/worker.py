@@ -23,6 +23,7 @@ from ..models.plan import make_plan
 from ..runtime import rt
 from ..spec.decoder import SeqSpec, SpecDecoder
 from ..spec.lookup import LookupIndex
+from ..spec.params import SamplingParams
 from ..utils.profile import Profiler
 from . import protocol as proto
 
@@ -252,7 +253,8 @@ class EngineServer:
         lv.prefix_hit = reuse
         self.totals["prefix_hit_tokens"] += reuse
         self.by_slot[plan.slot] = lv
-        lv.seq = SeqSpec(plan.slot, -1, temperature=float(msg.get("temperature", 0.0)), seed=int(msg.get("seed", 0)))
+        params = SamplingParams.from_message(msg)
+        lv.seq = SeqSpec(plan.slot, -1, temperature=params.temperature, seed=params.seed, params=params if params.shaped else None)
         lv.seq.lookup = LookupIndex(self.spec.lookup_n)
         lv.seq.lookup.extend([t for t in prompt[:reuse] if t < self.cfg.vocab])
         self._log("admit", id=lv.id, slot=plan.slot, kind=str(plan.kind).split(".")[-1], reuse=reuse, prompt=len(prompt),
@@ -300,8 +302,8 @@ class EngineServer:
             if c1 == len(prompt):
                 s = lv.seq
                 h_last = hid[seg.r0 + seg.n - 1].clone()
-                first = m.sample(logits[k], s.temperature, s.seed, len(prompt))
-                s.last_token, s.hidden = first, h_last
+                first = self.spec.first_token(s, logits[k], prompt)
+                s.hidden = h_last
                 s.pending_mtp = [(h_last.clone(), first)]
                 s.generated = [first]
                 s.lookup.extend([first])
@@ -348,6 +350,9 @@ class EngineServer:
         stop = set(msg.get("stop_token_ids", []))
         max_new = int(msg.get("max_new", 256))
         self.out.append({"id": lv.id, "delta": toks})
+        if lv.seq.logprobs:                     # [log-probability, rank, [[id, log-probability], ...]] of each
+            self.out[-1]["logprobs"] = [[lp, rank, [list(x) for x in top]] for lp, rank, top in lv.seq.logprobs[: len(toks)]]
+            lv.seq.logprobs = []
         lv.sent += len(toks)
         self.totals["generation_tokens"] += len(toks)
         done = lv.sent >= max_new or (toks and toks[-1] in stop)

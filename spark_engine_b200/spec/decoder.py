@@ -18,6 +18,7 @@ import torch
 from ..models.plan import make_plan
 from . import policy as P
 from .lookup import LookupIndex
+from .params import SamplingParams
 from .tree import Node, accept, chain, parents_of
 
 
@@ -31,6 +32,8 @@ class SeqSpec:
     lookup: Optional[LookupIndex] = None
     temperature: float = 0.0
     seed: int = 0
+    params: Optional[SamplingParams] = None            # of requests that ask for more than a temperature
+    logprobs: List[tuple] = field(default_factory=list)  # of the tokens that the last round emitted, where asked for
     generated: List[int] = field(default_factory=list)
     drafted: int = 0
     accepted: int = 0
@@ -91,8 +94,9 @@ class SpecDecoder:
         self.rounds = 0
 
     # ---------------------------------------------------------------------------------------------
-    def start(self, slot: int, prompt: Sequence[int], temperature: float = 0.0, seed: int = 0, chunk: int = 4096) -> SeqSpec:
-        """Prefill a fresh sequence and sample its first token."""
+    def start(self, slot: int, prompt: Sequence[int], temperature: float = 0.0, seed: int = 0, chunk: int = 4096,
+              params: Optional[SamplingParams] = None) -> SeqSpec:
+        """Prefill a fresh sequence and sample its first token (by `params` if given, which then hold temperature and seed too)."""
         m = self.m
         m.reset_slot(slot)
         pend, last, hid = [], None, None
@@ -107,13 +111,46 @@ class SpecDecoder:
                 mp = make_plan([(slot, nxt, c0)], device=m.device, all_logits=False) if nxt else None
                 if mp is not None:
                     m.mtp_forward(mp, hid[: len(nxt)])
-        first = m.sample(last, temperature, seed, len(prompt))
-        seq = SeqSpec(slot, first, hid[-1].clone(), temperature=temperature, seed=seed)
+        if params is not None:
+            temperature, seed = params.temperature, params.seed
+        seq = SeqSpec(slot, -1, hid[-1].clone(), temperature=temperature, seed=seed, params=params)
+        first = self.first_token(seq, last, prompt)
         seq.pending_mtp = [(hid[-1].clone(), first)]
         seq.lookup = LookupIndex(self.lookup_n)
         seq.lookup.extend(list(prompt) + [first])
         seq.generated = [first]
         return seq
+
+    def first_token(self, seq: SeqSpec, logits: torch.Tensor, prompt: Sequence[int]) -> int:
+        """The token behind a prompt, from its last row's logits; begins the counts of a request with penalties."""
+        m, p = self.m, seq.params
+        if p is None or not p.shaped:
+            seq.last_token = m.sample(logits, seq.temperature, seq.seed, len(prompt))
+            return seq.last_token
+        if p.counted:
+            m.count_prompt(seq.slot, prompt)
+        seq.last_token = m.draw_rows(logits, [p], [seq.slot], [len(prompt)])[0]
+        self._said([seq], [[seq.last_token]], logits.reshape(1, -1), [[0]])
+        return seq.last_token
+
+    @staticmethod
+    def _params(seq: SeqSpec) -> SamplingParams:
+        return seq.params if seq.params is not None else SamplingParams(seq.temperature, seq.seed)
+
+    def _said(self, seqs: List[SeqSpec], outs: List[List[int]], logits, rows: List[List[int]]):
+        """What a round emitted: counted, and its log-probabilities from the rows that its tokens come from (rows[i][j] for outs[i][j])."""
+        counted = [i for i, s in enumerate(seqs) if s.params is not None and s.params.counted]
+        if counted:
+            self.m.count_answer([seqs[i].slot for i in counted], [outs[i] for i in counted])
+        asked = [i for i, s in enumerate(seqs) if s.params is not None and s.params.logprobs >= 0]
+        if not asked:
+            return
+        at = [r for i in asked for r in rows[i][: len(outs[i])]]
+        got = self.m.logprobs(logits[at], [t for i in asked for t in outs[i]], max(seqs[i].params.logprobs for i in asked))
+        for i in asked:
+            n, got_i = len(outs[i]), got
+            got = got_i[n:]
+            seqs[i].logprobs = [(lp, rank, top[: seqs[i].params.logprobs]) for lp, rank, top in got_i[:n]]
 
     def _draft(self, seq: SeqSpec, depth: int):
         if depth <= 0:
@@ -185,14 +222,20 @@ class SpecDecoder:
             draft_confs.append(list(c[:k]))
         toks = [[s.last_token] + d for s, d in zip(seqs, drafts)]
         temps, seeds = [s.temperature for s in seqs], [s.seed for s in seqs]
+        shaped = any(s.params is not None and s.params.shaped for s in seqs)
         if use_g and max(len(t) for t in toks) <= k_graph:
             # captured verify: every sequence padded to the layout's rows; the commit replays device-side counts
             k = k_graph if any(drafts) else 1
             vg = self.graphs.round_graph([s.slot for s in seqs], k, max(L) + k)
-            vg.stage(toks, L, temps, seeds)
+            vg.stage(toks, L, None if shaped else temps, seeds)       # (shaped: logits stay as they are, draws follow the replay)
             vg.run(commit=(k == 1))
-            torch.cuda.current_stream().synchronize()
-            flat = vg.out_host.tolist()
+            logits = vg.logits
+            if shaped:
+                flat = self._draw(seqs, toks, L, logits)
+                flat = [x for i, t in enumerate(toks) for x in flat[i] + [0] * (k - len(t))]
+            else:
+                torch.cuda.current_stream().synchronize()
+                flat = vg.out_host.tolist()
             all_preds = [flat[i * k: i * k + len(t)] for i, t in enumerate(toks)]
             hidden = vg.hidden.clone()                   # the next replay overwrites the graph's buffer
             row0 = [i * k for i in range(len(seqs))]
@@ -202,11 +245,14 @@ class SpecDecoder:
             plan = make_plan([(s.slot, t, l) for s, t, l in zip(seqs, toks, L)], device=m.device)
             logits = m.forward(plan, commit=False)
             hidden = m.hidden_out
-            rows_of = [(s, seg.pos0 + 1 + j) for s, seg in zip(seqs, plan.segs) for j in range(seg.n)]
-            flat = m.sample_rows(logits, [s.temperature for s, _ in rows_of], [s.seed for s, _ in rows_of],
-                                 [p for _, p in rows_of])
-            all_preds = [flat[seg.r0: seg.r0 + seg.n] for seg in plan.segs]
             row0 = [seg.r0 for seg in plan.segs]
+            if shaped:
+                all_preds = self._draw(seqs, toks, L, logits, row0)
+            else:
+                rows_of = [(s, seg.pos0 + 1 + j) for s, seg in zip(seqs, plan.segs) for j in range(seg.n)]
+                flat = m.sample_rows(logits, [s.temperature for s, _ in rows_of], [s.seed for s, _ in rows_of],
+                                     [p for _, p in rows_of])
+                all_preds = [flat[seg.r0: seg.r0 + seg.n] for seg in plan.segs]
         emitted, accepted_rows = [], []
         for i, (s, d) in enumerate(zip(seqs, drafts)):
             preds = all_preds[i]
@@ -225,6 +271,8 @@ class SpecDecoder:
             s.drafted += len(d)
             s.accepted += n
             emitted.append(out)
+        if shaped:
+            self._said(seqs, emitted, logits, [[r0 + r for r in rows] for r0, rows in zip(row0, accepted_rows)])
         if vg is None:
             m.commit(accepted_rows)
         else:
@@ -292,7 +340,18 @@ class SpecDecoder:
             temps += [s.temperature] * seg.n
             seeds += [s.seed] * seg.n
             poss += [seg.pos0 + 1 + d for d in depth]
-        all_preds = m.sample_rows(logits, temps, seeds, poss)
+        shaped = any(s.params is not None and s.params.shaped for s in seqs)
+        if shaped:
+            paths = []
+            for nodes in trees:
+                lines = [[]]
+                for nd in nodes:
+                    lines.append(lines[nd.parent + 1] + [nd.token])
+                paths += lines
+            owners = [s for s, seg in zip(seqs, plan.segs) for _ in range(seg.n)]
+            all_preds = m.draw_rows(logits, [self._params(s) for s in owners], [s.slot for s in owners], poss, paths)
+        else:
+            all_preds = m.sample_rows(logits, temps, seeds, poss)
         for i, (s, nodes) in enumerate(zip(seqs, trees)):
             seg = plan.segs[i]
             preds = all_preds[seg.r0: seg.r0 + seg.n]
@@ -304,6 +363,8 @@ class SpecDecoder:
             s.drafted += len(nodes)
             s.accepted += len(path)
             emitted.append(out)
+        if shaped:
+            self._said(seqs, emitted, logits, [[seg.r0 + r for r in rows] for seg, rows in zip(plan.segs, accepted_rows)])
         m.commit(accepted_rows)
         for i, (s, out) in enumerate(zip(seqs, emitted)):
             seg, rows = plan.segs[i], accepted_rows[i]
@@ -316,9 +377,24 @@ class SpecDecoder:
         self.rounds += 1
         return emitted
 
+    def _draw(self, seqs: List[SeqSpec], toks: List[List[int]], L: List[int], logits: torch.Tensor, row0=None) -> List[List[int]]:
+        """Tokens of chains' rows by their requests' settings: toks[i] are the rows of sequence i (its last token, then drafts), of which the first is
+        row0[i] of the logits (None: every sequence has as many)."""
+        per = logits.shape[0] // len(seqs)
+        row0 = row0 if row0 is not None else [i * per for i in range(len(seqs))]
+        owners = [(s, i, j) for i, (s, t) in enumerate(zip(seqs, toks)) for j in range(len(t))]
+        at = [row0[i] + j for _, i, j in owners]
+        flat = self.m.draw_rows(logits if at == list(range(logits.shape[0])) else logits[at], [self._params(s) for s, _, _ in owners], [s.slot for s, _, _ in owners],
+                                [L[i] + 1 + j for _, i, j in owners], [toks[i][1: j + 1] for _, i, j in owners])
+        out, r = [], 0
+        for t in toks:
+            out.append(flat[r: r + len(t)])
+            r += len(t)
+        return out
+
     def generate(self, prompts: List[Sequence[int]], max_new: int, stop: Sequence[int] = (), temperature: float = 0.0,
-                 seed: int = 0) -> List[List[int]]:
-        seqs = [self.start(i, p, temperature, seed) for i, p in enumerate(prompts)]
+                 seed: int = 0, params: Optional[SamplingParams] = None) -> List[List[int]]:
+        seqs = [self.start(i, p, temperature, seed, params=params) for i, p in enumerate(prompts)]
         live = [s for s in seqs if len(s.generated) < max_new and s.generated[-1] not in stop]
         while live:
             budgets = [max_new - len(s.generated) for s in live]

@@ -1,0 +1,256 @@
+"""Requests with filters, penalties, biases and log-probabilities: in speculative rounds, the server and its HTTP front end, over a sharded vocabulary."""
+import json
+import threading
+import urllib.error
+import urllib.request
+
+import numpy as np
+import pytest
+import torch
+
+from spark_engine_b200.config import EngineConfig, tiny_hybrid
+from spark_engine_b200.models.model import Model
+from spark_engine_b200.models.weights import init_weights, to_device
+from spark_engine_b200.serving.protocol import validate_request
+from spark_engine_b200.serving.worker import EngineServer
+from spark_engine_b200.spec.decoder import SpecDecoder
+from spark_engine_b200.spec.params import SamplingParams
+from spark_engine_b200.spec.tree import Node
+from tests.sampling_util import want_logprobs, want_token
+
+WILD = SamplingParams(temperature=1.1, seed=5, top_k=40, top_p=0.9, min_p=0.01, repetition=1.3, presence=0.4, frequency=0.2, bias=((7, 3.0), (9, -100.0)), logprobs=3)
+SETTINGS = [WILD, SamplingParams(temperature=0.9, seed=8, top_p=0.7), SamplingParams(frequency=1.5, logprobs=0), SamplingParams(temperature=1.3, seed=2)]
+
+
+def _model(device="cpu", slots=4):
+    cfg = tiny_hybrid()
+    cfg.mtp_layers, cfg.mtp_depth = 1, 3
+    W = init_weights(cfg, seed=0)
+    if device != "cpu":
+        W = to_device(W, device)
+    return cfg, W, Model(cfg, W, device=device, dtype=torch.float32 if device == "cpu" else torch.bfloat16, n_slots=slots, kv_tokens=512 * slots)
+
+
+def _prompts(cfg, n, seed=1):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.randint(0, cfg.vocab, (20 + 9 * i,), generator=g).tolist() for i in range(n)]
+
+
+def _text(sd, prompts, params, n):
+    """Every sequence with settings of its own, n tokens each, and their log-probabilities."""
+    seqs = [sd.start(i, p, params=q) for i, (p, q) in enumerate(zip(prompts, params))]
+    lps = [list(s.logprobs) for s in seqs]
+    while any(len(s.generated) < n for s in seqs):
+        live = [s for s in seqs if len(s.generated) < n]
+        sd.round(live, [n - len(s.generated) for s in live])
+        for s in live:
+            lps[seqs.index(s)] += s.logprobs
+    return [s.generated for s in seqs], lps
+
+
+def _by_definition(z, p, seed_pos, prompt, said):
+    """Next token from fp32 logits `z` of a row behind prompt + said."""
+    z = z.copy()
+    f = np.float32
+    c = np.bincount(said, minlength=len(z)) if said else np.zeros(len(z), int)
+    seen = c > 0
+    seen[prompt] = True
+    z = np.where(seen, np.where(z > 0, z / f(p.repetition), z * f(p.repetition)), z)
+    z = z - f(p.frequency) * c.astype(f) - f(p.presence) * (c > 0).astype(f)
+    for t, b in p.bias:
+        z[t] += f(b)
+    return want_token(z, p.temperature, p.seed, seed_pos, p.top_k, p.top_p, p.min_p)
+
+
+def test_plain_rounds_draw_by_the_definitions(monkeypatch):
+    """One row at a time: every token is the definition's, from the row's own logits and what the request has said."""
+    cfg, _, m = _model()
+    prompts = _prompts(cfg, 4)
+    rows = []
+    real = m.draw_rows
+    monkeypatch.setattr(m, "draw_rows", lambda lg, *a: rows.append((lg.float().reshape(-1, cfg.vocab).numpy().copy(), a)) or real(lg, *a))
+    texts, lps = _text(SpecDecoder(m, lambda s, d: ([], []), depth=0), prompts, SETTINGS, 12)
+    logits = {(s, pos): z for lg, (_, slots, positions, *_) in rows for z, s, pos in zip(lg, slots, positions)}
+    for i, (p, text) in enumerate(zip(SETTINGS, texts)):
+        if not p.shaped:
+            continue
+        for j, t in enumerate(text):
+            z = logits[i, len(prompts[i]) + j]
+            assert t == _by_definition(z, p, len(prompts[i]) + j, prompts[i], text[:j]), (i, j)
+            if p.logprobs >= 0:
+                lp, rank, ids, top = want_logprobs(z, t, p.logprobs)
+                got = lps[i][j]
+                assert got[1] == rank and [a for a, _ in got[2]] == [int(a) for a in ids]
+                assert abs(got[0] - lp) < 1e-5 and all(abs(x - y) < 1e-5 for (_, x), y in zip(got[2], top))
+        assert len(lps[i]) == (len(text) if p.logprobs >= 0 else 0)
+    assert len(set(map(tuple, texts))) == 4
+
+
+def check_speculation(device, graphs):
+    """Drafts (right, half right, none; chains and trees) change nothing about the text."""
+    cfg, W, m = _model(device)
+    prompts = _prompts(cfg, 4)
+    want, want_lps = _text(SpecDecoder(m, lambda s, d: ([], []), depth=0), prompts, SETTINGS, 14)
+    by_slot = dict(enumerate(want))
+
+    def drafter(seq, depth):
+        d = by_slot[seq.slot][len(seq.generated): len(seq.generated) + depth]
+        if seq.slot == 1:
+            d = d[:1] + [(t + 1) % cfg.vocab for t in d[1:]]
+        return d, [0.9] * len(d)
+    _, _, m2 = _model(device)
+    sd = SpecDecoder(m2, drafter, depth=3, graphs=graphs)
+    got, lps = _text(sd, prompts, SETTINGS, 14)
+    assert got == want and sd.rounds < 14
+    assert bool(sd.graphs is not None and sd.graphs.rounds) == graphs
+    for a, b in zip(lps, want_lps):
+        assert [x[1] for x in a] == [x[1] for x in b]
+    if graphs:
+        return
+    _, _, m3 = _model(device)
+    sd = SpecDecoder(m3, lambda s, d: ([], []), depth=0)
+    seqs = [sd.start(i, p, params=q) for i, (p, q) in enumerate(zip(prompts, SETTINGS))]
+    while any(len(s.generated) < 14 for s in seqs):
+        live = [s for s in seqs if len(s.generated) < 14]
+        trees = []
+        for s in live:
+            right = (want[s.slot][len(s.generated): len(s.generated) + 2] + [0, 0])[:2]
+            wrong = (right[0] + 1) % cfg.vocab
+            trees.append([Node(token=t, parent=a) for t, a in ((wrong, -1), (right[0], -1), (right[1], 0), (right[1], 1))])
+        sd.round_tree(live, trees, [14 - len(s.generated) for s in live])
+    assert [s.generated for s in seqs] == want
+
+
+def test_speculation_keeps_the_text():
+    check_speculation("cpu", False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("graphs", [False, True])
+def test_speculation_keeps_the_text_on_the_device(graphs):
+    check_speculation("cuda", graphs)
+
+
+# ----------------------------------------------------------------------------- the server
+def _message(i, prompt, p, n):
+    return {"id": i, "prompt_ids": prompt, "max_new": n, "temperature": p.temperature, "seed": p.seed, "top_k": p.top_k, "top_p": p.top_p, "min_p": p.min_p,
+            "repetition_penalty": p.repetition, "presence_penalty": p.presence, "frequency_penalty": p.frequency, "logit_bias": [list(b) for b in p.bias], "logprobs": p.logprobs}
+
+
+def check_server(device):
+    """More requests than slots, shared rounds: the text and log-probabilities are those of a request alone."""
+    cfg, W, m = _model(device)
+    prompts = _prompts(cfg, 4)
+    alone, alone_lps = [], []
+    for p, q in zip(prompts, SETTINGS):
+        t, lp = _text(SpecDecoder(m, lambda s, d: ([], []), depth=0), [p], [q], 10)
+        alone += t
+        alone_lps += lp
+    es = EngineServer(cfg, W, EngineConfig(max_seqs=2, kv_tokens=2048, prefill_chunk=32, spec="mtp", spec_depth=2, cuda_graphs=device != "cpu"), device=device)
+    for turn in range(2):                                                # (the second time over used slots and kept prefixes)
+        for i, (p, q) in enumerate(zip(prompts, SETTINGS)):
+            es.submit(_message(10 * turn + i, p, q, 10))
+        while es.sched.has_work():
+            es.step()
+        out, es.out = es.out, []
+        for i, q in enumerate(SETTINGS):
+            mine = [x for x in out if x.get("id") == 10 * turn + i]
+            assert [x for x in mine if x.get("done")][0]["token_ids"] == alone[i], (turn, i)
+            got = sum((x.get("logprobs", []) for x in mine if "delta" in x), [])
+            assert len(got) == len(alone_lps[i]) and [x[1] for x in got] == [x[1] for x in alone_lps[i]]
+
+
+def test_server_draws_as_a_request_alone():
+    check_server("cpu")
+
+
+@pytest.mark.gpu
+def test_server_draws_as_a_request_alone_on_the_device():
+    check_server("cuda")
+
+
+@pytest.mark.parametrize("bad", [dict(top_p=1.5), dict(top_p="x"), dict(top_k=1.5), dict(top_k=True), dict(min_p=-0.1), dict(presence_penalty=float("nan")), dict(repetition_penalty=0),
+                                 dict(logprobs=21), dict(logit_bias=[[500000, 1.0]]), dict(logit_bias=[[1, 101]]), dict(logit_bias=[[1]]), dict(logit_bias=[[1.5, 1]]),
+                                 dict(logit_bias={"1": 2}), dict(logit_bias=[[1, 0.0]] * 1025), dict(frequency_penalty=11)])
+def test_requests_are_refused(bad):
+    assert validate_request({"prompt_ids": [1], "max_new": 3, **bad}, 1000, 64) != ""
+    assert validate_request({"prompt_ids": [1], "max_new": 3, "top_p": 0.5, "top_k": -1, "logit_bias": [[3, -100]], "logprobs": 20}, 1000, 64) == ""
+
+
+def test_http_front_end(tmp_path):
+    from spark_engine_b200.serving.openai_server import serve
+    cfg, W, _ = _model()
+    sock = str(tmp_path / "e.sock")
+    es = EngineServer(cfg, W, EngineConfig(max_seqs=2, kv_tokens=2048, prefill_chunk=32, spec="mtp", spec_depth=2))
+    ready = threading.Event()
+    threading.Thread(target=es.serve_forever, args=(sock,), kwargs={"ready_cb": ready.set}, daemon=True).start()
+    assert ready.wait(30)
+    srv, app = serve(sock, "127.0.0.1", 0, "tiny")
+    threading.Thread(target=srv.serve_forever, daemon=True).start()
+
+    def post(path, body):
+        req = urllib.request.Request(f"http://127.0.0.1:{srv.server_address[1]}{path}", json.dumps(body).encode(), {"Content-Type": "application/json"})
+        return urllib.request.urlopen(req, timeout=120).read().decode()
+    try:
+        ask = {"prompt": "abc", "max_tokens": 6, "temperature": 1.0, "seed": 3, "top_p": 0.8, "top_k": 30, "frequency_penalty": 0.5, "logit_bias": {"65": 2.0}}
+        plain = json.loads(post("/v1/completions", ask))["choices"][0]
+        assert "logprobs" not in plain
+        one = json.loads(post("/v1/completions", {**ask, "logprobs": 2}))["choices"][0]
+        assert one["text"] == plain["text"]
+        lp = one["logprobs"]
+        assert len(lp["tokens"]) == len(lp["token_logprobs"]) == len(lp["top_logprobs"]) == len(lp["text_offset"]) == 6 and all(x <= 0 for x in lp["token_logprobs"])
+        chat = {"messages": [{"role": "user", "content": "hi"}], "max_tokens": 5, "temperature": 0.9, "seed": 1, "min_p": 0.01, "logprobs": True, "top_logprobs": 3}
+        whole = json.loads(post("/v1/chat/completions", chat))["choices"][0]["logprobs"]["content"]
+        assert len(whole) == 5 and all(len(e["top_logprobs"]) == 3 for e in whole)
+        lines = [json.loads(x[6:]) for x in post("/v1/chat/completions", {**chat, "stream": True}).split("\n") if x.startswith("data: {")]
+        parts = sum((c["logprobs"]["content"] for x in lines for c in x["choices"] if c.get("logprobs")), [])
+        assert parts == whole
+        for bad in ({"top_p": 2.0}, {"logit_bias": {"x": 1}}, {"logit_bias": [1]}, {"logprobs": 50}):
+            with pytest.raises(urllib.error.HTTPError) as e:
+                post("/v1/completions", {**ask, **bad})
+            assert e.value.code == 400
+        with pytest.raises(urllib.error.HTTPError):
+            post("/v1/chat/completions", {**chat, "logprobs": False})
+    finally:
+        srv.shutdown()
+        es.shutdown = True
+
+
+# ----------------------------------------------------------------------------- a sharded vocabulary
+def _rank(rank, port, q):
+    import os
+
+    import torch.distributed as dist
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+    dist.init_process_group("gloo", rank=rank, world_size=2)
+    from spark_engine_b200.models.plan import make_plan
+    from spark_engine_b200.parallel.tp import CpuTP, shard_dense_weights
+    cfg = tiny_hybrid()
+    m = Model(cfg, shard_dense_weights(init_weights(cfg, seed=0), cfg, rank, 2), n_slots=1, kv_tokens=128, tp=CpuTP())
+    lg = m.forward(make_plan([(0, list(range(5, 37)), 0)]))
+    m.count_prompt(0, list(range(5, 37)))
+    got = m.draw_rows(lg, [WILD] * 32, [0] * 32, list(range(32)), [[3, 3]] * 32)
+    lps = m.logprobs(lg, got, 3)
+    q.put((rank, got, lps, m.tp.gather_vocab(lg).numpy()))
+    dist.barrier()
+    dist.destroy_process_group()
+
+
+def test_a_sharded_vocabulary_draws_the_same():
+    import torch.multiprocessing as mp
+    from test_tp_cpu import _free_port
+    ctx = mp.get_context("spawn")
+    q, port = ctx.Queue(), _free_port()
+    ps = [ctx.Process(target=_rank, args=(r, port, q)) for r in range(2)]
+    for p in ps:
+        p.start()
+    got = sorted((q.get(timeout=120) for _ in ps), key=lambda x: x[0])
+    for p in ps:
+        p.join(timeout=60)
+        assert p.exitcode == 0
+    assert got[0][1:3] == got[1][1:3] and np.array_equal(got[0][3], got[1][3])
+    z = got[0][3]
+    for r in range(32):
+        assert got[0][1][r] == _by_definition(z[r], WILD, r, list(range(5, 37)), [3, 3])
+        lp, rank, ids, _ = want_logprobs(z[r], got[0][1][r], 3)
+        assert got[0][2][r][1] == rank and abs(got[0][2][r][0] - lp) < 1e-5
