@@ -23,6 +23,7 @@ constexpr int BINS = 1024;                         // of a sixteenth of a bit of
 constexpr float BINS_PER_BIT = 16.f;
 constexpr int LIST = 2048;
 constexpr int HITS = 512;
+template <int NT> constexpr int FEW_OF = NT < 256 ? NT : 256;       // of the list: ordered by counting
 constexpr int CLUSTER_MAX = 8;
 
 using u64 = unsigned long long;
@@ -66,7 +67,7 @@ template <int NT>
 struct RowShared {
   Mailboxes mail;
   unsigned hist[BINS], hits[HITS];
-  u64 list[LIST], weight[NT / 2], wsum[NT / 32];
+  u64 list[LIST], weight[FEW_OF<NT>], wsum[NT / 32];
   float fsum[NT / 32];
   unsigned n_list, n_hits, before, kept;
   int bin, score;
@@ -134,13 +135,13 @@ struct Row {
       for (int e = 0; e < N; ++e) v[i * N + e] = plain_logit(f[e]);
     }
   }
-  // f(32 logits, chunk's number in the CTA) for each of a warp's chunks; what it reads AHEAD chunks later is asked for.
+  // f(32 logits, chunk's number in the CTA) for each of a warp's chunks; what it reads AHEAD chunks later is asked for (0: nothing).
   template <int AHEAD, class F>
   __device__ __forceinline__ void stream(F f) const {
     for (int k = threadIdx.x >> 5; k < chunks; k += WARPS) {
       float v[32];
       const int j = (chunk0 + k + AHEAD * WARPS) * CHUNK + (threadIdx.x & 31) * 32;          // (a lane: 128 bytes of fp32)
-      if (k + AHEAD * WARPS < chunks && j < hi) asm volatile("prefetch.global.L2 [%0];" ::"l"(base + j));
+      if (AHEAD && k + AHEAD * WARPS < chunks && j < hi) asm volatile("prefetch.global.L2 [%0];" ::"l"(base + j));
       load(chunk0 + k, 0, threadIdx.x & 31, v);
       f(v, k);
     }
@@ -171,27 +172,28 @@ struct Row {
   }
 };
 
-// The largest logits of groups of 8 << shift values of a lane; group (k, q, lane) at (k * (4 >> shift) + q) * 32 + lane.
+// The largest logits of groups of 1 << lg values of a lane (8 to 32); group (k, q, lane) at (k * (32 >> lg) + q) * 32 + lane.
 struct Groups {
   float* g;
-  int shift;
+  int lg;
   __device__ __forceinline__ void put(const float (&m)[4], int k) const {
     const int lane = threadIdx.x & 31;
-    if (shift == 0) {
+    if (lg == 3) {
 #pragma unroll
       for (int q = 0; q < 4; ++q) g[(k * 4 + q) * 32 + lane] = m[q];
-    } else if (shift == 1) {
+    } else if (lg == 4) {
       g[k * 64 + lane] = fmaxf(m[0], m[1]);
       g[k * 64 + 32 + lane] = fmaxf(m[2], m[3]);
     } else {
       g[k * 32 + lane] = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
     }
   }
+  __device__ __forceinline__ int number(int chunks) const { return chunks * CHUNK >> lg; }
   // Whether the chunk has a logit of `least` or more.
   __device__ __forceinline__ bool reaches(int k, float least) const {
     const int lane = threadIdx.x & 31;
     float m = -INFINITY;
-    for (int q = 0; q < 4 >> shift; ++q) m = fmaxf(m, g[(k * (4 >> shift) + q) * 32 + lane]);
+    for (int q = 0; q < 32 >> lg; ++q) m = fmaxf(m, g[(k * (32 >> lg) + q) * 32 + lane]);
     return __any_sync(0xffffffffu, m >= least);
   }
 };
@@ -202,11 +204,11 @@ struct Parts {
   Groups groups;
   float* maxima;
   u64* inbox;
-  static __host__ __device__ __forceinline__ int shift_of(int per) { return per <= 160 ? 0 : per <= 320 ? 1 : 2; }
-  static __host__ int bytes(int per, int size) { return per * (128 >> shift_of(per)) * 4 + (size > 1 ? size * NT * 4 + LIST * 8 : 0); }
+  static __host__ __device__ __forceinline__ int lg_of(int per) { return per <= 160 ? 3 : per <= 320 ? 4 : 5; }
+  static __host__ int bytes(int per, int size) { return (per * CHUNK >> lg_of(per)) * 4 + (size > 1 ? size * NT * 4 + LIST * 8 : 0); }
   __device__ __forceinline__ Parts(float* smem, int per, int size) {
-    groups = Groups{smem, shift_of(per)};
-    maxima = smem + per * (128 >> groups.shift);
+    groups = Groups{smem, lg_of(per)};
+    maxima = smem + (per * CHUNK >> groups.lg);
     inbox = reinterpret_cast<u64*>(maxima + size * NT);
   }
 };
@@ -464,7 +466,7 @@ __device__ __forceinline__ u64 nth_key(RowShared<NT>& sh, unsigned n, unsigned m
   return sh.total;
 }
 
-// Up to NT / 2 entries: how many of the list are in front of an entry, and their weight.  Threads share an entry; the first of them has it.
+// Up to FEW entries: how many of the list are in front of an entry, and their weight.  Threads share an entry; the first of them has it.
 struct Counted { u64 key, weight, before; unsigned rank; bool mine; };
 template <int NT>
 __device__ __forceinline__ Counted count_list(RowShared<NT>& sh, unsigned n, bool weights) {
@@ -503,18 +505,32 @@ template <int NT>
 __device__ __noinline__ void bins_of_groups(RowShared<NT>& sh, Cluster& c, const Groups groups, int chunks, const Weights w, float least, bool by_count, float target) {
   clear_bins(sh);
   __syncthreads();
-  for (int i = threadIdx.x; i < chunks * (128 >> groups.shift); i += NT)
+  for (int i = threadIdx.x; i < groups.number(chunks); i += NT)
     if (groups.g[i] >= least) to_bin(sh, w, groups.g[i], by_count);
+  c.sync();
+  find_bin(sh, c, true, by_count, target);
+}
+// The same from all logits, of short rows: their few groups may hide much.
+template <class T, int NT>
+__device__ __noinline__ void bins_of_all(RowShared<NT>& sh, Cluster& c, const Row<T, NT> row, const Weights w, float least, bool by_count, float target) {
+  c.sync();                                        // (nobody reads the bins any more)
+  clear_bins(sh);
+  __syncthreads();
+  row.again([](int) { return true; }, [&](const float* v, int, int) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (v[i] >= least) to_bin(sh, w, v[i], by_count);
+  });
   c.sync();
   find_bin(sh, c, true, by_count, target);
 }
 // What lies at `least` and above, in the leader's list.  First which groups of eight have any, then a thread for each of them.
 template <class T, int NT>
 __device__ __forceinline__ unsigned gather(RowShared<NT>& sh, Cluster& c, const Row<T, NT>& row, const Parts<NT>& parts, float mine, float least) {
-  const int lane = threadIdx.x & 31, shift = parts.groups.shift, per = 4 >> shift;
+  const int lane = threadIdx.x & 31, lg = parts.groups.lg, per = 32 >> lg;
   const auto read = [&](int i) {                   // group i
-    const int g = i >> 5, chunk = row.chunk0 + (g >> (2 - shift)), from = (g & (per - 1)) * (8 << shift);
-    for (int q = 0; q < 8 << shift; q += 8) {
+    const int g = i >> 5, chunk = row.chunk0 + g / per, from = g % per << lg;
+    for (int q = 0; q < 1 << lg; q += 8) {
       float v[8];
       row.load(chunk, from + q, i & 31, v);
 #pragma unroll
@@ -538,6 +554,14 @@ __device__ __forceinline__ unsigned gather(RowShared<NT>& sh, Cluster& c, const 
   __syncthreads();
   for (unsigned h = threadIdx.x; h < min(sh.n_hits, static_cast<unsigned>(HITS)); h += NT) read(sh.hits[h]);
   return join_lists(sh, c, parts.inbox);
+}
+
+// Whether so few groups of the row reach `least` that the list takes all they may hold.
+template <int NT>
+__device__ __noinline__ bool few_reach(Cluster& c, const Groups groups, int chunks, float least) {
+  unsigned n = 0;
+  for (int i = threadIdx.x; i < groups.number(chunks); i += NT) n += groups.g[i] >= least;
+  return (c.reduce(n, 0u, [](unsigned a, unsigned b) { return a + b; }) << groups.lg) <= LIST;
 }
 
 // ------------------------------------------------------------------------------------------------ draws
@@ -806,7 +830,7 @@ __device__ __noinline__ float min_p_logit(float top, float temp, float mp) {
   return at_least(v);
 }
 
-template <class T, int NT, int AHEAD>
+template <class T, int NT>
 __global__ void __launch_bounds__(NT, 1024 / NT)
 sample_kernel(const __grid_constant__ SampleRows a, int per) {
   extern __shared__ __align__(16) float smem[];
@@ -833,7 +857,7 @@ sample_kernel(const __grid_constant__ SampleRows a, int per) {
   Racer racer;
   float largest = -INFINITY;                       // of the thread
   if (all) {
-    row.template stream<AHEAD>([&](const float (&v)[32], int i) {
+    row.template stream<0>([&](const float (&v)[32], int i) {
       float m[4], mine;
       const float highest = look(row, v, i, m, mine, seen.top);
       if (!(highest > -INFINITY && highest < INFINITY)) return;
@@ -842,7 +866,7 @@ sample_kernel(const __grid_constant__ SampleRows a, int per) {
       for (int q = 0; q < 32; q += 8) racer.template run<true>(race, row, v + q, row.chunk0 + i, q, whole_row(), &sh.score);
     });
   } else if (sums) {
-    row.template stream<AHEAD>([&](const float (&v)[32], int i) {
+    row.template stream<0>([&](const float (&v)[32], int i) {
       float m[4], mine;
       const float highest = look(row, v, i, m, mine, seen.top);
       largest = fmaxf(largest, mine);
@@ -858,7 +882,7 @@ sample_kernel(const __grid_constant__ SampleRows a, int per) {
       seen.add(s, g, E);
     });
   } else {
-    row.template stream<AHEAD>([&](const float (&v)[32], int i) {
+    row.template stream<0>([&](const float (&v)[32], int i) {
       float m[4], mine;
       look(row, v, i, m, mine, seen.top);
       largest = fmaxf(largest, mine);
@@ -894,79 +918,84 @@ sample_kernel(const __grid_constant__ SampleRows a, int per) {
   double total = 0;
   if (sums && !far) total = seen.s * pow2(seen.E - weight.E);
   else if (by_p && !by_k) total = row_total(c, lap<false, true>(row, groups, race, weight, kept, &sh.score).s);
-  if (by_k || by_p) {
-    unsigned n = LIST + 1;
-    if (k <= LIST && !far) {
+  unsigned n = LIST + 1;
+  if (k <= LIST && !far) {
+    float least = kept.z;
+    bool found = false;
+    if (by_k || by_p) {
       const float need = by_k ? k : static_cast<float>(p * total * (1 + 1.0 / 262144));
       bins_of_threads(sh, c, parts.maxima, largest, weight, kept.z, by_k, need);
       // (the groups' largest may have the weight that the threads' have not, and they are more than these)
       if (sh.bin == BINS - 1 && (by_k || by_min || seen.g * pow2(seen.E - weight.E) >= need)) bins_of_groups(sh, c, groups, row.chunks, weight, kept.z, by_k, need);
-      if (sh.bin < BINS - 1 || a.V <= LIST) n = gather(sh, c, row, parts, largest, fmaxf(kept.z, weight.edge(sh.bin)));
+      if (NT == 128 && sh.bin == BINS - 1) bins_of_all(sh, c, row, weight, kept.z, by_k, need);
+      found = sh.bin < BINS - 1;
+      if (found) least = fmaxf(least, weight.edge(sh.bin));
     }
-    if (n <= LIST) {
-      if (c.rank) return;
-      // Weights in whole numbers of 2^-40: every token before the one that reaches top_p is kept.
-      const auto whole = [&](u64 key) { return __float2ull_rn(weight(list_z(key)) * 1099511627776.f); };
-      const unsigned n1 = by_k ? min(n, static_cast<unsigned>(k)) : n;
-      int token;
-      if (n <= NT / 2) {
-        if (by_p) {
-          if (t < n) sh.weight[t] = whole(sh.list[t]);
-          __syncthreads();
-        }
-        const Counted e = count_list(sh, n, by_p);
-        bool in = e.mine && e.rank < n1;
-        if (by_p) {
-          if (e.mine && e.rank + 1 == n1) sh.total = e.before + e.weight;
-          __syncthreads();
-          const double target = static_cast<double>(p) * (by_k ? static_cast<double>(sh.total) : total * 1099511627776.0);
-          in = in && (e.rank == 0 || static_cast<double>(e.before) < target);
-        }
-        token = draw_listed(sh, c, race, [&](auto f) { if (in) f(e.key); });
-      } else {
-        sort_list<NT>(sh.list, n);
-        unsigned m = n1;
-        if (by_p) {
-          constexpr int PER = LIST / NT;
-          u64 sum = 0;
-          for (int i = 0; i < PER; ++i) sum += t * PER + i < n ? whole(sh.list[t * PER + i]) : 0;
-          u64 before = sum;
-          const int lane = t & 31;
-#pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const u64 y = __shfl_up_sync(0xffffffffu, before, o);
-            if (lane >= o) before += y;
-          }
-          if (lane == 31) sh.wsum[t >> 5] = before;
-          if (t == 0) sh.kept = 0;
-          __syncthreads();
-          before -= sum;
-          for (int i = 0; i < t >> 5; ++i) before += sh.wsum[i];
-          u64 at = before;
-          for (int i = 0; i < PER && t * PER + i < n1; ++i) {
-            at += whole(sh.list[t * PER + i]);
-            if (t * PER + i + 1 == n1) sh.total = at;
-          }
-          __syncthreads();
-          const double target = static_cast<double>(p) * (by_k ? static_cast<double>(sh.total) : total * 1099511627776.0);
-          unsigned mine = 0;
-          at = before;
-          for (int i = 0; i < PER && t * PER + i < n1; ++i) {
-            mine += t * PER + i == 0 || static_cast<double>(at) < target;
-            at += whole(sh.list[t * PER + i]);
-          }
-          if (mine) atomicAdd(&sh.kept, mine);
-          __syncthreads();
-          m = sh.kept;
-          __syncthreads();
-        }
-        token = draw_listed(sh, c, race, [&](auto f) { for (unsigned i = t; i < m; i += NT) f(sh.list[i]); });
-      }
-      if (t == 0) a.out[r] = token;
-      return;
-    }
-    if (by_k) kept = kth_token(sh, row, groups, c, weight, kept, k, parts.inbox);
+    if (found || few_reach<NT>(c, groups, row.chunks, least)) n = gather(sh, c, row, parts, largest, least);
   }
+  if (n <= LIST) {
+    if (c.rank) return;
+    // Weights in whole numbers of 2^-40: every token before the one that reaches top_p is kept.
+    const auto whole = [&](u64 key) { return __float2ull_rn(weight(list_z(key)) * 1099511627776.f); };
+    const unsigned n1 = by_k ? min(n, static_cast<unsigned>(k)) : n;
+    int token;
+    if (n <= FEW_OF<NT>) {
+      if (by_p) {
+        if (t < n) sh.weight[t] = whole(sh.list[t]);
+        __syncthreads();
+      }
+      const Counted e = count_list(sh, n, by_p);
+      bool in = e.mine && e.rank < n1;
+      if (by_p) {
+        if (e.mine && e.rank + 1 == n1) sh.total = e.before + e.weight;
+        __syncthreads();
+        const double target = static_cast<double>(p) * (by_k ? static_cast<double>(sh.total) : total * 1099511627776.0);
+        in = in && (e.rank == 0 || static_cast<double>(e.before) < target);
+      }
+      token = draw_listed(sh, c, race, [&](auto f) { if (in) f(e.key); });
+    } else {
+      sort_list<NT>(sh.list, n);
+      unsigned m = n1;
+      if (by_p) {
+        constexpr int PER = LIST / NT;
+        u64 sum = 0;
+        for (int i = 0; i < PER; ++i) sum += t * PER + i < n ? whole(sh.list[t * PER + i]) : 0;
+        u64 before = sum;
+        const int lane = t & 31;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const u64 y = __shfl_up_sync(0xffffffffu, before, o);
+          if (lane >= o) before += y;
+        }
+        if (lane == 31) sh.wsum[t >> 5] = before;
+        if (t == 0) sh.kept = 0;
+        __syncthreads();
+        before -= sum;
+        for (int i = 0; i < t >> 5; ++i) before += sh.wsum[i];
+        u64 at = before;
+        for (int i = 0; i < PER && t * PER + i < n1; ++i) {
+          at += whole(sh.list[t * PER + i]);
+          if (t * PER + i + 1 == n1) sh.total = at;
+        }
+        __syncthreads();
+        const double target = static_cast<double>(p) * (by_k ? static_cast<double>(sh.total) : total * 1099511627776.0);
+        unsigned mine = 0;
+        at = before;
+        for (int i = 0; i < PER && t * PER + i < n1; ++i) {
+          mine += t * PER + i == 0 || static_cast<double>(at) < target;
+          at += whole(sh.list[t * PER + i]);
+        }
+        if (mine) atomicAdd(&sh.kept, mine);
+        __syncthreads();
+        m = sh.kept;
+        __syncthreads();
+      }
+      token = draw_listed(sh, c, race, [&](auto f) { for (unsigned i = t; i < m; i += NT) f(sh.list[i]); });
+    }
+    if (t == 0) a.out[r] = token;
+    return;
+  }
+  if (by_k) kept = kth_token(sh, row, groups, c, weight, kept, k, parts.inbox);
   const Lap l = by_k && by_p ? lap<true, true>(row, groups, race, weight, kept, &sh.score) : lap<true, false>(row, groups, race, weight, kept, &sh.score);
   if (by_k && by_p) total = row_total(c, l.s);
   Win win = settle(row, c, race, kept, l.m);
@@ -982,7 +1011,7 @@ sample_kernel(const __grid_constant__ SampleRows a, int per) {
   c.sync();
 }
 
-template <class T, int NT, int AHEAD>
+template <class T, int NT, int AHEAD, bool LISTING>
 __global__ void __launch_bounds__(NT, 1024 / NT)
 logprob_kernel(const __grid_constant__ LogprobRows a, int per) {
   extern __shared__ __align__(16) float smem[];
@@ -993,11 +1022,11 @@ logprob_kernel(const __grid_constant__ LogprobRows a, int per) {
   const int tid = threadIdx.x, r = blockIdx.x / c.size;
   const T* x = static_cast<const T*>(a.x) + r * a.ldx;
   const int t = a.tokens[r];
-  const bool there = t >= 0 && t < a.V, listing = a.top > 1;
+  const bool there = t >= 0 && t < a.V;
   const float zt = there ? plain_logit(logit(x + t)) : -INFINITY;
   const Row<T, NT> row(x, a.V, c.rank, per);
   const Parts<NT> parts(smem, per, c.size);
-  if (listing) {
+  if (LISTING) {
     clear_bins(sh);
     if (tid == 0) sh.n_list = sh.n_hits = 0;
   }
@@ -1010,8 +1039,10 @@ logprob_kernel(const __grid_constant__ LogprobRows a, int per) {
     const int chunk = row.chunk0 + i;
     float m[4], mine;
     const float highest = look(row, v, i, m, mine, seen.top);
-    largest = fmaxf(largest, mine);
-    if (listing) parts.groups.put(m, i);
+    if (LISTING) {
+      largest = fmaxf(largest, mine);
+      parts.groups.put(m, i);
+    }
     if (highest > -INFINITY && highest < INFINITY) {           // the chunk's sum in units of its own
       const float E = fmaxf(ceilf(highest * HI), -1e30f);
       float s = 0.f;
@@ -1037,7 +1068,7 @@ logprob_kernel(const __grid_constant__ LogprobRows a, int per) {
     }
   });
   c.ready();
-  if (c.size > 1 && listing)
+  if (c.size > 1 && LISTING)
     for (int i = 0; i < c.size; ++i) c.of(parts.maxima, i)[c.rank * NT + tid] = largest;
   seen = row_seen(c, seen, true, true);
   const Best top = seen.top;
@@ -1070,17 +1101,19 @@ logprob_kernel(const __grid_constant__ LogprobRows a, int per) {
       lps[0] = lp(top.v);
     }
   }
-  if (a.top < 2) { c.sync(); return; }
+  if (!LISTING) { c.sync(); return; }
   if (!far) {
     const Weights w{HI, ceilf(top.v * HI), 0.f};
     bins_of_threads(sh, c, parts.maxima, largest, w, LOWEST, true, a.top);
     if (sh.bin == BINS - 1) bins_of_groups(sh, c, parts.groups, row.chunks, w, LOWEST, true, a.top);
+    const bool found = sh.bin < BINS - 1;
+    const float least = found ? w.edge(sh.bin) : LOWEST;
     unsigned n = LIST + 1;
-    if (sh.bin < BINS - 1 || a.V <= LIST) n = gather(sh, c, row, parts, largest, w.edge(sh.bin));
+    if (found || few_reach<NT>(c, parts.groups, row.chunks, least)) n = gather(sh, c, row, parts, largest, least);
     if (n <= LIST) {
       if (c.rank) return;
       const auto put = [&](unsigned i, u64 key) { ids[i] = list_id(key); lps[i] = lp(list_z(key)); };
-      if (n <= NT / 2) {
+      if (n <= FEW_OF<NT>) {
         const Counted e = count_list(sh, n, false);
         if (e.mine && e.rank < static_cast<unsigned>(a.top)) put(e.rank, e.key);
       } else {
@@ -1126,21 +1159,24 @@ static int launch_rows(const char* name, K kern, const A& a, int chunks, int c, 
   spark_launch_pdl(kern, dim3(a.R * c), dim3(NT), bytes, s, dim3(c, 1, 1), a, per);
   return spark_launch_rc(name);
 }
-// Rows of a few chunks take CTAs of four warps.  How far ahead others are asked for goes by whether all CTAs run at once: then one chunk (256 draws from
-// 152k 43.9 us, two chunks 47.9: the groups that are read again wait behind what was asked for), else two (1024 scored rows 101 us, one chunk 107).
+// Rows of a few chunks take CTAs of four warps.
 template <class T>
 static int sample_rows(const SampleRows& a, cudaStream_t s) {
   const char* name = "spark_sample_rows";
   const int chunks = (a.V + 8 + CHUNK - 1) / CHUNK, c = row_cluster(a.R, chunks, a.sms, true);
-  if (chunks <= 8) return launch_rows<128>(name, sample_kernel<T, 128, 1>, a, chunks, c, s);
-  return a.R * c > 2 * a.sms ? launch_rows<512>(name, sample_kernel<T, 512, 2>, a, chunks, c, s) : launch_rows<512>(name, sample_kernel<T, 512, 1>, a, chunks, c, s);
+  return chunks <= 8 ? launch_rows<128>(name, sample_kernel<T, 128>, a, chunks, c, s) : launch_rows<512>(name, sample_kernel<T, 512>, a, chunks, c, s);
 }
+// Log-probabilities without lists of the best have a kernel of their own: without the code for lists the loads of a chunk stay together (1024 rows of 152k
+// logits 110 us, with it 118), and asking for what comes two chunks later helps (100 us; the other kernels, which read some of a row again, lose by
+// it: 256 draws 62 us without and 64 with it, 1024 rows of 66k with their first five 73 and 77).
 template <class T>
 static int logprob_rows(const LogprobRows& a, cudaStream_t s) {
   const char* name = "spark_logprob_rows";
   const int chunks = (a.V + 8 + CHUNK - 1) / CHUNK, c = row_cluster(a.R, chunks, a.sms, false);
-  if (chunks <= 8) return launch_rows<128>(name, logprob_kernel<T, 128, 1>, a, chunks, c, s);
-  return a.R * c > 2 * a.sms ? launch_rows<512>(name, logprob_kernel<T, 512, 2>, a, chunks, c, s) : launch_rows<512>(name, logprob_kernel<T, 512, 1>, a, chunks, c, s);
+  if (a.top > 1)
+    return chunks <= 8 ? launch_rows<128>(name, logprob_kernel<T, 128, 0, true>, a, chunks, c, s) : launch_rows<512>(name, logprob_kernel<T, 512, 0, true>, a, chunks, c, s);
+  if (chunks <= 8) return launch_rows<128>(name, logprob_kernel<T, 128, 0, false>, a, chunks, c, s);
+  return launch_rows<512>(name, logprob_kernel<T, 512, 2, false>, a, chunks, c, s);
 }
 
 }  // namespace spark
