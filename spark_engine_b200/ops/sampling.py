@@ -167,9 +167,10 @@ def sample_tokens(logits, temps, seeds, positions, top_k=None, top_p=None, min_p
     top_k int32 [R], seeds and positions int64 [R].  Kept are the first top_k tokens of the row's order (<= 0: all); of these the ones at least min_p
     times as probable as the first (<= 0: all); of these the shortest run of the order that has top_p of their probability (>= 1: all; one at least).
     Drawn is the arg-max over kept of fp32(logit / temperature) + fp32(g), g = -log(-log u), u from (seed, position, id); rows of temperature <= 0, and
-    rows whose best logit / temperature is infinite, take the first of the order.
+    rows whose best logit / temperature is 2^30 or more in size, beside which noise is nothing, take the first of the order.
 
-    Probabilities are summed in whole numbers of 2^-40 of the best token's: which token is the last one kept is the same in every batch."""
+    Weights are fp32 (to about 2^-20 of themselves), their sums 64 bits and the same in every batch: only where the probability up to a token comes that close
+    to top_p can the last one kept be its neighbour.  An `adjust` takes a workspace of R * V fp32 from torch's allocator, which a captured call keeps."""
     run = _kernels(logits)
     t = _native().sample_tokens(logits, temps, seeds, positions, top_k, top_p, min_p, adjust, run)
     if run:
@@ -187,7 +188,7 @@ def _plain_sample(z, temp, seed, position, k, p, m) -> int:
     if z[0] == -math.inf:
         return -1
     temp = torch.tensor(temp, dtype=torch.float32, device=z.device)
-    if not temp > 0 or not torch.isfinite(z[0] / temp):
+    if not temp > 0 or not torch.abs(z[0] / temp) < 2.0 ** 30:
         return int(ids[0])
     d = (z.double() - z[0].double()) / temp.double()
     n = int((z > -math.inf).sum())
@@ -212,8 +213,8 @@ class Logprobs(NamedTuple):
 
 
 def token_logprobs(logits, tokens, top: int = 0) -> Logprobs:
-    """log softmax(logits) of tokens int32 [R] and of the `top` most probable ones of every row, for logits [R, V] (fp32, bf16, fp16).  What is not in the
-    vocabulary has -inf and rank 0; tokens that are none (-inf, NaN) have -inf."""
+    """log softmax(logits) of tokens int32 [R] and of the `top` (256 at most) most probable ones of every row, for logits [R, V] (fp32, bf16, fp16).  What is
+    not in the vocabulary has -inf and rank 0; tokens that are none (-inf, NaN) have -inf."""
     run = _kernels(logits)
     out = Logprobs(*_native().token_logprobs(logits, tokens, top, run))
     if run:

@@ -82,11 +82,12 @@ def want_token(z, temp, seed, position, k, p, m):
     if not len(ids):
         return -1
     with np.errstate(over="ignore"):
-        if not temp > 0 or not np.isfinite(F32(z[ids[0]]) / F32(temp)):
+        if not temp > 0 or not abs(F32(z[ids[0]]) / F32(temp)) < 2.0 ** 30:      # (beside which noise is nothing)
             return int(ids[0])
     kept = want_kept(z, temp, k, p, m)
     u = uniform_ref(seed, position, z.shape[0]).numpy()[kept]
-    score = z[kept].astype(F32) / F32(temp) + (-np.log(-np.log(u))).astype(F32)
+    with np.errstate(over="ignore"):
+        score = z[kept].astype(F32) / F32(temp) + (-np.log(-np.log(u))).astype(F32)
     return int(kept[score == score.max()].min())
 
 

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from spark_engine_b200 import ops
-from tests.sampling_util import Rows, Table, near, want_logprobs
+from tests.sampling_util import Rows, Table, near, want_logprobs, want_token
 
 pytestmark = pytest.mark.gpu
 TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
@@ -327,4 +327,54 @@ def test_masks_of_the_lowest_value(V, dtype):
         assert got[1][r] == rank and got[2][r].tolist() == [int(i) for i in ids]
         near(np.maximum(got[0][r: r + 1], -3e38), np.maximum([lp], -3e38))
         near(np.maximum(got[3][r], -3e38), np.maximum(lps, -3e38))
+    _sound()
+
+
+# ----------------------------------------------------------------------------- ways through the kernels that sizes above do not take
+@pytest.mark.parametrize("R, V", [(300, 170001), (300, 400003), (200, 700001)])
+def test_many_long_rows(R, V):
+    """More rows than leave several CTAs for each, of more logits than groups of eight are kept for.  (One row under many settings.)"""
+    rows = Rows(1, V, "peaked", seed=V, device="cuda", pad=1)
+    one = rows.z[0]
+    rs = rows.rs
+    rows.R, rows.logits, rows.z = R, rows.logits.expand(R, V), np.broadcast_to(one, (R, V))
+    rows.seeds, rows.positions = rs.randint(0, 1 << 40, R), rs.randint(0, 1 << 20, R)
+    s = dict(top_k=rs.choice([0, 0, 30, 1500, 30000], R), top_p=rs.choice([1.0, 0.6, 0.97], R), min_p=rs.choice([0.0, 0.02], R))
+    T = rs.choice([0.0, 0.8, 1.5], R)
+    got = rows.draw(T, **s)
+    t = rs.randint(0, V, R)
+    lp = [x.cpu().numpy() for x in ops.token_logprobs(rows.logits, rows.t(t, torch.int32), 20)]
+    for r in range(0, R, 17):
+        assert got[r] == want_token(one, T[r], int(rows.seeds[r]), int(rows.positions[r]), int(s["top_k"][r]), s["top_p"][r], s["min_p"][r])
+        a, rank, ids, b = want_logprobs(one, int(t[r]), 20)
+        assert lp[1][r] == rank and lp[2][r].tolist() == [int(i) for i in ids]
+        near(lp[0][r: r + 1], [a])
+        near(lp[3][r], b)
+    _sound()
+
+
+@pytest.mark.parametrize("at", [0.0, 0.4, 0.97])
+def test_likely_tokens_side_by_side(at):
+    """All that is kept lies in one CTA's part of the row: more than its share of the leader's inbox."""
+    V = 151936
+    rows = Rows(2, V, "flat", seed=3, device="cuda")
+    z = rows.z.copy()
+    first = int(at * V)
+    z[:, first: first + 1700] += 12
+    rows.logits, rows.z = rows.t(z, torch.float32), z
+    for s in (dict(top_k=1200), dict(top_k=1600, top_p=0.9), dict(top_p=0.95), dict(min_p=1e-3), dict(top_k=200)):
+        assert np.array_equal(rows.draw(0.9, **s), rows.want(0.9, **s)), s
+    got = ops.token_logprobs(rows.logits, rows.t([first, 5], torch.int32), 256)
+    for r in range(2):
+        assert got.ids[r].tolist() == [int(i) for i in want_logprobs(z[r], 0, 256)[2]]
+    _sound()
+
+
+def test_scores_next_to_one_another():
+    """Thousands of draws among equal logits: in some of them the two best scores are too near for the rough ones."""
+    rows = Rows(3000, 500, "same", seed=12, device="cuda")
+    for s in (dict(), dict(top_k=100), dict(top_p=0.5), dict(top_k=400, top_p=0.9)):
+        assert np.array_equal(rows.draw(1.0, **s), rows.want(1.0, **s)), s
+    rows = Rows(400, 20000, "equal", seed=13, device="cuda")
+    assert np.array_equal(rows.draw(2.0), rows.want(2.0))
     _sound()
