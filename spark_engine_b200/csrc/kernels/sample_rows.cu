@@ -12,7 +12,7 @@
 // (76 KB of 152k logits, where the row itself is 608).  The largest that each thread has seen go to a histogram, whose first bins with k tokens (or top_p of
 // the weight) in them hold what is kept, since all others can only add to it; where they do not reach that far, the largest of every eight do.  The
 // groups that come into these bins are read again, and what of them lies there goes to a list, in which one CTA finds the prefix.  Where more are kept than
-// the list takes, the row is read again: the k-th token comes from a histogram of all, and for top_p a token is drawn first and the weight in front of it
+// the list takes, the row is read again: the k-th token comes from a histogram of all (what is kept then fits the CTAs' lists together), and for top_p a token is drawn first and the weight in front of it
 // looked at then: what lies in front of a token drawn in vain holds all that is kept, and half as much as before on average.
 //
 // Sums of weights: a chunk's in fp32 in units 2^E of its own, E whole, chunks' in 64 bits.  A sum is the same however chunks are dealt to CTAs and
@@ -827,6 +827,38 @@ __device__ __noinline__ Prefix kth_token(RowShared<NT>& sh, const Row<T, NT> row
   return sh.cut;
 }
 
+// What lies within `kept` in its CTA's own list; false (and of no use) where one of them is too short.
+template <class T, int NT>
+__device__ __noinline__ bool list_kept(RowShared<NT>& sh, Cluster& c, const Row<T, NT> row, const Groups groups, const Prefix kept) {
+  if (threadIdx.x == 0) sh.n_list = 0;
+  __syncthreads();
+  row.again([&](int i) { return groups.reaches(i, kept.z); }, [&](const float* v, int n, int q) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int id = row.id(Row<T, NT>::place(row.chunk0 + n, q + i, threadIdx.x & 31));
+      if (v[i] >= kept.z && within(kept, v[i], id)) to_list(sh, v[i], id);
+    }
+  });
+  __syncthreads();
+  return c.reduce(sh.n_list, 0u, [](unsigned a, unsigned b) { return max(a, b); }) <= LIST;
+}
+// A race over the list's entries within `front`, and their weight: in whole numbers, since entries come in any order.
+template <int NT>
+__device__ __noinline__ Lap list_lap(const RowShared<NT>& sh, const Race race, const Weights w, const Prefix front, bool race_too, bool mass_too) {
+  Top2 m = no_top();
+  u64 s = 0;
+  const unsigned n = sh.n_list;
+  for (unsigned i = threadIdx.x; i < n; i += NT) {
+    const u64 key = sh.list[i];
+    const float z = list_z(key);
+    const int id = list_id(key);
+    if (!within(front, z, id)) continue;
+    if (mass_too) s += __float2ull_rn(w(z) * 1099511627776.f);
+    if (race_too) m = best2(m, Top2{race.rough(z, id), id, -INFINITY, z});
+  }
+  return Lap{m, static_cast<double>(s) * (1.0 / 1099511627776.0)};
+}
+
 // ------------------------------------------------------------------------------------------------ kernels
 
 // The smallest logit that is not too improbable, decided in 64 bits.
@@ -1004,17 +1036,27 @@ sample_kernel(const __grid_constant__ SampleRows a, int per) {
     if (t == 0) a.out[r] = token;
     return;
   }
-  if (by_k) kept = kth_token(sh, row, groups, c, weight, kept, k, parts.inbox);
-  const Lap l = by_k && by_p ? lap<true, true>(row, groups, race, weight, kept, &sh.score) : lap<true, false>(row, groups, race, weight, kept, &sh.score);
+  bool listed = false;                             // what is kept is in the CTAs' own lists
+  if (by_k) {
+    kept = kth_token(sh, row, groups, c, weight, kept, k, parts.inbox);
+    if (k <= LIST * c.size) listed = list_kept(sh, c, row, groups, kept);
+  }
+  // A race among what lies within `front`, its weight, or both.
+  const auto go = [&](const Prefix& front, bool race_too, bool mass_too) {
+    if (listed) return list_lap(sh, race, weight, front, race_too, mass_too);
+    if (!race_too) return lap<false, true>(row, groups, race, weight, front, &sh.score);
+    return mass_too ? lap<true, true>(row, groups, race, weight, front, &sh.score) : lap<true, false>(row, groups, race, weight, front, &sh.score);
+  };
+  const Lap l = go(kept, true, by_k && by_p);
   if (by_k && by_p) total = row_total(c, l.s);
   Win win = settle(row, c, race, kept, l.m);
   const double target = p * total;
   while (by_p && win.id != top.id) {               // what lies in front of it; who wins there, should that be too much
     const Prefix front{win.z, win.id - 1};
-    if (row_total(c, lap<false, true>(row, groups, race, weight, front, &sh.score).s) < target) break;
+    if (row_total(c, go(front, false, true).s) < target) break;
     if (t == 0) sh.score = score_key(-INFINITY);   // (all warps are past the last race, and none begins the next before the barrier)
     __syncthreads();
-    win = settle(row, c, race, front, lap<true, false>(row, groups, race, weight, front, &sh.score).m);
+    win = settle(row, c, race, front, go(front, true, false).m);
   }
   if (lead) a.out[r] = win.id;
   c.sync();
@@ -1152,12 +1194,13 @@ logprob_kernel(const __grid_constant__ LogprobRows a, int per) {
   c.sync();
 }
 
-// CTAs of a row's cluster: as many as run at once, of four chunks each at least; draws take two while that is no more than twice as many, since a
-// row that keeps very many tokens holds the others up (256 draws of eight kinds from 152k logits 105 us, with one CTA each 148; without such rows 62
-// and 49.  1024 draws from 66k: 189 and 173).
+// CTAs of a row's cluster: as many as run at once, of four chunks each at least.  Clusters of four and eight do not fill every SM (36 rows by eight CTAs take
+// 26.5 us, by four 17.3; 74 by four 28.4, by two 18.0).  Draws take two also while that is up to twice as many as run at once, since a row that keeps
+// very many tokens holds the others up (256 draws of eight kinds from 152k logits 105 us, with one CTA each 148; without such rows 62 and 49.  1024
+// draws from 66k: 189 and 173).
 static int row_cluster(int R, int chunks, int sms, bool draws) {
   int c = 1;
-  while (c < CLUSTER_MAX && R * c * 2 <= 2 * sms && c * 4 < chunks) c *= 2;
+  while (c < CLUSTER_MAX && R * c * 2 <= (c == 1 ? 2 * sms : sms * 7 / 4) && c * 4 < chunks) c *= 2;
   return c == 1 && draws && R <= 2 * sms && chunks > 16 ? 2 : c;
 }
 
