@@ -76,7 +76,7 @@ template <int NT>
 struct RowShared {
   Mailboxes mail;
   unsigned hist[BINS], hits[HITS];
-  u64 list[LIST], weight[FEW_OF<NT>], wsum[NT / 32];
+  u64 list[LIST], weight[FEW_OF<NT>];
   float fsum[NT / 32];
   unsigned n_list, n_hits, before, kept;
   int bin, score;
@@ -744,18 +744,25 @@ __device__ __forceinline__ Win settle(const Row<T, NT>& row, Cluster& c, const R
   return photo_finish(row, c, race, kept, m.a1);
 }
 
-// The leader's: the winner among what `each` gives (f(key) for the thread's candidates).  Thread 0 has it.
+// The leader's: the winner among what `each` gives (f(key) for the thread's candidates).  All of its threads have it.
 template <int NT, class E>
-__device__ __forceinline__ int draw_listed(RowShared<NT>& sh, Cluster& c, const Race& race, E each) {
+__device__ __forceinline__ Prefix draw_listed(RowShared<NT>& sh, Cluster& c, const Race& race, E each) {
   Top2 m = no_top();
-  each([&](u64 k) { m = best2(m, Top2{race.rough(list_z(k), list_id(k)), list_id(k), -INFINITY, 0}); });
+  each([&](u64 k) { m = best2(m, Top2{race.rough(list_z(k), list_id(k)), list_id(k), -INFINITY, list_z(k)}); });
   m = c.block(m, no_top(), best2);
-  if (threadIdx.x == 0) sh.kept = m.a2 < m.a1 - Race::margin(m.a1);
+  if (threadIdx.x == 0) {
+    sh.kept = m.a2 < m.a1 - Race::margin(m.a1);
+    sh.cut = Prefix{m.z, m.id};
+  }
   __syncthreads();
-  if (sh.kept) return m.id;
-  Best b{-INFINITY, NO_ID};
-  each([&](u64 k) { b = first_of(b, Best{race.exact(list_z(k), list_id(k)), list_id(k)}); });
-  return c.block(b, Best{-INFINITY, NO_ID}, first_of).id;
+  if (!sh.kept) {
+    Win b{-INFINITY, NO_ID, -INFINITY, 0};
+    each([&](u64 k) { b = first_win(b, Win{race.exact(list_z(k), list_id(k)), list_id(k), list_z(k), 0}); });
+    b = c.block(b, Win{-INFINITY, NO_ID, -INFINITY, 0}, first_win);
+    if (threadIdx.x == 0) sh.cut = Prefix{b.z, b.id};
+    __syncthreads();
+  }
+  return sh.cut;
 }
 
 // ------------------------------------------------------------------------------------------------ the k-th token
@@ -976,7 +983,7 @@ sample_kernel(const __grid_constant__ SampleRows a, int per) {
   }
   if (n <= LIST) {
     if (c.rank) return;
-    // Weights in whole numbers of 2^-40: every token before the one that reaches top_p is kept.
+    // Weights in whole numbers of 2^-40, which no order changes: every token before the one that reaches top_p is kept.
     const auto whole = [&](u64 key) { return __float2ull_rn(weight(list_z(key)) * 1099511627776.f); };
     const unsigned n1 = by_k ? min(n, static_cast<unsigned>(k)) : n;
     int token;
@@ -993,45 +1000,38 @@ sample_kernel(const __grid_constant__ SampleRows a, int per) {
         const double target = static_cast<double>(p) * (by_k ? static_cast<double>(sh.total) : total * 1099511627776.0);
         in = in && (e.rank == 0 || static_cast<double>(e.before) < target);
       }
-      token = draw_listed(sh, c, race, [&](auto f) { if (in) f(e.key); });
-    } else {
-      sort_list<NT>(sh.list, n);
-      unsigned m = n1;
-      if (by_p) {
-        constexpr int PER = LIST / NT;
-        u64 sum = 0;
-        for (int i = 0; i < PER; ++i) sum += t * PER + i < n ? whole(sh.list[t * PER + i]) : 0;
-        u64 before = sum;
-        const int lane = t & 31;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const u64 y = __shfl_up_sync(0xffffffffu, before, o);
-          if (lane >= o) before += y;
-        }
-        if (lane == 31) sh.wsum[t >> 5] = before;
-        if (t == 0) sh.kept = 0;
-        __syncthreads();
-        before -= sum;
-        for (int i = 0; i < t >> 5; ++i) before += sh.wsum[i];
-        u64 at = before;
-        for (int i = 0; i < PER && t * PER + i < n1; ++i) {
-          at += whole(sh.list[t * PER + i]);
-          if (t * PER + i + 1 == n1) sh.total = at;
-        }
-        __syncthreads();
-        const double target = static_cast<double>(p) * (by_k ? static_cast<double>(sh.total) : total * 1099511627776.0);
-        unsigned mine = 0;
-        at = before;
-        for (int i = 0; i < PER && t * PER + i < n1; ++i) {
-          mine += t * PER + i == 0 || static_cast<double>(at) < target;
-          at += whole(sh.list[t * PER + i]);
-        }
-        if (mine) atomicAdd(&sh.kept, mine);
-        __syncthreads();
-        m = sh.kept;
-        __syncthreads();
+      token = draw_listed(sh, c, race, [&](auto f) { if (in) f(e.key); }).id;
+    } else {                                       // longer ones as rows are that keep very many: drawn first, looked at then
+      Prefix in = whole_row();
+      if (n1 < n) {
+        const u64 last = nth_key(sh, n, n1);
+        in = Prefix{list_z(last), list_id(last)};
       }
-      token = draw_listed(sh, c, race, [&](auto f) { for (unsigned i = t; i < m; i += NT) f(sh.list[i]); });
+      const auto weight_of = [&](const Prefix& f) {
+        u64 w = 0;
+        for (unsigned i = t; i < n; i += NT) {
+          const u64 key = sh.list[i];
+          w += within(f, list_z(key), list_id(key)) ? whole(key) : 0;
+        }
+        w = c.block(w, u64{0}, [](u64 x, u64 y) { return x + y; });
+        if (t == 0) sh.total = w;
+        __syncthreads();
+        return static_cast<double>(sh.total);
+      };
+      const auto draw = [&](const Prefix& f) {
+        return draw_listed(sh, c, race, [&](auto g) {
+          for (unsigned i = t; i < n; i += NT)
+            if (within(f, list_z(sh.list[i]), list_id(sh.list[i]))) g(sh.list[i]);
+        });
+      };
+      const double target = by_p ? p * (by_k ? weight_of(in) : total * 1099511627776.0) : 0;
+      Prefix win = draw(in);
+      while (by_p && win.id != top.id) {
+        const Prefix front{win.z, win.id - 1};
+        if (weight_of(front) < target) break;
+        win = draw(front);
+      }
+      token = win.id;
     }
     if (t == 0) a.out[r] = token;
     return;
