@@ -12,11 +12,13 @@
 // (76 KB of 152k logits, where the row itself is 608).  The largest that each thread has seen go to a histogram, whose first bins with k tokens (or top_p of
 // the weight) in them hold what is kept, since all others can only add to it; where they do not reach that far, the largest of every eight do.  The
 // groups that come into these bins are read again, and what of them lies there goes to a list, in which one CTA finds the prefix.  Where more are kept than
-// the list takes, the row is read again: the k-th token comes from a histogram of all (what is kept then fits the CTAs' lists together), and for top_p a token is drawn first and the weight in front of it
-// looked at then: what lies in front of a token drawn in vain holds all that is kept, and half as much as before on average.
+// the list takes, the row is read again: the k-th token comes from a histogram of all (what is kept then fits the
+// CTAs' lists together), and for top_p a token is drawn first and the weight in front of it looked at then: what lies in front of a token drawn in vain
+// holds all that is kept, and half as much as before on average.
 //
-// Sums of weights: a chunk's in fp32 in units 2^E of its own, E whole, chunks' in 64 bits.  A sum is the same however chunks are dealt to CTAs and
-// warps (to 2^-53), so that a row's result does not depend on the batch it comes in.
+// Sums of weights: a chunk's in fp32 in units 2^E of its own, E whole, chunks' in 64 bits; a list's in whole numbers of 2^-40.  Each is the same however
+// chunks are dealt to CTAs and warps (to 2^-53), and so are log-probabilities.  How many CTAs a row has can decide which of the two a prefix's weight is:
+// they differ by 2^-20 of it, and a row draws the same in every batch but where top_p falls between them.
 //
 // What bounds it (one B200, fp32 logits).  One row: ten trips to memory and barriers of a cluster one after the other, 12.7 us for 152k logits, of which
 // 2.5 are the row's own, 1.4 sums and best over eight CTAs, 1.4 bins, 4 the groups read again and lists joined, 2 the prefix and the draw.  Many rows whose
@@ -421,7 +423,8 @@ __device__ __forceinline__ unsigned join_lists(RowShared<NT>& sh, Cluster& c, u6
   return n;
 }
 
-// list[0, n) in the row's order (descending keys; all differ).  Bitonic: 2000 entries take 12 us, which is why what has few entries is counted instead.
+// list[0, n) in the row's order (descending keys; all differ), for the tokens that log-probabilities list.  Bitonic: 2000 entries take 12 us, which is why
+// few entries are counted and draws look for what they need in the list as it is.
 template <int NT>
 __device__ __noinline__ void sort_list(u64* list, unsigned n) {
   unsigned m = 32;

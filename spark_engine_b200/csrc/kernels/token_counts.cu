@@ -3,9 +3,9 @@
 //   count_tokens   counts[slot][t] = 2 * times generated + (1 if in the prompt), grown by a round's tokens or written anew for a request
 //   adjust_rows    z / rep or z * rep of tokens that are in the counts, - freq * generated - pres, + biases, -inf where not allowed
 //
-// Bound by memory where rows are many: 64 new rows of 152k counts in 13.7 us (39 MB written: 2.9 TB/s; every CTA looks through all of its request's tokens,
+// Bound by memory where rows are many: 64 new rows of 152k counts in 13.0 us (39 MB written: 3 TB/s; every CTA looks through all of its request's tokens,
 // 32000 at most here), 256 bf16 rows of 129k with counts, masks and 103 entries each in 69 us (236 MB: 3.4 TB/s; the lists' trips to memory come before
-// and after the columns'), four rows in 6.4 us.
+// and after the columns'), four rows in 6.3 us.
 #include "../common/token_rows.cuh"
 
 namespace spark {
