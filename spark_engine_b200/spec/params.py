@@ -1,7 +1,6 @@
 """What a request asks of its draws: temperature and seed, top-k / top-p / min-p, penalties, biases, log-probabilities of the answer."""
 from __future__ import annotations
 
-import math
 from dataclasses import dataclass
 from typing import Any, Dict, Tuple
 
@@ -50,7 +49,7 @@ def refusal(msg: Dict[str, Any], vocab: int) -> str:
     """Empty string if a request's settings can be served, else the reason."""
     def number(key, lo, hi, default, whole=False):
         v = msg.get(key, default)
-        if isinstance(v, bool) or not isinstance(v, int if whole else (int, float)) or not math.isfinite(v) or not lo <= v <= hi:
+        if isinstance(v, bool) or not isinstance(v, int if whole else (int, float)) or not lo <= v <= hi:    # (compared as it is: it may be no float's)
             return f"{key} must be {'an integer' if whole else 'a number'} from {lo} to {hi}"
         return ""
     bad = (number("top_k", -1, 1 << 30, 0, True) or number("top_p", 0.0, 1.0, 1.0) or number("min_p", 0.0, 1.0, 0.0)

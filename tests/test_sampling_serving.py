@@ -254,3 +254,29 @@ def test_a_sharded_vocabulary_draws_the_same():
         assert got[0][1][r] == _by_definition(z[r], WILD, r, list(range(5, 37)), [3, 3])
         lp, rank, ids, _ = want_logprobs(z[r], got[0][1][r], 3)
         assert got[0][2][r][1] == rank and abs(got[0][2][r][0] - lp) < 1e-5
+
+
+# ----------------------------------------------------------------------------- numbers that no float holds
+HUGE = 10 ** 400
+
+
+@pytest.mark.parametrize("field", ["top_k", "top_p", "min_p", "presence_penalty", "frequency_penalty", "repetition_penalty", "logprobs", "max_new"])
+@pytest.mark.parametrize("value", [HUGE, -HUGE, float("inf"), float("-inf"), float("nan")], ids=["huge", "-huge", "inf", "-inf", "nan"])
+def test_numbers_beyond_every_range_are_refused(field, value):
+    assert validate_request({"prompt_ids": [1], "max_new": 3, field: value}, 1000, 64) != ""
+
+
+@pytest.mark.parametrize("pair", [[HUGE, 1.0], [-HUGE, 1.0], [1, HUGE], [1, -HUGE], [1, float("nan")], [1, float("inf")]],
+                         ids=["huge id", "-huge id", "huge", "-huge", "nan", "inf"])
+def test_biases_beyond_every_range_are_refused(pair):
+    assert validate_request({"prompt_ids": [1], "max_new": 3, "logit_bias": [pair]}, 1000, 64) != ""
+
+
+def test_an_engine_outlives_numbers_beyond_every_range():
+    cfg, W, _ = _model()
+    es = EngineServer(cfg, W, EngineConfig(max_seqs=1, kv_tokens=512, prefill_chunk=32, spec="none"))
+    es.submit({"id": 1, "prompt_ids": [1, 2], "max_new": 2, "top_p": HUGE})
+    es.submit({"id": 2, "prompt_ids": [1, 2], "max_new": 2, "top_p": 0.5})
+    while es.sched.has_work():
+        es.step()
+    assert [x["id"] for x in es.out if "error" in x] == [1] and [x["id"] for x in es.out if x.get("done")] == [2]
