@@ -55,4 +55,17 @@ def validate_request(msg: Dict[str, Any], vocab: int, max_ctx: int) -> str:
         return "max_new must be a positive integer"
     if len(ids) + mn > max_ctx:
         return f"prompt ({len(ids)}) + max_new ({mn}) exceeds the context budget ({max_ctx})"
+    stop = msg.get("stop_token_ids", [])
+    if not isinstance(stop, (list, tuple)) or any((not isinstance(t, int)) or not -(1 << 31) <= t < 1 << 31 for t in stop):
+        return "stop_token_ids must be a list of token ids"
+    try:                                    # as the scheduler and the draws convert them
+        float(msg.get("temperature", 0.0))
+    except (TypeError, ValueError, OverflowError):
+        return "temperature must be a number"
+    try:
+        seed = int(msg.get("seed", 0))
+    except (TypeError, ValueError, OverflowError):
+        seed = -1
+    if not 0 <= seed < 1 << 63:
+        return "seed must be an integer from 0 to 2^63 - 1"
     return refusal(msg, vocab)

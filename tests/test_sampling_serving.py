@@ -280,3 +280,26 @@ def test_an_engine_outlives_numbers_beyond_every_range():
     while es.sched.has_work():
         es.step()
     assert [x["id"] for x in es.out if "error" in x] == [1] and [x["id"] for x in es.out if x.get("done")] == [2]
+
+
+BAD = [dict(seed=-1), dict(seed=1 << 63), dict(seed=1 << 64), dict(seed=HUGE), dict(seed="x"), dict(seed=None), dict(seed=float("inf")), dict(temperature=HUGE),
+       dict(temperature="x"), dict(temperature=None), dict(temperature=[1]), dict(stop_token_ids=[HUGE]), dict(stop_token_ids=["x"]), dict(stop_token_ids=[[1]]), dict(stop_token_ids=5)]
+
+
+def test_an_engine_outlives_settings_that_it_cannot_hold():
+    """Beside a request that goes on, which gets its whole answer; the largest seed and temperatures of every size are served."""
+    cfg, W, _ = _model()
+    es = EngineServer(cfg, W, EngineConfig(max_seqs=2, kv_tokens=2048, prefill_chunk=32, spec="mtp", spec_depth=2))
+    es.submit({"id": 1000, "prompt_ids": [5, 6, 7], "max_new": 40})
+    for i, bad in enumerate(BAD):
+        es.submit({"id": i, "prompt_ids": [1, 2], "max_new": 2, **bad})
+        es.step()
+    fine = [dict(seed=(1 << 63) - 1, temperature=0.8), dict(seed=3.0, temperature="0.5"), dict(temperature=1e300), dict(temperature=float("inf")), dict(temperature=float("nan")),
+            dict(temperature=-1), dict(stop_token_ids=[-5, 3])]
+    for i, good in enumerate(fine):
+        es.submit({"id": 100 + i, "prompt_ids": [1, 2], "max_new": 2, **good})
+    while es.sched.has_work():
+        es.step()
+    assert [x["id"] for x in es.out if "error" in x] == list(range(len(BAD)))
+    assert sorted(x["id"] for x in es.out if x.get("done")) == [100 + i for i in range(len(fine))] + [1000]
+    assert [len(x["token_ids"]) for x in es.out if x.get("done") and x["id"] == 1000] == [40]
