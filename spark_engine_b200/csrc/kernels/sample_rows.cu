@@ -1109,13 +1109,13 @@ logprob_kernel(const __grid_constant__ LogprobRows a, int per) {
       }
       seen.add(s, 0.0, E);
     }
-    if (zt == -INFINITY || (chunk * CHUNK <= tj && tj < (chunk + 1) * CHUNK)) {
+    if (isinf(zt) || (chunk * CHUNK <= tj && tj < (chunk + 1) * CHUNK)) {
 #pragma unroll
       for (int q = 0; q < 32; ++q) {
         const int j = Row<T, NT>::place(chunk, q, tid & 31);
         seen.n += v[q] > zt || (v[q] == zt && j < tj && j >= row.lo);
       }
-    } else {                                                   // (equal ones are in front of it in the chunks in front of its own)
+    } else {                                                   // (equal ones are in front of it in the chunks in front of its own; of a finite logit there is a next one)
       const float least = (chunk + 1) * CHUNK <= tj ? zt : nextafterf(zt, INFINITY);
 #pragma unroll
       for (int q = 0; q < 32; ++q) seen.n += v[q] >= least;

@@ -378,3 +378,22 @@ def test_scores_next_to_one_another():
     rows = Rows(400, 20000, "equal", seed=13, device="cuda")
     assert np.array_equal(rows.draw(2.0), rows.want(2.0))
     _sound()
+
+
+# ----------------------------------------------------------------------------- equal logits that are infinite
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("R, V", [(1, 5000), (1, 60001), (300, 5000)])
+def test_ranks_beside_several_infinite_logits(R, V, dtype):
+    """Of equal logits the lower id is first, infinite ones too, wherever in the row they are."""
+    z = np.random.RandomState(V).randn(V).astype(np.float32)
+    at = [0, 7, 1023, 1024, 2047, 4000, V - 1]
+    z[at] = np.inf
+    x = torch.tensor(z, device="cuda").to(TYPES[dtype]).expand(R, V)
+    z = x[0].float().cpu().numpy()
+    for t in at + [5, 3000]:
+        got = ops.token_logprobs(x, torch.full((R,), t, dtype=torch.int32, device="cuda"), 2)
+        lp, rank, ids, lps = want_logprobs(z, t, 2)
+        assert got.rank.tolist() == [rank] * R and got.ids.tolist() == [ids] * R
+        near(got.logprob.cpu(), [lp] * R)
+        near(got.logprobs.cpu(), [lps] * R)
+    _sound()
