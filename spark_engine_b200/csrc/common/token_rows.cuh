@@ -48,12 +48,13 @@ struct RowAdjust {
   int nd = 0, nb = 0;
 
   __device__ __forceinline__ RowAdjust(const Adjustments& a, int r, int* status) {
-    const int slot = a.slots ? a.slots[r] : r;
+    int slot = a.slots ? a.slots[r] : r;
+    if (a.counts && slot >= a.n_slots) {           // (what the row has said is not known: it has no penalties)
+      set_status(status, ST_BOUNDS, r, slot, a.n_slots);
+      slot = -1;
+    }
     if (slot >= 0) {
-      if (a.counts) {
-        if (slot < a.n_slots) counts = a.counts + slot * a.ld_counts;
-        else set_status(status, ST_BOUNDS, r, slot, a.n_slots);
-      }
+      if (a.counts) counts = a.counts + slot * a.ld_counts;
       if (a.repetition) rep = a.repetition[r];
       if (a.presence) pres = a.presence[r];
       if (a.frequency) freq = a.frequency[r];

@@ -6,7 +6,8 @@ noise that (seed, position, id) determine (`spec/sampling.py`): a row's token de
 that `gumbel_perturb` and `argmax` draw.
 
 Settings and state live on the device, the calls neither wait for it nor read from it, and a captured call may be replayed with others.  A slot outside
-the counts sets the device status word and the row goes without penalties (or its tokens are not counted); ids outside the vocabulary are left out."""
+the counts sets the device status word and the row goes without any penalties, drafted tokens' too (or its tokens are not counted); for tensors on the host
+it is a ValueError.  Ids outside the vocabulary are left out."""
 from __future__ import annotations
 
 import ctypes

@@ -397,3 +397,21 @@ def test_ranks_beside_several_infinite_logits(R, V, dtype):
         near(got.logprob.cpu(), [lp] * R)
         near(got.logprobs.cpu(), [lps] * R)
     _sound()
+
+
+# ----------------------------------------------------------------------------- slots outside the counts
+def test_a_slot_outside_the_counts_leaves_a_row_without_penalties():
+    """Without any: drafted tokens of the row are not penalised either; its biases and allowed tokens stay."""
+    from spark_engine_b200.ops import cuda
+    rows = Rows(4, 100, device="cuda")
+    i, f = torch.int32, torch.float32
+    a = ops.Adjust(counts=torch.full((2, 100), 3, dtype=i, device="cuda"), slots=rows.t([5, -1, 1, 2], i), drafted=rows.t([[3, 3, 60]] * 4, i), repetition=rows.t([1.5] * 4, f),
+                   presence=rows.t([0.5] * 4, f), frequency=rows.t([1.0] * 4, f), bias_ids=rows.t([[3, 9]] * 4, i), bias=rows.t([[2.0, -1.0]] * 4, f))
+    try:
+        got = ops.adjust_logits(rows.logits, a)
+        assert cuda.read_status(torch.device("cuda"))[0] != 0
+        want = ops.adjust_logits(rows.logits, a._replace(slots=rows.t([-1, -1, 1, -1], i)))
+        assert torch.equal(got, want) and not torch.equal(got[2, 10:], rows.logits[2, 10:])
+        assert torch.equal(got[0, 10:], rows.logits[0, 10:])
+    finally:
+        cuda.clear_status(torch.device("cuda"))
