@@ -16,9 +16,11 @@
 // CTAs' lists together), and for top_p a token is drawn first and the weight in front of it looked at then: what lies in front of a token drawn in vain
 // holds all that is kept, and half as much as before on average.
 //
-// Sums of weights: a chunk's in fp32 in units 2^E of its own, E whole, chunks' in 64 bits; a list's in whole numbers of 2^-40.  Each is the same however
-// chunks are dealt to CTAs and warps (to 2^-53), and so are log-probabilities.  How many CTAs a row has can decide which of the two a prefix's weight is:
-// they differ by 2^-20 of it, and a row draws the same in every batch but where top_p falls between them.
+// Sums of weights that decide what is kept are whole numbers of 2^-40, which no order changes: a row draws the same whatever CTAs it has and wherever in
+// memory it begins.  The weight of a row that top_p alone filters is streamed: a chunk's in fp32 in units 2^E of its own, E whole, chunks' in 64 bits.
+// Where what is kept ends within 2^-18 of that sum's share, the row is drawn again by a sum in whole numbers.  Log-probabilities go by the streamed sum:
+// they are the same however chunks are dealt to CTAs (to 2^-53); rows that begin elsewhere between two 16-byte boundaries have other chunks, and may have
+// another last bit.
 //
 // What bounds it (one B200, fp32 logits).  One row: ten trips to memory and barriers of a cluster one after the other, 12.7 us for 152k logits, of which
 // 2.5 are the row's own, 1.4 sums and best over eight CTAs, 1.4 bins, 4 the groups read again and lists joined, 2 the prefix and the draw.  Many rows whose
@@ -82,6 +84,7 @@ struct RowShared {
   float fsum[NT / 32];
   unsigned n_list, n_hits, before, kept;
   int bin, score;
+  bool unsure;
   float z;
   double log;
   Prefix cut;
@@ -318,6 +321,10 @@ struct Weights {
     return at_least(from + z - (fabsf(z) + fabsf(from)) * (1.f / 1048576) - (fabsf(E) + (b + 1)) * (1.f / 4194304) / c);
   }
 };
+
+// A weight in whole numbers of 2^-40: sums of them are the same in every order, so that what is kept does not depend on how a row is dealt out.
+__device__ __forceinline__ u64 whole(float w) { return __float2ull_rn(w * 1099511627776.f); }
+__device__ __forceinline__ double weight_of(u64 n) { return static_cast<double>(n) * (1.0 / 1099511627776.0); }
 
 template <int NT>
 __device__ __forceinline__ void clear_bins(RowShared<NT>& sh) {
@@ -693,38 +700,41 @@ struct Racer {
 };
 
 // A race over what lies within `front`, and the weight of that.
-struct Lap { Top2 m; double s; };
+struct Lap { Top2 m; u64 s; };
 template <bool RACE, bool MASS, class T, int NT>
 __device__ __noinline__ Lap lap(const Row<T, NT> row, const Groups groups, const Race race, const Weights w, const Prefix front, int* shared) {
   Racer racer;
-  double s = 0;
+  u64 s = 0;
   row.again([&](int k) { return groups.reaches(k, front.z); }, [&](const float* v, int k, int q) {
     const int chunk = row.chunk0 + k;
     const float mine = max8(v);
     if (__all_sync(0xffffffffu, !(mine >= front.z))) return;
     if (MASS) {
-      float f[8];
       bool last = false;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        f[i] = v[i] > front.z ? w(v[i]) : 0.f;
+        if (v[i] > front.z) s += whole(w(v[i]));
         last |= v[i] == front.z;
       }
       if (last) {                                  // as the last token of it: by their ids
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          if (v[i] == front.z && row.id(Row<T, NT>::place(chunk, q + i, threadIdx.x & 31)) <= front.id) f[i] = w(v[i]);
+          if (v[i] == front.z && row.id(Row<T, NT>::place(chunk, q + i, threadIdx.x & 31)) <= front.id) s += whole(w(v[i]));
       }
-      s += ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
     }
     if (RACE && (__any_sync(0xffffffffu, racer.bound > -INFINITY) || racer.template begin<8>(race, row, v, mine, chunk, q, front, shared)))
       racer.template run<false>(race, row, v, chunk, q, front, shared);
   });
   return Lap{racer.m, s};
 }
-__device__ __forceinline__ double row_total(Cluster& c, double s) {
-  return c.reduce(s, 0.0, [](double a, double b) { return a + b; });
+template <class S>
+__device__ __forceinline__ S row_total(Cluster& c, S s) {
+  return c.reduce(s, S{0}, [](S a, S b) { return a + b; });
 }
+// The streamed sum of a row is off from that in whole numbers by less than this of itself: 2^-20 for ten fp32 additions in a row at most (half a step
+// each), as much for the arguments of weights that count, seen from the chunk's best here and from the row's there.
+constexpr double SUM_OFF = 1.0 / 262144;
+__device__ __forceinline__ bool close_to(double in_front, double target) { return fabs(in_front - target) <= target * SUM_OFF; }
 
 // The winner among the tokens within `kept`, from the two best of a race.
 template <class T, int NT>
@@ -852,7 +862,7 @@ __device__ __noinline__ bool list_kept(RowShared<NT>& sh, Cluster& c, const Row<
   __syncthreads();
   return c.reduce(sh.n_list, 0u, [](unsigned a, unsigned b) { return max(a, b); }) <= LIST;
 }
-// A race over the list's entries within `front`, and their weight: in whole numbers, since entries come in any order.
+// A race over the list's entries within `front`, and their weight.
 template <int NT>
 __device__ __noinline__ Lap list_lap(const RowShared<NT>& sh, const Race race, const Weights w, const Prefix front, bool race_too, bool mass_too) {
   Top2 m = no_top();
@@ -863,10 +873,46 @@ __device__ __noinline__ Lap list_lap(const RowShared<NT>& sh, const Race race, c
     const float z = list_z(key);
     const int id = list_id(key);
     if (!within(front, z, id)) continue;
-    if (mass_too) s += __float2ull_rn(w(z) * 1099511627776.f);
+    if (mass_too) s += whole(w(z));
     if (race_too) m = best2(m, Top2{race.rough(z, id), id, -INFINITY, z});
   }
-  return Lap{m, static_cast<double>(s) * (1.0 / 1099511627776.0)};
+  return Lap{m, s};
+}
+
+// A draw by top_p alone, of a row whose tokens begin with `first`: by a sum in whole numbers and the scores as they are defined, by one CTA that reads
+// the row again and again (it is for what comes so near to the border that the streamed sum does not tell: 0.3 ms for 152k logits).  Other rows' sums are
+// in whole numbers from the start: `otherwise`.
+template <class T, int NT>
+__device__ __noinline__ int draw_in_whole(RowShared<NT>& sh, Cluster& c, const SampleRows& a, int r, const Weights w, int first, int otherwise) {
+  if ((a.top_k && a.top_k[r] > 0 && a.top_k[r] < a.V) || (a.min_p && a.min_p[r] > 0.f && isfinite(a.temps[r])) || w.from != 0.f) return otherwise;
+  const Row<T, NT> row(static_cast<const T*>(a.x) + r * a.ldx, a.V, 0, a.V);
+  const Race race(a.temps[r], w.c, a.seeds[r], a.positions[r]);
+  const auto every = [&](auto f) {
+    row.eights([](int) { return true; }, [&](const float (&v)[8], int k, int q) {
+#pragma unroll 1
+      for (int i = 0; i < 8; ++i) f(row.one(Row<T, NT>::place(k, q + i, threadIdx.x & 31)), row.id(Row<T, NT>::place(k, q + i, threadIdx.x & 31)));
+    });
+  };
+  const auto mass = [&](const Prefix& front) {
+    u64 s = 0;
+    every([&](float z, int id) { s += within(front, z, id) ? whole(w(z)) : 0; });
+    s = c.block(s, u64{0}, [](u64 x, u64 y) { return x + y; });
+    if (threadIdx.x == 0) sh.total = s;
+    __syncthreads();
+    return weight_of(sh.total);
+  };
+  Prefix front = whole_row();
+  const double target = a.top_p[r] * mass(front);
+  for (;;) {
+    Win b{-INFINITY, NO_ID, -INFINITY, 0};
+    every([&](float z, int id) { if (within(front, z, id)) b = first_win(b, Win{race.exact(z, id), id, z, 0}); });
+    b = c.block(b, Win{-INFINITY, NO_ID, -INFINITY, 0}, first_win);
+    if (threadIdx.x == 0) sh.cut = Prefix{b.z, b.id};
+    __syncthreads();
+    const Prefix win = sh.cut;
+    front = Prefix{win.z, win.id - 1};
+    if (win.id == first || mass(front) < target) return win.id;
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ kernels
@@ -901,7 +947,7 @@ sample_kernel(const __grid_constant__ SampleRows a, int per) {
   const float scale = greedy ? 0.f : fmaxf(fminf(__fdiv_rn(1.4426950408889634f, temp), -LOWEST), 1e-44f);
   const Race race(temp, scale, a.seeds[r], a.positions[r]);
   clear_bins(sh);
-  if (t == 0) { sh.n_list = sh.n_hits = 0; sh.score = score_key(-INFINITY); }
+  if (t == 0) { sh.n_list = sh.n_hits = 0; sh.unsure = false; sh.score = score_key(-INFINITY); }
   if (all) __syncthreads();
 
   Seen seen;
@@ -968,13 +1014,13 @@ sample_kernel(const __grid_constant__ SampleRows a, int per) {
   }
   double total = 0;
   if (sums && !far) total = seen.s * pow2(seen.E - weight.E);
-  else if (by_p && !by_k) total = row_total(c, lap<false, true>(row, groups, race, weight, kept, &sh.score).s);
+  else if (by_p && !by_k) total = weight_of(row_total(c, lap<false, true>(row, groups, race, weight, kept, &sh.score).s));
   unsigned n = LIST + 1;
   if (k <= LIST && !far) {
     float least = kept.z;
     bool found = false;
     if (by_k || by_p) {
-      const float need = by_k ? k : static_cast<float>(p * total * (1 + 1.0 / 262144));
+      const float need = by_k ? k : static_cast<float>(p * total * (1 + SUM_OFF));
       bins_of_threads(sh, c, parts.maxima, largest, weight, kept.z, by_k, need);
       // (the groups' largest may have the weight that the threads' have not, and they are more than these)
       if (sh.bin == BINS - 1 && (by_k || by_min || seen.g * pow2(seen.E - weight.E) >= need)) bins_of_groups(sh, c, groups, row.chunks, weight, kept.z, by_k, need);
@@ -986,13 +1032,12 @@ sample_kernel(const __grid_constant__ SampleRows a, int per) {
   }
   if (n <= LIST) {
     if (c.rank) return;
-    // Weights in whole numbers of 2^-40, which no order changes: every token before the one that reaches top_p is kept.
-    const auto whole = [&](u64 key) { return __float2ull_rn(weight(list_z(key)) * 1099511627776.f); };
+    const auto weighed = [&](u64 key) { return whole(weight(list_z(key))); };
     const unsigned n1 = by_k ? min(n, static_cast<unsigned>(k)) : n;
     int token;
     if (n <= FEW_OF<NT>) {
       if (by_p) {
-        if (t < n) sh.weight[t] = whole(sh.list[t]);
+        if (t < n) sh.weight[t] = weighed(sh.list[t]);
         __syncthreads();
       }
       const Counted e = count_list(sh, n, by_p);
@@ -1000,26 +1045,28 @@ sample_kernel(const __grid_constant__ SampleRows a, int per) {
       if (by_p) {
         if (e.mine && e.rank + 1 == n1) sh.total = e.before + e.weight;
         __syncthreads();
-        const double target = static_cast<double>(p) * (by_k ? static_cast<double>(sh.total) : total * 1099511627776.0);
-        in = in && (e.rank == 0 || static_cast<double>(e.before) < target);
+        const double before = weight_of(e.before), target = p * (by_k ? weight_of(sh.total) : total);
+        if (in && close_to(before, target)) sh.unsure = true;
+        in = in && (e.rank == 0 || before < target);                   // (every token before the one that reaches top_p)
       }
       token = draw_listed(sh, c, race, [&](auto f) { if (in) f(e.key); }).id;
+      if (sh.unsure) token = draw_in_whole<T, NT>(sh, c, a, r, weight, top.id, token);
     } else {                                       // longer ones as rows are that keep very many: drawn first, looked at then
       Prefix in = whole_row();
       if (n1 < n) {
         const u64 last = nth_key(sh, n, n1);
         in = Prefix{list_z(last), list_id(last)};
       }
-      const auto weight_of = [&](const Prefix& f) {
+      const auto in_front = [&](const Prefix& f) {
         u64 w = 0;
         for (unsigned i = t; i < n; i += NT) {
           const u64 key = sh.list[i];
-          w += within(f, list_z(key), list_id(key)) ? whole(key) : 0;
+          w += within(f, list_z(key), list_id(key)) ? weighed(key) : 0;
         }
         w = c.block(w, u64{0}, [](u64 x, u64 y) { return x + y; });
         if (t == 0) sh.total = w;
         __syncthreads();
-        return static_cast<double>(sh.total);
+        return weight_of(sh.total);
       };
       const auto draw = [&](const Prefix& f) {
         return draw_listed(sh, c, race, [&](auto g) {
@@ -1027,11 +1074,16 @@ sample_kernel(const __grid_constant__ SampleRows a, int per) {
             if (within(f, list_z(sh.list[i]), list_id(sh.list[i]))) g(sh.list[i]);
         });
       };
-      const double target = by_p ? p * (by_k ? weight_of(in) : total * 1099511627776.0) : 0;
+      const double target = by_p ? p * (by_k ? in_front(in) : total) : 0;
       Prefix win = draw(in);
       while (by_p && win.id != top.id) {
         const Prefix front{win.z, win.id - 1};
-        if (weight_of(front) < target) break;
+        const double w = in_front(front);
+        if (close_to(w, target)) {
+          const int exact = draw_in_whole<T, NT>(sh, c, a, r, weight, top.id, -1);
+          if (exact >= 0) { win.id = exact; break; }
+        }
+        if (w < target) break;
         win = draw(front);
       }
       token = win.id;
@@ -1051,12 +1103,17 @@ sample_kernel(const __grid_constant__ SampleRows a, int per) {
     return mass_too ? lap<true, true>(row, groups, race, weight, front, &sh.score) : lap<true, false>(row, groups, race, weight, front, &sh.score);
   };
   const Lap l = go(kept, true, by_k && by_p);
-  if (by_k && by_p) total = row_total(c, l.s);
+  if (by_k && by_p) total = weight_of(row_total(c, l.s));
   Win win = settle(row, c, race, kept, l.m);
   const double target = p * total;
   while (by_p && win.id != top.id) {               // what lies in front of it; who wins there, should that be too much
     const Prefix front{win.z, win.id - 1};
-    if (row_total(c, go(front, false, true).s) < target) break;
+    const double w = weight_of(row_total(c, go(front, false, true).s));
+    if (close_to(w, target)) {
+      const int exact = draw_in_whole<T, NT>(sh, c, a, r, weight, top.id, -1);
+      if (exact >= 0) { win.id = exact; break; }
+    }
+    if (w < target) break;
     if (t == 0) sh.score = score_key(-INFINITY);   // (all warps are past the last race, and none begins the next before the barrier)
     __syncthreads();
     win = settle(row, c, race, front, go(front, true, false).m);

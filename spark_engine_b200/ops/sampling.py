@@ -170,8 +170,8 @@ def sample_tokens(logits, temps, seeds, positions, top_k=None, top_p=None, min_p
     Drawn is the arg-max over kept of fp32(logit / temperature) + fp32(g), g = -log(-log u), u from (seed, position, id); rows of temperature <= 0, and
     rows whose best logit / temperature is 2^30 or more in size, beside which noise is nothing, take the first of the order.
 
-    Weights are fp32 (to about 2^-20 of themselves), their sums 64 bits: only where the probability up to a token comes that close to top_p can the last
-    one kept be its neighbour, or another one in another batch.  An `adjust` takes a workspace of R * V fp32 from torch's allocator, which a captured call keeps."""
+    Weights are fp32 (to about 2^-20 of themselves), their sums whole numbers of 2^-40: only where the probability up to a token comes that close to top_p
+    can the last one kept be its neighbour, and it is the same one in every batch and wherever the row lies.  An `adjust` takes a workspace of R * V fp32 from torch's allocator, which a captured call keeps."""
     run = _kernels(logits)
     t = _native().sample_tokens(logits, temps, seeds, positions, top_k, top_p, min_p, adjust, run)
     if run:

@@ -415,3 +415,67 @@ def test_a_slot_outside_the_counts_leaves_a_row_without_penalties():
         assert torch.equal(got[0, 10:], rows.logits[0, 10:])
     finally:
         cuda.clear_status(torch.device("cuda"))
+
+
+# ----------------------------------------------------------------------------- sums that decide
+def _borders(z, T, k, n, least):
+    """(seed, top_p) of n rows at position 0 whose race has a record at the token that top_p just keeps or just leaves out, as sums are rounded."""
+    from spark_engine_b200.spec.sampling import uniform_ref
+    from tests.sampling_util import order
+    ids = order(z)[:k]
+    w = np.exp((z[ids].astype(np.float64) - float(z[ids[0]])) / T)
+    before, total = np.cumsum(w) - w, w.sum()
+    got, seed = [], 0
+    while len(got) < n:
+        score = z[ids].astype(np.float64) / T - np.log(-np.log(uniform_ref(seed, 0, len(z)).numpy()[ids]))
+        record = np.flatnonzero(score[1:] > np.maximum.accumulate(score)[:-1]) + 1
+        got += [(seed, np.float32(before[i] / total)) for i in record if i >= least]
+        seed += 1
+    return got[:n]
+
+
+@pytest.mark.parametrize("k, m", [(3000, 0.0), (1500, 0.0), (0, 0.025), (0, 0.0)])
+def test_sums_decide_the_same_in_every_batch(k, m):
+    """top_p right at the border of a token that wins if it is kept: drawn in one batch of many rows, in batches of few, one by one, and wherever the row begins."""
+    V, T, R = 50001, 1.0, 1200
+    z = Rows(1, V, "flat", seed=21).z[0]
+    n = k or (int((z >= z.max() + T * np.log(m)).sum()) if m else V)
+    seeds, p = zip(*_borders(z, T, n, R, 50))
+    one = lambda x, d: torch.tensor(np.asarray(x), dtype=d, device="cuda")
+    a = dict(temps=one([T] * R, torch.float32), seeds=one(seeds, torch.int64), positions=one([0] * R, torch.int64), top_k=one([k] * R, torch.int32), top_p=one(p, torch.float32),
+             min_p=one([m] * R, torch.float32))
+
+    def draws(x, rows, size):
+        part = lambda i, j: ops.sample_tokens(x.expand(j - i, V), **{name: y[i:j].contiguous() for name, y in a.items()}).tolist()
+        return sum((part(i, min(i + size, rows)) for i in range(0, rows, size)), [])
+    every = None
+    for shift in range(4):
+        x = torch.full((V + 4,), 99.0, device="cuda")[shift: shift + V].unsqueeze(0)
+        x.copy_(one(z, torch.float32).unsqueeze(0))
+        for rows, size in ((R, R), (R, 200), (R, 60), (R, 8), (100, 1)):
+            got = draws(x, rows, size)
+            every = every or got
+            assert got == every[:rows], (shift, size, sum(g != e for g, e in zip(got, every)))
+    _sound()
+
+
+@pytest.mark.parametrize("V, spread", [(300, 1.0), (4099, 3.0), (50001, 3.0)])
+def test_borders_of_short_prefixes_are_the_same_in_every_batch(V, spread):
+    """The same where few tokens are kept."""
+    T, R = 0.7, 600
+    z = (np.random.RandomState(V).randn(V) * spread).astype(np.float32)
+    seeds, p = zip(*_borders(z, T, 200, R, 1))
+    w = np.exp((np.sort(z.astype(np.float64))[::-1] - float(z.max())) / T)
+    p = np.float32(np.asarray(p) * (w[:200].sum() / w.sum()))            # (of the whole row's weight)
+    one = lambda x, d: torch.tensor(np.asarray(x), dtype=d, device="cuda")
+    f, i = torch.float32, torch.int64
+    every = None
+    for shift in range(4):
+        x = torch.full((V + 4,), 99.0, device="cuda")[shift: shift + V].unsqueeze(0)
+        x.copy_(one(z, f).unsqueeze(0))
+        for size in (R, 40, 1):
+            got = sum((ops.sample_tokens(x.expand(len(seeds[j: j + size]), V), one([T] * len(seeds[j: j + size]), f), one(seeds[j: j + size], i), one([0] * len(seeds[j: j + size]), i),
+                                         top_p=one(p[j: j + size], f)).tolist() for j in range(0, R if size > 1 else 100, size)), [])
+            every = every or got
+            assert got == every[: len(got)], (shift, size, sum(g != e for g, e in zip(got, every)))
+    _sound()
