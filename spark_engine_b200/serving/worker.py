@@ -303,6 +303,9 @@ class EngineServer:
                 s = lv.seq
                 h_last = hid[seg.r0 + seg.n - 1].clone()
                 first = self.spec.first_token(s, logits[k], prompt)
+                if s.failed:
+                    self._fail(slot)
+                    continue
                 s.hidden = h_last
                 s.pending_mtp = [(h_last.clone(), first)]
                 s.generated = [first]
@@ -397,7 +400,22 @@ class EngineServer:
                 cut.append(t)
                 if t in own_stop:
                     break
-            self._emit(lv, cut)
+            if cut:
+                self._emit(lv, cut)
+            if lv.seq.failed and lv.seq.slot in self.by_slot:        # (and it has not come to its end with these)
+                self._fail(lv.seq.slot)
+
+    def _fail(self, slot: int):
+        """Ends a request whose logits are no numbers.  What its slot holds is of no use to another one."""
+        lv = self.by_slot.pop(slot)
+        self.totals["requests"] += 1
+        self.totals["drafted_tokens"] += lv.seq.drafted
+        self.totals["accepted_drafts"] += lv.seq.accepted
+        self.out.append({"id": lv.id, "error": "the model's logits are not numbers: no token can be drawn"})
+        self.kv.release(slot)
+        self.model.reset_slot(slot)
+        self.sched.on_finished(slot)
+        self.live.pop(lv.id, None)
 
     def _finish(self, slot: int, reason: str):
         lv = self.by_slot.pop(slot, None)

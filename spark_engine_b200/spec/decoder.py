@@ -35,6 +35,7 @@ class SeqSpec:
     params: Optional[SamplingParams] = None            # of requests that ask for more than a temperature
     logprobs: List[tuple] = field(default_factory=list)  # of the tokens that the last round emitted, where asked for
     generated: List[int] = field(default_factory=list)
+    failed: bool = False                               # the last round came to a row without any token (NaN logits): there is no next one
     drafted: int = 0
     accepted: int = 0
     table: P.AcceptanceTable = field(default_factory=P.AcceptanceTable)
@@ -115,23 +116,32 @@ class SpecDecoder:
             temperature, seed = params.temperature, params.seed
         seq = SeqSpec(slot, -1, hid[-1].clone(), temperature=temperature, seed=seed, params=params)
         first = self.first_token(seq, last, prompt)
-        seq.pending_mtp = [(hid[-1].clone(), first)]
         seq.lookup = LookupIndex(self.lookup_n)
-        seq.lookup.extend(list(prompt) + [first])
-        seq.generated = [first]
+        seq.lookup.extend(list(prompt))
+        if not seq.failed:
+            seq.pending_mtp = [(hid[-1].clone(), first)]
+            seq.lookup.extend([first])
+            seq.generated = [first]
         return seq
 
     def first_token(self, seq: SeqSpec, logits: torch.Tensor, prompt: Sequence[int]) -> int:
-        """The token behind a prompt, from its last row's logits; begins the counts of a request with penalties."""
+        """The token behind a prompt, from its last row's logits (`seq.failed` where there is none); begins the counts of a request with penalties."""
         m, p = self.m, seq.params
         if p is None or not p.shaped:
             seq.last_token = m.sample(logits, seq.temperature, seq.seed, len(prompt))
+            self._tokens(seq, [seq.last_token])
             return seq.last_token
         if p.counted:
             m.count_prompt(seq.slot, prompt)
         seq.last_token = m.draw_rows(logits, [p], [seq.slot], [len(prompt)])[0]
-        self._said([seq], [[seq.last_token]], logits.reshape(1, -1), [[0]])
+        self._said([seq], [self._tokens(seq, [seq.last_token])], logits.reshape(1, -1), [[0]])
         return seq.last_token
+
+    def _tokens(self, seq: SeqSpec, out: List[int]) -> List[int]:
+        """What of a round's tokens are tokens: a row whose logits are no numbers has none (-1, or an id behind the vocabulary), and ends the sequence."""
+        n = next((j for j, t in enumerate(out) if not 0 <= t < self.m.cfg.vocab), len(out))
+        seq.failed = n < len(out)
+        return out[:n]
 
     @staticmethod
     def _params(seq: SeqSpec) -> SamplingParams:
@@ -199,8 +209,8 @@ class SpecDecoder:
     @torch.no_grad()
     def round(self, seqs: List[SeqSpec], budgets: Optional[List[int]] = None, stop: Sequence[int] = (),
               proposals: Optional[List[tuple]] = None) -> List[List[int]]:
-        """One speculative round over all given sequences.  Returns the tokens emitted per sequence.  `proposals`:
-        (draft tokens, confidences) per sequence from the caller instead of the drafter."""
+        """One speculative round over all given sequences.  Returns the tokens emitted per sequence (fewer, or none, of one that
+        has `failed`).  `proposals`: (draft tokens, confidences) per sequence from the caller instead of the drafter."""
         m = self.m
         L = [m.seqs[s.slot].length for s in seqs]
         k_graph = 1 + self.depth
@@ -270,7 +280,7 @@ class SpecDecoder:
                 s.table.observe(j, cj[j] if j < len(cj) else 0.5, j < n)
             s.drafted += len(d)
             s.accepted += n
-            emitted.append(out)
+            emitted.append(self._tokens(s, out))
         if shaped:
             self._said(seqs, emitted, logits, [[r0 + r for r in rows] for r0, rows in zip(row0, accepted_rows)])
         if vg is None:
@@ -289,7 +299,7 @@ class SpecDecoder:
                 if nxt is not None:
                     new_pairs.append((hidden[r0 + j] if vg is not None else hidden[r0 + j].clone(), nxt))
             s.pending_mtp = new_pairs
-            s.last_token = out[-1]
+            s.last_token = out[-1] if out else s.last_token
             s.hidden = hidden[r0 + rows[-1]] if vg is not None else hidden[r0 + rows[-1]].clone()
             s.generated.extend(out)
             if s.lookup is not None:
@@ -362,14 +372,14 @@ class SpecDecoder:
             accepted_rows.append(rows)
             s.drafted += len(nodes)
             s.accepted += len(path)
-            emitted.append(out)
+            emitted.append(self._tokens(s, out))
         if shaped:
             self._said(seqs, emitted, logits, [[seg.r0 + r for r in rows] for seg, rows in zip(plan.segs, accepted_rows)])
         m.commit(accepted_rows)
         for i, (s, out) in enumerate(zip(seqs, emitted)):
             seg, rows = plan.segs[i], accepted_rows[i]
             s.pending_mtp = [(hidden[seg.r0 + r].clone(), out[j]) for j, r in enumerate(rows) if j < len(out)]
-            s.last_token = out[-1]
+            s.last_token = out[-1] if out else s.last_token
             s.hidden = hidden[seg.r0 + rows[-1]].clone()
             s.generated.extend(out)
             if s.lookup is not None:
@@ -395,9 +405,10 @@ class SpecDecoder:
     def generate(self, prompts: List[Sequence[int]], max_new: int, stop: Sequence[int] = (), temperature: float = 0.0,
                  seed: int = 0, params: Optional[SamplingParams] = None) -> List[List[int]]:
         seqs = [self.start(i, p, temperature, seed, params=params) for i, p in enumerate(prompts)]
-        live = [s for s in seqs if len(s.generated) < max_new and s.generated[-1] not in stop]
+        goes_on = lambda s: not s.failed and len(s.generated) < max_new and s.generated[-1] not in stop     # noqa: E731
+        live = [s for s in seqs if goes_on(s)]
         while live:
             budgets = [max_new - len(s.generated) for s in live]
             self.round(live, budgets, stop)
-            live = [s for s in live if len(s.generated) < max_new and s.generated[-1] not in stop]
+            live = [s for s in live if goes_on(s)]
         return [s.generated[:max_new] for s in seqs]

@@ -303,3 +303,82 @@ def test_an_engine_outlives_settings_that_it_cannot_hold():
     assert [x["id"] for x in es.out if "error" in x] == list(range(len(BAD)))
     assert sorted(x["id"] for x in es.out if x.get("done")) == [100 + i for i in range(len(fine))] + [1000]
     assert [len(x["token_ids"]) for x in es.out if x.get("done") and x["id"] == 1000] == [40]
+
+
+# ----------------------------------------------------------------------------- rows without any token
+NOTHING = SamplingParams(temperature=0.9, seed=4, top_p=0.8, frequency=0.3, logprobs=2)
+
+
+def _blind(m, slot, length):
+    """The model's logits of a slot's rows are NaN from position `length` on."""
+    forward = m.forward
+
+    def blinded(plan, *a, **k):
+        logits = forward(plan, *a, **k)
+        for i, s in enumerate(plan.segs):
+            rows = range(s.r0, s.r0 + s.n) if logits.shape[0] == sum(x.n for x in plan.segs) else [i]
+            if s.slot == slot() and s.pos0 + s.n >= length:
+                logits[list(rows)] = float("nan")
+        return logits
+    m.forward = blinded
+    return lambda: setattr(m, "forward", forward)
+
+
+@pytest.mark.parametrize("tree", [False, True])
+def test_a_round_without_a_token_ends_its_sequence(tree):
+    """Nothing that is no token is emitted, counted or drafted from; the sequences beside it go on."""
+    cfg, W, m = _model()
+    prompts = _prompts(cfg, 2)
+    want, _ = _text(SpecDecoder(m, lambda s, d: ([], []), depth=0), prompts, [NOTHING, WILD], 12)
+    _, _, m = _model()
+    sd = SpecDecoder(m, lambda s, d: ([], []), depth=0)
+    seqs = [sd.start(i, p, params=q) for i, (p, q) in enumerate(zip(prompts, [NOTHING, WILD]))]
+    _blind(m, lambda: 0, len(prompts[0]) + 4)
+    while any(len(s.generated) < 12 and not s.failed for s in seqs):
+        live = [s for s in seqs if len(s.generated) < 12 and not s.failed]
+        budgets = [12 - len(s.generated) for s in live]
+        if tree:
+            sd.round_tree(live, [[Node(token=(want[s.slot] + [0])[len(s.generated)], parent=-1)] for s in live], budgets)
+        else:
+            sd.round(live, budgets)
+    assert seqs[0].failed and seqs[0].generated == want[0][: len(seqs[0].generated)] and 2 <= len(seqs[0].generated) < 6
+    assert not seqs[1].failed and seqs[1].generated == want[1]
+    assert int((m.token_counts()[0] >> 1).sum()) == len(seqs[0].generated)
+
+
+def test_a_prompt_without_a_token():
+    cfg, W, m = _model()
+    prompts = _prompts(cfg, 1)
+    sd = SpecDecoder(m, lambda s, d: ([], []), depth=0)
+    see = _blind(m, lambda: 0, 0)
+    seq = sd.start(0, prompts[0], params=NOTHING)
+    assert seq.failed and seq.generated == [] and seq.logprobs == [] and not (m.token_counts()[0] >> 1).any()
+    assert sd.generate(prompts, 5, params=NOTHING) == [[]]
+    see()
+    assert len(sd.generate(prompts, 5, params=NOTHING)[0]) == 5
+
+
+@pytest.mark.parametrize("after", [0, 4])
+def test_a_server_ends_requests_without_a_token(after):
+    """With an error and what was said before; the request again (over what its slot was left with) has its whole text, and so have those beside it."""
+    cfg, W, m = _model()
+    prompts = _prompts(cfg, 2)
+    alone = []
+    for p, q in zip(prompts, [NOTHING, WILD]):
+        alone += _text(SpecDecoder(m, lambda s, d: ([], []), depth=0), [p], [q], 10)[0]
+    es = EngineServer(cfg, W, EngineConfig(max_seqs=2, kv_tokens=2048, prefill_chunk=32, spec="mtp", spec_depth=2))
+    see = _blind(es.model, lambda: next((s for s, lv in es.by_slot.items() if lv.id == 0), -1), len(prompts[0]) + after)
+    for i, q in enumerate([NOTHING, WILD]):
+        es.submit(_message(i, prompts[i], q, 10))
+    while es.sched.has_work():
+        es.step()
+    see()
+    es.submit(_message(2, prompts[0], NOTHING, 10))
+    while es.sched.has_work():
+        es.step()
+    mine = [x for x in es.out if x.get("id") == 0]
+    said = sum((x["delta"] for x in mine if "delta" in x), [])
+    assert "error" in mine[-1] and not any(x.get("done") for x in mine) and said == alone[0][: len(said)] and (len(said) == 0) == (after == 0)
+    assert sum(len(x.get("logprobs", [])) for x in mine) == len(said)
+    done = {x["id"]: x["token_ids"] for x in es.out if x.get("done")}
+    assert done == {1: alone[1], 2: alone[0]} and not es.live and not es.by_slot
