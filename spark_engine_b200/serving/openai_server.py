@@ -189,7 +189,9 @@ def sampling_fields(body: dict, chat: bool) -> dict:
         f["logit_bias"] = [[int(t), b] for t, b in bias.items()]
     if chat:
         if body.get("logprobs"):
-            f["logprobs"] = body.get("top_logprobs") or 0
+            f["logprobs"] = top = body.get("top_logprobs") or 0
+            if isinstance(body.get("top_logprobs"), bool) or not isinstance(top, int) or top < 0:
+                raise ValueError("top_logprobs must be a whole number")
         elif body.get("top_logprobs"):
             raise ValueError("top_logprobs needs logprobs")
     elif body.get("logprobs") is not None and body.get("logprobs") is not False:
@@ -264,9 +266,9 @@ class App:
         eos = getattr(self.tok, "eos_token_id", None)
         t0 = time.time()
         sampling = sampling_fields(body, chat)
+        lps = LogprobLog(self.tok, chat) if sampling.get("logprobs", -1) >= 0 else None
         rid, q = self.engine.generate(prompt_ids, max_new, [eos] if eos is not None else [], float(body.get("temperature", 0.0) or 0.0),
                                       int(body.get("seed", 0) or 0), mm=mm, **({"sampling": sampling} if sampling else {}))
-        lps = LogprobLog(self.tok, chat) if sampling.get("logprobs", -1) >= 0 else None
         if lps is not None and write_event:
             plain_event = write_event
             write_event = lambda r, c: plain_event(r, c, lps.take())       # noqa: E731

@@ -382,3 +382,42 @@ def test_a_server_ends_requests_without_a_token(after):
     assert sum(len(x.get("logprobs", [])) for x in mine) == len(said)
     done = {x["id"]: x["token_ids"] for x in es.out if x.get("done")}
     assert done == {1: alone[1], 2: alone[0]} and not es.live and not es.by_slot
+
+
+# ----------------------------------------------------------------------------- the front end alone
+class Engine:
+    """An engine that answers with the given messages."""
+    alive = True
+
+    def __init__(self, messages=()):
+        self.messages, self.queues, self.asked, self.cancelled = list(messages), {}, [], []
+
+    def generate(self, ids, max_new, stop, temperature, seed, mm=None, sampling=None):
+        import queue
+        rid = len(self.asked)
+        q = self.queues[rid] = queue.Queue()
+        self.asked.append(sampling or {})
+        for m in self.messages:
+            q.put(dict(m, id=rid))
+        return rid, q
+
+    def cancel(self, rid):
+        self.cancelled.append(rid)
+
+    def release(self, rid):
+        self.queues.pop(rid, None)
+
+
+def _app(messages=(), tok=None):
+    from spark_engine_b200.serving.openai_server import App
+    from spark_engine_b200.serving.tokenizer import ByteTokenizer
+    return App(Engine(messages), tok or ByteTokenizer(), "tiny")
+
+
+@pytest.mark.parametrize("top", ["3", "x", [3], 3.5, -1, True, {"a": 1}])
+def test_top_logprobs_that_are_no_number_are_refused(top):
+    """Before the engine hears of the request."""
+    app = _app([{"error": "it has heard of it"}])
+    with pytest.raises(ValueError, match="top_logprobs"):
+        app.run([1], {"logprobs": True, "top_logprobs": top}, True)
+    assert not app.engine.asked and not app.engine.queues
