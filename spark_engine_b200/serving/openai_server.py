@@ -200,24 +200,37 @@ def sampling_fields(body: dict, chat: bool) -> dict:
 
 
 class LogprobLog:
-    """Log-probabilities of an answer in the API's form; `take` gives those since it was last asked."""
+    """Log-probabilities of an answer in the API's form; `take` gives those since it was last asked.  Tokens are named by their text, those that end or begin
+    inside a character by their bytes ("bytes:\\xe4\\xbd"), and where a name is taken by a more probable one, by their number ("token_id:5").  -9999 is
+    what the API has for a probability of nothing (JSON has no infinities)."""
 
     def __init__(self, tok, chat: bool):
-        self.tok, self.chat, self.entries, self.taken, self.offset = tok, chat, [], 0, 0
+        self.tok, self.chat, self.entries, self.taken, self.offset, self.names = tok, chat, [], 0, 0, {}
 
-    def _text(self, i: int) -> str:
-        return self.tok.decode([i])
+    def _name(self, i: int):
+        """(name, bytes) of a token."""
+        if i not in self.names:
+            raw = self.tok.token_bytes(i)
+            try:
+                self.names[i] = raw.decode(), list(raw)
+            except UnicodeDecodeError:
+                self.names[i] = "bytes:" + "".join(f"\\x{b:02x}" for b in raw), list(raw)
+        return self.names[i]
 
     def feed(self, ids: List[int], got: List[list]):
+        number = lambda x: max(x, -9999.0)                               # noqa: E731
         for t, (lp, _, top) in zip(ids, got):
-            text = self._text(t)
-            raw = lambda s: list(s.encode())
+            name, raw = self._name(t)
+            listed = {}
+            for i, x in top:
+                n, b = self._name(i)
+                listed[n if n not in listed else f"token_id:{i}"] = number(x), b
             if self.chat:
-                self.entries.append({"token": text, "logprob": lp, "bytes": raw(text),
-                                     "top_logprobs": [{"token": self._text(i), "logprob": x, "bytes": raw(self._text(i))} for i, x in top]})
+                self.entries.append({"token": name, "logprob": number(lp), "bytes": raw,
+                                     "top_logprobs": [{"token": n, "logprob": x, "bytes": b} for n, (x, b) in listed.items()]})
             else:
-                self.entries.append((text, lp, {self._text(i): x for i, x in top}, self.offset))
-                self.offset += len(text)
+                self.entries.append((name, number(lp), {n: x for n, (x, _) in listed.items()}, self.offset))
+                self.offset += len(self.tok.decode([t]))
 
     def form(self, entries) -> dict:
         if self.chat:

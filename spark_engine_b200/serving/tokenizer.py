@@ -3,6 +3,7 @@ given, otherwise a byte-level fallback (ids 0..255 = bytes, 256 = BOS, 257 = EOS
 without any checkpoint.  Incremental detokenisation holds back incomplete UTF-8 sequences."""
 from __future__ import annotations
 
+import re
 from typing import List, Optional
 
 
@@ -18,6 +19,9 @@ class ByteTokenizer:
 
     def decode(self, ids: List[int]) -> str:
         return bytes(i for i in ids if i < 256).decode("utf-8", errors="replace")
+
+    def token_bytes(self, i: int) -> bytes:
+        return bytes([i]) if i < 256 else b""
 
     def apply_chat_template(self, messages, add_generation_prompt=True, tools=None) -> List[int]:
         parts = []
@@ -39,6 +43,16 @@ class ByteTokenizer:
         return ids
 
 
+def _byte_letters():
+    """Letters that byte-level vocabularies write bytes as: Latin-1's visible ones stand for themselves, U+0100 and on for the other bytes in order."""
+    visible = [b for b in range(256) if 0x21 <= b <= 0x7e or 0xa1 <= b <= 0xff and b != 0xad]
+    other = [b for b in range(256) if b not in visible]
+    return {**{chr(b): b for b in visible}, **{chr(0x100 + i): b for i, b in enumerate(other)}}
+
+
+_BYTE_LETTERS = _byte_letters()
+
+
 class HfTokenizer:
     def __init__(self, path: str):
         from transformers import AutoTokenizer
@@ -58,6 +72,17 @@ class HfTokenizer:
 
     def decode(self, ids):
         return self.tk.decode(ids, skip_special_tokens=True)
+
+    def token_bytes(self, i: int) -> bytes:
+        """What a token adds to the text.  Where it ends or begins inside a character its decoded text does not say; its piece of the vocabulary does."""
+        text = self.tk.decode([i], skip_special_tokens=True)
+        piece = self.tk.convert_ids_to_tokens(i) if "\ufffd" in text else None
+        if not piece:
+            return text.encode()
+        one = re.fullmatch("<0x([0-9A-Fa-f]{2})>", piece)
+        if one:
+            return bytes([int(one[1], 16)])
+        return bytes(_BYTE_LETTERS[c] for c in piece) if all(c in _BYTE_LETTERS for c in piece) else text.encode()
 
     def apply_chat_template(self, messages, add_generation_prompt=True, tools=None):
         return self.tk.apply_chat_template(messages, add_generation_prompt=add_generation_prompt, tools=tools, tokenize=True)

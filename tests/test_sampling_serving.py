@@ -421,3 +421,78 @@ def test_top_logprobs_that_are_no_number_are_refused(top):
     with pytest.raises(ValueError, match="top_logprobs"):
         app.run([1], {"logprobs": True, "top_logprobs": top}, True)
     assert not app.engine.asked and not app.engine.queues
+
+
+def _byte_level(tmp_path):
+    """A tokenizer of the byte-level kind: every byte a token, and a few longer ones of which one ends inside a character."""
+    from tokenizers import Tokenizer, decoders, models, pre_tokenizers
+    from transformers import PreTrainedTokenizerFast
+    from spark_engine_b200.serving.tokenizer import HfTokenizer
+    letters = sorted(pre_tokenizers.ByteLevel.alphabet())
+    tk = PreTrainedTokenizerFast(tokenizer_object=Tokenizer(models.BPE({c: i for i, c in enumerate(letters)}, [])), eos_token="</s>")
+    tk.backend_tokenizer.pre_tokenizer = pre_tokenizers.ByteLevel(add_prefix_space=False, use_regex=False)
+    tk.backend_tokenizer.decoder = decoders.ByteLevel()
+    tk.save_pretrained(str(tmp_path))
+    return HfTokenizer(str(tmp_path))
+
+
+def _byte_fallback(tmp_path):
+    """One of the kind that has a piece <0xXX> for every byte that no other piece covers."""
+    from tokenizers import Tokenizer, decoders, models
+    from transformers import PreTrainedTokenizerFast
+    from spark_engine_b200.serving.tokenizer import HfTokenizer
+    vocab = {f"<0x{i:02X}>": i for i in range(256)}
+    vocab.update({"h": 256, "i": 257})
+    tk = PreTrainedTokenizerFast(tokenizer_object=Tokenizer(models.BPE(vocab, [], byte_fallback=True)), eos_token="</s>")
+    tk.backend_tokenizer.decoder = decoders.Sequence([decoders.ByteFallback(), decoders.Fuse()])
+    tk.save_pretrained(str(tmp_path))
+    return HfTokenizer(str(tmp_path))
+
+
+TEXT = "hé 你\U0001f600i"
+
+
+def _toks(kind, tmp_path):
+    """(tokenizer, ids of TEXT's bytes one by one)."""
+    from spark_engine_b200.serving.tokenizer import ByteTokenizer
+    raw = TEXT.encode()
+    if kind == "bytes":
+        return ByteTokenizer(), list(raw)
+    if kind == "fallback":
+        return _byte_fallback(tmp_path), list(raw)
+    tok = _byte_level(tmp_path)
+    ids = tok.encode(TEXT)
+    assert len(ids) == len(raw)
+    return tok, ids
+
+
+@pytest.mark.parametrize("kind", ["bytes", "level", "fallback"])
+def test_bytes_of_tokens_are_the_tokens_own(kind, tmp_path):
+    """A character over several tokens: their bytes together are the text's, and tokens with the same text stay apart."""
+    tok, ids = _toks(kind, tmp_path)
+    assert tok.decode(ids) == TEXT
+    order = list(dict.fromkeys(ids))
+    top = [[t, -float(i)] for i, t in enumerate(order)]
+    messages = [{"delta": ids[:5], "logprobs": [[-0.5, 1, top]] * 5}, {"delta": ids[5:], "logprobs": [[-0.5, 1, top]] * (len(ids) - 5)},
+                {"done": True, "token_ids": ids, "finish_reason": "length"}]
+    chat = _app(messages, tok).run([1], {"logprobs": True, "top_logprobs": 20}, True)
+    assert chat["content"] == TEXT
+    got = chat["logprobs"]["content"]
+    assert b"".join(bytes(e["bytes"]) for e in got) == TEXT.encode()
+    byte_of = dict(zip(ids, TEXT.encode()))
+    for e in got:
+        assert [x["bytes"] for x in e["top_logprobs"]] == [[byte_of[t]] for t in order]
+        assert len({x["token"] for x in e["top_logprobs"]}) == len(order)
+        assert e["token"] == (chr(e["bytes"][0]) if e["bytes"][0] < 128 else "bytes:\\x%02x" % e["bytes"][0])
+    plain = _app(messages, tok).run([1], {"logprobs": 20}, False)["logprobs"]
+    assert plain["tokens"] == [e["token"] for e in got]
+    assert all(list(t.values()) == [x for _, x in top] for t in plain["top_logprobs"])
+
+
+def test_tokens_of_the_same_text_stay_apart():
+    """Ids without text of their own (all of the byte tokenizer's beyond 255) beside one another, and probabilities of nothing."""
+    top = [[256, -0.1], [258, -2.0], [300, -3.0], [65, float("-inf")]]
+    messages = [{"delta": [256], "logprobs": [[-0.1, 1, top]]}, {"done": True, "token_ids": [256], "finish_reason": "length"}]
+    got = _app(messages).run([1], {"logprobs": 4}, False)["logprobs"]
+    assert list(got["top_logprobs"][0].values()) == [-0.1, -2.0, -3.0, -9999.0] and got["top_logprobs"][0]["A"] == -9999.0
+    json.loads(json.dumps(got, allow_nan=False))
