@@ -299,7 +299,7 @@ class App:
                     continue
                 if "error" in msg:
                     raise RuntimeError(msg["error"])
-                if "delta" in msg:
+                if "delta" in msg and finish != "stop":        # (what the engine said before it heard of a stop string is no text)
                     now = time.time()
                     if last_t is not None:
                         itls.append((now - last_t) / max(len(msg["delta"]), 1))

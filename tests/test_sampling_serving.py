@@ -496,3 +496,18 @@ def test_tokens_of_the_same_text_stay_apart():
     got = _app(messages).run([1], {"logprobs": 4}, False)["logprobs"]
     assert list(got["top_logprobs"][0].values()) == [-0.1, -2.0, -3.0, -9999.0] and got["top_logprobs"][0]["A"] == -9999.0
     json.loads(json.dumps(got, allow_nan=False))
+
+
+def _answer(parts):
+    """An engine's messages for a text in the given pieces (bytes as tokens)."""
+    out = [{"delta": list(p), "logprobs": [[-float(b), 1, []] for b in p]} for p in parts]
+    return out + [{"done": True, "token_ids": list(b"".join(parts)), "finish_reason": "length"}]
+
+
+@pytest.mark.parametrize("parts", [[b"one t", b"w", b"o", b" three"], [b"one two", b" three ", b"four"], [bytes([b]) for b in b"one two three"]])
+def test_nothing_behind_a_stop_string_is_text(parts):
+    """However late the engine hears of it."""
+    events = []
+    app = _app(_answer(parts))
+    r = app.run([1], {"stop": ["two", "xyz"]}, False, lambda *a: events.append(a))
+    assert r["content"] == "one " and r["finish"] == "stop" and "".join(e[1] for e in events) == "one " and app.engine.cancelled == [0]
