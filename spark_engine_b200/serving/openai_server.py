@@ -200,12 +200,13 @@ def sampling_fields(body: dict, chat: bool) -> dict:
 
 
 class LogprobLog:
-    """Log-probabilities of an answer in the API's form; `take` gives those since it was last asked.  Tokens are named by their text, those that end or begin
+    """Log-probabilities of an answer in the API's form: of tokens that begin in the text that was `given` out, of which `take` gives those since it was
+    last asked (text that may be a stop string's begin is held back, and so are they).  Tokens are named by their text, those that end or begin
     inside a character by their bytes ("bytes:\\xe4\\xbd"), and where a name is taken by a more probable one, by their number ("token_id:5").  -9999 is
     what the API has for a probability of nothing (JSON has no infinities)."""
 
     def __init__(self, tok, chat: bool):
-        self.tok, self.chat, self.entries, self.taken, self.offset, self.names = tok, chat, [], 0, 0, {}
+        self.tok, self.chat, self.entries, self.taken, self.given, self.names = tok, chat, [], 0, 0, {}
 
     def _name(self, i: int):
         """(name, bytes) of a token."""
@@ -217,30 +218,37 @@ class LogprobLog:
                 self.names[i] = "bytes:" + "".join(f"\\x{b:02x}" for b in raw), list(raw)
         return self.names[i]
 
-    def feed(self, ids: List[int], got: List[list]):
+    def add(self, t: int, got: list, at: int):
+        """A token whose text begins at character `at`: (log-probability, rank, most probable ones)."""
         number = lambda x: max(x, -9999.0)                               # noqa: E731
-        for t, (lp, _, top) in zip(ids, got):
-            name, raw = self._name(t)
-            listed = {}
-            for i, x in top:
-                n, b = self._name(i)
-                listed[n if n not in listed else f"token_id:{i}"] = number(x), b
-            if self.chat:
-                self.entries.append({"token": name, "logprob": number(lp), "bytes": raw,
-                                     "top_logprobs": [{"token": n, "logprob": x, "bytes": b} for n, (x, b) in listed.items()]})
-            else:
-                self.entries.append((name, number(lp), {n: x for n, (x, _) in listed.items()}, self.offset))
-                self.offset += len(self.tok.decode([t]))
+        lp, _, top = got
+        name, raw = self._name(t)
+        listed = {}
+        for i, x in top:
+            n, b = self._name(i)
+            listed[n if n not in listed else f"token_id:{i}"] = number(x), b
+        if self.chat:
+            entry = {"token": name, "logprob": number(lp), "bytes": raw, "top_logprobs": [{"token": n, "logprob": x, "bytes": b} for n, (x, b) in listed.items()]}
+        else:
+            entry = name, number(lp), {n: x for n, (x, _) in listed.items()}, at
+        self.entries.append((at, entry))
+
+    def cut(self):
+        """The text ends with what was given out."""
+        self.entries = [e for e in self.entries if e[0] < self.given]
 
     def form(self, entries) -> dict:
+        entries = [e for _, e in entries]
         if self.chat:
             return {"content": entries}
         return {"tokens": [e[0] for e in entries], "token_logprobs": [e[1] for e in entries], "top_logprobs": [e[2] for e in entries],
                 "text_offset": [e[3] for e in entries]}
 
-    def take(self) -> dict:
-        new, self.taken = self.entries[self.taken:], len(self.entries)
-        return self.form(new)
+    def take(self, rest: bool = False) -> dict:
+        first = self.taken
+        while self.taken < len(self.entries) and (rest or self.entries[self.taken][0] < self.given):
+            self.taken += 1
+        return self.form(self.entries[first: self.taken])
 
 
 class App:
@@ -304,10 +312,20 @@ class App:
                     if last_t is not None:
                         itls.append((now - last_t) / max(len(msg["delta"]), 1))
                     last_t = now
+                    new = [(t, i) for i, t in enumerate(msg["delta"]) if t != eos]
+                    if lps is None:
+                        text = detok.feed([t for t, _ in new])
+                    else:                       # one by one: where each begins
+                        text = ""
+                        for t, i in new:
+                            if i < len(msg.get("logprobs", ())):
+                                lps.add(t, msg["logprobs"][i], detok.emitted)
+                            text += detok.feed([t])
+                    text, hit = ss.feed(text)
                     if lps is not None:
-                        keep = [i for i, t in enumerate(msg["delta"]) if t != eos and i < len(msg.get("logprobs", ()))]
-                        lps.feed([msg["delta"][i] for i in keep], [msg["logprobs"][i] for i in keep])
-                    text, hit = ss.feed(detok.feed([t for t in msg["delta"] if t != eos]))
+                        lps.given += len(text)
+                        if hit:
+                            lps.cut()
                     r, c = rs.feed(text)
                     reasoning += r
                     content += c
@@ -320,7 +338,10 @@ class App:
                     done = msg
                     if finish != "stop":
                         finish = {"stop": "stop", "length": "length", "cancelled": finish}.get(msg.get("finish_reason"), "stop")
-                        r, c = rs.feed(ss.flush())
+                        text = ss.flush()
+                        if lps is not None:
+                            lps.given += len(text)
+                        r, c = rs.feed(text)
                         reasoning += r
                         content += c
                         if write_event and (r or c):
@@ -333,7 +354,7 @@ class App:
         usage = {"prompt_tokens": len(prompt_ids), "completion_tokens": len(done.get("token_ids", [])),
                  "total_tokens": len(prompt_ids) + len(done.get("token_ids", []))}
         return {"content": content, "reasoning": reasoning, "finish": finish, "usage": usage, "engine": done,
-                "logprobs": None if lps is None else lps.form(lps.entries), "logprobs_left": lps.take() if lps is not None and lps.taken < len(lps.entries) else None}
+                "logprobs": None if lps is None else lps.form(lps.entries), "logprobs_left": lps.take(rest=True) if lps is not None and lps.taken < len(lps.entries) else None}
 
 
 def make_handler(app: App):

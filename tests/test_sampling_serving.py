@@ -511,3 +511,31 @@ def test_nothing_behind_a_stop_string_is_text(parts):
     app = _app(_answer(parts))
     r = app.run([1], {"stop": ["two", "xyz"]}, False, lambda *a: events.append(a))
     assert r["content"] == "one " and r["finish"] == "stop" and "".join(e[1] for e in events) == "one " and app.engine.cancelled == [0]
+
+
+@pytest.mark.parametrize("parts", [[b"one two three"], [b"one t", b"w", b"o three"], [b"one t", b"wo", b" three"], [bytes([b]) for b in b"one two three"]])
+@pytest.mark.parametrize("chat", [False, True])
+def test_log_probabilities_end_where_the_text_does(parts, chat):
+    """At a stop string, however it comes; what was given out before does not have to be taken back, and nothing behind it is text."""
+    body = {"stop": ["two", "xyz"], "logprobs": True if chat else 0}
+    events = []
+    app = _app(_answer(parts))
+    r = app.run([1], body, chat, lambda *a: events.append(a))
+    assert r["content"] == "one " and r["finish"] == "stop" and app.engine.cancelled == [0]
+    flat = lambda x: [e["logprob"] for e in x["content"]] if chat else x["token_logprobs"]
+    want = [-float(b) for b in b"one "]
+    assert flat(r["logprobs"]) == want
+    given = sum((flat(e[2]) for e in events), []) + (flat(r["logprobs_left"]) if r["logprobs_left"] else [])
+    assert given == want and "".join(e[1] for e in events) == "one "
+    whole = app.run([1], {**body, "stop": ["xyz"]}, chat)
+    assert whole["content"] == "one two three" and flat(whole["logprobs"]) == [-float(b) for b in b"one two three"]
+
+
+def test_offsets_are_where_the_tokens_begin_in_the_text():
+    raw = TEXT.encode()
+    want = [len(raw[:i].decode(errors="ignore")) for i in range(len(raw))]
+    for n in (1, 2, 3, len(raw)):
+        got = _app(_answer([raw[i: i + n] for i in range(0, len(raw), n)])).run([1], {"logprobs": 0}, False)
+        assert got["content"] == TEXT and got["logprobs"]["text_offset"] == want
+    cut = _app(_answer([raw])).run([1], {"logprobs": 0, "stop": "你"}, False)
+    assert cut["content"] == "hé " and len(cut["logprobs"]["tokens"]) == len("hé ".encode())
