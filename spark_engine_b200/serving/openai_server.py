@@ -467,7 +467,18 @@ def make_handler(app: App):
             if chat:
                 chunk(json.dumps({"id": cid, "object": obj + ".chunk", "created": created, "model": app.model_name,
                                   "choices": [{"index": 0, "delta": {"role": "assistant"}, "finish_reason": None}]}))
-            r = app.run(ids, body, chat, ev, lambda: gone["v"], mm=mm)
+
+            def end():
+                chunk("[DONE]")
+                try:
+                    self.wfile.write(b"0\r\n\r\n")
+                except OSError:
+                    pass
+            try:
+                r = app.run(ids, body, chat, ev, lambda: gone["v"], mm=mm)
+            except (ValueError, TypeError, OverflowError, RuntimeError) as e:      # (the answer has begun: its status is out)
+                chunk(json.dumps({"error": {"message": str(e), "type": "invalid_request_error"}}))
+                return end()
             last = {"index": 0, "finish_reason": r["finish"]}
             last["delta" if chat else "text"] = {} if chat else ""
             if r["logprobs_left"] is not None:
@@ -476,11 +487,7 @@ def make_handler(app: App):
             if (body.get("stream_options") or {}).get("include_usage"):
                 final["usage"] = r["usage"]
             chunk(json.dumps(final))
-            chunk("[DONE]")
-            try:
-                self.wfile.write(b"0\r\n\r\n")
-            except OSError:
-                pass
+            end()
     return H
 
 

@@ -539,3 +539,22 @@ def test_offsets_are_where_the_tokens_begin_in_the_text():
         assert got["content"] == TEXT and got["logprobs"]["text_offset"] == want
     cut = _app(_answer([raw])).run([1], {"logprobs": 0, "stop": "你"}, False)
     assert cut["content"] == "hé " and len(cut["logprobs"]["tokens"]) == len("hé ".encode())
+
+
+@pytest.mark.parametrize("body", [{"top_p": 2.0}, {"logprobs": True, "top_logprobs": "x"}])
+def test_a_stream_that_is_refused_ends_with_an_error(body):
+    """As an event of the stream, which begins before the engine answers."""
+    from http.server import ThreadingHTTPServer
+    from spark_engine_b200.serving.openai_server import make_handler
+    app = _app([{"error": "it does not want to"}])
+    srv = ThreadingHTTPServer(("127.0.0.1", 0), make_handler(app))
+    srv.daemon_threads = True
+    threading.Thread(target=srv.serve_forever, daemon=True).start()
+    try:
+        ask = {"messages": [{"role": "user", "content": "hi"}], "stream": True, **body}
+        req = urllib.request.Request(f"http://127.0.0.1:{srv.server_address[1]}/v1/chat/completions", json.dumps(ask).encode(), {"Content-Type": "application/json"})
+        lines = [x[6:] for x in urllib.request.urlopen(req, timeout=30).read().decode().split("\n") if x.startswith("data: ")]
+        assert lines[-1] == "[DONE]" and json.loads(lines[-2])["error"]["message"] == ("it does not want to" if "top_p" in body else "top_logprobs must be a whole number")
+        assert all("choices" in json.loads(x) for x in lines[:-2]) and not app.engine.queues
+    finally:
+        srv.shutdown()
