@@ -136,11 +136,11 @@ Tensor adjust_logits(const Tensor& given, const py::object& adjust, int64_t offs
 void count_tokens(const Tensor& counts, const Tensor& tokens, const Tensor& n, const Opt& slots, bool prompt, bool reset, bool run) {
   const at::Device dev = counts.device();
   need_counts(counts, -1, dev);
-  NEED(counts.size(1) >= 1 && counts.size(1) < 1ll << 31, "counts must have 1 to 2^31 - 1 columns");
+  NEED(counts.size(1) >= 1 && counts.size(1) <= 1ll << 30, "counts must have 1 to 2^30 columns");
   NEED(tokens.scalar_type() == at::kInt && tokens.device() == dev && tokens.dim() == 2 && (tokens.size(1) < 2 || tokens.stride(1) == 1), "tokens must be an int32 tensor [requests, tokens] on ",
        dev, ", its rows contiguous");
   const int64_t S = tokens.size(0), P = tokens.size(1);
-  NEED(S <= MAX_ROWS && P < 1ll << 31, "at most ", MAX_ROWS, " requests of 2^31 - 1 tokens");
+  NEED(S <= MAX_ROWS && P <= 1ll << 30, "at most ", MAX_ROWS, " requests of 2^30 tokens");     // (CTAs step beyond both by some thousands)
   need_vec("n", n, at::kInt, S, dev);
   need_vec("slots", slots, at::kInt, S, dev);
   NEED(slots || S <= counts.size(0), "more requests than slots of the counts, and no `slots`");

@@ -203,3 +203,11 @@ def test_kernels_of_other_sources_are_refused():
     dll.spark_sampling_layout = Fn(mod.layout() ^ 1)
     with pytest.raises(RuntimeError, match="different sources"):
         sampling._same_layout(mod, dll)
+
+
+@pytest.mark.parametrize("V, P", [(2**30 + 1, 4), (2**31 - 1, 4), (8, 2**30 + 1), (8, 2**31 - 1)])
+def test_counts_refuse_what_32_bit_places_do_not_reach(V, P):
+    """A CTA's steps through tokens and columns go beyond their number by up to some thousands."""
+    none = lambda *s: torch.empty(*s, dtype=torch.int32, device="meta")
+    with pytest.raises(ValueError, match=r"2\^30"):
+        ops.count_tokens(none(2, V), none(1, P), none(1))
