@@ -144,7 +144,7 @@ void count_tokens(const Tensor& counts, const Tensor& tokens, const Tensor& n, c
   need_vec("n", n, at::kInt, S, dev);
   need_vec("slots", slots, at::kInt, S, dev);
   NEED(slots || S <= counts.size(0), "more requests than slots of the counts, and no `slots`");
-  if (!run || S == 0) return;
+  if (!run || S == 0 || (P == 0 && !reset)) return;
   const On on(counts);
   spark::CountTokens arg{ptr<int>(counts), ptr<int>(tokens), ptr<int>(n), ptr<int>(slots), on.dev.status, row_step(counts), row_step(tokens), static_cast<int>(S),
                          static_cast<int>(P), static_cast<int>(counts.size(1)), static_cast<int>(counts.size(0)), prompt, reset};

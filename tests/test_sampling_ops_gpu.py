@@ -479,3 +479,19 @@ def test_borders_of_short_prefixes_are_the_same_in_every_batch(V, spread):
             every = every or got
             assert got == every[: len(got)], (shift, size, sum(g != e for g, e in zip(got, every)))
     _sound()
+
+
+# ----------------------------------------------------------------------------- launches
+def test_only_kernels_that_run_are_counted():
+    from spark_engine_b200.ops import cuda as cu
+    i = torch.int32
+    c, n = torch.zeros(2, 9, dtype=i, device="cuda"), torch.zeros(2, dtype=i, device="cuda")
+
+    def launches(f):
+        cu.reset_launch_count()
+        f()
+        return cu.launch_count()
+    assert launches(lambda: ops.count_tokens(c, c[:, :0], n)) == 0 and launches(lambda: ops.count_tokens(c, c[:0, :3], n[:0])) == 0
+    assert launches(lambda: ops.count_tokens(c, c[:, :0], n, reset=True)) == 1 and launches(lambda: ops.count_tokens(c, c[:, :3].clone(), n)) == 1
+    x = torch.zeros(0, 9, device="cuda")
+    assert launches(lambda: ops.adjust_logits(x, ops.Adjust())) == 0 and launches(lambda: ops.token_logprobs(x, n[:0], 2)) == 0
