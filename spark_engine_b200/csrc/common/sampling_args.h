@@ -9,7 +9,7 @@ namespace spark {
 #define SPARK_SAMPLING_LAYOUT 0u
 #endif
 
-constexpr int SAMPLE_MAX_V = 16 * 49152;           // columns of a row: 16 CTAs of a cluster hold 192 KB each
+constexpr int SAMPLE_MAX_V = 768 * 1024;           // columns of a row: 98 KB of the largest of every 32 logits, if one CTA has it (asserted in sample_rows.cu)
 constexpr int SAMPLE_MAX_LIST = 1024;              // drafted tokens, biases of a row
 constexpr int SAMPLE_MAX_TOP = 256;                // most probable tokens of a row
 

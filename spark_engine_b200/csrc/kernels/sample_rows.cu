@@ -218,14 +218,21 @@ struct Parts {
   Groups groups;
   float* maxima;
   u64* inbox;
-  static __host__ __device__ __forceinline__ int lg_of(int per) { return per <= 160 ? 3 : per <= 320 ? 4 : 5; }
-  static __host__ int bytes(int per, int size) { return (per * CHUNK >> lg_of(per)) * 4 + (size > 1 ? size * NT * 4 + LIST * 8 : 0); }
+  static constexpr __host__ __device__ __forceinline__ int lg_of(int per) { return per <= 160 ? 3 : per <= 320 ? 4 : 5; }
+  static constexpr __host__ int bytes(int per, int size) { return (per * CHUNK >> lg_of(per)) * 4 + (size > 1 ? size * NT * 4 + LIST * 8 : 0); }
   __device__ __forceinline__ Parts(float* smem, int per, int size) {
     groups = Groups{smem, lg_of(per)};
     maxima = smem + (per * CHUNK >> groups.lg);
     inbox = reinterpret_cast<u64*>(maxima + size * NT);
   }
 };
+
+// What the longest row needs: shared memory of the CTA that has it alone, or of those that share one of the widest clusters; bins whose sums of weights, 2^16
+// a group at most, and numbers, which become fp32, do not leave 32 and 24 bits; ids that kth_by_bits looks for by 21 of them.
+constexpr int MAX_CHUNKS = (SAMPLE_MAX_V + 8 + CHUNK - 1) / CHUNK, MAX_SMEM = 227 * 1024;
+static_assert(Parts<512>::bytes(MAX_CHUNKS, 1) + sizeof(RowShared<512>) <= MAX_SMEM && Parts<512>::bytes(320, CLUSTER_MAX) + sizeof(RowShared<512>) <= MAX_SMEM, "shared memory");
+static_assert((MAX_CHUNKS * CHUNK >> Parts<512>::lg_of(MAX_CHUNKS)) < 65536 && (320 * CHUNK >> Parts<512>::lg_of(320)) < 65536 && SAMPLE_MAX_V < 1 << 24, "bins");
+static_assert(SAMPLE_MAX_V <= 1 << 21, "ids");
 
 __device__ __forceinline__ float max8(const float* v) {
   float m = v[0];
