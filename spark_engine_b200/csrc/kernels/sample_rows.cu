@@ -18,7 +18,7 @@
 //
 // Sums of weights that decide what is kept are whole numbers of 2^-40, which no order changes: a row draws the same whatever CTAs it has and wherever in
 // memory it begins.  The weight of a row that top_p alone filters is streamed: a chunk's in fp32 in units 2^E of its own, E whole, chunks' in 64 bits.
-// Where what is kept ends within 2^-18 of that sum's share, the row is drawn again by a sum in whole numbers.  Log-probabilities go by the streamed sum:
+// Where the weight in front of the token drawn is within 2^-18 of top_p of that sum, the row is drawn again by a sum in whole numbers.  Log-probabilities go by the streamed sum:
 // they are the same however chunks are dealt to CTAs (to 2^-53); rows that begin elsewhere between two 16-byte boundaries have other chunks, and may have
 // another last bit.
 //
@@ -26,7 +26,7 @@
 // 2.5 are the row's own, 1.4 sums and best over eight CTAs, 1.4 bins, 4 the groups read again and lists joined, 2 the prefix and the draw.  Many rows whose
 // distributions have few likely tokens: memory latency of what is read again, 62 us for 256 rows (24 at the copy rate).  Rows without filters: issue slots,
 // 40 instructions per logit and lane, two thirds of them the hash: 79 us for 256.  Rows that keep most of 152k tokens: one such race and one look at
-// the weights, 228 us for 256 of them.  Scored rows: 1024 of 152k in 100 us, 6.2 TB/s.
+// the weights, 229 us for 256 of them.  Scored rows: 1024 of 152k in 100 us, 6.2 TB/s.
 #include "../common/token_rows.cuh"
 
 namespace spark {
@@ -84,11 +84,10 @@ struct RowShared {
   float fsum[NT / 32];
   unsigned n_list, n_hits, before, kept;
   int bin, score;
-  bool unsure;
   float z;
   double log;
   Prefix cut;
-  u64 total;
+  u64 total, unsure;
 };
 
 // ------------------------------------------------------------------------------------------------ a CTA's part of a row
@@ -329,8 +328,25 @@ struct Weights {
   }
 };
 
-// A weight in whole numbers of 2^-40: sums of them are the same in every order, so that what is kept does not depend on how a row is dealt out.
-__device__ __forceinline__ u64 whole(float w) { return __float2ull_rn(w * 1099511627776.f); }
+// Weights (less than 2) in whole numbers of 2^-40, rounded to nearest: sums of them are the same in every order, so that what is kept does not depend on how
+// a row is dealt out.  Of w + 2 the last bit is 2^-22, and what it leaves of w is exact: both parts are read from the bits of a sum (a conversion to 64 bits
+// would take the unit that exponentials wait for: 256 rows that keep most 233 us with it, 230 without, 228 with fp32 sums of eight; two by two in packed
+// additions 232).
+struct Whole {
+  static constexpr uint32_t TWO = 0x40000000u, SMALL = 0x37400000u;    // 2 and 1.5 * 2^-17
+  uint32_t hi = 0, lo = 0;                         // of 2^-22, and of 2^-40 (with a sign): up to 512 weights
+  __device__ __forceinline__ void add(float w) {
+    const float a = w + 2.f;
+    hi += __float_as_uint(a) - TWO;
+    lo += __float_as_uint(w - (a - 2.f) + __uint_as_float(SMALL)) - SMALL;
+  }
+  __device__ __forceinline__ u64 sum() const { return (static_cast<u64>(hi) << 18) + static_cast<u64>(static_cast<long long>(static_cast<int>(lo))); }
+};
+__device__ __forceinline__ u64 whole(float w) {
+  Whole s;
+  s.add(w);
+  return s.sum();
+}
 __device__ __forceinline__ double weight_of(u64 n) { return static_cast<double>(n) * (1.0 / 1099511627776.0); }
 
 template <int NT>
@@ -718,16 +734,18 @@ __device__ __noinline__ Lap lap(const Row<T, NT> row, const Groups groups, const
     if (__all_sync(0xffffffffu, !(mine >= front.z))) return;
     if (MASS) {
       bool last = false;
+      Whole eight;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        if (v[i] > front.z) s += whole(w(v[i]));
+        eight.add(v[i] > front.z ? w(v[i]) : 0.f);
         last |= v[i] == front.z;
       }
       if (last) {                                  // as the last token of it: by their ids
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          if (v[i] == front.z && row.id(Row<T, NT>::place(chunk, q + i, threadIdx.x & 31)) <= front.id) s += whole(w(v[i]));
+          if (v[i] == front.z && row.id(Row<T, NT>::place(chunk, q + i, threadIdx.x & 31)) <= front.id) eight.add(w(v[i]));
       }
+      s += eight.sum();
     }
     if (RACE && (__any_sync(0xffffffffu, racer.bound > -INFINITY) || racer.template begin<8>(race, row, v, mine, chunk, q, front, shared)))
       racer.template run<false>(race, row, v, chunk, q, front, shared);
@@ -873,25 +891,36 @@ __device__ __noinline__ bool list_kept(RowShared<NT>& sh, Cluster& c, const Row<
 template <int NT>
 __device__ __noinline__ Lap list_lap(const RowShared<NT>& sh, const Race race, const Weights w, const Prefix front, bool race_too, bool mass_too) {
   Top2 m = no_top();
-  u64 s = 0;
+  Whole s;
   const unsigned n = sh.n_list;
   for (unsigned i = threadIdx.x; i < n; i += NT) {
     const u64 key = sh.list[i];
     const float z = list_z(key);
     const int id = list_id(key);
     if (!within(front, z, id)) continue;
-    if (mass_too) s += whole(w(z));
+    if (mass_too) s.add(w(z));
     if (race_too) m = best2(m, Top2{race.rough(z, id), id, -INFINITY, z});
   }
-  return Lap{m, s};
+  return Lap{m, s.sum()};
 }
 
+// Whether the row's sum is the streamed one.
+__device__ __forceinline__ bool streamed(const SampleRows& a, int r, const Weights& w) {
+  return !(a.top_k && a.top_k[r] > 0 && a.top_k[r] < a.V) && !(a.min_p && a.min_p[r] > 0.f && isfinite(a.temps[r])) && w.from == 0.f;
+}
+// Whether a listed token that is as near to the border as the streamed sum is off may be drawn: it may, and if it or one behind it is, the draw is made again.
+template <int NT>
+__device__ __noinline__ bool perhaps(RowShared<NT>& sh, const SampleRows& a, int r, const Weights w, u64 key, bool otherwise) {
+  if (!streamed(a, r, w)) return otherwise;
+  atomicMax(&sh.unsure, key);
+  return true;
+}
 // A draw by top_p alone, of a row whose tokens begin with `first`: by a sum in whole numbers and the scores as they are defined, by one CTA that reads
 // the row again and again (it is for what comes so near to the border that the streamed sum does not tell: 0.3 ms for 152k logits).  Other rows' sums are
 // in whole numbers from the start: `otherwise`.
 template <class T, int NT>
 __device__ __noinline__ int draw_in_whole(RowShared<NT>& sh, Cluster& c, const SampleRows& a, int r, const Weights w, int first, int otherwise) {
-  if ((a.top_k && a.top_k[r] > 0 && a.top_k[r] < a.V) || (a.min_p && a.min_p[r] > 0.f && isfinite(a.temps[r])) || w.from != 0.f) return otherwise;
+  if (!streamed(a, r, w)) return otherwise;
   const Row<T, NT> row(static_cast<const T*>(a.x) + r * a.ldx, a.V, 0, a.V);
   const Race race(a.temps[r], w.c, a.seeds[r], a.positions[r]);
   const auto every = [&](auto f) {
@@ -954,7 +983,7 @@ sample_kernel(const __grid_constant__ SampleRows a, int per) {
   const float scale = greedy ? 0.f : fmaxf(fminf(__fdiv_rn(1.4426950408889634f, temp), -LOWEST), 1e-44f);
   const Race race(temp, scale, a.seeds[r], a.positions[r]);
   clear_bins(sh);
-  if (t == 0) { sh.n_list = sh.n_hits = 0; sh.unsure = false; sh.score = score_key(-INFINITY); }
+  if (t == 0) { sh.n_list = sh.n_hits = 0; sh.unsure = 0; sh.score = score_key(-INFINITY); }
   if (all) __syncthreads();
 
   Seen seen;
@@ -1039,25 +1068,23 @@ sample_kernel(const __grid_constant__ SampleRows a, int per) {
   }
   if (n <= LIST) {
     if (c.rank) return;
-    const auto weighed = [&](u64 key) { return whole(weight(list_z(key))); };
     const unsigned n1 = by_k ? min(n, static_cast<unsigned>(k)) : n;
     int token;
     if (n <= FEW_OF<NT>) {
       if (by_p) {
-        if (t < n) sh.weight[t] = weighed(sh.list[t]);
+        if (t < n) sh.weight[t] = whole(weight(list_z(sh.list[t])));
         __syncthreads();
       }
       const Counted e = count_list(sh, n, by_p);
       bool in = e.mine && e.rank < n1;
-      if (by_p) {
+      if (by_p) {                                  // every token before the one that reaches top_p
         if (e.mine && e.rank + 1 == n1) sh.total = e.before + e.weight;
         __syncthreads();
         const double before = weight_of(e.before), target = p * (by_k ? weight_of(sh.total) : total);
-        if (in && close_to(before, target)) sh.unsure = true;
-        in = in && (e.rank == 0 || before < target);                   // (every token before the one that reaches top_p)
+        if (in && e.rank) in = close_to(before, target) ? perhaps(sh, a, r, weight, e.key, before < target) : before < target;
       }
-      token = draw_listed(sh, c, race, [&](auto f) { if (in) f(e.key); }).id;
-      if (sh.unsure) token = draw_in_whole<T, NT>(sh, c, a, r, weight, top.id, token);
+      const Prefix win = draw_listed(sh, c, race, [&](auto f) { if (in) f(e.key); });
+      token = list_key(win.z, win.id) > sh.unsure ? win.id : draw_in_whole<T, NT>(sh, c, a, r, weight, top.id, win.id);
     } else {                                       // longer ones as rows are that keep very many: drawn first, looked at then
       Prefix in = whole_row();
       if (n1 < n) {
@@ -1065,12 +1092,12 @@ sample_kernel(const __grid_constant__ SampleRows a, int per) {
         in = Prefix{list_z(last), list_id(last)};
       }
       const auto in_front = [&](const Prefix& f) {
-        u64 w = 0;
+        Whole mine;
         for (unsigned i = t; i < n; i += NT) {
           const u64 key = sh.list[i];
-          w += within(f, list_z(key), list_id(key)) ? weighed(key) : 0;
+          mine.add(within(f, list_z(key), list_id(key)) ? weight(list_z(key)) : 0.f);
         }
-        w = c.block(w, u64{0}, [](u64 x, u64 y) { return x + y; });
+        const u64 w = c.block(mine.sum(), u64{0}, [](u64 x, u64 y) { return x + y; });
         if (t == 0) sh.total = w;
         __syncthreads();
         return weight_of(sh.total);
