@@ -358,30 +358,42 @@ def test_a_prompt_without_a_token():
     assert len(sd.generate(prompts, 5, params=NOTHING)[0]) == 5
 
 
-@pytest.mark.parametrize("after", [0, 4])
-def test_a_server_ends_requests_without_a_token(after):
+def check_a_server_ends_requests_without_a_token(after, device, one):
     """With an error and what was said before; the request again (over what its slot was left with) has its whole text, and so have those beside it."""
-    cfg, W, m = _model()
+    cfg, W, m = _model(device)
     prompts = _prompts(cfg, 2)
     alone = []
-    for p, q in zip(prompts, [NOTHING, WILD]):
+    for p, q in zip(prompts, [one, WILD]):
         alone += _text(SpecDecoder(m, lambda s, d: ([], []), depth=0), [p], [q], 10)[0]
-    es = EngineServer(cfg, W, EngineConfig(max_seqs=2, kv_tokens=2048, prefill_chunk=32, spec="mtp", spec_depth=2))
+    es = EngineServer(cfg, W, EngineConfig(max_seqs=2, kv_tokens=2048, prefill_chunk=32, spec="mtp", spec_depth=2, cuda_graphs=False), device=device)
     see = _blind(es.model, lambda: next((s for s, lv in es.by_slot.items() if lv.id == 0), -1), len(prompts[0]) + after)
-    for i, q in enumerate([NOTHING, WILD]):
+    for i, q in enumerate([one, WILD]):
         es.submit(_message(i, prompts[i], q, 10))
     while es.sched.has_work():
         es.step()
     see()
-    es.submit(_message(2, prompts[0], NOTHING, 10))
+    es.submit(_message(2, prompts[0], one, 10))
     while es.sched.has_work():
         es.step()
     mine = [x for x in es.out if x.get("id") == 0]
     said = sum((x["delta"] for x in mine if "delta" in x), [])
     assert "error" in mine[-1] and not any(x.get("done") for x in mine) and said == alone[0][: len(said)] and (len(said) == 0) == (after == 0)
-    assert sum(len(x.get("logprobs", [])) for x in mine) == len(said)
+    assert sum(len(x.get("logprobs", [])) for x in mine) == (len(said) if one.logprobs >= 0 else 0)
     done = {x["id"]: x["token_ids"] for x in es.out if x.get("done")}
     assert done == {1: alone[1], 2: alone[0]} and not es.live and not es.by_slot
+
+
+@pytest.mark.parametrize("after", [0, 4])
+def test_a_server_ends_requests_without_a_token(after):
+    check_a_server_ends_requests_without_a_token(after, "cpu", NOTHING)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("one", [NOTHING, SamplingParams(temperature=0.9, seed=4), SamplingParams()], ids=["filtered", "plain", "greedy"])
+@pytest.mark.parametrize("after", [0, 4])
+def test_a_server_ends_requests_without_a_token_on_the_device(after, one):
+    """There plain rounds know no token of such rows either."""
+    check_a_server_ends_requests_without_a_token(after, "cuda", one)
 
 
 # ----------------------------------------------------------------------------- the front end alone
