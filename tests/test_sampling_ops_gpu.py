@@ -495,3 +495,24 @@ def test_only_kernels_that_run_are_counted():
     assert launches(lambda: ops.count_tokens(c, c[:, :0], n, reset=True)) == 1 and launches(lambda: ops.count_tokens(c, c[:, :3].clone(), n)) == 1
     x = torch.zeros(0, 9, device="cuda")
     assert launches(lambda: ops.adjust_logits(x, ops.Adjust())) == 0 and launches(lambda: ops.token_logprobs(x, n[:0], 2)) == 0
+
+
+# ----------------------------------------------------------------------------- cold rows
+@pytest.mark.parametrize("R", [1, 40, 300])
+@pytest.mark.parametrize("bias", [0.0, 100.0])
+def test_cold_rows_with_top_k(R, bias):
+    """The k-th token weighs less than 2^-64 of the first: at low temperatures, or beside a strong bias."""
+    V = 151936
+    rows = Rows(3, V, "peaked", seed=R, device="cuda")
+    if bias:
+        rows.logits[:, 777] += bias
+        rows.z = rows.logits.cpu().numpy()
+    z = rows.z
+    rows.logits, rows.z, rows.R = rows.logits.repeat(-(-R // 3), 1)[:R].contiguous(), np.tile(z, (-(-R // 3), 1))[:R], R
+    rows.seeds, rows.positions = rows.rs.randint(0, 1 << 40, R), rows.rs.randint(0, 1 << 20, R)
+    T = rows.rs.choice([0.7] if bias else [0.05, 0.1, 0.2], R)
+    s = dict(top_k=rows.rs.choice([20, 40, 64, 3000], R), top_p=rows.rs.choice([1.0, 0.9], R), min_p=rows.rs.choice([0.0, 1e-25], R))
+    got = rows.draw(T, **s)
+    for r in range(0, R, 1 + R // 40):
+        assert got[r] == want_token(rows.z[r], T[r], int(rows.seeds[r]), int(rows.positions[r]), int(s["top_k"][r]), s["top_p"][r], s["min_p"][r])
+    _sound()
