@@ -48,17 +48,20 @@ struct RowAdjust {
   int nd = 0, nb = 0;
 
   __device__ __forceinline__ RowAdjust(const Adjustments& a, int r, int* status) {
-    int slot = a.slots ? a.slots[r] : r;
-    if (a.counts && slot >= a.n_slots) {           // (what the row has said is not known: it has no penalties)
-      set_status(status, ST_BOUNDS, r, slot, a.n_slots);
-      slot = -1;
-    }
+    const int slot = a.slots ? a.slots[r] : r;
     if (slot >= 0) {
-      if (a.counts) counts = a.counts + slot * a.ld_counts;
       if (a.repetition) rep = a.repetition[r];
       if (a.presence) pres = a.presence[r];
       if (a.frequency) freq = a.frequency[r];
       if (a.drafted) { nd = a.n_drafted; drafted = a.drafted + static_cast<long long>(r) * nd; }
+      if (a.counts) {
+        if (slot < a.n_slots) {
+          counts = a.counts + slot * a.ld_counts;
+        } else {                                   // (what the row has said is not known: it has no penalties)
+          set_status(status, ST_BOUNDS, r, slot, a.n_slots);
+          rep = 1.f; pres = freq = 0.f; nd = 0;
+        }
+      }
     }
     if (a.bias_ids) { nb = a.n_bias; bias_ids = a.bias_ids + static_cast<long long>(r) * nb; bias = a.bias + static_cast<long long>(r) * nb; }
     if (a.allowed) allowed = a.allowed + static_cast<long long>(r) * a.words;
