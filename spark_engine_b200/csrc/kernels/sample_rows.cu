@@ -816,7 +816,8 @@ __device__ __forceinline__ u64 row_count(const Row<T, NT>& row, Cluster& c, F f)
   return c.reduce(n, u64{0}, [](u64 a, u64 b) { return a + b; });
 }
 
-// By the bits of keys and ids, for the rare row in which more tokens than a list takes share a bin.
+// By the bits of keys and ids, where more tokens than a list takes share the k-th one's bin: many equal logits, or a k-th one in the last bin, below 2^-64 of
+// the first (top_k 40 at temperature 0.1, or beside a bias of 100).  Up to 55 readings of the row: 0.29 ms for 152k logits, 1.8 ms for 256 such rows.
 template <class T, int NT>
 __device__ __noinline__ Prefix kth_by_bits(const Row<T, NT> row, Cluster& c, const Prefix of, u64 k) {
   if (row_count(row, c, [&](float z, int id) { return within(of, z, id); }) <= k) return of;
