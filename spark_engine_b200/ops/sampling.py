@@ -215,7 +215,10 @@ class Logprobs(NamedTuple):
 
 def token_logprobs(logits, tokens, top: int = 0) -> Logprobs:
     """log softmax(logits) of tokens int32 [R] and of the `top` (256 at most) most probable ones of every row, for logits [R, V] (fp32, bf16, fp16).  What is
-    not in the vocabulary has -inf and rank 0; tokens that are none (-inf, NaN) have -inf."""
+    not in the vocabulary has -inf and rank 0; tokens that are none (-inf, NaN) have -inf.
+
+    Exponentials are fp32, their sums 64 bits beyond 32 of them, differences 64 bits: results are off by about a step of fp32 (2^-21 of the sum at most, and half a
+    step).  They are the same in every batch; where rows begin elsewhere between two 16-byte boundaries the last bit may be another."""
     run = _kernels(logits)
     out = Logprobs(*_native().token_logprobs(logits, tokens, top, run))
     if run:
